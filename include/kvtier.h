@@ -302,6 +302,67 @@ int kvt_prefill_attn(const void* q, int64_t sq_n, int64_t sq_h, const void* cu_q
  * reference (its prefill kernel takes one block per query row). */
 int kvt_prefill_work_bytes(int batch, int H, int Hq, int max_q, int spread_blocks, int64_t* bytes);
 
+/* ------------------------------------------------------------------------------------- 8-bit block cache */
+
+/* A paged cache in 8 bits with one scale per block of tokens and KV head (no counterpart in the reference).  Per layer:
+ * codes k8 / v8 [n_blocks, H, block, D], one byte each (code 0: e4m3, code 1: int8), 16-byte aligned; scales ks / vs
+ * fp32 [n_blocks, H]: a code c stands for c * s.  block = 16, 32 or 64 tokens, D = 64, 128 or 256.  Position p of a
+ * request sits in row p % block of block block_table[row][p / block] (int32, row stride bt_stride >= max_blocks).
+ * Entry points that take `rows` (int32 [n]) use table row rows[j] for request j, or row j where it is NULL.
+ * Lengths, tables and counts are read on the device; whatever they hold, no entry point reads or writes outside the
+ * buffers: positions whose table entry is no block (< 0 or >= n_blocks), or past the table's columns, are not written
+ * and not attended. */
+
+/* Block tables and slot maps of a step.  Request j < n (n <= 1,024) appends counts[j] (int32) tokens to table row
+ * seqs[j] (int32, distinct, < rows) behind its seq_lens[row] tokens: the blocks that it opens take the next entries of
+ * free_list (int32 [n_free], block ids; read from *free_head on) in request order and are written into block_table.
+ * Writes cu int32 [n + 1] (prefix sums of the counts, cu[n] <= n_tokens), slots int32 [n_tokens] (block id * block + row
+ * of every token, -1 behind cu[n] and where no block could be given), kv_lens int32 [n] (lengths with the step's tokens)
+ * and *next_head (the free list's next entry after the plan); with req_to_token (int32 [rows, rtt_cols], row stride
+ * rtt_stride; NULL: none) also req_to_token[row][p] = slot of every position p < rtt_cols.  commit: seq_lens and *free_head
+ * advance as well; without it they stay, and the same call gives the same plan again.  *status (NULL: none) is or-ed
+ * with 1 the free list ran out (the requests behind get -1 entries), 2 a table row is full, 4 the counts exceed n_tokens
+ * (cut off there), 8 a row out of range or listed twice (the later request appends nothing, kv_lens 0).  n_free * block
+ * <= 2^31 and n_tokens <= 2^30, else KVT_ERANGE. */
+int kvt_block_plan(int n, const void* seqs, const void* counts, void* seq_lens, int rows, void* block_table,
+                   int64_t bt_stride, int max_blocks, const void* free_list, int n_free, void* free_head, int block,
+                   int n_tokens, void* cu, void* slots, void* kv_lens, void* next_head, void* status,
+                   void* req_to_token, int64_t rtt_stride, int rtt_cols, int commit, void* stream);
+
+/* Quantizing write of N = n_tokens rows k / v [N, H, D] (dtype codes as above; element strides, unit last stride, rows
+ * 16-byte aligned) into the blocks of their positions: rows cu[j] .. cu[j+1] of k / v are the last positions of request
+ * j's kv_lens[j].  A block's scale is the smallest power of two that holds the largest finite |x| of the call's rows in the
+ * code's range (448 or 127; within 2^-64 .. 2^122), or the scale it has if that is larger and the request held rows of
+ * the block before; where it grows, those rows' codes are rounded to the new scale.  Codes are rounded to nearest even;
+ * infinities become the largest code, NaN the e4m3 NaN or the int8 0.  Other rows of a block are left as they are.  A block
+ * must not be in the tables of two of the call's requests.  n <= 4,096. */
+int kvt_block_store(const void* k, const void* v, int dtype, int64_t sk_n, int64_t sk_h, int64_t sv_n, int64_t sv_h,
+                    int n_tokens, int H, int D, const void* cu, const void* kv_lens, int n, const void* rows,
+                    const void* block_table, int64_t bt_stride, int n_rows, int max_blocks, int code, void* k8, void* v8,
+                    void* ks, void* vs, int n_blocks, int block, void* stream);
+
+/* Decode attention of one query token per request: out[j, h] = softmax(scale q K^T) V over positions < kv_lens[j].  q
+ * (q_type 0 bf16, 1 fp16; 16-byte aligned, strides multiples of 8) and out (out_type 0 bf16, 1 fp16, 2 fp32) are [n, Hq, D]
+ * with element strides of token and head.  Hq / H <= 16, n <= 4,096.  n_splits > 1: the positions of a request are shared
+ * by up to n_splits workgroups, merged by a second launch; part_o fp32 [n * H * n_splits * 16 * D] and part_ml fp32 [n *
+ * H * n_splits * 32] hold their parts.  A request without positions gives NaN (0/0). */
+int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q_type, const void* kv_lens, int n, int H, int Hq,
+                     int D, int code, const void* k8, const void* v8, const void* ks, const void* vs, int n_blocks,
+                     int block, const void* block_table, int64_t bt_stride, int n_rows, int max_blocks, const void* rows,
+                     float scale, int n_splits, void* part_o, void* part_ml, void* out, int out_type, int64_t so_n,
+                     int64_t so_h, void* stream);
+
+/* Attention of chunks of queries: request j owns rows cu_q[j] .. cu_q[j+1] (int32 [n + 1], at most n_q) of q / out.  causal: its
+ * queries are the last positions of kv_lens[j] and see the positions up to their own; else every query sees all kv_lens[j]
+ * positions (cross attention).  Rows of q / out behind cu_q[n] are left as they are.  Otherwise as kvt_block_decode, with the
+ * parts per item: items = n_q * (Hq / H) / 16 + n in the place of n. */
+int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int q_type, const void* cu_q, int n_q,
+                      const void* kv_lens, int n, int H, int Hq, int D, int code, const void* k8, const void* v8,
+                      const void* ks, const void* vs, int n_blocks, int block, const void* block_table,
+                      int64_t bt_stride, int n_rows, int max_blocks, const void* rows, int causal, float scale,
+                      int n_splits, void* part_o, void* part_ml, void* out, int out_type, int64_t so_n, int64_t so_h,
+                      void* stream);
+
 /* ----------------------------------------------------------------------------- lazy backing (HIP VMM) */
 
 /* Lazily backed device memory for the KV pool (reference: patches/kv_lazy.py -- the pool is reserved as address

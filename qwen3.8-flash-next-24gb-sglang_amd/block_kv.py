@@ -1,0 +1,338 @@
+"""8-bit paged KV cache with one scale per block of tokens and KV head, and its operators.
+
+The slot pools of this package keep a scale per token and channel group; here a block of 16, 32 or 64 tokens of one KV head
+shares one power-of-two fp32 scale for K and one for V, over e4m3 or int8 codes: H * D * 2 bytes per token and 8 * H bytes
+per block.  The step of a serving program is four calls, all on the device (no host lengths, capturable):
+
+    cache = BlockKVCache(layers, H, D, n_blocks, max_seqs, max_blocks, device)
+    s = cache.add_seq()
+    plan = cache.plan(seqs, counts, n_tokens)            # kvt_block_plan: blocks, slots, lengths
+    for layer: cache.append(layer, plan, k, v)           # kvt_block_store
+               out = cache.decode(layer, plan, q)        # kvt_block_decode, one query per request
+               out = cache.prefill(layer, plan, q)       # kvt_block_prefill, the step's tokens as queries
+
+The functions take the buffers themselves.  k8 / v8: float8_e4m3fn or int8 [n_blocks, H, block, D]; ks / vs: fp32
+[n_blocks, H]; block_table: int32 [rows, max_blocks], -1 where there is no block; seqs: the table row of each request
+(default: its number).  The reference has no counterpart.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import List, Optional, Sequence, Union
+
+import torch
+
+from . import _lib
+
+CODE = {torch.float8_e4m3fn: 0, torch.int8: 1}
+BLOCKS = (16, 32, 64)
+HEAD_DIMS = (64, 128, 256)
+POOL_SHORT, ROW_FULL, TOKENS_OVER, BAD_ROW = 1, 2, 4, 8   # status bits of a plan
+_SPLIT_BLOCKS = 1024     # workgroups of a split launch
+
+
+@dataclass
+class BlockPlan:
+    """A step: cu int32 [n + 1] (prefix sums of the token counts), slots int32 [n_tokens] (block * block size + row of every
+    token, -1 for none), kv_lens int32 [n] (lengths with the step's tokens), next_head int32 [1] (the free list's next
+    entry after the step), seqs int32 [n] (table rows)."""
+    seqs: torch.Tensor
+    cu: torch.Tensor
+    slots: torch.Tensor
+    kv_lens: torch.Tensor
+    next_head: torch.Tensor
+
+
+def _stream(*tensors: Optional[torch.Tensor]) -> int:
+    """The current stream of the tensors' device, which has to be the current one (launches go there)."""
+    cur = torch.cuda.current_device() if tensors[0].is_cuda else -1
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != cur):
+            _lib.require_device(t)
+            raise ValueError(f"tensor on {t.device}, but the current device is cuda:{cur}")
+    return _lib.stream(cur)
+
+
+def _i32(name: str, t: torch.Tensor, n: int) -> None:
+    assert t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous(), f"{name} must be a contiguous int32 vector"
+    if t.numel() < n:
+        raise ValueError(f"{name} has {t.numel()} entries, {n} are needed")
+
+
+def _pool(k8, v8, ks, vs, block_table, n, seqs):
+    """Checks of a layer's buffers; (n_blocks, H, block, D)."""
+    assert k8.dtype in CODE and v8.dtype == k8.dtype, "block codes are float8_e4m3fn or int8"
+    assert k8.dim() == 4 and v8.shape == k8.shape and k8.is_contiguous() and v8.is_contiguous()
+    nb, H, B, D = k8.shape
+    assert ks.dtype == torch.float32 and vs.dtype == torch.float32 and ks.is_contiguous() and vs.is_contiguous()
+    assert ks.shape == (nb, H) and vs.shape == (nb, H)
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1
+    if B not in BLOCKS or D not in HEAD_DIMS:
+        raise ValueError(f"blocks of {B} tokens x {D} channels: {BLOCKS} tokens and {HEAD_DIMS} channels are served")
+    if seqs is not None:
+        _i32("seqs", seqs, n)
+    elif block_table.shape[0] < n:
+        raise ValueError(f"{n} requests, but the block table has {block_table.shape[0]} rows")
+    return nb, H, B, D
+
+
+def kvt_block_plan(seqs: torch.Tensor, counts: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor,
+                   free_list: torch.Tensor, free_head: torch.Tensor, n_tokens: int, block: int = 64,
+                   status: Optional[torch.Tensor] = None, req_to_token: Optional[torch.Tensor] = None,
+                   commit: bool = True) -> BlockPlan:
+    """Plan a step on the device: request j appends counts[j] tokens to table row seqs[j], whose length is seq_lens[row].
+
+    The blocks that the requests open come from free_list (int32 [n_blocks], read from free_head[0] on) in request order
+    and are written into block_table; every token gets its slot (block * block size + row: a location of the slot-indexed
+    pools too), and with req_to_token (int32 [rows, context]) the slot of every position is recorded there.  n_tokens:
+    the length of `slots`, a host int >= the counts' sum.  commit=False leaves seq_lens and free_head as they are, to look
+    at a plan (its status, its next_head) before it is taken: the next plan starts from the same state.
+    status (int32 [1]): bits POOL_SHORT, ROW_FULL, TOKENS_OVER, BAD_ROW (a row out of range, or listed twice: the later
+    request appends nothing) are or-ed in.  At most 1,024 requests."""
+    n = seqs.numel()
+    _i32("seqs", seqs, n)
+    _i32("counts", counts, n)
+    _i32("seq_lens", seq_lens, 1)
+    _i32("free_list", free_list, 0)
+    _i32("free_head", free_head, 1)
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1
+    rows = block_table.shape[0]
+    if seq_lens.numel() < rows:
+        raise ValueError(f"seq_lens has {seq_lens.numel()} entries for {rows} table rows")
+    if status is not None:
+        _i32("status", status, 1)
+    rtt, rtt_stride, rtt_cols = None, 0, 0
+    if req_to_token is not None:
+        assert req_to_token.dtype == torch.int32 and req_to_token.dim() == 2 and req_to_token.stride(1) == 1
+        if req_to_token.shape[0] < rows:
+            raise ValueError(f"req_to_token has {req_to_token.shape[0]} rows, the block table {rows}")
+        rtt, rtt_stride, rtt_cols = req_to_token.data_ptr(), req_to_token.stride(0), req_to_token.shape[1]
+    st = _stream(seqs, counts, seq_lens, block_table, free_list, free_head, status, req_to_token)
+    dev = seqs.device
+    cu = torch.empty(n + 1, dtype=torch.int32, device=dev)
+    slots = torch.empty(n_tokens, dtype=torch.int32, device=dev)
+    kv_lens = torch.empty(n, dtype=torch.int32, device=dev)
+    next_head = torch.empty(1, dtype=torch.int32, device=dev)
+    _lib.call("kvt_block_plan", n, seqs.data_ptr(), counts.data_ptr(), seq_lens.data_ptr(), rows, block_table.data_ptr(),
+              block_table.stride(0), block_table.shape[1], free_list.data_ptr(), free_list.numel(), free_head.data_ptr(),
+              block, n_tokens, cu.data_ptr(), slots.data_ptr(), kv_lens.data_ptr(), next_head.data_ptr(),
+              _lib.ptr(status), rtt, rtt_stride, rtt_cols, int(commit), st)
+    return BlockPlan(seqs, cu, slots, kv_lens, next_head)
+
+
+def _rows16(x: torch.Tensor, per16: int) -> torch.Tensor:
+    """x itself where its rows start at 16-byte boundaries, else a contiguous copy."""
+    if x.data_ptr() % 16 or x.stride(0) % per16 or x.stride(1) % per16 or x.stride(2) != 1:
+        return x.contiguous() if not x.is_contiguous() else x.clone()
+    return x
+
+
+def kvt_block_store(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, kv_lens: torch.Tensor, k8: torch.Tensor,
+                    v8: torch.Tensor, ks: torch.Tensor, vs: torch.Tensor, block_table: torch.Tensor,
+                    seqs: Optional[torch.Tensor] = None) -> None:
+    """Quantize rows k, v ([N, H, D] bf16 / fp16 / fp32) into the blocks of their positions: rows cu[j] .. cu[j + 1] are the
+    last positions of request j's kv_lens[j] (both int32, as a plan gives them).
+
+    A block's scale is the smallest power of two s with |x| <= 448 s (e4m3) or 127 s (int8) for the call's finite values,
+    and never shrinks while the block fills: where it grows, the rows that the request held before are rounded to the new
+    scale (exact for e4m3 codes, but for those that become subnormal).  Rows of a block that the request does not hold yet
+    are left as they are.  A block must be in the table of one request of the call only."""
+    N, H, D = k.shape
+    n = kv_lens.numel()
+    nb, H8, B, D8 = _pool(k8, v8, ks, vs, block_table, n, seqs)
+    assert v.shape == k.shape and (H, D) == (H8, D8), f"rows of {H} x {D} for blocks of {H8} x {D8}"
+    assert k.dtype == v.dtype and k.dtype in _lib.DTYPE_CODE, k.dtype
+    _i32("kv_lens", kv_lens, n)
+    _i32("cu", cu, n + 1)
+    if N == 0 or n == 0:
+        return
+    st = _stream(k, v, cu, kv_lens, k8, v8, ks, vs, block_table, seqs)
+    per16 = 4 if k.dtype == torch.float32 else 8
+    k, v = _rows16(k, per16), _rows16(v, per16)
+    _lib.call("kvt_block_store", k.data_ptr(), v.data_ptr(), _lib.DTYPE_CODE[k.dtype], k.stride(0), k.stride(1),
+              v.stride(0), v.stride(1), N, H, D, cu.data_ptr(), kv_lens.data_ptr(), n, _lib.ptr(seqs),
+              block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1], CODE[k8.dtype],
+              k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B, st)
+
+
+def _parts(workspace: Optional[dict], need: int, D: int, device):
+    """Partial buffers of a split launch: need rows of D values and of (maximum, sum)."""
+    ws = workspace if workspace is not None else {}
+    o = ws.get("block_o")
+    if o is None or o.numel() < need * D or ws["block_ml"].numel() < need * 2 or o.device != device:
+        o = ws["block_o"] = torch.empty(need * D, dtype=torch.float32, device=device)
+        ws["block_ml"] = torch.empty(need * 2, dtype=torch.float32, device=device)
+    return o.data_ptr(), ws["block_ml"].data_ptr()
+
+
+def _attn_args(q, out, H, D):
+    assert q.dim() == 3 and q.dtype in (torch.bfloat16, torch.float16), "queries are bf16 or fp16 [rows, Hq, D]"
+    Hq = q.shape[1]
+    assert q.shape[2] == D, f"queries of {q.shape[2]} channels over blocks of {D}"
+    if Hq % H or Hq // H > 16 or Hq == 0:
+        raise ValueError(f"{Hq} q heads over {H} KV heads: a multiple, at most 16 each, is served")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    assert out.shape == q.shape and out.dtype in _lib.DTYPE_CODE and out.stride(2) == 1
+    return _rows16(q, 8), out, Hq
+
+
+def _splits(items: int, cap: int) -> int:
+    """Workgroups that share an item's positions: about _SPLIT_BLOCKS in all, none with fewer than 128 positions of the
+    table's capacity."""
+    return max(1, min(_SPLIT_BLOCKS // items, -(-cap // 128)))
+
+
+def kvt_block_decode(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: torch.Tensor, vs: torch.Tensor,
+                     block_table: torch.Tensor, kv_lens: torch.Tensor, seqs: Optional[torch.Tensor] = None,
+                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                     workspace: Optional[dict] = None, splits: Optional[int] = None) -> torch.Tensor:
+    """Decode attention of one query token per request: q [n, Hq, D] (bf16 / fp16), request j over its kv_lens[j] positions.
+
+    Returns out ([n, Hq, D], q's dtype unless a bf16 / fp16 / fp32 `out` is given); a request without positions gives
+    NaN (0/0).  scale: default D ** -0.5.  The lengths are read on the device; `splits` (workgroups that share a request's
+    positions) follows from the number of requests and the block table's width unless given.  `workspace` (a dict) keeps
+    the partial buffers across calls; calls that share one must not overlap."""
+    n = kv_lens.numel()
+    nb, H, B, D = _pool(k8, v8, ks, vs, block_table, n, seqs)
+    q, out, Hq = _attn_args(q, out, H, D)
+    if q.shape[0] != n:
+        raise ValueError(f"{q.shape[0]} queries for {n} requests")
+    _i32("kv_lens", kv_lens, n)
+    if n == 0:
+        return out
+    st = _stream(q, k8, v8, ks, vs, block_table, kv_lens, seqs, out)
+    cap = block_table.shape[1] * B
+    ns = _splits(n * H, cap) if splits is None else int(splits)
+    o = ml = None
+    if ns > 1:
+        o, ml = _parts(workspace, n * H * ns * 16, D, q.device)
+    _lib.call("kvt_block_decode", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], kv_lens.data_ptr(), n,
+              H, Hq, D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B,
+              block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1], _lib.ptr(seqs),
+              D ** -0.5 if scale is None else float(scale), ns, o, ml, out.data_ptr(), _lib.DTYPE_CODE[out.dtype],
+              out.stride(0), out.stride(1), st)
+    return out
+
+
+def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: torch.Tensor,
+                      vs: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
+                      seqs: Optional[torch.Tensor] = None, causal: bool = True, scale: Optional[float] = None,
+                      out: Optional[torch.Tensor] = None, workspace: Optional[dict] = None,
+                      splits: Optional[int] = None) -> torch.Tensor:
+    """Attention of chunks: q [total, Hq, D] (bf16 / fp16), request j owns rows cu_q[j] .. cu_q[j + 1] (int32 [n + 1]).
+
+    causal: the chunk's queries are the last positions of request j (its keys are in the cache already) and each sees the
+    positions up to its own: kv_lens[j] - chunk + i + 1 of them for query i.  causal=False: every query sees all
+    kv_lens[j] positions -- cross attention to another sequence's states, of any length.  A query that sees nothing gives
+    NaN (0/0).  Other arguments as kvt_block_decode."""
+    n = kv_lens.numel()
+    nb, H, B, D = _pool(k8, v8, ks, vs, block_table, n, seqs)
+    q, out, Hq = _attn_args(q, out, H, D)
+    _i32("kv_lens", kv_lens, n)
+    _i32("cu_q", cu_q, n + 1)
+    total = q.shape[0]
+    if n == 0 or total == 0:
+        return out
+    st = _stream(q, cu_q, k8, v8, ks, vs, block_table, kv_lens, seqs, out)
+    items = total * (Hq // H) // 16 + n
+    ns = _splits(items * H, block_table.shape[1] * B) if splits is None else int(splits)
+    o = ml = None
+    if ns > 1:
+        o, ml = _parts(workspace, items * H * ns * 16, D, q.device)
+    _lib.call("kvt_block_prefill", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], cu_q.data_ptr(), total,
+              kv_lens.data_ptr(), n, H, Hq, D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(),
+              nb, B, block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1],
+              _lib.ptr(seqs), int(bool(causal)), D ** -0.5 if scale is None else float(scale), ns, o, ml, out.data_ptr(),
+              _lib.DTYPE_CODE[out.dtype], out.stride(0), out.stride(1), st)
+    return out
+
+
+class BlockKVCache:
+    """Buffers of the 8-bit block cache for all layers of a model, and the step's calls over them.
+
+    Per layer k8 / v8 [n_blocks, H, block, D] and ks / vs [n_blocks, H]; shared by the layers: block_table
+    [max_seqs, max_blocks], seq_lens [max_seqs], the free list (a seeded permutation of the blocks) and its head.  Lengths, blocks and
+    the free list live on the device only; add_seq and release hand out table rows on the host."""
+
+    def __init__(self, layers: int, H: int, D: int, n_blocks: int, max_seqs: int, max_blocks: int, device="cuda",
+                 dtype: torch.dtype = torch.float8_e4m3fn, block: int = 64, seed: int = 0):
+        if dtype not in CODE:
+            raise ValueError(f"block codes are float8_e4m3fn or int8, not {dtype}")
+        if block not in BLOCKS or D not in HEAD_DIMS:
+            raise ValueError(f"blocks of {block} tokens x {D} channels: {BLOCKS} tokens and {HEAD_DIMS} channels are served")
+        if n_blocks * block > 2 ** 31:
+            raise ValueError(f"{n_blocks} blocks of {block} tokens: slots are int32")
+        self.L, self.H, self.D, self.block, self.dtype = layers, H, D, block, dtype
+        self.device = torch.device(device)
+        z = dict(device=self.device)
+        self.k8 = [torch.zeros(n_blocks, H, block, D, dtype=torch.int8, **z).view(dtype) for _ in range(layers)]
+        self.v8 = [torch.zeros(n_blocks, H, block, D, dtype=torch.int8, **z).view(dtype) for _ in range(layers)]
+        self.ks = [torch.zeros(n_blocks, H, dtype=torch.float32, **z) for _ in range(layers)]
+        self.vs = [torch.zeros(n_blocks, H, dtype=torch.float32, **z) for _ in range(layers)]
+        self.block_table = torch.full((max_seqs, max_blocks), -1, dtype=torch.int32, **z)
+        self.seq_lens = torch.zeros(max_seqs, dtype=torch.int32, **z)
+        g = torch.Generator().manual_seed(seed)
+        self.free_list = torch.randperm(n_blocks, generator=g).to(torch.int32).to(self.device)
+        self.free_head = torch.zeros(1, dtype=torch.int32, **z)
+        self.status = torch.zeros(1, dtype=torch.int32, **z)
+        self._rows: List[int] = list(range(max_seqs - 1, -1, -1))
+
+    def add_seq(self) -> int:
+        """A free table row for a new sequence."""
+        if not self._rows:
+            raise RuntimeError("no free sequence row")
+        return self._rows.pop()
+
+    def release(self, s: int) -> None:
+        """Give a sequence's blocks back to the free list and its row back to add_seq (synchronizes the device)."""
+        if s in self._rows or not 0 <= s < self.block_table.shape[0]:
+            raise ValueError(f"row {s} holds no sequence")
+        used = -(-int(self.seq_lens[s]) // self.block)
+        blocks = self.block_table[s, :used]
+        blocks = blocks[blocks >= 0]
+        head = int(self.free_head) - blocks.numel()
+        self.free_list[head:head + blocks.numel()] = blocks
+        self.free_head.fill_(head)
+        self.block_table[s].fill_(-1)
+        self.seq_lens[s] = 0
+        self._rows.append(s)
+
+    def _vec(self, x: Union[torch.Tensor, Sequence[int]]) -> torch.Tensor:
+        return x if isinstance(x, torch.Tensor) else torch.tensor(list(x), dtype=torch.int32).to(self.device)
+
+    def plan(self, seqs, counts, n_tokens: Optional[int] = None, req_to_token: Optional[torch.Tensor] = None,
+             commit: bool = True) -> BlockPlan:
+        """kvt_block_plan over this cache.  seqs / counts: int32 device vectors or lists; n_tokens: a host bound of the
+        counts' sum (needed with device counts)."""
+        if n_tokens is None:
+            if isinstance(counts, torch.Tensor):
+                raise ValueError("plan: pass n_tokens (a host int >= the counts' sum) with counts on the device")
+            n_tokens = sum(counts)
+        return kvt_block_plan(self._vec(seqs), self._vec(counts), self.seq_lens, self.block_table, self.free_list,
+                              self.free_head, n_tokens, self.block, self.status, req_to_token, commit)
+
+    def check(self) -> None:
+        """Raise RuntimeError if a plan could not be carried out in full since the last check (synchronizes the device)."""
+        bits = int(self.status)
+        if bits:
+            self.status.zero_()
+            names = [name for bit, name in ((POOL_SHORT, "block pool exhausted"), (ROW_FULL, "block table row full"),
+                                            (TOKENS_OVER, "more tokens than n_tokens"),
+                                            (BAD_ROW, "table row out of range or listed twice")) if bits & bit]
+            raise RuntimeError("block plan: " + ", ".join(names))
+
+    def append(self, layer: int, plan: BlockPlan, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Write the plan's tokens (k, v: [n_tokens, H, D]) into layer `layer`."""
+        kvt_block_store(k, v, plan.cu, plan.kv_lens, self.k8[layer], self.v8[layer], self.ks[layer], self.vs[layer],
+                        self.block_table, plan.seqs)
+
+    def decode(self, layer: int, plan: BlockPlan, q: torch.Tensor, **kw) -> torch.Tensor:
+        """Attention of one query per request of the plan, over everything appended so far."""
+        return kvt_block_decode(q, self.k8[layer], self.v8[layer], self.ks[layer], self.vs[layer], self.block_table,
+                                plan.kv_lens, plan.seqs, **kw)
+
+    def prefill(self, layer: int, plan: BlockPlan, q: torch.Tensor, **kw) -> torch.Tensor:
+        """Attention of the plan's tokens (q: [n_tokens, Hq, D])."""
+        return kvt_block_prefill(q, plan.cu, self.k8[layer], self.v8[layer], self.ks[layer], self.vs[layer],
+                                 self.block_table, plan.kv_lens, plan.seqs, **kw)

@@ -1,0 +1,477 @@
+// Attention of few rows over the 8-bit block cache on the matrix cores: decode (one query token per request) and short
+// chunks (kvt_block_decode, and kvt_block_prefill where a call has few rows).
+//
+//   out[row] = sum_p w_p sv_p vc_p / sum_p w_p,   w_p = exp(scale * sk_p * q . kc_p)
+// over the positions p that the row sees; kc, vc are codes, sk, sv the scales of p's block and KV head.  A row is a
+// (query, q head) pair of one KV head; 16 of them are one side of a matrix product.
+//
+// One workgroup of 4 wavefronts per (16 rows, KV head, split of the positions); a wavefront takes every fourth tile of 32
+// positions.  Nothing is staged in LDS: both products take their 8-bit operand from registers as it was loaded.
+//   S^T = K Q^T (v_mfma_f32_16x16x32_f16): lane (l, g) (l = lane % 16, g = lane / 16) loads 16 bytes of position l at a
+//     time; the k order of the product is the order of the bytes, and Q is loaded in the same order.
+//   The result gives a lane four positions (4 g + i) of row l in each of the tile's two halves: these eight weights are
+//     the lane's column of P^T in O^T += V^T P^T as they stand.  V^T's operand needs the same eight positions of one channel: a
+//     lane loads D / 16 channels of each of them and pairs the bytes of two positions (v_perm_b32) before the conversion.
+// Codes are exact in fp16.  The scale of K multiplies the fp32 scores.  The scale of V is folded into P, relative to a
+// running unit u: P holds w sv / u and O is kept in units of u, which changes only when a tile's scale leaves [u / 4, u]
+// (O is then multiplied by the ratio; two blocks of one tile whose scales differ by more than 4 take a product each).  The softmax keeps a running maximum m per row that moves only when a tile
+// exceeds it by more than 4 (in powers of two), and P = 2^(x - m + 10): fp16 has weights down to 2^-24 of the largest before
+// they lose bits, and up to 2^14 for a row whose maximum lags.  Sums, scores and O are fp32.  bf16 queries are scaled by
+// a power of two per row to fit fp16 (exact down to 2^-14 of the row's largest entry, and to 2^-25 of it below).
+#include "block_common.h"
+
+using namespace kvt;
+using namespace kvt::blk;
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kTile = 32;
+constexpr float kLag = 4.0f, kLift = 10.0f;
+
+struct Attn {
+  const void* q;               // [rows, Hq, D]
+  const uint8_t* k8;
+  const uint8_t* v8;
+  const float* ks;
+  const float* vs;
+  const int32_t* table;
+  const int32_t* kv_lens;
+  const int32_t* rows;         // table row of a request (NULL: its number)
+  const int32_t* cu;           // NULL: one query per request
+  void* out;
+  float* part_o;
+  float* part_ml;
+  int64_t sq_n, sq_h, so_n, so_h, stride;
+  float scale_log2;
+  int n, n_rows, n_q, H, gs, n_blocks, max_blocks, log2b, splits, causal;
+};
+
+// What a workgroup has: request r, query rows [row0, row0 + n_row) of it in (query, q head) order, the query base, and the
+// positions that any of its rows sees.
+struct Item {
+  int r, trow, q0, q_len, row0, n_row, kv, len, limit;
+};
+
+// Positions that query qi of the item's request sees.
+KVT_DEV int sees(const Attn& P, const Item& t, int qi) {
+  return P.causal ? min(t.len, max(t.kv - t.q_len + qi + 1, 0)) : t.len;
+}
+
+KVT_DEV Item item_of(const Attn& P, int w) {
+  Item t;
+  if (P.cu == nullptr) {
+    t.r = w, t.q0 = w, t.q_len = 1, t.row0 = 0, t.n_row = P.gs;
+  } else {
+    t.r = find_request(P.cu, P.n, w, P.gs, 16, 1);
+    t.q0 = min(max(P.cu[t.r], 0), P.n_q);
+    t.q_len = min(max(P.cu[t.r + 1], t.q0), P.n_q) - t.q0;
+    const int64_t row0 = (w - first_item(P.cu[t.r], t.r, P.gs, 16, 1)) * 16;
+    const int64_t left = (int64_t)t.q_len * P.gs - row0;
+    t.row0 = (int)row0;
+    t.n_row = row0 < 0 || left <= 0 ? 0 : (int)min(left, (int64_t)16);
+  }
+  t.trow = P.rows ? P.rows[t.r] : t.r;
+  t.kv = max(P.kv_lens[t.r], 0);
+  t.len = (int)min((int64_t)t.kv, (int64_t)P.max_blocks << P.log2b);
+  if (t.trow < 0 || t.trow >= P.n_rows) t.len = 0, t.trow = 0;
+  t.limit = t.n_row > 0 ? sees(P, t, (t.row0 + t.n_row - 1) / P.gs) : 0;
+  return t;
+}
+
+// Tiles of 32 positions per split: a multiple of the wavefronts.
+KVT_DEV int tiles_per_split(int limit, int splits) {
+  const int tiles = (limit + kTile - 1) / kTile;
+  return max(((tiles + splits - 1) / splits + kWaves - 1) / kWaves * kWaves, kWaves);
+}
+
+template <int BYTES> struct Raw { uint32_t w[BYTES / 4]; };
+template <int BYTES>
+KVT_DEV Raw<BYTES> load(const uint8_t* base, uint32_t off) {
+  Raw<BYTES> r;
+  if constexpr (BYTES == 16) {
+    const u4v x = *reinterpret_cast<const u4v*>(base + off);
+    r.w[0] = x.x, r.w[1] = x.y, r.w[2] = x.z, r.w[3] = x.w;
+  } else if constexpr (BYTES == 8) {
+    const u2v x = *reinterpret_cast<const u2v*>(base + off);
+    r.w[0] = x.x, r.w[1] = x.y;
+  } else {
+    r.w[0] = *reinterpret_cast<const uint32_t*>(base + off);
+  }
+  return r;
+}
+
+KVT_DEV f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+KVT_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }   // (v_exp_f32: results below 2^-126 are 0)
+KVT_DEV float bits_f(uint32_t u) { return __uint_as_float(u); }
+KVT_DEV float lane_f(float v, int lane) {
+  return bits_f((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
+}
+
+// A row of Q in operand order: chunk c (16 channels of group g at 64 c + 16 g) is two operands.  bf16 rows are scaled by
+// 2^-e to fp16 range; returns 2^e.
+template <int QT, int D>
+KVT_DEV float load_q(const void* q, int64_t at, bool live, int g, h8 (&out)[D / 32]) {
+  constexpr int NC = D / 64;
+  uint4 raw[NC][2];
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      raw[c][i] = live ? *reinterpret_cast<const uint4*>((const uint16_t*)q + at + 64 * c + 16 * g + 8 * i) : make_uint4(0, 0, 0, 0);
+  if constexpr (QT == kF16) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) out[2 * c + i] = __builtin_bit_cast(h8, raw[c][i]);
+    return 1.0f;
+  } else {
+    float top = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t w[4] = {raw[c][i].x, raw[c][i].y, raw[c][i].z, raw[c][i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(bits_f(w[k] << 16)), fabsf(bits_f(w[k] & 0xFFFF0000u))));
+      }
+    top = max_xor16_32(top);
+    int e = (int)(__float_as_uint(top) >> 23) - 127;
+    e = top > 0.0f && top < __builtin_inff() ? min(max(e, -120), 120) : 0;
+    const float f = bits_f((uint32_t)(127 - e) << 23);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t w[4] = {raw[c][i].x, raw[c][i].y, raw[c][i].z, raw[c][i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          out[2 * c + i][2 * k] = (_Float16)(bits_f(w[k] << 16) * f);
+          out[2 * c + i][2 * k + 1] = (_Float16)(bits_f(w[k] & 0xFFFF0000u) * f);
+        }
+      }
+    return bits_f((uint32_t)(127 + e) << 23);
+  }
+}
+
+KVT_DEV void store_out(void* out, int ot, int64_t at, float v) {
+  if (ot == kF32) ((float*)out)[at] = v;
+  else if (ot == kBF16) ((uint16_t*)out)[at] = bf16_rne(v);
+  else ((uint16_t*)out)[at] = f32_to_f16_bits(v);
+}
+
+template <int CODE, int QT, int D>
+__global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot) {
+  constexpr int NC = D / 64;          // 16-byte chunks of a K row per lane
+  constexpr int VB = D / 16;          // bytes (channels) of a V row per lane
+  constexpr int LD = D + 4;
+  __shared__ float lo[kWaves][16][LD];
+  __shared__ float lm[kWaves][16], ll[kWaves][16], lu[kWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+  const int split = blockIdx.x, h = blockIdx.y, w = blockIdx.z;
+  const Item it = item_of(P, w);
+  if (it.n_row == 0) return;
+  const int tps = tiles_per_split(it.limit, P.splits);
+  const int tile0 = split * tps, tile1 = min(tile0 + tps, (it.limit + kTile - 1) / kTile);
+  if (tile0 >= tile1 && P.splits > 1) return;       // (the merge knows which splits there are)
+
+  const int my = it.row0 + l, qi = my / P.gs, hq = h * P.gs + my % P.gs;
+  const bool live = l < it.n_row;
+  h8 Q[D / 32];
+  const float qf = load_q<QT, D>(P.q, (int64_t)(it.q0 + qi) * P.sq_n + (int64_t)hq * P.sq_h, live, g, Q) * P.scale_log2;
+  const int see = sees(P, it, qi);
+  const int all_see = sees(P, it, it.row0 / P.gs);   // (the fewest of the item's rows: positions below it need no comparison)
+
+  f4 acc[VB];
+#pragma unroll
+  for (int c = 0; c < VB; ++c) acc[c] = f4{0, 0, 0, 0};
+  float m = -__builtin_inff(), sum = 0.0f, unit = 0.0f;
+
+  const uint32_t koff = (uint32_t)l * D + 16u * g, voff = 4u * g * D + (uint32_t)l * VB;
+  const int64_t tbl = (int64_t)it.trow * P.stride;
+
+  for (int base = tile0 + wave; base < tile1; base += 32 * kWaves) {
+    // blocks and scales of the next 32 tiles: lane 2 i + s has half s of tile base + 4 i
+    int id = -1;
+    float sk = 0.0f, sv = 0.0f;
+    {
+      const int p = (base + (lane >> 1) * kWaves) * kTile + 16 * (lane & 1);
+      if (p < it.limit) id = P.table[tbl + (p >> P.log2b)];
+      if (id < 0 || id >= P.n_blocks) id = -1;
+      if (id >= 0) sk = P.ks[(int64_t)id * P.H + h], sv = P.vs[(int64_t)id * P.H + h];
+    }
+    for (int i = 0; i < 32; ++i) {
+      const int tile = base + i * kWaves;
+      if (tile >= tile1) break;
+      const int p0 = tile * kTile;
+      int valid[2];
+      const uint8_t *kp[2], *vp[2];
+      float fk[2], fv[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int b = __builtin_amdgcn_readlane(id, 2 * i + s);
+        valid[s] = b < 0 ? 0 : min(max(it.limit - (p0 + 16 * s), 0), 16);
+        const int64_t at = ((((int64_t)max(b, 0) * P.H + h) << P.log2b) + ((p0 + 16 * s) & ((1 << P.log2b) - 1))) * D;
+        kp[s] = P.k8 + at, vp[s] = P.v8 + at;
+        fk[s] = lane_f(sk, 2 * i + s), fv[s] = lane_f(sv, 2 * i + s);
+      }
+      Raw<16> kr[2][NC];
+      Raw<VB> vr[2][4];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) kr[s][c] = load<16>(kp[s], koff + 64u * c);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vr[s][j] = load<VB>(vp[s], voff + (uint32_t)j * D);
+
+      float x[2][4];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        f4 sc = {0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          sc = mfma(operand<CODE>(kr[s][c].w[0], kr[s][c].w[1]), Q[2 * c], sc);
+          sc = mfma(operand<CODE>(kr[s][c].w[2], kr[s][c].w[3]), Q[2 * c + 1], sc);
+        }
+        const float f = qf * fk[s];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[s][j] = sc[j] * f;
+      }
+      if (valid[0] + valid[1] < 32 || p0 + 32 > all_see) {
+        // positions past a row's end, in a block that is not there, or stale (their V may hold anything: it counts as 0)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int at = 4 * g + j;
+            x[s][j] = at < valid[s] && p0 + 16 * s + at < see ? x[s][j] : -__builtin_inff();
+#pragma unroll
+            for (int d = 0; d < VB / 4; ++d) vr[s][j].w[d] = at < valid[s] ? vr[s][j].w[d] : 0u;
+          }
+      }
+      float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                        fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+      top = max_xor16_32(top);
+      const bool rise = top > m + kLag;
+      if (__any(rise)) {
+        const float m1 = rise ? top : m;
+        const float a = m1 == m ? 1.0f : exp2_(m - m1);             // (m = -inf: 0)
+        sum *= a;
+        m = m1;
+#pragma unroll
+        for (int c = 0; c < VB; ++c) acc[c] *= a;
+      }
+      const float ms = (m == -__builtin_inff() ? 0.0f : m) - kLift;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[s][j] = exp2_(x[s][j] - ms);
+          sum += x[s][j];
+        }
+      // (two blocks whose scales are far apart in one tile: one product for each, so that neither's weights leave fp16)
+      const bool far = fminf(fv[0], fv[1]) > 0.0f && (fv[0] < 0.25f * fv[1] || fv[1] < 0.25f * fv[0]);
+      for (int pass = 0; pass <= (int)far; ++pass) {
+        const float big = far ? fv[pass] : fmaxf(fv[0], fv[1]);
+        if (big > unit || big < 0.25f * unit) {                     // uniform
+          const float u1 = fmaxf(big, unit * 0x1p-90f);             // (the ratio stays finite)
+          const float a = u1 > 0.0f ? unit / u1 : 1.0f;
+          unit = u1;
+#pragma unroll
+          for (int c = 0; c < VB; ++c) acc[c] *= a;
+        }
+        h8 p;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const float ru = unit > 0.0f && !(far && s != pass) ? fv[s] / unit : 0.0f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p[4 * s + j] = (_Float16)(x[s][j] * ru);
+        }
+#pragma unroll
+        for (int d = 0; d < VB / 4; ++d) {
+          uint32_t lo4[4], hi4[4];                                  // {pair (0,1), (2,3) of half 0, of half 1}
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t a = flip<CODE>(vr[s][2 * j].w[d]), b = flip<CODE>(vr[s][2 * j + 1].w[d]);
+              lo4[2 * s + j] = __builtin_amdgcn_perm(b, a, 0x05010400u);   // a0 b0 a1 b1
+              hi4[2 * s + j] = __builtin_amdgcn_perm(b, a, 0x07030602u);   // a2 b2 a3 b3
+            }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            h2 y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t u = c < 2 ? lo4[k] : hi4[k];
+              y[k] = c & 1 ? pair<CODE, true>(u) : pair<CODE, false>(u);
+            }
+            const h8 a = {y[0].x, y[0].y, y[1].x, y[1].y, y[2].x, y[2].y, y[3].x, y[3].y};
+            acc[4 * d + c] = mfma(a, p, acc[4 * d + c]);
+          }
+        }
+      }
+    }
+  }
+
+  // the wavefronts' parts -> one: acc[c][i] is channel VB (4 g + i) + c of row l
+  sum = sum_xor16_32(sum);
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < VB; c += 4)
+        *reinterpret_cast<f4*>(&lo[wave][l][VB * (4 * g + i) + c]) = f4{acc[c][i], acc[c + 1][i], acc[c + 2][i], acc[c + 3][i]};
+    if (g == 0) lm[wave][l] = m, ll[wave][l] = sum;
+  }
+  if (lane == 0) lu[wave] = unit;
+  __syncthreads();
+  for (int e = threadIdx.x; e < it.n_row * (D / 4); e += 256) {
+    const int row = e / (D / 4), d = 4 * (e % (D / 4));
+    float M = -__builtin_inff();
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) M = fmaxf(M, lm[v][row]);
+    float L = 0.0f;
+    f4 O = {0, 0, 0, 0};
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      const float mv = lm[v][row], f = mv == -__builtin_inff() ? 0.0f : exp2_(mv - M);
+      L += f * ll[v][row];
+      const float fu = f * lu[v];
+      const f4 o = *reinterpret_cast<const f4*>(&lo[v][row][d]);
+      // (a wavefront without positions counts 0, whatever its state holds)
+      O += mv == -__builtin_inff() && ll[v][row] == 0.0f ? f4{0, 0, 0, 0} : o * fu;
+    }
+    if (P.splits == 1) {
+      const int at = it.row0 + row;
+      const int64_t o = (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + d;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) store_out(P.out, ot, o + i, O[i] / L);
+    } else {
+      const int64_t part = (((int64_t)w * P.H + h) * P.splits + split) * 16 + row;
+      *reinterpret_cast<f4*>(P.part_o + part * D + d) = O;
+      if (d == 0) P.part_ml[2 * part] = M, P.part_ml[2 * part + 1] = L;
+    }
+  }
+}
+
+// Merge of a row's splits: one workgroup per (16 rows, KV head, row); D / 4 threads per split side by side.
+template <int D>
+__global__ __launch_bounds__(256) void block_merge_kernel(const Attn P, int ot) {
+  constexpr int TP = D / 4, NG = 256 / TP;
+  __shared__ float red[4];
+  __shared__ f4 os[NG][TP];
+  __shared__ float ls[NG];
+  const int row = blockIdx.x, h = blockIdx.y, w = blockIdx.z;
+  const Item it = item_of(P, w);
+  if (row >= it.n_row) return;
+  const int tps = tiles_per_split(it.limit, P.splits);
+  const int used = ((it.limit + kTile - 1) / kTile + tps - 1) / tps;
+  const int64_t part = ((int64_t)w * P.H + h) * P.splits * 16 + row;
+  float M = -__builtin_inff();
+  for (int s = threadIdx.x; s < used; s += 256) M = fmaxf(M, P.part_ml[2 * (part + 16 * s)]);
+  M = group_max<64>(M);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const int grp = threadIdx.x / TP, d = threadIdx.x % TP;
+  f4 O = {0, 0, 0, 0};
+  float L = 0.0f;
+  for (int s = grp; s < used; s += NG) {
+    const int64_t at = part + 16 * s;
+    const float ms = P.part_ml[2 * at], f = ms == -__builtin_inff() ? 0.0f : exp2_(ms - M);
+    L += f * P.part_ml[2 * at + 1];
+    O += f * *reinterpret_cast<const f4*>(P.part_o + at * D + 4 * d);
+  }
+  os[grp][d] = O;
+  if (d == 0) ls[grp] = L;
+  __syncthreads();
+  if (grp) return;
+#pragma unroll
+  for (int i = 1; i < NG; ++i) O += os[i][d], L += ls[i];
+  const int at = it.row0 + row;
+  const int64_t o = (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + 4 * d;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) store_out(P.out, ot, o + i, O[i] / L);
+}
+
+template <int CODE, int QT, int D>
+void launch(const Attn& P, int items, int rows, int ot, hipStream_t st) {
+  block_rows_kernel<CODE, QT, D><<<dim3(P.splits, P.H, items), 256, 0, st>>>(P, ot);
+  if (P.splits > 1) block_merge_kernel<D><<<dim3(rows, P.H, items), 256, 0, st>>>(P, ot);
+}
+template <int CODE, int QT>
+void launch_d(const Attn& P, int D, int items, int rows, int ot, hipStream_t st) {
+  if (D == 64) launch<CODE, QT, 64>(P, items, rows, ot, st);
+  else if (D == 128) launch<CODE, QT, 128>(P, items, rows, ot, st);
+  else launch<CODE, QT, 256>(P, items, rows, ot, st);
+}
+void launch_all(const Attn& P, int code, int qt, int D, int items, int rows, int ot, hipStream_t st) {
+  if (code == kE4M3) {
+    if (qt == kBF16) launch_d<kE4M3, kBF16>(P, D, items, rows, ot, st);
+    else launch_d<kE4M3, kF16>(P, D, items, rows, ot, st);
+  } else {
+    if (qt == kBF16) launch_d<kI8, kBF16>(P, D, items, rows, ot, st);
+    else launch_d<kI8, kF16>(P, D, items, rows, ot, st);
+  }
+}
+
+int check(const Attn& P, int Hq, int D, int block, int code, int qt, int ot) {
+  if (P.n < 1 || P.n > kMaxReq || P.H < 1 || Hq < P.H || Hq % P.H || Hq / P.H > 16 || P.n_rows < 1 || P.n_blocks < 1 ||
+      P.max_blocks < 1 || P.stride < P.max_blocks || (!P.rows && P.n_rows < P.n) || P.splits < 1)
+    return KVT_EINVAL;
+  if ((D != 64 && D != 128 && D != 256) || (block != 16 && block != 32 && block != 64)) return KVT_EINVAL;
+  if ((code != kE4M3 && code != kI8) || (qt != kBF16 && qt != kF16) || (ot != kBF16 && ot != kF16 && ot != kF32))
+    return KVT_EINVAL;
+  if ((uintptr_t)P.q & 15 || P.sq_n % 8 || P.sq_h % 8 || ((uintptr_t)P.k8 | (uintptr_t)P.v8) & 15) return KVT_EINVAL;
+  if (P.H > 65535 || (int64_t)P.max_blocks * block > 0x7FFFFFFF) return KVT_ERANGE;
+  return KVT_OK;
+}
+
+}  // namespace
+
+extern "C" int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q_type, const void* kv_lens, int n, int H,
+                                int Hq, int D, int code, const void* k8, const void* v8, const void* ks, const void* vs,
+                                int n_blocks, int block, const void* block_table, int64_t bt_stride, int n_rows,
+                                int max_blocks, const void* rows, float scale, int n_splits, void* part_o,
+                                void* part_ml, void* out, int out_type, int64_t so_n, int64_t so_h, void* stream) {
+  Attn P;
+  P.q = q, P.k8 = (const uint8_t*)k8, P.v8 = (const uint8_t*)v8, P.ks = (const float*)ks, P.vs = (const float*)vs;
+  P.table = (const int32_t*)block_table, P.kv_lens = (const int32_t*)kv_lens, P.rows = (const int32_t*)rows;
+  P.cu = nullptr, P.out = out, P.part_o = (float*)part_o, P.part_ml = (float*)part_ml;
+  P.sq_n = sq_n, P.sq_h = sq_h, P.so_n = so_n, P.so_h = so_h, P.stride = bt_stride, P.scale_log2 = scale * kLog2e;
+  P.n = n, P.n_rows = n_rows, P.n_q = n, P.H = H, P.gs = H > 0 ? Hq / H : 0, P.n_blocks = n_blocks;
+  P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.splits = n_splits, P.causal = 0;
+  const int st = check(P, Hq, D, block, code, q_type, out_type);
+  if (st != KVT_OK) return st;
+  if (n_splits > 1 && (!part_o || !part_ml)) return KVT_EINVAL;
+  launch_all(P, code, q_type, D, n, P.gs, out_type, (hipStream_t)stream);
+  KVT_CHECK_LAUNCH();
+  return KVT_OK;
+}
+
+extern "C" int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int q_type, const void* cu_q, int n_q,
+                                 const void* kv_lens, int n, int H, int Hq, int D, int code, const void* k8,
+                                 const void* v8, const void* ks, const void* vs, int n_blocks, int block,
+                                 const void* block_table, int64_t bt_stride, int n_rows, int max_blocks,
+                                 const void* rows, int causal, float scale, int n_splits, void* part_o, void* part_ml,
+                                 void* out, int out_type, int64_t so_n, int64_t so_h, void* stream) {
+  Attn P;
+  P.q = q, P.k8 = (const uint8_t*)k8, P.v8 = (const uint8_t*)v8, P.ks = (const float*)ks, P.vs = (const float*)vs;
+  P.table = (const int32_t*)block_table, P.kv_lens = (const int32_t*)kv_lens, P.rows = (const int32_t*)rows;
+  P.cu = (const int32_t*)cu_q, P.out = out, P.part_o = (float*)part_o, P.part_ml = (float*)part_ml;
+  P.sq_n = sq_n, P.sq_h = sq_h, P.so_n = so_n, P.so_h = so_h, P.stride = bt_stride, P.scale_log2 = scale * kLog2e;
+  P.n = n, P.n_rows = n_rows, P.n_q = n_q, P.H = H, P.gs = H > 0 ? Hq / H : 0, P.n_blocks = n_blocks;
+  P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.splits = n_splits, P.causal = causal;
+  const int st = check(P, Hq, D, block, code, q_type, out_type);
+  if (st != KVT_OK) return st;
+  if (!cu_q || n_q < 0 || (n_splits > 1 && (!part_o || !part_ml))) return KVT_EINVAL;
+  if (n_q == 0) return KVT_OK;
+  const int64_t items = (int64_t)n_q * P.gs / 16 + n;
+  if (items > 65535) return KVT_ERANGE;
+  launch_all(P, code, q_type, D, (int)items, 16, out_type, (hipStream_t)stream);
+  KVT_CHECK_LAUNCH();
+  return KVT_OK;
+}

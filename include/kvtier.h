@@ -344,7 +344,7 @@ int kvt_block_store(const void* k, const void* v, int dtype, int64_t sk_n, int64
 /* Decode attention of one query token per request: out[j, h] = softmax(scale q K^T) V over positions < kv_lens[j].  q
  * (q_type 0 bf16, 1 fp16; 16-byte aligned, strides multiples of 8) and out (out_type 0 bf16, 1 fp16, 2 fp32) are [n, Hq, D]
  * with element strides of token and head.  Hq / H <= 16, n <= 4,096.  n_splits > 1: the positions of a request are shared
- * by up to n_splits workgroups, merged by a second launch; part_o fp32 [n * H * n_splits * 16 * D] and part_ml fp32 [n *
+ * by up to n_splits workgroups, merged by a second launch (at most 1,024; n * H <= 65,535 then); part_o fp32 [n * H * n_splits * 16 * D] and part_ml fp32 [n *
  * H * n_splits * 32] hold their parts.  A request without positions gives NaN (0/0). */
 int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q_type, const void* kv_lens, int n, int H, int Hq,
                      int D, int code, const void* k8, const void* v8, const void* ks, const void* vs, int n_blocks,
@@ -354,13 +354,15 @@ int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q_type, cons
 
 /* Attention of chunks of queries: request j owns rows cu_q[j] .. cu_q[j+1] (int32 [n + 1], at most n_q) of q / out.  causal: its
  * queries are the last positions of kv_lens[j] and see the positions up to their own; else every query sees all kv_lens[j]
- * positions (cross attention).  Rows of q / out behind cu_q[n] are left as they are.  Otherwise as kvt_block_decode, with the
- * parts per item: items = n_q * (Hq / H) / 16 + n in the place of n. */
+ * positions (cross attention).  Rows of q / out behind cu_q[n] are left as they are.  item_rows = 128: query tiles of 128
+ * (query, q head) rows per workgroup; 16: the decode kernel, for requests of few rows (at most 65,535 items).  Otherwise as
+ * kvt_block_decode, with n_splits <= 1,024 and the parts per item: items = n_q * (Hq / H) / item_rows + n in the place of
+ * n, item_rows rows in the place of 16; n_splits > 1 takes at most 65,535 / H items. */
 int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int q_type, const void* cu_q, int n_q,
                       const void* kv_lens, int n, int H, int Hq, int D, int code, const void* k8, const void* v8,
                       const void* ks, const void* vs, int n_blocks, int block, const void* block_table,
                       int64_t bt_stride, int n_rows, int max_blocks, const void* rows, int causal, float scale,
-                      int n_splits, void* part_o, void* part_ml, void* out, int out_type, int64_t so_n, int64_t so_h,
+                      int item_rows, int n_splits, void* part_o, void* part_ml, void* out, int out_type, int64_t so_n, int64_t so_h,
                       void* stream);
 
 /* ----------------------------------------------------------------------------- lazy backing (HIP VMM) */

@@ -29,6 +29,8 @@ BLOCKS = (16, 32, 64)
 HEAD_DIMS = (64, 128, 256)
 POOL_SHORT, ROW_FULL, TOKENS_OVER, BAD_ROW = 1, 2, 4, 8   # status bits of a plan
 _SPLIT_BLOCKS = 1024     # workgroups of a split launch
+_TILE_ROWS = 128         # (query, q head) rows of a workgroup of the query-tile kernel
+_TILE_MIN = 64           # rows per request and KV head from which it serves a call
 
 
 @dataclass
@@ -235,15 +237,16 @@ def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8:
     if n == 0 or total == 0:
         return out
     st = _stream(q, cu_q, k8, v8, ks, vs, block_table, kv_lens, seqs, out)
-    items = total * (Hq // H) // 16 + n
+    rows = _TILE_ROWS if total * (Hq // H) >= _TILE_MIN * n else 16
+    items = total * (Hq // H) // rows + n
     ns = _splits(items * H, block_table.shape[1] * B) if splits is None else int(splits)
     o = ml = None
     if ns > 1:
-        o, ml = _parts(workspace, items * H * ns * 16, D, q.device)
+        o, ml = _parts(workspace, items * H * ns * rows, D, q.device)
     _lib.call("kvt_block_prefill", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], cu_q.data_ptr(), total,
               kv_lens.data_ptr(), n, H, Hq, D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(),
               nb, B, block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1],
-              _lib.ptr(seqs), int(bool(causal)), D ** -0.5 if scale is None else float(scale), ns, o, ml, out.data_ptr(),
+              _lib.ptr(seqs), int(bool(causal)), D ** -0.5 if scale is None else float(scale), rows, ns, o, ml, out.data_ptr(),
               _lib.DTYPE_CODE[out.dtype], out.stride(0), out.stride(1), st)
     return out
 

@@ -1,0 +1,133 @@
+// What the attention kernels of the 8-bit block cache share (block_rows.hip, block_tile.hip): arguments, work items, the
+// division of an item's positions into splits, and query rows in operand order.
+#pragma once
+
+#include "block_common.h"
+
+namespace kvt {
+namespace blk {
+
+constexpr float kLag = 4.0f;     // a row's running maximum moves when a tile exceeds it by more (powers of two)
+constexpr float kLift = 10.0f;   // weights are held times 2^10: P = 2^(x - m + 10), at most 2^14, in fp16
+
+struct Attn {
+  const void* q;               // [rows, Hq, D]
+  const uint8_t* k8;
+  const uint8_t* v8;
+  const float* ks;
+  const float* vs;
+  const int32_t* table;
+  const int32_t* kv_lens;
+  const int32_t* rows;         // table row of a request (NULL: its number)
+  const int32_t* cu;           // NULL: one query per request
+  void* out;
+  float* part_o;
+  float* part_ml;
+  int64_t sq_n, sq_h, so_n, so_h, stride;
+  float scale_log2;
+  int n, n_rows, n_q, H, gs, n_blocks, max_blocks, log2b, splits, causal;
+  int item_rows;               // rows of a work item
+  int tile, least;             // positions of a tile, fewest tiles of a split
+};
+
+// What a workgroup has: request r, query rows [row0, row0 + n_row) of it in (query, q head) order, the query base, and the
+// positions that any of its rows sees.
+struct Item {
+  int r, trow, q0, q_len, row0, n_row, kv, len, limit;
+};
+
+// Positions that query qi of the item's request sees.
+KVT_DEV int sees(const Attn& P, const Item& t, int qi) {
+  return P.causal ? min(t.len, max(t.kv - t.q_len + qi + 1, 0)) : t.len;
+}
+
+KVT_DEV Item item_of(const Attn& P, int w) {
+  Item t;
+  if (P.cu == nullptr) {
+    t.r = w, t.q0 = w, t.q_len = 1, t.row0 = 0, t.n_row = P.gs;
+  } else {
+    t.r = find_request(P.cu, P.n, w, P.gs, P.item_rows, 1);
+    t.q0 = min(max(P.cu[t.r], 0), P.n_q);
+    t.q_len = min(max(P.cu[t.r + 1], t.q0), P.n_q) - t.q0;
+    const int64_t row0 = (w - first_item(P.cu[t.r], t.r, P.gs, P.item_rows, 1)) * P.item_rows;
+    const int64_t left = (int64_t)t.q_len * P.gs - row0;
+    t.row0 = (int)row0;
+    t.n_row = row0 < 0 || left <= 0 ? 0 : (int)min(left, (int64_t)P.item_rows);
+  }
+  t.trow = P.rows ? P.rows[t.r] : t.r;
+  t.kv = max(P.kv_lens[t.r], 0);
+  t.len = (int)min((int64_t)t.kv, (int64_t)P.max_blocks << P.log2b);
+  if (t.trow < 0 || t.trow >= P.n_rows) t.len = 0, t.trow = 0;
+  t.limit = t.n_row > 0 ? sees(P, t, (t.row0 + t.n_row - 1) / P.gs) : 0;
+  return t;
+}
+
+// Tiles per split of an item whose rows see `limit` positions: a multiple of `least`.  Splits behind the last tile are empty.
+KVT_DEV int tiles_of(const Attn& P, int limit) { return (limit + P.tile - 1) / P.tile; }
+KVT_DEV int tiles_per_split(const Attn& P, int limit) {
+  const int per = (tiles_of(P, limit) + P.splits - 1) / P.splits;
+  return max((per + P.least - 1) / P.least, 1) * P.least;
+}
+
+KVT_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }   // (v_exp_f32: results below 2^-126 are 0)
+KVT_DEV float bits_f(uint32_t u) { return __uint_as_float(u); }
+
+// O's unit becomes the V scale fv > 0, but no less than 2^-80 of the largest so far (|O| in units of that is below 2^40, so
+// it stays finite); returns the factor for O.
+KVT_DEV float new_unit(float fv, float& unit, float& peak) {
+  peak = fmaxf(peak, fv);
+  const float u = fmaxf(fv, peak * 0x1p-80f), a = unit / u;
+  unit = u;
+  return a;
+}
+
+KVT_DEV void store_out(void* out, int ot, int64_t at, float v) {
+  if (ot == kF32) ((float*)out)[at] = v;
+  else if (ot == kBF16) ((uint16_t*)out)[at] = bf16_rne(v);
+  else ((uint16_t*)out)[at] = f32_to_f16_bits(v);
+}
+
+// Eight elements of a query row each at at(k), k < N -> operands.  bf16 rows are scaled by a power of two to fit fp16;
+// returns its inverse.  top_of reduces a lane's largest |q| over the lanes that share its row.
+template <int QT, int N, class At, class Top>
+KVT_DEV float load_q(const void* q, int64_t row, bool live, At at, Top top_of, h8 (&out)[N]) {
+  uint4 raw[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    raw[k] = live ? *reinterpret_cast<const uint4*>((const uint16_t*)q + row + at(k)) : make_uint4(0, 0, 0, 0);
+  if constexpr (QT == kF16) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) out[k] = __builtin_bit_cast(h8, raw[k]);
+    return 1.0f;
+  } else {
+    float top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(bits_f(w[i] << 16)), fabsf(bits_f(w[i] & 0xFFFF0000u))));
+    }
+    top = top_of(top);
+    int e = (int)(__float_as_uint(top) >> 23) - 127;
+    e = top > 0.0f && top < __builtin_inff() ? min(max(e, -120), 120) : 0;
+    const float f = bits_f((uint32_t)(127 - e) << 23);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const uint32_t w[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        out[k][2 * i] = (_Float16)(bits_f(w[i] << 16) * f);
+        out[k][2 * i + 1] = (_Float16)(bits_f(w[i] & 0xFFFF0000u) * f);
+      }
+    }
+    return bits_f((uint32_t)(127 + e) << 23);
+  }
+}
+
+// Launch of the query-tile kernel (block_tile.hip): one workgroup per (kTileRows rows, KV head, split).
+constexpr int kTileRows = 128;
+int tile_positions(int D);
+void tile_launch(const Attn& P, int code, int qt, int D, int items, int ot, hipStream_t st);
+
+}  // namespace blk
+}  // namespace kvt

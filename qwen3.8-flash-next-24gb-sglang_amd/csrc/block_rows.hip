@@ -18,7 +18,7 @@
 // exceeds it by more than 4 (in powers of two), and P = 2^(x - m + 10): fp16 has weights down to 2^-24 of the largest before
 // they lose bits, and up to 2^14 for a row whose maximum lags.  Sums, scores and O are fp32.  bf16 queries are scaled by
 // a power of two per row to fit fp16 (exact down to 2^-14 of the row's largest entry, and to 2^-25 of it below).
-#include "block_common.h"
+#include "block_attn.h"
 
 using namespace kvt;
 using namespace kvt::blk;
@@ -27,63 +27,7 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr int kTile = 32;
-constexpr float kLag = 4.0f, kLift = 10.0f;
-
-struct Attn {
-  const void* q;               // [rows, Hq, D]
-  const uint8_t* k8;
-  const uint8_t* v8;
-  const float* ks;
-  const float* vs;
-  const int32_t* table;
-  const int32_t* kv_lens;
-  const int32_t* rows;         // table row of a request (NULL: its number)
-  const int32_t* cu;           // NULL: one query per request
-  void* out;
-  float* part_o;
-  float* part_ml;
-  int64_t sq_n, sq_h, so_n, so_h, stride;
-  float scale_log2;
-  int n, n_rows, n_q, H, gs, n_blocks, max_blocks, log2b, splits, causal;
-};
-
-// What a workgroup has: request r, query rows [row0, row0 + n_row) of it in (query, q head) order, the query base, and the
-// positions that any of its rows sees.
-struct Item {
-  int r, trow, q0, q_len, row0, n_row, kv, len, limit;
-};
-
-// Positions that query qi of the item's request sees.
-KVT_DEV int sees(const Attn& P, const Item& t, int qi) {
-  return P.causal ? min(t.len, max(t.kv - t.q_len + qi + 1, 0)) : t.len;
-}
-
-KVT_DEV Item item_of(const Attn& P, int w) {
-  Item t;
-  if (P.cu == nullptr) {
-    t.r = w, t.q0 = w, t.q_len = 1, t.row0 = 0, t.n_row = P.gs;
-  } else {
-    t.r = find_request(P.cu, P.n, w, P.gs, 16, 1);
-    t.q0 = min(max(P.cu[t.r], 0), P.n_q);
-    t.q_len = min(max(P.cu[t.r + 1], t.q0), P.n_q) - t.q0;
-    const int64_t row0 = (w - first_item(P.cu[t.r], t.r, P.gs, 16, 1)) * 16;
-    const int64_t left = (int64_t)t.q_len * P.gs - row0;
-    t.row0 = (int)row0;
-    t.n_row = row0 < 0 || left <= 0 ? 0 : (int)min(left, (int64_t)16);
-  }
-  t.trow = P.rows ? P.rows[t.r] : t.r;
-  t.kv = max(P.kv_lens[t.r], 0);
-  t.len = (int)min((int64_t)t.kv, (int64_t)P.max_blocks << P.log2b);
-  if (t.trow < 0 || t.trow >= P.n_rows) t.len = 0, t.trow = 0;
-  t.limit = t.n_row > 0 ? sees(P, t, (t.row0 + t.n_row - 1) / P.gs) : 0;
-  return t;
-}
-
-// Tiles of 32 positions per split: a multiple of the wavefronts.
-KVT_DEV int tiles_per_split(int limit, int splits) {
-  const int tiles = (limit + kTile - 1) / kTile;
-  return max(((tiles + splits - 1) / splits + kWaves - 1) / kWaves * kWaves, kWaves);
-}
+constexpr int kMostSplits = 1024;
 
 template <int BYTES> struct Raw { uint32_t w[BYTES / 4]; };
 template <int BYTES>
@@ -102,62 +46,8 @@ KVT_DEV Raw<BYTES> load(const uint8_t* base, uint32_t off) {
 }
 
 KVT_DEV f4 mfma(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-KVT_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }   // (v_exp_f32: results below 2^-126 are 0)
-KVT_DEV float bits_f(uint32_t u) { return __uint_as_float(u); }
 KVT_DEV float lane_f(float v, int lane) {
   return bits_f((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
-}
-
-// A row of Q in operand order: chunk c (16 channels of group g at 64 c + 16 g) is two operands.  bf16 rows are scaled by
-// 2^-e to fp16 range; returns 2^e.
-template <int QT, int D>
-KVT_DEV float load_q(const void* q, int64_t at, bool live, int g, h8 (&out)[D / 32]) {
-  constexpr int NC = D / 64;
-  uint4 raw[NC][2];
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      raw[c][i] = live ? *reinterpret_cast<const uint4*>((const uint16_t*)q + at + 64 * c + 16 * g + 8 * i) : make_uint4(0, 0, 0, 0);
-  if constexpr (QT == kF16) {
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) out[2 * c + i] = __builtin_bit_cast(h8, raw[c][i]);
-    return 1.0f;
-  } else {
-    float top = 0.0f;
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t w[4] = {raw[c][i].x, raw[c][i].y, raw[c][i].z, raw[c][i].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(bits_f(w[k] << 16)), fabsf(bits_f(w[k] & 0xFFFF0000u))));
-      }
-    top = max_xor16_32(top);
-    int e = (int)(__float_as_uint(top) >> 23) - 127;
-    e = top > 0.0f && top < __builtin_inff() ? min(max(e, -120), 120) : 0;
-    const float f = bits_f((uint32_t)(127 - e) << 23);
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t w[4] = {raw[c][i].x, raw[c][i].y, raw[c][i].z, raw[c][i].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          out[2 * c + i][2 * k] = (_Float16)(bits_f(w[k] << 16) * f);
-          out[2 * c + i][2 * k + 1] = (_Float16)(bits_f(w[k] & 0xFFFF0000u) * f);
-        }
-      }
-    return bits_f((uint32_t)(127 + e) << 23);
-  }
-}
-
-KVT_DEV void store_out(void* out, int ot, int64_t at, float v) {
-  if (ot == kF32) ((float*)out)[at] = v;
-  else if (ot == kBF16) ((uint16_t*)out)[at] = bf16_rne(v);
-  else ((uint16_t*)out)[at] = f32_to_f16_bits(v);
 }
 
 template <int CODE, int QT, int D>
@@ -171,21 +61,23 @@ __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot
   const int split = blockIdx.x, h = blockIdx.y, w = blockIdx.z;
   const Item it = item_of(P, w);
   if (it.n_row == 0) return;
-  const int tps = tiles_per_split(it.limit, P.splits);
-  const int tile0 = split * tps, tile1 = min(tile0 + tps, (it.limit + kTile - 1) / kTile);
+  const int tps = tiles_per_split(P, it.limit);
+  const int tile0 = split * tps, tile1 = min(tile0 + tps, tiles_of(P, it.limit));
   if (tile0 >= tile1 && P.splits > 1) return;       // (the merge knows which splits there are)
 
   const int my = it.row0 + l, qi = my / P.gs, hq = h * P.gs + my % P.gs;
   const bool live = l < it.n_row;
   h8 Q[D / 32];
-  const float qf = load_q<QT, D>(P.q, (int64_t)(it.q0 + qi) * P.sq_n + (int64_t)hq * P.sq_h, live, g, Q) * P.scale_log2;
+  // (chunk c of 64 channels: 16 of them per group g, two operands)
+  const float qf = load_q<QT>(P.q, (int64_t)(it.q0 + qi) * P.sq_n + (int64_t)hq * P.sq_h, live,
+                              [g](int k) { return 64 * (k >> 1) + 16 * g + 8 * (k & 1); }, max_xor16_32, Q) * P.scale_log2;
   const int see = sees(P, it, qi);
   const int all_see = sees(P, it, it.row0 / P.gs);   // (the fewest of the item's rows: positions below it need no comparison)
 
   f4 acc[VB];
 #pragma unroll
   for (int c = 0; c < VB; ++c) acc[c] = f4{0, 0, 0, 0};
-  float m = -__builtin_inff(), sum = 0.0f, unit = 0.0f;
+  float m = -__builtin_inff(), sum = 0.0f, unit = 0.0f, peak = 0.0f;
 
   const uint32_t koff = (uint32_t)l * D + 16u * g, voff = 4u * g * D + (uint32_t)l * VB;
   const int64_t tbl = (int64_t)it.trow * P.stride;
@@ -275,10 +167,8 @@ __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot
       const bool far = fminf(fv[0], fv[1]) > 0.0f && (fv[0] < 0.25f * fv[1] || fv[1] < 0.25f * fv[0]);
       for (int pass = 0; pass <= (int)far; ++pass) {
         const float big = far ? fv[pass] : fmaxf(fv[0], fv[1]);
-        if (big > unit || big < 0.25f * unit) {                     // uniform
-          const float u1 = fmaxf(big, unit * 0x1p-90f);             // (the ratio stays finite)
-          const float a = u1 > 0.0f ? unit / u1 : 1.0f;
-          unit = u1;
+        if (big > unit || (big > 0.0f && big < 0.25f * unit)) {     // uniform
+          const float a = new_unit(big, unit, peak);
 #pragma unroll
           for (int c = 0; c < VB; ++c) acc[c] *= a;
         }
@@ -333,22 +223,22 @@ __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot
     float M = -__builtin_inff();
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) M = fmaxf(M, lm[v][row]);
-    float L = 0.0f;
-    f4 O = {0, 0, 0, 0};
+    float L = 0.0f, f[kWaves];
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) {
-      const float mv = lm[v][row], f = mv == -__builtin_inff() ? 0.0f : exp2_(mv - M);
-      L += f * ll[v][row];
-      const float fu = f * lu[v];
-      const f4 o = *reinterpret_cast<const f4*>(&lo[v][row][d]);
-      // (a wavefront without positions counts 0, whatever its state holds)
-      O += mv == -__builtin_inff() && ll[v][row] == 0.0f ? f4{0, 0, 0, 0} : o * fu;
+      f[v] = lm[v][row] == -__builtin_inff() ? 0.0f : exp2_(lm[v][row] - M);
+      L += f[v] * ll[v][row];
     }
+    // (divided by the sum before the unit comes in: no product is larger than the values themselves)
+    f4 O = {0, 0, 0, 0};
+    const float per = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) O += *reinterpret_cast<const f4*>(&lo[v][row][d]) * (f[v] * per) * lu[v];
     if (P.splits == 1) {
       const int at = it.row0 + row;
       const int64_t o = (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + d;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) store_out(P.out, ot, o + i, O[i] / L);
+      for (int i = 0; i < 4; ++i) store_out(P.out, ot, o + i, L == 0.0f ? __builtin_nanf("") : O[i]);
     } else {
       const int64_t part = (((int64_t)w * P.H + h) * P.splits + split) * 16 + row;
       *reinterpret_cast<f4*>(P.part_o + part * D + d) = O;
@@ -357,50 +247,64 @@ __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot
   }
 }
 
-// Merge of a row's splits: one workgroup per (16 rows, KV head, row); D / 4 threads per split side by side.
-template <int D>
-__global__ __launch_bounds__(256) void block_merge_kernel(const Attn P, int ot) {
-  constexpr int TP = D / 4, NG = 256 / TP;
-  __shared__ float red[4];
-  __shared__ f4 os[NG][TP];
-  __shared__ float ls[NG];
-  const int row = blockIdx.x, h = blockIdx.y, w = blockIdx.z;
+// Merge of the splits of a row: one workgroup per (row, 64 channels, KV head and item).  A part is a split's own result with
+// its maximum m and sum l; their weights 2^(m - M) l / (the sum of these) go to LDS first, then groups of 16 lanes add up every NG-th split, all their loads in flight side by side.
+template <int NT>
+__global__ __launch_bounds__(NT) void block_merge_kernel(const Attn P, int D, int ot) {
+  constexpr int NG = NT / 16;
+  __shared__ float wgt[kMostSplits], red[NT / 64], red2[NT / 64];
+  __shared__ f4 os[NG][16];
+  const int row = blockIdx.x, dc = blockIdx.y, h = blockIdx.z % P.H, w = blockIdx.z / P.H;
   const Item it = item_of(P, w);
   if (row >= it.n_row) return;
-  const int tps = tiles_per_split(it.limit, P.splits);
-  const int used = ((it.limit + kTile - 1) / kTile + tps - 1) / tps;
-  const int64_t part = ((int64_t)w * P.H + h) * P.splits * 16 + row;
-  float M = -__builtin_inff();
-  for (int s = threadIdx.x; s < used; s += 256) M = fmaxf(M, P.part_ml[2 * (part + 16 * s)]);
+  const int tps = tiles_per_split(P, it.limit);
+  const int used = (tiles_of(P, it.limit) + tps - 1) / tps;
+  const int64_t part = ((int64_t)w * P.H + h) * P.splits * P.item_rows + row;
+  float M = -__builtin_inff(), L = 0.0f;
+  for (int s = threadIdx.x; s < used; s += NT) M = fmaxf(M, P.part_ml[2 * (part + (int64_t)P.item_rows * s)]);
   M = group_max<64>(M);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = M;
   __syncthreads();
-  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const int grp = threadIdx.x / TP, d = threadIdx.x % TP;
-  f4 O = {0, 0, 0, 0};
-  float L = 0.0f;
-  for (int s = grp; s < used; s += NG) {
-    const int64_t at = part + 16 * s;
-    const float ms = P.part_ml[2 * at], f = ms == -__builtin_inff() ? 0.0f : exp2_(ms - M);
-    L += f * P.part_ml[2 * at + 1];
-    O += f * *reinterpret_cast<const f4*>(P.part_o + at * D + 4 * d);
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) M = fmaxf(M, red[i]);
+  for (int s = threadIdx.x; s < used; s += NT) {
+    const float* ml = P.part_ml + 2 * (part + (int64_t)P.item_rows * s);
+    const float f = ml[0] == -__builtin_inff() ? 0.0f : exp2_(ml[0] - M);
+    wgt[s] = f * ml[1];
+    L += wgt[s];
   }
-  os[grp][d] = O;
-  if (d == 0) ls[grp] = L;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
+  if ((threadIdx.x & 63) == 0) red2[threadIdx.x >> 6] = L;
+  __syncthreads();
+  L = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) L += red2[i];
+  const float per = 1.0f / L;
+  const int grp = threadIdx.x >> 4, d = 64 * dc + 4 * (threadIdx.x & 15);
+  f4 O = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int s = grp; s < used; s += NG)
+    O += (wgt[s] * per) * *reinterpret_cast<const f4*>(P.part_o + (part + (int64_t)P.item_rows * s) * D + d);
+  os[grp][threadIdx.x & 15] = O;
   __syncthreads();
   if (grp) return;
-#pragma unroll
-  for (int i = 1; i < NG; ++i) O += os[i][d], L += ls[i];
+  for (int i = 1; i < NG; ++i) O += os[i][threadIdx.x];
   const int at = it.row0 + row;
-  const int64_t o = (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + 4 * d;
+  const int64_t o = (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + d;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) store_out(P.out, ot, o + i, O[i] / L);
+  for (int i = 0; i < 4; ++i) store_out(P.out, ot, o + i, L == 0.0f ? __builtin_nanf("") : O[i]);
+}
+void merge(const Attn& P, int D, int items, int rows, int ot, hipStream_t st) {
+  const dim3 grid(rows, D / 64, P.H * items);
+  if (P.splits > 64) block_merge_kernel<1024><<<grid, 1024, 0, st>>>(P, D, ot);
+  else block_merge_kernel<256><<<grid, 256, 0, st>>>(P, D, ot);
 }
 
 template <int CODE, int QT, int D>
 void launch(const Attn& P, int items, int rows, int ot, hipStream_t st) {
   block_rows_kernel<CODE, QT, D><<<dim3(P.splits, P.H, items), 256, 0, st>>>(P, ot);
-  if (P.splits > 1) block_merge_kernel<D><<<dim3(rows, P.H, items), 256, 0, st>>>(P, ot);
+  if (P.splits > 1) merge(P, D, items, rows, ot, st);
 }
 template <int CODE, int QT>
 void launch_d(const Attn& P, int D, int items, int rows, int ot, hipStream_t st) {
@@ -420,13 +324,14 @@ void launch_all(const Attn& P, int code, int qt, int D, int items, int rows, int
 
 int check(const Attn& P, int Hq, int D, int block, int code, int qt, int ot) {
   if (P.n < 1 || P.n > kMaxReq || P.H < 1 || Hq < P.H || Hq % P.H || Hq / P.H > 16 || P.n_rows < 1 || P.n_blocks < 1 ||
-      P.max_blocks < 1 || P.stride < P.max_blocks || (!P.rows && P.n_rows < P.n) || P.splits < 1)
+      P.max_blocks < 1 || P.stride < P.max_blocks || (!P.rows && P.n_rows < P.n) || P.splits < 1 ||
+      !(P.scale_log2 > 0.0f))
     return KVT_EINVAL;
   if ((D != 64 && D != 128 && D != 256) || (block != 16 && block != 32 && block != 64)) return KVT_EINVAL;
   if ((code != kE4M3 && code != kI8) || (qt != kBF16 && qt != kF16) || (ot != kBF16 && ot != kF16 && ot != kF32))
     return KVT_EINVAL;
   if ((uintptr_t)P.q & 15 || P.sq_n % 8 || P.sq_h % 8 || ((uintptr_t)P.k8 | (uintptr_t)P.v8) & 15) return KVT_EINVAL;
-  if (P.H > 65535 || (int64_t)P.max_blocks * block > 0x7FFFFFFF) return KVT_ERANGE;
+  if (P.H > 65535 || P.splits > kMostSplits || (int64_t)P.max_blocks * block > 0x7FFFFFFF) return KVT_ERANGE;
   return KVT_OK;
 }
 
@@ -444,9 +349,11 @@ extern "C" int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q
   P.sq_n = sq_n, P.sq_h = sq_h, P.so_n = so_n, P.so_h = so_h, P.stride = bt_stride, P.scale_log2 = scale * kLog2e;
   P.n = n, P.n_rows = n_rows, P.n_q = n, P.H = H, P.gs = H > 0 ? Hq / H : 0, P.n_blocks = n_blocks;
   P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.splits = n_splits, P.causal = 0;
+  P.item_rows = 16, P.tile = kTile, P.least = kWaves;
   const int st = check(P, Hq, D, block, code, q_type, out_type);
   if (st != KVT_OK) return st;
   if (n_splits > 1 && (!part_o || !part_ml)) return KVT_EINVAL;
+  if (n_splits > 1 && (int64_t)n * H > 65535) return KVT_ERANGE;
   launch_all(P, code, q_type, D, n, P.gs, out_type, (hipStream_t)stream);
   KVT_CHECK_LAUNCH();
   return KVT_OK;
@@ -456,8 +363,8 @@ extern "C" int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int 
                                  const void* kv_lens, int n, int H, int Hq, int D, int code, const void* k8,
                                  const void* v8, const void* ks, const void* vs, int n_blocks, int block,
                                  const void* block_table, int64_t bt_stride, int n_rows, int max_blocks,
-                                 const void* rows, int causal, float scale, int n_splits, void* part_o, void* part_ml,
-                                 void* out, int out_type, int64_t so_n, int64_t so_h, void* stream) {
+                                 const void* rows, int causal, float scale, int item_rows, int n_splits, void* part_o,
+                                 void* part_ml, void* out, int out_type, int64_t so_n, int64_t so_h, void* stream) {
   Attn P;
   P.q = q, P.k8 = (const uint8_t*)k8, P.v8 = (const uint8_t*)v8, P.ks = (const float*)ks, P.vs = (const float*)vs;
   P.table = (const int32_t*)block_table, P.kv_lens = (const int32_t*)kv_lens, P.rows = (const int32_t*)rows;
@@ -465,13 +372,20 @@ extern "C" int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int 
   P.sq_n = sq_n, P.sq_h = sq_h, P.so_n = so_n, P.so_h = so_h, P.stride = bt_stride, P.scale_log2 = scale * kLog2e;
   P.n = n, P.n_rows = n_rows, P.n_q = n_q, P.H = H, P.gs = H > 0 ? Hq / H : 0, P.n_blocks = n_blocks;
   P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.splits = n_splits, P.causal = causal;
+  const bool tiled = item_rows == kTileRows;
+  P.item_rows = item_rows, P.tile = tiled ? tile_positions(D) : kTile, P.least = tiled ? 1 : kWaves;
   const int st = check(P, Hq, D, block, code, q_type, out_type);
   if (st != KVT_OK) return st;
-  if (!cu_q || n_q < 0 || (n_splits > 1 && (!part_o || !part_ml))) return KVT_EINVAL;
+  if (!cu_q || n_q < 0 || (item_rows != 16 && !tiled) || (n_splits > 1 && (!part_o || !part_ml))) return KVT_EINVAL;
   if (n_q == 0) return KVT_OK;
-  const int64_t items = (int64_t)n_q * P.gs / 16 + n;
-  if (items > 65535) return KVT_ERANGE;
-  launch_all(P, code, q_type, D, (int)items, 16, out_type, (hipStream_t)stream);
+  const int64_t items = (int64_t)n_q * P.gs / item_rows + n;
+  if (items > (tiled ? 0x7FFFFFFF / P.H : 65535) || (n_splits > 1 && items * P.H > 65535)) return KVT_ERANGE;
+  if (tiled) {
+    tile_launch(P, code, q_type, D, (int)items, out_type, (hipStream_t)stream);
+    if (n_splits > 1) merge(P, D, (int)items, kTileRows, out_type, (hipStream_t)stream);
+  } else {
+    launch_all(P, code, q_type, D, (int)items, 16, out_type, (hipStream_t)stream);
+  }
   KVT_CHECK_LAUNCH();
   return KVT_OK;
 }

@@ -1,0 +1,299 @@
+// Attention of query chunks over the 8-bit block cache on the matrix cores: the kernel of calls with many rows
+// (kvt_block_prefill; block_rows.hip has the mathematics and the calls with few rows).
+//
+// A row is a (query, q head) pair of one KV head, in that order; one workgroup of 4 wavefronts has 128 of them (32 per
+// wavefront) and walks the positions that they see in tiles of T.  The 256 threads convert a tile's codes to fp16 once,
+// into LDS, and the four wavefronts multiply from there:
+//   S^T = K Q^T on v_mfma_f32_32x32x16_f16 (A = 32 positions from LDS, B = the wavefront's 32 rows in registers).  A lane
+//     gets 16 scores of one row, the other 16 of the tile's 32 sit in lane ^ 32: the row maximum takes one cross-lane step.
+//   O^T += V^T P^T: the weights stay where they are (register 8 s + j of lane (l, g) is position 16 s + 8 (j / 4) + 4 g + j % 4,
+//     its operand's k), and V^T is stored so that these eight positions of a channel are 16 consecutive bytes.  Each product
+//     covers 16 positions, i.e. one block of the cache, so a block's V scale is one factor for the whole operand.
+// Two LDS buffers: a tile's codes are loaded into registers before the products of the tile before, converted and stored
+// behind them; one barrier per tile.  Positions' block ids are loaded a tile ahead of the codes.
+// LDS rows are padded by 16 bytes: the operand reads (16 bytes per lane, 32 consecutive rows) meet no bank conflicts.
+// T = 32 positions at D = 256, 64 below: 32 KB of fp16 per buffer, so that two workgroups fit a CU, whose wavefronts run
+// their softmax under each other's products.
+#include "block_attn.h"
+
+using namespace kvt;
+using namespace kvt::blk;
+
+namespace {
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+KVT_DEV f16v mfma(h8 a, h8 b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+KVT_DEV float max_xor32(float v) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(bits_f(b[0]), bits_f(b[1]));
+}
+KVT_DEV float sum_xor32(float v) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return bits_f(b[0]) + bits_f(b[1]);
+}
+
+// fp32 pair -> fp16, to nearest even (one v_cvt_pk_f16_f32)
+KVT_DEV h2 h2_rne(float a, float b) { return __builtin_convertvector((f2){a, b}, h2); }
+
+constexpr float kLeast = 0x1p-120f;   // (a factor of 0 would make a masked score, -inf, a NaN)
+
+template <int D>
+struct Tile {
+  static constexpr int T = D == 256 ? 32 : 64;
+  static constexpr int KP = 2 * D + 16;         // bytes per K row (a position)
+  static constexpr int VP = 2 * T + 16;         // bytes per V^T row (a channel)
+  static constexpr int TPK = 256 / T;           // threads per K row
+  static constexpr int NK = D / 16 / TPK;       // 16-byte pieces of a K row per thread
+  static constexpr int VT = T * D / 32;         // threads that convert V (8 positions x 4 channels each)
+};
+
+template <int D>
+struct __align__(16) Buf {
+  uint8_t k[Tile<D>::T * Tile<D>::KP];
+  uint8_t v[D * Tile<D>::VP];
+  float ks[Tile<D>::T / 16], vs[Tile<D>::T / 16];
+  int there[Tile<D>::T / 16];                   // 0: no such block
+};
+
+// A thread's share of a tile as loaded: pieces of one K row, and 4 channels of 8 positions of V.
+template <int D>
+struct Raw {
+  u4v k[Tile<D>::NK];
+  uint32_t v[8];
+  float ks, vs;
+};
+
+template <int CODE, int QT, int D>
+__global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int items, int ot) {
+  using C = Tile<D>;
+  constexpr int T = C::T, SUB = T / 32, DT = D / 32;
+  __shared__ Buf<D> buf[2];
+  const int tid = threadIdx.x, lane = tid & 63, l = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // head fastest: with H = 2, 4 or 8 the workgroups of a head share the caches of the same XCDs; the last rows, which see
+  // the most positions, first
+  const int h = blockIdx.x % P.H, w = items - 1 - (int)(blockIdx.x / P.H), split = blockIdx.y;
+  const Item it = item_of(P, w);
+  if (it.n_row == 0) return;
+  const int tps = tiles_per_split(P, it.limit);
+  const int tile0 = split * tps, tile1 = min(tile0 + tps, tiles_of(P, it.limit));
+  if (tile0 >= tile1 && P.splits > 1) return;
+
+  const int my = it.row0 + 32 * wave + l, qi = my / P.gs, hq = h * P.gs + my % P.gs;
+  const bool live = 32 * wave + l < it.n_row;
+  h8 Q[D / 16];
+  const float qf = load_q<QT>(P.q, (int64_t)(it.q0 + qi) * P.sq_n + (int64_t)hq * P.sq_h, live,
+                              [g](int k) { return 16 * k + 8 * g; }, max_xor32, Q) * P.scale_log2;
+  const int see = live ? sees(P, it, qi) : 0;
+  const int first_row = it.row0 + 32 * wave, last_row = it.row0 + min(32 * wave + 31, it.n_row - 1);
+  const bool any_row = 32 * wave < it.n_row;
+  const int all_see = any_row ? sees(P, it, first_row / P.gs) : 0;   // positions that every row of the wavefront sees
+  const int most_see = any_row ? sees(P, it, last_row / P.gs) : 0;   // and that any of them sees
+
+  // this thread's share of a tile
+  const int krow = tid / C::TPK, kpc = tid % C::TPK;
+  const int vc = (tid & 3) + 4 * (tid >> (D == 256 ? 8 : D == 128 ? 7 : 6)), vd = 4 * ((tid >> 2) & (D / 4 - 1));
+  const int vrow = 16 * (vc >> 1) + 4 * (vc & 1);                    // positions vrow + {0 .. 3, 8 .. 11}
+  const bool has_v = C::VT == 256 || tid < C::VT;
+  const int32_t* table = P.table + it.trow * P.stride;
+
+  const auto id_at = [&](int p) {
+    const int id = p < it.limit ? table[p >> P.log2b] : -1;
+    return id >= 0 && id < P.n_blocks ? id : -1;
+  };
+  const auto row_at = [&](int id, int p) {
+    return ((((int64_t)max(id, 0) * P.H + h) << P.log2b) + (p & ((1 << P.log2b) - 1))) * D;
+  };
+  const auto fetch = [&](int tile, int idk, int idv, Raw<D>& r) {
+    const int pk = tile * T + krow, pv = tile * T + vrow;
+    const uint8_t* kp = P.k8 + row_at(idk, pk) + 16 * kpc;
+#pragma unroll
+    for (int i = 0; i < C::NK; ++i) r.k[i] = *reinterpret_cast<const u4v*>(kp + 16 * C::TPK * i);
+    if (has_v) {
+      const uint8_t* vp = P.v8 + row_at(idv, pv) + vd;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r.v[i] = *reinterpret_cast<const uint32_t*>(vp + (i + (i & 4)) * D);
+    }
+    if ((krow & 15) == 0 && kpc == 0) {
+      const int64_t at = (int64_t)max(idk, 0) * P.H + h;
+      r.ks = P.ks[at], r.vs = P.vs[at];
+    }
+  };
+  const auto convert = [&](int tile, int idk, int idv, Raw<D>& r, Buf<D>& b) {
+    uint8_t* kr = b.k + krow * C::KP;
+#pragma unroll
+    for (int i = 0; i < C::NK; ++i) {
+      h8* to = reinterpret_cast<h8*>(kr + 32 * (kpc + C::TPK * i));
+      to[0] = operand<CODE>(r.k[i].x, r.k[i].y);
+      to[1] = operand<CODE>(r.k[i].z, r.k[i].w);
+    }
+    if ((krow & 15) == 0 && kpc == 0) {
+      b.ks[krow >> 4] = idk < 0 ? 0.0f : r.ks;
+      b.vs[krow >> 4] = idk < 0 ? 0.0f : r.vs;
+      b.there[krow >> 4] = idk >= 0;
+    }
+    if (!has_v) return;
+    const int left = it.limit - (tile * T + vrow);                   // positions behind the last one, or in no block: 0
+    if (idv < 0 || left < 12) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r.v[i] = idv >= 0 && i + (i & 4) < left ? r.v[i] : 0u;
+    }
+    uint32_t lo[4], hi[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t a = flip<CODE>(r.v[2 * j]), c = flip<CODE>(r.v[2 * j + 1]);
+      lo[j] = __builtin_amdgcn_perm(c, a, 0x05010400u);
+      hi[j] = __builtin_amdgcn_perm(c, a, 0x07030602u);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      h2 y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t u = c < 2 ? lo[j] : hi[j];
+        y[j] = c & 1 ? pair<CODE, true>(u) : pair<CODE, false>(u);
+      }
+      *reinterpret_cast<h8*>(b.v + (vd + c) * C::VP + 16 * vc) = h8{y[0].x, y[0].y, y[1].x, y[1].y, y[2].x, y[2].y, y[3].x, y[3].y};
+    }
+  };
+
+  f16v acc[DT];
+#pragma unroll
+  for (int c = 0; c < DT; ++c) acc[c] = f16v{};
+  float m = -__builtin_inff(), sum = 0.0f, unit = 0.0f, per_unit = 0.0f, peak = 0.0f;
+
+  if (tile0 < tile1) {
+    Raw<D> raw;
+    int idk = id_at(tile0 * T + krow), idv = id_at(tile0 * T + vrow);
+    fetch(tile0, idk, idv, raw);
+    convert(tile0, idk, idv, raw, buf[0]);
+    idk = id_at((tile0 + 1) * T + krow), idv = id_at((tile0 + 1) * T + vrow);
+    __syncthreads();
+    for (int tile = tile0; tile < tile1; ++tile) {
+      const Buf<D>& b = buf[(tile - tile0) & 1];
+      const bool more = tile + 1 < tile1;
+      int nk = -1, nv = -1;
+      if (more) {
+        fetch(tile + 1, idk, idv, raw);
+        nk = id_at((tile + 2) * T + krow), nv = id_at((tile + 2) * T + vrow);
+      }
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        const int p0 = tile * T + 32 * u;
+        if (p0 >= most_see) continue;
+        f16v sc = {};
+        const uint8_t* kb = b.k + (32 * u + l) * C::KP + 16 * g;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) sc = mfma(*reinterpret_cast<const h8*>(kb + 32 * k), Q[k], sc);
+        if (p0 + 32 > all_see || !(b.there[2 * u] & b.there[2 * u + 1])) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int at = p0 + 8 * (i >> 2) + 4 * g + (i & 3);
+            sc[i] = at < see && b.there[2 * u + (i >> 3)] ? sc[i] : -__builtin_inff();
+          }
+        }
+        // (the factors are positive, so the largest score of a half is its largest product times the factor)
+        const float f[2] = {fmaxf(qf * b.ks[2 * u], kLeast), fmaxf(qf * b.ks[2 * u + 1], kLeast)};
+        float top2[2] = {sc[0], sc[8]};
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top2[0] = fmaxf(top2[0], sc[j]), top2[1] = fmaxf(top2[1], sc[8 + j]);
+        const float top = max_xor32(fmaxf(top2[0] * f[0], top2[1] * f[1]));
+        const bool rise = top > m + kLag;
+        if (__any(rise)) {
+          const float m1 = rise ? top : m;
+          const float a = m1 == m ? 1.0f : exp2_(m - m1);
+          sum *= a;
+          m = m1;
+#pragma unroll
+          for (int c = 0; c < DT; ++c) acc[c] *= a;
+        }
+        const float ms = (m == -__builtin_inff() ? 0.0f : m) - kLift;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          x[i] = exp2_(fmaf(sc[i], f[i >> 3], -ms));
+          sum += x[i];
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const float fv = bits_f((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(b.vs[2 * u + s])));
+          if (fv > unit || (fv > 0.0f && fv < 0.25f * unit)) {       // uniform
+            const float a = new_unit(fv, unit, peak);
+            per_unit = 1.0f / unit;
+#pragma unroll
+            for (int c = 0; c < DT; ++c) acc[c] *= a;
+          }
+          const float ru = fv * per_unit;
+          h8 p;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const h2 y = h2_rne(x[8 * s + 2 * j] * ru, x[8 * s + 2 * j + 1] * ru);
+            p[2 * j] = y.x, p[2 * j + 1] = y.y;
+          }
+          const uint8_t* vb = b.v + l * C::VP + 16 * (4 * u + 2 * s + g);
+#pragma unroll
+          for (int c = 0; c < DT; ++c) acc[c] = mfma(*reinterpret_cast<const h8*>(vb + 32 * c * C::VP), p, acc[c]);
+        }
+      }
+      if (more) convert(tile + 1, idk, idv, raw, buf[(tile + 1 - tile0) & 1]);
+      idk = nk, idv = nv;
+      __syncthreads();
+    }
+  }
+
+  // register i of acc[c]: channel 32 c + 8 (i / 4) + 4 g + i % 4 of row l
+  sum = sum_xor32(sum);
+  if (!live) return;
+  const float f = sum == 0.0f ? 0.0f : unit / sum;
+  if (P.splits == 1) {
+    const int64_t o = (int64_t)(it.q0 + qi) * P.so_n + (int64_t)hq * P.so_h + 4 * g;
+#pragma unroll
+    for (int c = 0; c < DT; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        store_out(P.out, ot, o + 32 * c + 8 * (i >> 2) + (i & 3), sum == 0.0f ? __builtin_nanf("") : acc[c][i] * f);
+  } else {
+    const int64_t part = (((int64_t)w * P.H + h) * P.splits + split) * kTileRows + 32 * wave + l;
+#pragma unroll
+    for (int c = 0; c < DT; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f4 o = {acc[c][4 * i], acc[c][4 * i + 1], acc[c][4 * i + 2], acc[c][4 * i + 3]};
+        *reinterpret_cast<f4*>(P.part_o + part * D + 32 * c + 8 * i + 4 * g) = o * f;
+      }
+    if (g == 0) P.part_ml[2 * part] = m, P.part_ml[2 * part + 1] = sum;
+  }
+}
+
+template <int CODE, int QT, int D>
+void launch(const Attn& P, int items, int ot, hipStream_t st) {
+  block_tile_kernel<CODE, QT, D><<<dim3(P.H * items, P.splits), 256, 0, st>>>(P, items, ot);
+}
+template <int CODE, int QT>
+void launch_d(const Attn& P, int D, int items, int ot, hipStream_t st) {
+  if (D == 64) launch<CODE, QT, 64>(P, items, ot, st);
+  else if (D == 128) launch<CODE, QT, 128>(P, items, ot, st);
+  else launch<CODE, QT, 256>(P, items, ot, st);
+}
+
+}  // namespace
+
+namespace kvt {
+namespace blk {
+
+int tile_positions(int D) { return D == 256 ? Tile<256>::T : 64; }
+
+void tile_launch(const Attn& P, int code, int qt, int D, int items, int ot, hipStream_t st) {
+  if (code == kE4M3) {
+    if (qt == kBF16) launch_d<kE4M3, kBF16>(P, D, items, ot, st);
+    else launch_d<kE4M3, kF16>(P, D, items, ot, st);
+  } else {
+    if (qt == kBF16) launch_d<kI8, kBF16>(P, D, items, ot, st);
+    else launch_d<kI8, kF16>(P, D, items, ot, st);
+  }
+}
+
+}  // namespace blk
+}  // namespace kvt

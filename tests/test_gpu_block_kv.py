@@ -346,15 +346,30 @@ def test_attention_ignores_what_a_request_does_not_hold(kvt_pkg, decode, kv):
 
 @pytest.mark.parametrize("decode", [True, False])
 def test_attention_scales_far_apart(kvt_pkg, decode):
-    """V scales that differ by 2^60 from block to block (and blocks of zeros), K scales by 2^6."""
+    """V scales that differ by 2^60 from block to block (and blocks of zeros, and blocks that are not there between them),
+    K scales by 2^6."""
     def change(codes, sc, table):
         n, H = sc[1].shape
+        for row in table:
+            row[3] = row[4] = row[9] = row[11] = -1
         e = torch.tensor([[-30, 30, 0, -64, 12][(i + h) % 5] for i in range(n) for h in range(H)]).view(n, H)
         sc[1].copy_(2.0 ** e.float())
         sc[0].mul_(2.0 ** ((torch.arange(n) % 4).float()[:, None] - 3))
         codes[1].view(torch.int8)[::7] = 0
     new = [1, 1] if decode else [70, 300]
     _check_attn("fp8", torch.bfloat16, 8, 2, 128, 16, new, [700, 333], decode=decode, change=change, seed=4,
+                out_dtype=torch.float32)
+
+
+@pytest.mark.parametrize("decode", [True, False])
+def test_attention_scales_at_the_ends(kvt_pkg, decode):
+    """V scales from 2^-64 to 2^110 in one row: finite, and as exact as the largest ones ask."""
+    def change(codes, sc, table):
+        n, H = sc[1].shape
+        e = torch.tensor([[-64, 110, -64, 0, 30][(i + h) % 5] for i in range(n) for h in range(H)]).view(n, H)
+        sc[1].copy_(2.0 ** e.float())
+    new = [1, 1] if decode else [70, 300]
+    _check_attn("int8", torch.float16, 8, 2, 64, 16, new, [900, 333], decode=decode, change=change, seed=6,
                 out_dtype=torch.float32)
 
 

@@ -69,6 +69,9 @@ KVT_DEV int tiles_per_split(const Attn& P, int limit) {
   return max((per + P.least - 1) / P.least, 1) * P.least;
 }
 
+// fp32 pair -> fp16, to nearest even (one v_cvt_pk_f16_f32)
+KVT_DEV h2 h2_rne(float a, float b) { return __builtin_convertvector((f2){a, b}, h2); }
+
 KVT_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }   // (v_exp_f32: results below 2^-126 are 0)
 KVT_DEV float bits_f(uint32_t u) { return __uint_as_float(u); }
 
@@ -81,10 +84,16 @@ KVT_DEV float new_unit(float fv, float& unit, float& peak) {
   return a;
 }
 
-KVT_DEV void store_out(void* out, int ot, int64_t at, float v) {
-  if (ot == kF32) ((float*)out)[at] = v;
-  else if (ot == kBF16) ((uint16_t*)out)[at] = bf16_rne(v);
-  else ((uint16_t*)out)[at] = f32_to_f16_bits(v);
+// Four consecutive channels of an output row (rows are 16-byte aligned: the entry points see to it).
+KVT_DEV void store_out4(void* out, int ot, int64_t at, float a, float b, float c, float d) {
+  if (ot == kF32) {
+    *reinterpret_cast<float4*>((float*)out + at) = make_float4(a, b, c, d);
+  } else if (ot == kBF16) {
+    *reinterpret_cast<uint2*>((uint16_t*)out + at) = make_uint2(bf16x2(a, b), bf16x2(c, d));
+  } else {
+    const h2 x = h2_rne(a, b), y = h2_rne(c, d);
+    *reinterpret_cast<uint2*>((uint16_t*)out + at) = make_uint2(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y));
+  }
 }
 
 // Eight elements of a query row each at at(k), k < N -> operands.  bf16 rows are scaled by a power of two to fit fp16;

@@ -237,8 +237,8 @@ __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot
     if (P.splits == 1) {
       const int at = it.row0 + row;
       const int64_t o = (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + d;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) store_out(P.out, ot, o + i, L == 0.0f ? __builtin_nanf("") : O[i]);
+      if (L == 0.0f) O = f4{1, 1, 1, 1} * __builtin_nanf("");
+      store_out4(P.out, ot, o, O[0], O[1], O[2], O[3]);
     } else {
       const int64_t part = (((int64_t)w * P.H + h) * P.splits + split) * 16 + row;
       *reinterpret_cast<f4*>(P.part_o + part * D + d) = O;
@@ -292,8 +292,8 @@ __global__ __launch_bounds__(NT) void block_merge_kernel(const Attn P, int D, in
   for (int i = 1; i < NG; ++i) O += os[i][threadIdx.x];
   const int at = it.row0 + row;
   const int64_t o = (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + d;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) store_out(P.out, ot, o + i, L == 0.0f ? __builtin_nanf("") : O[i]);
+  if (L == 0.0f) O = f4{1, 1, 1, 1} * __builtin_nanf("");
+  store_out4(P.out, ot, o, O[0], O[1], O[2], O[3]);
 }
 void merge(const Attn& P, int D, int items, int rows, int ot, hipStream_t st) {
   const dim3 grid(rows, D / 64, P.H * items);
@@ -331,6 +331,8 @@ int check(const Attn& P, int Hq, int D, int block, int code, int qt, int ot) {
   if ((code != kE4M3 && code != kI8) || (qt != kBF16 && qt != kF16) || (ot != kBF16 && ot != kF16 && ot != kF32))
     return KVT_EINVAL;
   if ((uintptr_t)P.q & 15 || P.sq_n % 8 || P.sq_h % 8 || ((uintptr_t)P.k8 | (uintptr_t)P.v8) & 15) return KVT_EINVAL;
+  const int out8 = ot == kF32 ? 4 : 8;   // 16-byte aligned output rows
+  if ((uintptr_t)P.out & 15 || P.so_n % out8 || P.so_h % out8) return KVT_EINVAL;
   if (P.H > 65535 || P.splits > kMostSplits || (int64_t)P.max_blocks * block > 0x7FFFFFFF) return KVT_ERANGE;
   return KVT_OK;
 }

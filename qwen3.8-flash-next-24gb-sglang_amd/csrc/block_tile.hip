@@ -34,9 +34,8 @@ KVT_DEV float sum_xor32(float v) {
   return bits_f(b[0]) + bits_f(b[1]);
 }
 
-// fp32 pair -> fp16, to nearest even (one v_cvt_pk_f16_f32)
-KVT_DEV h2 h2_rne(float a, float b) { return __builtin_convertvector((f2){a, b}, h2); }
-
+constexpr int kDsRead = 0x100, kMfma = 0x8;   // instruction classes of the scheduling hints
+constexpr int kAhead = 4;             // operands read ahead of their product
 constexpr float kLeast = 0x1p-120f;   // (a factor of 0 would make a masked score, -inf, a NaN)
 
 template <int D>
@@ -99,27 +98,22 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
   const bool has_v = C::VT == 256 || tid < C::VT;
   const int32_t* table = P.table + it.trow * P.stride;
 
-  const auto id_at = [&](int p) {
-    const int id = p < it.limit ? table[p >> P.log2b] : -1;
-    return id >= 0 && id < P.n_blocks ? id : -1;
-  };
+  // (no branch around a load: the wait for it would move to where the paths join)
+  const auto id_at = [&](int p) { return table[min(p, it.limit - 1) >> P.log2b]; };
+  const auto in_pool = [&](int id) { return (uint32_t)id < (uint32_t)P.n_blocks; };
   const auto row_at = [&](int id, int p) {
-    return ((((int64_t)max(id, 0) * P.H + h) << P.log2b) + (p & ((1 << P.log2b) - 1))) * D;
+    return ((((int64_t)(in_pool(id) ? id : 0) * P.H + h) << P.log2b) + (p & ((1 << P.log2b) - 1))) * D;
   };
   const auto fetch = [&](int tile, int idk, int idv, Raw<D>& r) {
     const int pk = tile * T + krow, pv = tile * T + vrow;
     const uint8_t* kp = P.k8 + row_at(idk, pk) + 16 * kpc;
 #pragma unroll
     for (int i = 0; i < C::NK; ++i) r.k[i] = *reinterpret_cast<const u4v*>(kp + 16 * C::TPK * i);
-    if (has_v) {
-      const uint8_t* vp = P.v8 + row_at(idv, pv) + vd;
+    const uint8_t* vp = P.v8 + row_at(idv, pv) + vd;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r.v[i] = *reinterpret_cast<const uint32_t*>(vp + (i + (i & 4)) * D);
-    }
-    if ((krow & 15) == 0 && kpc == 0) {
-      const int64_t at = (int64_t)max(idk, 0) * P.H + h;
-      r.ks = P.ks[at], r.vs = P.vs[at];
-    }
+    for (int i = 0; i < 8; ++i) r.v[i] = *reinterpret_cast<const uint32_t*>(vp + (i + (i & 4)) * D);
+    const int64_t at = (int64_t)(in_pool(idk) ? idk : 0) * P.H + h;
+    r.ks = P.ks[at], r.vs = P.vs[at];
   };
   const auto convert = [&](int tile, int idk, int idv, Raw<D>& r, Buf<D>& b) {
     uint8_t* kr = b.k + krow * C::KP;
@@ -130,15 +124,15 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
       to[1] = operand<CODE>(r.k[i].z, r.k[i].w);
     }
     if ((krow & 15) == 0 && kpc == 0) {
-      b.ks[krow >> 4] = idk < 0 ? 0.0f : r.ks;
-      b.vs[krow >> 4] = idk < 0 ? 0.0f : r.vs;
-      b.there[krow >> 4] = idk >= 0;
+      b.ks[krow >> 4] = r.ks;
+      b.vs[krow >> 4] = in_pool(idk) ? r.vs : 0.0f;
+      b.there[krow >> 4] = in_pool(idk);
     }
     if (!has_v) return;
     const int left = it.limit - (tile * T + vrow);                   // positions behind the last one, or in no block: 0
-    if (idv < 0 || left < 12) {
+    if (!in_pool(idv) || left < 12) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r.v[i] = idv >= 0 && i + (i & 4) < left ? r.v[i] : 0u;
+      for (int i = 0; i < 8; ++i) r.v[i] = in_pool(idv) && i + (i & 4) < left ? r.v[i] : 0u;
     }
     uint32_t lo[4], hi[4];
 #pragma unroll
@@ -174,25 +168,34 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
     for (int tile = tile0; tile < tile1; ++tile) {
       const Buf<D>& b = buf[(tile - tile0) & 1];
       const bool more = tile + 1 < tile1;
-      int nk = -1, nv = -1;
-      if (more) {
-        fetch(tile + 1, idk, idv, raw);
-        nk = id_at((tile + 2) * T + krow), nv = id_at((tile + 2) * T + vrow);
-      }
+      // (behind the last tile: the same addresses as its own last position's block, unused)
+      fetch(tile + 1, idk, idv, raw);
+      const int nk = id_at((tile + 2) * T + krow), nv = id_at((tile + 2) * T + vrow);
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
         const int p0 = tile * T + 32 * u;
         if (p0 >= most_see) continue;
         f16v sc = {};
         const uint8_t* kb = b.k + (32 * u + l) * C::KP + 16 * g;
+        h8 a[kAhead];
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) sc = mfma(*reinterpret_cast<const h8*>(kb + 32 * k), Q[k], sc);
-        if (p0 + 32 > all_see || !(b.there[2 * u] & b.there[2 * u + 1])) {
+        for (int k = 0; k < kAhead; ++k) a[k] = *reinterpret_cast<const h8*>(kb + 32 * k);
+        __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int at = p0 + 8 * (i >> 2) + 4 * g + (i & 3);
-            sc[i] = at < see && b.there[2 * u + (i >> 3)] ? sc[i] : -__builtin_inff();
+        for (int k = 0; k < D / 16; ++k) {
+          sc = mfma(a[k % kAhead], Q[k], sc);
+          __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+          if (k + kAhead < D / 16) {
+            a[k % kAhead] = *reinterpret_cast<const h8*>(kb + 32 * (k + kAhead));
+            __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
           }
+        }
+        const int there[2] = {b.there[2 * u], b.there[2 * u + 1]};
+        if (p0 + 32 > all_see || !(there[0] & there[1])) {
+          const int seen[2] = {there[0] ? see : 0, there[1] ? see : 0};
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            sc[i] = p0 + 8 * (i >> 2) + 4 * g + (i & 3) < seen[i >> 3] ? sc[i] : -__builtin_inff();
         }
         // (the factors are positive, so the largest score of a half is its largest product times the factor)
         const float f[2] = {fmaxf(qf * b.ks[2 * u], kLeast), fmaxf(qf * b.ks[2 * u + 1], kLeast)};
@@ -233,8 +236,20 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
             p[2 * j] = y.x, p[2 * j + 1] = y.y;
           }
           const uint8_t* vb = b.v + l * C::VP + 16 * (4 * u + 2 * s + g);
+          constexpr int AV = DT < kAhead ? DT : kAhead;
+          h8 a[AV];
 #pragma unroll
-          for (int c = 0; c < DT; ++c) acc[c] = mfma(*reinterpret_cast<const h8*>(vb + 32 * c * C::VP), p, acc[c]);
+          for (int c = 0; c < AV; ++c) a[c] = *reinterpret_cast<const h8*>(vb + 32 * c * C::VP);
+          __builtin_amdgcn_sched_group_barrier(kDsRead, AV, 0);
+#pragma unroll
+          for (int c = 0; c < DT; ++c) {
+            acc[c] = mfma(a[c % AV], p, acc[c]);
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+            if (c + AV < DT) {
+              a[c % AV] = *reinterpret_cast<const h8*>(vb + 32 * (c + AV) * C::VP);
+              __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+            }
+          }
         }
       }
       if (more) convert(tile + 1, idk, idv, raw, buf[(tile + 1 - tile0) & 1]);
@@ -249,11 +264,13 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
   const float f = sum == 0.0f ? 0.0f : unit / sum;
   if (P.splits == 1) {
     const int64_t o = (int64_t)(it.q0 + qi) * P.so_n + (int64_t)hq * P.so_h + 4 * g;
+    const float nan = sum == 0.0f ? __builtin_nanf("") : 0.0f;
 #pragma unroll
     for (int c = 0; c < DT; ++c)
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        store_out(P.out, ot, o + 32 * c + 8 * (i >> 2) + (i & 3), sum == 0.0f ? __builtin_nanf("") : acc[c][i] * f);
+      for (int i = 0; i < 4; ++i)
+        store_out4(P.out, ot, o + 32 * c + 8 * i, acc[c][4 * i] * f + nan, acc[c][4 * i + 1] * f + nan,
+                   acc[c][4 * i + 2] * f + nan, acc[c][4 * i + 3] * f + nan);
   } else {
     const int64_t part = (((int64_t)w * P.H + h) * P.splits + split) * kTileRows + 32 * wave + l;
 #pragma unroll

@@ -47,15 +47,16 @@ KVT_DEV Item item_of(const Attn& P, int w) {
     t.r = w, t.q0 = w, t.q_len = 1, t.row0 = 0, t.n_row = P.gs;
   } else {
     t.r = find_request(P.cu, P.n, w, P.gs, P.item_rows, 1);
-    t.q0 = min(max(P.cu[t.r], 0), P.n_q);
-    t.q_len = min(max(P.cu[t.r + 1], t.q0), P.n_q) - t.q0;
-    const int64_t row0 = (w - first_item(P.cu[t.r], t.r, P.gs, P.item_rows, 1)) * P.item_rows;
+    const int cu0 = uniform(P.cu[t.r]);
+    t.q0 = min(max(cu0, 0), P.n_q);
+    t.q_len = min(max(uniform(P.cu[t.r + 1]), t.q0), P.n_q) - t.q0;
+    const int64_t row0 = (w - first_item(cu0, t.r, P.gs, P.item_rows, 1)) * P.item_rows;
     const int64_t left = (int64_t)t.q_len * P.gs - row0;
     t.row0 = (int)row0;
     t.n_row = row0 < 0 || left <= 0 ? 0 : (int)min(left, (int64_t)P.item_rows);
   }
-  t.trow = P.rows ? P.rows[t.r] : t.r;
-  t.kv = max(P.kv_lens[t.r], 0);
+  t.trow = P.rows ? uniform(P.rows[t.r]) : t.r;
+  t.kv = max(uniform(P.kv_lens[t.r]), 0);
   t.len = (int)min((int64_t)t.kv, (int64_t)P.max_blocks << P.log2b);
   if (t.trow < 0 || t.trow >= P.n_rows) t.len = 0, t.trow = 0;
   t.limit = t.n_row > 0 ? sees(P, t, (t.row0 + t.n_row - 1) / P.gs) : 0;
@@ -99,14 +100,17 @@ KVT_DEV void store_out4(void* out, int ot, int64_t at, float a, float b, float c
 // Eight elements of a query row each at at(k), k < N -> operands.  bf16 rows are scaled by a power of two to fit fp16;
 // returns its inverse.  top_of reduces a lane's largest |q| over the lanes that share its row.
 template <int QT, int N, class At, class Top>
-KVT_DEV float load_q(const void* q, int64_t row, bool live, At at, Top top_of, h8 (&out)[N]) {
+KVT_DEV float load_q(const void* q, int64_t row, At at, Top top_of, h8 (&out)[N]) {
   uint4 raw[N];
 #pragma unroll
   for (int k = 0; k < N; ++k)
-    raw[k] = live ? *reinterpret_cast<const uint4*>((const uint16_t*)q + row + at(k)) : make_uint4(0, 0, 0, 0);
+raw[k] = *reinterpret_cast<const uint4*>((const uint16_t*)q + row + at(k));
   if constexpr (QT == kF16) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) out[k] = __builtin_bit_cast(h8, raw[k]);
+    for (int k = 0; k < N; ++k) {
+      asm("" : "+v"(raw[k].x), "+v"(raw[k].y), "+v"(raw[k].z), "+v"(raw[k].w));   // (as plain registers: loaded tuples cost spills)
+      out[k] = __builtin_bit_cast(h8, raw[k]);
+    }
     return 1.0f;
   } else {
     float top = 0.0f;

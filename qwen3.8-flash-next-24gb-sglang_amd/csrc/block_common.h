@@ -22,7 +22,9 @@ enum Code : int { kE4M3 = 0, kI8 = 1 };
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxReq = 4096;          // requests of one call (the search below takes two rounds of 64)
 
-KVT_DEV float qmax_of(int code) { return code == kE4M3 ? 448.0f : 127.0f; }
+// A value that every lane has, in a scalar register (what a uniform address loads is not taken for one by itself).
+KVT_DEV int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+KVT_DEV float uniform(float v) { return __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(v))); }
 
 // The smallest power of two s with a / s <= qmax (both codes' qmax = t * 2^p, t in [1, 2)), within 2^-64 .. 2^122.
 template <int CODE>

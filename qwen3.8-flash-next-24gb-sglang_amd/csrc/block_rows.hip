@@ -65,11 +65,13 @@ __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot
   const int tile0 = split * tps, tile1 = min(tile0 + tps, tiles_of(P, it.limit));
   if (tile0 >= tile1 && P.splits > 1) return;       // (the merge knows which splits there are)
 
-  const int my = it.row0 + l, qi = my / P.gs, hq = h * P.gs + my % P.gs;
+  const int my = it.row0 + l, qi = my / P.gs;
   const bool live = l < it.n_row;
   h8 Q[D / 32];
   // (chunk c of 64 channels: 16 of them per group g, two operands)
-  const float qf = load_q<QT>(P.q, (int64_t)(it.q0 + qi) * P.sq_n + (int64_t)hq * P.sq_h, live,
+  // (rows behind the item's last compute what its first does; nothing is stored of them)
+  const int lq = live ? my : it.row0;
+  const float qf = load_q<QT>(P.q, (int64_t)(it.q0 + lq / P.gs) * P.sq_n + (int64_t)(h * P.gs + lq % P.gs) * P.sq_h,
                               [g](int k) { return 64 * (k >> 1) + 16 * g + 8 * (k & 1); }, max_xor16_32, Q) * P.scale_log2;
   const int see = sees(P, it, qi);
   const int all_see = sees(P, it, it.row0 / P.gs);   // (the fewest of the item's rows: positions below it need no comparison)
@@ -333,7 +335,8 @@ int check(const Attn& P, int Hq, int D, int block, int code, int qt, int ot) {
   if ((uintptr_t)P.q & 15 || P.sq_n % 8 || P.sq_h % 8 || ((uintptr_t)P.k8 | (uintptr_t)P.v8) & 15) return KVT_EINVAL;
   const int out8 = ot == kF32 ? 4 : 8;   // 16-byte aligned output rows
   if ((uintptr_t)P.out & 15 || P.so_n % out8 || P.so_h % out8) return KVT_EINVAL;
-  if (P.H > 65535 || P.splits > kMostSplits || (int64_t)P.max_blocks * block > 0x7FFFFFFF) return KVT_ERANGE;
+  if (P.H > 65535 || P.splits > kMostSplits || (int64_t)P.max_blocks * block > 0x7FFFFFFF ||
+      (int64_t)P.H * block * D > 0xFFFFFFFFll) return KVT_ERANGE;
   return KVT_OK;
 }
 

@@ -35,9 +35,14 @@ KVT_DEV float sum_xor32(float v) {
 }
 
 constexpr int kDsRead = 0x100, kMfma = 0x8;   // instruction classes of the scheduling hints
-constexpr int kAhead = 4;             // operands read ahead of their product
 constexpr float kLeast = 0x1p-120f;   // (a factor of 0 would make a masked score, -inf, a NaN)
 
+// The largest of three (asm: no canonicalizing v_max_f32 x, x for values out of a matrix product)
+KVT_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 template <int D>
 struct Tile {
   static constexpr int T = D == 256 ? 32 : 64;
@@ -45,7 +50,6 @@ struct Tile {
   static constexpr int VP = 2 * T + 16;         // bytes per V^T row (a channel)
   static constexpr int TPK = 256 / T;           // threads per K row
   static constexpr int NK = D / 16 / TPK;       // 16-byte pieces of a K row per thread
-  static constexpr int VT = T * D / 32;         // threads that convert V (8 positions x 4 channels each)
 };
 
 template <int D>
@@ -58,16 +62,19 @@ struct __align__(16) Buf {
 
 // A thread's share of a tile as loaded: pieces of one K row, and 4 channels of 8 positions of V.
 template <int D>
-struct Raw {
-  u4v k[Tile<D>::NK];
-  uint32_t v[8];
+struct RawK {
+  u4v c[Tile<D>::NK];
   float ks, vs;
+};
+struct RawV {
+  uint32_t c[8];
 };
 
 template <int CODE, int QT, int D>
 __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int items, int ot) {
   using C = Tile<D>;
   constexpr int T = C::T, SUB = T / 32, DT = D / 32;
+  constexpr int kAhead = D == 256 ? 2 : 4;     // operands read ahead of their product (what the registers hold)
   __shared__ Buf<D> buf[2];
   const int tid = threadIdx.x, lane = tid & 63, l = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -83,7 +90,9 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
   const int my = it.row0 + 32 * wave + l, qi = my / P.gs, hq = h * P.gs + my % P.gs;
   const bool live = 32 * wave + l < it.n_row;
   h8 Q[D / 16];
-  const float qf = load_q<QT>(P.q, (int64_t)(it.q0 + qi) * P.sq_n + (int64_t)hq * P.sq_h, live,
+  // (rows behind the item's last compute what its first does; nothing is stored of them)
+  const int lq = live ? my : it.row0;
+  const float qf = load_q<QT>(P.q, (int64_t)(it.q0 + lq / P.gs) * P.sq_n + (int64_t)(h * P.gs + lq % P.gs) * P.sq_h,
                               [g](int k) { return 16 * k + 8 * g; }, max_xor32, Q) * P.scale_log2;
   const int see = live ? sees(P, it, qi) : 0;
   const int first_row = it.row0 + 32 * wave, last_row = it.row0 + min(32 * wave + 31, it.n_row - 1);
@@ -91,53 +100,63 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
   const int all_see = any_row ? sees(P, it, first_row / P.gs) : 0;   // positions that every row of the wavefront sees
   const int most_see = any_row ? sees(P, it, last_row / P.gs) : 0;   // and that any of them sees
 
-  // this thread's share of a tile
+  // This thread's share of a tile: 16-byte pieces kpc, kpc + TPK, .. of K row krow; channels vd .. vd + 3 of V rows vrow +
+  // {0 .. 3, 8 .. 11}.  A wavefront's rows all lie in the 16 positions `sub` of the tile, i.e. in one block: its id and the
+  // addresses' bases are uniform.
   const int krow = tid / C::TPK, kpc = tid % C::TPK;
-  const int vc = (tid & 3) + 4 * (tid >> (D == 256 ? 8 : D == 128 ? 7 : 6)), vd = 4 * ((tid >> 2) & (D / 4 - 1));
-  const int vrow = 16 * (vc >> 1) + 4 * (vc & 1);                    // positions vrow + {0 .. 3, 8 .. 11}
-  const bool has_v = C::VT == 256 || tid < C::VT;
+  const int sub = T == 32 ? wave >> 1 : wave;
+  const int vc = 2 * sub + (lane & 1), vd = 4 * ((lane >> 1) + (T == 32 ? 32 * (wave & 1) : 0));
+  const int vrow = 16 * sub + 4 * (lane & 1);
+  const bool has_v = vd < D;
   const int32_t* table = P.table + it.trow * P.stride;
+  const int bmask = (1 << P.log2b) - 1;
+  const int64_t head = (int64_t)h * (D << P.log2b);
+  const uint32_t block_bytes = (uint32_t)P.H * (D << P.log2b);        // (of one block: < 2^32, the entry point sees to it)
+  const uint32_t koff = (uint32_t)(krow & 15) * D + 16 * kpc, voff = 4u * (lane & 1) * D + (has_v ? vd : 0);
 
   // (no branch around a load: the wait for it would move to where the paths join)
-  const auto id_at = [&](int p) { return table[min(p, it.limit - 1) >> P.log2b]; };
+  const auto id_at = [&](int tile) { return table[min(tile * T + 16 * sub, it.limit - 1) >> P.log2b]; };
   const auto in_pool = [&](int id) { return (uint32_t)id < (uint32_t)P.n_blocks; };
-  const auto row_at = [&](int id, int p) {
-    return ((((int64_t)(in_pool(id) ? id : 0) * P.H + h) << P.log2b) + (p & ((1 << P.log2b) - 1))) * D;
+  const auto offset = [&](int id, int tile) {   // of the wavefront's 16 positions
+    return (uint64_t)(in_pool(id) ? (uint32_t)id : 0u) * block_bytes + (uint32_t)((tile * T + 16 * sub) & bmask) * D;
   };
-  const auto fetch = [&](int tile, int idk, int idv, Raw<D>& r) {
-    const int pk = tile * T + krow, pv = tile * T + vrow;
-    const uint8_t* kp = P.k8 + row_at(idk, pk) + 16 * kpc;
+  const auto fetch_k = [&](int tile, int id, RawK<D>& r) {
+    const uint8_t* p = P.k8 + head + offset(id, tile);
 #pragma unroll
-    for (int i = 0; i < C::NK; ++i) r.k[i] = *reinterpret_cast<const u4v*>(kp + 16 * C::TPK * i);
-    const uint8_t* vp = P.v8 + row_at(idv, pv) + vd;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i] = *reinterpret_cast<const uint32_t*>(vp + (i + (i & 4)) * D);
-    const int64_t at = (int64_t)(in_pool(idk) ? idk : 0) * P.H + h;
+    for (int i = 0; i < C::NK; ++i) r.c[i] = *reinterpret_cast<const u4v*>(p + (koff + 16 * C::TPK * i));
+    const uint32_t at = (in_pool(id) ? (uint32_t)id : 0u) * (uint32_t)P.H + h;   // (< 2^32 / 1,024: blocks of 1,024 bytes at least)
     r.ks = P.ks[at], r.vs = P.vs[at];
   };
-  const auto convert = [&](int tile, int idk, int idv, Raw<D>& r, Buf<D>& b) {
+  const auto fetch_v = [&](int tile, int id, RawV& r) {
+    const uint8_t* p = P.v8 + head + offset(id, tile);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.c[i] = *reinterpret_cast<const uint32_t*>(p + (voff + (i + (i & 4)) * D));
+  };
+  const auto convert_k = [&](int id, const RawK<D>& r, Buf<D>& b) {
     uint8_t* kr = b.k + krow * C::KP;
 #pragma unroll
     for (int i = 0; i < C::NK; ++i) {
       h8* to = reinterpret_cast<h8*>(kr + 32 * (kpc + C::TPK * i));
-      to[0] = operand<CODE>(r.k[i].x, r.k[i].y);
-      to[1] = operand<CODE>(r.k[i].z, r.k[i].w);
+      to[0] = operand<CODE>(r.c[i].x, r.c[i].y);
+      to[1] = operand<CODE>(r.c[i].z, r.c[i].w);
     }
     if ((krow & 15) == 0 && kpc == 0) {
       b.ks[krow >> 4] = r.ks;
-      b.vs[krow >> 4] = in_pool(idk) ? r.vs : 0.0f;
-      b.there[krow >> 4] = in_pool(idk);
+      b.vs[krow >> 4] = r.vs;
+      b.there[krow >> 4] = in_pool(id);
     }
+  };
+  const auto convert_v = [&](int tile, int id, RawV& r, Buf<D>& b) {
     if (!has_v) return;
     const int left = it.limit - (tile * T + vrow);                   // positions behind the last one, or in no block: 0
-    if (!in_pool(idv) || left < 12) {
+    if (!in_pool(id) || left < 12) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r.v[i] = in_pool(idv) && i + (i & 4) < left ? r.v[i] : 0u;
+      for (int i = 0; i < 8; ++i) r.c[i] = in_pool(id) && i + (i & 4) < left ? r.c[i] : 0u;
     }
     uint32_t lo[4], hi[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t a = flip<CODE>(r.v[2 * j]), c = flip<CODE>(r.v[2 * j + 1]);
+      const uint32_t a = flip<CODE>(r.c[2 * j]), c = flip<CODE>(r.c[2 * j + 1]);
       lo[j] = __builtin_amdgcn_perm(c, a, 0x05010400u);
       hi[j] = __builtin_amdgcn_perm(c, a, 0x07030602u);
     }
@@ -156,40 +175,55 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
   f16v acc[DT];
 #pragma unroll
   for (int c = 0; c < DT; ++c) acc[c] = f16v{};
-  float m = -__builtin_inff(), sum = 0.0f, unit = 0.0f, per_unit = 0.0f, peak = 0.0f;
+  float m = -__builtin_inff(), sum = 0.0f;
+  float unit = 0.0f, per_unit = 0.0f, peak = 0.0f;                   // uniform
 
   if (tile0 < tile1) {
-    Raw<D> raw;
-    int idk = id_at(tile0 * T + krow), idv = id_at(tile0 * T + vrow);
-    fetch(tile0, idk, idv, raw);
-    convert(tile0, idk, idv, raw, buf[0]);
-    idk = id_at((tile0 + 1) * T + krow), idv = id_at((tile0 + 1) * T + vrow);
+    RawK<D> rk;
+    RawV rv;
+    int id = uniform(id_at(tile0));
+    fetch_k(tile0, id, rk);
+    fetch_v(tile0, id, rv);
+    convert_k(id, rk, buf[0]);
+    convert_v(tile0, id, rv, buf[0]);
+    int then = id_at(tile0 + 1);
     __syncthreads();
     for (int tile = tile0; tile < tile1; ++tile) {
       const Buf<D>& b = buf[(tile - tile0) & 1];
-      const bool more = tile + 1 < tile1;
-      // (behind the last tile: the same addresses as its own last position's block, unused)
-      fetch(tile + 1, idk, idv, raw);
-      const int nk = id_at((tile + 2) * T + krow), nv = id_at((tile + 2) * T + vrow);
+      Buf<D>& next = buf[(tile + 1 - tile0) & 1];
+      // The next tile's codes (behind the last tile: the block of its last position again, unused).  At D = 256 the registers
+      // hold only one side at a time: K's codes under the first product, V's under the second.
+      constexpr bool kApart = D == 256;
+      id = uniform(then);
+      fetch_k(tile + 1, id, rk);
+      if (!kApart) fetch_v(tile + 1, id, rv);
+      then = id_at(tile + 2);
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
         const int p0 = tile * T + 32 * u;
-        if (p0 >= most_see) continue;
+        const bool work = p0 < most_see;
         f16v sc = {};
-        const uint8_t* kb = b.k + (32 * u + l) * C::KP + 16 * g;
-        h8 a[kAhead];
+        if (work) {
+          const uint8_t* kb = b.k + (32 * u + l) * C::KP + 16 * g;
+          h8 a[kAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) a[k] = *reinterpret_cast<const h8*>(kb + 32 * k);
-        __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
+          for (int k = 0; k < kAhead; ++k) a[k] = *reinterpret_cast<const h8*>(kb + 32 * k);
+          __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          sc = mfma(a[k % kAhead], Q[k], sc);
-          __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
-          if (k + kAhead < D / 16) {
-            a[k % kAhead] = *reinterpret_cast<const h8*>(kb + 32 * (k + kAhead));
-            __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+          for (int k = 0; k < D / 16; ++k) {
+            sc = mfma(a[k % kAhead], Q[k], sc);
+            __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+            if (k + kAhead < D / 16) {
+              a[k % kAhead] = *reinterpret_cast<const h8*>(kb + 32 * (k + kAhead));
+              __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+            }
           }
         }
+        if (kApart) {
+          convert_k(id, rk, next);
+          fetch_v(tile + 1, id, rv);
+        }
+        if (!work) continue;
         const int there[2] = {b.there[2 * u], b.there[2 * u + 1]};
         if (p0 + 32 > all_see || !(there[0] & there[1])) {
           const int seen[2] = {there[0] ? see : 0, there[1] ? see : 0};
@@ -199,9 +233,11 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
         }
         // (the factors are positive, so the largest score of a half is its largest product times the factor)
         const float f[2] = {fmaxf(qf * b.ks[2 * u], kLeast), fmaxf(qf * b.ks[2 * u + 1], kLeast)};
-        float top2[2] = {sc[0], sc[8]};
+        float top2[2];
 #pragma unroll
-        for (int j = 1; j < 8; ++j) top2[0] = fmaxf(top2[0], sc[j]), top2[1] = fmaxf(top2[1], sc[8 + j]);
+        for (int s = 0; s < 2; ++s)
+          top2[s] = max3(max3(sc[8 * s], sc[8 * s + 1], sc[8 * s + 2]), max3(sc[8 * s + 3], sc[8 * s + 4], sc[8 * s + 5]),
+                         fmaxf(sc[8 * s + 6], sc[8 * s + 7]));
         const float top = max_xor32(fmaxf(top2[0] * f[0], top2[1] * f[1]));
         const bool rise = top > m + kLag;
         if (__any(rise)) {
@@ -213,28 +249,30 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
           for (int c = 0; c < DT; ++c) acc[c] *= a;
         }
         const float ms = (m == -__builtin_inff() ? 0.0f : m) - kLift;
-        float x[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          x[i] = exp2_(fmaf(sc[i], f[i >> 3], -ms));
-          sum += x[i];
-        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const float fv = bits_f((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(b.vs[2 * u + s])));
-          if (fv > unit || (fv > 0.0f && fv < 0.25f * unit)) {       // uniform
+          // V's scale relative to the unit goes into the exponent: P = 2^(x - m + 10 + log2 ru), and the row sum adds P / ru.
+          const float fv = uniform(b.vs[2 * u + s]);
+          if (fv > unit || (fv > 0.0f && fv < 0.25f * unit)) {
             const float a = new_unit(fv, unit, peak);
             per_unit = 1.0f / unit;
 #pragma unroll
             for (int c = 0; c < DT; ++c) acc[c] *= a;
           }
-          const float ru = fv * per_unit;
+          float ru = fv * per_unit;
+          const bool small = !(ru >= 0.25f);                         // (a scale of 0, or 2^-80 below the largest)
+          const float rs = small ? 1.0f : ru;
+          const float off = __builtin_amdgcn_logf(rs) - ms;
           h8 p;
+          float add = 0.0f;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const h2 y = h2_rne(x[8 * s + 2 * j] * ru, x[8 * s + 2 * j + 1] * ru);
+            const h2 y = h2_rne(exp2_(fmaf(sc[8 * s + 2 * j], f[s], off)), exp2_(fmaf(sc[8 * s + 2 * j + 1], f[s], off)));
+            add = __builtin_amdgcn_fdot2(y, h2{(_Float16)1.0f, (_Float16)1.0f}, add, false);
             p[2 * j] = y.x, p[2 * j + 1] = y.y;
           }
+          sum = fmaf(add, 1.0f / rs, sum);
+          if (small) p = p * (_Float16)ru;
           const uint8_t* vb = b.v + l * C::VP + 16 * (4 * u + 2 * s + g);
           constexpr int AV = DT < kAhead ? DT : kAhead;
           h8 a[AV];
@@ -252,8 +290,8 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
           }
         }
       }
-      if (more) convert(tile + 1, idk, idv, raw, buf[(tile + 1 - tile0) & 1]);
-      idk = nk, idv = nv;
+      if (!kApart) convert_k(id, rk, next);
+      convert_v(tile + 1, id, rv, next);
       __syncthreads();
     }
   }

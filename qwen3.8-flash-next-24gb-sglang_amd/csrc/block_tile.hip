@@ -56,8 +56,7 @@ template <int D>
 struct __align__(16) Buf {
   uint8_t k[Tile<D>::T * Tile<D>::KP];
   uint8_t v[D * Tile<D>::VP];
-  float ks[Tile<D>::T / 16], vs[Tile<D>::T / 16];
-  int there[Tile<D>::T / 16];                   // 0: no such block
+  float scale[Tile<D>::T / 32][4];              // of K in the two halves of 32 positions (-1: no such block), and of V
 };
 
 // A thread's share of a tile as loaded: pieces of one K row, and 4 channels of 8 positions of V.
@@ -71,7 +70,7 @@ struct RawV {
 };
 
 template <int CODE, int QT, int D>
-__global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int items, int ot) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const Attn P, int items, int ot) {
   using C = Tile<D>;
   constexpr int T = C::T, SUB = T / 32, DT = D / 32;
   constexpr int kAhead = D == 256 ? 2 : 4;     // operands read ahead of their product (what the registers hold)
@@ -141,17 +140,18 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
       to[1] = operand<CODE>(r.c[i].z, r.c[i].w);
     }
     if ((krow & 15) == 0 && kpc == 0) {
-      b.ks[krow >> 4] = r.ks;
-      b.vs[krow >> 4] = r.vs;
-      b.there[krow >> 4] = in_pool(id);
+      float* to = b.scale[sub >> 1] + (sub & 1);
+      to[0] = in_pool(id) ? r.ks : -1.0f;
+      to[2] = in_pool(id) ? r.vs : 0.0f;
     }
   };
   const auto convert_v = [&](int tile, int id, RawV& r, Buf<D>& b) {
     if (!has_v) return;
-    const int left = it.limit - (tile * T + vrow);                   // positions behind the last one, or in no block: 0
-    if (!in_pool(id) || left < 12) {
+    const int left = in_pool(id) ? it.limit - (tile * T + 16 * sub) : 0;   // positions behind the last one, or in no block: 0
+    if (left < 16) {
+      const int mine = left - (vrow & 15);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r.c[i] = in_pool(id) && i + (i & 4) < left ? r.c[i] : 0u;
+      for (int i = 0; i < 8; ++i) r.c[i] = i + (i & 4) < mine ? r.c[i] : 0u;
     }
     uint32_t lo[4], hi[4];
 #pragma unroll
@@ -175,8 +175,9 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
   f16v acc[DT];
 #pragma unroll
   for (int c = 0; c < DT; ++c) acc[c] = f16v{};
-  float m = -__builtin_inff(), sum = 0.0f;
-  float unit = 0.0f, per_unit = 0.0f, peak = 0.0f;                   // uniform
+  float m = -__builtin_inff(), lift = 0x1p120f, sum = 0.0f, part = 0.0f;   // (part: of the sum, in units of ru)
+  float unit = 0.0f, peak = 0.0f, ru = 0.0f, log_ru = 0.0f, per_ru = 1.0f;   // uniform, as the next two
+  int last = -1, lost = 0;
 
   if (tile0 < tile1) {
     RawK<D> rk;
@@ -203,12 +204,14 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
         const int p0 = tile * T + 32 * u;
         const bool work = p0 < most_see;
         f16v sc = {};
+        f4 scale;
         if (work) {
+          scale = *reinterpret_cast<const f4*>(b.scale[u]);
           const uint8_t* kb = b.k + (32 * u + l) * C::KP + 16 * g;
           h8 a[kAhead];
 #pragma unroll
           for (int k = 0; k < kAhead; ++k) a[k] = *reinterpret_cast<const h8*>(kb + 32 * k);
-          __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
+          __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead + 1, 0);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             sc = mfma(a[k % kAhead], Q[k], sc);
@@ -224,15 +227,19 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
           fetch_v(tile + 1, id, rv);
         }
         if (!work) continue;
-        const int there[2] = {b.there[2 * u], b.there[2 * u + 1]};
-        if (p0 + 32 > all_see || !(there[0] & there[1])) {
-          const int seen[2] = {there[0] ? see : 0, there[1] ? see : 0};
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            sc[i] = p0 + 8 * (i >> 2) + 4 * g + (i & 3) < seen[i >> 3] ? sc[i] : -__builtin_inff();
-        }
+        const float ks[2] = {uniform(scale[0]), uniform(scale[1])}, vs[2] = {uniform(scale[2]), uniform(scale[3])};
         // (the factors are positive, so the largest score of a half is its largest product times the factor)
-        const float f[2] = {fmaxf(qf * b.ks[2 * u], kLeast), fmaxf(qf * b.ks[2 * u + 1], kLeast)};
+        float f[2] = {qf * ks[0], qf * ks[1]};
+        if (p0 + 32 > all_see || ks[0] < 0.0f || ks[1] < 0.0f) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const int seen = ks[s] < 0.0f ? 0 : see;
+            f[s] = f[s] < kLeast ? kLeast : f[s];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              sc[8 * s + j] = p0 + 16 * s + 8 * (j >> 2) + 4 * g + (j & 3) < seen ? sc[8 * s + j] : -__builtin_inff();
+          }
+        }
         float top2[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -243,36 +250,38 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
         if (__any(rise)) {
           const float m1 = rise ? top : m;
           const float a = m1 == m ? 1.0f : exp2_(m - m1);
-          sum *= a;
+          sum *= a, part *= a;
           m = m1;
+          lift = kLift - fmaxf(m, -0x1p120f);                        // (a row that has seen nothing: 2^-inf is 0 for any of these)
 #pragma unroll
           for (int c = 0; c < DT; ++c) acc[c] *= a;
         }
-        const float ms = (m == -__builtin_inff() ? 0.0f : m) - kLift;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          // V's scale relative to the unit goes into the exponent: P = 2^(x - m + 10 + log2 ru), and the row sum adds P / ru.
-          const float fv = uniform(b.vs[2 * u + s]);
-          if (fv > unit || (fv > 0.0f && fv < 0.25f * unit)) {
-            const float a = new_unit(fv, unit, peak);
-            per_unit = 1.0f / unit;
+          // V's scale relative to the unit (ru) goes into the exponent: P = 2^(x - m + 10 + log2 ru), and the row sum adds P / ru.
+          // Most halves have the scale of the one before.
+          if (__float_as_int(vs[s]) != last) {
+            last = __float_as_int(vs[s]);
+            if (vs[s] > unit || (vs[s] > 0.0f && vs[s] < 0.25f * unit)) {
+              const float a = new_unit(vs[s], unit, peak);
 #pragma unroll
-            for (int c = 0; c < DT; ++c) acc[c] *= a;
+              for (int c = 0; c < DT; ++c) acc[c] *= a;
+            }
+            ru = unit > 0.0f ? vs[s] / unit : 0.0f;
+            lost = uniform((int)(ru < 0.25f));                       // (a scale of 0, or 2^-80 below the largest)
+            const float rs = lost ? 1.0f : ru;
+            sum = fmaf(part, per_ru, sum), part = 0.0f;
+            log_ru = __builtin_amdgcn_logf(rs), per_ru = 1.0f / rs;
           }
-          float ru = fv * per_unit;
-          const bool small = !(ru >= 0.25f);                         // (a scale of 0, or 2^-80 below the largest)
-          const float rs = small ? 1.0f : ru;
-          const float off = __builtin_amdgcn_logf(rs) - ms;
+          const float off = log_ru + lift;
           h8 p;
-          float add = 0.0f;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const h2 y = h2_rne(exp2_(fmaf(sc[8 * s + 2 * j], f[s], off)), exp2_(fmaf(sc[8 * s + 2 * j + 1], f[s], off)));
-            add = __builtin_amdgcn_fdot2(y, h2{(_Float16)1.0f, (_Float16)1.0f}, add, false);
+            part = __builtin_amdgcn_fdot2(y, h2{(_Float16)1.0f, (_Float16)1.0f}, part, false);
             p[2 * j] = y.x, p[2 * j + 1] = y.y;
           }
-          sum = fmaf(add, 1.0f / rs, sum);
-          if (small) p = p * (_Float16)ru;
+          if (lost) p = p * (_Float16)ru;
           const uint8_t* vb = b.v + l * C::VP + 16 * (4 * u + 2 * s + g);
           constexpr int AV = DT < kAhead ? DT : kAhead;
           h8 a[AV];
@@ -297,7 +306,7 @@ __global__ __launch_bounds__(256, 2) void block_tile_kernel(const Attn P, int it
   }
 
   // register i of acc[c]: channel 32 c + 8 (i / 4) + 4 g + i % 4 of row l
-  sum = sum_xor32(sum);
+  sum = sum_xor32(fmaf(part, per_ru, sum));
   if (!live) return;
   const float f = sum == 0.0f ? 0.0f : unit / sum;
   if (P.splits == 1) {

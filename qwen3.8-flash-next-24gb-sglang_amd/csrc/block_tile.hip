@@ -43,11 +43,21 @@ KVT_DEV float max3(float a, float b, float c) {
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
+// v, where the compiler does not know it: what follows from it is computed here, not kept in registers from further up.
+KVT_DEV int again(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 template <int D>
 struct Tile {
   static constexpr int T = D == 256 ? 32 : 64;
   static constexpr int KP = 2 * D + 16;         // bytes per K row (a position)
-  static constexpr int VP = 2 * T + 16;         // bytes per V^T row (a channel)
+  // V^T rows (a channel each): 16-byte pieces in an order that depends on the channel, where T = 32 (the padding would not
+  // leave room for what D = 256 keeps of Q in LDS), else padded
+  static constexpr int VP = T == 32 ? 64 : 2 * T + 16;
+  static KVT_DEV int piece(int channel, int i) { return T == 32 ? i ^ (channel >> 2 & 3) : i; }
+  static constexpr int QL = D == 256 ? 3 : 0;   // operands of Q that are kept in LDS: the registers hold no more than 13
   static constexpr int TPK = 256 / T;           // threads per K row
   static constexpr int NK = D / 16 / TPK;       // 16-byte pieces of a K row per thread
 };
@@ -63,10 +73,10 @@ struct __align__(16) Buf {
 template <int D>
 struct RawK {
   u4v c[Tile<D>::NK];
-  float ks, vs;
 };
 struct RawV {
   uint32_t c[8];
+  float ks, vs;
 };
 
 template <int CODE, int QT, int D>
@@ -75,6 +85,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
   constexpr int T = C::T, SUB = T / 32, DT = D / 32;
   constexpr int kAhead = D == 256 ? 2 : 4;     // operands read ahead of their product (what the registers hold)
   __shared__ Buf<D> buf[2];
+  __shared__ h8 qlds[C::QL ? C::QL : 1][256];
   const int tid = threadIdx.x, lane = tid & 63, l = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // head fastest: with H = 2, 4 or 8 the workgroups of a head share the caches of the same XCDs; the last rows, which see
@@ -86,23 +97,25 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
   const int tile0 = split * tps, tile1 = min(tile0 + tps, tiles_of(P, it.limit));
   if (tile0 >= tile1 && P.splits > 1) return;
 
-  const int my = it.row0 + 32 * wave + l, qi = my / P.gs, hq = h * P.gs + my % P.gs;
+  const int my = it.row0 + 32 * wave + l;
   const bool live = 32 * wave + l < it.n_row;
+  constexpr int QR = D / 16 - C::QL;
   h8 Q[D / 16];
   // (rows behind the item's last compute what its first does; nothing is stored of them)
   const int lq = live ? my : it.row0;
   const float qf = load_q<QT>(P.q, (int64_t)(it.q0 + lq / P.gs) * P.sq_n + (int64_t)(h * P.gs + lq % P.gs) * P.sq_h,
                               [g](int k) { return 16 * k + 8 * g; }, max_xor32, Q) * P.scale_log2;
-  const int see = live ? sees(P, it, qi) : 0;
+#pragma unroll
+  for (int k = 0; k < C::QL; ++k) qlds[k][tid] = Q[QR + k];          // (each lane its own: no barrier)
+  const int see = live ? sees(P, it, my / P.gs) : 0;
   const int first_row = it.row0 + 32 * wave, last_row = it.row0 + min(32 * wave + 31, it.n_row - 1);
   const bool any_row = 32 * wave < it.n_row;
   const int all_see = any_row ? sees(P, it, first_row / P.gs) : 0;   // positions that every row of the wavefront sees
   const int most_see = any_row ? sees(P, it, last_row / P.gs) : 0;   // and that any of them sees
 
-  // This thread's share of a tile: 16-byte pieces kpc, kpc + TPK, .. of K row krow; channels vd .. vd + 3 of V rows vrow +
+  // This thread's share of a tile: 16-byte pieces tid % TPK, + TPK, .. of K row tid / TPK; channels vd .. vd + 3 of V rows vrow +
   // {0 .. 3, 8 .. 11}.  A wavefront's rows all lie in the 16 positions `sub` of the tile, i.e. in one block: its id and the
   // addresses' bases are uniform.
-  const int krow = tid / C::TPK, kpc = tid % C::TPK;
   const int sub = T == 32 ? wave >> 1 : wave;
   const int vc = 2 * sub + (lane & 1), vd = 4 * ((lane >> 1) + (T == 32 ? 32 * (wave & 1) : 0));
   const int vrow = 16 * sub + 4 * (lane & 1);
@@ -111,7 +124,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
   const int bmask = (1 << P.log2b) - 1;
   const int64_t head = (int64_t)h * (D << P.log2b);
   const uint32_t block_bytes = (uint32_t)P.H * (D << P.log2b);        // (of one block: < 2^32, the entry point sees to it)
-  const uint32_t koff = (uint32_t)(krow & 15) * D + 16 * kpc, voff = 4u * (lane & 1) * D + (has_v ? vd : 0);
+
+  // At D = 256 the registers hold only one side of the next tile at a time: K's codes under the first product, V's under the
+  // second, and addresses are computed where they are used.
+  constexpr bool kApart = D == 256;
 
   // (no branch around a load: the wait for it would move to where the paths join)
   const auto id_at = [&](int tile) { return table[min(tile * T + 16 * sub, it.limit - 1) >> P.log2b]; };
@@ -121,31 +137,35 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
   };
   const auto fetch_k = [&](int tile, int id, RawK<D>& r) {
     const uint8_t* p = P.k8 + head + offset(id, tile);
+    const int t = kApart ? again(tid) : tid;
+    const uint32_t koff = (uint32_t)(t / C::TPK & 15) * D + 16 * (t % C::TPK);
 #pragma unroll
     for (int i = 0; i < C::NK; ++i) r.c[i] = *reinterpret_cast<const u4v*>(p + (koff + 16 * C::TPK * i));
-    const uint32_t at = (in_pool(id) ? (uint32_t)id : 0u) * (uint32_t)P.H + h;   // (< 2^32 / 1,024: blocks of 1,024 bytes at least)
-    r.ks = P.ks[at], r.vs = P.vs[at];
   };
   const auto fetch_v = [&](int tile, int id, RawV& r) {
     const uint8_t* p = P.v8 + head + offset(id, tile);
+    const uint32_t voff = 4u * (lane & 1) * D + (has_v ? vd : 0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) r.c[i] = *reinterpret_cast<const uint32_t*>(p + (voff + (i + (i & 4)) * D));
+    const uint32_t at = (in_pool(id) ? (uint32_t)id : 0u) * (uint32_t)P.H + h;   // (< 2^32: a block and head is 1 KiB at least)
+    r.ks = P.ks[at], r.vs = P.vs[at];
   };
-  const auto convert_k = [&](int id, const RawK<D>& r, Buf<D>& b) {
-    uint8_t* kr = b.k + krow * C::KP;
+  const auto convert_k = [&](const RawK<D>& r, Buf<D>& b) {
+    const int t = kApart ? again(tid) : tid;
+    uint8_t* kr = b.k + t / C::TPK * C::KP + 32 * (t % C::TPK);
 #pragma unroll
     for (int i = 0; i < C::NK; ++i) {
-      h8* to = reinterpret_cast<h8*>(kr + 32 * (kpc + C::TPK * i));
+      h8* to = reinterpret_cast<h8*>(kr + 32 * C::TPK * i);
       to[0] = operand<CODE>(r.c[i].x, r.c[i].y);
       to[1] = operand<CODE>(r.c[i].z, r.c[i].w);
     }
-    if ((krow & 15) == 0 && kpc == 0) {
+  };
+  const auto convert_v = [&](int tile, int id, RawV& r, Buf<D>& b) {
+    if ((T == 64 || !(wave & 1)) && lane == 0) {
       float* to = b.scale[sub >> 1] + (sub & 1);
       to[0] = in_pool(id) ? r.ks : -1.0f;
       to[2] = in_pool(id) ? r.vs : 0.0f;
     }
-  };
-  const auto convert_v = [&](int tile, int id, RawV& r, Buf<D>& b) {
     if (!has_v) return;
     const int left = in_pool(id) ? it.limit - (tile * T + 16 * sub) : 0;   // positions behind the last one, or in no block: 0
     if (left < 16) {
@@ -168,7 +188,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
         const uint32_t u = c < 2 ? lo[j] : hi[j];
         y[j] = c & 1 ? pair<CODE, true>(u) : pair<CODE, false>(u);
       }
-      *reinterpret_cast<h8*>(b.v + (vd + c) * C::VP + 16 * vc) = h8{y[0].x, y[0].y, y[1].x, y[1].y, y[2].x, y[2].y, y[3].x, y[3].y};
+      *reinterpret_cast<h8*>(b.v + (vd + c) * C::VP + 16 * C::piece(vd, vc)) = h8{y[0].x, y[0].y, y[1].x, y[1].y, y[2].x, y[2].y, y[3].x, y[3].y};
     }
   };
 
@@ -185,16 +205,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
     int id = uniform(id_at(tile0));
     fetch_k(tile0, id, rk);
     fetch_v(tile0, id, rv);
-    convert_k(id, rk, buf[0]);
+    convert_k(rk, buf[0]);
     convert_v(tile0, id, rv, buf[0]);
     int then = id_at(tile0 + 1);
     __syncthreads();
     for (int tile = tile0; tile < tile1; ++tile) {
       const Buf<D>& b = buf[(tile - tile0) & 1];
       Buf<D>& next = buf[(tile + 1 - tile0) & 1];
-      // The next tile's codes (behind the last tile: the block of its last position again, unused).  At D = 256 the registers
-      // hold only one side at a time: K's codes under the first product, V's under the second.
-      constexpr bool kApart = D == 256;
+      // the next tile's codes (behind the last tile: the block of its last position again, unused)
       id = uniform(then);
       fetch_k(tile + 1, id, rk);
       if (!kApart) fetch_v(tile + 1, id, rv);
@@ -203,30 +221,43 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
       for (int u = 0; u < SUB; ++u) {
         const int p0 = tile * T + 32 * u;
         const bool work = p0 < most_see;
-        f16v sc = {};
+        if (!kApart && !work) continue;
+        f16v sc;
         f4 scale;
-        if (work) {
-          scale = *reinterpret_cast<const f4*>(b.scale[u]);
-          const uint8_t* kb = b.k + (32 * u + l) * C::KP + 16 * g;
-          h8 a[kAhead];
+        if (!kApart || work) {
+          sc = f16v{};
+          const int lz = kApart ? again(lane) : lane;
+          const uint8_t* kb = b.k + (32 * u + (lz & 31)) * C::KP + 16 * (lz >> 5);
+          h8 a[kAhead], q[C::QL ? C::QL : 1];
 #pragma unroll
           for (int k = 0; k < kAhead; ++k) a[k] = *reinterpret_cast<const h8*>(kb + 32 * k);
-          __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead + 1, 0);
+          __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead, 0);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
-            sc = mfma(a[k % kAhead], Q[k], sc);
+            sc = mfma(a[k % kAhead], k < QR ? Q[k < QR ? k : 0] : q[k < QR ? 0 : k - QR], sc);
             __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
             if (k + kAhead < D / 16) {
               a[k % kAhead] = *reinterpret_cast<const h8*>(kb + 32 * (k + kAhead));
               __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
             }
+            if (k + kAhead >= QR && k + kAhead < D / 16) {
+              q[k + kAhead - QR] = qlds[k + kAhead - QR][tid];
+              __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+            }
+            if (k + kAhead == D / 16) {
+              scale = *reinterpret_cast<const f4*>(b.scale[u]);
+              __builtin_amdgcn_sched_group_barrier(kDsRead, 1, 0);
+            }
           }
         }
         if (kApart) {
-          convert_k(id, rk, next);
+          __builtin_amdgcn_sched_barrier(0);
+          convert_k(rk, next);
+          __builtin_amdgcn_sched_barrier(0);
           fetch_v(tile + 1, id, rv);
+          __builtin_amdgcn_sched_barrier(0);
         }
-        if (!work) continue;
+        if (kApart && !work) continue;
         const float ks[2] = {uniform(scale[0]), uniform(scale[1])}, vs[2] = {uniform(scale[2]), uniform(scale[3])};
         // (the factors are positive, so the largest score of a half is its largest product times the factor)
         float f[2] = {qf * ks[0], qf * ks[1]};
@@ -264,15 +295,17 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
             last = __float_as_int(vs[s]);
             if (vs[s] > unit || (vs[s] > 0.0f && vs[s] < 0.25f * unit)) {
               const float a = new_unit(vs[s], unit, peak);
+              unit = uniform(unit), peak = uniform(peak);
 #pragma unroll
               for (int c = 0; c < DT; ++c) acc[c] *= a;
             }
-            ru = unit > 0.0f ? vs[s] / unit : 0.0f;
+            ru = uniform(unit > 0.0f ? vs[s] / unit : 0.0f);
             lost = uniform((int)(ru < 0.25f));                       // (a scale of 0, or 2^-80 below the largest)
             const float rs = lost ? 1.0f : ru;
             sum = fmaf(part, per_ru, sum), part = 0.0f;
-            log_ru = __builtin_amdgcn_logf(rs), per_ru = 1.0f / rs;
+            log_ru = uniform(__builtin_amdgcn_logf(rs)), per_ru = uniform(1.0f / rs);
           }
+          __builtin_amdgcn_sched_barrier(0);
           const float off = log_ru + lift;
           h8 p;
 #pragma unroll
@@ -282,7 +315,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
             p[2 * j] = y.x, p[2 * j + 1] = y.y;
           }
           if (lost) p = p * (_Float16)ru;
-          const uint8_t* vb = b.v + l * C::VP + 16 * (4 * u + 2 * s + g);
+          const int lz = kApart ? again(lane) : lane;
+          const uint8_t* vb = b.v + (lz & 31) * C::VP + 16 * C::piece(lz, 4 * u + 2 * s + (lz >> 5));
           constexpr int AV = DT < kAhead ? DT : kAhead;
           h8 a[AV];
 #pragma unroll
@@ -299,7 +333,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
           }
         }
       }
-      if (!kApart) convert_k(id, rk, next);
+      if (!kApart) convert_k(rk, next);
       convert_v(tile + 1, id, rv, next);
       __syncthreads();
     }
@@ -307,7 +341,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
 
   // register i of acc[c]: channel 32 c + 8 (i / 4) + 4 g + i % 4 of row l
   sum = sum_xor32(fmaf(part, per_ru, sum));
-  if (!live) return;
+  int row = again(l);                           // (its query and head are computed again: no registers for them till now)
+  row += 32 * wave;
+  if (row >= it.n_row) return;
+  const int qi = (it.row0 + row) / P.gs, hq = h * P.gs + (it.row0 + row) % P.gs;
   const float f = sum == 0.0f ? 0.0f : unit / sum;
   if (P.splits == 1) {
     const int64_t o = (int64_t)(it.q0 + qi) * P.so_n + (int64_t)hq * P.so_h + 4 * g;
@@ -319,7 +356,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
         store_out4(P.out, ot, o + 32 * c + 8 * i, acc[c][4 * i] * f + nan, acc[c][4 * i + 1] * f + nan,
                    acc[c][4 * i + 2] * f + nan, acc[c][4 * i + 3] * f + nan);
   } else {
-    const int64_t part = (((int64_t)w * P.H + h) * P.splits + split) * kTileRows + 32 * wave + l;
+    const int64_t part = (((int64_t)w * P.H + h) * P.splits + split) * kTileRows + row;
 #pragma unroll
     for (int c = 0; c < DT; ++c)
 #pragma unroll

@@ -29,6 +29,7 @@ BLOCKS = (16, 32, 64)
 HEAD_DIMS = (64, 128, 256)
 POOL_SHORT, ROW_FULL, TOKENS_OVER, BAD_ROW = 1, 2, 4, 8   # status bits of a plan
 _SPLIT_BLOCKS = 1024     # workgroups of a split launch
+_DECODE_BLOCKS = {64: 1024, 128: 768, 256: 512}   # workgroups of a decode launch: what the 256 CUs hold at once
 _TILE_ROWS = 128         # (query, q head) rows of a workgroup of the query-tile kernel
 _TILE_MIN = 64           # rows per request and KV head from which it serves a call
 
@@ -204,11 +205,10 @@ def kvt_block_decode(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: to
     if n == 0:
         return out
     st = _stream(q, k8, v8, ks, vs, block_table, kv_lens, seqs, out)
-    cap = block_table.shape[1] * B
-    ns = _splits(n * H, cap) if splits is None else int(splits)
+    ns = min(_DECODE_BLOCKS[D], n * H * -(-block_table.shape[1] * B // 128)) if splits is None else int(splits)
     o = ml = None
     if ns > 1:
-        o, ml = _parts(workspace, n * H * ns * 16, D, q.device)
+        o, ml = _parts(workspace, 2 * ns * 16, D, q.device)
     _lib.call("kvt_block_decode", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], kv_lens.data_ptr(), n,
               H, Hq, D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B,
               block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1], _lib.ptr(seqs),

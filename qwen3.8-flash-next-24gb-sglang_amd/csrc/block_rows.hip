@@ -28,6 +28,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kTile = 32;
 constexpr int kMostSplits = 1024;
+constexpr int kFewPairs = 32;        // (request, KV head) pairs up to which decode's merge is spread over many workgroups
 
 template <int BYTES> struct Raw { uint32_t w[BYTES / 4]; };
 template <int BYTES>
@@ -50,21 +51,20 @@ KVT_DEV float lane_f(float v, int lane) {
   return bits_f((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
 }
 
+// The wavefronts' results: O (rows x channels), maximum, sum, unit.
+template <int D>
+struct Join {
+  float o[kWaves][16][D + 4];
+  float m[kWaves][16], l[kWaves][16], u[kWaves];
+};
+
+// Tiles tile0 .. tile1 - 1 of an item and KV head: into out where they are all that the item has (whole), else as part
+// `slot`: its own result with its maximum and sum.
 template <int CODE, int QT, int D>
-__global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot) {
+KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, bool whole, int64_t slot, int ot, Join<D>& J) {
   constexpr int NC = D / 64;          // 16-byte chunks of a K row per lane
   constexpr int VB = D / 16;          // bytes (channels) of a V row per lane
-  constexpr int LD = D + 4;
-  __shared__ float lo[kWaves][16][LD];
-  __shared__ float lm[kWaves][16], ll[kWaves][16], lu[kWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x, h = blockIdx.y, w = blockIdx.z;
-  const Item it = item_of(P, w);
-  if (it.n_row == 0) return;
-  const int tps = tiles_per_split(P, it.limit);
-  const int tile0 = split * tps, tile1 = min(tile0 + tps, tiles_of(P, it.limit));
-  if (tile0 >= tile1 && P.splits > 1) return;       // (the merge knows which splits there are)
-
   const int my = it.row0 + l, qi = my / P.gs;
   const bool live = l < it.n_row;
   h8 Q[D / 32];
@@ -215,38 +215,209 @@ __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int c = 0; c < VB; c += 4)
-        *reinterpret_cast<f4*>(&lo[wave][l][VB * (4 * g + i) + c]) = f4{acc[c][i], acc[c + 1][i], acc[c + 2][i], acc[c + 3][i]};
-    if (g == 0) lm[wave][l] = m, ll[wave][l] = sum;
+        *reinterpret_cast<f4*>(&J.o[wave][l][VB * (4 * g + i) + c]) = f4{acc[c][i], acc[c + 1][i], acc[c + 2][i], acc[c + 3][i]};
+    if (g == 0) J.m[wave][l] = m, J.l[wave][l] = sum;
   }
-  if (lane == 0) lu[wave] = unit;
+  if (lane == 0) J.u[wave] = unit;
   __syncthreads();
   for (int e = threadIdx.x; e < it.n_row * (D / 4); e += 256) {
     const int row = e / (D / 4), d = 4 * (e % (D / 4));
     float M = -__builtin_inff();
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) M = fmaxf(M, lm[v][row]);
+    for (int v = 0; v < kWaves; ++v) M = fmaxf(M, J.m[v][row]);
     float L = 0.0f, f[kWaves];
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) {
-      f[v] = lm[v][row] == -__builtin_inff() ? 0.0f : exp2_(lm[v][row] - M);
-      L += f[v] * ll[v][row];
+      f[v] = J.m[v][row] == -__builtin_inff() ? 0.0f : exp2_(J.m[v][row] - M);
+      L += f[v] * J.l[v][row];
     }
     // (divided by the sum before the unit comes in: no product is larger than the values themselves)
     f4 O = {0, 0, 0, 0};
     const float per = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) O += *reinterpret_cast<const f4*>(&lo[v][row][d]) * (f[v] * per) * lu[v];
-    if (P.splits == 1) {
+    for (int v = 0; v < kWaves; ++v) O += *reinterpret_cast<const f4*>(&J.o[v][row][d]) * (f[v] * per) * J.u[v];
+    if (whole) {
       const int at = it.row0 + row;
       const int64_t o = (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + d;
       if (L == 0.0f) O = f4{1, 1, 1, 1} * __builtin_nanf("");
       store_out4(P.out, ot, o, O[0], O[1], O[2], O[3]);
     } else {
-      const int64_t part = (((int64_t)w * P.H + h) * P.splits + split) * 16 + row;
+      const int64_t part = slot * 16 + row;
       *reinterpret_cast<f4*>(P.part_o + part * D + d) = O;
       if (d == 0) P.part_ml[2 * part] = M, P.part_ml[2 * part + 1] = L;
     }
   }
+}
+
+template <int CODE, int QT, int D>
+__global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot) {
+  __shared__ Join<D> J;
+  const int split = blockIdx.x, h = blockIdx.y, w = blockIdx.z;
+  const Item it = item_of(P, w);
+  if (it.n_row == 0) return;
+  const int tps = tiles_per_split(P, it.limit);
+  const int tile0 = split * tps, tile1 = min(tile0 + tps, tiles_of(P, it.limit));
+  if (tile0 >= tile1 && P.splits > 1) return;       // (the merge knows which splits there are)
+  attend<CODE, QT, D>(P, it, h, tile0, tile1, P.splits == 1, ((int64_t)w * P.H + h) * P.splits + split, ot, J);
+}
+
+// Decode shares all tiles of a call equally: the (request, KV head) pairs stand in a line, each as long as its tiles plus
+// kPad (what beginning with a pair costs, about), and workgroup w takes [w share, (w + 1) share) of it.  A pair that one
+// workgroup has is written at once; of a pair that several have, each leaves a part, and a second launch merges them.  A
+// workgroup has at most two such pairs, its first (slot 2 w) and its last (2 w + 1): 2 slots per workgroup whatever the
+// lengths are.  (With a fixed number of splits per pair, workgroups of a ragged batch were short and unequal: 64
+// requests of 512 to 8,191 positions, 8 KV heads, 116 us.)
+constexpr int kPad = 4;
+
+// A request's table row and length; rows out of range hold nothing.
+struct Held {
+  int row, len;
+};
+KVT_DEV Held held(const Attn& P, int r) {
+  const int row = P.rows ? P.rows[r] : r, len = (int)min((int64_t)max(P.kv_lens[r], 0), (int64_t)P.max_blocks << P.log2b);
+  return row < 0 || row >= P.n_rows ? Held{0, 0} : Held{row, len};
+}
+KVT_DEV int tiles_in(int len) { return (len + kTile - 1) / kTile; }
+
+// Inclusive sums over the wavefront's lanes (all active).
+KVT_DEV uint32_t wave_scan(uint32_t v) {
+  int x = (int)v;
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8: within 16 lanes
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);   // lane 15 of rows 0, 2 to rows 1, 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);   // lane 31 to the upper half
+  return (uint32_t)x;
+}
+// The line of a call, per head, in steps of 2^shift tiles (the entry point picks the shift so that 32 bits hold it): its
+// length, where request r begins, and what r holds.
+struct Line {
+  uint32_t total, at;
+  int r;
+  Held has;
+};
+KVT_DEV uint32_t steps_of(const Attn& P, int tiles) { return (uint32_t)((tiles + kPad + (1 << P.shift) - 1) >> P.shift); }
+// find(total, before, own, r): whether r, which takes `own` steps behind `before`, is the request sought.
+template <class Find>
+KVT_DEV Line line_of(const Attn& P, Find find) {
+  const int lane = threadIdx.x & 63;
+  Line s{0, 0, 0, {0, 0}};
+  Held has{0, 0};
+  uint32_t own = 0, sum = 0;
+  const auto look = [&](int c) {
+    has = held(P, min(c + lane, P.n - 1));
+    own = c + lane < P.n ? steps_of(P, tiles_in(has.len)) : 0u;
+    sum = wave_scan(own);
+  };
+  for (int c = 0; c < P.n; c += 64) {
+    look(c);
+    s.total += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+  }
+  uint32_t before = 0;
+  for (int c = 0; c < P.n; c += 64) {
+    if (P.n > 64) look(c);
+    const uint64_t hit = __ballot(c + lane < P.n && find(s.total, before + sum - own, own, c + lane));
+    if (hit) {
+      const int i = __builtin_ctzll(hit);
+      s.r = c + i, s.at = before + (uint32_t)__builtin_amdgcn_readlane((int)(sum - own), i);
+      s.has = Held{__builtin_amdgcn_readlane(has.row, i), __builtin_amdgcn_readlane(has.len, i)};
+      break;
+    }
+    before += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+  }
+  return s;
+}
+KVT_DEV uint32_t share_of(const Attn& P, uint32_t total) {
+  return max((total * P.H + P.splits - 1) / P.splits, ((kWaves + kPad) + (1u << P.shift) - 1) >> P.shift);
+}
+
+template <int CODE, int QT, int D>
+__global__ __launch_bounds__(256, 2) void block_decode_kernel(const Attn P, int ot) {
+  __shared__ Join<D> J;
+  const uint32_t w = blockIdx.x;
+  const Line s = line_of(P, [&](uint32_t total, uint32_t before, uint32_t own, int) {
+    const uint32_t x = w * share_of(P, total);
+    return before * P.H <= x && x < (before + own) * P.H;
+  });
+  const uint32_t share = share_of(P, s.total), all = s.total * P.H, x0 = w * share, x1 = min(x0 + share, all);
+  if (x0 >= x1) return;
+  int r = s.r;
+  uint32_t at = s.at * P.H;                         // of request r's head 0
+  Held has = s.has;
+  uint32_t steps = steps_of(P, tiles_in(has.len));
+  int h = (int)((x0 - at) / steps);                 // (the first pair)
+  for (;;) {
+    Item it;
+    it.r = r, it.trow = has.row, it.q0 = r, it.q_len = 1, it.row0 = 0, it.n_row = P.gs;
+    it.kv = it.len = it.limit = has.len;
+    const Held then = held(P, min(r + 1, P.n - 1));  // (the next request's: under this one's work)
+    const int tiles = tiles_in(has.len);
+    for (; h < P.H; ++h) {
+      const uint32_t a = at + (uint32_t)h * steps;
+      if (a >= x1) return;
+      const int t0 = a < x0 ? (int)min((uint64_t)(x0 - a) << P.shift, (uint64_t)tiles) : 0;
+      const int t1 = (int)min((uint64_t)(x1 - a) << P.shift, (uint64_t)tiles);
+      if (t0 < t1 || (tiles == 0 && a >= x0)) {
+        attend<CODE, QT, D>(P, it, h, t0, t1, t0 == 0 && t1 == tiles, 2 * (int64_t)w + (a > x0), ot, J);
+        __syncthreads();                            // (J is free again)
+      }
+    }
+    h = 0;
+    at += P.H * steps;
+    if (++r >= P.n || at >= x1) return;
+    has = Held{uniform(then.row), uniform(then.len)};
+    steps = steps_of(P, tiles_in(has.len));
+  }
+}
+
+// The merge of decode: pair (blockIdx.z, blockIdx.y)'s parts, where it has several.  D / 4 lanes per row, or (SPREAD, for
+// calls of few pairs, which may have hundreds of parts) one workgroup per row and 64 channels.
+template <int D, bool SPREAD>
+__global__ __launch_bounds__(256) void block_decode_merge_kernel(const Attn P, int ot) {
+  constexpr int LPR = SPREAD ? 16 : D / 4, NG = 256 / LPR;
+  __shared__ f4 os[SPREAD ? NG : 1][LPR];
+  __shared__ float ls[SPREAD ? NG : 1], red[4];
+  const int h = blockIdx.y, r = blockIdx.z, grp = threadIdx.x / LPR, lp = threadIdx.x % LPR;
+  const int row = SPREAD ? blockIdx.x / (D / 64) : blockIdx.x * NG + grp;
+  const int d = 4 * lp + (SPREAD ? 64 * (blockIdx.x % (D / 64)) : 0);
+  const Line s = line_of(P, [&](uint32_t, uint32_t, uint32_t, int i) { return i == r; });
+  const uint32_t share = share_of(P, s.total);
+  const int tiles = tiles_in(s.has.len);
+  const uint32_t a = s.at * P.H + (uint32_t)h * steps_of(P, tiles);
+  const int w0 = (int)(a / share), w1 = (int)((a + (uint32_t)(max(tiles - 1, 0) >> P.shift)) / share);
+  if (w0 == w1 || row >= P.gs) return;              // (uniform where the barriers below are)
+  const auto part_of = [&](int w) { return (2 * (int64_t)w + (a > (uint32_t)w * share)) * 16 + row; };
+  float M = -__builtin_inff(), L = 0.0f;
+  if (SPREAD) {
+    for (int w = w0 + threadIdx.x; w <= w1; w += 256) M = fmaxf(M, P.part_ml[2 * part_of(w)]);
+    M = group_max<64>(M);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  } else {
+    for (int w = w0; w <= w1; ++w) M = fmaxf(M, P.part_ml[2 * part_of(w)]);
+  }
+  // (weights are scaled by 2^-45 (l is below 2^45): their sums times the largest values stay finite)
+  f4 O = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int w = SPREAD ? w0 + grp : w0; w <= w1; w += SPREAD ? NG : 1) {
+    const int64_t p = part_of(w);
+    const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * p);
+    const float f = ml.x == -__builtin_inff() ? 0.0f : exp2_(ml.x - M) * ml.y * 0x1p-45f;
+    L += f;
+    O += f * *reinterpret_cast<const f4*>(P.part_o + p * D + d);
+  }
+  if (SPREAD) {
+    os[grp][lp] = O;
+    if (lp == 0) ls[grp] = L;
+    __syncthreads();
+    if (grp) return;
+#pragma unroll
+    for (int i = 1; i < NG; ++i) O += os[i][lp], L += ls[i];
+  }
+  O = L == 0.0f ? f4{1, 1, 1, 1} * __builtin_nanf("") : O / L;
+  store_out4(P.out, ot, (int64_t)r * P.so_n + (int64_t)(h * P.gs + row) * P.so_h + d, O[0], O[1], O[2], O[3]);
 }
 
 // Merge of the splits of a row: one workgroup per (row, 64 channels, KV head and item).  A part is a split's own result with
@@ -297,30 +468,80 @@ __global__ __launch_bounds__(NT) void block_merge_kernel(const Attn P, int D, in
   if (L == 0.0f) O = f4{1, 1, 1, 1} * __builtin_nanf("");
   store_out4(P.out, ot, o, O[0], O[1], O[2], O[3]);
 }
-void merge(const Attn& P, int D, int items, int rows, int ot, hipStream_t st) {
-  const dim3 grid(rows, D / 64, P.H * items);
-  if (P.splits > 64) block_merge_kernel<1024><<<grid, 1024, 0, st>>>(P, D, ot);
-  else block_merge_kernel<256><<<grid, 256, 0, st>>>(P, D, ot);
+// The same for up to kFew splits: D / 4 lanes per row, which read its parts side by side.
+constexpr int kFew = 16;
+template <int D>
+__global__ __launch_bounds__(256) void block_merge_few_kernel(const Attn P, int ot) {
+  constexpr int LPR = D / 4;
+  const int row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, d = 4 * (threadIdx.x % LPR), h = blockIdx.y, w = blockIdx.z;
+  const Item it = item_of(P, w);
+  if (row >= it.n_row) return;
+  const int tps = tiles_per_split(P, it.limit);
+  const int used = (tiles_of(P, it.limit) + tps - 1) / tps;
+  const int64_t part = ((int64_t)w * P.H + h) * P.splits * P.item_rows + row;
+  float wgt[kFew], l[kFew], M = -__builtin_inff(), L = 0.0f;
+#pragma unroll
+  for (int s = 0; s < kFew; ++s) {
+    const float2 ml = s < used ? *reinterpret_cast<const float2*>(P.part_ml + 2 * (part + (int64_t)P.item_rows * s))
+                               : make_float2(-__builtin_inff(), 0.0f);
+    wgt[s] = ml.x, l[s] = ml.y;
+  }
+#pragma unroll
+  for (int s = 0; s < kFew; ++s) M = fmaxf(M, wgt[s]);
+#pragma unroll
+  for (int s = 0; s < kFew; ++s) {
+    wgt[s] = wgt[s] == -__builtin_inff() ? 0.0f : exp2_(wgt[s] - M) * l[s];
+    L += wgt[s];
+  }
+  const float per = 1.0f / L;                                       // (no product is larger than the values themselves)
+  f4 O = {0, 0, 0, 0};
+#pragma unroll
+  for (int s = 0; s < kFew; ++s)
+    if (s < used) O += (wgt[s] * per) * *reinterpret_cast<const f4*>(P.part_o + (part + (int64_t)P.item_rows * s) * D + d);
+  const int at = it.row0 + row;
+  const int64_t o = (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + d;
+  if (L == 0.0f) O = f4{1, 1, 1, 1} * __builtin_nanf("");
+  store_out4(P.out, ot, o, O[0], O[1], O[2], O[3]);
+}
+template <int D>
+void merge(const Attn& P, int items, int rows, int ot, hipStream_t st) {
+  if (P.splits <= kFew) {
+    block_merge_few_kernel<D><<<dim3((rows * (D / 4) + 255) / 256, P.H, items), 256, 0, st>>>(P, ot);
+  } else {
+    const dim3 grid(rows, D / 64, P.H * items);
+    if (P.splits > 64) block_merge_kernel<1024><<<grid, 1024, 0, st>>>(P, D, ot);
+    else block_merge_kernel<256><<<grid, 256, 0, st>>>(P, D, ot);
+  }
 }
 
 template <int CODE, int QT, int D>
-void launch(const Attn& P, int items, int rows, int ot, hipStream_t st) {
-  block_rows_kernel<CODE, QT, D><<<dim3(P.splits, P.H, items), 256, 0, st>>>(P, ot);
-  if (P.splits > 1) merge(P, D, items, rows, ot, st);
+void launch(const Attn& P, int items, int ot, hipStream_t st) {
+  if (P.cu) {
+    block_rows_kernel<CODE, QT, D><<<dim3(P.splits, P.H, items), 256, 0, st>>>(P, ot);
+    if (P.splits > 1) merge<D>(P, items, 16, ot, st);
+    return;
+  }
+  block_decode_kernel<CODE, QT, D><<<P.splits, 256, 0, st>>>(P, ot);
+  if (P.splits == 1) return;
+  if (P.n * P.H <= kFewPairs) {
+    block_decode_merge_kernel<D, true><<<dim3(P.gs * (D / 64), P.H, P.n), 256, 0, st>>>(P, ot);
+  } else {
+    block_decode_merge_kernel<D, false><<<dim3((P.gs * (D / 4) + 255) / 256, P.H, P.n), 256, 0, st>>>(P, ot);
+  }
 }
 template <int CODE, int QT>
-void launch_d(const Attn& P, int D, int items, int rows, int ot, hipStream_t st) {
-  if (D == 64) launch<CODE, QT, 64>(P, items, rows, ot, st);
-  else if (D == 128) launch<CODE, QT, 128>(P, items, rows, ot, st);
-  else launch<CODE, QT, 256>(P, items, rows, ot, st);
+void launch_d(const Attn& P, int D, int items, int ot, hipStream_t st) {
+  if (D == 64) launch<CODE, QT, 64>(P, items, ot, st);
+  else if (D == 128) launch<CODE, QT, 128>(P, items, ot, st);
+  else launch<CODE, QT, 256>(P, items, ot, st);
 }
-void launch_all(const Attn& P, int code, int qt, int D, int items, int rows, int ot, hipStream_t st) {
+void launch_all(const Attn& P, int code, int qt, int D, int items, int ot, hipStream_t st) {
   if (code == kE4M3) {
-    if (qt == kBF16) launch_d<kE4M3, kBF16>(P, D, items, rows, ot, st);
-    else launch_d<kE4M3, kF16>(P, D, items, rows, ot, st);
+    if (qt == kBF16) launch_d<kE4M3, kBF16>(P, D, items, ot, st);
+    else launch_d<kE4M3, kF16>(P, D, items, ot, st);
   } else {
-    if (qt == kBF16) launch_d<kI8, kBF16>(P, D, items, rows, ot, st);
-    else launch_d<kI8, kF16>(P, D, items, rows, ot, st);
+    if (qt == kBF16) launch_d<kI8, kBF16>(P, D, items, ot, st);
+    else launch_d<kI8, kF16>(P, D, items, ot, st);
   }
 }
 
@@ -335,7 +556,7 @@ int check(const Attn& P, int Hq, int D, int block, int code, int qt, int ot) {
   if ((uintptr_t)P.q & 15 || P.sq_n % 8 || P.sq_h % 8 || ((uintptr_t)P.k8 | (uintptr_t)P.v8) & 15) return KVT_EINVAL;
   const int out8 = ot == kF32 ? 4 : 8;   // 16-byte aligned output rows
   if ((uintptr_t)P.out & 15 || P.so_n % out8 || P.so_h % out8) return KVT_EINVAL;
-  if (P.H > 65535 || P.splits > kMostSplits || (int64_t)P.max_blocks * block > 0x7FFFFFFF ||
+  if (P.H > 65535 || P.splits > (P.cu ? kMostSplits : 65535) || (int64_t)P.max_blocks * block > 0x7FFFFFFF ||
       (int64_t)P.H * block * D > 0xFFFFFFFFll) return KVT_ERANGE;
   return KVT_OK;
 }
@@ -354,12 +575,12 @@ extern "C" int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q
   P.sq_n = sq_n, P.sq_h = sq_h, P.so_n = so_n, P.so_h = so_h, P.stride = bt_stride, P.scale_log2 = scale * kLog2e;
   P.n = n, P.n_rows = n_rows, P.n_q = n, P.H = H, P.gs = H > 0 ? Hq / H : 0, P.n_blocks = n_blocks;
   P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.splits = n_splits, P.causal = 0;
-  P.item_rows = 16, P.tile = kTile, P.least = kWaves;
+  P.item_rows = 16, P.tile = kTile, P.least = kWaves, P.shift = 0;
+  while (P.shift < 31 && ((double)n * H * (((double)max_blocks * block / kTile + kPad) / (1 << P.shift) + 2) + n_splits) > 2e9) ++P.shift;
   const int st = check(P, Hq, D, block, code, q_type, out_type);
   if (st != KVT_OK) return st;
   if (n_splits > 1 && (!part_o || !part_ml)) return KVT_EINVAL;
-  if (n_splits > 1 && (int64_t)n * H > 65535) return KVT_ERANGE;
-  launch_all(P, code, q_type, D, n, P.gs, out_type, (hipStream_t)stream);
+  launch_all(P, code, q_type, D, n, out_type, (hipStream_t)stream);
   KVT_CHECK_LAUNCH();
   return KVT_OK;
 }
@@ -387,9 +608,13 @@ extern "C" int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int 
   if (items > (tiled ? 0x7FFFFFFF / P.H : 65535) || (n_splits > 1 && items * P.H > 65535)) return KVT_ERANGE;
   if (tiled) {
     tile_launch(P, code, q_type, D, (int)items, out_type, (hipStream_t)stream);
-    if (n_splits > 1) merge(P, D, (int)items, kTileRows, out_type, (hipStream_t)stream);
+    if (n_splits > 1) {
+      if (D == 64) merge<64>(P, (int)items, kTileRows, out_type, (hipStream_t)stream);
+      else if (D == 128) merge<128>(P, (int)items, kTileRows, out_type, (hipStream_t)stream);
+      else merge<256>(P, (int)items, kTileRows, out_type, (hipStream_t)stream);
+    }
   } else {
-    launch_all(P, code, q_type, D, (int)items, 16, out_type, (hipStream_t)stream);
+    launch_all(P, code, q_type, D, (int)items, out_type, (hipStream_t)stream);
   }
   KVT_CHECK_LAUNCH();
   return KVT_OK;

@@ -28,8 +28,13 @@ CODE = {torch.float8_e4m3fn: 0, torch.int8: 1}
 BLOCKS = (16, 32, 64)
 HEAD_DIMS = (64, 128, 256)
 POOL_SHORT, ROW_FULL, TOKENS_OVER, BAD_ROW = 1, 2, 4, 8   # status bits of a plan
-_SPLIT_BLOCKS = 1024     # workgroups of a split launch
-_DECODE_BLOCKS = {64: 1024, 128: 768, 256: 512}   # workgroups of a decode launch: what the 256 CUs hold at once
+# Decode: a number of splits for each (request, KV head) pair, about 768 workgroups in all (512 for one request, whose splits
+# are equal), or, for many pairs over long tables, equal shares of all positions.  Measured, device us per call with the
+# merge, best splits against shares, up to 8,191 positions ragged: 64 pairs (8 requests, D 128) 19.8 / 37.9; 128 (D 256)
+# 39.2 / 43.1; 256 (D 128) 44.3 / 45.4; 256 (D 256) 99.3 / 86.6; 512 (D 128) 100.2 / 92.8; up to 1,000 positions, 256
+# pairs 23.6 / 25.6.
+_SHARE_PAIRS, _SHARE_CAP = 256, 2048
+_DECODE_BLOCKS = {64: 1024, 128: 768, 256: 512}   # workgroups of a launch in equal shares: what the 256 CUs hold at once
 _TILE_ROWS = 128         # (query, q head) rows of a workgroup of the query-tile kernel
 _TILE_MIN = 64           # rows per request and KV head from which it serves a call
 
@@ -180,10 +185,10 @@ def _attn_args(q, out, H, D):
     return _rows16(q, 8), out, Hq
 
 
-def _splits(items: int, cap: int) -> int:
-    """Workgroups that share an item's positions: about _SPLIT_BLOCKS in all, none with fewer than 128 positions of the
-    table's capacity."""
-    return max(1, min(_SPLIT_BLOCKS // items, -(-cap // 128)))
+def _splits(items: int, cap: int, blocks: int) -> int:
+    """Workgroups that share an item's positions: about `blocks` in all, none with fewer than 128 positions of the table's
+    capacity."""
+    return max(1, min(blocks // items, -(-cap // 128)))
 
 
 def kvt_block_decode(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: torch.Tensor, vs: torch.Tensor,
@@ -205,10 +210,16 @@ def kvt_block_decode(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: to
     if n == 0:
         return out
     st = _stream(q, k8, v8, ks, vs, block_table, kv_lens, seqs, out)
-    ns = min(_DECODE_BLOCKS[D], n * H * -(-block_table.shape[1] * B // 128)) if splits is None else int(splits)
+    cap = block_table.shape[1] * B
+    if splits is not None:
+        ns = int(splits)
+    elif n * H >= _SHARE_PAIRS and cap >= _SHARE_CAP:
+        ns = -_DECODE_BLOCKS[D]
+    else:
+        ns = _splits(n * H, cap, 768 if n > 1 else 512)
     o = ml = None
-    if ns > 1:
-        o, ml = _parts(workspace, 2 * ns * 16, D, q.device)
+    if ns > 1 or ns < -1:
+        o, ml = _parts(workspace, n * H * ns * 16 if ns > 1 else -2 * ns * 16, D, q.device)
     _lib.call("kvt_block_decode", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], kv_lens.data_ptr(), n,
               H, Hq, D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B,
               block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1], _lib.ptr(seqs),
@@ -239,7 +250,7 @@ def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8:
     st = _stream(q, cu_q, k8, v8, ks, vs, block_table, kv_lens, seqs, out)
     rows = _TILE_ROWS if total * (Hq // H) >= _TILE_MIN * n else 16
     items = total * (Hq // H) // rows + n
-    ns = _splits(items * H, block_table.shape[1] * B) if splits is None else int(splits)
+    ns = _splits(items * H, block_table.shape[1] * B, 384 if rows > 16 else 1024) if splits is None else int(splits)
     o = ml = None
     if ns > 1:
         o, ml = _parts(workspace, items * H * ns * rows, D, q.device)

@@ -28,7 +28,7 @@ struct Attn {
   int n, n_rows, n_q, H, gs, n_blocks, max_blocks, log2b, splits, causal;
   int item_rows;               // rows of a work item
   int tile, least;             // positions of a tile, fewest tiles of a split
-  int shift;                   // decode: steps of the line are 2^shift tiles
+  int shares, shift;           // decode in equal shares (0: in splits): workgroups; steps of their line are 2^shift tiles
 };
 
 // What a workgroup has: request r, query rows [row0, row0 + n_row) of it in (query, q head) order, the query base, and the

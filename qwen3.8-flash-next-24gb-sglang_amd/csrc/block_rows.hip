@@ -28,7 +28,6 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kTile = 32;
 constexpr int kMostSplits = 1024;
-constexpr int kFewPairs = 32;        // (request, KV head) pairs up to which decode's merge is spread over many workgroups
 
 template <int BYTES> struct Raw { uint32_t w[BYTES / 4]; };
 template <int BYTES>
@@ -267,7 +266,7 @@ __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot
 // workgroup has at most two such pairs, its first (slot 2 w) and its last (2 w + 1): 2 slots per workgroup whatever the
 // lengths are.  (With a fixed number of splits per pair, workgroups of a ragged batch were short and unequal: 64
 // requests of 512 to 8,191 positions, 8 KV heads, 116 us.)
-constexpr int kPad = 4;
+constexpr int kPad = 8;
 
 // A request's table row and length; rows out of range hold nothing.
 struct Held {
@@ -329,7 +328,7 @@ KVT_DEV Line line_of(const Attn& P, Find find) {
   return s;
 }
 KVT_DEV uint32_t share_of(const Attn& P, uint32_t total) {
-  return max((total * P.H + P.splits - 1) / P.splits, ((kWaves + kPad) + (1u << P.shift) - 1) >> P.shift);
+  return max((total * P.H + P.shares - 1) / P.shares, (kWaves + (1u << P.shift) - 1) >> P.shift);
 }
 
 template <int CODE, int QT, int D>
@@ -371,50 +370,29 @@ __global__ __launch_bounds__(256, 2) void block_decode_kernel(const Attn P, int 
   }
 }
 
-// The merge of decode: pair (blockIdx.z, blockIdx.y)'s parts, where it has several.  D / 4 lanes per row, or (SPREAD, for
-// calls of few pairs, which may have hundreds of parts) one workgroup per row and 64 channels.
-template <int D, bool SPREAD>
+// The merge of shared decode: pair (blockIdx.z, blockIdx.y)'s parts, where it has several.  D / 4 lanes per row.
+template <int D>
 __global__ __launch_bounds__(256) void block_decode_merge_kernel(const Attn P, int ot) {
-  constexpr int LPR = SPREAD ? 16 : D / 4, NG = 256 / LPR;
-  __shared__ f4 os[SPREAD ? NG : 1][LPR];
-  __shared__ float ls[SPREAD ? NG : 1], red[4];
-  const int h = blockIdx.y, r = blockIdx.z, grp = threadIdx.x / LPR, lp = threadIdx.x % LPR;
-  const int row = SPREAD ? blockIdx.x / (D / 64) : blockIdx.x * NG + grp;
-  const int d = 4 * lp + (SPREAD ? 64 * (blockIdx.x % (D / 64)) : 0);
+  constexpr int LPR = D / 4;
+  const int h = blockIdx.y, r = blockIdx.z, row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, d = 4 * (threadIdx.x % LPR);
   const Line s = line_of(P, [&](uint32_t, uint32_t, uint32_t, int i) { return i == r; });
   const uint32_t share = share_of(P, s.total);
   const int tiles = tiles_in(s.has.len);
   const uint32_t a = s.at * P.H + (uint32_t)h * steps_of(P, tiles);
   const int w0 = (int)(a / share), w1 = (int)((a + (uint32_t)(max(tiles - 1, 0) >> P.shift)) / share);
-  if (w0 == w1 || row >= P.gs) return;              // (uniform where the barriers below are)
+  if (w0 == w1 || row >= P.gs) return;
   const auto part_of = [&](int w) { return (2 * (int64_t)w + (a > (uint32_t)w * share)) * 16 + row; };
   float M = -__builtin_inff(), L = 0.0f;
-  if (SPREAD) {
-    for (int w = w0 + threadIdx.x; w <= w1; w += 256) M = fmaxf(M, P.part_ml[2 * part_of(w)]);
-    M = group_max<64>(M);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  } else {
-    for (int w = w0; w <= w1; ++w) M = fmaxf(M, P.part_ml[2 * part_of(w)]);
-  }
+  for (int w = w0; w <= w1; ++w) M = fmaxf(M, P.part_ml[2 * part_of(w)]);
   // (weights are scaled by 2^-45 (l is below 2^45): their sums times the largest values stay finite)
   f4 O = {0, 0, 0, 0};
 #pragma unroll 4
-  for (int w = SPREAD ? w0 + grp : w0; w <= w1; w += SPREAD ? NG : 1) {
+  for (int w = w0; w <= w1; ++w) {
     const int64_t p = part_of(w);
     const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * p);
     const float f = ml.x == -__builtin_inff() ? 0.0f : exp2_(ml.x - M) * ml.y * 0x1p-45f;
     L += f;
     O += f * *reinterpret_cast<const f4*>(P.part_o + p * D + d);
-  }
-  if (SPREAD) {
-    os[grp][lp] = O;
-    if (lp == 0) ls[grp] = L;
-    __syncthreads();
-    if (grp) return;
-#pragma unroll
-    for (int i = 1; i < NG; ++i) O += os[i][lp], L += ls[i];
   }
   O = L == 0.0f ? f4{1, 1, 1, 1} * __builtin_nanf("") : O / L;
   store_out4(P.out, ot, (int64_t)r * P.so_n + (int64_t)(h * P.gs + row) * P.so_h + d, O[0], O[1], O[2], O[3]);
@@ -516,18 +494,13 @@ void merge(const Attn& P, int items, int rows, int ot, hipStream_t st) {
 
 template <int CODE, int QT, int D>
 void launch(const Attn& P, int items, int ot, hipStream_t st) {
-  if (P.cu) {
+  if (!P.shares) {
     block_rows_kernel<CODE, QT, D><<<dim3(P.splits, P.H, items), 256, 0, st>>>(P, ot);
-    if (P.splits > 1) merge<D>(P, items, 16, ot, st);
+    if (P.splits > 1) merge<D>(P, items, P.cu ? 16 : P.gs, ot, st);
     return;
   }
-  block_decode_kernel<CODE, QT, D><<<P.splits, 256, 0, st>>>(P, ot);
-  if (P.splits == 1) return;
-  if (P.n * P.H <= kFewPairs) {
-    block_decode_merge_kernel<D, true><<<dim3(P.gs * (D / 64), P.H, P.n), 256, 0, st>>>(P, ot);
-  } else {
-    block_decode_merge_kernel<D, false><<<dim3((P.gs * (D / 4) + 255) / 256, P.H, P.n), 256, 0, st>>>(P, ot);
-  }
+  block_decode_kernel<CODE, QT, D><<<P.shares, 256, 0, st>>>(P, ot);
+  if (P.shares > 1) block_decode_merge_kernel<D><<<dim3((P.gs * (D / 4) + 255) / 256, P.H, P.n), 256, 0, st>>>(P, ot);
 }
 template <int CODE, int QT>
 void launch_d(const Attn& P, int D, int items, int ot, hipStream_t st) {
@@ -556,7 +529,7 @@ int check(const Attn& P, int Hq, int D, int block, int code, int qt, int ot) {
   if ((uintptr_t)P.q & 15 || P.sq_n % 8 || P.sq_h % 8 || ((uintptr_t)P.k8 | (uintptr_t)P.v8) & 15) return KVT_EINVAL;
   const int out8 = ot == kF32 ? 4 : 8;   // 16-byte aligned output rows
   if ((uintptr_t)P.out & 15 || P.so_n % out8 || P.so_h % out8) return KVT_EINVAL;
-  if (P.H > 65535 || P.splits > (P.cu ? kMostSplits : 65535) || (int64_t)P.max_blocks * block > 0x7FFFFFFF ||
+  if (P.H > 65535 || P.splits > kMostSplits || (int64_t)P.max_blocks * block > 0x7FFFFFFF ||
       (int64_t)P.H * block * D > 0xFFFFFFFFll) return KVT_ERANGE;
   return KVT_OK;
 }
@@ -574,12 +547,14 @@ extern "C" int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q
   P.cu = nullptr, P.out = out, P.part_o = (float*)part_o, P.part_ml = (float*)part_ml;
   P.sq_n = sq_n, P.sq_h = sq_h, P.so_n = so_n, P.so_h = so_h, P.stride = bt_stride, P.scale_log2 = scale * kLog2e;
   P.n = n, P.n_rows = n_rows, P.n_q = n, P.H = H, P.gs = H > 0 ? Hq / H : 0, P.n_blocks = n_blocks;
-  P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.splits = n_splits, P.causal = 0;
+  P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.causal = 0;
+  P.splits = n_splits >= 0 ? n_splits : 1, P.shares = n_splits >= 0 ? 0 : -n_splits;
   P.item_rows = 16, P.tile = kTile, P.least = kWaves, P.shift = 0;
-  while (P.shift < 31 && ((double)n * H * (((double)max_blocks * block / kTile + kPad) / (1 << P.shift) + 2) + n_splits) > 2e9) ++P.shift;
+  while (P.shift < 31 && ((double)n * H * (((double)max_blocks * block / kTile + kPad) / (1 << P.shift) + 2) + P.shares) > 2e9) ++P.shift;
   const int st = check(P, Hq, D, block, code, q_type, out_type);
   if (st != KVT_OK) return st;
-  if (n_splits > 1 && (!part_o || !part_ml)) return KVT_EINVAL;
+  if ((P.splits > 1 || P.shares > 1) && (!part_o || !part_ml)) return KVT_EINVAL;
+  if (P.shares > 65535 || (n_splits > 1 && (int64_t)n * H > 65535)) return KVT_ERANGE;
   launch_all(P, code, q_type, D, n, out_type, (hipStream_t)stream);
   KVT_CHECK_LAUNCH();
   return KVT_OK;
@@ -597,7 +572,7 @@ extern "C" int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int 
   P.cu = (const int32_t*)cu_q, P.out = out, P.part_o = (float*)part_o, P.part_ml = (float*)part_ml;
   P.sq_n = sq_n, P.sq_h = sq_h, P.so_n = so_n, P.so_h = so_h, P.stride = bt_stride, P.scale_log2 = scale * kLog2e;
   P.n = n, P.n_rows = n_rows, P.n_q = n_q, P.H = H, P.gs = H > 0 ? Hq / H : 0, P.n_blocks = n_blocks;
-  P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.splits = n_splits, P.causal = causal;
+  P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.splits = n_splits, P.causal = causal, P.shares = 0;
   const bool tiled = item_rows == kTileRows;
   P.item_rows = item_rows, P.tile = tiled ? tile_positions(D) : kTile, P.least = tiled ? 1 : kWaves;
   const int st = check(P, Hq, D, block, code, q_type, out_type);

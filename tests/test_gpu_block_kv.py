@@ -293,11 +293,19 @@ def test_decode(kvt_pkg, kv, qt, Hq, H, D, B):
     _check_attn(kv, qt, Hq, H, D, B, [1] * len(LENS), LENS, decode=True, seed=Hq + D + B)
 
 
-@pytest.mark.parametrize("splits", [1, 2, 3, 8, 40])
+@pytest.mark.parametrize("splits", [1, 2, 3, 8, 40, -1, -2, -7, -64, -500])
 @pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_decode_splits_and_output_types(kvt_pkg, splits, out_dtype):
     _check_attn("fp8", torch.bfloat16, 16, 2, 128, 32, [1] * 4, [5000, 0, 129, 1000], decode=True, splits=splits,
                 out_dtype=out_dtype, seed=splits)
+
+
+@pytest.mark.parametrize("shares", [None, -1, -5, -300])
+def test_decode_many_requests(kvt_pkg, shares):
+    """More requests than a wavefront has lanes, empty ones among them: the equal shares' line is looked up in rounds."""
+    rng = random.Random(17)
+    lens = [rng.choice([0, 0, 1, 5, 33, 64, 200, rng.randint(1, 700)]) for _ in range(150)]
+    _check_attn("fp8", torch.float16, 4, 2, 64, 16, [1] * 150, lens, decode=True, splits=shares, seed=18)
 
 
 @pytest.mark.parametrize("kv", ["fp8", "int8"])

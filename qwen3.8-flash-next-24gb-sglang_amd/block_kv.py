@@ -28,15 +28,24 @@ CODE = {torch.float8_e4m3fn: 0, torch.int8: 1}
 BLOCKS = (16, 32, 64)
 HEAD_DIMS = (64, 128, 256)
 POOL_SHORT, ROW_FULL, TOKENS_OVER, BAD_ROW = 1, 2, 4, 8   # status bits of a plan
-# Decode: a number of splits for each (request, KV head) pair, about 768 workgroups in all (512 for one request, whose splits
-# are equal), or, for many pairs over long tables, equal shares of all positions.  Measured, device us per call with the
-# merge, best splits against shares, up to 8,191 positions ragged: 64 pairs (8 requests, D 128) 19.8 / 37.9; 128 (D 256)
-# 39.2 / 43.1; 256 (D 128) 44.3 / 45.4; 256 (D 256) 99.3 / 86.6; 512 (D 128) 100.2 / 92.8; up to 1,000 positions, 256
-# pairs 23.6 / 25.6.
-_SHARE_PAIRS, _SHARE_CAP = 256, 2048
-_DECODE_BLOCKS = {64: 1024, 128: 768, 256: 512}   # workgroups of a launch in equal shares: what the 256 CUs hold at once
+# Decode.  Few requests: a number of splits for each (request, KV head) pair.  From _SHARE_REQUESTS on, over long tables:
+# equal shares of all positions.  Measured, device us per call with the merge, caches cold, best splits against shares, up
+# to 8,191 positions ragged: 8 requests x 8 heads (D 128) 19.7 / 22.7; 32 x 2 (D 256, up to 16,384) 65.7 / 52.9; 64 x 2
+# (D 256) 50.2 / 44.9; 16 x 20 (D 64) 40.0 / 37.6; 64 x 8 (D 128) 117 / 98; up to 1,000 positions, 64 x 2 17.9 / 20.5.
+_SHARE_REQUESTS, _SHARE_CAP = 16, 2048
+# Workgroups of a launch in equal shares, and of one request's splits (D 256: one per CU, whose four wavefronts keep enough
+# loads in flight: 52.9 us for 32 x 2 against 57.9 with two; D 128: 98 against 113 with one and 103 with three).
+_DECODE_BLOCKS = {64: 512, 128: 512, 256: 256}
 _TILE_ROWS = 128         # (query, q head) rows of a workgroup of the query-tile kernel
-_TILE_MIN = 64           # rows per request and KV head from which it serves a call
+# Workgroups of a split launch of it, us per call (merge included): D 256, 16 items x 30,000 positions 256 workgroups 150, 512
+# 110; D 128, 6 x 60,000 258 59.7, 384 57.9, 510 63.5; D 64, 20 x 30,000 320 86, 480 77, 640 65.
+_TILE_BLOCKS = {64: 768, 128: 384, 256: 512}
+_TILE_LEAST = 512        # positions of a split at least: its part of 128 rows is 512 D bytes written and read again
+# Rows per request and KV head (on average) from which it serves a call.  us per call against the 16-row kernel's, one request
+# behind 30,000 positions: D 128, 64 rows 41 / 42, 128 rows 66 / 64, 256 rows 72 / 102; D 64, 128 rows 78 / 79, 256 rows 116 /
+# 143; D 256, 128 rows 59 / 44, 256 rows 60 / 61, 512 rows 82 / 90.  Eight ragged requests behind 4,000: D 128, 116 rows 54
+# / 45, 230 rows 70 / 77.
+_TILE_MIN = {64: 128, 128: 128, 256: 256}
 
 
 @dataclass
@@ -185,10 +194,10 @@ def _attn_args(q, out, H, D):
     return _rows16(q, 8), out, Hq
 
 
-def _splits(items: int, cap: int, blocks: int) -> int:
-    """Workgroups that share an item's positions: about `blocks` in all, none with fewer than 128 positions of the table's
-    capacity."""
-    return max(1, min(blocks // items, -(-cap // 128)))
+def _splits(items: int, cap: int, blocks: int, least: int = 128) -> int:
+    """Workgroups that share an item's positions: about `blocks` in all, none with fewer than `least` positions of the
+    table's capacity."""
+    return max(1, min(blocks // items, -(-cap // least)))
 
 
 def kvt_block_decode(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: torch.Tensor, vs: torch.Tensor,
@@ -213,10 +222,10 @@ def kvt_block_decode(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: to
     cap = block_table.shape[1] * B
     if splits is not None:
         ns = int(splits)
-    elif n * H >= _SHARE_PAIRS and cap >= _SHARE_CAP:
+    elif n >= _SHARE_REQUESTS and cap >= _SHARE_CAP:
         ns = -_DECODE_BLOCKS[D]
     else:
-        ns = _splits(n * H, cap, 768 if n > 1 else 512)
+        ns = _splits(n * H, cap, 768 if n > 1 else _DECODE_BLOCKS[D])
     o = ml = None
     if ns > 1 or ns < -1:
         o, ml = _parts(workspace, n * H * ns * 16 if ns > 1 else -2 * ns * 16, D, q.device)
@@ -248,9 +257,13 @@ def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8:
     if n == 0 or total == 0:
         return out
     st = _stream(q, cu_q, k8, v8, ks, vs, block_table, kv_lens, seqs, out)
-    rows = _TILE_ROWS if total * (Hq // H) >= _TILE_MIN * n else 16
+    rows = _TILE_ROWS if total * (Hq // H) >= _TILE_MIN[D] * n else 16
     items = total * (Hq // H) // rows + n
-    ns = _splits(items * H, block_table.shape[1] * B, 384 if rows > 16 else 1024) if splits is None else int(splits)
+    if splits is not None:
+        ns = int(splits)
+    else:
+        full = max(-(-total * (Hq // H) // rows), n) * H     # (items less the empty ones)
+        ns = _splits(full, block_table.shape[1] * B, *((_TILE_BLOCKS[D], _TILE_LEAST) if rows > 16 else (1024,)))
     o = ml = None
     if ns > 1:
         o, ml = _parts(workspace, items * H * ns * rows, D, q.device)

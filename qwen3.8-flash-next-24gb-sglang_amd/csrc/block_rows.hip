@@ -383,10 +383,11 @@ __global__ __launch_bounds__(256) void block_decode_merge_kernel(const Attn P, i
   if (w0 == w1 || row >= P.gs) return;
   const auto part_of = [&](int w) { return (2 * (int64_t)w + (a > (uint32_t)w * share)) * 16 + row; };
   float M = -__builtin_inff(), L = 0.0f;
+#pragma unroll 8
   for (int w = w0; w <= w1; ++w) M = fmaxf(M, P.part_ml[2 * part_of(w)]);
   // (weights are scaled by 2^-45 (l is below 2^45): their sums times the largest values stay finite)
   f4 O = {0, 0, 0, 0};
-#pragma unroll 4
+#pragma unroll 8
   for (int w = w0; w <= w1; ++w) {
     const int64_t p = part_of(w);
     const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * p);

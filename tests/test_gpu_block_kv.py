@@ -313,7 +313,19 @@ def test_decode_many_requests(kvt_pkg, shares):
 @pytest.mark.parametrize("causal", [True, False])
 def test_prefill(kvt_pkg, kv, Hq, H, D, B, causal):
     """Ragged chunks: whole prompts, chunks behind a prefix, one token, none, more queries than positions (rows that see
-    nothing), lengths around the tiles."""
+    nothing), lengths around the tiles; few rows (the decode kernel), then enough for query tiles."""
+    for new, kv_lens in (([65, 17, 1, 0, 40, 128, 5], [65, 200, 1, 50, 23, 131, 5]), ([513, 300, 0, 1, 257], [513, 700, 9, 77, 130])):
+        _check_attn(kv, torch.bfloat16 if D != 64 else torch.float16, Hq, H, D, B, new, kv_lens, causal, seed=D + Hq)
+
+
+@pytest.mark.parametrize("kv", ["fp8", "int8"])
+@pytest.mark.parametrize("Hq,H,D,B", [(16, 2, 256, 16), (5, 1, 256, 64), (8, 1, 128, 32), (20, 4, 64, 64)])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("rows", [16, 128])
+def test_prefill_kernels(kvt_pkg, monkeypatch, kv, Hq, H, D, B, causal, rows):
+    """Both kernels over the same chunks, whatever the rule would take."""
+    from kvtier import block_kv
+    monkeypatch.setattr(block_kv, "_TILE_MIN", {D: 0 if rows == 128 else 10 ** 9})
     new = [65, 17, 1, 0, 40, 128, 5]
     kv_lens = [65, 200, 1, 50, 23, 131, 5]
     _check_attn(kv, torch.bfloat16 if D != 64 else torch.float16, Hq, H, D, B, new, kv_lens, causal, seed=D + Hq)

@@ -349,8 +349,8 @@ int kvt_block_store(const void* k, const void* v, int dtype, int64_t sk_n, int64
 int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q_type, const void* kv_lens, int n, int H, int Hq,
                      int D, int code, const void* k8, const void* v8, const void* ks, const void* vs, int n_blocks,
                      int block, const void* block_table, int64_t bt_stride, int n_rows, int max_blocks, const void* rows,
-                     float scale, int n_splits, void* part_o, void* part_ml, void* out, int out_type, int64_t so_n,
-                     int64_t so_h, void* stream);
+                     float scale, int n_splits, void* part_o, void* part_ml, void* counters, void* out, int out_type,
+                     int64_t so_n, int64_t so_h, void* stream);
 
 /* Attention of chunks of queries: request j owns rows cu_q[j] .. cu_q[j+1] (int32 [n + 1], at most n_q) of q / out.  causal: its
  * queries are the last positions of kv_lens[j] and see the positions up to their own; else every query sees all kv_lens[j]
@@ -362,8 +362,8 @@ int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int q_type, con
                       const void* kv_lens, int n, int H, int Hq, int D, int code, const void* k8, const void* v8,
                       const void* ks, const void* vs, int n_blocks, int block, const void* block_table,
                       int64_t bt_stride, int n_rows, int max_blocks, const void* rows, int causal, float scale,
-                      int item_rows, int n_splits, void* part_o, void* part_ml, void* out, int out_type, int64_t so_n, int64_t so_h,
-                      void* stream);
+                      int item_rows, int n_splits, void* part_o, void* part_ml, void* counters, void* out, int out_type,
+                      int64_t so_n, int64_t so_h, void* stream);
 
 /* ----------------------------------------------------------------------------- lazy backing (HIP VMM) */
 

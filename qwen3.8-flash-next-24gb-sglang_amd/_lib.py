@@ -60,9 +60,9 @@ SIGNATURES = {
     "kvt_block_store": [_P, _P, _I, _L, _L, _L, _L, _I, _I, _I, _P, _P, _I, _P, _P, _L, _I, _I, _I, _P, _P, _P, _P, _I,
                         _I, _P],
     "kvt_block_decode": [_P, _L, _L, _I, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P, _L, _I, _I, _P, _F, _I, _P,
-                         _P, _P, _I, _L, _L, _P],
+                         _P, _P, _P, _I, _L, _L, _P],
     "kvt_block_prefill": [_P, _L, _L, _I, _P, _I, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P, _L, _I, _I, _P,
-                          _I, _F, _I, _I, _P, _P, _P, _I, _L, _L, _P],
+                          _I, _F, _I, _I, _P, _P, _P, _P, _I, _L, _L, _P],
     "kvt_vmm_granularity": [_I, _P],
     "kvt_vmm_reserve": [_I, _U, _P, _P],
     "kvt_vmm_commit": [_P, _U],

@@ -34,8 +34,15 @@ POOL_SHORT, ROW_FULL, TOKENS_OVER, BAD_ROW = 1, 2, 4, 8   # status bits of a pla
 # (D 256) 50.2 / 44.9; 16 x 20 (D 64) 40.0 / 37.6; 64 x 8 (D 128) 117 / 98; up to 1,000 positions, 64 x 2 17.9 / 20.5.
 _SHARE_REQUESTS, _SHARE_CAP = 16, 2048
 # Workgroups of a launch in equal shares, and of one request's splits (D 256: one per CU, whose four wavefronts keep enough
-# loads in flight: 52.9 us for 32 x 2 against 57.9 with two; D 128: 98 against 113 with one and 103 with three).
+# loads in flight: 52.9 us for 32 x 2 against 57.9 with two; D 128: 98 against 113 with one and 103 with three), and of chunks of few rows (4
+# queries a request: 8 x 8, D 128, up to 4,000 positions 19.9 with 8 splits, 24.7 with 16; 32 x 2, D 256, up to 1,000 21.1 with
+# 4, 32.6 with 8).
 _DECODE_BLOCKS = {64: 512, 128: 512, 256: 256}
+# Splits of a pair that a launch with a kept workspace merges itself.  us per call, merged by a second launch / by itself: 8
+# requests x 2 heads (D 256, up to 2,000 positions, 16 splits) 15.8 / 13.8; one x 8 (D 128, 2,000, 16 splits) 12.8 / 9.5; 8 x 8
+# (D 128, up to 4,000, 12 splits) 19.0 / 15.7; chunks of four queries over the same (8 splits) 22.1 / 19.9.  Past 16 the
+# second launch's many workgroups read the parts faster than the last one does.
+_MERGE_SPLITS = 16
 _TILE_ROWS = 128         # (query, q head) rows of a workgroup of the query-tile kernel
 # Workgroups of a split launch of it, us per call (merge included): D 256, 16 items x 30,000 positions 256 workgroups 150, 512
 # 110; D 128, 6 x 60,000 258 59.7, 384 57.9, 510 63.5; D 64, 20 x 30,000 320 86, 480 77, 640 65.
@@ -62,10 +69,11 @@ class BlockPlan:
 
 def _stream(*tensors: Optional[torch.Tensor]) -> int:
     """The current stream of the tensors' device, which has to be the current one (launches go there)."""
-    cur = torch.cuda.current_device() if tensors[0].is_cuda else -1
+    dev = tensors[0].get_device()
+    cur = torch.cuda.current_device() if dev >= 0 else -1
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != cur):
-            _lib.require_device(t)
+        if t is not None and (t.get_device() != cur or dev < 0):
+            _lib.require_device(*tensors)
             raise ValueError(f"tensor on {t.device}, but the current device is cuda:{cur}")
     return _lib.stream(cur)
 
@@ -125,11 +133,7 @@ def kvt_block_plan(seqs: torch.Tensor, counts: torch.Tensor, seq_lens: torch.Ten
             raise ValueError(f"req_to_token has {req_to_token.shape[0]} rows, the block table {rows}")
         rtt, rtt_stride, rtt_cols = req_to_token.data_ptr(), req_to_token.stride(0), req_to_token.shape[1]
     st = _stream(seqs, counts, seq_lens, block_table, free_list, free_head, status, req_to_token)
-    dev = seqs.device
-    cu = torch.empty(n + 1, dtype=torch.int32, device=dev)
-    slots = torch.empty(n_tokens, dtype=torch.int32, device=dev)
-    kv_lens = torch.empty(n, dtype=torch.int32, device=dev)
-    next_head = torch.empty(1, dtype=torch.int32, device=dev)
+    slots, cu, kv_lens, next_head = seqs.new_empty(n_tokens + 2 * n + 2).split((n_tokens, n + 1, n, 1))   # (one allocation)
     _lib.call("kvt_block_plan", n, seqs.data_ptr(), counts.data_ptr(), seq_lens.data_ptr(), rows, block_table.data_ptr(),
               block_table.stride(0), block_table.shape[1], free_list.data_ptr(), free_list.numel(), free_head.data_ptr(),
               block, n_tokens, cu.data_ptr(), slots.data_ptr(), kv_lens.data_ptr(), next_head.data_ptr(),
@@ -172,14 +176,32 @@ def kvt_block_store(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, kv_lens:
               k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B, st)
 
 
-def _parts(workspace: Optional[dict], need: int, D: int, device):
-    """Partial buffers of a split launch: need rows of D values and of (maximum, sum)."""
-    ws = workspace if workspace is not None else {}
-    o = ws.get("block_o")
-    if o is None or o.numel() < need * D or ws["block_ml"].numel() < need * 2 or o.device != device:
-        o = ws["block_o"] = torch.empty(need * D, dtype=torch.float32, device=device)
-        ws["block_ml"] = torch.empty(need * 2, dtype=torch.float32, device=device)
-    return o.data_ptr(), ws["block_ml"].data_ptr()
+def _grown(ws: dict, name: str, n: int, dtype, device, zero: bool = False) -> torch.Tensor:
+    """A buffer of at least n entries kept in ws.  One that is outgrown stays there too (a captured graph may use it), so
+    each is at least twice the last."""
+    t = ws.get(name)
+    if t is None or t.numel() < n or t.device != device:
+        if t is not None:
+            ws.setdefault("block_outgrown", []).append(t)
+            n = max(n, 2 * t.numel()) if t.device == device else n
+        t = ws[name] = (torch.zeros if zero else torch.empty)(n, dtype=dtype, device=device)
+    return t
+
+
+def _parts(workspace: Optional[dict], need: int, D: int, device, items: int = 0):
+    """Pointers of a split launch's partial buffers: need rows of D values and of (maximum, sum), and the counters of
+    `items` whose parts the launch itself merges.  Those have to be zero, which every call leaves them: they live in a
+    kept workspace, and not in one that a capture makes (its zeros would only be written by a replay)."""
+    if workspace is None:
+        ws, items = {}, 0
+    else:
+        ws = workspace
+    o = _grown(ws, "block_o", need * D, torch.float32, device)
+    ml = _grown(ws, "block_ml", need * 2, torch.float32, device)
+    c = ws.get("block_counters")
+    if items and (c is None or c.numel() < items or c.device != device):
+        c = None if torch.cuda.is_current_stream_capturing() else _grown(ws, "block_counters", items, torch.int32, device, True)
+    return o.data_ptr(), ml.data_ptr(), c.data_ptr() if items and c is not None else None
 
 
 def _attn_args(q, out, H, D):
@@ -226,13 +248,14 @@ def kvt_block_decode(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: to
         ns = -_DECODE_BLOCKS[D]
     else:
         ns = _splits(n * H, cap, 768 if n > 1 else _DECODE_BLOCKS[D])
-    o = ml = None
+    o = ml = counters = None
     if ns > 1 or ns < -1:
-        o, ml = _parts(workspace, n * H * ns * 16 if ns > 1 else -2 * ns * 16, D, q.device)
+        o, ml, counters = _parts(workspace, n * H * ns * 16 if ns > 1 else -2 * ns * 16, D, q.device,
+                                 n * H if 1 < ns <= _MERGE_SPLITS else 0)
     _lib.call("kvt_block_decode", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], kv_lens.data_ptr(), n,
               H, Hq, D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B,
               block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1], _lib.ptr(seqs),
-              D ** -0.5 if scale is None else float(scale), ns, o, ml, out.data_ptr(), _lib.DTYPE_CODE[out.dtype],
+              D ** -0.5 if scale is None else float(scale), ns, o, ml, counters, out.data_ptr(), _lib.DTYPE_CODE[out.dtype],
               out.stride(0), out.stride(1), st)
     return out
 
@@ -263,14 +286,15 @@ def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8:
         ns = int(splits)
     else:
         full = max(-(-total * (Hq // H) // rows), n) * H     # (items less the empty ones)
-        ns = _splits(full, block_table.shape[1] * B, *((_TILE_BLOCKS[D], _TILE_LEAST) if rows > 16 else (1024,)))
-    o = ml = None
+        ns = _splits(full, block_table.shape[1] * B, *((_TILE_BLOCKS[D], _TILE_LEAST) if rows > 16 else (_DECODE_BLOCKS[D],)))
+    o = ml = counters = None
     if ns > 1:
-        o, ml = _parts(workspace, items * H * ns * rows, D, q.device)
+        o, ml, counters = _parts(workspace, items * H * ns * rows, D, q.device,
+                                 items * H if rows == 16 and ns <= _MERGE_SPLITS else 0)
     _lib.call("kvt_block_prefill", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], cu_q.data_ptr(), total,
               kv_lens.data_ptr(), n, H, Hq, D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(),
               nb, B, block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1],
-              _lib.ptr(seqs), int(bool(causal)), D ** -0.5 if scale is None else float(scale), rows, ns, o, ml, out.data_ptr(),
+              _lib.ptr(seqs), int(bool(causal)), D ** -0.5 if scale is None else float(scale), rows, ns, o, ml, counters, out.data_ptr(),
               _lib.DTYPE_CODE[out.dtype], out.stride(0), out.stride(1), st)
     return out
 

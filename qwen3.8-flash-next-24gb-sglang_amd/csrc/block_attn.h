@@ -23,6 +23,7 @@ struct Attn {
   void* out;
   float* part_o;
   float* part_ml;
+  int32_t* counters;           // of the items whose splits the launch merges itself (NULL: a launch of its own does)
   int64_t sq_n, sq_h, so_n, so_h, stride;
   float scale_log2;
   int n, n_rows, n_q, H, gs, n_blocks, max_blocks, log2b, splits, causal;
@@ -69,6 +70,11 @@ KVT_DEV int tiles_of(const Attn& P, int limit) { return (limit + P.tile - 1) / P
 KVT_DEV int tiles_per_split(const Attn& P, int limit) {
   const int per = (tiles_of(P, limit) + P.splits - 1) / P.splits;
   return max((per + P.least - 1) / P.least, 1) * P.least;
+}
+// Splits that have tiles (one where there are none: it writes the NaN).  An item of one split is not merged.
+KVT_DEV int splits_used(const Attn& P, int limit) {
+  const int tps = tiles_per_split(P, limit);
+  return P.splits == 1 ? 1 : max((tiles_of(P, limit) + tps - 1) / tps, 1);
 }
 
 // fp32 pair -> fp16, to nearest even (one v_cvt_pk_f16_f32)

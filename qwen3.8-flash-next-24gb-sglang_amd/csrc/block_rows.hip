@@ -28,6 +28,16 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kTile = 32;
 constexpr int kMostSplits = 1024;
+constexpr int kFew = 16;               // splits that the launch itself may merge, or a merge without LDS
+
+// The parts of an item that the launch merges itself cross XCDs, whose L2s do not see each other: they are written and
+// read at device scope (cache policy sc1).
+typedef unsigned int b16v __attribute__((vector_size(16)));
+typedef unsigned int b8v __attribute__((vector_size(8)));
+constexpr int kSc1 = 16;
+KVT_DEV __amdgpu_buffer_rsrc_t part_rsrc(float* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(p, 0, bytes, 0x00020000);
+}
 
 template <int BYTES> struct Raw { uint32_t w[BYTES / 4]; };
 template <int BYTES>
@@ -55,6 +65,8 @@ template <int D>
 struct Join {
   float o[kWaves][16][D + 4];
   float m[kWaves][16], l[kWaves][16], u[kWaves];
+  float w[16][kFew];           // (weights of the splits of a row, where the launch merges them)
+  int last;
 };
 
 // Tiles tile0 .. tile1 - 1 of an item and KV head: into out where they are all that the item has (whole), else as part
@@ -242,9 +254,63 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
       store_out4(P.out, ot, o, O[0], O[1], O[2], O[3]);
     } else {
       const int64_t part = slot * 16 + row;
-      *reinterpret_cast<f4*>(P.part_o + part * D + d) = O;
-      if (d == 0) P.part_ml[2 * part] = M, P.part_ml[2 * part + 1] = L;
+      if (P.counters) {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(b16v, O), part_rsrc(P.part_o + slot * 16 * D, 64 * D),
+                                               (row * D + d) * 4, 0, kSc1);
+        if (d == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(b8v, make_float2(M, L)), part_rsrc(P.part_ml + slot * 32, 128),
+                                                row * 8, 0, kSc1);
+      } else {
+        *reinterpret_cast<f4*>(P.part_o + part * D + d) = O;
+        if (d == 0) P.part_ml[2 * part] = M, P.part_ml[2 * part + 1] = L;
+      }
     }
+  }
+}
+
+// The merge of an item's splits by the workgroup that finishes last (counters: zero before and after every call).  Parts
+// cross XCDs, whose L2s do not see each other: they are stored and loaded at device scope, and a workgroup counts itself
+// when its stores have arrived.  Nobody waits for another workgroup.
+template <int D>
+KVT_DEV void merge_last(const Attn& P, const Item& it, int h, int64_t item, int used, int ot, Join<D>& J) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();                                  // every thread's parts have arrived
+  if (threadIdx.x == 0) {
+    int32_t* c = P.counters + item;
+    J.last = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == used - 1;
+    if (J.last) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!J.last) return;
+  const auto ro = part_rsrc(P.part_o + item * P.splits * 16 * D, P.splits * 64 * D);
+  const auto rml = part_rsrc(P.part_ml + item * P.splits * 32, P.splits * 128);
+  const int row = threadIdx.x >> 4, s = threadIdx.x & 15;   // 16 rows x 16 splits
+  float m = -__builtin_inff(), l = 0.0f;
+  if (row < it.n_row && s < used) {
+    const float2 ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rml, (16 * s + row) * 8, 0, kSc1));
+    m = ml.x, l = ml.y;
+  }
+  const float M = group_max<16>(m);
+  J.w[row][s] = m == -__builtin_inff() ? 0.0f : exp2_(m - M) * l;
+  __syncthreads();
+  for (int e = threadIdx.x; e < it.n_row * (D / 4); e += 256) {
+    const int r = e / (D / 4), d = 4 * (e % (D / 4));
+    f4 O = {0, 0, 0, 0}, o[kFew];
+    float L = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kFew; ++k)
+      if (k < used) o[k] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(ro, ((16 * k + r) * D + d) * 4, 0, kSc1));
+#pragma unroll
+    for (int k = 0; k < kFew; ++k)
+      L += J.w[r][k];
+    const float per = 1.0f / L;
+#pragma unroll
+    for (int k = 0; k < kFew; ++k)                  // (the order of the merge by a second launch: the same bits)
+      if (k < used) O += (J.w[r][k] * per) * o[k];
+    if (L == 0.0f) O = f4{1, 1, 1, 1} * __builtin_nanf("");
+    const int at = it.row0 + r;
+    store_out4(P.out, ot, (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + d, O[0], O[1], O[2],
+               O[3]);
   }
 }
 
@@ -256,8 +322,11 @@ __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot
   if (it.n_row == 0) return;
   const int tps = tiles_per_split(P, it.limit);
   const int tile0 = split * tps, tile1 = min(tile0 + tps, tiles_of(P, it.limit));
-  if (tile0 >= tile1 && P.splits > 1) return;       // (the merge knows which splits there are)
-  attend<CODE, QT, D>(P, it, h, tile0, tile1, P.splits == 1, ((int64_t)w * P.H + h) * P.splits + split, ot, J);
+  const int used = splits_used(P, it.limit);
+  if (split >= used) return;                        // (the merge knows which splits there are)
+  const int64_t item = (int64_t)w * P.H + h;
+  attend<CODE, QT, D>(P, it, h, tile0, tile1, used == 1, item * P.splits + split, ot, J);
+  if (P.counters && used > 1) merge_last<D>(P, it, h, item, used, ot, J);
 }
 
 // Decode shares all tiles of a call equally: the (request, KV head) pairs stand in a line, each as long as its tiles plus
@@ -408,9 +477,8 @@ __global__ __launch_bounds__(NT) void block_merge_kernel(const Attn P, int D, in
   __shared__ f4 os[NG][16];
   const int row = blockIdx.x, dc = blockIdx.y, h = blockIdx.z % P.H, w = blockIdx.z / P.H;
   const Item it = item_of(P, w);
-  if (row >= it.n_row) return;
-  const int tps = tiles_per_split(P, it.limit);
-  const int used = (tiles_of(P, it.limit) + tps - 1) / tps;
+  const int used = splits_used(P, it.limit);
+  if (row >= it.n_row || used == 1) return;
   const int64_t part = ((int64_t)w * P.H + h) * P.splits * P.item_rows + row;
   float M = -__builtin_inff(), L = 0.0f;
   for (int s = threadIdx.x; s < used; s += NT) M = fmaxf(M, P.part_ml[2 * (part + (int64_t)P.item_rows * s)]);
@@ -448,15 +516,13 @@ __global__ __launch_bounds__(NT) void block_merge_kernel(const Attn P, int D, in
   store_out4(P.out, ot, o, O[0], O[1], O[2], O[3]);
 }
 // The same for up to kFew splits: D / 4 lanes per row, which read its parts side by side.
-constexpr int kFew = 16;
 template <int D>
 __global__ __launch_bounds__(256) void block_merge_few_kernel(const Attn P, int ot) {
   constexpr int LPR = D / 4;
   const int row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, d = 4 * (threadIdx.x % LPR), h = blockIdx.y, w = blockIdx.z;
   const Item it = item_of(P, w);
-  if (row >= it.n_row) return;
-  const int tps = tiles_per_split(P, it.limit);
-  const int used = (tiles_of(P, it.limit) + tps - 1) / tps;
+  const int used = splits_used(P, it.limit);
+  if (row >= it.n_row || used == 1) return;
   const int64_t part = ((int64_t)w * P.H + h) * P.splits * P.item_rows + row;
   float wgt[kFew], l[kFew], M = -__builtin_inff(), L = 0.0f;
 #pragma unroll
@@ -497,7 +563,7 @@ template <int CODE, int QT, int D>
 void launch(const Attn& P, int items, int ot, hipStream_t st) {
   if (!P.shares) {
     block_rows_kernel<CODE, QT, D><<<dim3(P.splits, P.H, items), 256, 0, st>>>(P, ot);
-    if (P.splits > 1) merge<D>(P, items, P.cu ? 16 : P.gs, ot, st);
+    if (P.splits > 1 && !P.counters) merge<D>(P, items, P.cu ? 16 : P.gs, ot, st);
     return;
   }
   block_decode_kernel<CODE, QT, D><<<P.shares, 256, 0, st>>>(P, ot);
@@ -541,10 +607,11 @@ extern "C" int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q
                                 int Hq, int D, int code, const void* k8, const void* v8, const void* ks, const void* vs,
                                 int n_blocks, int block, const void* block_table, int64_t bt_stride, int n_rows,
                                 int max_blocks, const void* rows, float scale, int n_splits, void* part_o,
-                                void* part_ml, void* out, int out_type, int64_t so_n, int64_t so_h, void* stream) {
+                                void* part_ml, void* counters, void* out, int out_type, int64_t so_n, int64_t so_h, void* stream) {
   Attn P;
   P.q = q, P.k8 = (const uint8_t*)k8, P.v8 = (const uint8_t*)v8, P.ks = (const float*)ks, P.vs = (const float*)vs;
   P.table = (const int32_t*)block_table, P.kv_lens = (const int32_t*)kv_lens, P.rows = (const int32_t*)rows;
+  P.counters = n_splits > 1 && n_splits <= kFew ? (int32_t*)counters : nullptr;
   P.cu = nullptr, P.out = out, P.part_o = (float*)part_o, P.part_ml = (float*)part_ml;
   P.sq_n = sq_n, P.sq_h = sq_h, P.so_n = so_n, P.so_h = so_h, P.stride = bt_stride, P.scale_log2 = scale * kLog2e;
   P.n = n, P.n_rows = n_rows, P.n_q = n, P.H = H, P.gs = H > 0 ? Hq / H : 0, P.n_blocks = n_blocks;
@@ -566,10 +633,11 @@ extern "C" int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int 
                                  const void* v8, const void* ks, const void* vs, int n_blocks, int block,
                                  const void* block_table, int64_t bt_stride, int n_rows, int max_blocks,
                                  const void* rows, int causal, float scale, int item_rows, int n_splits, void* part_o,
-                                 void* part_ml, void* out, int out_type, int64_t so_n, int64_t so_h, void* stream) {
+                                 void* part_ml, void* counters, void* out, int out_type, int64_t so_n, int64_t so_h, void* stream) {
   Attn P;
   P.q = q, P.k8 = (const uint8_t*)k8, P.v8 = (const uint8_t*)v8, P.ks = (const float*)ks, P.vs = (const float*)vs;
   P.table = (const int32_t*)block_table, P.kv_lens = (const int32_t*)kv_lens, P.rows = (const int32_t*)rows;
+  P.counters = n_splits > 1 && n_splits <= kFew && item_rows == 16 ? (int32_t*)counters : nullptr;
   P.cu = (const int32_t*)cu_q, P.out = out, P.part_o = (float*)part_o, P.part_ml = (float*)part_ml;
   P.sq_n = sq_n, P.sq_h = sq_h, P.so_n = so_n, P.so_h = so_h, P.stride = bt_stride, P.scale_log2 = scale * kLog2e;
   P.n = n, P.n_rows = n_rows, P.n_q = n_q, P.H = H, P.gs = H > 0 ? Hq / H : 0, P.n_blocks = n_blocks;

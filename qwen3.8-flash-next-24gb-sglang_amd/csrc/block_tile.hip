@@ -97,7 +97,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
   if (it.n_row == 0) return;
   const int tps = tiles_per_split(P, it.limit);
   const int tile0 = split * tps, tile1 = min(tile0 + tps, tiles_of(P, it.limit));
-  if (tile0 >= tile1 && P.splits > 1) return;
+  const int used = splits_used(P, it.limit);
+  if (split >= used) return;
 
   const int my = it.row0 + 32 * wave + l;
   const bool live = 32 * wave + l < it.n_row;
@@ -348,7 +349,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
   if (row >= it.n_row) return;
   const int qi = (it.row0 + row) / P.gs, hq = h * P.gs + (it.row0 + row) % P.gs;
   const float f = sum == 0.0f ? 0.0f : unit / sum;
-  if (P.splits == 1) {
+  if (used == 1) {
     const int64_t o = (int64_t)(it.q0 + qi) * P.so_n + (int64_t)hq * P.so_h + 4 * g;
     const float nan = sum == 0.0f ? __builtin_nanf("") : 0.0f;
 #pragma unroll

@@ -254,7 +254,7 @@ def _pool(kv, nb, H, B, D, g, spread=2):
 
 
 def _check_attn(kv, qt, Hq, H, D, B, new, kv_lens, causal=True, seed=0, decode=False, out_dtype=None, splits=None,
-                change=None, q=None, scale=None, stream=None):
+                change=None, q=None, scale=None, workspace=None):
     """change(codes, scales, table): alters the pool before both sides see it."""
     from kvtier import block_kv
     g = torch.Generator().manual_seed(seed)
@@ -272,10 +272,11 @@ def _check_attn(kv, qt, Hq, H, D, B, new, kv_lens, causal=True, seed=0, decode=F
     dc, ds, tab, kl = [c.to(dev) for c in codes], [s.to(dev) for s in sc], i32(table), i32(kv_lens)
     out = torch.full(q.shape, 5.0, dtype=out_dtype or qt, device=dev)
     if decode:
-        got = block_kv.kvt_block_decode(q.to(dev), dc[0], dc[1], ds[0], ds[1], tab, kl, scale=scale, out=out, splits=splits)
+        got = block_kv.kvt_block_decode(q.to(dev), dc[0], dc[1], ds[0], ds[1], tab, kl, scale=scale, out=out, splits=splits,
+                                        workspace=workspace)
     else:
         got = block_kv.kvt_block_prefill(q.to(dev), i32(cu), dc[0], dc[1], ds[0], ds[1], tab, kl, causal=causal,
-                                         scale=scale, out=out, splits=splits)
+                                         scale=scale, out=out, splits=splits, workspace=workspace)
     assert got is out
     ref.close(got[:cu[-1]], *want, D)
     assert bool((got[cu[-1]:] == 5.0).all()), "rows behind the last request"
@@ -611,3 +612,19 @@ def test_slots_serve_the_slot_pools(kvt_pkg):
     for got, want in ((ok, x[0]), (ov, x[1])):
         top = want.float().view(200, H, 4, 64).abs().amax(-1, keepdim=True).expand(-1, -1, -1, 64).reshape(200, H, D)
         assert bool(((got.float() - want.float()).abs() <= top * (0.5 / 127 + 2.0 ** -8 + 2.0 ** -10)).all())
+
+
+@pytest.mark.parametrize("kv", ["fp8", "int8"])
+@pytest.mark.parametrize("Hq,H,D,B,splits", [(1, 1, 64, 16, 2), (8, 2, 128, 32, 8), (32, 8, 128, 64, None), (32, 2, 256, 16, 16),
+                                             (10, 2, 256, 64, None), (4, 4, 64, 64, 5)])
+def test_merge_in_the_launch(kvt_pkg, kv, Hq, H, D, B, splits):
+    """A kept workspace, over which few splits are merged inside the launch, used by decode steps and chunks of several sizes:
+    64 bits, and the bits of a call without one; the counters are zero after every call."""
+    ws = {}
+    for lens, new in (([700], [3]), (LENS, [min(n, 4) for n in LENS]), ([2000, 0, 1, 900], [1, 0, 1, 2]), (LENS[3:5], [5, 1])):
+        for decode in (True, False):
+            got = [_check_attn(kv, torch.bfloat16, Hq, H, D, B, [1] * len(lens) if decode else new, lens, decode=decode, seed=19,
+                               splits=splits, workspace=w, out_dtype=torch.float32) for w in (ws, ws, None)]
+            for other in got[1:]:
+                assert torch.equal(got[0].view(torch.int32), other.view(torch.int32))
+            assert not ws["block_counters"].any()

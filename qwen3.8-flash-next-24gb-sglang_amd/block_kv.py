@@ -211,7 +211,7 @@ def _attn_args(q, out, H, D):
     if Hq % H or Hq // H > 16 or Hq == 0:
         raise ValueError(f"{Hq} q heads over {H} KV heads: a multiple, at most 16 each, is served")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     assert out.shape == q.shape and out.dtype in _lib.DTYPE_CODE and out.stride(2) == 1
     return _rows16(q, 8), out, Hq
 

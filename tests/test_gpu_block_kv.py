@@ -170,6 +170,19 @@ def test_store_many_requests(kvt_pkg, kv):
     _check_store(kv, torch.bfloat16, 1, 64, 16, old, new, seed=9)
 
 
+@pytest.mark.parametrize("kv,dt", [("fp8", torch.bfloat16), ("int8", torch.float16), ("fp8", torch.float32), ("int8", torch.bfloat16)])
+@pytest.mark.parametrize("H,D,B", [(2, 256, 64), (5, 128, 16), (3, 64, 32)])
+def test_store_few_rows_on_average(kvt_pkg, kv, dt, H, D, B):
+    """Decode steps among which one request writes a prompt over several blocks, with values that are not finite."""
+    old, new = [5, 0, 63, 64, 100, 17, 1, 31] * 12, [1, 0, 2, 1, 1, 1, 3, 1] * 12
+    new[20] = 150
+    x = torch.randn(2, sum(new), H, D, generator=torch.Generator().manual_seed(B)).to(dt)
+    first = sum(new[:20])
+    x[0, first + 3, 1, 5], x[1, first + 70, 0, 0], x[0, first + 149, H - 1, D - 1] = float("inf"), float("nan"), -float("inf")
+    x[0, 0, 0, 0], x[1, -1, -1, -1] = float("nan"), float("inf")
+    _check_store(kv, dt, H, D, B, old, new, seed=21, x=x)
+
+
 @pytest.mark.parametrize("kv", ["fp8", "int8"])
 def test_store_special_values(kvt_pkg, kv):
     """Infinities, NaN, zeros, the largest and the smallest values, ties: each in rows of its own block."""

@@ -44,8 +44,10 @@ _DECODE_BLOCKS = {64: 512, 128: 512, 256: 256}
 # second launch's many workgroups read the parts faster than the last one does.
 _MERGE_SPLITS = 16
 _TILE_ROWS = 128         # (query, q head) rows of a workgroup of the query-tile kernel
-# Workgroups of a split launch of it, us per call (merge included): D 256, 16 items x 30,000 positions 256 workgroups 150, 512
-# 110; D 128, 6 x 60,000 258 59.7, 384 57.9, 510 63.5; D 64, 20 x 30,000 320 86, 480 77, 640 65.
+# Workgroups of a split launch of it for one request, us per call (merge included): D 256, 16 items x 30,000 positions 256
+# workgroups 150, 512 110; D 128, 6 x 60,000 258 59.7, 384 57.9, 510 63.5; D 64, 20 x 30,000 320 86, 480 77, 640 65.  Half as
+# many again for several, whose lengths differ: 4 x 8 heads (D 128), 64 queries, up to 6,000 positions 75 / 58, 8 x 20 heads (D
+# 64) up to 1,500 52.5 / 45.5, 8 x 2 (D 256) up to 4,000 124 / 110, 8 x 8 (D 128) up to 3,000 53 / 55.
 _TILE_BLOCKS = {64: 768, 128: 384, 256: 512}
 _TILE_LEAST = 512        # positions of a split at least: its part of 128 rows is 512 D bytes written and read again
 # Rows per request and KV head (on average) from which it serves a call.  us per call against the 16-row kernel's, one request
@@ -286,7 +288,11 @@ def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8:
         ns = int(splits)
     else:
         full = max(-(-total * (Hq // H) // rows), n) * H     # (items less the empty ones)
-        ns = _splits(full, block_table.shape[1] * B, *((_TILE_BLOCKS[D], _TILE_LEAST) if rows > 16 else (_DECODE_BLOCKS[D],)))
+        cap = block_table.shape[1] * B
+        if rows > 16:
+            ns = _splits(full, cap, _TILE_BLOCKS[D] * (3 if n > 1 else 2) // 2, _TILE_LEAST)
+        else:
+            ns = _splits(full, cap, _DECODE_BLOCKS[D])
     o = ml = counters = None
     if ns > 1:
         o, ml, counters = _parts(workspace, items * H * ns * rows, D, q.device,

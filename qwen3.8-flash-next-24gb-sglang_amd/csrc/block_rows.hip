@@ -643,7 +643,10 @@ extern "C" int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int 
   P.n = n, P.n_rows = n_rows, P.n_q = n_q, P.H = H, P.gs = H > 0 ? Hq / H : 0, P.n_blocks = n_blocks;
   P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.splits = n_splits, P.causal = causal, P.shares = 0;
   const bool tiled = item_rows == kTileRows;
-  P.item_rows = item_rows, P.tile = tiled ? tile_positions(D) : kTile, P.least = tiled ? 1 : kWaves;
+  P.item_rows = item_rows, P.tile = tiled ? tile_positions(D) : kTile;
+  // (requests of several lengths: splits of a multiple of 512 positions, so that the long ones' are not much longer than the
+  // others', and a short one is not split: 8 x 20 heads (D 64), 448 ragged queries over 1,500 ragged positions 52.5 -> 45.5 us)
+  P.least = !tiled ? kWaves : n > 1 ? 512 / P.tile : 1;
   const int st = check(P, Hq, D, block, code, q_type, out_type);
   if (st != KVT_OK) return st;
   if (!cu_q || n_q < 0 || (item_rows != 16 && !tiled) || (n_splits > 1 && (!part_o || !part_ml))) return KVT_EINVAL;

@@ -41,7 +41,7 @@ _DECODE_BLOCKS = {64: 512, 128: 512, 256: 256}
 # Splits of a pair that a launch with a kept workspace merges itself.  us per call, merged by a second launch / by itself: 8
 # requests x 2 heads (D 256, up to 2,000 positions, 16 splits) 15.8 / 13.8; one x 8 (D 128, 2,000, 16 splits) 12.8 / 9.5; 8 x 8
 # (D 128, up to 4,000, 12 splits) 19.0 / 15.7; chunks of four queries over the same (8 splits) 22.1 / 19.9.  Past 16 the
-# second launch's many workgroups read the parts faster than the last one does.
+# second launch's many workgroups read the parts faster than the last one does.  (Equal shares: the entry point decides.)
 _MERGE_SPLITS = 16
 _TILE_ROWS = 128         # (query, q head) rows of a workgroup of the query-tile kernel
 # Workgroups of a split launch of it for one request, us per call (merge included): D 256, 16 items x 30,000 positions 256
@@ -253,7 +253,7 @@ def kvt_block_decode(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: to
     o = ml = counters = None
     if ns > 1 or ns < -1:
         o, ml, counters = _parts(workspace, n * H * ns * 16 if ns > 1 else -2 * ns * 16, D, q.device,
-                                 n * H if 1 < ns <= _MERGE_SPLITS else 0)
+                                 n * H if ns <= _MERGE_SPLITS else 0)
     _lib.call("kvt_block_decode", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], kv_lens.data_ptr(), n,
               H, Hq, D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B,
               block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1], _lib.ptr(seqs),

@@ -28,6 +28,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kTile = 32;
 constexpr int kMostSplits = 1024;
+constexpr int kMostParts = 128;        // parts of a pair, at most, where the launch of equal shares merges them
 constexpr int kFew = 16;               // splits that the launch itself may merge, or a merge without LDS
 
 // The parts of an item that the launch merges itself cross XCDs, whose L2s do not see each other: they are written and
@@ -38,6 +39,10 @@ constexpr int kSc1 = 16;
 KVT_DEV __amdgpu_buffer_rsrc_t part_rsrc(float* p, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(p, 0, bytes, 0x00020000);
 }
+
+// A part's weight in the merge of normalized parts, from its maximum and sum and the row's maximum.  Sums are below 2^45: times
+// 2^-45 no product with a part is larger than the part, and their sums stay finite.
+KVT_DEV float weight_of(float m, float l, float M) { return m == -__builtin_inff() ? 0.0f : exp2_(m - M) * l * 0x1p-45f; }
 
 template <int BYTES> struct Raw { uint32_t w[BYTES / 4]; };
 template <int BYTES>
@@ -268,49 +273,72 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
   }
 }
 
-// The merge of an item's splits by the workgroup that finishes last (counters: zero before and after every call).  Parts
-// cross XCDs, whose L2s do not see each other: they are stored and loaded at device scope, and a workgroup counts itself
-// when its stores have arrived.  Nobody waits for another workgroup.
+// The merge of an item's parts by the workgroup that finishes last (counters: zero before and after every call): part 0 is in
+// slot s0, part k > 0 in slot sb + step k.  Parts cross XCDs, whose L2s do not see each other: they are stored and loaded at
+// device scope, and a workgroup counts itself when its stores have arrived.  Nobody waits for another workgroup.  The
+// parts are added in their order whoever merges them, as the merge by a second launch does: the same bits.
 template <int D>
-KVT_DEV void merge_last(const Attn& P, const Item& it, int h, int64_t item, int used, int ot, Join<D>& J) {
+KVT_DEV void merge_last(const Attn& P, const Item& it, int h, int64_t item, int parts, int64_t s0, int64_t sb, int step, int ot,
+                        Join<D>& J) {
+  constexpr int NE = D / 64;                        // four channels each: 16 rows over 256 threads
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();                                  // every thread's parts have arrived
   if (threadIdx.x == 0) {
     int32_t* c = P.counters + item;
-    J.last = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == used - 1;
+    J.last = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
     if (J.last) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   if (!J.last) return;
-  const auto ro = part_rsrc(P.part_o + item * P.splits * 16 * D, P.splits * 64 * D);
-  const auto rml = part_rsrc(P.part_ml + item * P.splits * 32, P.splits * 128);
-  const int row = threadIdx.x >> 4, s = threadIdx.x & 15;   // 16 rows x 16 splits
-  float m = -__builtin_inff(), l = 0.0f;
-  if (row < it.n_row && s < used) {
-    const float2 ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rml, (16 * s + row) * 8, 0, kSc1));
-    m = ml.x, l = ml.y;
+  const auto ro = part_rsrc(P.part_o + s0 * 16 * D, (step * parts + 1) * 64 * D);
+  const auto rml = part_rsrc(P.part_ml + s0 * 32, (step * parts + 1) * 128);
+  const int base = (int)(sb - s0);                  // (slots from here on count from s0)
+  const auto slot = [&](int k) { return k ? base + step * k : 0; };
+  const int row = threadIdx.x >> 4, lane = threadIdx.x & 15;   // 16 rows x 16 parts at a time
+  const auto read_ml = [&](int k) {
+    return row < it.n_row && k < parts
+               ? __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rml, (16 * slot(k) + row) * 8, 0, kSc1))
+               : make_float2(-__builtin_inff(), 0.0f);
+  };
+  const float2 first = read_ml(lane);
+  float M = first.x;
+  for (int k = lane + kFew; k < parts; k += kFew) M = fmaxf(M, read_ml(k).x);
+  M = group_max<16>(M);
+  f4 O[NE];
+  float L[NE];
+#pragma unroll
+  for (int n = 0; n < NE; ++n) O[n] = f4{0, 0, 0, 0}, L[n] = 0.0f;
+  for (int k0 = 0; k0 < parts; k0 += kFew) {
+    const float2 ml = k0 ? read_ml(k0 + lane) : first;
+    J.w[row][lane] = weight_of(ml.x, ml.y, M);
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NE; ++n) {
+      const int e = threadIdx.x + 256 * n, r = e / (D / 4), d = 4 * (e % (D / 4));
+      if (r >= it.n_row) continue;
+      f4 o[kFew];
+#pragma unroll
+      for (int k = 0; k < kFew; ++k)
+        if (k0 + k < parts)
+          o[k] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(ro, ((16 * slot(k0 + k) + r) * D + d) * 4, 0, kSc1));
+#pragma unroll
+      for (int k = 0; k < kFew; ++k)
+        if (k0 + k < parts) {
+          const float f = J.w[r][k];
+          L[n] += f;
+          O[n] += f * o[k];
+        }
+    }
+    __syncthreads();
   }
-  const float M = group_max<16>(m);
-  J.w[row][s] = m == -__builtin_inff() ? 0.0f : exp2_(m - M) * l;
-  __syncthreads();
-  for (int e = threadIdx.x; e < it.n_row * (D / 4); e += 256) {
-    const int r = e / (D / 4), d = 4 * (e % (D / 4));
-    f4 O = {0, 0, 0, 0}, o[kFew];
-    float L = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kFew; ++k)
-      if (k < used) o[k] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(ro, ((16 * k + r) * D + d) * 4, 0, kSc1));
-#pragma unroll
-    for (int k = 0; k < kFew; ++k)
-      L += J.w[r][k];
-    const float per = 1.0f / L;
-#pragma unroll
-    for (int k = 0; k < kFew; ++k)                  // (the order of the merge by a second launch: the same bits)
-      if (k < used) O += (J.w[r][k] * per) * o[k];
-    if (L == 0.0f) O = f4{1, 1, 1, 1} * __builtin_nanf("");
+  for (int n = 0; n < NE; ++n) {
+    const int e = threadIdx.x + 256 * n, r = e / (D / 4), d = 4 * (e % (D / 4));
+    if (r >= it.n_row) continue;
+    const f4 y = L[n] == 0.0f ? f4{1, 1, 1, 1} * __builtin_nanf("") : O[n] / L[n];
     const int at = it.row0 + r;
-    store_out4(P.out, ot, (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + d, O[0], O[1], O[2],
-               O[3]);
+    store_out4(P.out, ot, (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + d, y[0], y[1], y[2],
+               y[3]);
   }
 }
 
@@ -326,7 +354,7 @@ __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot
   if (split >= used) return;                        // (the merge knows which splits there are)
   const int64_t item = (int64_t)w * P.H + h;
   attend<CODE, QT, D>(P, it, h, tile0, tile1, used == 1, item * P.splits + split, ot, J);
-  if (P.counters && used > 1) merge_last<D>(P, it, h, item, used, ot, J);
+  if (P.counters && used > 1) merge_last<D>(P, it, h, item, used, item * P.splits, item * P.splits, 1, ot, J);
 }
 
 // Decode shares all tiles of a call equally: the (request, KV head) pairs stand in a line, each as long as its tiles plus
@@ -427,7 +455,13 @@ __global__ __launch_bounds__(256, 2) void block_decode_kernel(const Attn P, int 
       const int t0 = a < x0 ? (int)min((uint64_t)(x0 - a) << P.shift, (uint64_t)tiles) : 0;
       const int t1 = (int)min((uint64_t)(x1 - a) << P.shift, (uint64_t)tiles);
       if (t0 < t1 || (tiles == 0 && a >= x0)) {
-        attend<CODE, QT, D>(P, it, h, t0, t1, t0 == 0 && t1 == tiles, 2 * (int64_t)w + (a > x0), ot, J);
+        const bool whole = t0 == 0 && t1 == tiles;
+        attend<CODE, QT, D>(P, it, h, t0, t1, whole, 2 * (int64_t)w + (a > x0), ot, J);
+        if (D < 256 && P.counters && !whole) {// (at D 256 the merge's registers would spill)
+          const int w0 = (int)(a / share), w1 = (int)((a + (uint32_t)((tiles - 1) >> P.shift)) / share);
+          merge_last<D>(P, it, h, (int64_t)r * P.H + h, w1 - w0 + 1, 2 * (int64_t)w0 + (a > (uint32_t)w0 * share), 2 * (int64_t)w0, 2,
+                        ot, J);
+        }
         __syncthreads();                            // (J is free again)
       }
     }
@@ -454,13 +488,12 @@ __global__ __launch_bounds__(256) void block_decode_merge_kernel(const Attn P, i
   float M = -__builtin_inff(), L = 0.0f;
 #pragma unroll 8
   for (int w = w0; w <= w1; ++w) M = fmaxf(M, P.part_ml[2 * part_of(w)]);
-  // (weights are scaled by 2^-45 (l is below 2^45): their sums times the largest values stay finite)
   f4 O = {0, 0, 0, 0};
 #pragma unroll 8
   for (int w = w0; w <= w1; ++w) {
     const int64_t p = part_of(w);
     const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * p);
-    const float f = ml.x == -__builtin_inff() ? 0.0f : exp2_(ml.x - M) * ml.y * 0x1p-45f;
+    const float f = weight_of(ml.x, ml.y, M);
     L += f;
     O += f * *reinterpret_cast<const f4*>(P.part_o + p * D + d);
   }
@@ -535,17 +568,16 @@ __global__ __launch_bounds__(256) void block_merge_few_kernel(const Attn P, int 
   for (int s = 0; s < kFew; ++s) M = fmaxf(M, wgt[s]);
 #pragma unroll
   for (int s = 0; s < kFew; ++s) {
-    wgt[s] = wgt[s] == -__builtin_inff() ? 0.0f : exp2_(wgt[s] - M) * l[s];
+    wgt[s] = weight_of(wgt[s], l[s], M);
     L += wgt[s];
   }
-  const float per = 1.0f / L;                                       // (no product is larger than the values themselves)
   f4 O = {0, 0, 0, 0};
 #pragma unroll
   for (int s = 0; s < kFew; ++s)
-    if (s < used) O += (wgt[s] * per) * *reinterpret_cast<const f4*>(P.part_o + (part + (int64_t)P.item_rows * s) * D + d);
+    if (s < used) O += wgt[s] * *reinterpret_cast<const f4*>(P.part_o + (part + (int64_t)P.item_rows * s) * D + d);
   const int at = it.row0 + row;
   const int64_t o = (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + d;
-  if (L == 0.0f) O = f4{1, 1, 1, 1} * __builtin_nanf("");
+  O = L == 0.0f ? f4{1, 1, 1, 1} * __builtin_nanf("") : O / L;
   store_out4(P.out, ot, o, O[0], O[1], O[2], O[3]);
 }
 template <int D>
@@ -567,7 +599,7 @@ void launch(const Attn& P, int items, int ot, hipStream_t st) {
     return;
   }
   block_decode_kernel<CODE, QT, D><<<P.shares, 256, 0, st>>>(P, ot);
-  if (P.shares > 1) block_decode_merge_kernel<D><<<dim3((P.gs * (D / 4) + 255) / 256, P.H, P.n), 256, 0, st>>>(P, ot);
+  if (P.shares > 1 && !P.counters) block_decode_merge_kernel<D><<<dim3((P.gs * (D / 4) + 255) / 256, P.H, P.n), 256, 0, st>>>(P, ot);
 }
 template <int CODE, int QT>
 void launch_d(const Attn& P, int D, int items, int ot, hipStream_t st) {
@@ -611,7 +643,12 @@ extern "C" int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q
   Attn P;
   P.q = q, P.k8 = (const uint8_t*)k8, P.v8 = (const uint8_t*)v8, P.ks = (const float*)ks, P.vs = (const float*)vs;
   P.table = (const int32_t*)block_table, P.kv_lens = (const int32_t*)kv_lens, P.rows = (const int32_t*)rows;
-  P.counters = n_splits > 1 && n_splits <= kFew ? (int32_t*)counters : nullptr;
+  // One workgroup merges a pair's parts inside the launch: up to kFew splits, or kMostParts parts, which is about the most that a
+  // pair can have of equal shares (one long request among short ones).  us per call, by a second launch / inside: 64 requests x 8
+  // heads (D 128), up to 8,191 positions 110 / 106, 32 x 8 up to 3,000 29.5 / 27.6, 32 x 4 up to 16,000 52.3 / 46.2; of one of them
+  // alone among short ones 20.0 / 16.3, 15.5 / 11.8, 21.3 / 23.2; 32 x 1 (16 q heads, 512 parts) 29.3 / 43.5.
+  const bool few = n_splits > 1 ? n_splits <= kFew : n_splits < -1 && D < 256 && -n_splits / (H > 0 ? H : 1) <= kMostParts;
+  P.counters = few ? (int32_t*)counters : nullptr;
   P.cu = nullptr, P.out = out, P.part_o = (float*)part_o, P.part_ml = (float*)part_ml;
   P.sq_n = sq_n, P.sq_h = sq_h, P.so_n = so_n, P.so_h = so_h, P.stride = bt_stride, P.scale_log2 = scale * kLog2e;
   P.n = n, P.n_rows = n_rows, P.n_q = n, P.H = H, P.gs = H > 0 ? Hq / H : 0, P.n_blocks = n_blocks;

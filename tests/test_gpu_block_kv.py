@@ -641,3 +641,17 @@ def test_merge_in_the_launch(kvt_pkg, kv, Hq, H, D, B, splits):
             for other in got[1:]:
                 assert torch.equal(got[0].view(torch.int32), other.view(torch.int32))
             assert not ws["block_counters"].any()
+
+
+@pytest.mark.parametrize("kv", ["fp8", "int8"])
+@pytest.mark.parametrize("Hq,H,D,B,shares", [(4, 4, 64, 16, 7), (8, 1, 128, 64, 40), (32, 2, 128, 16, 33), (6, 2, 64, 32, 512),
+                                             (16, 1, 64, 16, 128), (12, 2, 256, 64, 24)])
+def test_merge_of_shares_in_the_launch(kvt_pkg, kv, Hq, H, D, B, shares):
+    """The same over equal shares: pairs of two parts and of more than a wavefront's worth, several pairs of a workgroup, none."""
+    ws = {}
+    for lens in ([5000, 0, 3, 17], LENS * 2, [900, 1000, 1], [0, 0]):
+        got = [_check_attn(kv, torch.bfloat16, Hq, H, D, B, [1] * len(lens), lens, decode=True, seed=20, splits=-shares, workspace=w,
+                           out_dtype=torch.float32) for w in (ws, ws, None)]
+        for other in got[1:]:
+            assert torch.equal(got[0].view(torch.int32), other.view(torch.int32))
+        assert not ws["block_counters"].any()

@@ -341,23 +341,29 @@ int kvt_block_store(const void* k, const void* v, int dtype, int64_t sk_n, int64
                     const void* block_table, int64_t bt_stride, int n_rows, int max_blocks, int code, void* k8, void* v8,
                     void* ks, void* vs, int n_blocks, int block, void* stream);
 
-/* Decode attention of one query token per request: out[j, h] = softmax(scale q K^T) V over positions < kv_lens[j].  q
- * (q_type 0 bf16, 1 fp16; 16-byte aligned, strides multiples of 8) and out (out_type 0 bf16, 1 fp16, 2 fp32) are [n, Hq, D]
- * with element strides of token and head.  Hq / H <= 16, n <= 4,096.  n_splits > 1: the positions of a request are shared
- * by up to n_splits workgroups, merged by a second launch (at most 1,024; n * H <= 65,535 then); part_o fp32 [n * H * n_splits * 16 * D] and part_ml fp32 [n *
- * H * n_splits * 32] hold their parts.  A request without positions gives NaN (0/0). */
+/* Decode attention of one query token per request: out[j, h] = softmax(scale q K^T) V over positions < kv_lens[j], scale
+ * > 0.  q (q_type 0 bf16, 1 fp16) and out (out_type 0 bf16, 1 fp16, 2 fp32) are [n, Hq, D] with element strides of token and
+ * head and unit last stride, rows 16-byte aligned.  Hq / H <= 16, n <= 4,096.  ks, vs >= 0, of any values (a NaN scale makes
+ * its positions' scores or values NaN).  A request without positions gives NaN (0/0).
+ * n_splits 1: a workgroup per request and KV head.  n_splits > 1 (at most 1,024; n * H <= 65,535 then): up to n_splits
+ * workgroups for each; parts as fp32 in part_o [n * H * n_splits * 16 * D] and part_ml [n * H * n_splits * 32].  n_splits < -1
+ * (at least -65,535): |n_splits| workgroups share all positions of the call equally; part_o [|n_splits| * 32 * D], part_ml
+ * [|n_splits| * 64].  Parts are merged by a second launch, or with counters (int32 [n * H], zero before the first call;
+ * every call leaves them zero; NULL: none) inside the first one where it has few of them: the same bits either way.  Calls
+ * that share part_o, part_ml or counters must not overlap. */
 int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q_type, const void* kv_lens, int n, int H, int Hq,
                      int D, int code, const void* k8, const void* v8, const void* ks, const void* vs, int n_blocks,
                      int block, const void* block_table, int64_t bt_stride, int n_rows, int max_blocks, const void* rows,
                      float scale, int n_splits, void* part_o, void* part_ml, void* counters, void* out, int out_type,
                      int64_t so_n, int64_t so_h, void* stream);
 
-/* Attention of chunks of queries: request j owns rows cu_q[j] .. cu_q[j+1] (int32 [n + 1], at most n_q) of q / out.  causal: its
- * queries are the last positions of kv_lens[j] and see the positions up to their own; else every query sees all kv_lens[j]
- * positions (cross attention).  Rows of q / out behind cu_q[n] are left as they are.  item_rows = 128: query tiles of 128
- * (query, q head) rows per workgroup; 16: the decode kernel, for requests of few rows (at most 65,535 items).  Otherwise as
- * kvt_block_decode, with n_splits <= 1,024 and the parts per item: items = n_q * (Hq / H) / item_rows + n in the place of
- * n, item_rows rows in the place of 16; n_splits > 1 takes at most 65,535 / H items. */
+/* Attention of chunks of queries: request j owns rows cu_q[j] .. cu_q[j+1] (int32 [n + 1], at most n_q) of q / out.
+ * causal: its queries are the last positions of kv_lens[j] and see the positions up to their own; else every query sees all
+ * kv_lens[j] positions (cross attention).  A query that sees nothing gives NaN.  Rows of q / out behind cu_q[n] are left as
+ * they are.  item_rows = 128: query tiles of 128 (query, q head) rows per workgroup (at most 2^24 - 1 workgroups); 16: the
+ * decode kernel, for requests of few rows (at most 65,535 items).  items = n_q * (Hq / H) / item_rows + n.  n_splits > 1 (at
+ * most 1,024; items * H <= 65,535 then): part_o fp32 [items * H * n_splits * item_rows * D], part_ml [items * H * n_splits *
+ * item_rows * 2]; counters (int32 [items * H]) are used at item_rows = 16.  Otherwise as kvt_block_decode. */
 int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int q_type, const void* cu_q, int n_q,
                       const void* kv_lens, int n, int H, int Hq, int D, int code, const void* k8, const void* v8,
                       const void* ks, const void* vs, int n_blocks, int block, const void* block_table,

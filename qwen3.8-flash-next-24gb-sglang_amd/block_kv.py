@@ -178,19 +178,20 @@ def kvt_block_store(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, kv_lens:
               k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B, st)
 
 
-def _grown(ws: dict, name: str, n: int, dtype, device, zero: bool = False) -> torch.Tensor:
-    """A buffer of at least n entries kept in ws.  One that is outgrown stays there too (a captured graph may use it), so
-    each is at least twice the last."""
-    t = ws.get(name)
-    if t is None or t.numel() < n or t.device != device:
+def _grown(ws: dict, name: str, n: int, like: torch.Tensor, dtype=torch.float32, zero: bool = False) -> torch.Tensor:
+    """A buffer of at least n entries on the device of `like`, kept in ws.  One that is outgrown stays there too (a captured
+    graph may use it), so each is at least twice the last."""
+    key = name, like.get_device()
+    t = ws.get(key)
+    if t is None or t.numel() < n:
         if t is not None:
             ws.setdefault("block_outgrown", []).append(t)
-            n = max(n, 2 * t.numel()) if t.device == device else n
-        t = ws[name] = (torch.zeros if zero else torch.empty)(n, dtype=dtype, device=device)
+            n = max(n, 2 * t.numel())
+        t = ws[key] = (torch.zeros if zero else torch.empty)(n, dtype=dtype, device=like.device)
     return t
 
 
-def _parts(workspace: Optional[dict], need: int, D: int, device, items: int = 0):
+def _parts(workspace: Optional[dict], need: int, D: int, q: torch.Tensor, items: int = 0):
     """Pointers of a split launch's partial buffers: need rows of D values and of (maximum, sum), and the counters of
     `items` whose parts the launch itself merges.  Those have to be zero, which every call leaves them: they live in a
     kept workspace, and not in one that a capture makes (its zeros would only be written by a replay)."""
@@ -198,12 +199,15 @@ def _parts(workspace: Optional[dict], need: int, D: int, device, items: int = 0)
         ws, items = {}, 0
     else:
         ws = workspace
-    o = _grown(ws, "block_o", need * D, torch.float32, device)
-    ml = _grown(ws, "block_ml", need * 2, torch.float32, device)
-    c = ws.get("block_counters")
-    if items and (c is None or c.numel() < items or c.device != device):
-        c = None if torch.cuda.is_current_stream_capturing() else _grown(ws, "block_counters", items, torch.int32, device, True)
-    return o.data_ptr(), ml.data_ptr(), c.data_ptr() if items and c is not None else None
+    o, ml = _grown(ws, "block_o", need * D, q), _grown(ws, "block_ml", need * 2, q)
+    if items == 0:
+        return o.data_ptr(), ml.data_ptr(), None
+    c = ws.get(("block_counters", q.get_device()))
+    if c is None or c.numel() < items:
+        if torch.cuda.is_current_stream_capturing():
+            return o.data_ptr(), ml.data_ptr(), None
+        c = _grown(ws, "block_counters", items, q, torch.int32, True)
+    return o.data_ptr(), ml.data_ptr(), c.data_ptr()
 
 
 def _attn_args(q, out, H, D):
@@ -231,9 +235,11 @@ def kvt_block_decode(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: to
     """Decode attention of one query token per request: q [n, Hq, D] (bf16 / fp16), request j over its kv_lens[j] positions.
 
     Returns out ([n, Hq, D], q's dtype unless a bf16 / fp16 / fp32 `out` is given); a request without positions gives
-    NaN (0/0).  scale: default D ** -0.5.  The lengths are read on the device; `splits` (workgroups that share a request's
-    positions) follows from the number of requests and the block table's width unless given.  `workspace` (a dict) keeps
-    the partial buffers across calls; calls that share one must not overlap."""
+    NaN (0/0).  scale: > 0, default D ** -0.5.  The lengths are read on the device; `splits` follows from the number of
+    requests and the block table's width unless given: workgroups that share the positions of a request and KV head, or
+    minus the number of workgroups that share those of the whole call.  `workspace` (a dict) keeps the partial buffers across
+    calls, and spares a launch where there are few parts: calls that share one must not overlap, a captured graph needs it
+    as long as it is replayed, and one made before the capture is the faster one.  The results do not depend on it."""
     n = kv_lens.numel()
     nb, H, B, D = _pool(k8, v8, ks, vs, block_table, n, seqs)
     q, out, Hq = _attn_args(q, out, H, D)
@@ -252,7 +258,7 @@ def kvt_block_decode(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: to
         ns = _splits(n * H, cap, 768 if n > 1 else _DECODE_BLOCKS[D])
     o = ml = counters = None
     if ns > 1 or ns < -1:
-        o, ml, counters = _parts(workspace, n * H * ns * 16 if ns > 1 else -2 * ns * 16, D, q.device,
+        o, ml, counters = _parts(workspace, n * H * ns * 16 if ns > 1 else -2 * ns * 16, D, q,
                                  n * H if ns <= _MERGE_SPLITS else 0)
     _lib.call("kvt_block_decode", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], kv_lens.data_ptr(), n,
               H, Hq, D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B,
@@ -282,7 +288,7 @@ def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8:
     if n == 0 or total == 0:
         return out
     st = _stream(q, cu_q, k8, v8, ks, vs, block_table, kv_lens, seqs, out)
-    rows = _TILE_ROWS if total * (Hq // H) >= _TILE_MIN[D] * n else 16
+    rows = _TILE_ROWS if total * (Hq // H) >= _TILE_MIN[D] * n or total * (Hq // H) // 16 + n > 65535 else 16
     items = total * (Hq // H) // rows + n
     if splits is not None:
         ns = int(splits)
@@ -295,7 +301,7 @@ def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8:
             ns = _splits(full, cap, _DECODE_BLOCKS[D])
     o = ml = counters = None
     if ns > 1:
-        o, ml, counters = _parts(workspace, items * H * ns * rows, D, q.device,
+        o, ml, counters = _parts(workspace, items * H * ns * rows, D, q,
                                  items * H if rows == 16 and ns <= _MERGE_SPLITS else 0)
     _lib.call("kvt_block_prefill", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], cu_q.data_ptr(), total,
               kv_lens.data_ptr(), n, H, Hq, D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(),

@@ -14,10 +14,17 @@
 //     lane loads D / 16 channels of each of them and pairs the bytes of two positions (v_perm_b32) before the conversion.
 // Codes are exact in fp16.  The scale of K multiplies the fp32 scores.  The scale of V is folded into P, relative to a
 // running unit u: P holds w sv / u and O is kept in units of u, which changes only when a tile's scale leaves [u / 4, u]
-// (O is then multiplied by the ratio; two blocks of one tile whose scales differ by more than 4 take a product each).  The softmax keeps a running maximum m per row that moves only when a tile
-// exceeds it by more than 4 (in powers of two), and P = 2^(x - m + 10): fp16 has weights down to 2^-24 of the largest before
-// they lose bits, and up to 2^14 for a row whose maximum lags.  Sums, scores and O are fp32.  bf16 queries are scaled by
-// a power of two per row to fit fp16 (exact down to 2^-14 of the row's largest entry, and to 2^-25 of it below).
+// (O is then multiplied by the ratio; two blocks of one tile whose scales differ by more than 4 take a product each).  The
+// softmax keeps a running maximum m per row that moves only when a tile exceeds it by more than 4 (in powers of two), and
+// P = 2^(x - m + 10): fp16 has weights down to 2^-24 of the largest before they lose bits, and up to 2^14 for a row whose
+// maximum lags.  Sums, scores and O are fp32.  bf16 queries are scaled by a power of two per row to fit fp16 (exact down
+// to 2^-14 of the row's largest entry, and to 2^-25 of it below).
+//
+// Decode is bound by the cache's bytes, each read once (counted: 269 MB for 262,144 positions of 2 heads, D 256): 45.3 us
+// there, 5.9 TB/s (a large copy 5.2), where more than half of the wavefronts' time is waiting for memory and the vector
+// instructions take 30 %, the matrix instructions 9 % of theirs; e4m3, 32 requests of 12,000 positions and less (204 MB)
+// 38.4 us, 5.3 TB/s; int8, 64 requests x 8 heads, D 128 (456 MB) 94 us, 4.9 TB/s.  Short calls are launch and load latency:
+// 777 positions of 2 heads 12 us with the merge in the launch.
 #include "block_attn.h"
 
 using namespace kvt;
@@ -357,12 +364,12 @@ __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot
   if (P.counters && used > 1) merge_last<D>(P, it, h, item, used, item * P.splits, item * P.splits, 1, ot, J);
 }
 
-// Decode shares all tiles of a call equally: the (request, KV head) pairs stand in a line, each as long as its tiles plus
-// kPad (what beginning with a pair costs, about), and workgroup w takes [w share, (w + 1) share) of it.  A pair that one
-// workgroup has is written at once; of a pair that several have, each leaves a part, and a second launch merges them.  A
-// workgroup has at most two such pairs, its first (slot 2 w) and its last (2 w + 1): 2 slots per workgroup whatever the
-// lengths are.  (With a fixed number of splits per pair, workgroups of a ragged batch were short and unequal: 64
-// requests of 512 to 8,191 positions, 8 KV heads, 116 us.)
+// Decode in equal shares of all tiles of a call: the (request, KV head) pairs stand in a line, each as long as its tiles plus
+// kPad (what beginning with a pair costs, about: Q, the first loads, the join), and workgroup w takes [w share, (w + 1) share)
+// of it.  A pair that one workgroup has is written at once; of a pair that several have, each leaves a part, which the last
+// of them or a second launch merges.  A workgroup has at most two such pairs, its first (slot 2 w) and its last (2 w + 1): 2
+// slots per workgroup whatever the lengths are.  (With a fixed number of splits per pair, workgroups of a ragged batch are
+// short and unequal: 64 requests x 8 heads (D 128), up to 8,191 positions 117 us against 98.)
 constexpr int kPad = 8;
 
 // A request's table row and length; rows out of range hold nothing.
@@ -647,13 +654,13 @@ extern "C" int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q
   // pair can have of equal shares (one long request among short ones).  us per call, by a second launch / inside: 64 requests x 8
   // heads (D 128), up to 8,191 positions 110 / 106, 32 x 8 up to 3,000 29.5 / 27.6, 32 x 4 up to 16,000 52.3 / 46.2; of one of them
   // alone among short ones 20.0 / 16.3, 15.5 / 11.8, 21.3 / 23.2; 32 x 1 (16 q heads, 512 parts) 29.3 / 43.5.
-  const bool few = n_splits > 1 ? n_splits <= kFew : n_splits < -1 && D < 256 && -n_splits / (H > 0 ? H : 1) <= kMostParts;
+  const bool few = n_splits > 1 ? n_splits <= kFew : n_splits < -1 && D < 256 && -(n_splits / (H > 0 ? H : 1)) <= kMostParts;
   P.counters = few ? (int32_t*)counters : nullptr;
   P.cu = nullptr, P.out = out, P.part_o = (float*)part_o, P.part_ml = (float*)part_ml;
   P.sq_n = sq_n, P.sq_h = sq_h, P.so_n = so_n, P.so_h = so_h, P.stride = bt_stride, P.scale_log2 = scale * kLog2e;
   P.n = n, P.n_rows = n_rows, P.n_q = n, P.H = H, P.gs = H > 0 ? Hq / H : 0, P.n_blocks = n_blocks;
   P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.causal = 0;
-  P.splits = n_splits >= 0 ? n_splits : 1, P.shares = n_splits >= 0 ? 0 : -n_splits;
+  P.splits = n_splits >= 0 ? n_splits : 1, P.shares = n_splits >= 0 ? 0 : -max(n_splits, -65536);
   P.item_rows = 16, P.tile = kTile, P.least = kWaves, P.shift = 0;
   while (P.shift < 31 && ((double)n * H * (((double)max_blocks * block / kTile + kPad) / (1 << P.shift) + 2) + P.shares) > 2e9) ++P.shift;
   const int st = check(P, Hq, D, block, code, q_type, out_type);
@@ -689,7 +696,7 @@ extern "C" int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int 
   if (!cu_q || n_q < 0 || (item_rows != 16 && !tiled) || (n_splits > 1 && (!part_o || !part_ml))) return KVT_EINVAL;
   if (n_q == 0) return KVT_OK;
   const int64_t items = (int64_t)n_q * P.gs / item_rows + n;
-  if (items > (tiled ? 0x7FFFFFFF / P.H : 65535) || (n_splits > 1 && items * P.H > 65535)) return KVT_ERANGE;
+  if (items > (tiled ? 0xFFFFFF / P.H : 65535) || (n_splits > 1 && items * P.H > 65535)) return KVT_ERANGE;
   if (tiled) {
     tile_launch(P, code, q_type, D, (int)items, out_type, (hipStream_t)stream);
     if (n_splits > 1) {

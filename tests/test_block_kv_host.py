@@ -127,25 +127,27 @@ def test_c_entries_refuse_sizes(kvt_pkg):
                 dict(n=4097, n_rows=4097), dict(n=2), dict(stride=3), dict(max_blocks=0), dict(code=2), dict(n_blocks=0),
                 dict(block=8), dict(k=8)):
         assert store(**bad) == -1, bad
-    assert store(H=65536) == -3
+    assert store(H=65536) == -3 and store(n_tokens=2 ** 30, H=16, block=16) == -3
     assert store(n_tokens=0) == 0                # nothing to do, nothing launched
 
     def attn(fn, n=1, H=1, Hq=1, D=64, code=0, n_blocks=1, block=64, stride=4, n_rows=1, max_blocks=4, splits=1, s=64, qt=0,
-             ot=0, q=N, n_q=1, cu=64, item_rows=16, scale=1.0, part=N):
+             ot=0, q=N, n_q=1, cu=64, item_rows=16, scale=1.0, part=N, so=None, out=N):
         head = (q, s, s, qt) + ((cu, n_q) if fn == "kvt_block_prefill" else ())
         mid = (0,) if fn == "kvt_block_prefill" else ()
         rows = (item_rows,) if fn == "kvt_block_prefill" else ()
         return getattr(L, fn)(*head, N, n, H, Hq, D, code, N, N, N, N, n_blocks, block, N, stride, n_rows, max_blocks, N, *mid,
-                              scale, *rows, splits, part, part, N, ot, s, s, N)
+                              scale, *rows, splits, part, part, N, out, ot, s if so is None else so, s if so is None else so, N)
     for fn in ("kvt_block_decode", "kvt_block_prefill"):
         for bad in (dict(n=0), dict(n=4097, n_rows=4097), dict(n=2), dict(H=0), dict(Hq=0), dict(H=2, Hq=3), dict(Hq=17),
                     dict(D=32), dict(code=2), dict(n_blocks=0), dict(block=128), dict(stride=3), dict(n_rows=0),
                     dict(max_blocks=0), dict(splits=0), dict(splits=2), dict(s=60), dict(qt=2), dict(ot=3), dict(q=8),
-                    dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan"))):
+                    dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(out=8), dict(so=60), dict(ot=2, so=62)):
             assert attn(fn, **bad) == -1, (fn, bad)
         assert attn(fn, max_blocks=2 ** 26, stride=2 ** 26) == -3
     assert attn("kvt_block_prefill", n_q=-1) == -1 and attn("kvt_block_prefill", cu=N) == -1
     assert attn("kvt_block_prefill", item_rows=32) == -1 and attn("kvt_block_prefill", n_q=2 ** 20, Hq=1) == -3
     assert attn("kvt_block_decode", splits=1025) == -3 and attn("kvt_block_decode", splits=-65536) == -1
     assert attn("kvt_block_decode", splits=-65536, part=64) == -3 and attn("kvt_block_prefill", splits=-2) == -1
+    assert attn("kvt_block_decode", splits=-2 ** 31, part=64) == -3 and attn("kvt_block_decode", splits=-65536, H=2 ** 16, Hq=2 ** 16) == -3
+    assert attn("kvt_block_prefill", n_q=2 ** 30, H=2 ** 4, Hq=2 ** 4, item_rows=128) == -3      # (2^32 threads)
     assert attn("kvt_block_prefill", n_q=0) == 0

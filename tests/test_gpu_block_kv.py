@@ -640,7 +640,7 @@ def test_merge_in_the_launch(kvt_pkg, kv, Hq, H, D, B, splits):
                                splits=splits, workspace=w, out_dtype=torch.float32) for w in (ws, ws, None)]
             for other in got[1:]:
                 assert torch.equal(got[0].view(torch.int32), other.view(torch.int32))
-            assert not ws["block_counters"].any()
+            assert not ws["block_counters", 0].any()
 
 
 @pytest.mark.parametrize("kv", ["fp8", "int8"])
@@ -654,4 +654,48 @@ def test_merge_of_shares_in_the_launch(kvt_pkg, kv, Hq, H, D, B, shares):
                            out_dtype=torch.float32) for w in (ws, ws, None)]
         for other in got[1:]:
             assert torch.equal(got[0].view(torch.int32), other.view(torch.int32))
-        assert not ws["block_counters"].any()
+        assert not ws["block_counters", 0].any()
+
+
+@pytest.mark.parametrize("warm", [True, False])
+def test_workspace_of_a_captured_call_is_outgrown(kvt_pkg, warm):
+    """A decode and a chunk captured over a workspace, made before the capture or inside it, which larger eager calls outgrow
+    and use between the replays: every replay gives the eager bits."""
+    from kvtier import block_kv
+    H, D, Hq, B = 2, 128, 8, 32
+    g = torch.Generator().manual_seed(23)
+    lens = [900, 33, 1500, 1, 64, 700]
+    table, nb = _tables(lens, B, 2, 23)
+    codes, sc = _pool("fp8", nb, H, B, D, g)
+    buf = (codes[0].to(dev), codes[1].to(dev), sc[0].to(dev), sc[1].to(dev))
+    tab, kl = i32(table), i32(lens)
+    q = torch.randn(6, Hq, D, generator=g).to(torch.bfloat16).to(dev)
+    cq = torch.randn(6 * 5, Hq, D, generator=g).to(torch.bfloat16).to(dev)
+    few = (tab[:2].contiguous(), kl[:2].contiguous())
+    cu2, cu6 = i32([0, 5, 10]), i32([5 * i for i in range(7)])
+    ws = {}
+
+    def small(w, x, y):
+        return (block_kv.kvt_block_decode(x[:2], *buf, *few, workspace=w),
+                block_kv.kvt_block_prefill(y[:10], cu2, *buf, *few, workspace=w))
+
+    def large(w):
+        return (block_kv.kvt_block_decode(q, *buf, tab, kl, workspace=w),
+                block_kv.kvt_block_prefill(cq, cu6, *buf, tab, kl, workspace=w))
+
+    if warm:
+        small(ws, q, cq)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        outs = small(ws, q, cq)
+    for i in range(4):
+        q.normal_()
+        cq.normal_()
+        gr.replay()
+        want = small(None, q, cq)
+        torch.cuda.synchronize()
+        # (the bits: queries of the request with fewer positions than queries see nothing and are NaN, which equals nothing)
+        for a, b in (*zip(outs, want), *zip(large(ws), large(None))):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16)), i
+    assert ("block_outgrown" in ws) and not ws["block_counters", 0].any()

@@ -25,6 +25,7 @@ import torch
 from . import _lib
 
 CODE = {torch.float8_e4m3fn: 0, torch.int8: 1}
+_I32, _F32 = torch.int32, torch.float32
 BLOCKS = (16, 32, 64)
 HEAD_DIMS = (64, 128, 256)
 POOL_SHORT, ROW_FULL, TOKENS_OVER, BAD_ROW = 1, 2, 4, 8   # status bits of a plan
@@ -71,29 +72,29 @@ class BlockPlan:
 
 def _stream(*tensors: Optional[torch.Tensor]) -> int:
     """The current stream of the tensors' device, which has to be the current one (launches go there)."""
-    dev = tensors[0].get_device()
-    cur = torch.cuda.current_device() if dev >= 0 else -1
+    cur = torch.cuda.current_device() if tensors[0].is_cuda else -1
     for t in tensors:
-        if t is not None and (t.get_device() != cur or dev < 0):
+        if t is not None and t.get_device() != cur or cur < 0:
             _lib.require_device(*tensors)
             raise ValueError(f"tensor on {t.device}, but the current device is cuda:{cur}")
     return _lib.stream(cur)
 
 
 def _i32(name: str, t: torch.Tensor, n: int) -> None:
-    assert t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous(), f"{name} must be a contiguous int32 vector"
+    assert t.dtype == _I32 and t.dim() == 1 and t.is_contiguous(), f"{name} must be a contiguous int32 vector"
     if t.numel() < n:
         raise ValueError(f"{name} has {t.numel()} entries, {n} are needed")
 
 
 def _pool(k8, v8, ks, vs, block_table, n, seqs):
     """Checks of a layer's buffers; (n_blocks, H, block, D)."""
-    assert k8.dtype in CODE and v8.dtype == k8.dtype, "block codes are float8_e4m3fn or int8"
-    assert k8.dim() == 4 and v8.shape == k8.shape and k8.is_contiguous() and v8.is_contiguous()
-    nb, H, B, D = k8.shape
-    assert ks.dtype == torch.float32 and vs.dtype == torch.float32 and ks.is_contiguous() and vs.is_contiguous()
-    assert ks.shape == (nb, H) and vs.shape == (nb, H)
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1
+    shape, dtype = k8.shape, k8.dtype
+    assert dtype in CODE and v8.dtype == dtype, "block codes are float8_e4m3fn or int8"
+    assert len(shape) == 4 and v8.shape == shape and k8.is_contiguous() and v8.is_contiguous()
+    nb, H, B, D = shape
+    assert ks.dtype == vs.dtype == _F32 and ks.is_contiguous() and vs.is_contiguous()
+    assert ks.shape == vs.shape == (nb, H)
+    assert block_table.dtype == _I32 and block_table.dim() == 2 and block_table.stride(1) == 1
     if B not in BLOCKS or D not in HEAD_DIMS:
         raise ValueError(f"blocks of {B} tokens x {D} channels: {BLOCKS} tokens and {HEAD_DIMS} channels are served")
     if seqs is not None:
@@ -122,7 +123,7 @@ def kvt_block_plan(seqs: torch.Tensor, counts: torch.Tensor, seq_lens: torch.Ten
     _i32("seq_lens", seq_lens, 1)
     _i32("free_list", free_list, 0)
     _i32("free_head", free_head, 1)
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1
+    assert block_table.dtype == _I32 and block_table.dim() == 2 and block_table.stride(1) == 1
     rows = block_table.shape[0]
     if seq_lens.numel() < rows:
         raise ValueError(f"seq_lens has {seq_lens.numel()} entries for {rows} table rows")
@@ -143,11 +144,13 @@ def kvt_block_plan(seqs: torch.Tensor, counts: torch.Tensor, seq_lens: torch.Ten
     return BlockPlan(seqs, cu, slots, kv_lens, next_head)
 
 
-def _rows16(x: torch.Tensor, per16: int) -> torch.Tensor:
-    """x itself where its rows start at 16-byte boundaries, else a contiguous copy."""
-    if x.data_ptr() % 16 or x.stride(0) % per16 or x.stride(1) % per16 or x.stride(2) != 1:
-        return x.contiguous() if not x.is_contiguous() else x.clone()
-    return x
+def _rows16(x: torch.Tensor, per16: int):
+    """Rows that start at 16-byte boundaries (x itself, else a contiguous copy): tensor, pointer, strides of token and head."""
+    p, (a, b, c) = x.data_ptr(), x.stride()
+    if p & 15 or a % per16 or b % per16 or c != 1:
+        x = x.contiguous() if not x.is_contiguous() else x.clone()
+        p, (a, b, c) = x.data_ptr(), x.stride()
+    return x, p, a, b
 
 
 def kvt_block_store(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, kv_lens: torch.Tensor, k8: torch.Tensor,
@@ -171,11 +174,10 @@ def kvt_block_store(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, kv_lens:
         return
     st = _stream(k, v, cu, kv_lens, k8, v8, ks, vs, block_table, seqs)
     per16 = 4 if k.dtype == torch.float32 else 8
-    k, v = _rows16(k, per16), _rows16(v, per16)
-    _lib.call("kvt_block_store", k.data_ptr(), v.data_ptr(), _lib.DTYPE_CODE[k.dtype], k.stride(0), k.stride(1),
-              v.stride(0), v.stride(1), N, H, D, cu.data_ptr(), kv_lens.data_ptr(), n, _lib.ptr(seqs),
-              block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1], CODE[k8.dtype],
-              k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B, st)
+    k, kp, kn, kh = _rows16(k, per16)
+    v, vp, vn, vh = _rows16(v, per16)
+    _lib.call("kvt_block_store", kp, vp, _lib.DTYPE_CODE[k.dtype], kn, kh, vn, vh, N, H, D, cu.data_ptr(), kv_lens.data_ptr(), n, _lib.ptr(seqs),
+              block_table.data_ptr(), block_table.stride(0), *block_table.shape, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B, st)
 
 
 def _grown(ws: dict, name: str, n: int, like: torch.Tensor, dtype=torch.float32, zero: bool = False) -> torch.Tensor:
@@ -191,14 +193,10 @@ def _grown(ws: dict, name: str, n: int, like: torch.Tensor, dtype=torch.float32,
     return t
 
 
-def _parts(workspace: Optional[dict], need: int, D: int, q: torch.Tensor, items: int = 0):
-    """Pointers of a split launch's partial buffers: need rows of D values and of (maximum, sum), and the counters of
-    `items` whose parts the launch itself merges.  Those have to be zero, which every call leaves them: they live in a
-    kept workspace, and not in one that a capture makes (its zeros would only be written by a replay)."""
-    if workspace is None:
-        ws, items = {}, 0
-    else:
-        ws = workspace
+def _parts(ws: dict, need: int, D: int, q: torch.Tensor, items: int):
+    """Pointers of a split launch's partial buffers in ws: need rows of D values and of (maximum, sum), and the counters of
+    `items` (0: none) whose parts the launch itself merges.  Those have to be zero, which every call leaves them; a capture
+    does not make them, since its zeros would only be written by a replay."""
     o, ml = _grown(ws, "block_o", need * D, q), _grown(ws, "block_ml", need * 2, q)
     if items == 0:
         return o.data_ptr(), ml.data_ptr(), None
@@ -206,20 +204,20 @@ def _parts(workspace: Optional[dict], need: int, D: int, q: torch.Tensor, items:
     if c is None or c.numel() < items:
         if torch.cuda.is_current_stream_capturing():
             return o.data_ptr(), ml.data_ptr(), None
-        c = _grown(ws, "block_counters", items, q, torch.int32, True)
+        c = _grown(ws, "block_counters", items, q, _I32, True)
     return o.data_ptr(), ml.data_ptr(), c.data_ptr()
 
 
 def _attn_args(q, out, H, D):
     assert q.dim() == 3 and q.dtype in (torch.bfloat16, torch.float16), "queries are bf16 or fp16 [rows, Hq, D]"
-    Hq = q.shape[1]
-    assert q.shape[2] == D, f"queries of {q.shape[2]} channels over blocks of {D}"
-    if Hq % H or Hq // H > 16 or Hq == 0:
+    _, Hq, d = q.shape
+    assert d == D, f"queries of {d} channels over blocks of {D}"
+    if H == 0 or Hq == 0 or Hq % H or Hq // H > 16:
         raise ValueError(f"{Hq} q heads over {H} KV heads: a multiple, at most 16 each, is served")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     assert out.shape == q.shape and out.dtype in _lib.DTYPE_CODE and out.stride(2) == 1
-    return _rows16(q, 8), out, Hq
+    return (*_rows16(q, 8), out, Hq)
 
 
 def _splits(items: int, cap: int, blocks: int, least: int = 128) -> int:
@@ -242,7 +240,7 @@ def kvt_block_decode(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: to
     as long as it is replayed, and one made before the capture is the faster one.  The results do not depend on it."""
     n = kv_lens.numel()
     nb, H, B, D = _pool(k8, v8, ks, vs, block_table, n, seqs)
-    q, out, Hq = _attn_args(q, out, H, D)
+    q, qp, qn, qh, out, Hq = _attn_args(q, out, H, D)
     if q.shape[0] != n:
         raise ValueError(f"{q.shape[0]} queries for {n} requests")
     _i32("kv_lens", kv_lens, n)
@@ -258,13 +256,13 @@ def kvt_block_decode(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: to
         ns = _splits(n * H, cap, 768 if n > 1 else _DECODE_BLOCKS[D])
     o = ml = counters = None
     if ns > 1 or ns < -1:
-        o, ml, counters = _parts(workspace, n * H * ns * 16 if ns > 1 else -2 * ns * 16, D, q,
-                                 n * H if ns <= _MERGE_SPLITS else 0)
-    _lib.call("kvt_block_decode", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], kv_lens.data_ptr(), n,
-              H, Hq, D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B,
-              block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1], _lib.ptr(seqs),
-              D ** -0.5 if scale is None else float(scale), ns, o, ml, counters, out.data_ptr(), _lib.DTYPE_CODE[out.dtype],
-              out.stride(0), out.stride(1), st)
+        ws = {} if workspace is None else workspace          # (held until the launch)
+        o, ml, counters = _parts(ws, n * H * ns * 16 if ns > 1 else -2 * ns * 16, D, q,
+                                 n * H if workspace is not None and ns <= _MERGE_SPLITS else 0)
+    _lib.call("kvt_block_decode", qp, qn, qh, _lib.DTYPE_CODE[q.dtype], kv_lens.data_ptr(), n, H, Hq, D, CODE[k8.dtype],
+              k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B, block_table.data_ptr(), block_table.stride(0),
+              *block_table.shape, _lib.ptr(seqs), D ** -0.5 if scale is None else float(scale), ns, o, ml, counters,
+              out.data_ptr(), _lib.DTYPE_CODE[out.dtype], out.stride(0), out.stride(1), st)
     return out
 
 
@@ -281,7 +279,7 @@ def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8:
     NaN (0/0).  Other arguments as kvt_block_decode."""
     n = kv_lens.numel()
     nb, H, B, D = _pool(k8, v8, ks, vs, block_table, n, seqs)
-    q, out, Hq = _attn_args(q, out, H, D)
+    q, qp, qn, qh, out, Hq = _attn_args(q, out, H, D)
     _i32("kv_lens", kv_lens, n)
     _i32("cu_q", cu_q, n + 1)
     total = q.shape[0]
@@ -301,12 +299,13 @@ def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8:
             ns = _splits(full, cap, _DECODE_BLOCKS[D])
     o = ml = counters = None
     if ns > 1:
-        o, ml, counters = _parts(workspace, items * H * ns * rows, D, q,
-                                 items * H if rows == 16 and ns <= _MERGE_SPLITS else 0)
-    _lib.call("kvt_block_prefill", q.data_ptr(), q.stride(0), q.stride(1), _lib.DTYPE_CODE[q.dtype], cu_q.data_ptr(), total,
-              kv_lens.data_ptr(), n, H, Hq, D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(),
-              nb, B, block_table.data_ptr(), block_table.stride(0), block_table.shape[0], block_table.shape[1],
-              _lib.ptr(seqs), int(bool(causal)), D ** -0.5 if scale is None else float(scale), rows, ns, o, ml, counters, out.data_ptr(),
+        ws = {} if workspace is None else workspace          # (held until the launch)
+        o, ml, counters = _parts(ws, items * H * ns * rows, D, q,
+                                 items * H if workspace is not None and rows == 16 and ns <= _MERGE_SPLITS else 0)
+    _lib.call("kvt_block_prefill", qp, qn, qh, _lib.DTYPE_CODE[q.dtype], cu_q.data_ptr(), total, kv_lens.data_ptr(), n, H, Hq,
+              D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B, block_table.data_ptr(),
+              block_table.stride(0), *block_table.shape, _lib.ptr(seqs), int(bool(causal)),
+              D ** -0.5 if scale is None else float(scale), rows, ns, o, ml, counters, out.data_ptr(),
               _lib.DTYPE_CODE[out.dtype], out.stride(0), out.stride(1), st)
     return out
 

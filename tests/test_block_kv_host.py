@@ -53,7 +53,7 @@ def test_decode_contract(kvt_pkg, over):
 @pytest.mark.parametrize("over", [dict(q=torch.zeros(3, 4, 64, dtype=torch.bfloat16)), dict(q=torch.zeros(2, 5, 64, dtype=torch.bfloat16)),
                                   dict(q=torch.zeros(2, 34, 64, dtype=torch.bfloat16)), dict(seqs=torch.zeros(1, dtype=torch.int32)),
                                   dict(block_table=torch.zeros(1, 3, dtype=torch.int32)),
-                                  dict(_pool(B=48)), dict(_pool(D=96), q=torch.zeros(2, 4, 96, dtype=torch.bfloat16))])
+                                  dict(_pool(H=0)), dict(_pool(B=48)), dict(_pool(D=96), q=torch.zeros(2, 4, 96, dtype=torch.bfloat16))])
 def test_decode_sizes(kvt_pkg, over):
     with pytest.raises(ValueError):
         _decode(**over)

@@ -40,9 +40,10 @@ _SHARE_REQUESTS, _SHARE_CAP = 16, 2048
 # 4, 32.6 with 8).
 _DECODE_BLOCKS = {64: 512, 128: 512, 256: 256}
 # Splits of a pair that a launch with a kept workspace merges itself.  us per call, merged by a second launch / by itself: 8
-# requests x 2 heads (D 256, up to 2,000 positions, 16 splits) 15.8 / 13.8; one x 8 (D 128, 2,000, 16 splits) 12.8 / 9.5; 8 x 8
-# (D 128, up to 4,000, 12 splits) 19.0 / 15.7; chunks of four queries over the same (8 splits) 22.1 / 19.9.  Past 16 the
-# second launch's many workgroups read the parts faster than the last one does.  (Equal shares: the entry point decides.)
+# requests x 2 heads (D 256, up to 2,000 positions, 16 splits) 15.4 / 12.4; one x 8 (D 128, 2,000, 16 splits) 12.7 / 8.6; 8 x 8
+# (D 128, up to 4,000, 12 splits) 18.7 / 15.5; chunks of four queries over the same (8 splits) 22.1 / 19.9; but two of 300
+# positions x 2 heads (24 q heads) 11.5 / 12.1.  Past 16 the second launch's many workgroups read the parts faster than the
+# last one does.  (Equal shares: the entry point decides.)
 _MERGE_SPLITS = 16
 _TILE_ROWS = 128         # (query, q head) rows of a workgroup of the query-tile kernel
 # Workgroups of a split launch of it for one request, us per call (merge included): D 256, 16 items x 30,000 positions 256

@@ -24,7 +24,7 @@
 // there, 5.9 TB/s (a large copy 5.2), where more than half of the wavefronts' time is waiting for memory and the vector
 // instructions take 30 %, the matrix instructions 9 % of theirs; e4m3, 32 requests of 12,000 positions and less (204 MB)
 // 38.4 us, 5.3 TB/s; int8, 64 requests x 8 heads, D 128 (456 MB) 94 us, 4.9 TB/s.  Short calls are launch and load latency:
-// 777 positions of 2 heads 12 us with the merge in the launch.
+// 777 positions of 2 heads 11 us with the merge in the launch.
 #include "block_attn.h"
 
 using namespace kvt;
@@ -284,10 +284,12 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
 // slot s0, part k > 0 in slot sb + step k.  Parts cross XCDs, whose L2s do not see each other: they are stored and loaded at
 // device scope, and a workgroup counts itself when its stores have arrived.  Nobody waits for another workgroup.  The
 // parts are added in their order whoever merges them, as the merge by a second launch does: the same bits.
-template <int D>
+//
+// A thread has four channels of a row at a time, and loads them of 16 parts at once: of its first row beside the parts' maxima.
+// Most items have no more parts (MANY: they may, D 64 and 128; at D 256 the registers would spill).
+template <int D, bool MANY>
 KVT_DEV void merge_last(const Attn& P, const Item& it, int h, int64_t item, int parts, int64_t s0, int64_t sb, int step, int ot,
                         Join<D>& J) {
-  constexpr int NE = D / 64;                        // four channels each: 16 rows over 256 threads
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();                                  // every thread's parts have arrived
   if (threadIdx.x == 0) {
@@ -299,54 +301,81 @@ KVT_DEV void merge_last(const Attn& P, const Item& it, int h, int64_t item, int 
   if (!J.last) return;
   const auto ro = part_rsrc(P.part_o + s0 * 16 * D, (step * parts + 1) * 64 * D);
   const auto rml = part_rsrc(P.part_ml + s0 * 32, (step * parts + 1) * 128);
-  const int base = (int)(sb - s0);                  // (slots from here on count from s0)
+  const int base = (int)(sb - s0), end = it.n_row * (D / 4);   // (slots from here on count from s0)
   const auto slot = [&](int k) { return k ? base + step * k : 0; };
-  const int row = threadIdx.x >> 4, lane = threadIdx.x & 15;   // 16 rows x 16 parts at a time
-  const auto read_ml = [&](int k) {
-    return row < it.n_row && k < parts
-               ? __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rml, (16 * slot(k) + row) * 8, 0, kSc1))
-               : make_float2(-__builtin_inff(), 0.0f);
+  // (no branch around a load, which would wait for it: what is not there is an offset past the buffer, and reads 0)
+  f4 o[kFew];
+  const auto load = [&](int e, int k0) {            // row e / (D / 4), channels 4 (e % (D / 4)) ..
+#pragma unroll
+    for (int k = 0; k < kFew; ++k)
+      o[k] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(
+                                        ro, k0 + k < parts && e < end ? 64 * D * slot(k0 + k) + 16 * e : -16, 0, kSc1));
   };
-  const float2 first = read_ml(lane);
-  float M = first.x;
-  for (int k = lane + kFew; k < parts; k += kFew) M = fmaxf(M, read_ml(k).x);
+  const int row = threadIdx.x >> 4, lane = threadIdx.x & 15;   // 16 rows x 16 parts
+  const auto read_ml = [&](int k) {
+    const bool is = row < it.n_row && k < parts;
+    const float2 ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rml, is ? (16 * slot(k) + row) * 8 : -8, 0, kSc1));
+    return make_float2(is ? ml.x : -__builtin_inff(), ml.y);
+  };
+  const auto add = [&](int e, f4& O, float& L) {
+    const int r = e / (D / 4);
+#pragma unroll
+    for (int k = 0; k < kFew; ++k) {
+      const float f = J.w[r][k];
+      L += f;
+      O += f * o[k];
+    }
+  };
+  const auto write = [&](int e, const f4& O, float L) {
+    const int at = it.row0 + e / (D / 4), d = 4 * (e % (D / 4));
+    const f4 y = L == 0.0f ? f4{1, 1, 1, 1} * __builtin_nanf("") : O / L;
+    store_out4(P.out, ot, (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + d, y[0], y[1], y[2],
+               y[3]);
+  };
+  load(threadIdx.x, 0);
+  float2 ml = read_ml(lane);
+  float M = ml.x;
+  if (MANY)
+    for (int k = lane + kFew; k < parts; k += kFew) M = fmaxf(M, read_ml(k).x);
   M = group_max<16>(M);
+  if (!MANY || parts <= kFew) {
+    J.w[row][lane] = weight_of(ml.x, ml.y, M);
+    __syncthreads();
+    for (int e = threadIdx.x;;) {
+      f4 O = {0, 0, 0, 0};
+      float L = 0.0f;
+      if (e < end) {
+        add(e, O, L);
+        write(e, O, L);
+      }
+      e += 256;
+      if (e - (int)threadIdx.x >= end) break;
+      load(e, 0);
+    }
+    return;
+  }
+  constexpr int NE = MANY ? D / 64 : 1;             // 16 rows over 256 threads
   f4 O[NE];
   float L[NE];
 #pragma unroll
   for (int n = 0; n < NE; ++n) O[n] = f4{0, 0, 0, 0}, L[n] = 0.0f;
   for (int k0 = 0; k0 < parts; k0 += kFew) {
-    const float2 ml = k0 ? read_ml(k0 + lane) : first;
+    if (k0) {
+      load(threadIdx.x, k0);
+      ml = read_ml(k0 + lane);
+    }
     J.w[row][lane] = weight_of(ml.x, ml.y, M);
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NE; ++n) {
-      const int e = threadIdx.x + 256 * n, r = e / (D / 4), d = 4 * (e % (D / 4));
-      if (r >= it.n_row) continue;
-      f4 o[kFew];
-#pragma unroll
-      for (int k = 0; k < kFew; ++k)
-        if (k0 + k < parts)
-          o[k] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(ro, ((16 * slot(k0 + k) + r) * D + d) * 4, 0, kSc1));
-#pragma unroll
-      for (int k = 0; k < kFew; ++k)
-        if (k0 + k < parts) {
-          const float f = J.w[r][k];
-          L[n] += f;
-          O[n] += f * o[k];
-        }
+      if (n) load(threadIdx.x + 256 * n, k0);
+      add(threadIdx.x + 256 * n, O[n], L[n]);
     }
     __syncthreads();
   }
 #pragma unroll
-  for (int n = 0; n < NE; ++n) {
-    const int e = threadIdx.x + 256 * n, r = e / (D / 4), d = 4 * (e % (D / 4));
-    if (r >= it.n_row) continue;
-    const f4 y = L[n] == 0.0f ? f4{1, 1, 1, 1} * __builtin_nanf("") : O[n] / L[n];
-    const int at = it.row0 + r;
-    store_out4(P.out, ot, (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + d, y[0], y[1], y[2],
-               y[3]);
-  }
+  for (int n = 0; n < NE; ++n)
+    if ((int)threadIdx.x + 256 * n < end) write(threadIdx.x + 256 * n, O[n], L[n]);
 }
 
 template <int CODE, int QT, int D>
@@ -361,7 +390,7 @@ __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot
   if (split >= used) return;                        // (the merge knows which splits there are)
   const int64_t item = (int64_t)w * P.H + h;
   attend<CODE, QT, D>(P, it, h, tile0, tile1, used == 1, item * P.splits + split, ot, J);
-  if (P.counters && used > 1) merge_last<D>(P, it, h, item, used, item * P.splits, item * P.splits, 1, ot, J);
+  if (P.counters && used > 1) merge_last<D, false>(P, it, h, item, used, item * P.splits, item * P.splits, 1, ot, J);
 }
 
 // Decode in equal shares of all tiles of a call: the (request, KV head) pairs stand in a line, each as long as its tiles plus
@@ -466,8 +495,8 @@ __global__ __launch_bounds__(256, 2) void block_decode_kernel(const Attn P, int 
         attend<CODE, QT, D>(P, it, h, t0, t1, whole, 2 * (int64_t)w + (a > x0), ot, J);
         if (D < 256 && P.counters && !whole) {// (at D 256 the merge's registers would spill)
           const int w0 = (int)(a / share), w1 = (int)((a + (uint32_t)((tiles - 1) >> P.shift)) / share);
-          merge_last<D>(P, it, h, (int64_t)r * P.H + h, w1 - w0 + 1, 2 * (int64_t)w0 + (a > (uint32_t)w0 * share), 2 * (int64_t)w0, 2,
-                        ot, J);
+          merge_last<D, (D < 256)>(P, it, h, (int64_t)r * P.H + h, w1 - w0 + 1, 2 * (int64_t)w0 + (a > (uint32_t)w0 * share),
+                                   2 * (int64_t)w0, 2, ot, J);
         }
         __syncthreads();                            // (J is free again)
       }
@@ -652,8 +681,8 @@ extern "C" int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q
   P.table = (const int32_t*)block_table, P.kv_lens = (const int32_t*)kv_lens, P.rows = (const int32_t*)rows;
   // One workgroup merges a pair's parts inside the launch: up to kFew splits, or kMostParts parts, which is about the most that a
   // pair can have of equal shares (one long request among short ones).  us per call, by a second launch / inside: 64 requests x 8
-  // heads (D 128), up to 8,191 positions 110 / 106, 32 x 8 up to 3,000 29.5 / 27.6, 32 x 4 up to 16,000 52.3 / 46.2; of one of them
-  // alone among short ones 20.0 / 16.3, 15.5 / 11.8, 21.3 / 23.2; 32 x 1 (16 q heads, 512 parts) 29.3 / 43.5.
+  // heads (D 128), up to 8,191 positions 103 / 100, 32 x 8 up to 3,000 29.8 / 27.7, 32 x 4 up to 16,000 51.5 / 46.8; of one of them
+  // alone among short ones 20.9 / 16.3, 16.4 / 11.4, 21.7 / 23.0; 32 x 1 (16 q heads, 512 parts) 29.3 / 43.5.
   const bool few = n_splits > 1 ? n_splits <= kFew : n_splits < -1 && D < 256 && -(n_splits / (H > 0 ? H : 1)) <= kMostParts;
   P.counters = few ? (int32_t*)counters : nullptr;
   P.cu = nullptr, P.out = out, P.part_o = (float*)part_o, P.part_ml = (float*)part_ml;

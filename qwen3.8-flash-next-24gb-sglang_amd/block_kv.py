@@ -51,7 +51,10 @@ _TILE_ROWS = 128         # (query, q head) rows of a workgroup of the query-tile
 # many again for several, whose lengths differ: 4 x 8 heads (D 128), 64 queries, up to 6,000 positions 75 / 58, 8 x 20 heads (D
 # 64) up to 1,500 52.5 / 45.5, 8 x 2 (D 256) up to 4,000 124 / 110, 8 x 8 (D 128) up to 3,000 53 / 55.
 _TILE_BLOCKS = {64: 768, 128: 384, 256: 512}
-_TILE_LEAST = 512        # positions of a split at least: its part of 128 rows is 512 D bytes written and read again
+# Positions of a split at least: its part of 128 rows is 512 D bytes written and read again.  Half of it where those splits
+# would leave half of the CUs idle: 5 query tiles (D 128) behind 1,758 positions 26.0 us with 512, 20.7 with 256, 19.3 with 128;
+# 24 (D 256) behind 1,000 42 / 34 / 33; but 34 (D 256) behind 3,428 49 / 51 / 80, 44 (D 64) behind 4,000 36 / 35 / 47.
+_TILE_LEAST = 512
 # Rows per request and KV head (on average) from which it serves a call.  us per call against the 16-row kernel's, one request
 # behind 30,000 positions: D 128, 64 rows 41 / 42, 128 rows 66 / 64, 256 rows 72 / 102; D 64, 128 rows 78 / 79, 256 rows 116 /
 # 143; D 256, 128 rows 59 / 44, 256 rows 60 / 61, 512 rows 82 / 90.  Eight ragged requests behind 4,000: D 128, 116 rows 54
@@ -295,7 +298,8 @@ def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8:
         full = max(-(-total * (Hq // H) // rows), n) * H     # (items less the empty ones)
         cap = block_table.shape[1] * B
         if rows > 16:
-            ns = _splits(full, cap, _TILE_BLOCKS[D] * (3 if n > 1 else 2) // 2, _TILE_LEAST)
+            least = _TILE_LEAST if full * -(-cap // _TILE_LEAST) >= 128 else _TILE_LEAST // 2
+            ns = _splits(full, cap, _TILE_BLOCKS[D] * (3 if n > 1 else 2) // 2, least)
         else:
             ns = _splits(full, cap, _DECODE_BLOCKS[D])
     o = ml = counters = None

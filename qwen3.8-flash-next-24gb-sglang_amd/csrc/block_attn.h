@@ -111,7 +111,7 @@ KVT_DEV float load_q(const void* q, int64_t row, At at, Top top_of, h8 (&out)[N]
   uint4 raw[N];
 #pragma unroll
   for (int k = 0; k < N; ++k)
-raw[k] = *reinterpret_cast<const uint4*>((const uint16_t*)q + row + at(k));
+    raw[k] = *reinterpret_cast<const uint4*>((const uint16_t*)q + row + at(k));
   if constexpr (QT == kF16) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {

@@ -717,9 +717,11 @@ extern "C" int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int 
   P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.splits = n_splits, P.causal = causal, P.shares = 0;
   const bool tiled = item_rows == kTileRows;
   P.item_rows = item_rows, P.tile = tiled ? tile_positions(D) : kTile;
-  // (requests of several lengths: splits of a multiple of 512 positions, so that the long ones' are not much longer than the
-  // others', and a short one is not split: 8 x 20 heads (D 64), 448 ragged queries over 1,500 ragged positions 52.5 -> 45.5 us)
-  P.least = !tiled ? kWaves : n > 1 ? 512 / P.tile : 1;
+  // (requests of several lengths: splits of a multiple of 512 positions, or 256 where the call asks for that many of the table's
+  // width, so that the long requests' splits are not much longer than the others', and a short one is not split: 8 x 20 heads
+  // (D 64), 448 ragged queries over 1,500 ragged positions 52.5 -> 45.5 us)
+  const int grain = (int64_t)max_blocks * block <= (int64_t)n_splits * 256 ? 256 : 512;
+  P.least = !tiled ? kWaves : n > 1 ? grain / P.tile : 1;
   const int st = check(P, Hq, D, block, code, q_type, out_type);
   if (st != KVT_OK) return st;
   if (!cu_q || n_q < 0 || (item_rows != 16 && !tiled) || (n_splits > 1 && (!part_o || !part_ml))) return KVT_EINVAL;

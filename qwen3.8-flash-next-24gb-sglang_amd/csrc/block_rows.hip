@@ -521,12 +521,30 @@ __global__ __launch_bounds__(256) void block_decode_merge_kernel(const Attn P, i
   const int w0 = (int)(a / share), w1 = (int)((a + (uint32_t)(max(tiles - 1, 0) >> P.shift)) / share);
   if (w0 == w1 || row >= P.gs) return;
   const auto part_of = [&](int w) { return (2 * (int64_t)w + (a > (uint32_t)w * share)) * 16 + row; };
+  // (the first eight parts beside their maxima: most pairs have no more; those that are not there are the last again, of no weight)
+  constexpr int kNow = 8;
+  f4 o[kNow];
+  float2 now[kNow];
+#pragma unroll
+  for (int k = 0; k < kNow; ++k) {
+    const int64_t p = part_of(min(w0 + k, w1));
+    now[k] = *reinterpret_cast<const float2*>(P.part_ml + 2 * p);
+    o[k] = *reinterpret_cast<const f4*>(P.part_o + p * D + d);
+  }
   float M = -__builtin_inff(), L = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kNow; ++k) M = fmaxf(M, now[k].x);
 #pragma unroll 8
-  for (int w = w0; w <= w1; ++w) M = fmaxf(M, P.part_ml[2 * part_of(w)]);
+  for (int w = w0 + kNow; w <= w1; ++w) M = fmaxf(M, P.part_ml[2 * part_of(w)]);
   f4 O = {0, 0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < kNow; ++k) {
+    const float f = weight_of(now[k].x, now[k].y, M);
+    L = w0 + k <= w1 ? L + f : L;
+    O = w0 + k <= w1 ? O + f * o[k] : O;
+  }
 #pragma unroll 8
-  for (int w = w0; w <= w1; ++w) {
+  for (int w = w0 + kNow; w <= w1; ++w) {
     const int64_t p = part_of(w);
     const float2 ml = *reinterpret_cast<const float2*>(P.part_ml + 2 * p);
     const float f = weight_of(ml.x, ml.y, M);

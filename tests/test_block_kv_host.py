@@ -151,3 +151,16 @@ def test_c_entries_refuse_sizes(kvt_pkg):
     assert attn("kvt_block_decode", splits=-2 ** 31, part=64) == -3 and attn("kvt_block_decode", splits=-65536, H=2 ** 16, Hq=2 ** 16) == -3
     assert attn("kvt_block_prefill", n_q=2 ** 30, H=2 ** 4, Hq=2 ** 4, item_rows=128) == -3      # (2^32 threads)
     assert attn("kvt_block_prefill", n_q=0) == 0
+
+
+def test_attention_refuses_tables_whose_positions_run_past_32_bits(kvt_pkg):
+    """The kernels' 32-bit positions run up to 4,096 ahead of a request's last one: tables within 8,192 of 2^31 are ERANGE."""
+    L = kvt_pkg._lib.lib()
+    for block in (16, 32, 64):
+        for positions in (2 ** 31 - block, 2 ** 31 - 8192 + block):
+            m = positions // block
+            tail = (1.0, 1, None, None, None, None, 0, 64, 64, None)
+            pool = (0, None, None, None, None, 1, block, None, m, 1, m, None)
+            assert L.kvt_block_decode(None, 64, 64, 0, None, 1, 1, 1, 64, *pool, *tail) == -3, (block, positions)
+            for rows in (16, 128):
+                assert L.kvt_block_prefill(None, 64, 64, 0, 64, 1, None, 1, 1, 1, 64, *pool, 1, 1.0, rows, *tail[1:]) == -3

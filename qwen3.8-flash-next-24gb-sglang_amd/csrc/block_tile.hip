@@ -43,13 +43,10 @@ KVT_DEV float sum_xor32(float v) {
 constexpr int kDsRead = 0x100, kMfma = 0x8;   // instruction classes of the scheduling hints
 constexpr float kLeast = 0x1p-120f;   // (a factor of 0 would make a masked score, -inf, a NaN)
 
-// The largest of three (asm: no canonicalizing v_max_f32 x, x for values out of a matrix product).  The compiler does not
-// see asm read the result of a matrix product, and puts no wait before it: one operand has to come from an instruction that it
-// sees read the same result.
+// The largest of three (one v_maximum3_f32; fmaxf of a matrix product's result costs a canonicalizing v_max_f32 x, x each).  Not as
+// asm: the compiler sees no asm read the result of a matrix product, and puts no wait before it.
 KVT_DEV float max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 // v, where the compiler does not know it: what follows from it is computed here, not kept in registers from further up.
 KVT_DEV int again(int v) {
@@ -292,8 +289,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
         float top2[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
-          top2[s] = max3(max3(max3(fmaxf(sc[8 * s], sc[8 * s + 1]), sc[8 * s + 2], sc[8 * s + 3]), sc[8 * s + 4], sc[8 * s + 5]),
-                         sc[8 * s + 6], sc[8 * s + 7]);
+          top2[s] = max3(max3(max3(sc[8 * s], sc[8 * s + 1], sc[8 * s + 2]), sc[8 * s + 3], sc[8 * s + 4]),
+                         sc[8 * s + 5], __builtin_elementwise_maximum(sc[8 * s + 6], sc[8 * s + 7]));
         const float top = max_xor32(fmaxf(top2[0] * f[0], top2[1] * f[1]));
         const bool rise = top > m + kLag;
         if (__any(rise)) {

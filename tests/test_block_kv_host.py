@@ -164,3 +164,15 @@ def test_attention_refuses_tables_whose_positions_run_past_32_bits(kvt_pkg):
             assert L.kvt_block_decode(None, 64, 64, 0, None, 1, 1, 1, 64, *pool, *tail) == -3, (block, positions)
             for rows in (16, 128):
                 assert L.kvt_block_prefill(None, 64, 64, 0, 64, 1, None, 1, 1, 1, 64, *pool, 1, 1.0, rows, *tail[1:]) == -3
+
+
+def test_block_kernels_hold_no_instructions_in_asm(kvt_pkg):
+    """The compiler puts no wait before asm that reads a matrix product's result, so the kernels' asm is empty (a register is
+    pinned) or a wait."""
+    import os
+    import re
+    src = os.path.join(os.path.dirname(kvt_pkg._lib.__file__), "csrc")
+    for name in sorted(f for f in os.listdir(src) if f.startswith("block_")):
+        with open(os.path.join(src, name)) as f:
+            for text in re.findall(r"\basm\b(?:\s+volatile)?\s*\(\s*((?:\"[^\"]*\"\s*)+)", f.read()):
+                assert re.fullmatch(r'"(s_waitcnt vmcnt\(0\))?"\s*', text), (name, text)

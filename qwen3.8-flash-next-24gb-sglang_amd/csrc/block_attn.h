@@ -83,6 +83,10 @@ KVT_DEV h2 h2_rne(float a, float b) { return __builtin_convertvector((f2){a, b},
 KVT_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }   // (v_exp_f32: results below 2^-126 are 0)
 KVT_DEV float bits_f(uint32_t u) { return __uint_as_float(u); }
 
+// A row that sees a position of a block with a scale that is not finite is NaN, in every channel; to other rows such a block is one
+// that is not there, so that no 0 * NaN of a position that they do not see reaches them.  (Scales are >= 0.)
+KVT_DEV bool finite_scales(float k, float v) { return max(__float_as_uint(k) << 1, __float_as_uint(v) << 1) < 0xFF000000u; }
+
 // O's unit becomes the V scale fv > 0, but no less than 2^-80 of the largest so far (|O| in units of that is below 2^40, so
 // it stays finite); returns the factor for O.
 KVT_DEV float new_unit(float fv, float& unit, float& peak) {

@@ -106,6 +106,7 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
 #pragma unroll
   for (int c = 0; c < VB; ++c) acc[c] = f4{0, 0, 0, 0};
   float m = -__builtin_inff(), sum = 0.0f, unit = 0.0f, peak = 0.0f;
+  int poison = 0x7FFFFFFF;            // the wavefront's first position whose block has a scale that is not finite (uniform)
 
   const uint32_t koff = (uint32_t)l * D + 16u * g, voff = 4u * g * D + (uint32_t)l * VB;
   const int64_t tbl = (int64_t)it.trow * P.stride;
@@ -119,6 +120,11 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
       if (p < it.limit) id = P.table[tbl + (p >> P.log2b)];
       if (id < 0 || id >= P.n_blocks) id = -1;
       if (id >= 0) sk = P.ks[(int64_t)id * P.H + h], sv = P.vs[(int64_t)id * P.H + h];
+      const uint64_t bad = __ballot(!finite_scales(sk, sv));
+      if (bad) {                                                    // (lanes are in the order of positions)
+        poison = min(poison, __builtin_amdgcn_readlane(p, __builtin_ctzll(bad)));
+        if (bad >> lane & 1) id = -1, sk = sv = 0.0f;
+      }
     }
     for (int i = 0; i < 32; ++i) {
       const int tile = base + i * kWaves;
@@ -236,6 +242,7 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
 
   // the wavefronts' parts -> one: acc[c][i] is channel VB (4 g + i) + c of row l
   sum = sum_xor16_32(sum);
+  if (poison < see) sum = __builtin_nanf("");
   if (live) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)

@@ -71,7 +71,8 @@ template <int D>
 struct __align__(16) Buf {
   uint8_t k[Tile<D>::T * Tile<D>::KP];
   uint8_t v[D * Tile<D>::VP];
-  float scale[Tile<D>::T / 32][4];              // of K in the two halves of 32 positions (-1: no such block), and of V
+  // of K in the two halves of 32 positions (-1: no such block, NaN: one with a scale that is not finite), and of V
+  float scale[Tile<D>::T / 32][4];
 };
 
 // A thread's share of a tile as loaded: pieces of one K row, and 4 channels of 8 positions of V.
@@ -170,13 +171,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
     }
   };
   const auto convert_v = [&](int tile, int id, RawV& r, Buf<D>& b) {
+    const bool fin = finite_scales(r.ks, r.vs), ok = in_pool(id) && fin;
     if ((T == 64 || !(wave & 1)) && lane == 0) {
       float* to = b.scale[sub >> 1] + (sub & 1);
-      to[0] = in_pool(id) ? r.ks : -1.0f;
-      to[2] = in_pool(id) ? r.vs : 0.0f;
+      to[0] = ok ? r.ks : in_pool(id) ? __builtin_nanf("") : -1.0f;
+      to[2] = ok ? r.vs : 0.0f;
     }
     if (!has_v) return;
-    const int left = in_pool(id) ? it.limit - (tile * T + 16 * sub) : 0;   // positions behind the last one, or in no block: 0
+    const int left = ok ? it.limit - (tile * T + 16 * sub) : 0;   // positions behind the last one, or in no block: 0
     if (left < 16) {
       const int mine = left - (vrow & 15);
 #pragma unroll
@@ -207,6 +209,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
   float m = -__builtin_inff(), lift = 0x1p120f, sum = 0.0f, part = 0.0f;   // (part: of the sum, in units of ru)
   float unit = 0.0f, peak = 0.0f, ru = 0.0f, log_ru = 0.0f, per_ru = 1.0f;   // uniform, as the next two
   int last = -1, lost = 0;
+  int poison = 0x7FFFFFFF;                       // the first position whose block has a scale that is not finite (uniform)
 
   if (tile0 < tile1) {
     RawK<D> rk;
@@ -276,11 +279,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
         const float ks[2] = {uniform(scale[0]), uniform(scale[1])}, vs[2] = {uniform(scale[2]), uniform(scale[3])};
         // (the factors are positive, so the largest score of a half is its largest product times the factor)
         float f[2] = {qf * ks[0], qf * ks[1]};
-        if (p0 + 32 > all_see || ks[0] < 0.0f || ks[1] < 0.0f) {
+        if (p0 + 32 > all_see || !(ks[0] >= 0.0f) || !(ks[1] >= 0.0f)) {
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            const int seen = ks[s] < 0.0f ? 0 : see;
-            f[s] = f[s] < kLeast ? kLeast : f[s];
+            if (ks[s] != ks[s]) poison = min(poison, p0 + 16 * s);
+            const int seen = ks[s] >= 0.0f ? see : 0;
+            f[s] = f[s] >= kLeast ? f[s] : kLeast;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               sc[8 * s + j] = p0 + 16 * s + 8 * (j >> 2) + 4 * g + (j & 3) < seen ? sc[8 * s + j] : -__builtin_inff();
@@ -356,6 +360,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
 
   // register i of acc[c]: channel 32 c + 8 (i / 4) + 4 g + i % 4 of row l
   sum = sum_xor32(fmaf(part, per_ru, sum));
+  if (poison < see) sum = __builtin_nanf("");
   int row = again(l);                           // (its query and head are computed again: no registers for them till now)
   row += 32 * wave;
   if (row >= it.n_row) return;

@@ -345,7 +345,8 @@ int kvt_block_store(const void* k, const void* v, int dtype, int64_t sk_n, int64
  * > 0.  q (q_type 0 bf16, 1 fp16) and out (out_type 0 bf16, 1 fp16, 2 fp32) are [n, Hq, D] with element strides of token and
  * head and unit last stride, rows 16-byte aligned.  Hq / H <= 16, n <= 4,096, max_blocks * block <= 2^31 - 8,192 (else
  * KVT_ERANGE).  ks, vs >= 0: rows that see a position of a block with a scale that is not finite are NaN, others are not
- * touched by it.  A request without positions gives NaN (0/0).
+ * touched by it; nor do NaN codes (e4m3) reach rows that do not see their position.  A request without positions gives NaN
+ * (0/0).
  * n_splits 1: a workgroup per request and KV head.  n_splits > 1 (at most 1,024; n * H <= 65,535 then): up to n_splits
  * workgroups for each; parts as fp32 in part_o [n * H * n_splits * 16 * D] and part_ml [n * H * n_splits * 32].  n_splits < -1
  * (at least -65,535): |n_splits| workgroups share all positions of the call equally; part_o [|n_splits| * 32 * D], part_ml

@@ -87,6 +87,48 @@ KVT_DEV float bits_f(uint32_t u) { return __uint_as_float(u); }
 // that is not there, so that no 0 * NaN of a position that they do not see reaches them.  (Scales are >= 0.)
 KVT_DEV bool finite_scales(float k, float v) { return max(__float_as_uint(k) << 1, __float_as_uint(v) << 1) < 0xFF000000u; }
 
+// NaN codes of V (e4m3) in tiles that some row of a workgroup does not see to their end: a product would take them to all of its
+// rows, as 0 * NaN.  They are taken out of the codes, and what remains is the first position where each channel has one:
+// a row sees positions 0 .. n - 1, so the channel is NaN for it where that position is below n.
+template <int CODE, int D>
+struct NanAt {
+  int at[CODE == kE4M3 ? D : 1], found;
+  KVT_DEV void clear() {                        // (every thread of a workgroup, and a barrier before the first take)
+    for (int i = threadIdx.x; i < D; i += 256) at[i] = 0x7FFFFFFF;
+    if (threadIdx.x == 0) found = 0;
+  }
+  KVT_DEV bool any() const { return found != 0; }
+  // N dwords of codes: dword i has channels ch + step i .. + 3 of position pos(i).
+  template <int N, class Pos>
+  KVT_DEV void take(uint32_t (&w)[N], Pos pos, int ch, int step = 0) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) any |= (w[i] & 0x7F7F7F7Fu) + 0x01010101u;
+    if (!(any & 0x80808080u)) return;
+    found = 1;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t nan = ((w[i] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c)
+        if (nan >> (8 * c + 7) & 1) atomicMin(&at[ch + step * i + c], pos(i));
+      w[i] &= ~((nan >> 7) * 0xFFu);
+    }
+  }
+  // Converted codes of channels ch .. + 3 in LDS, rows of `pitch` bytes: positions pos .. + 3, + 8 .. + 11.
+  KVT_DEV void take_f16(uint8_t* p, int pitch, int pos, int ch) {
+    found = 1;
+#pragma unroll 1
+    for (int k = 0; k < 32; ++k) {
+      uint16_t* x = reinterpret_cast<uint16_t*>(p + (k >> 3) * pitch) + (k & 7);
+      if ((*x & 0x7FFF) > 0x7C00) {
+        atomicMin(&at[ch + (k >> 3)], pos + (k & 7) + (k & 4));
+        *x = 0;
+      }
+    }
+  }
+};
+
 // O's unit becomes the V scale fv > 0, but no less than 2^-80 of the largest so far (|O| in units of that is below 2^40, so
 // it stays finite); returns the factor for O.
 KVT_DEV float new_unit(float fv, float& unit, float& peak) {

@@ -75,19 +75,20 @@ KVT_DEV float lane_f(float v, int lane) {
   return bits_f((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
 }
 
-// The wavefronts' results: O (rows x channels), maximum, sum, unit.
-template <int D>
+// The wavefronts' results: O (rows x channels), maximum, sum, unit; NaN codes of V.
+template <int CODE, int D>
 struct Join {
   float o[kWaves][16][D + 4];
   float m[kWaves][16], l[kWaves][16], u[kWaves];
   float w[16][kFew];           // (weights of the splits of a row, where the launch merges them)
+  NanAt<CODE, D> nans;
   int last;
 };
 
 // Tiles tile0 .. tile1 - 1 of an item and KV head: into out where they are all that the item has (whole), else as part
-// `slot`: its own result with its maximum and sum.
-template <int CODE, int QT, int D>
-KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, bool whole, int64_t slot, int ot, Join<D>& J) {
+// `slot`: its own result with its maximum and sum.  CHUNK: its rows may see different positions.
+template <int CODE, int QT, int D, bool CHUNK>
+KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, bool whole, int64_t slot, int ot, Join<CODE, D>& J) {
   constexpr int NC = D / 64;          // 16-byte chunks of a K row per lane
   constexpr int VB = D / 16;          // bytes (channels) of a V row per lane
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
@@ -106,7 +107,7 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
 #pragma unroll
   for (int c = 0; c < VB; ++c) acc[c] = f4{0, 0, 0, 0};
   float m = -__builtin_inff(), sum = 0.0f, unit = 0.0f, peak = 0.0f;
-  int poison = 0x7FFFFFFF;            // the wavefront's first position whose block has a scale that is not finite (uniform)
+  int poison = 0x7FFFFFFF;            // the wavefront's first position whose block has a V scale that is not finite (uniform)
 
   const uint32_t koff = (uint32_t)l * D + 16u * g, voff = 4u * g * D + (uint32_t)l * VB;
   const int64_t tbl = (int64_t)it.trow * P.stride;
@@ -120,11 +121,6 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
       if (p < it.limit) id = P.table[tbl + (p >> P.log2b)];
       if (id < 0 || id >= P.n_blocks) id = -1;
       if (id >= 0) sk = P.ks[(int64_t)id * P.H + h], sv = P.vs[(int64_t)id * P.H + h];
-      const uint64_t bad = __ballot(!finite_scales(sk, sv));
-      if (bad) {                                                    // (lanes are in the order of positions)
-        poison = min(poison, __builtin_amdgcn_readlane(p, __builtin_ctzll(bad)));
-        if (bad >> lane & 1) id = -1, sk = sv = 0.0f;
-      }
     }
     for (int i = 0; i < 32; ++i) {
       const int tile = base + i * kWaves;
@@ -136,10 +132,10 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const int b = __builtin_amdgcn_readlane(id, 2 * i + s);
-        valid[s] = b < 0 ? 0 : min(max(it.limit - (p0 + 16 * s), 0), 16);
         const int64_t at = ((((int64_t)max(b, 0) * P.H + h) << P.log2b) + ((p0 + 16 * s) & ((1 << P.log2b) - 1))) * D;
         kp[s] = P.k8 + at, vp[s] = P.v8 + at;
         fk[s] = lane_f(sk, 2 * i + s), fv[s] = lane_f(sv, 2 * i + s);
+        valid[s] = b < 0 ? 0 : min(max(it.limit - (p0 + 16 * s), 0), 16);
       }
       Raw<16> kr[2][NC];
       Raw<VB> vr[2][4];
@@ -161,7 +157,7 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
           sc = mfma(operand<CODE>(kr[s][c].w[0], kr[s][c].w[1]), Q[2 * c], sc);
           sc = mfma(operand<CODE>(kr[s][c].w[2], kr[s][c].w[3]), Q[2 * c + 1], sc);
         }
-        const float f = qf * fk[s];
+        const float f = fmaf(qf, fk[s], fk[s] - fk[s]);            // (NaN for a scale that is not finite)
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[s][j] = sc[j] * f;
       }
@@ -176,6 +172,13 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
 #pragma unroll
             for (int d = 0; d < VB / 4; ++d) vr[s][j].w[d] = at < valid[s] ? vr[s][j].w[d] : 0u;
           }
+        if (CHUNK && CODE == kE4M3 && P.causal) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              J.nans.template take<VB / 4>(vr[s][j].w, [&](int) { return p0 + 16 * s + 4 * g + j; }, l * VB, 4);
+        }
       }
       float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
                         fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
@@ -200,11 +203,19 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
       // (two blocks whose scales are far apart in one tile: one product for each, so that neither's weights leave fp16)
       const bool far = fminf(fv[0], fv[1]) > 0.0f && (fv[0] < 0.25f * fv[1] || fv[1] < 0.25f * fv[0]);
       for (int pass = 0; pass <= (int)far; ++pass) {
-        const float big = far ? fv[pass] : fmaxf(fv[0], fv[1]);
-        if (big > unit || (big > 0.0f && big < 0.25f * unit)) {     // uniform
-          const float a = new_unit(big, unit, peak);
+        float big = far ? fv[pass] : __builtin_elementwise_maximum(fv[0], fv[1]);
+        if (!(big <= unit) || (big > 0.0f && big < 0.25f * unit)) { // uniform
+          if (!finite_scales(big, big)) {
 #pragma unroll
-          for (int c = 0; c < VB; ++c) acc[c] *= a;
+            for (int s = 0; s < 2; ++s)
+              if (!finite_scales(fv[s], fv[s])) poison = min(poison, p0 + 16 * s), fv[s] = 0.0f;
+            big = fmaxf(fv[0], fv[1]);
+          }
+          if (big > 0.0f) {
+            const float a = new_unit(big, unit, peak);
+#pragma unroll
+            for (int c = 0; c < VB; ++c) acc[c] *= a;
+          }
         }
         h8 p;
 #pragma unroll
@@ -269,6 +280,12 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
     const float per = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) O += *reinterpret_cast<const f4*>(&J.o[v][row][d]) * (f[v] * per) * J.u[v];
+    if (CHUNK && CODE == kE4M3 && P.causal && J.nans.any()) {
+      const int seen = sees(P, it, (it.row0 + row) / P.gs);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (J.nans.at[d + i] < seen) O[i] = __builtin_nanf("");
+    }
     if (whole) {
       const int at = it.row0 + row;
       const int64_t o = (int64_t)(it.q0 + at / P.gs) * P.so_n + (int64_t)(h * P.gs + at % P.gs) * P.so_h + d;
@@ -297,9 +314,9 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
 //
 // A thread has four channels of a row at a time, and loads them of 16 parts at once: of its first row beside the parts' maxima.
 // Most items have no more parts (MANY: they may, D 64 and 128; at D 256 the registers would spill).
-template <int D, bool MANY>
+template <int CODE, int D, bool MANY>
 KVT_DEV void merge_last(const Attn& P, const Item& it, int h, int64_t item, int parts, int64_t s0, int64_t sb, int step, int ot,
-                        Join<D>& J) {
+                        Join<CODE, D>& J) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();                                  // every thread's parts have arrived
   if (threadIdx.x == 0) {
@@ -390,7 +407,7 @@ KVT_DEV void merge_last(const Attn& P, const Item& it, int h, int64_t item, int 
 
 template <int CODE, int QT, int D>
 __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot) {
-  __shared__ Join<D> J;
+  __shared__ Join<CODE, D> J;
   const int split = blockIdx.x, h = blockIdx.y, w = blockIdx.z;
   const Item it = item_of(P, w);
   if (it.n_row == 0) return;
@@ -399,8 +416,12 @@ __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot
   const int used = splits_used(P, it.limit);
   if (split >= used) return;                        // (the merge knows which splits there are)
   const int64_t item = (int64_t)w * P.H + h;
-  attend<CODE, QT, D>(P, it, h, tile0, tile1, used == 1, item * P.splits + split, ot, J);
-  if (P.counters && used > 1) merge_last<D, false>(P, it, h, item, used, item * P.splits, item * P.splits, 1, ot, J);
+  if (CODE == kE4M3 && P.causal) {
+    J.nans.clear();
+    __syncthreads();
+  }
+  attend<CODE, QT, D, true>(P, it, h, tile0, tile1, used == 1, item * P.splits + split, ot, J);
+  if (P.counters && used > 1) merge_last<CODE, D, false>(P, it, h, item, used, item * P.splits, item * P.splits, 1, ot, J);
 }
 
 // Decode in equal shares of all tiles of a call: the (request, KV head) pairs stand in a line, each as long as its tiles plus
@@ -476,7 +497,7 @@ KVT_DEV uint32_t share_of(const Attn& P, uint32_t total) {
 
 template <int CODE, int QT, int D>
 __global__ __launch_bounds__(256, 2) void block_decode_kernel(const Attn P, int ot) {
-  __shared__ Join<D> J;
+  __shared__ Join<CODE, D> J;
   const uint32_t w = blockIdx.x;
   const Line s = line_of(P, [&](uint32_t total, uint32_t before, uint32_t own, int) {
     const uint32_t x = w * share_of(P, total);
@@ -502,10 +523,10 @@ __global__ __launch_bounds__(256, 2) void block_decode_kernel(const Attn P, int 
       const int t1 = (int)min((uint64_t)(x1 - a) << P.shift, (uint64_t)tiles);
       if (t0 < t1 || (tiles == 0 && a >= x0)) {
         const bool whole = t0 == 0 && t1 == tiles;
-        attend<CODE, QT, D>(P, it, h, t0, t1, whole, 2 * (int64_t)w + (a > x0), ot, J);
+        attend<CODE, QT, D, false>(P, it, h, t0, t1, whole, 2 * (int64_t)w + (a > x0), ot, J);
         if (D < 256 && P.counters && !whole) {// (at D 256 the merge's registers would spill)
           const int w0 = (int)(a / share), w1 = (int)((a + (uint32_t)((tiles - 1) >> P.shift)) / share);
-          merge_last<D, (D < 256)>(P, it, h, (int64_t)r * P.H + h, w1 - w0 + 1, 2 * (int64_t)w0 + (a > (uint32_t)w0 * share),
+          merge_last<CODE, D, (D < 256)>(P, it, h, (int64_t)r * P.H + h, w1 - w0 + 1, 2 * (int64_t)w0 + (a > (uint32_t)w0 * share),
                                    2 * (int64_t)w0, 2, ot, J);
         }
         __syncthreads();                            // (J is free again)

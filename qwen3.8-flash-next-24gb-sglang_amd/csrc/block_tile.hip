@@ -92,6 +92,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
   constexpr int kAhead = D == 256 ? 2 : 4;     // operands read ahead of their product (what the registers hold)
   __shared__ Buf<D> buf[2];
   __shared__ h8 qlds[C::QL ? C::QL : 1][256];
+  __shared__ NanAt<CODE, D> nans;
   const int tid = threadIdx.x, lane = tid & 63, l = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // head fastest: with H = 2, 4 or 8 the workgroups of a head share the caches of the same XCDs; the last rows, which see
@@ -104,6 +105,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
   const int used = splits_used(P, it.limit);
   if (split >= used) return;
 
+  const int fewest = uniform(sees(P, it, it.row0 / P.gs));             // positions that every row of the workgroup sees
+  if (CODE == kE4M3) {                         // (the first tile is searched for NaN codes only if it ends behind those)
+    nans.clear();
+    if (tile0 * T + T > fewest) __syncthreads();
+  }
   const int my = it.row0 + 32 * wave + l;
   const bool live = 32 * wave + l < it.n_row;
   constexpr int QR = D / 16 - C::QL;
@@ -117,8 +123,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
   const int see = live ? sees(P, it, my / P.gs) : 0;
   const int first_row = it.row0 + 32 * wave, last_row = it.row0 + min(32 * wave + 31, it.n_row - 1);
   const bool any_row = 32 * wave < it.n_row;
-  const int all_see = any_row ? sees(P, it, first_row / P.gs) : 0;   // positions that every row of the wavefront sees
-  const int most_see = any_row ? sees(P, it, last_row / P.gs) : 0;   // and that any of them sees
+  const int all_see = uniform(any_row ? sees(P, it, first_row / P.gs) : 0);   // positions that every row of the wavefront sees
+  const int most_see = uniform(any_row ? sees(P, it, last_row / P.gs) : 0);   // and that any of them sees
 
   // This thread's share of a tile: 16-byte pieces tid % TPK, + TPK, .. of K row tid / TPK; channels vd .. vd + 3 of V rows vrow +
   // {0 .. 3, 8 .. 11}.  A wavefront's rows all lie in the 16 positions `sub` of the tile, i.e. in one block: its id and the
@@ -170,7 +176,20 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
       to[1] = operand<CODE>(r.c[i].z, r.c[i].w);
     }
   };
-  const auto convert_v = [&](int tile, int id, RawV& r, Buf<D>& b) {
+  // NaN codes of V in a tile that some row does not see to its end (this thread's share, read back from LDS).
+  const auto nans_of = [&](int tile, Buf<D>& b) {
+    const int lz = again(lane), d = 4 * ((lz >> 1) + (T == 32 ? 32 * (wave & 1) : 0));
+    uint8_t* p = b.v + d * C::VP + 16 * C::piece(d, 2 * sub + (lz & 1));
+    uint32_t any = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const u4v w = *reinterpret_cast<u4v*>(p + c * C::VP);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) any |= (w[i] & 0x7FFF7FFFu) + 0x03FF03FFu;
+    }
+    if (any & 0x80008000u) nans.take_f16(p, C::VP, tile * T + 16 * sub + 4 * (lz & 1), d);
+  };
+  const auto convert_v = [&](int tile, int id, RawV& r, Buf<D>& b, bool checked) {
     const bool fin = finite_scales(r.ks, r.vs), ok = in_pool(id) && fin;
     if ((T == 64 || !(wave & 1)) && lane == 0) {
       float* to = b.scale[sub >> 1] + (sub & 1);
@@ -201,6 +220,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
       }
       *reinterpret_cast<h8*>(b.v + (vd + c) * C::VP + 16 * C::piece(vd, vc)) = h8{y[0].x, y[0].y, y[1].x, y[1].y, y[2].x, y[2].y, y[3].x, y[3].y};
     }
+    if (checked) nans_of(tile, b);
   };
 
   f16v acc[DT];
@@ -218,10 +238,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
     fetch_k(tile0, id, rk);
     fetch_v(tile0, id, rv);
     convert_k(rk, buf[0]);
-    convert_v(tile0, id, rv, buf[0]);
+    convert_v(tile0, id, rv, buf[0], CODE == kE4M3 && tile0 * T + T > fewest);
     int then = id_at(tile0 + 1);
     __syncthreads();
-    for (int tile = tile0; tile < tile1; ++tile) {
+    const auto step = [&](int tile, bool checked) __attribute__((always_inline)) {
       const Buf<D>& b = buf[(tile - tile0) & 1];
       Buf<D>& next = buf[(tile + 1 - tile0) & 1];
       // the next tile's codes (behind the last tile: the block of its last position again, unused)
@@ -282,7 +302,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
         if (p0 + 32 > all_see || !(ks[0] >= 0.0f) || !(ks[1] >= 0.0f)) {
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            if (ks[s] != ks[s]) poison = min(poison, p0 + 16 * s);
+            if (ks[s] != ks[s]) poison = uniform(min(poison, p0 + 16 * s));
             const int seen = ks[s] >= 0.0f ? see : 0;
             f[s] = f[s] >= kLeast ? f[s] : kLeast;
 #pragma unroll
@@ -353,9 +373,17 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
         }
       }
       if (!kApart) convert_k(rk, next);
-      convert_v(tile + 1, id, rv, next);
+      convert_v(tile + 1, id, rv, next, checked);
       __syncthreads();
-    }
+    };
+    // Tiles that some row does not see to their end are the last few: only those (each as the next tile, behind the products) are
+    // searched for NaN codes, in a loop of their own.  In one loop the search takes registers that spill at D = 256 (10,001
+    // tokens 912 -> 933 us).
+    const int plain = CODE == kE4M3 ? min(max(fewest / T - 1, tile0), tile1) : tile1;
+    int tile = tile0;
+    for (; tile < plain; ++tile) step(tile, false);
+    if (CODE == kE4M3)
+      for (; tile < tile1; ++tile) step(tile, true);
   }
 
   // register i of acc[c]: channel 32 c + 8 (i / 4) + 4 g + i % 4 of row l
@@ -366,6 +394,16 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
   if (row >= it.n_row) return;
   const int qi = (it.row0 + row) / P.gs, hq = h * P.gs + (it.row0 + row) % P.gs;
   const float f = sum == 0.0f ? 0.0f : unit / sum;
+  if (CODE == kE4M3 && nans.any()) {
+    const int seen = sees(P, it, qi), gz = again(lane) >> 5;
+#pragma unroll
+    for (int c = 0; c < DT; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (nans.at[32 * c + 8 * (i >> 2) + 4 * gz + (i & 3)] < seen) acc[c][i] = __builtin_nanf("");
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+  }
   if (used == 1) {
     const int64_t o = (int64_t)(it.q0 + qi) * P.so_n + (int64_t)hq * P.so_h + 4 * g;
     const float nan = sum == 0.0f ? __builtin_nanf("") : 0.0f;

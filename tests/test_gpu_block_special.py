@@ -82,3 +82,60 @@ def test_scales_that_are_not_finite_in_parts(kvt_pkg, monkeypatch, kernel, split
 def test_scales_that_are_not_finite_cross(kvt_pkg, monkeypatch, kernel):
     """Without the causal mask every query of the request sees the block."""
     _check(monkeypatch, kernel, "int8", 4, 4, 64, 32, [33, 40], [100, 77], {(1, 2): (None, NAN)}, causal=False, seed=2)
+
+
+@pytest.mark.parametrize("kernel", ["decode", 16, 128])
+@pytest.mark.parametrize("Hq,H,D,B", [(2, 2, 64, 16), (8, 2, 128, 64), (16, 2, 256, 32)])
+@pytest.mark.parametrize("splits", [None, 1, 3])
+def test_nan_codes_reach_the_rows_that_see_them(kvt_pkg, monkeypatch, kernel, Hq, H, D, B, splits):
+    """NaN codes of K and of V (e4m3) inside a causal chunk: a NaN in V makes its channel NaN for the queries from its position on,
+    one in K every channel; earlier queries of the same tile are what they are without it."""
+    from kvtier import block_kv
+    if kernel != "decode":
+        monkeypatch.setattr(block_kv, "_TILE_MIN", {D: 0 if kernel == 128 else 10 ** 9})
+    lens = [70, 200, 333, 5, 40]
+    new = [1] * 5 if kernel == "decode" else [70, 150, 9, 5, 1]
+    g = torch.Generator().manual_seed(D)
+    table, nb = _tables(lens, B, 2, D)
+    codes, sc = _pool("fp8", nb, H, B, D, g)
+    cu, causal = prefix(new), kernel != "decode"
+    q = torch.randn(cu[-1], Hq, D, generator=g).to(torch.bfloat16)
+    # (request, position, channel or None for K): in the first tile, at tile borders, near and at the end, twice in a channel
+    spots = [(0, 0, 3), (0, 63, 5), (0, 64, 0), (0, 69, D - 1), (0, 20, 3), (0, 11, None), (1, 51, 7), (1, 100, 7), (1, 128, 8),
+             (1, 199, 9), (1, 170, None), (2, 332, 1), (2, 326, 2), (2, 5, 4), (3, 4, 0), (4, 39, 60)]
+    bits = [c.clone().view(torch.uint8) for c in codes]
+    for j, (r, p, d) in enumerate(spots):
+        at = (table[r][p // B], 0, p % B)
+        codes[d is not None].view(torch.uint8)[at][d or 0] = 0
+        bits[d is not None][at][d or 0] = 0x7F if j % 2 else 0xFF
+    val = [ref.values(codes[i]) * sc[i].double()[..., None, None] for i in range(2)]
+    want = list(ref.attention(q.double(), cu, lens, range(len(new)), table, val[0], val[1], causal, D ** -0.5))
+    t = 0
+    for r, n in enumerate(new):
+        for s in _sees([n], [lens[r]], causal):
+            for b, p, d in spots:
+                if b == r and p < s:
+                    want[0][t, :Hq // H, slice(None) if d is None else d] = math.nan
+            t += 1
+    args = [b.view(torch.float8_e4m3fn).to(dev) for b in bits] + [s.to(dev) for s in sc] + [i32(table), i32(lens)]
+    if kernel == "decode":
+        got = block_kv.kvt_block_decode(q.to(dev), *args, splits=splits)
+    else:
+        got = block_kv.kvt_block_prefill(q.to(dev), i32(cu), *args, splits=splits)
+    # (a zero code for a NaN changes the other channels of rows that see it only through K, and those rows are NaN)
+    ref.close(got, *want, D)
+
+
+def test_a_nan_row_that_is_appended(kvt_pkg):
+    """Through the cache: a token whose V is NaN leaves the queries before it, of its own prompt and of others, finite."""
+    from kvtier import block_kv
+    c = block_kv.BlockKVCache(1, 2, 128, n_blocks=20, max_seqs=2, max_blocks=10, block=32)
+    rows = [c.add_seq(), c.add_seq()]
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = torch.randn(2, 150, 2, 128, device=dev, generator=g).to(torch.bfloat16)
+    x[1, 80] = math.nan
+    q = torch.randn(150, 8, 128, device=dev, generator=g).to(torch.bfloat16)
+    plan = c.plan(rows, [100, 50])
+    c.append(0, plan, x[0], x[1])
+    bad = torch.isnan(c.prefill(0, plan, q)).flatten(1)
+    assert not bad[:80].any() and bad[80:100].all() and not bad[100:].any()

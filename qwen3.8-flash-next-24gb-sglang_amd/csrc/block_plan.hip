@@ -95,7 +95,7 @@ __global__ __launch_bounds__(kThreads) void block_plan_kernel(const Plan P) {
   int len = 0, count = 0;
   if (row >= 0) {
     len = max(P.seq_lens[row], 0);
-    count = min(max(P.counts[j], 0), P.n_tokens);
+    count = max(P.counts[j], 0);     // (the sums are 64 bits: not cut to n_tokens before kTokensOver is looked for)
   }
   const int64_t upto = block_scan(count, S.sums[0]);
   const int c1 = (int)min(upto, (int64_t)P.n_tokens), c0 = (int)min(upto - count, (int64_t)P.n_tokens);

@@ -104,6 +104,14 @@ def test_plan_of_nothing(kvt_pkg):
     _run_plan(_plan_case(3, 64, [5, 0, 64], [0, 0, 0], 2, 3, 4, 3), 0, 64)
 
 
+@pytest.mark.parametrize("counts,n_tokens", [([100], 60), ([0, 100, 0], 60), ([0, 0, 7], 0), ([2 ** 31 - 1] * 3, 50),
+                                             ([50, 0, 1], 50), ([30, -5, 20], 50)])
+def test_plan_of_more_tokens_than_it_is_given(kvt_pkg, counts, n_tokens):
+    """One request alone over n_tokens, none of the others with a token, no room at all; and counts that just fit."""
+    n = len(counts)
+    _run_plan(_plan_case(n, 16, [5, 0, 16][:n], counts, 30, 4, 40, 5), n_tokens, 16)
+
+
 # ------------------------------------------------------------------------------------------------------------ store
 def _tables(kv_lens, B, extra, seed):
     rng = random.Random(seed)

@@ -110,7 +110,7 @@ __global__ __launch_bounds__(kThreads) void block_plan_kernel(const Plan P) {
     S.cu[j + 1] = c1;
     S.len[j] = len;
     S.base[j] = (int)min(taken - opens, (int64_t)P.n_free) - first;
-    int f = (bad ? kBadRow : 0) | (upto > P.n_tokens ? kTokensOver : 0) | (last > P.max_blocks ? kRowFull : 0) |
+    int f = (bad ? kBadRow : 0) | (upto > P.n_tokens ? kTokensOver : 0) | (c1 > c0 && last > P.max_blocks ? kRowFull : 0) |
             (head + taken > P.n_free ? kPoolShort : 0);
     if (f) atomicOr(&S.flags, f);
   }

@@ -112,6 +112,15 @@ def test_plan_of_more_tokens_than_it_is_given(kvt_pkg, counts, n_tokens):
     _run_plan(_plan_case(n, 16, [5, 0, 16][:n], counts, 30, 4, 40, 5), n_tokens, 16)
 
 
+def test_plan_behind_a_full_row(kvt_pkg):
+    """A row that an earlier step ran over is reported where tokens are appended to it, not where none are."""
+    for counts, lens in (([0, 2], [70, 5]), ([1, 2], [70, 5]), ([0, 0], [64, 64])):
+        case = _plan_case(2, 16, [min(n, 64) for n in lens], counts, 4, 3, 20, 6)
+        for s, n in zip(case[0], lens):
+            case[2][s] = n
+        _run_plan(case, 4, 16)
+
+
 # ------------------------------------------------------------------------------------------------------------ store
 def _tables(kv_lens, B, extra, seed):
     rng = random.Random(seed)

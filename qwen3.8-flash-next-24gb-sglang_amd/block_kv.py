@@ -148,12 +148,20 @@ def kvt_block_plan(seqs: torch.Tensor, counts: torch.Tensor, seq_lens: torch.Ten
     return BlockPlan(seqs, cu, slots, kv_lens, next_head)
 
 
+def _strides(x: torch.Tensor):
+    """Strides of token and head; 0 for a dimension of one entry, whose stride may be anything."""
+    (n, h, _), (a, b, _) = x.shape, x.stride()
+    return a if n > 1 else 0, b if h > 1 else 0
+
+
 def _rows16(x: torch.Tensor, per16: int):
     """Rows that start at 16-byte boundaries (x itself, else a contiguous copy): tensor, pointer, strides of token and head."""
     p, (a, b, c) = x.data_ptr(), x.stride()
     if p & 15 or a % per16 or b % per16 or c != 1:
-        x = x.contiguous() if not x.is_contiguous() else x.clone()
-        p, (a, b, c) = x.data_ptr(), x.stride()
+        a, b = _strides(x)
+        if p & 15 or a % per16 or b % per16 or c != 1:
+            x = x.contiguous() if not x.is_contiguous() else x.clone()
+            p, (a, b) = x.data_ptr(), _strides(x)
     return x, p, a, b
 
 
@@ -219,9 +227,11 @@ def _attn_args(q, out, H, D):
     if H == 0 or Hq == 0 or Hq % H or Hq // H > 16:
         raise ValueError(f"{Hq} q heads over {H} KV heads: a multiple, at most 16 each, is served")
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    assert out.shape == q.shape and out.dtype in _lib.DTYPE_CODE and out.stride(2) == 1
-    return (*_rows16(q, 8), out, Hq)
+        out, so = torch.empty_like(q, memory_format=torch.contiguous_format), (Hq * D, D)
+    else:
+        assert out.shape == q.shape and out.dtype in _lib.DTYPE_CODE and out.stride(2) == 1
+        so = _strides(out)
+    return (*_rows16(q, 8), out, so, Hq)
 
 
 def _splits(items: int, cap: int, blocks: int, least: int = 128) -> int:
@@ -244,7 +254,7 @@ def kvt_block_decode(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: to
     as long as it is replayed, and one made before the capture is the faster one.  The results do not depend on it."""
     n = kv_lens.numel()
     nb, H, B, D = _pool(k8, v8, ks, vs, block_table, n, seqs)
-    q, qp, qn, qh, out, Hq = _attn_args(q, out, H, D)
+    q, qp, qn, qh, out, so, Hq = _attn_args(q, out, H, D)
     if q.shape[0] != n:
         raise ValueError(f"{q.shape[0]} queries for {n} requests")
     _i32("kv_lens", kv_lens, n)
@@ -266,7 +276,7 @@ def kvt_block_decode(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: to
     _lib.call("kvt_block_decode", qp, qn, qh, _lib.DTYPE_CODE[q.dtype], kv_lens.data_ptr(), n, H, Hq, D, CODE[k8.dtype],
               k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B, block_table.data_ptr(), block_table.stride(0),
               *block_table.shape, _lib.ptr(seqs), D ** -0.5 if scale is None else float(scale), ns, o, ml, counters,
-              out.data_ptr(), _lib.DTYPE_CODE[out.dtype], out.stride(0), out.stride(1), st)
+              out.data_ptr(), _lib.DTYPE_CODE[out.dtype], *so, st)
     return out
 
 
@@ -283,7 +293,7 @@ def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8:
     NaN (0/0).  Other arguments as kvt_block_decode."""
     n = kv_lens.numel()
     nb, H, B, D = _pool(k8, v8, ks, vs, block_table, n, seqs)
-    q, qp, qn, qh, out, Hq = _attn_args(q, out, H, D)
+    q, qp, qn, qh, out, so, Hq = _attn_args(q, out, H, D)
     _i32("kv_lens", kv_lens, n)
     _i32("cu_q", cu_q, n + 1)
     total = q.shape[0]
@@ -311,7 +321,7 @@ def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8:
               D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B, block_table.data_ptr(),
               block_table.stride(0), *block_table.shape, _lib.ptr(seqs), int(bool(causal)),
               D ** -0.5 if scale is None else float(scale), rows, ns, o, ml, counters, out.data_ptr(),
-              _lib.DTYPE_CODE[out.dtype], out.stride(0), out.stride(1), st)
+              _lib.DTYPE_CODE[out.dtype], *so, st)
     return out
 
 

@@ -176,3 +176,22 @@ def test_block_kernels_hold_no_instructions_in_asm(kvt_pkg):
         with open(os.path.join(src, name)) as f:
             for text in re.findall(r"\basm\b(?:\s+volatile)?\s*\(\s*((?:\"[^\"]*\"\s*)+)", f.read()):
                 assert re.fullmatch(r'"(s_waitcnt vmcnt\(0\))?"\s*', text), (name, text)
+
+
+@pytest.mark.parametrize("shape,strides", [((1, 2, 64), (133, 64, 1)), ((3, 1, 64), (64, 1, 1)), ((1, 1, 64), (7, 5, 1)),
+                                           ((3, 1, 64), (72, 3, 1))])
+def test_strides_of_single_entries_do_not_matter(kvt_pkg, shape, strides):
+    """One token, or one head, out of an odd-pitched buffer is taken as it is; off a 16-byte boundary it is copied once, and the
+    copy's strides are ones that the entry points take."""
+    from kvtier import block_kv
+    buf = torch.arange(1024, dtype=torch.float32)
+    for dtype, per16 in ((torch.float16, 8), (torch.float32, 4)):
+        b = buf.to(dtype)
+        base = -b.data_ptr() % 16 // b.element_size()
+        for off in (0, 1):
+            x = b.as_strided(shape, strides, base + off)
+            y, p, sn, sh = block_kv._rows16(x, per16)
+            assert p == y.data_ptr() and p % 16 == 0 and sn % per16 == 0 and sh % per16 == 0
+            assert (y is x) == (off == 0)
+            at = y.as_strided(shape, (sn, sh, 1)) if off == 0 else y
+            assert torch.equal(at, x)

@@ -488,6 +488,34 @@ def test_attention_strided_queries_and_rows(kvt_pkg):
     assert bool(torch.isnan(got[:2]).all()) and bool(torch.isfinite(got[2]).all())
 
 
+@pytest.mark.parametrize("Hq,H,n", [(4, 2, 1), (1, 1, 3), (1, 1, 1)])
+def test_one_row_or_head_of_an_odd_buffer(kvt_pkg, Hq, H, n):
+    """Rows, queries and outputs whose dimensions of one entry have odd strides, on a 16-byte boundary and off it."""
+    from kvtier import block_kv
+    D, B = 64, 16
+    g = torch.Generator().manual_seed(31)
+
+    def odd(x, off):
+        w = x.shape[1] * D
+        buf = torch.zeros(x.shape[0] * (w + (8 if n > 1 else 5)) + off, dtype=x.dtype, device=dev)
+        t = buf.as_strided(x.shape, (w + (8 if n > 1 else 5), D if x.shape[1] > 1 else 3, 1), off)
+        return t.copy_(x)
+    x = torch.randn(2, n, H, D, generator=g).to(torch.bfloat16)
+    q = torch.randn(n, Hq, D, generator=g).to(torch.bfloat16)
+    for off in (0, 1):
+        c = block_kv.BlockKVCache(1, H, D, n_blocks=2, max_seqs=1, max_blocks=2, block=B)
+        plan = c.plan([c.add_seq()], [n])
+        c.append(0, plan, odd(x[0], off), odd(x[1], off))
+        codes, sc = (c.k8[0], c.v8[0]), (c.ks[0], c.vs[0])
+        val = [ref.values(codes[i].cpu()) * sc[i].cpu().double()[..., None, None] for i in range(2)]
+        out = odd(torch.zeros(n, Hq, D), 0)
+        got = c.prefill(0, plan, odd(q, off), out=out)
+        assert got is out
+        ref.close(got, *ref.attention(q.double(), [0, n], [n], [0], c.block_table.tolist(), val[0], val[1], True, D ** -0.5), D)
+        if n == 1:
+            assert torch.equal(c.decode(0, plan, odd(q, off), out=odd(torch.zeros(n, Hq, D), 0)), got)
+
+
 # ----------------------------------------------------------------------------------------------------- the four together
 def _step_reference(x, kv, B, H, D):
     """The cache that appending x (a list of [n, H, D] float64 per step, one sequence) leaves, as [1 + blocks] values."""

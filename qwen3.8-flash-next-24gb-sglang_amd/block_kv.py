@@ -120,7 +120,7 @@ def kvt_block_plan(seqs: torch.Tensor, counts: torch.Tensor, seq_lens: torch.Ten
     the length of `slots`, a host int >= the counts' sum.  commit=False leaves seq_lens and free_head as they are, to look
     at a plan (its status, its next_head) before it is taken: the next plan starts from the same state.
     status (int32 [1]): bits POOL_SHORT, ROW_FULL, TOKENS_OVER, BAD_ROW (a row out of range, or listed twice: the later
-    request appends nothing) are or-ed in.  At most 1,024 requests."""
+    request appends nothing) are or-ed in.  At most 1,024 requests; of none, the plan is empty."""
     n = seqs.numel()
     _i32("seqs", seqs, n)
     _i32("counts", counts, n)
@@ -140,6 +140,9 @@ def kvt_block_plan(seqs: torch.Tensor, counts: torch.Tensor, seq_lens: torch.Ten
             raise ValueError(f"req_to_token has {req_to_token.shape[0]} rows, the block table {rows}")
         rtt, rtt_stride, rtt_cols = req_to_token.data_ptr(), req_to_token.stride(0), req_to_token.shape[1]
     st = _stream(seqs, counts, seq_lens, block_table, free_list, free_head, status, req_to_token)
+    if n == 0:                                             # (an idle step: no slots, and the state as it is)
+        zero = seqs.new_zeros(1)
+        return BlockPlan(seqs, zero, seqs.new_full((n_tokens,), -1), zero[:0], free_head[:1].clamp(0, free_list.numel()))
     slots, cu, kv_lens, next_head = seqs.new_empty(n_tokens + 2 * n + 2).split_with_sizes((n_tokens, n + 1, n, 1))   # (one allocation)
     _lib.call("kvt_block_plan", n, seqs.data_ptr(), counts.data_ptr(), seq_lens.data_ptr(), rows, block_table.data_ptr(),
               block_table.stride(0), block_table.shape[1], free_list.data_ptr(), free_list.numel(), free_head.data_ptr(),

@@ -121,6 +121,26 @@ def test_plan_behind_a_full_row(kvt_pkg):
         _run_plan(case, 4, 16)
 
 
+def test_a_step_of_no_requests(kvt_pkg):
+    """An idle step: an empty plan, and calls over it that do nothing."""
+    from kvtier import block_kv
+    c = block_kv.BlockKVCache(1, 2, 64, n_blocks=4, max_seqs=2, max_blocks=2, block=16)
+    c.plan([c.add_seq()], [20])
+    none = i32([])
+    for n_tokens in (0, 3):
+        before = [t.clone() for t in (c.block_table, c.seq_lens, c.free_head)]
+        p = c.plan(none, none, n_tokens=n_tokens)
+        assert p.cu.tolist() == [0] and p.slots.tolist() == [-1] * n_tokens and p.kv_lens.tolist() == [] and p.next_head.tolist() == [2]
+        x = torch.randn(n_tokens, 2, 64, device=dev)
+        c.append(0, p, x, x)
+        assert c.decode(0, p, x[:0].half()).shape == (0, 2, 64)
+        assert c.prefill(0, p, x.half()).shape == (n_tokens, 2, 64)
+        assert all(torch.equal(a, b) for a, b in zip(before, (c.block_table, c.seq_lens, c.free_head)))
+        c.check()
+    p = c.plan([], [])
+    assert p.cu.tolist() == [0] and p.slots.numel() == 0
+
+
 # ------------------------------------------------------------------------------------------------------------ store
 def _tables(kv_lens, B, extra, seed):
     rng = random.Random(seed)

@@ -28,7 +28,8 @@ struct Attn {
   float scale_log2;
   int n, n_rows, n_q, H, gs, n_blocks, max_blocks, log2b, splits, causal;
   int item_rows;               // rows of a work item
-  int tile, least;             // positions of a tile, fewest tiles of a split
+  int tile, least;             // positions of a tile; the tiles of a split are a multiple of this
+  int single;                  // query tiles over one request: (item, KV head) pairs of the launch (else 0)
   int shares, shift;           // decode in equal shares (0: in splits): workgroups; steps of their line are 2^shift tiles
 };
 
@@ -65,10 +66,16 @@ KVT_DEV Item item_of(const Attn& P, int w) {
   return t;
 }
 
-// Tiles per split of an item whose rows see `limit` positions: a multiple of `least`.  Splits behind the last tile are empty.
+// Tiles per split of an item whose rows see `limit` positions.  Splits behind the last tile are empty.  The number of splits follows
+// from the table's width, which a short request does not fill, so what a split has at least follows from what the rows see:
+// a multiple of `least` tiles, or for query tiles over one request 512 positions, 256 where those splits would leave half of the CUs
+// idle (as _TILE_LEAST of block_kv.py has it, where both are measured).  In a table of 262,144 positions, us per call, splits of a
+// tile or two / so many: 272 queries behind 3,156 positions (16 / 2 heads, D 256) 65 / 48, a prompt of 512 36.6 / 33.8, 61
+// queries behind 1,697 (12 / 1, D 128) 21.6 / 22.5.
 KVT_DEV int tiles_of(const Attn& P, int limit) { return (limit + P.tile - 1) / P.tile; }
 KVT_DEV int tiles_per_split(const Attn& P, int limit) {
   const int per = (tiles_of(P, limit) + P.splits - 1) / P.splits;
+  if (P.single) return max(per, ((int64_t)P.single * ((limit + 511) >> 9) >= 128 ? 512 : 256) / P.tile);
   return max((per + P.least - 1) / P.least, 1) * P.least;
 }
 // Splits that have tiles (one where there are none: it writes the NaN).  An item of one split is not merged.

@@ -739,7 +739,7 @@ extern "C" int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q
   P.n = n, P.n_rows = n_rows, P.n_q = n, P.H = H, P.gs = H > 0 ? Hq / H : 0, P.n_blocks = n_blocks;
   P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.causal = 0;
   P.splits = n_splits >= 0 ? n_splits : 1, P.shares = n_splits >= 0 ? 0 : -max(n_splits, -65536);
-  P.item_rows = 16, P.tile = kTile, P.least = kWaves, P.shift = 0;
+  P.item_rows = 16, P.tile = kTile, P.least = kWaves, P.single = 0, P.shift = 0;
   while (P.shift < 31 && ((double)n * H * (((double)max_blocks * block / kTile + kPad) / (1 << P.shift) + 2) + P.shares) > 2e9) ++P.shift;
   const int st = check(P, Hq, D, block, code, q_type, out_type);
   if (st != KVT_OK) return st;
@@ -770,7 +770,8 @@ extern "C" int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int 
   // width, so that the long requests' splits are not much longer than the others', and a short one is not split: 8 x 20 heads
   // (D 64), 448 ragged queries over 1,500 ragged positions 52.5 -> 45.5 us)
   const int grain = (int64_t)max_blocks * block <= (int64_t)n_splits * 256 ? 256 : 512;
-  P.least = !tiled ? kWaves : n > 1 ? grain / P.tile : 1;
+  P.least = !tiled ? kWaves : grain / P.tile;
+  P.single = 0;
   const int st = check(P, Hq, D, block, code, q_type, out_type);
   if (st != KVT_OK) return st;
   if (!cu_q || n_q < 0 || (item_rows != 16 && !tiled) || (n_splits > 1 && (!part_o || !part_ml))) return KVT_EINVAL;
@@ -778,6 +779,7 @@ extern "C" int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int 
   const int64_t items = (int64_t)n_q * P.gs / item_rows + n;
   if (items > (tiled ? 0xFFFFFF / P.H : 65535) || (n_splits > 1 && items * P.H > 65535)) return KVT_ERANGE;
   if (tiled) {
+    if (n == 1) P.single = (int)(((int64_t)n_q * P.gs + kTileRows - 1) / kTileRows * P.H);
     tile_launch(P, code, q_type, D, (int)items, out_type, (hipStream_t)stream);
     if (n_splits > 1) {
       if (D == 64) merge<64>(P, (int)items, kTileRows, out_type, (hipStream_t)stream);

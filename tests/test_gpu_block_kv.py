@@ -484,6 +484,46 @@ def test_attention_offsets_past_32_bits(kvt_pkg, decode):
     ref.close(got, *want, D)
 
 
+@pytest.mark.parametrize("kernel", ["decode", 16, 128])
+@pytest.mark.parametrize("Hq,H,D,B,new,lens", [(12, 1, 128, 64, [61], [1758]), (16, 2, 256, 64, [70], [777]), (4, 4, 64, 16, [300], [300]),
+                                               (8, 2, 128, 32, [33, 2, 300], [900, 700, 310]),
+                                               (4, 2, 256, 16, [1] * 20, list(range(0, 1000, 50)))])
+def test_attention_in_a_wide_table(kvt_pkg, monkeypatch, kernel, Hq, H, D, B, new, lens):
+    """A table of 262,144 positions, as a cache for long contexts has it, over requests that fill little of it: 64 bits, with a
+    kept workspace and without; and splits of one request's query tiles that hold 256 positions at least."""
+    from kvtier import block_kv
+    decode = kernel == "decode"
+    monkeypatch.setattr(block_kv, "_TILE_MIN", {D: 0 if kernel == 128 else 10 ** 9})
+    if decode:
+        new = [1] * len(lens)
+    g = torch.Generator().manual_seed(D)
+    table, nb = _tables(lens, B, 2, D)
+    codes, sc = _pool("fp8", nb, H, B, D, g)
+    tab = torch.full((len(lens), 262_144 // B), -1, dtype=torch.int32)
+    tab[:, :len(table[0])] = torch.tensor(table, dtype=torch.int32)
+    cu = prefix(new)
+    q = torch.randn(cu[-1], Hq, D, generator=g).to(torch.bfloat16)
+    val = [ref.values(codes[i]) * sc[i].double()[..., None, None] for i in range(2)]
+    want = ref.attention(q.double(), cu, lens, range(len(new)), table, val[0], val[1], not decode, D ** -0.5)
+    args = [c.to(dev) for c in codes] + [s.to(dev) for s in sc] + [tab.to(dev), i32(lens)]
+
+    def call(ws):
+        out = torch.full(q.shape, 5.0, dtype=torch.float32, device=dev)
+        if decode:
+            return block_kv.kvt_block_decode(q.to(dev), *args, out=out, workspace=ws)
+        return block_kv.kvt_block_prefill(q.to(dev), i32(cu), *args, out=out, workspace=ws)
+    ws = {}
+    for w in (None, ws, ws):
+        ref.close(call(w), *want, D)
+    if kernel == 128 and len(lens) == 1:
+        ml = ws["block_ml", 0]
+        ml.fill_(-7.0)
+        call(ws)
+        items = (cu[-1] * (Hq // H) // 128 + 1) * H
+        used = (ml.view(items, -1, 128, 2) != -7.0).flatten(2).any(2).any(0).nonzero()
+        assert 1 < used.numel() and int(used.max()) < -(-lens[0] // 256)
+
+
 def test_attention_strided_queries_and_rows(kvt_pkg):
     """Queries as a slice of a fused projection (strided, and at an odd offset), table rows through seqs, a strided out."""
     from kvtier import block_kv

@@ -2,7 +2,7 @@
 //
 // With a = max |x| over the rows that the call writes into a block (finite ones), need = the smallest power of two with
 // a / need <= Q (448 for e4m3, 127 for int8), within 2^-64 .. 2^122:
-//   s    = need where the call opens the block, else max(need, s_old)
+//   s    = need where the call opens the block, else max(need, s_old) (an s_old that is not finite stays)
 //   old codes (rows that the request held in the block) -> rne(code * s_old / s) where s grew
 //   new codes = rne(x / s)
 // Powers of two, because a block fills up over many calls: x / s is exact, a growing scale moves the exponent of an e4m3
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(256) void block_store_kernel(const Store P) {
     t = widest(t);
   }
   float s = pow2_scale<CODE>(magnitude<DT>(t));
-  if (held) s = fmaxf(s, was);
+  if (held && !(was <= s)) s = was;                                 // (a NaN stays: the rows held are NaN with it)
   const float inv = 1.0f / s;
   uint8_t* out = P.codes[side] + ((at << P.log2b) * D);
   if (held && s > was) {

@@ -139,3 +139,31 @@ def test_a_nan_row_that_is_appended(kvt_pkg):
     c.append(0, plan, x[0], x[1])
     bad = torch.isnan(c.prefill(0, plan, q)).flatten(1)
     assert not bad[:80].any() and bad[80:100].all() and not bad[100:].any()
+
+
+@pytest.mark.parametrize("kv", ["fp8", "int8"])
+@pytest.mark.parametrize("n", [1, 30])
+def test_a_scale_that_is_not_finite_stays(kvt_pkg, kv, n):
+    """Rows appended to a block whose scale is NaN or infinite do not give the rows held there a finite scale; a block that the
+    call opens takes no notice of what its scale was."""
+    from kvtier import block_kv
+    c = block_kv.BlockKVCache(1, 3, 64, n_blocks=4, max_seqs=1, max_blocks=4, block=16, dtype=ref.CODE[kv])
+    s = c.add_seq()
+    g = torch.Generator(device=dev).manual_seed(2)
+    x = torch.randn(2, 5 + n, 3, 64, device=dev, generator=g).to(torch.bfloat16)
+    for t in (c.ks[0], c.vs[0]):
+        t.fill_(math.nan)
+    c.append(0, c.plan([s], [5]), x[0, :5], x[1, :5])
+    first, later = int(c.block_table[s, 0]), [i for i in range(4) if i != int(c.block_table[s, 0])]
+    for t in (c.ks[0], c.vs[0]):
+        assert bool(torch.isfinite(t[first]).all()) and bool(torch.isnan(t[later]).all())
+        t[first, 0], t[first, 1] = math.nan, math.inf
+    plan = c.plan([s], [n])
+    c.append(0, plan, x[0, 5:], x[1, 5:])
+    for t in (c.ks[0], c.vs[0]):
+        assert math.isnan(t[first, 0]) and math.isinf(t[first, 1]) and bool(torch.isfinite(t[first, 2]))
+        for lp in range(1, -(-(5 + n) // 16)):
+            assert bool(torch.isfinite(t[c.block_table[s, lp]]).all())
+    q = torch.randn(n, 3, 64, device=dev, generator=g).to(torch.bfloat16)
+    bad = torch.isnan(c.prefill(0, plan, q))
+    assert bool(bad[:, :2].all()) and not bool(bad[:, 2].any())

@@ -331,7 +331,7 @@ int kvt_block_plan(int n, const void* seqs, const void* counts, void* seq_lens, 
 
 /* Quantizing write of N = n_tokens rows k / v [N, H, D] (dtype codes as above; element strides, unit last stride, rows
  * 16-byte aligned) into the blocks of their positions: rows cu[j] .. cu[j+1] of k / v are the last positions of request
- * j's kv_lens[j].  A block's scale is the smallest power of two that holds the largest finite |x| of the call's rows in the
+ * j's kv_lens[j] (cu[n] <= N; rows behind cu[n] are not read).  A block's scale is the smallest power of two that holds the largest finite |x| of the call's rows in the
  * code's range (448 or 127; within 2^-64 .. 2^122), or the scale it has if that is larger and the request held rows of
  * the block before (or is not finite); where it grows, those rows' codes are rounded to the new scale.  Codes are rounded to nearest even;
  * infinities become the largest code, NaN the e4m3 NaN or the int8 0.  Other rows of a block are left as they are.  A block

@@ -117,7 +117,7 @@ def kvt_block_plan(seqs: torch.Tensor, counts: torch.Tensor, seq_lens: torch.Ten
     The blocks that the requests open come from free_list (int32 [n_blocks], read from free_head[0] on) in request order
     and are written into block_table; every token gets its slot (block * block size + row: a location of the slot-indexed
     pools too), and with req_to_token (int32 [rows, context]) the slot of every position is recorded there.  n_tokens:
-    the length of `slots`, a host int >= the counts' sum.  commit=False leaves seq_lens and free_head as they are, to look
+    the length of `slots`, a host int >= the counts' sum (slots behind that are -1).  commit=False leaves seq_lens and free_head as they are, to look
     at a plan (its status, its next_head) before it is taken: the next plan starts from the same state.
     status (int32 [1]): bits POOL_SHORT, ROW_FULL, TOKENS_OVER, BAD_ROW (a row out of range, or listed twice: the later
     request appends nothing) are or-ed in.  At most 1,024 requests; of none, the plan is empty."""
@@ -177,7 +177,8 @@ def kvt_block_store(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, kv_lens:
     A block's scale is the smallest power of two s with |x| <= 448 s (e4m3) or 127 s (int8) for the call's finite values,
     and never shrinks while the block fills: where it grows, the rows that the request held before are rounded to the new
     scale (exact for e4m3 codes, but for those that become subnormal).  Rows of a block that the request does not hold yet
-    are left as they are.  A block must be in the table of one request of the call only."""
+    are left as they are, rows of k and v behind cu[n] are not read; N has to be cu[n] at least.  A block must be in the table of one
+    request of the call only."""
     N, H, D = k.shape
     n = kv_lens.numel()
     nb, H8, B, D8 = _pool(k8, v8, ks, vs, block_table, n, seqs)
@@ -293,7 +294,8 @@ def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8:
     causal: the chunk's queries are the last positions of request j (its keys are in the cache already) and each sees the
     positions up to its own: kv_lens[j] - chunk + i + 1 of them for query i.  causal=False: every query sees all
     kv_lens[j] positions -- cross attention to another sequence's states, of any length.  A query that sees nothing gives
-    NaN (0/0).  Other arguments as kvt_block_decode."""
+    NaN (0/0).  Rows behind cu_q[n] (a padded step) are neither read nor written: they keep what a given `out` holds, and are
+    uninitialized memory in one that is made here.  Other arguments as kvt_block_decode."""
     n = kv_lens.numel()
     nb, H, B, D = _pool(k8, v8, ks, vs, block_table, n, seqs)
     q, qp, qn, qh, out, so, Hq = _attn_args(q, out, H, D)
@@ -384,7 +386,8 @@ class BlockKVCache:
     def plan(self, seqs, counts, n_tokens: Optional[int] = None, req_to_token: Optional[torch.Tensor] = None,
              commit: bool = True) -> BlockPlan:
         """kvt_block_plan over this cache.  seqs / counts: int32 device vectors or lists; n_tokens: a host bound of the
-        counts' sum (needed with device counts)."""
+        counts' sum (needed with device counts; tokens and queries behind the sum are padding, which no call reads or
+        writes)."""
         if n_tokens is None:
             if isinstance(counts, torch.Tensor):
                 raise ValueError("plan: pass n_tokens (a host int >= the counts' sum) with counts on the device")
@@ -413,6 +416,7 @@ class BlockKVCache:
                                 plan.kv_lens, plan.seqs, **kw)
 
     def prefill(self, layer: int, plan: BlockPlan, q: torch.Tensor, **kw) -> torch.Tensor:
-        """Attention of the plan's tokens (q: [n_tokens, Hq, D])."""
+        """Attention of the plan's tokens (q: [n_tokens, Hq, D]).  Where n_tokens is more than the counts' sum, the rows behind that
+        are not written: pass an `out` that holds what they should be, or do not read them."""
         return kvt_block_prefill(q, plan.cu, self.k8[layer], self.v8[layer], self.ks[layer], self.vs[layer],
                                  self.block_table, plan.kv_lens, plan.seqs, **kw)

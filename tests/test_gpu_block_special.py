@@ -167,3 +167,34 @@ def test_a_scale_that_is_not_finite_stays(kvt_pkg, kv, n):
     q = torch.randn(n, 3, 64, device=dev, generator=g).to(torch.bfloat16)
     bad = torch.isnan(c.prefill(0, plan, q))
     assert bool(bad[:, :2].all()) and not bool(bad[:, 2].any())
+
+
+@pytest.mark.parametrize("counts", [[5, 0, 33], [300, 1, 200]])
+def test_a_padded_step(kvt_pkg, counts):
+    """More rows than the counts' sum, NaN behind it: the cache and the queries' rows are those of the step without padding, a
+    given out keeps its rows behind the sum, and one that is made there has the rows before it."""
+    from kvtier import block_kv
+    H, D, n = 2, 128, sum(counts)
+    g = torch.Generator(device=dev).manual_seed(3)
+    x = torch.randn(2, n + 70, H, D, device=dev, generator=g).to(torch.bfloat16)
+    q = torch.randn(n + 70, 8, D, device=dev, generator=g).to(torch.bfloat16)
+    x[:, n:] = q[n:] = math.nan
+    made = []
+    for rows in (n, n + 70):
+        c = block_kv.BlockKVCache(1, H, D, n_blocks=60, max_seqs=3, max_blocks=30, block=32, seed=4)
+        seqs = i32([c.add_seq() for _ in counts])
+        plan = c.plan(seqs, i32(counts), n_tokens=rows)
+        c.append(0, plan, x[0, :rows], x[1, :rows])
+        out = torch.full((rows, 8, D), 5.0, dtype=torch.bfloat16, device=dev)
+        got = c.prefill(0, plan, q[:rows], out=out)
+        assert got is out and bool((out[n:] == 5.0).all())
+        val = [ref.values(x8[0].cpu()) * s[0].cpu().double()[..., None, None] for x8, s in ((c.k8, c.ks), (c.v8, c.vs))]
+        want = ref.attention(q[:n].cpu().double(), prefix(counts), counts, seqs.tolist(), c.block_table.tolist(), *val, True, D ** -0.5)
+        for y in (out, c.prefill(0, plan, q[:rows])):
+            ref.close(y[:n], *want, D)
+        c.check()
+        made.append(c)
+    a, b = made
+    for i, j in ((a.k8, b.k8), (a.v8, b.v8)):
+        assert torch.equal(i[0].view(torch.int8), j[0].view(torch.int8))
+    assert torch.equal(a.ks[0], b.ks[0]) and torch.equal(a.vs[0], b.vs[0]) and torch.equal(a.block_table, b.block_table)

@@ -331,10 +331,11 @@ int kvt_block_plan(int n, const void* seqs, const void* counts, void* seq_lens, 
 
 /* Quantizing write of N = n_tokens rows k / v [N, H, D] (dtype codes as above; element strides, unit last stride, rows
  * 16-byte aligned) into the blocks of their positions: rows cu[j] .. cu[j+1] of k / v are the last positions of request
- * j's kv_lens[j] (cu[n] <= N; rows behind cu[n] are not read).  A block's scale is the smallest power of two that holds the largest finite |x| of the call's rows in the
- * code's range (448 or 127; within 2^-64 .. 2^122), or the scale it has if that is larger and the request held rows of
- * the block before (or is not finite); where it grows, those rows' codes are rounded to the new scale.  Codes are rounded to nearest even;
- * infinities become the largest code, NaN the e4m3 NaN or the int8 0.  Other rows of a block are left as they are.  A block
+ * j's kv_lens[j] (cu[n] <= N; rows behind cu[n] are not read).  A block's scale is the smallest power of two that
+ * holds the largest finite |x| of the call's rows in the code's range (448 or 127; within 2^-64 .. 2^122), or the scale
+ * it has if the request held rows of the block before and that is larger or not finite; where it grows, those rows'
+ * codes are rounded to the new scale.  Codes are rounded to nearest even; infinities become the largest code, NaN the
+ * e4m3 NaN or the int8 0.  Other rows of a block are left as they are.  A block
  * must not be in the tables of two of the call's requests.  n <= 4,096. */
 int kvt_block_store(const void* k, const void* v, int dtype, int64_t sk_n, int64_t sk_h, int64_t sv_n, int64_t sv_h,
                     int n_tokens, int H, int D, const void* cu, const void* kv_lens, int n, const void* rows,

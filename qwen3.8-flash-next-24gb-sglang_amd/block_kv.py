@@ -29,36 +29,43 @@ _I32, _F32 = torch.int32, torch.float32
 BLOCKS = (16, 32, 64)
 HEAD_DIMS = (64, 128, 256)
 POOL_SHORT, ROW_FULL, TOKENS_OVER, BAD_ROW = 1, 2, 4, 8   # status bits of a plan
-# Decode.  Few requests: a number of splits for each (request, KV head) pair.  From _SHARE_REQUESTS on, over long tables:
-# equal shares of all positions.  Measured, device us per call with the merge, caches cold, best splits against shares, up
-# to 8,191 positions ragged: 8 requests x 8 heads (D 128) 19.7 / 22.7; 32 x 2 (D 256, up to 16,384) 65.7 / 52.9; 64 x 2
-# (D 256) 50.2 / 44.9; 16 x 20 (D 64) 40.0 / 37.6; 64 x 8 (D 128) 117 / 98; up to 1,000 positions, 64 x 2 17.9 / 20.5.
+# Decode.  Few requests: a number of splits for each (request, KV head) pair.  From _SHARE_REQUESTS on, over long
+# tables: equal shares of all positions.  Measured, device us per call with the merge, caches cold, best splits against
+# shares, up to 8,191 positions ragged: 8 requests x 8 heads (D 128) 19.7 / 22.7; 32 x 2 (D 256, up to 16,384) 65.7 /
+# 52.9; 64 x 2 (D 256) 50.2 / 44.9; 16 x 20 (D 64) 40.0 / 37.6; 64 x 8 (D 128) 117 / 98; up to 1,000 positions, 64 x 2
+# 17.9 / 20.5.  Both this choice and the number of splits follow from the table's width, since the lengths stay on the
+# device: in a table that is much wider than its requests they are those of long requests (one of 777 positions in a
+# table of 262,144 14.0 - 15.4 us against 12.1 - 12.8 in one of its own width, 8 up to 2,000 16.4 against 14.2; 32 up
+# to 1,000 14.8 against 16.6, 24 / 2 heads, D 256).
 _SHARE_REQUESTS, _SHARE_CAP = 16, 2048
-# Workgroups of a launch in equal shares, and of one request's splits (D 256: one per CU, whose four wavefronts keep enough
-# loads in flight: 52.9 us for 32 x 2 against 57.9 with two; D 128: 98 against 113 with one and 103 with three), and of chunks of few rows (4
-# queries a request: 8 x 8, D 128, up to 4,000 positions 19.9 with 8 splits, 24.7 with 16; 32 x 2, D 256, up to 1,000 21.1 with
-# 4, 32.6 with 8).
+# Workgroups of a launch in equal shares, and of one request's splits (D 256: one per CU, whose four wavefronts keep
+# enough loads in flight: 52.9 us for 32 x 2 against 57.9 with two; D 128: 98 against 113 with one and 103 with three),
+# and of chunks of few rows (4 queries a request: 8 x 8, D 128, up to 4,000 positions 19.9 with 8 splits, 24.7 with 16;
+# 32 x 2, D 256, up to 1,000 21.1 with 4, 32.6 with 8).  (Two workgroups a CU are what the kernel of equal shares has
+# registers for: at D 64 and 128 the merge inside the launch takes the most of them, 239 and 255 where
+# block_rows_kernel, with the same loop, has 96 and 135.)
 _DECODE_BLOCKS = {64: 512, 128: 512, 256: 256}
-# Splits of a pair that a launch with a kept workspace merges itself.  us per call, merged by a second launch / by itself: 8
-# requests x 2 heads (D 256, up to 2,000 positions, 16 splits) 15.4 / 12.4; one x 8 (D 128, 2,000, 16 splits) 12.7 / 8.6; 8 x 8
-# (D 128, up to 4,000, 12 splits) 18.7 / 15.5; chunks of four queries over the same (8 splits) 22.1 / 19.9; but two of 300
-# positions x 2 heads (24 q heads) 11.5 / 12.1.  Past 16 the second launch's many workgroups read the parts faster than the
-# last one does.  (Equal shares: the entry point decides.)
+# Splits of a pair that a launch with a kept workspace merges itself.  us per call, merged by a second launch / by
+# itself: 8 requests x 2 heads (D 256, up to 2,000 positions, 16 splits) 15.4 / 12.4; one x 8 (D 128, 2,000, 16 splits)
+# 12.7 / 8.6; 8 x 8 (D 128, up to 4,000, 12 splits) 18.7 / 15.5; chunks of four queries over the same (8 splits) 22.1 /
+# 19.9; but two of 300 positions x 2 heads (24 q heads) 11.5 / 12.1.  Past 16 the second launch's many workgroups read
+# the parts faster than the last one does.  (Equal shares: the entry point decides.)
 _MERGE_SPLITS = 16
 _TILE_ROWS = 128         # (query, q head) rows of a workgroup of the query-tile kernel
-# Workgroups of a split launch of it for one request, us per call (merge included): D 256, 16 items x 30,000 positions 256
-# workgroups 150, 512 110; D 128, 6 x 60,000 258 59.7, 384 57.9, 510 63.5; D 64, 20 x 30,000 320 86, 480 77, 640 65.  Half as
-# many again for several, whose lengths differ: 4 x 8 heads (D 128), 64 queries, up to 6,000 positions 75 / 58, 8 x 20 heads (D
-# 64) up to 1,500 52.5 / 45.5, 8 x 2 (D 256) up to 4,000 124 / 110, 8 x 8 (D 128) up to 3,000 53 / 55.
+# Workgroups of a split launch of it for one request, us per call (merge included): D 256, 16 items x 30,000 positions
+# 256 workgroups 150, 512 110; D 128, 6 x 60,000 258 59.7, 384 57.9, 510 63.5; D 64, 20 x 30,000 320 86, 480 77, 640 65.
+# Half as many again for several, whose lengths differ: 4 x 8 heads (D 128), 64 queries, up to 6,000 positions 75 / 58,
+# 8 x 20 heads (D 64) up to 1,500 52.5 / 45.5, 8 x 2 (D 256) up to 4,000 124 / 110, 8 x 8 (D 128) up to 3,000 53 / 55.
 _TILE_BLOCKS = {64: 768, 128: 384, 256: 512}
-# Positions of a split at least: its part of 128 rows is 512 D bytes written and read again.  Half of it where those splits
-# would leave half of the CUs idle: 5 query tiles (D 128) behind 1,758 positions 26.0 us with 512, 20.7 with 256, 19.3 with 128;
-# 24 (D 256) behind 1,000 42 / 34 / 33; but 34 (D 256) behind 3,428 49 / 51 / 80, 44 (D 64) behind 4,000 36 / 35 / 47.
+# Positions of a split at least: its part of 128 rows is 512 D bytes written and read again.  Half of it where those
+# splits would leave half of the CUs idle: 5 query tiles (D 128) behind 1,758 positions 26.0 us with 512, 20.7 with 256,
+# 19.3 with 128; 24 (D 256) behind 1,000 42 / 34 / 33; but 34 (D 256) behind 3,428 49 / 51 / 80, 44 (D 64) behind 4,000
+# 36 / 35 / 47.
 _TILE_LEAST = 512
-# Rows per request and KV head (on average) from which it serves a call.  us per call against the 16-row kernel's, one request
-# behind 30,000 positions: D 128, 64 rows 41 / 42, 128 rows 66 / 64, 256 rows 72 / 102; D 64, 128 rows 78 / 79, 256 rows 116 /
-# 143; D 256, 128 rows 59 / 44, 256 rows 60 / 61, 512 rows 82 / 90.  Eight ragged requests behind 4,000: D 128, 116 rows 54
-# / 45, 230 rows 70 / 77.
+# Rows per request and KV head (on average) from which it serves a call.  us per call against the 16-row kernel's, one
+# request behind 30,000 positions: D 128, 64 rows 41 / 42, 128 rows 66 / 64, 256 rows 72 / 102; D 64, 128 rows 78 / 79,
+# 256 rows 116 / 143; D 256, 128 rows 59 / 44, 256 rows 60 / 61, 512 rows 82 / 90.  Eight ragged requests behind 4,000:
+# D 128, 116 rows 54 / 45, 230 rows 70 / 77.
 _TILE_MIN = {64: 128, 128: 128, 256: 256}
 
 
@@ -117,8 +124,8 @@ def kvt_block_plan(seqs: torch.Tensor, counts: torch.Tensor, seq_lens: torch.Ten
     The blocks that the requests open come from free_list (int32 [n_blocks], read from free_head[0] on) in request order
     and are written into block_table; every token gets its slot (block * block size + row: a location of the slot-indexed
     pools too), and with req_to_token (int32 [rows, context]) the slot of every position is recorded there.  n_tokens:
-    the length of `slots`, a host int >= the counts' sum (slots behind that are -1).  commit=False leaves seq_lens and free_head as they are, to look
-    at a plan (its status, its next_head) before it is taken: the next plan starts from the same state.
+    the length of `slots`, a host int >= the counts' sum (slots behind that are -1).  commit=False leaves seq_lens and
+    free_head as they are, to look at a plan (its status, its next_head) before it is taken: the next plan starts from the same state.
     status (int32 [1]): bits POOL_SHORT, ROW_FULL, TOKENS_OVER, BAD_ROW (a row out of range, or listed twice: the later
     request appends nothing) are or-ed in.  At most 1,024 requests; of none, the plan is empty."""
     n = seqs.numel()
@@ -143,7 +150,8 @@ def kvt_block_plan(seqs: torch.Tensor, counts: torch.Tensor, seq_lens: torch.Ten
     if n == 0:                                             # (an idle step: no slots, and the state as it is)
         zero = seqs.new_zeros(1)
         return BlockPlan(seqs, zero, seqs.new_full((n_tokens,), -1), zero[:0], free_head[:1].clamp(0, free_list.numel()))
-    slots, cu, kv_lens, next_head = seqs.new_empty(n_tokens + 2 * n + 2).split_with_sizes((n_tokens, n + 1, n, 1))   # (one allocation)
+    one = seqs.new_empty(n_tokens + 2 * n + 2)              # (one allocation)
+    slots, cu, kv_lens, next_head = one.split_with_sizes((n_tokens, n + 1, n, 1))
     _lib.call("kvt_block_plan", n, seqs.data_ptr(), counts.data_ptr(), seq_lens.data_ptr(), rows, block_table.data_ptr(),
               block_table.stride(0), block_table.shape[1], free_list.data_ptr(), free_list.numel(), free_head.data_ptr(),
               block, n_tokens, cu.data_ptr(), slots.data_ptr(), kv_lens.data_ptr(), next_head.data_ptr(),
@@ -177,8 +185,8 @@ def kvt_block_store(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, kv_lens:
     A block's scale is the smallest power of two s with |x| <= 448 s (e4m3) or 127 s (int8) for the call's finite values,
     and never shrinks while the block fills: where it grows, the rows that the request held before are rounded to the new
     scale (exact for e4m3 codes, but for those that become subnormal).  Rows of a block that the request does not hold yet
-    are left as they are, rows of k and v behind cu[n] are not read; N has to be cu[n] at least.  A block must be in the table of one
-    request of the call only."""
+    are left as they are, rows of k and v behind cu[n] are not read; N has to be cu[n] at least.  A block must be in the
+    table of one request of the call only."""
     N, H, D = k.shape
     n = kv_lens.numel()
     nb, H8, B, D8 = _pool(k8, v8, ks, vs, block_table, n, seqs)
@@ -192,8 +200,9 @@ def kvt_block_store(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, kv_lens:
     per16 = 4 if k.dtype == torch.float32 else 8
     k, kp, kn, kh = _rows16(k, per16)
     v, vp, vn, vh = _rows16(v, per16)
-    _lib.call("kvt_block_store", kp, vp, _lib.DTYPE_CODE[k.dtype], kn, kh, vn, vh, N, H, D, cu.data_ptr(), kv_lens.data_ptr(), n, _lib.ptr(seqs),
-              block_table.data_ptr(), block_table.stride(0), *block_table.shape, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B, st)
+    _lib.call("kvt_block_store", kp, vp, _lib.DTYPE_CODE[k.dtype], kn, kh, vn, vh, N, H, D, cu.data_ptr(),
+              kv_lens.data_ptr(), n, _lib.ptr(seqs), block_table.data_ptr(), block_table.stride(0), *block_table.shape,
+              CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(), ks.data_ptr(), vs.data_ptr(), nb, B, st)
 
 
 def _grown(ws: dict, name: str, n: int, like: torch.Tensor, dtype=torch.float32, zero: bool = False) -> torch.Tensor:
@@ -334,8 +343,8 @@ class BlockKVCache:
     """Buffers of the 8-bit block cache for all layers of a model, and the step's calls over them.
 
     Per layer k8 / v8 [n_blocks, H, block, D] and ks / vs [n_blocks, H]; shared by the layers: block_table
-    [max_seqs, max_blocks], seq_lens [max_seqs], the free list (a seeded permutation of the blocks) and its head.  Lengths, blocks and
-    the free list live on the device only; add_seq and release hand out table rows on the host."""
+    [max_seqs, max_blocks], seq_lens [max_seqs], the free list (a seeded permutation of the blocks) and its head.
+    Lengths, blocks and the free list live on the device only; add_seq and release hand out table rows on the host."""
 
     def __init__(self, layers: int, H: int, D: int, n_blocks: int, max_seqs: int, max_blocks: int, device="cuda",
                  dtype: torch.dtype = torch.float8_e4m3fn, block: int = 64, seed: int = 0):
@@ -416,7 +425,7 @@ class BlockKVCache:
                                 plan.kv_lens, plan.seqs, **kw)
 
     def prefill(self, layer: int, plan: BlockPlan, q: torch.Tensor, **kw) -> torch.Tensor:
-        """Attention of the plan's tokens (q: [n_tokens, Hq, D]).  Where n_tokens is more than the counts' sum, the rows behind that
-        are not written: pass an `out` that holds what they should be, or do not read them."""
+        """Attention of the plan's tokens (q: [n_tokens, Hq, D]).  Where n_tokens is more than the counts' sum, the rows
+        behind that are not written: pass an `out` that holds what they should be, or do not read them."""
         return kvt_block_prefill(q, plan.cu, self.k8[layer], self.v8[layer], self.ks[layer], self.vs[layer],
                                  self.block_table, plan.kv_lens, plan.seqs, **kw)

@@ -1,5 +1,5 @@
-// What the attention kernels of the 8-bit block cache share (block_rows.hip, block_tile.hip): arguments, work items, the
-// division of an item's positions into splits, and query rows in operand order.
+// What the attention kernels of the 8-bit block cache share (block_rows.hip, block_tile.hip): arguments, work items,
+// the division of an item's positions into splits, and query rows in operand order.
 #pragma once
 
 #include "block_common.h"
@@ -33,8 +33,8 @@ struct Attn {
   int shares, shift;           // decode in equal shares (0: in splits): workgroups; steps of their line are 2^shift tiles
 };
 
-// What a workgroup has: request r, query rows [row0, row0 + n_row) of it in (query, q head) order, the query base, and the
-// positions that any of its rows sees.
+// What a workgroup has: request r, query rows [row0, row0 + n_row) of it in (query, q head) order, the query base, and
+// the positions that any of its rows sees.
 struct Item {
   int r, trow, q0, q_len, row0, n_row, kv, len, limit;
 };
@@ -66,12 +66,12 @@ KVT_DEV Item item_of(const Attn& P, int w) {
   return t;
 }
 
-// Tiles per split of an item whose rows see `limit` positions.  Splits behind the last tile are empty.  The number of splits follows
-// from the table's width, which a short request does not fill, so what a split has at least follows from what the rows see:
-// a multiple of `least` tiles, or for query tiles over one request 512 positions, 256 where those splits would leave half of the CUs
-// idle (as _TILE_LEAST of block_kv.py has it, where both are measured).  In a table of 262,144 positions, us per call, splits of a
-// tile or two / so many: 272 queries behind 3,156 positions (16 / 2 heads, D 256) 65 / 48, a prompt of 512 36.6 / 33.8, 61
-// queries behind 1,697 (12 / 1, D 128) 21.6 / 22.5.
+// Tiles per split of an item whose rows see `limit` positions.  Splits behind the last tile are empty.  The number of
+// splits follows from the table's width, which a short request does not fill, so what a split has at least follows from
+// what the rows see: a multiple of `least` tiles, or for query tiles over one request 512 positions, 256 where those
+// splits would leave half of the CUs idle (as _TILE_LEAST of block_kv.py has it, where both are measured).  In a table
+// of 262,144 positions, us per call, splits of a tile or two / so many: 272 queries behind 3,156 positions (16 / 2
+// heads, D 256) 65 / 48, a prompt of 512 36.6 / 33.8, 61 queries behind 1,697 (12 / 1, D 128) 21.6 / 22.5.
 KVT_DEV int tiles_of(const Attn& P, int limit) { return (limit + P.tile - 1) / P.tile; }
 KVT_DEV int tiles_per_split(const Attn& P, int limit) {
   const int per = (tiles_of(P, limit) + P.splits - 1) / P.splits;
@@ -90,13 +90,14 @@ KVT_DEV h2 h2_rne(float a, float b) { return __builtin_convertvector((f2){a, b},
 KVT_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }   // (v_exp_f32: results below 2^-126 are 0)
 KVT_DEV float bits_f(uint32_t u) { return __uint_as_float(u); }
 
-// A row that sees a position of a block with a scale that is not finite is NaN, in every channel; to other rows such a block is one
-// that is not there, so that no 0 * NaN of a position that they do not see reaches them.  (Scales are >= 0.)
+// A row that sees a position of a block with a scale that is not finite is NaN, in every channel; to other rows such a
+// block is one that is not there, so that no 0 * NaN of a position that they do not see reaches them.  (Scales are >=
+// 0.)
 KVT_DEV bool finite_scales(float k, float v) { return max(__float_as_uint(k) << 1, __float_as_uint(v) << 1) < 0xFF000000u; }
 
-// NaN codes of V (e4m3) in tiles that some row of a workgroup does not see to their end: a product would take them to all of its
-// rows, as 0 * NaN.  They are taken out of the codes, and what remains is the first position where each channel has one:
-// a row sees positions 0 .. n - 1, so the channel is NaN for it where that position is below n.
+// NaN codes of V (e4m3) in tiles that some row of a workgroup does not see to their end: a product would take them to
+// all of its rows, as 0 * NaN.  They are taken out of the codes, and what remains is the first position where each
+// channel has one: a row sees positions 0 .. n - 1, so the channel is NaN for it where that position is below n.
 template <int CODE, int D>
 struct NanAt {
   int at[CODE == kE4M3 ? D : 1], found;
@@ -136,8 +137,8 @@ struct NanAt {
   }
 };
 
-// O's unit becomes the V scale fv > 0, but no less than 2^-80 of the largest so far (|O| in units of that is below 2^40, so
-// it stays finite); returns the factor for O.
+// O's unit becomes the V scale fv > 0, but no less than 2^-80 of the largest so far (|O| in units of that is below
+// 2^40, so it stays finite); returns the factor for O.
 KVT_DEV float new_unit(float fv, float& unit, float& peak) {
   peak = fmaxf(peak, fv);
   const float u = fmaxf(fv, peak * 0x1p-80f), a = unit / u;
@@ -168,7 +169,7 @@ KVT_DEV float load_q(const void* q, int64_t row, At at, Top top_of, h8 (&out)[N]
   if constexpr (QT == kF16) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      asm("" : "+v"(raw[k].x), "+v"(raw[k].y), "+v"(raw[k].z), "+v"(raw[k].w));   // (as plain registers: loaded tuples cost spills)
+      asm("" : "+v"(raw[k].x), "+v"(raw[k].y), "+v"(raw[k].z), "+v"(raw[k].w));   // (loaded tuples cost spills)
       out[k] = __builtin_bit_cast(h8, raw[k]);
     }
     return 1.0f;

@@ -1,4 +1,4 @@
-// Device helpers of the 8-bit block cache (block_plan.hip, block_store.hip, block_attn.hip).
+// Device helpers of the 8-bit block cache (block_plan.hip, block_store.hip, block_rows.hip, block_tile.hip).
 //
 // Layout, per layer: codes k8 / v8 [n_blocks, H, B, D], one byte each (e4m3 or int8), B = 16, 32 or 64 tokens; scales
 // ks / vs fp32 [n_blocks, H]: the value of a code c is c * s.  A request's position p sits in row p % B of block
@@ -88,9 +88,9 @@ KVT_DEV h8 operand(uint32_t w0, uint32_t w1) {
 }
 
 // The work items of request r are numbered from first_item(cu[r], r) = floor(cu[r] * mul / div) + per * r on: an upper
-// bound of what the requests before it need, so that a launch finds (request, item) from its block index and the
-// prefix sums alone, with no list of items.  find_request returns the largest r < n with first_item(r) <= w (0 if none),
-// for n <= 4,096: two rounds of one load per lane.  All 64 lanes take part; the result is uniform.
+// bound of what the requests before it need, so that a launch finds (request, item) from its block index and the prefix
+// sums alone, with no list of items.  find_request returns the largest r < n with first_item(r) <= w (0 if none), for n
+// <= 4,096: two rounds of one load per lane.  All 64 lanes take part; the result is uniform.
 KVT_DEV int64_t first_item(int cu, int r, int mul, int div, int per) {
   return (int64_t)max(cu, 0) * mul / div + (int64_t)per * r;
 }

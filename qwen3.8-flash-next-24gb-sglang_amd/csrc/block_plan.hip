@@ -1,16 +1,16 @@
 // Block tables and slot maps of a step, from the requests' lengths on the device (kvt_block_plan).
 //
-// Request j (table row s = seqs[j], L0 = seq_lens[s] tokens held) appends c = counts[j] tokens at positions L0 .. L0 + c - 1.
-// It opens the blocks ceil(L0 / B) .. ceil((L0 + c) / B) - 1, which take the next entries of the free list in request
-// order; position p goes to slot block * B + p % B.  With exclusive prefix sums C of the token counts and O of the opened
-// blocks, token t of request j (C_j <= t < C_j+1) has p = L0 + t - C_j, and an opened block lp is free_list[head + O_j + lp -
-// ceil(L0 / B)]: every token's slot follows from the sums alone.
+// Request j (table row s = seqs[j], L0 = seq_lens[s] tokens held) appends c = counts[j] tokens at positions L0 .. L0 +
+// c - 1.  It opens the blocks ceil(L0 / B) .. ceil((L0 + c) / B) - 1, which take the next entries of the free list in
+// request order; position p goes to slot block * B + p % B.  With exclusive prefix sums C of the token counts and O of
+// the opened blocks, token t of request j (C_j <= t < C_j+1) has p = L0 + t - C_j, and an opened block lp is
+// free_list[head + O_j + lp - ceil(L0 / B)]: every token's slot follows from the sums alone.
 //
-// A block of 1,024 threads scans the (at most 1,024) requests by itself, keeps the sums in LDS and writes the slots of 4,096
-// tokens, four per thread (one 16-byte store): no second launch, no communication.  With `commit`, lengths and head advance
-// in the same launch when it has one block, else in a launch behind it (other blocks may still be reading them).
-// Launch and load latency bound it: 64 requests of one token 5.9 us, 512 requests and 538,000 tokens with req_to_token 8.4
-// (4.6 MB written, 132 blocks that all scan).
+// A block of 1,024 threads scans the (at most 1,024) requests by itself, keeps the sums in LDS and writes the slots of
+// 4,096 tokens, four per thread (one 16-byte store): no second launch, no communication.  With `commit`, lengths and
+// head advance in the same launch when it has one block, else in a launch behind it (other blocks may still be reading
+// them).  Launch and load latency bound it: 64 requests of one token 6.0 us, 512 requests and 538,000 tokens with
+// req_to_token 8.3 (4.6 MB written, 132 blocks that all scan).
 #include "block_common.h"
 
 using namespace kvt;
@@ -110,8 +110,8 @@ __global__ __launch_bounds__(kThreads) void block_plan_kernel(const Plan P) {
     S.cu[j + 1] = c1;
     S.len[j] = len;
     S.base[j] = (int)min(taken - opens, (int64_t)P.n_free) - first;
-    int f = (bad ? kBadRow : 0) | (upto > P.n_tokens ? kTokensOver : 0) | (c1 > c0 && last > P.max_blocks ? kRowFull : 0) |
-            (head + taken > P.n_free ? kPoolShort : 0);
+    int f = (bad ? kBadRow : 0) | (upto > P.n_tokens ? kTokensOver : 0) |
+            (c1 > c0 && last > P.max_blocks ? kRowFull : 0) | (head + taken > P.n_free ? kPoolShort : 0);
     if (f) atomicOr(&S.flags, f);
   }
   __syncthreads();

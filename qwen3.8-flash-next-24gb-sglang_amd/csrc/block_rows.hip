@@ -5,26 +5,33 @@
 // over the positions p that the row sees; kc, vc are codes, sk, sv the scales of p's block and KV head.  A row is a
 // (query, q head) pair of one KV head; 16 of them are one side of a matrix product.
 //
-// One workgroup of 4 wavefronts per (16 rows, KV head, split of the positions); a wavefront takes every fourth tile of 32
-// positions.  Nothing is staged in LDS: both products take their 8-bit operand from registers as it was loaded.
+// One workgroup of 4 wavefronts per (16 rows, KV head, split of the positions); a wavefront takes every fourth tile of
+// 32 positions.  Nothing is staged in LDS: both products take their 8-bit operand from registers as it was loaded.
 //   S^T = K Q^T (v_mfma_f32_16x16x32_f16): lane (l, g) (l = lane % 16, g = lane / 16) loads 16 bytes of position l at a
 //     time; the k order of the product is the order of the bytes, and Q is loaded in the same order.
 //   The result gives a lane four positions (4 g + i) of row l in each of the tile's two halves: these eight weights are
-//     the lane's column of P^T in O^T += V^T P^T as they stand.  V^T's operand needs the same eight positions of one channel: a
-//     lane loads D / 16 channels of each of them and pairs the bytes of two positions (v_perm_b32) before the conversion.
+//     the lane's column of P^T in O^T += V^T P^T as they stand.  V^T's operand needs the same eight positions of one
+//     channel: a lane loads D / 16 channels of each of them and pairs the bytes of two positions (v_perm_b32) before
+//     the conversion.
 // Codes are exact in fp16.  The scale of K multiplies the fp32 scores.  The scale of V is folded into P, relative to a
-// running unit u: P holds w sv / u and O is kept in units of u, which changes only when a tile's scale leaves [u / 4, u]
-// (O is then multiplied by the ratio; two blocks of one tile whose scales differ by more than 4 take a product each).  The
-// softmax keeps a running maximum m per row that moves only when a tile exceeds it by more than 4 (in powers of two), and
-// P = 2^(x - m + 10): fp16 has weights down to 2^-24 of the largest before they lose bits, and up to 2^14 for a row whose
-// maximum lags.  Sums, scores and O are fp32.  bf16 queries are scaled by a power of two per row to fit fp16 (exact down
-// to 2^-14 of the row's largest entry, and to 2^-25 of it below).
+// running unit u: P holds w sv / u and O is kept in units of u, which changes only when a tile's scale leaves [u / 4,
+// u] (O is then multiplied by the ratio; two blocks of one tile whose scales differ by more than 4 take a product
+// each).  The softmax keeps a running maximum m per row that moves only when a tile exceeds it by more than 4 (in
+// powers of two), and P = 2^(x - m + 10): fp16 has weights down to 2^-24 of the largest before they lose bits, and up
+// to 2^14 for a row whose maximum lags.  Sums, scores and O are fp32.  bf16 queries are scaled by a power of two per
+// row to fit fp16 (exact down to 2^-14 of the row's largest entry, and to 2^-25 of it below).
 //
-// Decode is bound by the cache's bytes, each read once (counted: 269 MB for 262,144 positions of 2 heads, D 256): 45.3 us
-// there, 5.9 TB/s (a large copy 5.2), where more than half of the wavefronts' time is waiting for memory and the vector
-// instructions take 30 %, the matrix instructions 9 % of theirs; e4m3, 32 requests of 12,000 positions and less (204 MB)
-// 38.4 us, 5.3 TB/s; int8, 64 requests x 8 heads, D 128 (456 MB) 94 us, 4.9 TB/s.  Short calls are launch and load latency:
-// 777 positions of 2 heads 11 us with the merge in the launch.
+// So two things have fewer bits than 32, both because a matrix operand has 16: the weights, and bf16 queries' smallest
+// entries.  The row sums add the weights before that rounding here (they stand in fp32 registers), behind it in
+// block_tile.hip (a dot product with ones).  Half a step of fp16 is an eighth of a bf16 output's: against 64 bits those
+// are as far off as a form that holds fp32 throughout (relative 1.7e-3); fp16 outputs are 2.3 - 2.5e-4 off against
+// 2.1e-4, and fp32 outputs have the weights' error too.
+//
+// Decode is bound by the cache's bytes, each read once (counted: 269 MB for 262,144 positions of 2 heads, D 256): 45.4
+// us there, 5.9 TB/s (a large copy 5.2), where more than half of the wavefronts' time is waiting for memory and the
+// vector instructions take 28 %, the matrix instructions 8 % of theirs; e4m3, 32 requests of 16,384 positions and less
+// (204 MB) 37.5 us, 5.4 TB/s; int8, 64 requests x 8 heads, D 128 (456 MB) 96.7 us, 4.7 TB/s.  Short calls are launch
+// and load latency: 777 positions of 2 heads 12.6 us with the merge in the launch.
 #include "block_attn.h"
 
 using namespace kvt;
@@ -35,8 +42,8 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kTile = 32;
 constexpr int kMostSplits = 1024;
-// Positions of a table that the kernels take: their 32-bit positions run ahead of an item's last one, by the most in block_rows_kernel
-// (a wavefront asks for the block ids of its next 32 tiles, 4,096 positions).
+// Positions of a table that the kernels take: their 32-bit positions run ahead of an item's last one, by the most in
+// block_rows_kernel (a wavefront asks for the block ids of its next 32 tiles, 4,096 positions).
 constexpr int64_t kMostPositions = ((int64_t)1 << 31) - 8192;
 constexpr int kMostParts = 128;        // parts of a pair, at most, where the launch of equal shares merges them
 constexpr int kFew = 16;               // splits that the launch itself may merge, or a merge without LDS
@@ -50,8 +57,8 @@ KVT_DEV __amdgpu_buffer_rsrc_t part_rsrc(float* p, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(p, 0, bytes, 0x00020000);
 }
 
-// A part's weight in the merge of normalized parts, from its maximum and sum and the row's maximum.  Sums are below 2^45: times
-// 2^-45 no product with a part is larger than the part, and their sums stay finite.
+// A part's weight in the merge of normalized parts, from its maximum and sum and the row's maximum.  Sums are below
+// 2^45: times 2^-45 no product with a part is larger than the part, and their sums stay finite.
 KVT_DEV float weight_of(float m, float l, float M) { return m == -__builtin_inff() ? 0.0f : exp2_(m - M) * l * 0x1p-45f; }
 
 template <int BYTES> struct Raw { uint32_t w[BYTES / 4]; };
@@ -88,7 +95,8 @@ struct Join {
 // Tiles tile0 .. tile1 - 1 of an item and KV head: into out where they are all that the item has (whole), else as part
 // `slot`: its own result with its maximum and sum.  CHUNK: its rows may see different positions.
 template <int CODE, int QT, int D, bool CHUNK>
-KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, bool whole, int64_t slot, int ot, Join<CODE, D>& J) {
+KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, bool whole, int64_t slot, int ot,
+                    Join<CODE, D>& J) {
   constexpr int NC = D / 64;          // 16-byte chunks of a K row per lane
   constexpr int VB = D / 16;          // bytes (channels) of a V row per lane
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
@@ -107,7 +115,7 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
 #pragma unroll
   for (int c = 0; c < VB; ++c) acc[c] = f4{0, 0, 0, 0};
   float m = -__builtin_inff(), sum = 0.0f, unit = 0.0f, peak = 0.0f;
-  int poison = 0x7FFFFFFF;            // the wavefront's first position whose block has a V scale that is not finite (uniform)
+  int poison = 0x7FFFFFFF;            // the wavefront's first position of a V scale that is not finite (uniform)
 
   const uint32_t koff = (uint32_t)l * D + 16u * g, voff = 4u * g * D + (uint32_t)l * VB;
   const int64_t tbl = (int64_t)it.trow * P.stride;
@@ -162,7 +170,8 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
         for (int j = 0; j < 4; ++j) x[s][j] = sc[j] * f;
       }
       if (valid[0] + valid[1] < 32 || p0 + 32 > all_see) {
-        // positions past a row's end, in a block that is not there, or stale (their V may hold anything: it counts as 0)
+        // positions past a row's end, in a block that is not there, or stale (their V may hold anything: it counts as
+        // 0)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -307,13 +316,14 @@ KVT_DEV void attend(const Attn& P, const Item& it, int h, int tile0, int tile1, 
   }
 }
 
-// The merge of an item's parts by the workgroup that finishes last (counters: zero before and after every call): part 0 is in
-// slot s0, part k > 0 in slot sb + step k.  Parts cross XCDs, whose L2s do not see each other: they are stored and loaded at
-// device scope, and a workgroup counts itself when its stores have arrived.  Nobody waits for another workgroup.  The
-// parts are added in their order whoever merges them, as the merge by a second launch does: the same bits.
+// The merge of an item's parts by the workgroup that finishes last (counters: zero before and after every call): part 0
+// is in slot s0, part k > 0 in slot sb + step k.  Parts cross XCDs, whose L2s do not see each other: they are stored
+// and loaded at device scope, and a workgroup counts itself when its stores have arrived.  Nobody waits for another
+// workgroup.  The parts are added in their order whoever merges them, as the merge by a second launch does: the same
+// bits.
 //
-// A thread has four channels of a row at a time, and loads them of 16 parts at once: of its first row beside the parts' maxima.
-// Most items have no more parts (MANY: they may, D 64 and 128; at D 256 the registers would spill).
+// A thread has four channels of a row at a time, and loads them of 16 parts at once: of its first row beside the parts'
+// maxima.  Most items have no more parts (MANY: they may, D 64 and 128; at D 256 the registers would spill).
 template <int CODE, int D, bool MANY>
 KVT_DEV void merge_last(const Attn& P, const Item& it, int h, int64_t item, int parts, int64_t s0, int64_t sb, int step, int ot,
                         Join<CODE, D>& J) {
@@ -341,7 +351,8 @@ KVT_DEV void merge_last(const Attn& P, const Item& it, int h, int64_t item, int 
   const int row = threadIdx.x >> 4, lane = threadIdx.x & 15;   // 16 rows x 16 parts
   const auto read_ml = [&](int k) {
     const bool is = row < it.n_row && k < parts;
-    const float2 ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(rml, is ? (16 * slot(k) + row) * 8 : -8, 0, kSc1));
+    const float2 ml = __builtin_bit_cast(
+        float2, __builtin_amdgcn_raw_buffer_load_b64(rml, is ? (16 * slot(k) + row) * 8 : -8, 0, kSc1));
     return make_float2(is ? ml.x : -__builtin_inff(), ml.y);
   };
   const auto add = [&](int e, f4& O, float& L) {
@@ -424,12 +435,13 @@ __global__ __launch_bounds__(256, 2) void block_rows_kernel(const Attn P, int ot
   if (P.counters && used > 1) merge_last<CODE, D, false>(P, it, h, item, used, item * P.splits, item * P.splits, 1, ot, J);
 }
 
-// Decode in equal shares of all tiles of a call: the (request, KV head) pairs stand in a line, each as long as its tiles plus
-// kPad (what beginning with a pair costs, about: Q, the first loads, the join), and workgroup w takes [w share, (w + 1) share)
-// of it.  A pair that one workgroup has is written at once; of a pair that several have, each leaves a part, which the last
-// of them or a second launch merges.  A workgroup has at most two such pairs, its first (slot 2 w) and its last (2 w + 1): 2
-// slots per workgroup whatever the lengths are.  (With a fixed number of splits per pair, workgroups of a ragged batch are
-// short and unequal: 64 requests x 8 heads (D 128), up to 8,191 positions 117 us against 98.)
+// Decode in equal shares of all tiles of a call: the (request, KV head) pairs stand in a line, each as long as its
+// tiles plus kPad (what beginning with a pair costs, about: Q, the first loads, the join), and workgroup w takes [w
+// share, (w + 1) share) of it.  A pair that one workgroup has is written at once; of a pair that several have, each
+// leaves a part, which the last of them or a second launch merges.  A workgroup has at most two such pairs, its first
+// (slot 2 w) and its last (2 w + 1): 2 slots per workgroup whatever the lengths are.  (With a fixed number of splits
+// per pair, workgroups of a ragged batch are short and unequal: 64 requests x 8 heads (D 128), up to 8,191 positions
+// 117 us against 98.)
 constexpr int kPad = 8;
 
 // A request's table row and length; rows out of range hold nothing.
@@ -453,8 +465,8 @@ KVT_DEV uint32_t wave_scan(uint32_t v) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);   // lane 31 to the upper half
   return (uint32_t)x;
 }
-// The line of a call, per head, in steps of 2^shift tiles (the entry point picks the shift so that 32 bits hold it): its
-// length, where request r begins, and what r holds.
+// The line of a call, per head, in steps of 2^shift tiles (the entry point picks the shift so that 32 bits hold it):
+// its length, where request r begins, and what r holds.
 struct Line {
   uint32_t total, at;
   int r;
@@ -524,10 +536,10 @@ __global__ __launch_bounds__(256, 2) void block_decode_kernel(const Attn P, int 
       if (t0 < t1 || (tiles == 0 && a >= x0)) {
         const bool whole = t0 == 0 && t1 == tiles;
         attend<CODE, QT, D, false>(P, it, h, t0, t1, whole, 2 * (int64_t)w + (a > x0), ot, J);
-        if (D < 256 && P.counters && !whole) {// (at D 256 the merge's registers would spill)
+        if (D < 256 && P.counters && !whole) {      // (at D 256 the merge's registers would spill)
           const int w0 = (int)(a / share), w1 = (int)((a + (uint32_t)((tiles - 1) >> P.shift)) / share);
-          merge_last<CODE, D, (D < 256)>(P, it, h, (int64_t)r * P.H + h, w1 - w0 + 1, 2 * (int64_t)w0 + (a > (uint32_t)w0 * share),
-                                   2 * (int64_t)w0, 2, ot, J);
+          merge_last<CODE, D, (D < 256)>(P, it, h, (int64_t)r * P.H + h, w1 - w0 + 1,
+                                         2 * (int64_t)w0 + (a > (uint32_t)w0 * share), 2 * (int64_t)w0, 2, ot, J);
         }
         __syncthreads();                            // (J is free again)
       }
@@ -552,7 +564,8 @@ __global__ __launch_bounds__(256) void block_decode_merge_kernel(const Attn P, i
   const int w0 = (int)(a / share), w1 = (int)((a + (uint32_t)(max(tiles - 1, 0) >> P.shift)) / share);
   if (w0 == w1 || row >= P.gs) return;
   const auto part_of = [&](int w) { return (2 * (int64_t)w + (a > (uint32_t)w * share)) * 16 + row; };
-  // (the first eight parts beside their maxima: most pairs have no more; those that are not there are the last again, of no weight)
+  // (the first eight parts beside their maxima: most pairs have no more; those that are not there are the last again,
+  // of no weight)
   constexpr int kNow = 8;
   f4 o[kNow];
   float2 now[kNow];
@@ -586,8 +599,9 @@ __global__ __launch_bounds__(256) void block_decode_merge_kernel(const Attn P, i
   store_out4(P.out, ot, (int64_t)r * P.so_n + (int64_t)(h * P.gs + row) * P.so_h + d, O[0], O[1], O[2], O[3]);
 }
 
-// Merge of the splits of a row: one workgroup per (row, 64 channels, KV head and item).  A part is a split's own result with
-// its maximum m and sum l; their weights 2^(m - M) l / (the sum of these) go to LDS first, then groups of 16 lanes add up every NG-th split, all their loads in flight side by side.
+// Merge of the splits of a row: one workgroup per (row, 64 channels, KV head and item).  A part is a split's own result
+// with its maximum m and sum l; their weights 2^(m - M) l / (the sum of these) go to LDS first, then groups of 16 lanes
+// add up every NG-th split, all their loads in flight side by side.
 template <int NT>
 __global__ __launch_bounds__(NT) void block_merge_kernel(const Attn P, int D, int ot) {
   constexpr int NG = NT / 16;
@@ -684,7 +698,8 @@ void launch(const Attn& P, int items, int ot, hipStream_t st) {
     return;
   }
   block_decode_kernel<CODE, QT, D><<<P.shares, 256, 0, st>>>(P, ot);
-  if (P.shares > 1 && !P.counters) block_decode_merge_kernel<D><<<dim3((P.gs * (D / 4) + 255) / 256, P.H, P.n), 256, 0, st>>>(P, ot);
+  if (P.shares > 1 && !P.counters)
+    block_decode_merge_kernel<D><<<dim3((P.gs * (D / 4) + 255) / 256, P.H, P.n), 256, 0, st>>>(P, ot);
 }
 template <int CODE, int QT>
 void launch_d(const Attn& P, int D, int items, int ot, hipStream_t st) {
@@ -724,14 +739,16 @@ extern "C" int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q
                                 int Hq, int D, int code, const void* k8, const void* v8, const void* ks, const void* vs,
                                 int n_blocks, int block, const void* block_table, int64_t bt_stride, int n_rows,
                                 int max_blocks, const void* rows, float scale, int n_splits, void* part_o,
-                                void* part_ml, void* counters, void* out, int out_type, int64_t so_n, int64_t so_h, void* stream) {
+                                void* part_ml, void* counters, void* out, int out_type, int64_t so_n, int64_t so_h,
+                                void* stream) {
   Attn P;
   P.q = q, P.k8 = (const uint8_t*)k8, P.v8 = (const uint8_t*)v8, P.ks = (const float*)ks, P.vs = (const float*)vs;
   P.table = (const int32_t*)block_table, P.kv_lens = (const int32_t*)kv_lens, P.rows = (const int32_t*)rows;
-  // One workgroup merges a pair's parts inside the launch: up to kFew splits, or kMostParts parts, which is about the most that a
-  // pair can have of equal shares (one long request among short ones).  us per call, by a second launch / inside: 64 requests x 8
-  // heads (D 128), up to 8,191 positions 103 / 100, 32 x 8 up to 3,000 29.8 / 27.7, 32 x 4 up to 16,000 51.5 / 46.8; of one of them
-  // alone among short ones 20.9 / 16.3, 16.4 / 11.4, 21.7 / 23.0; 32 x 1 (16 q heads, 512 parts) 29.3 / 43.5.
+  // One workgroup merges a pair's parts inside the launch: up to kFew splits, or kMostParts parts, which is about the
+  // most that a pair can have of equal shares (one long request among short ones).  us per call, by a second launch /
+  // inside: 64 requests x 8 heads (D 128), up to 8,191 positions 103 / 100, 32 x 8 up to 3,000 29.8 / 27.7, 32 x 4 up
+  // to 16,000 51.5 / 46.8; of one of them alone among short ones 20.9 / 16.3, 16.4 / 11.4, 21.7 / 23.0; 32 x 1 (16 q
+  // heads, 512 parts) 29.3 / 43.5.
   const bool few = n_splits > 1 ? n_splits <= kFew : n_splits < -1 && D < 256 && -(n_splits / (H > 0 ? H : 1)) <= kMostParts;
   P.counters = few ? (int32_t*)counters : nullptr;
   P.cu = nullptr, P.out = out, P.part_o = (float*)part_o, P.part_ml = (float*)part_ml;
@@ -740,7 +757,8 @@ extern "C" int kvt_block_decode(const void* q, int64_t sq_n, int64_t sq_h, int q
   P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.causal = 0;
   P.splits = n_splits >= 0 ? n_splits : 1, P.shares = n_splits >= 0 ? 0 : -max(n_splits, -65536);
   P.item_rows = 16, P.tile = kTile, P.least = kWaves, P.single = 0, P.shift = 0;
-  while (P.shift < 31 && ((double)n * H * (((double)max_blocks * block / kTile + kPad) / (1 << P.shift) + 2) + P.shares) > 2e9) ++P.shift;
+  const double longest = (double)max_blocks * block / kTile + kPad;
+  while (P.shift < 31 && (double)n * H * (longest / (1 << P.shift) + 2) + P.shares > 2e9) ++P.shift;
   const int st = check(P, Hq, D, block, code, q_type, out_type);
   if (st != KVT_OK) return st;
   if ((P.splits > 1 || P.shares > 1) && (!part_o || !part_ml)) return KVT_EINVAL;
@@ -755,7 +773,8 @@ extern "C" int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int 
                                  const void* v8, const void* ks, const void* vs, int n_blocks, int block,
                                  const void* block_table, int64_t bt_stride, int n_rows, int max_blocks,
                                  const void* rows, int causal, float scale, int item_rows, int n_splits, void* part_o,
-                                 void* part_ml, void* counters, void* out, int out_type, int64_t so_n, int64_t so_h, void* stream) {
+                                 void* part_ml, void* counters, void* out, int out_type, int64_t so_n, int64_t so_h,
+                                 void* stream) {
   Attn P;
   P.q = q, P.k8 = (const uint8_t*)k8, P.v8 = (const uint8_t*)v8, P.ks = (const float*)ks, P.vs = (const float*)vs;
   P.table = (const int32_t*)block_table, P.kv_lens = (const int32_t*)kv_lens, P.rows = (const int32_t*)rows;
@@ -763,12 +782,13 @@ extern "C" int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int 
   P.cu = (const int32_t*)cu_q, P.out = out, P.part_o = (float*)part_o, P.part_ml = (float*)part_ml;
   P.sq_n = sq_n, P.sq_h = sq_h, P.so_n = so_n, P.so_h = so_h, P.stride = bt_stride, P.scale_log2 = scale * kLog2e;
   P.n = n, P.n_rows = n_rows, P.n_q = n_q, P.H = H, P.gs = H > 0 ? Hq / H : 0, P.n_blocks = n_blocks;
-  P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.splits = n_splits, P.causal = causal, P.shares = 0;
+  P.max_blocks = max_blocks, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.splits = n_splits;
+  P.causal = causal, P.shares = 0;
   const bool tiled = item_rows == kTileRows;
   P.item_rows = item_rows, P.tile = tiled ? tile_positions(D) : kTile;
-  // (requests of several lengths: splits of a multiple of 512 positions, or 256 where the call asks for that many of the table's
-  // width, so that the long requests' splits are not much longer than the others', and a short one is not split: 8 x 20 heads
-  // (D 64), 448 ragged queries over 1,500 ragged positions 52.5 -> 45.5 us)
+  // (requests of several lengths: splits of a multiple of 512 positions, or 256 where the call asks for that many of
+  // the table's width, so that the long requests' splits are not much longer than the others', and a short one is not
+  // split: 8 x 20 heads (D 64), 448 ragged queries over 1,500 ragged positions 52.5 -> 45.5 us)
   const int grain = (int64_t)max_blocks * block <= (int64_t)n_splits * 256 ? 256 : 512;
   P.least = !tiled ? kWaves : grain / P.tile;
   P.single = 0;

@@ -1,31 +1,32 @@
-// Quantizing write of a step's K/V rows into 8-bit blocks with one scale per (block, KV head) and side (kvt_block_store).
+// Quantizing write of a step's K/V rows into 8-bit blocks with one scale per (block, KV head) and side
+// (kvt_block_store).
 //
 // With a = max |x| over the rows that the call writes into a block (finite ones), need = the smallest power of two with
 // a / need <= Q (448 for e4m3, 127 for int8), within 2^-64 .. 2^122:
 //   s    = need where the call opens the block, else max(need, s_old) (an s_old that is not finite stays)
 //   old codes (rows that the request held in the block) -> rne(code * s_old / s) where s grew
 //   new codes = rne(x / s)
-// Powers of two, because a block fills up over many calls: x / s is exact, a growing scale moves the exponent of an e4m3
-// code and rounds nothing but subnormals (with s = a / Q every growth would round every code again), and the readers'
-// products with the scale are exact.  The price is up to one bit of int8's range.
+// Powers of two, because a block fills up over many calls: x / s is exact, a growing scale moves the exponent of an
+// e4m3 code and rounds nothing but subnormals (with s = a / Q every growth would round every code again), and the
+// readers' products with the scale are exact.  The price is up to one bit of int8's range.
 //
 // Bytes bound it: the rows are read once and the codes written once.  An item is a (request's block, KV head, side): a
 // request's tokens are consecutive, so a cache block is written by one workgroup or wavefront and its maximum needs no
-// atomics.  Which (request, block) an item is follows from the prefix sums of the token counts (find_request).  A thread keeps
-// its eight channels of NP rows as they are in memory between the maximum and the codes.  32,000 rows of 1,024 channels
-// (197 MB of bf16 or fp16 rows and codes) take 38 - 41 us for every block size and head length, 4.8 - 5.2 TB/s, a large copy's
-// rate; fp32 rows (328 MB) 62 - 65.
+// atomics.  Which (request, block) an item is follows from the prefix sums of the token counts (find_request).  A
+// thread keeps its eight channels of NP rows as they are in memory between the maximum and the codes.  32,000 rows of
+// 1,024 channels (197 MB of bf16 or fp16 rows and codes) take 38 - 41 us for every block size and head length, 4.8 -
+// 5.2 TB/s, a large copy's rate; fp32 rows (328 MB) 62 - 65.
 //
-// Up to 4,096 values a block an item is a wavefront, and a workgroup takes four heads of a block, whose rows are side by
-// side in memory; more values need the registers of four wavefronts.  With 256 threads for every item, heads apart: blocks of
-// 16 x 64 101 us, 16 x 128 59, 64 x 256 53.  Heads before blocks in the grid's order, for the same reason.  Magnitudes are
-// compared as bits, two at a time, and finite rows are converted without clamps: int8 from fp16 38 us, with three
-// instructions per value for the maximum and a clamp 51.
+// Up to 4,096 values a block an item is a wavefront, and a workgroup takes four heads of a block, whose rows are side
+// by side in memory; more values need the registers of four wavefronts.  With 256 threads for every item, heads apart:
+// blocks of 16 x 64 101 us, 16 x 128 59, 64 x 256 53.  Heads before blocks in the grid's order, for the same reason.
+// Magnitudes are compared as bits, two at a time, and finite rows are converted without clamps: int8 from fp16 38 us,
+// with three instructions per value for the maximum and a clamp 51.
 //
 // Calls of a few rows per request (decode steps) take a wavefront per item and a loop over its rows, read twice: 256
-// requests x 8 heads, blocks of 64 x 128, one row each 5.8 us against 12.9 with 256 threads, four rows 6.6 / 12.9; 32 x 2
-// heads (64 x 256) 3.4 / 3.6.  From eight rows on a request writes more than the loop's lanes hold, and blocks of 16 gain
-// nothing (6.2 / 6.0).
+// requests x 8 heads, blocks of 64 x 128, one row each 5.8 us against 12.9 with 256 threads, four rows 6.6 / 12.9; 32 x
+// 2 heads (64 x 256) 3.4 / 3.6.  From eight rows on a request writes more than the loop's lanes hold, and blocks of 16
+// gain nothing (6.2 / 6.0).
 #include "block_common.h"
 
 using namespace kvt;
@@ -71,13 +72,15 @@ KVT_DEV float elem(const Raw<DT>& r, int i) {
   return (float)as_h2(w)[i & 1];
 }
 
-// Magnitudes are ordered as their bits are (NaN above infinity): the largest one's bits, two at a time where they are 16.
+// Magnitudes are ordered as their bits are (NaN above infinity): the largest one's bits, two at a time where they are
+// 16.
 typedef uint16_t us2 __attribute__((ext_vector_type(2)));
 template <int DT> constexpr uint32_t kInfBits = DT == kBF16 ? 0x7F80u : DT == kF16 ? 0x7C00u : 0x7F800000u;
 template <int DT>
 KVT_DEV uint32_t top(uint32_t t, uint32_t w) {
   if constexpr (DT == kF32) return max(t, w & 0x7FFFFFFFu);
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, t), __builtin_bit_cast(us2, w & 0x7FFF7FFFu)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, t),
+                                                                __builtin_bit_cast(us2, w & 0x7FFF7FFFu)));
 }
 template <int DT>
 KVT_DEV float magnitude(uint32_t bits) {            // (of one element)
@@ -92,8 +95,8 @@ KVT_DEV uint32_t group_umax(uint32_t v) {
   return v;
 }
 
-// Codes of finite x, which are in range (|x * inv| <= 448 or 127; the largest fp32 is less than 127 * 2^122): no clamp.  int8: the sum with 1.5 * 2^23 is rounded to an integer, to
-// even, whose low byte is the code.
+// Codes of finite x, which are in range (|x * inv| <= 448 or 127; the largest fp32 is less than 127 * 2^122): no clamp.
+// int8: the sum with 1.5 * 2^23 is rounded to an integer, to even, whose low byte is the code.
 template <int CODE>
 KVT_DEV uint32_t pack4_plain(float a, float b, float c, float d, float inv) {
   if constexpr (CODE == kE4M3) {
@@ -106,8 +109,8 @@ KVT_DEV uint32_t pack4_plain(float a, float b, float c, float d, float inv) {
   }
 }
 
-// T threads per item (64: one wavefront, 256 / T heads per workgroup; 256: a workgroup).  NP rows of a thread, kept in registers;
-// NP = 0: any number, each read twice.
+// T threads per item (64: one wavefront, 256 / T heads per workgroup; 256: a workgroup).  NP rows of a thread, kept in
+// registers; NP = 0: any number, each read twice.
 template <int DT, int CODE, int D, int T, int NP>
 __global__ __launch_bounds__(256) void block_store_kernel(const Store P) {
   constexpr int TPR = D / 8;          // threads per row
@@ -150,7 +153,8 @@ __global__ __launch_bounds__(256) void block_store_kernel(const Store P) {
       for (int i = 0; i < NP; ++i) f(i * RPP + tr, x[i]);
     }
   };
-  // the largest magnitude's bits over the item (T == 256: also the barrier before which every thread has read the scale)
+  // the largest magnitude's bits over the item (T == 256: also the barrier before which every thread has read the
+  // scale)
   auto widest = [&](uint32_t t) {
     t = group_umax(t);
     if constexpr (T == 256) {
@@ -208,7 +212,7 @@ __global__ __launch_bounds__(256) void block_store_kernel(const Store P) {
     each([&](int q, Raw<DT> v) {
       if (q < held || q >= end) return;
 #pragma unroll
-      for (int c = 0; c < Raw<DT>::N; ++c) asm volatile("" : "+v"(v.w[c]));   // (converted here, not for all rows ahead: registers)
+      for (int c = 0; c < Raw<DT>::N; ++c) asm volatile("" : "+v"(v.w[c]));   // (converted here, not all rows ahead)
       u2v c;
       c.x = pack(elem<DT>(v, 0), elem<DT>(v, 1), elem<DT>(v, 2), elem<DT>(v, 3));
       c.y = pack(elem<DT>(v, 4), elem<DT>(v, 5), elem<DT>(v, 6), elem<DT>(v, 7));

@@ -4,22 +4,25 @@
 // A row is a (query, q head) pair of one KV head, in that order; one workgroup of 4 wavefronts has 128 of them (32 per
 // wavefront) and walks the positions that they see in tiles of T.  The 256 threads convert a tile's codes to fp16 once,
 // into LDS, and the four wavefronts multiply from there:
-//   S^T = K Q^T on v_mfma_f32_32x32x16_f16 (A = 32 positions from LDS, B = the wavefront's 32 rows in registers).  A lane
-//     gets 16 scores of one row, the other 16 of the tile's 32 sit in lane ^ 32: the row maximum takes one cross-lane step.
-//   O^T += V^T P^T: the weights stay where they are (register 8 s + j of lane (l, g) is position 16 s + 8 (j / 4) + 4 g + j % 4,
-//     its operand's k), and V^T is stored so that these eight positions of a channel are 16 consecutive bytes.  Each product
-//     covers 16 positions, i.e. one block of the cache, so a block's V scale is one factor for the whole operand.
-// Two LDS buffers: a tile's codes are loaded into registers before the products of the tile before, converted and stored
-// behind them; one barrier per tile.  Positions' block ids are loaded a tile ahead of the codes.
-// LDS rows are padded by 16 bytes (V^T at D = 256: 16-byte pieces in an order that depends on the channel), which spreads the
-// operand reads (16 bytes per lane, 32 consecutive rows) over the banks.
-// T = 32 positions at D = 256, 64 below: 32 KB of fp16 per buffer, so that two workgroups (D = 64: three, 16 KB) fit a CU, whose
-// wavefronts run their softmax under each other's products.
+//   S^T = K Q^T on v_mfma_f32_32x32x16_f16 (A = 32 positions from LDS, B = the wavefront's 32 rows in registers).  A
+//     lane gets 16 scores of one row, the other 16 of the tile's 32 sit in lane ^ 32: the row maximum takes one
+//     cross-lane step.
+//   O^T += V^T P^T: the weights stay where they are (register 8 s + j of lane (l, g) is position 16 s + 8 (j / 4) + 4 g
+//     + j % 4, its operand's k), and V^T is stored so that these eight positions of a channel are 16 consecutive bytes.
+//     Each product covers 16 positions, i.e. one block of the cache, so a block's V scale is one factor for the whole
+//     operand.
+// Two LDS buffers: a tile's codes are loaded into registers before the products of the tile before, converted and
+// stored behind them; one barrier per tile.  Positions' block ids are loaded a tile ahead of the codes.  LDS rows are
+// padded by 16 bytes (V^T at D = 256: 16-byte pieces in an order that depends on the channel), which spreads the
+// operand reads (16 bytes per lane, 32 consecutive rows) over the banks.  T = 32 positions at D = 256, 64 below: 32 KB
+// of fp16 per buffer, so that two workgroups (D = 64: three, 16 KB) fit a CU, whose wavefronts run their softmax under
+// each other's products.
 //
-// Matrix and vector instructions bound it together: causal prompts of 10,001 tokens, 16 / 2 heads, D 256, e4m3 880 us, 930
-// TFLOP/s (a large library product 1,192): the matrix pipes are busy 42 % of the cycles, 7 vector instructions stand beside
-// each matrix instruction, a third of the wavefronts' time is waiting (barrier, LDS); 8,192 tokens, 32 / 8 heads, D 128 646 us,
-// 850 TFLOP/s; 16 / 16, D 64 220 us, 624 TFLOP/s; int8 codes take 5 - 7 % longer.
+// Matrix and vector instructions bound it together: causal prompts of 10,001 tokens, 16 / 2 heads, D 256, e4m3 875 us,
+// 936 TFLOP/s (a large library product 1,192): the matrix pipes are busy 42 % of the cycles, 7 vector instructions
+// stand beside each matrix instruction, a third of the wavefronts' time is waiting (barrier, LDS); 8,192 tokens, 32 / 8
+// heads, D 128 620 us, 887 TFLOP/s; 16 / 16, D 64 210 us, 656 TFLOP/s; int8 codes take 2 - 5 % longer.  At D 256 the
+// kernels have 252 - 254 of 256 registers, and none is spilled.
 #include "block_attn.h"
 
 using namespace kvt;
@@ -43,8 +46,8 @@ KVT_DEV float sum_xor32(float v) {
 constexpr int kDsRead = 0x100, kMfma = 0x8;   // instruction classes of the scheduling hints
 constexpr float kLeast = 0x1p-120f;   // (a factor of 0 would make a masked score, -inf, a NaN)
 
-// The largest of three (one v_maximum3_f32; fmaxf of a matrix product's result costs a canonicalizing v_max_f32 x, x each).  Not as
-// asm: the compiler sees no asm read the result of a matrix product, and puts no wait before it.
+// The largest of three (one v_maximum3_f32; fmaxf of a matrix product's result costs a canonicalizing v_max_f32 x, x
+// each).  Not as asm: the compiler sees no asm read the result of a matrix product, and puts no wait before it.
 KVT_DEV float max3(float a, float b, float c) {
   return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
@@ -58,8 +61,8 @@ template <int D>
 struct Tile {
   static constexpr int T = D == 256 ? 32 : 64;
   static constexpr int KP = 2 * D + 16;         // bytes per K row (a position)
-  // V^T rows (a channel each): 16-byte pieces in an order that depends on the channel, where T = 32 (the padding would not
-  // leave room for what D = 256 keeps of Q in LDS), else padded
+  // V^T rows (a channel each): 16-byte pieces in an order that depends on the channel, where T = 32 (the padding would
+  // not leave room for what D = 256 keeps of Q in LDS), else padded
   static constexpr int VP = T == 32 ? 64 : 2 * T + 16;
   static KVT_DEV int piece(int channel, int i) { return T == 32 ? i ^ (channel >> 2 & 3) : i; }
   static constexpr int QL = D == 256 ? 3 : 0;   // operands of Q that are kept in LDS: the registers hold no more than 13
@@ -95,8 +98,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
   __shared__ NanAt<CODE, D> nans;
   const int tid = threadIdx.x, lane = tid & 63, l = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // head fastest: with H = 2, 4 or 8 the workgroups of a head share the caches of the same XCDs; the last rows, which see
-  // the most positions, first
+  // head fastest: with H = 2, 4 or 8 the workgroups of a head share the caches of the same XCDs; the last rows, which
+  // see the most positions, first
   const int h = blockIdx.x % P.H, w = items - 1 - (int)(blockIdx.x / P.H), split = blockIdx.y;
   const Item it = item_of(P, w);
   if (it.n_row == 0) return;
@@ -126,9 +129,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
   const int all_see = uniform(any_row ? sees(P, it, first_row / P.gs) : 0);   // positions that every row of the wavefront sees
   const int most_see = uniform(any_row ? sees(P, it, last_row / P.gs) : 0);   // and that any of them sees
 
-  // This thread's share of a tile: 16-byte pieces tid % TPK, + TPK, .. of K row tid / TPK; channels vd .. vd + 3 of V rows vrow +
-  // {0 .. 3, 8 .. 11}.  A wavefront's rows all lie in the 16 positions `sub` of the tile, i.e. in one block: its id and the
-  // addresses' bases are uniform.
+  // This thread's share of a tile: 16-byte pieces tid % TPK, + TPK, .. of K row tid / TPK; channels vd .. vd + 3 of V
+  // rows vrow + {0 .. 3, 8 .. 11}.  A wavefront's rows all lie in the 16 positions `sub` of the tile, i.e. in one
+  // block: its id and the addresses' bases are uniform.
   const int sub = T == 32 ? wave >> 1 : wave;
   const int vc = 2 * sub + (lane & 1), vd = 4 * ((lane >> 1) + (T == 32 ? 32 * (wave & 1) : 0));
   const int vrow = 16 * sub + 4 * (lane & 1);
@@ -138,11 +141,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
   const int64_t head = (int64_t)h * (D << P.log2b);
   const uint32_t block_bytes = (uint32_t)P.H * (D << P.log2b);        // (of one block: < 2^32, the entry point sees to it)
 
-  // At D = 256 the registers hold only one side of the next tile at a time: K's codes under the first product, V's under the
-  // second, and addresses are computed where they are used.
+  // At D = 256 the registers hold only one side of the next tile at a time: K's codes under the first product, V's
+  // under the second, and addresses are computed where they are used.
   constexpr bool kApart = D == 256;
-  // At D = 64 both halves of a tile are multiplied with Q before the first one's softmax, under which the second product runs
-  // (8,192 tokens, 16 heads: 249 -> 220 us, 624 TFLOP/s; at D = 128, whose products are twice as long, 641 -> 646).
+  // At D = 64 both halves of a tile are multiplied with Q before the first one's softmax, under which the second
+  // product runs (8,192 tokens, 16 heads: 249 -> 220 us, 624 TFLOP/s; at D = 128, whose products are twice as long, 641
+  // -> 646).
   constexpr bool kBoth = D == 64;
 
   // (no branch around a load: the wait for it would move to where the paths join)
@@ -218,7 +222,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
         const uint32_t u = c < 2 ? lo[j] : hi[j];
         y[j] = c & 1 ? pair<CODE, true>(u) : pair<CODE, false>(u);
       }
-      *reinterpret_cast<h8*>(b.v + (vd + c) * C::VP + 16 * C::piece(vd, vc)) = h8{y[0].x, y[0].y, y[1].x, y[1].y, y[2].x, y[2].y, y[3].x, y[3].y};
+      *reinterpret_cast<h8*>(b.v + (vd + c) * C::VP + 16 * C::piece(vd, vc)) =
+          h8{y[0].x, y[0].y, y[1].x, y[1].y, y[2].x, y[2].y, y[3].x, y[3].y};
     }
     if (checked) nans_of(tile, b);
   };
@@ -322,14 +327,14 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
           const float a = m1 == m ? 1.0f : exp2_(m - m1);
           sum *= a, part *= a;
           m = m1;
-          lift = kLift - fmaxf(m, -0x1p120f);                        // (a row that has seen nothing: 2^-inf is 0 for any of these)
+          lift = kLift - fmaxf(m, -0x1p120f);          // (a row that has seen nothing: 2^-inf is 0 for any of these)
 #pragma unroll
           for (int c = 0; c < DT; ++c) acc[c] *= a;
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          // V's scale relative to the unit (ru) goes into the exponent: P = 2^(x - m + 10 + log2 ru), and the row sum adds P / ru.
-          // Most halves have the scale of the one before.
+          // V's scale relative to the unit (ru) goes into the exponent: P = 2^(x - m + 10 + log2 ru), and the row sum
+          // adds P / ru.  Most halves have the scale of the one before.
           if (__float_as_int(vs[s]) != last) {
             last = __float_as_int(vs[s]);
             if (vs[s] > unit || (vs[s] > 0.0f && vs[s] < 0.25f * unit)) {
@@ -376,9 +381,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void block_tile_kernel(const 
       convert_v(tile + 1, id, rv, next, checked);
       __syncthreads();
     };
-    // Tiles that some row does not see to their end are the last few: only those (each as the next tile, behind the products) are
-    // searched for NaN codes, in a loop of their own.  In one loop the search takes registers that spill at D = 256 (10,001
-    // tokens 912 -> 933 us).
+    // Tiles that some row does not see to their end are the last few: only those (each as the next tile, behind the
+    // products) are searched for NaN codes, in a loop of their own.  In one loop the search takes registers that spill
+    // at D = 256 (10,001 tokens 912 -> 933 us).
     const int plain = CODE == kE4M3 ? min(max(fewest / T - 1, tile0), tile1) : tile1;
     int tile = tile0;
     for (; tile < plain; ++tile) step(tile, false);

@@ -67,7 +67,8 @@ def test_scales_that_are_not_finite(kvt_pkg, monkeypatch, kernel, kv, Hq, H, D, 
            seed=D + B)
 
 
-@pytest.mark.parametrize("kernel,splits", [("decode", -9), ("decode", -40)] + [(k, s) for k in ("decode", 16, 128) for s in (2, 7, 30)])
+@pytest.mark.parametrize("kernel,splits",
+                         [("decode", -9), ("decode", -40)] + [(k, s) for k in ("decode", 16, 128) for s in (2, 7, 30)])
 @pytest.mark.parametrize("D", [64, 256])
 def test_scales_that_are_not_finite_in_parts(kvt_pkg, monkeypatch, kernel, splits, D):
     """The same where the positions are split: a part without any finite score, merged in the launch and behind it."""
@@ -75,7 +76,8 @@ def test_scales_that_are_not_finite_in_parts(kvt_pkg, monkeypatch, kernel, split
     new = [1] * 3 if kernel == "decode" else [300, 40, 64]
     bad = {(0, lp): (NAN, NAN) for lp in range(26, 31)}
     for ws in (None, {}):
-        _check(monkeypatch, kernel, "fp8", 8, 2, D, 64, new, lens, {**bad, (1, 0): (None, NAN)}, splits=splits, seed=5, workspace=ws)
+        _check(monkeypatch, kernel, "fp8", 8, 2, D, 64, new, lens, {**bad, (1, 0): (None, NAN)}, splits=splits, seed=5,
+               workspace=ws)
 
 
 @pytest.mark.parametrize("kernel", [16, 128])
@@ -189,7 +191,8 @@ def test_a_padded_step(kvt_pkg, counts):
         got = c.prefill(0, plan, q[:rows], out=out)
         assert got is out and bool((out[n:] == 5.0).all())
         val = [ref.values(x8[0].cpu()) * s[0].cpu().double()[..., None, None] for x8, s in ((c.k8, c.ks), (c.v8, c.vs))]
-        want = ref.attention(q[:n].cpu().double(), prefix(counts), counts, seqs.tolist(), c.block_table.tolist(), *val, True, D ** -0.5)
+        want = ref.attention(q[:n].cpu().double(), prefix(counts), counts, seqs.tolist(), c.block_table.tolist(), *val,
+                             True, D ** -0.5)
         for y in (out, c.prefill(0, plan, q[:rows])):
             ref.close(y[:n], *want, D)
         c.check()

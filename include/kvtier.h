@@ -374,6 +374,68 @@ int kvt_block_prefill(const void* q, int64_t sq_n, int64_t sq_h, int q_type, con
                       int item_rows, int n_splits, void* part_o, void* part_ml, void* counters, void* out, int out_type,
                       int64_t so_n, int64_t so_h, void* stream);
 
+/* ------------------------------------------------------------------------- a block cache within a budget */
+
+/* Rotary positions of q [n_tokens, Hq, D] and k [n_tokens, Hk, D] (NULL: none; dtype codes as above, element strides, unit
+ * last stride) into out_q / out_k: the first rot channels are pairs (i, i + rot / 2), or (2 i, 2 i + 1) where interleaved, each
+ * rotated by position * inv_freq[i] (fp64 [rot / 2], radians; the angle is formed in 64 bits) and times `scale`; inverse:
+ * by minus that.  The others are copied.  out == in (with the same strides) is in place; other overlaps are not served.
+ * cu NULL: positions int32 or int64 [n_tokens].  Else positions int32 [n] are lengths whose last cu[j+1] - cu[j] positions
+ * are rows cu[j] .. cu[j+1] - 1; ahead[rows[j]] (NULL: 0; rows NULL: j; out of n_rows: 0) is added; rows behind cu[n] are
+ * left as they are.  rot even, 2 <= rot <= D <= 256; n <= 4,096; n_tokens < 2^24. */
+int kvt_rope(const void* q, int64_t sq_n, int64_t sq_h, int Hq, void* out_q, int64_t oq_n, int64_t oq_h, const void* k,
+             int64_t sk_n, int64_t sk_h, int Hk, void* out_k, int64_t ok_n, int64_t ok_h, int dtype, int n_tokens, int D,
+             int rot, const void* inv_freq, const void* positions, int positions_are_int64, const void* cu, int n,
+             const void* rows, const void* ahead, int n_rows, float scale, int interleaved, int inverse, void* stream);
+
+/* Attention weight of each entry: out[row, h, p] = (p < since[j] ? weights[row, h, p] : 0) + the sum over request j's queries
+ * that see p and the q heads of KV head h of softmax(scale q K^T), for p < kv_lens[j]; weights and out fp32 with element
+ * strides of row and head, unit last stride, max_blocks * block entries, by table row (out may be weights).  since NULL: the
+ * first position of the call's queries.  cu_q NULL: one query per request, n_q >= n rows; else rows cu_q[j] .. cu_q[j+1] (at
+ * most n_q) are request j's last positions and see the entries up to their own.  A query that sees nothing adds nothing;
+ * one that sees a NaN or a block whose scale is not finite makes NaN of every entry that it sees.  The table rows of a
+ * call's requests have to be distinct.  Types, sizes and limits of q, k8, ks and the table as kvt_block_decode.
+ * work: fp32, 16-byte aligned; with cap = max_blocks * block: cu_q NULL: n * Hq * cap + n * H * splits * 32; else
+ * n_q * Hq * 2, splits times that more where splits > 1, and row_splits * n * H * cap where row_splits > 1.  splits (at most 1,024): workgroups that share the entries that a row or a tile of rows sees; row_splits
+ * (1,024): those that share a request's rows; pos_splits: those that share its entries.  Results depend on the first two
+ * by the order of fp32 sums only.  Calls that share work must not overlap. */
+int kvt_block_weigh(const void* q, int64_t sq_n, int64_t sq_h, int q_type, const void* cu_q, int n_q, const void* kv_lens,
+                    int n, int H, int Hq, int D, int code, const void* k8, const void* ks, int n_blocks, int block,
+                    const void* block_table, int64_t bt_stride, int n_rows, int max_blocks, const void* rows, float scale,
+                    const void* since, const void* weights, int64_t sw_r, int64_t sw_h, void* out, int64_t so_r,
+                    int64_t so_h, int splits, int row_splits, int pos_splits, void* work, int64_t work_floats, void* stream);
+
+/* The `budget` entries that a request (kv_lens[j] entries, at most cap) keeps of each KV head, into src int32
+ * [n, H, budget]: entries below `sinks`, those at positions >= length + evicted - recent, then by weight, equal ones by the
+ * lower entry, NaN below all.  src[e] is the entry that goes to place e: e where that stays; entries from behind the budget,
+ * ascending, take the free places, ascending.  A request of no more than `budget` entries keeps all: e below its length, -1
+ * behind.  pos (int32, strides of row and head), held and evicted (int32 by table row), all or none: entry e sits at
+ * position pos[e] if e < held, else at e + evicted (none: at e).  recent + sinks <= budget; n * H < 2^22.  work: int32
+ * [n * H * budget]. */
+int kvt_block_keep(const void* weights, int64_t sw_r, int64_t sw_h, const void* kv_lens, int n, int H, int n_rows,
+                   const void* rows, int64_t cap, int budget, int recent, int sinks, const void* pos, int64_t sp_r,
+                   int64_t sp_h, const void* held, const void* evicted, void* src, void* work, void* stream);
+
+/* Moves the entries of requests with kv_lens[j] > budget to where src has them: codes of both sides, and weights and pos
+ * (either may be NULL; pos with held and evicted, as above; every entry below the budget gets its pos).  budget is a
+ * multiple of the block size.  A block that gets another entry takes as scale the smallest power of two that holds its rows'
+ * finite values in the codes' range (within 2^-64 .. 2^122) and its rows are rounded to it; one of whose rows has a scale
+ * that is not finite becomes NaN with it.  Other blocks are left as they are.  An entry of src that is neither e nor in
+ * [budget, kv_lens[j]), or whose block is not there, stays.  n * H * budget / block < 2^24. */
+int kvt_block_evict(const void* src, const void* kv_lens, int n, int H, int D, int code, void* k8, void* v8, void* ks,
+                    void* vs, int n_blocks, int block, const void* block_table, int64_t bt_stride, int n_rows,
+                    int max_blocks, const void* rows, int budget, void* weights, int64_t sw_r, int64_t sw_h, void* pos,
+                    int64_t sp_r, int64_t sp_h, const void* held, const void* evicted, void* stream);
+
+/* Cuts table rows seqs[j] of more than `budget` entries: their blocks behind it return in front of
+ * free_list[*free_head] in request order, kv_lens[j] = min(length, budget), *next_head the list's head after that.  commit:
+ * their table entries become -1, seq_lens[row] = held[row] = budget, evicted[row] += the entries cut (held and evicted: both
+ * or none), *free_head = *next_head.  status (may be NULL): 8 a row out of range or listed twice (kv_lens 0), 16 more blocks
+ * than the list had handed out are or-ed in.  n <= 1,024. */
+int kvt_block_trim(int n, const void* seqs, void* seq_lens, int rows, void* block_table, int64_t bt_stride, int max_blocks,
+                   void* free_list, int n_free, void* free_head, int block, int budget, void* held, void* evicted,
+                   void* kv_lens, void* next_head, void* status, int commit, void* stream);
+
 /* ----------------------------------------------------------------------------- lazy backing (HIP VMM) */
 
 /* Lazily backed device memory for the KV pool (reference: patches/kv_lazy.py -- the pool is reserved as address

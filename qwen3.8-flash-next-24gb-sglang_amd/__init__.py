@@ -6,6 +6,8 @@ Modules:
   tiered_kv_pool  MHATokenToKVPoolTiered / Int4 / Int8 pool classes
   kvt             position-indexed (evict) cache, page allocator, split-K decode attention
   block_kv        8-bit paged cache with a scale per block: block plan, quantizing write, decode and chunk attention
+  block_evict     the block cache within a budget: accumulated attention weight, eviction, blocks given back
+  rope            rotary positions of queries and keys
   build           compiles libkvtier.so
 """
 __version__ = "0.1.0"

@@ -1,0 +1,240 @@
+"""Eviction from the 8-bit block cache: a conversation that grows without end keeps a budget of entries, the ones that
+its queries have attended to most, with the first and the most recent positions among them.
+
+    cache = BlockKVCache(..., evicting=True)                        # with weights and positions per entry
+    plan = cache.plan(seqs, counts, n_tokens)
+    for layer: q, k = cache.rotate(plan, q, k, inv_freq, scale)     # positions go on where entries were evicted
+               cache.append(layer, plan, k, v)
+               out = cache.decode(layer, plan, q)
+               cache.weigh_decode(layer, plan, q)                   # kvt_block_weigh: the attention weight of each entry
+    cache.evict(seqs, budget, recent, sinks)                        # kvt_block_keep and _evict per layer, kvt_block_trim
+
+Every KV head keeps its own entries, all of them the same number, so the heads and layers share one block table.  Entries
+that stay below the budget stay where they are, and those from behind it fill the places that become free: a cache's
+entries are in no order of positions after that, which attention does not ask for.  All of it happens on the device,
+without host lengths, and captures into a graph.  The functions take the buffers themselves:
+
+    weights fp32 [rows, H, width]      accumulated attention weight of each entry
+    pos int32 [rows, H, width], held int32 [rows], evicted int32 [rows]
+                                       entry e of a table row sits at position pos[e] of its conversation if e < held,
+                                       else (it was never moved) at e + evicted
+with width >= max_blocks * block.  The reference has no counterpart.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .block_kv import BLOCKS, CODE, FREE_OVER, _grown, _i32, _pool, _rows16, _stream
+
+# Workgroups of a launch that few requests are split for.
+_WORKGROUPS = 2048
+
+
+@dataclass
+class BlockTrim:
+    """What a trim leaves: kv_lens int32 [n] (the requests' lengths after it), next_head int32 [1] (of the free list)."""
+    kv_lens: torch.Tensor
+    next_head: torch.Tensor
+
+
+def _per_entry(name: str, x: torch.Tensor, dtype: torch.dtype, rows: int, H: int, width: int) -> None:
+    assert x.dtype == dtype and x.dim() == 3 and x.stride(2) == 1, f"{name} must be {dtype} [rows, H, width], unit last stride"
+    if x.shape[0] < rows or x.shape[1] != H or x.shape[2] < width:
+        raise ValueError(f"{name} of {tuple(x.shape)} for {rows} rows x {H} heads x {width} entries")
+
+
+def kvt_block_weigh(q: torch.Tensor, k8: torch.Tensor, ks: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
+                    weights: torch.Tensor, cu_q: Optional[torch.Tensor] = None, seqs: Optional[torch.Tensor] = None,
+                    since: Optional[torch.Tensor] = None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                    workspace: Optional[dict] = None) -> torch.Tensor:
+    """Add to each entry's weight the attention that the step's queries pay it: softmax(scale q K^T), summed over the
+    queries that see the entry and the q heads of its KV head.
+
+    q [rows, Hq, D] (bf16 / fp16).  cu_q None: one query per request, which sees all kv_lens[j] entries.  cu_q (int32 [n + 1]):
+    request j owns rows cu_q[j] .. cu_q[j + 1]; they are its last positions and each sees the entries up to its own, as in
+    kvt_block_prefill.  They may be the end of a longer chunk: its last queries alone, as a sample of all.
+    Entries from since[j] on (int32 [n]; default: the call's own positions) start from zero, whatever `weights` holds there;
+    since = 0 weighs anew.  The sums go to `out` (default: weights itself; else a tensor of its own: a step that may be
+    taken back), entries behind kv_lens[j] are left as they are.  A query that sees nothing adds nothing; one that sees a
+    NaN, or a block whose scale is not finite, makes NaN of every entry that it sees.  Rows of seqs have to be distinct.
+    scale: > 0, default D ** -0.5.  workspace as in kvt_block_decode: its buffers follow from the table's width (one query
+    per request: 4 * Hq bytes per entry of every request)."""
+    n = kv_lens.numel()
+    nb, H, B, D = _pool(k8, k8, ks, ks, block_table, n, seqs)
+    assert q.dim() == 3 and q.dtype in (torch.bfloat16, torch.float16), "queries are bf16 or fp16 [rows, Hq, D]"
+    rows, Hq, d = q.shape
+    assert d == D, f"queries of {d} channels over blocks of {D}"
+    if H == 0 or Hq == 0 or Hq % H or Hq // H > 16:
+        raise ValueError(f"{Hq} q heads over {H} KV heads: a multiple, at most 16 each, is served")
+    _i32("kv_lens", kv_lens, n)
+    if cu_q is not None:
+        _i32("cu_q", cu_q, n + 1)
+    elif rows != n:
+        raise ValueError(f"{rows} queries for {n} requests")
+    if since is not None:
+        _i32("since", since, n)
+    max_blocks = block_table.shape[1]
+    cap = max_blocks * B
+    _per_entry("weights", weights, torch.float32, block_table.shape[0], H, cap)
+    if out is None:
+        out = weights
+    else:
+        _per_entry("out", out, torch.float32, block_table.shape[0], H, cap)
+    if n == 0:
+        return out
+    st = _stream(q, k8, ks, block_table, kv_lens, weights, cu_q, seqs, since, out)
+    q, qp, qn, qh = _rows16(q, 8)
+    gs, pairs = Hq // H, n * H
+    row_splits = 1
+    if cu_q is None:
+        splits = max(1, min(1024, _WORKGROUPS // pairs, -(-cap // 256)))
+        pos_splits = max(1, min(_WORKGROUPS // pairs, -(-cap // 1024)))
+        need = pairs * gs * cap + pairs * splits * 32
+    else:
+        items = rows * gs // 256 + n
+        splits = max(1, min(1024, _WORKGROUPS // (items * H), -(-cap // 256)))
+        pos_splits = max(1, min(2 * _WORKGROUPS // pairs, -(-cap // 256)))
+        row_splits = max(1, min(1024, _WORKGROUPS // (pairs * pos_splits), -(-rows * gs // 512)))
+        need = rows * Hq * 2 * (splits + 1) + (row_splits * pairs * cap if row_splits > 1 else 0)
+    ws = {} if workspace is None else workspace             # (held until the launch)
+    work = _grown(ws, "weigh", need, q)
+    _lib.call("kvt_block_weigh", qp, qn, qh, _lib.DTYPE_CODE[q.dtype], _lib.ptr(cu_q), rows, kv_lens.data_ptr(), n, H, Hq, D,
+              CODE[k8.dtype], k8.data_ptr(), ks.data_ptr(), nb, B, block_table.data_ptr(), block_table.stride(0),
+              *block_table.shape, _lib.ptr(seqs), D ** -0.5 if scale is None else float(scale), _lib.ptr(since),
+              weights.data_ptr(), weights.stride(0), weights.stride(1), out.data_ptr(), out.stride(0), out.stride(1), splits,
+              row_splits, pos_splits, work.data_ptr(), work.numel(), st)
+    return out
+
+
+def _cut(budget: int, block: int) -> None:
+    if block not in BLOCKS:
+        raise ValueError(f"blocks of {block} tokens: {BLOCKS} are served")
+    if budget < block or budget % block:
+        raise ValueError(f"a budget of {budget} entries: a multiple of the block size {block} is served")
+
+
+def kvt_block_keep(weights: torch.Tensor, kv_lens: torch.Tensor, budget: int, seqs: Optional[torch.Tensor] = None,
+                   recent: int = 0, sinks: int = 0, pos: Optional[torch.Tensor] = None,
+                   held: Optional[torch.Tensor] = None, evicted: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None, workspace: Optional[dict] = None) -> torch.Tensor:
+    """Choose the `budget` entries that each request and KV head keeps: entries below `sinks`, those at its last `recent`
+    positions, and the heaviest of the others; equal weights by the lower entry, NaN below all.
+
+    Returns src int32 [n, H, budget] (or writes `out`): the entry that goes to place e.  It is e itself where that stays;
+    entries from behind the budget, in ascending order, go to the places that become free, in ascending order.  A request of
+    no more than `budget` entries keeps all: src is e up to its length, -1 behind.  pos, held and evicted (together; see the
+    module) say which positions moved entries have: without them, entry e sits at position e."""
+    assert weights.dtype == torch.float32 and weights.dim() == 3 and weights.stride(2) == 1
+    rows, H, width = weights.shape
+    n = kv_lens.numel()
+    _i32("kv_lens", kv_lens, n)
+    if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
+        raise ValueError(f"a budget of {budget} entries with {sinks} first and {recent} recent ones")
+    if seqs is not None:
+        _i32("seqs", seqs, n)
+    elif rows < n:
+        raise ValueError(f"{n} requests, but weights has {rows} rows")
+    if (pos is None) != (held is None) or (pos is None) != (evicted is None):
+        raise ValueError("pos, held and evicted go together")
+    if pos is not None:
+        _per_entry("pos", pos, torch.int32, rows, H, width)
+        _i32("held", held, rows)
+        _i32("evicted", evicted, rows)
+    if out is None:
+        out = torch.empty(n, H, budget, dtype=torch.int32, device=weights.device)
+    else:
+        assert out.dtype == torch.int32 and out.shape == (n, H, budget) and out.is_contiguous()
+    if n == 0 or H == 0:
+        return out
+    if width == 0:
+        raise ValueError("weights of no entries")
+    st = _stream(weights, kv_lens, seqs, pos, held, evicted, out)
+    ws = {} if workspace is None else workspace             # (held until the launch)
+    work = _grown(ws, "keep", n * H * budget, weights, torch.int32)
+    sp = (0, 0) if pos is None else (pos.stride(0), pos.stride(1))
+    _lib.call("kvt_block_keep", weights.data_ptr(), weights.stride(0), weights.stride(1), kv_lens.data_ptr(), n, H, rows,
+              _lib.ptr(seqs), width, budget, recent, sinks, _lib.ptr(pos), *sp, _lib.ptr(held), _lib.ptr(evicted),
+              out.data_ptr(), work.data_ptr(), st)
+    return out
+
+
+def kvt_block_evict(src: torch.Tensor, kv_lens: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, ks: torch.Tensor,
+                    vs: torch.Tensor, block_table: torch.Tensor, seqs: Optional[torch.Tensor] = None,
+                    weights: Optional[torch.Tensor] = None, pos: Optional[torch.Tensor] = None,
+                    held: Optional[torch.Tensor] = None, evicted: Optional[torch.Tensor] = None) -> None:
+    """Move the entries of one layer to where src (int32 [n, H, budget], as kvt_block_keep gives it) has them: codes,
+    weights and positions of request j's entries below the budget, a multiple of the block size.  Requests of no more than
+    `budget` entries (kv_lens) are left as they are.
+
+    A block that gets no other entry is left as it is.  Another one's scales become the smallest powers of two that hold
+    its rows, as if their values were stored anew: exact for e4m3 codes but for those that become subnormal, int8 codes are
+    rounded to a scale that grew.  Where a row's scale is not finite, the block's becomes NaN.  An entry of src that is
+    neither its own place nor behind the budget and within the length stays where it is.  weights and pos are optional; pos
+    takes held and evicted with it, which kvt_block_trim updates once all layers are done."""
+    n = kv_lens.numel()
+    nb, H, B, D = _pool(k8, v8, ks, vs, block_table, n, seqs)
+    assert src.dtype == torch.int32 and src.dim() == 3 and src.is_contiguous(), "src is a contiguous int32 [n, H, budget]"
+    if src.shape[:2] != (n, H):
+        raise ValueError(f"src of {tuple(src.shape)} for {n} requests x {H} heads")
+    budget = src.shape[2]
+    _cut(budget, B)
+    _i32("kv_lens", kv_lens, n)
+    rows, max_blocks = block_table.shape
+    if weights is not None:
+        _per_entry("weights", weights, torch.float32, rows, H, max_blocks * B)
+    if pos is not None:
+        if held is None or evicted is None:
+            raise ValueError("pos goes with held and evicted")
+        _per_entry("pos", pos, torch.int32, rows, H, max_blocks * B)
+        _i32("held", held, rows)
+        _i32("evicted", evicted, rows)
+    if n == 0 or H == 0 or budget > max_blocks * B:          # (no request can be over its budget)
+        return
+    st = _stream(src, kv_lens, k8, v8, ks, vs, block_table, seqs, weights, pos, held, evicted)
+    sw = (0, 0) if weights is None else (weights.stride(0), weights.stride(1))
+    sp = (0, 0) if pos is None else (pos.stride(0), pos.stride(1))
+    _lib.call("kvt_block_evict", src.data_ptr(), kv_lens.data_ptr(), n, H, D, CODE[k8.dtype], k8.data_ptr(), v8.data_ptr(),
+              ks.data_ptr(), vs.data_ptr(), nb, B, block_table.data_ptr(), block_table.stride(0), rows, max_blocks,
+              _lib.ptr(seqs), budget, _lib.ptr(weights), *sw, _lib.ptr(pos), *sp, _lib.ptr(held), _lib.ptr(evicted), st)
+
+
+def kvt_block_trim(seqs: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, free_list: torch.Tensor,
+                   free_head: torch.Tensor, budget: int, block: int = 64, held: Optional[torch.Tensor] = None,
+                   evicted: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None,
+                   commit: bool = True) -> BlockTrim:
+    """Cut the table rows seqs[j] to `budget` entries, once their entries have been moved in every layer: the counterpart
+    of kvt_block_plan.  The blocks behind the budget go back in front of free_list[free_head[0]], in request order; their
+    table entries become -1, seq_lens[row] the budget, and held and evicted (int32 [rows]) say how many entries have
+    positions of their own and how many positions are gone.  Rows of no more entries are left as they are.
+
+    commit=False writes the free list's entries, which are nobody's until its head moves, and leaves everything else as it
+    is.  status (int32 [1]): bits BAD_ROW (a row out of range, or listed twice: the first one counts) and FREE_OVER (more
+    blocks come back than were handed out; those over are lost) are or-ed in.  At most 1,024 requests."""
+    n = seqs.numel()
+    _i32("seqs", seqs, n)
+    _i32("seq_lens", seq_lens, 1)
+    _i32("free_list", free_list, 0)
+    _i32("free_head", free_head, 1)
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1
+    rows = block_table.shape[0]
+    _cut(budget, block)
+    if (held is None) != (evicted is None):
+        raise ValueError("held and evicted go together")
+    for name, x in (("seq_lens", seq_lens), ("held", held), ("evicted", evicted)):
+        if x is not None:
+            _i32(name, x, rows)
+    if status is not None:
+        _i32("status", status, 1)
+    st = _stream(seqs, seq_lens, block_table, free_list, free_head, held, evicted, status)
+    if n == 0:
+        return BlockTrim(seqs.new_empty(0), free_head[:1].clamp(0, free_list.numel()))
+    kv_lens, next_head = seqs.new_empty(n + 1).split_with_sizes((n, 1))
+    _lib.call("kvt_block_trim", n, seqs.data_ptr(), seq_lens.data_ptr(), rows, block_table.data_ptr(), block_table.stride(0),
+              block_table.shape[1], free_list.data_ptr(), free_list.numel(), free_head.data_ptr(), block, budget,
+              _lib.ptr(held), _lib.ptr(evicted), kv_lens.data_ptr(), next_head.data_ptr(), _lib.ptr(status),
+              int(bool(commit)), st)
+    return BlockTrim(kv_lens, next_head)

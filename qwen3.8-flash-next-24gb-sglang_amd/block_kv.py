@@ -29,6 +29,7 @@ _I32, _F32 = torch.int32, torch.float32
 BLOCKS = (16, 32, 64)
 HEAD_DIMS = (64, 128, 256)
 POOL_SHORT, ROW_FULL, TOKENS_OVER, BAD_ROW = 1, 2, 4, 8   # status bits of a plan
+FREE_OVER = 16                                            # and of a trim
 # Decode.  Few requests: a number of splits for each (request, KV head) pair.  From _SHARE_REQUESTS on, over long
 # tables: equal shares of all positions.  Measured, device us per call with the merge, caches cold, best splits against
 # shares, up to 8,191 positions ragged: 8 requests x 8 heads (D 128) 19.7 / 22.7; 32 x 2 (D 256, up to 16,384) 65.7 /
@@ -342,12 +343,16 @@ def kvt_block_prefill(q: torch.Tensor, cu_q: torch.Tensor, k8: torch.Tensor, v8:
 class BlockKVCache:
     """Buffers of the 8-bit block cache for all layers of a model, and the step's calls over them.
 
+    evicting=True adds what a cache within a budget keeps (see block_evict): weights and pos of every layer
+    [layers, max_seqs, H, max_blocks * block], held and evicted [max_seqs].
+
     Per layer k8 / v8 [n_blocks, H, block, D] and ks / vs [n_blocks, H]; shared by the layers: block_table
     [max_seqs, max_blocks], seq_lens [max_seqs], the free list (a seeded permutation of the blocks) and its head.
     Lengths, blocks and the free list live on the device only; add_seq and release hand out table rows on the host."""
 
     def __init__(self, layers: int, H: int, D: int, n_blocks: int, max_seqs: int, max_blocks: int, device="cuda",
-                 dtype: torch.dtype = torch.float8_e4m3fn, block: int = 64, seed: int = 0):
+                 dtype: torch.dtype = torch.float8_e4m3fn, block: int = 64, seed: int = 0,
+                 evicting: bool = False):
         if dtype not in CODE:
             raise ValueError(f"block codes are float8_e4m3fn or int8, not {dtype}")
         if block not in BLOCKS or D not in HEAD_DIMS:
@@ -367,6 +372,13 @@ class BlockKVCache:
         self.free_list = torch.randperm(n_blocks, generator=g).to(torch.int32).to(self.device)
         self.free_head = torch.zeros(1, dtype=torch.int32, **z)
         self.status = torch.zeros(1, dtype=torch.int32, **z)
+        self.weights = self.pos = self.held = self.evicted = None
+        if evicting:
+            per_entry = (layers, max_seqs, H, max_blocks * block)
+            self.weights = torch.zeros(per_entry, dtype=torch.float32, **z)
+            self.pos = torch.zeros(per_entry, dtype=torch.int32, **z)
+            self.held = torch.zeros(max_seqs, dtype=torch.int32, **z)
+            self.evicted = torch.zeros(max_seqs, dtype=torch.int32, **z)
         self._rows: List[int] = list(range(max_seqs - 1, -1, -1))
 
     def add_seq(self) -> int:
@@ -387,6 +399,9 @@ class BlockKVCache:
         self.free_head.fill_(head)
         self.block_table[s].fill_(-1)
         self.seq_lens[s] = 0
+        if self.evicted is not None:
+            self.held[s] = 0
+            self.evicted[s] = 0
         self._rows.append(s)
 
     def _vec(self, x: Union[torch.Tensor, Sequence[int]]) -> torch.Tensor:
@@ -411,7 +426,8 @@ class BlockKVCache:
             self.status.zero_()
             names = [name for bit, name in ((POOL_SHORT, "block pool exhausted"), (ROW_FULL, "block table row full"),
                                             (TOKENS_OVER, "more tokens than n_tokens"),
-                                            (BAD_ROW, "table row out of range or listed twice")) if bits & bit]
+                                            (BAD_ROW, "table row out of range or listed twice"),
+                                            (FREE_OVER, "more blocks given back than were handed out")) if bits & bit]
             raise RuntimeError("block plan: " + ", ".join(names))
 
     def append(self, layer: int, plan: BlockPlan, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -429,3 +445,43 @@ class BlockKVCache:
         behind that are not written: pass an `out` that holds what they should be, or do not read them."""
         return kvt_block_prefill(q, plan.cu, self.k8[layer], self.v8[layer], self.ks[layer], self.vs[layer],
                                  self.block_table, plan.kv_lens, plan.seqs, **kw)
+
+    def rotate(self, plan: BlockPlan, q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor,
+               scale: float = 1.0, **kw):
+        """Rotary positions of the plan's tokens (kvt_rope): the entries that were evicted before them count."""
+        from .rope import kvt_rope
+        return kvt_rope(q, k, plan.kv_lens, inv_freq, scale, cu=plan.cu, seqs=plan.seqs, ahead=self.evicted, **kw)
+
+    def _evicting(self) -> None:
+        if self.weights is None:
+            raise ValueError("a cache made with evicting=True is needed")
+
+    def weigh_decode(self, layer: int, plan: BlockPlan, q: torch.Tensor, **kw) -> torch.Tensor:
+        """Add the attention weight of one query per request of the plan (the queries of `decode`)."""
+        from .block_evict import kvt_block_weigh
+        self._evicting()
+        return kvt_block_weigh(q, self.k8[layer], self.ks[layer], self.block_table, plan.kv_lens, self.weights[layer],
+                               seqs=plan.seqs, **kw)
+
+    def weigh_prefill(self, layer: int, plan: BlockPlan, q: torch.Tensor, **kw) -> torch.Tensor:
+        """Add the attention weight of the plan's tokens (the queries of `prefill`)."""
+        from .block_evict import kvt_block_weigh
+        self._evicting()
+        return kvt_block_weigh(q, self.k8[layer], self.ks[layer], self.block_table, plan.kv_lens, self.weights[layer],
+                               cu_q=plan.cu, seqs=plan.seqs, **kw)
+
+    def evict(self, seqs, budget: int, recent: int = 0, sinks: int = 0) -> None:
+        """Cut sequences to `budget` entries (a multiple of the block size) in every layer: the first `sinks`, those at the
+        last `recent` positions and the heaviest others stay, and the blocks behind go back to the free list.  Sequences of
+        no more entries are left as they are.  On the device (capturable with device `seqs`); a plan made before is void."""
+        from .block_evict import kvt_block_evict, kvt_block_keep, kvt_block_trim
+        self._evicting()
+        seqs = self._vec(seqs)
+        lens = self.plan(seqs, torch.zeros_like(seqs), 0, commit=False).kv_lens     # (0 for rows that are not served)
+        for layer in range(self.L):
+            w, pos = self.weights[layer], self.pos[layer]
+            src = kvt_block_keep(w, lens, budget, seqs, recent, sinks, pos, self.held, self.evicted)
+            kvt_block_evict(src, lens, self.k8[layer], self.v8[layer], self.ks[layer], self.vs[layer], self.block_table,
+                            seqs, w, pos, self.held, self.evicted)
+        kvt_block_trim(seqs, self.seq_lens, self.block_table, self.free_list, self.free_head, budget, self.block, self.held,
+                       self.evicted, self.status)

@@ -1,0 +1,618 @@
+// Attention weight of a step's queries per cache entry of the 8-bit block cache (kvt_block_weigh).
+//
+//   out[row, h, p] = prior[row, h, p] + sum over the request's queries i that see p and the q heads g of KV head h of
+//                    exp(x_igp - M_ig) / L_ig,   x_igp = scale * sk_p * q_ig . kc_p
+// with M and L the maximum and the sum of exponentials of (i, g)'s scores: the column sums of softmax(Q K^T), whose rows
+// have to be complete before any column can be.
+//
+// One query per request (a (request, KV head) has at most 16 rows): the scores are formed once, by 16 x 16 products with
+// K's codes from registers as they were loaded, and kept as fp32 (4 Hq / H bytes an entry against D bytes of codes: less
+// than a second read of K); a second launch joins the splits' maxima and sums and adds up the columns.
+//
+// Chunks: a row has too many scores to keep, so they are formed twice.  The first launch holds 256 rows of Q in
+// registers (64 a wavefront) and streams K through LDS for maxima and sums; each lane keeps them for a row of its own, over the
+// positions that it sees, so that nothing crosses lanes in the loop.  The second one holds 256 positions of K in
+// registers and streams Q; a lane adds up the weights of its position.  Splits are joined in their order by launches of
+// their own: no atomics, the same bits for every call.
+//
+// Operands have q's type (codes of 8 bits are exact in bf16 and fp16); scores, maxima, sums and weights are fp32.
+#include "block_common.h"
+
+using namespace kvt;
+using namespace kvt::blk;
+
+namespace {
+
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+constexpr float kInf = __builtin_inff();
+constexpr int kTileRows = 256;         // rows (query, q head) of a workgroup of the first chunk launch
+constexpr int kTilePos = 256;          // positions of a workgroup's step of the second one
+constexpr int kStep = 64;              // positions (rows) of a streamed tile
+constexpr int kMostSplits = 1024;
+constexpr int64_t kMostPositions = ((int64_t)1 << 31) - 8192;
+
+struct Weigh {
+  const void* q;
+  const uint8_t* k8;
+  const float* ks;
+  const int32_t* table;
+  const int32_t* kv_lens;
+  const int32_t* rows;
+  const int32_t* cu;           // NULL: one query per request
+  const int32_t* since;        // entries from here on start from zero (NULL: those of the call's queries)
+  const float* prior;
+  float* out;
+  float* scores;               // decode: [n * H, gs, cap]
+  float2* part;                // (maximum, sum): decode [n * H, splits, 16]; chunks [splits, H, n_q * gs]
+  float2* norm;                // chunks: (maximum, 1 / sum) [H, n_q * gs]
+  float* sums;                 // chunks: [row_splits, n * H, cap]
+  int64_t sq_n, sq_h, stride, sw_r, sw_h, so_r, so_h;
+  float scale_log2;
+  int n, n_rows, n_q, H, gs, n_blocks, max_blocks, log2b, splits, row_splits, pos_splits;
+};
+
+KVT_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+KVT_DEV float lane_f(float v, int lane) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), lane));
+}
+
+// Two codes (bytes 0, 1 or 2, 3 of a dword) -> two operand halves, exact.
+template <int CODE, int QT, bool HI>
+KVT_DEV uint32_t two(uint32_t w) {
+  if constexpr (QT == kF16) {
+    return __builtin_bit_cast(uint32_t, pair<CODE, HI>(w));
+  } else if constexpr (CODE == kE4M3) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+  } else {
+    return bf16x2((float)(int8_t)(w >> (HI ? 16 : 0)), (float)(int8_t)(w >> (HI ? 24 : 8)));
+  }
+}
+// Eight codes in order -> an operand.
+template <int CODE, int QT>
+KVT_DEV u4v eight(uint32_t w0, uint32_t w1) {
+  if constexpr (QT == kF16) w0 = flip<CODE>(w0), w1 = flip<CODE>(w1);
+  return u4v{two<CODE, QT, false>(w0), two<CODE, QT, true>(w0), two<CODE, QT, false>(w1), two<CODE, QT, true>(w1)};
+}
+template <int QT>
+KVT_DEV f4 mfma16(u4v a, u4v b, f4 c) {
+  if constexpr (QT == kF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+template <int QT>
+KVT_DEV f16v mfma32(u4v a, u4v b, f16v c) {
+  if constexpr (QT == kF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+
+// K's scale times the softmax scale in powers of two; NaN for a scale that is not finite (>= 0).
+KVT_DEV float factor(const Weigh& P, float sk) { return fmaf(P.scale_log2, sk, sk - sk); }
+
+struct Req {
+  int trow, q0, q_len, kv, len;      // table row, first query, queries, entries, entries of the table
+};
+KVT_DEV Req request(const Weigh& P, int r) {
+  Req t;
+  t.q0 = r, t.q_len = 1;
+  if (P.cu) {
+    t.q0 = min(max(uniform(P.cu[r]), 0), P.n_q);
+    t.q_len = min(max(uniform(P.cu[r + 1]), t.q0), P.n_q) - t.q0;
+  }
+  t.trow = P.rows ? uniform(P.rows[r]) : r;
+  t.kv = max(uniform(P.kv_lens[r]), 0);
+  t.len = (int)min((int64_t)t.kv, (int64_t)P.max_blocks << P.log2b);
+  if (t.trow < 0 || t.trow >= P.n_rows) t.len = 0, t.trow = 0;
+  return t;
+}
+// Entries that query i of the request sees.
+KVT_DEV int sees(const Req& t, int i) { return (int)min((int64_t)t.len, max((int64_t)t.kv - t.q_len + i + 1, (int64_t)0)); }
+
+// x and its maximum and sum: a running pair takes another one.
+KVT_DEV void join(float& m, float& l, float m2, float l2) {
+  const float M = fmaxf(m, m2);
+  l = (m == -kInf ? l : l * exp2_(m - M)) + (m2 == -kInf ? l2 : l2 * exp2_(m2 - M));
+  m = M;
+}
+
+KVT_DEV void finish(const Weigh& P, const Req& t, int r, int h, int p, float sum) {
+  const int since = P.since ? P.since[r] : t.kv - t.q_len;
+  if (p < since) sum += P.prior[t.trow * P.sw_r + h * P.sw_h + p];
+  P.out[t.trow * P.so_r + h * P.so_h + p] = sum;
+}
+
+// ------------------------------------------------------------------------------------------------- one query per request
+// Positions per split: equal shares in multiples of 128 (a tile of 32 for each wavefront), 256 at least.
+KVT_DEV int per_split(int len, int splits) { return max(((len + splits - 1) / splits + 127) & ~127, 256); }
+
+template <int CODE, int QT, int D>
+__global__ __launch_bounds__(256) void weigh_rows_kernel(const Weigh P) {
+  constexpr int NC = D / 64;
+  __shared__ float2 J[4][16];
+  const int h = blockIdx.x % P.H, w = blockIdx.x / P.H, split = w % P.splits, r = w / P.splits;
+  const Req t = request(P, r);
+  const int per = per_split(t.len, P.splits);
+  const int64_t from = (int64_t)split * per;
+  if (from >= t.len) return;
+  const int p_begin = (int)from, p_end = (int)min(from + per, (int64_t)t.len);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+  const bool live = l < P.gs;
+  const uint16_t* qrow = (const uint16_t*)P.q + (int64_t)t.q0 * P.sq_n + (int64_t)(h * P.gs + (live ? l : 0)) * P.sq_h;
+  u4v Q[D / 32];
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) Q[k] = *reinterpret_cast<const u4v*>(qrow + 64 * (k >> 1) + 16 * g + 8 * (k & 1));
+  const int64_t pair_id = (int64_t)r * P.H + h, cap = (int64_t)P.max_blocks << P.log2b;
+  float* score = P.scores + (pair_id * P.gs + l) * cap;
+  const uint32_t koff = (uint32_t)l * D + 16u * g;
+  const int64_t tbl = (int64_t)t.trow * P.stride;
+  float m = -kInf, sum = 0.0f;
+
+  for (int base = p_begin + 32 * wave; base < p_end; base += 32 * 128) {
+    // blocks and scales of the next 32 tiles: lane 2 i + s has half s of the tile at base + 128 i
+    int id = -1;
+    float sk = 0.0f;
+    const int mine = base + (lane >> 1) * 128 + 16 * (lane & 1);
+    if (mine < p_end) id = P.table[tbl + (mine >> P.log2b)];
+    if (id < 0 || id >= P.n_blocks) id = -1;
+    if (id >= 0) sk = P.ks[(int64_t)id * P.H + h];
+    for (int i = 0; i < 32; ++i) {
+      const int p0 = base + 128 * i;
+      if (p0 >= p_end) break;
+      int valid[2];
+      float f[2];
+      u4v kr[2][NC];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int b = __builtin_amdgcn_readlane(id, 2 * i + s);
+        const int64_t at = ((((int64_t)max(b, 0) * P.H + h) << P.log2b) + ((p0 + 16 * s) & ((1 << P.log2b) - 1))) * D;
+        f[s] = factor(P, lane_f(sk, 2 * i + s));
+        valid[s] = b < 0 ? 0 : min(max(p_end - (p0 + 16 * s), 0), 16);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) kr[s][c] = *reinterpret_cast<const u4v*>(P.k8 + at + koff + 64u * c);
+      }
+      float x[2][4];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        f4 acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          acc = mfma16<QT>(eight<CODE, QT>(kr[s][c][0], kr[s][c][1]), Q[2 * c], acc);
+          acc = mfma16<QT>(eight<CODE, QT>(kr[s][c][2], kr[s][c][3]), Q[2 * c + 1], acc);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[s][j] = 4 * g + j < valid[s] ? acc[j] * f[s] : -kInf;
+        if (live && p0 + 16 * s < p_end) *reinterpret_cast<f4*>(score + p0 + 16 * s + 4 * g) = f4{x[s][0], x[s][1], x[s][2], x[s][3]};
+      }
+      float top = m;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, x[s][j]);
+      const float ref = top == -kInf ? 0.0f : top;
+      sum *= exp2_(m - ref);
+      m = top;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += exp2_(x[s][j] - ref);
+    }
+  }
+  const float M = max_xor16_32(m);
+  sum = sum_xor16_32(m == -kInf ? sum : sum * exp2_(m - M));
+  if (g == 0) J[wave][l] = make_float2(M, sum);
+  __syncthreads();
+  if (threadIdx.x < 16) {
+    float2 a = J[0][l];
+#pragma unroll
+    for (int v = 1; v < 4; ++v) join(a.x, a.y, J[v][l].x, J[v][l].y);
+    P.part[(pair_id * P.splits + split) * 16 + l] = a;
+  }
+}
+
+// Maximum and 1 / sum of the pair's rows from the splits' parts, then the columns of 1,024 positions at a time.
+__global__ __launch_bounds__(256) void weigh_columns_kernel(const Weigh P) {
+  __shared__ float2 J[16][16];
+  __shared__ float2 norm[16];
+  const int h = blockIdx.x % P.H, w = blockIdx.x / P.H, split = w % P.pos_splits, r = w / P.pos_splits;
+  const Req t = request(P, r);
+  if ((int64_t)split * 1024 >= t.len) return;
+  const int64_t pair_id = (int64_t)r * P.H + h, cap = (int64_t)P.max_blocks << P.log2b;
+  const int used = (t.len + per_split(t.len, P.splits) - 1) / per_split(t.len, P.splits);
+  {
+    const int l = threadIdx.x & 15, c = threadIdx.x >> 4;
+    float m = -kInf, s = 0.0f;
+    for (int i = c; i < used; i += 16) {
+      const float2 a = P.part[(pair_id * P.splits + i) * 16 + l];
+      join(m, s, a.x, a.y);
+    }
+    J[c][l] = make_float2(m, s);
+  }
+  __syncthreads();
+  if (threadIdx.x < 16) {
+    float2 a = J[0][threadIdx.x];
+#pragma unroll
+    for (int c = 1; c < 16; ++c) join(a.x, a.y, J[c][threadIdx.x].x, J[c][threadIdx.x].y);
+    norm[threadIdx.x] = make_float2(a.x, 1.0f / a.y);
+  }
+  __syncthreads();
+  const float* score = P.scores + pair_id * P.gs * cap;
+  for (int64_t base = (int64_t)split * 1024; base < t.len; base += (int64_t)P.pos_splits * 1024) {
+    float sum[4] = {0, 0, 0, 0};
+    const int p = (int)base + threadIdx.x;
+    for (int g = 0; g < P.gs; ++g) {
+      const float2 a = norm[g];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (p + 256 * i < t.len) sum[i] = fmaf(exp2_(score[g * cap + p + 256 * i] - a.x), a.y, sum[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = p + 256 * i;
+      if (e >= t.len) break;
+      const int id = P.table[(int64_t)t.trow * P.stride + (e >> P.log2b)];
+      finish(P, t, r, h, e, id >= 0 && id < P.n_blocks ? sum[i] : 0.0f);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------- chunks
+// A streamed tile in LDS: kStep rows of D halves, padded so that 32 rows' 16-byte reads spread over the banks.
+template <int D> constexpr int kPitch = 2 * D + 16;
+
+// Operand k of a streamed row: with a held operand whose lanes have 16 codes in a row (K in registers), channels
+// 32 k' + 16 hl + 8 (k & 1); else 16 k + 8 hl.
+template <bool SIXTEEN>
+KVT_DEV int channel(int k, int hl) { return SIXTEEN ? 32 * (k >> 1) + 16 * hl + 8 * (k & 1) : 16 * k + 8 * hl; }
+
+// Row (of 32) that register i of a 32 x 32 product has in lanes of half hl.
+KVT_DEV int prow(int i, int hl) { return 8 * (i >> 2) + 4 * hl + (i & 3); }
+
+// Maxima and sums of 256 rows over a split of the positions.
+template <int CODE, int QT, int D>
+__global__ __launch_bounds__(256) void weigh_norm_kernel(const Weigh P, int items) {
+  constexpr int KS = D / 16, NL = D / 64;     // products per tile of 32; 16-byte loads per thread and tile
+  constexpr int TPR = D / 16;                 // threads per streamed row
+  __shared__ __attribute__((aligned(16))) uint8_t tile[2][kStep * kPitch<D>];
+  const int item = blockIdx.x % items, w = blockIdx.x / items, h = w % P.H, split = w / P.H;
+  const int r = find_request(P.cu, P.n, item, P.gs, kTileRows, 1);
+  const Req t = request(P, r);
+  const int64_t row0 = (item - first_item(uniform(P.cu[r]), r, P.gs, kTileRows, 1)) * kTileRows;
+  const int64_t n_rows = (int64_t)t.q_len * P.gs;
+  if (row0 < 0 || row0 >= n_rows) return;
+  const int live = (int)min(n_rows - row0, (int64_t)kTileRows);
+  const int limit = sees(t, (int)((row0 + live - 1) / P.gs));
+  const int per = (((limit + kStep - 1) / kStep + P.splits - 1) / P.splits) * kStep;
+  const int p_begin = (int)min((int64_t)split * per, (int64_t)limit), p_end = (int)min((int64_t)p_begin + per, (int64_t)limit);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 31, hl = lane >> 5;
+
+  u4v Q[2][KS];
+  int see[2];
+  float m[2] = {-kInf, -kInf}, sum[2] = {0, 0};
+  int64_t at_row[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int mine = 64 * wave + 32 * c + l;
+    const int64_t row = row0 + (mine < live ? mine : 0);
+    at_row[c] = mine < live ? (int64_t)t.q0 * P.gs + row : -1;
+    see[c] = sees(t, (int)(row / P.gs));
+    const uint16_t* p = (const uint16_t*)P.q + (t.q0 + row / P.gs) * P.sq_n + (h * P.gs + row % P.gs) * P.sq_h;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) Q[c][k] = *reinterpret_cast<const u4v*>(p + channel<false>(k, hl));
+  }
+  const int all_see = sees(t, (int)(row0 / P.gs));
+  const bool idle = 64 * wave >= live;
+  const int64_t tbl = (int64_t)t.trow * P.stride;
+
+  int id = -1;
+  float sk = 0.0f;
+  auto ids = [&](int base) {      // blocks and scales of the next 16 tiles: lane 4 i + s has quarter s of tile base / 64 + i
+    const int p = base + 16 * lane;
+    id = p < p_end ? P.table[tbl + (p >> P.log2b)] : -1;
+    if (id < 0 || id >= P.n_blocks) id = -1;
+    sk = id >= 0 ? P.ks[(int64_t)id * P.H + h] : 0.0f;
+  };
+  u4v raw[NL];
+  const int tr = threadIdx.x / TPR, tc = threadIdx.x % TPR;
+  auto load = [&](int p0, int i) {
+#pragma unroll
+    for (int k = 0; k < NL; ++k) {
+      const int row = tr + k * (256 / TPR);
+      const int b = __shfl(id, 4 * i + (row >> 4), 64);
+      raw[k] = u4v{0, 0, 0, 0};
+      if (b >= 0)
+        raw[k] = *reinterpret_cast<const u4v*>(
+            P.k8 + ((((int64_t)b * P.H + h) << P.log2b) + ((p0 + row) & ((1 << P.log2b) - 1))) * D + 16 * tc);
+    }
+  };
+  if (p_begin < p_end) {
+    ids(p_begin);
+    load(p_begin, 0);
+  }
+  int buf = 0, slot = 0;
+  for (int p0 = p_begin; p0 < p_end; p0 += kStep, buf ^= 1) {
+    uint8_t* T = tile[buf];
+#pragma unroll
+    for (int k = 0; k < NL; ++k) {
+      u4v* o = reinterpret_cast<u4v*>(T + (tr + k * (256 / TPR)) * kPitch<D> + 32 * tc);
+      o[0] = eight<CODE, QT>(raw[k][0], raw[k][1]);
+      o[1] = eight<CODE, QT>(raw[k][2], raw[k][3]);
+    }
+    float f[4];
+    int valid[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      f[s] = factor(P, lane_f(sk, 4 * slot + s));
+      valid[s] = __builtin_amdgcn_readlane(id, 4 * slot + s) < 0 ? 0 : min(max(p_end - (p0 + 16 * s), 0), 16);
+    }
+    const bool edge = valid[0] + valid[1] + valid[2] + valid[3] < kStep || p0 + kStep > all_see;
+    ++slot;
+    if (p0 + kStep < p_end) {
+      if (slot == 16) ids(p0 + kStep), slot = 0;
+      load(p0 + kStep, slot);
+    }
+    __syncthreads();
+    if (!idle) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        f16v acc[2] = {};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const u4v a = *reinterpret_cast<const u4v*>(T + (32 * s + l) * kPitch<D> + 2 * channel<false>(k, hl));
+#pragma unroll
+          for (int c = 0; c < 2; ++c) acc[c] = mfma32<QT>(a, Q[c][k], acc[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x[16], top = m[c];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int sub = 2 * s + (i >> 3);
+            x[i] = acc[c][i] * f[sub];
+            if (edge) {
+              const int at = prow(i, hl);
+              x[i] = (at & 15) < valid[sub] && p0 + 32 * s + at < see[c] ? x[i] : -kInf;
+            }
+            top = fmaxf(top, x[i]);
+          }
+          const float ref = top == -kInf ? 0.0f : top;
+          sum[c] *= exp2_(m[c] - ref);
+          m[c] = top;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum[c] += exp2_(x[i] - ref);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const float m2 = __shfl_xor(m[c], 32, 64), s2 = __shfl_xor(sum[c], 32, 64);
+    join(m[c], sum[c], m2, s2);
+    if (hl == 0 && at_row[c] >= 0) {
+      const int64_t at = (int64_t)h * P.n_q * P.gs + at_row[c];
+      if (P.splits == 1) P.norm[at] = make_float2(m[c], 1.0f / sum[c]);
+      else P.part[split * ((int64_t)P.H * P.n_q * P.gs) + at] = make_float2(m[c], sum[c]);
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void weigh_join_kernel(const Weigh P) {
+  const int64_t total = (int64_t)P.H * P.n_q * P.gs, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  if ((i / P.gs) % P.n_q >= P.cu[P.n]) return;      // (padding: no parts)
+  float m = -kInf, s = 0.0f;
+  for (int k = 0; k < P.splits; ++k) {
+    const float2 a = P.part[k * total + i];
+    join(m, s, a.x, a.y);
+  }
+  P.norm[i] = make_float2(m, 1.0f / s);
+}
+
+// Rows per split of a request's (query, q head) rows: equal shares in multiples of 64, 512 at least.
+KVT_DEV int64_t per_row_split(int64_t n_rows, int splits) { 
+  return max(((n_rows + splits - 1) / splits + 63) & ~(int64_t)63, (int64_t)512);
+}
+
+// Column sums of 256 positions over a split of the request's rows.
+template <int CODE, int QT, int D>
+__global__ __launch_bounds__(256) void weigh_sums_kernel(const Weigh P) {
+  constexpr int KS = D / 16, NL = D / 32;     // products per tile of 32 rows; 16-byte loads per thread and tile of Q
+  constexpr int TPR = D / 8;
+  __shared__ __attribute__((aligned(16))) uint8_t tile[2][kStep * kPitch<D>];
+  __shared__ __attribute__((aligned(16))) float top[2][kStep], inv[2][kStep];
+  int w = blockIdx.x;
+  const int split = w % P.pos_splits;
+  w /= P.pos_splits;
+  const int h = w % P.H;
+  w /= P.H;
+  const int rs = w % P.row_splits, r = w / P.row_splits;
+  const Req t = request(P, r);
+  const int64_t n_rows = (int64_t)t.q_len * P.gs, per = per_row_split(n_rows, P.row_splits);
+  const int64_t r_begin = rs * per, r_end = min(r_begin + per, n_rows);
+  if (r_begin >= r_end && rs > 0) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 31, hl = lane >> 5;
+  const int64_t cap = (int64_t)P.max_blocks << P.log2b;
+  const int tr = threadIdx.x / TPR, tc = threadIdx.x % TPR;
+  const float2* norm = P.norm + ((int64_t)h * P.n_q + t.q0) * P.gs;
+
+  for (int64_t p0 = (int64_t)split * kTilePos; p0 < t.len; p0 += (int64_t)P.pos_splits * kTilePos) {
+    u4v K[2][KS];
+    float f[2], sum[2] = {0, 0};
+    int64_t first[2];           // the first row that sees the lane's position
+    bool there[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int64_t p = p0 + 64 * wave + 32 * c + l;
+      int id = p < t.len ? P.table[(int64_t)t.trow * P.stride + (p >> P.log2b)] : -1;
+      there[c] = id >= 0 && id < P.n_blocks;
+      f[c] = there[c] ? factor(P, P.ks[(int64_t)id * P.H + h]) : 0.0f;
+      first[c] = max(p - ((int64_t)t.kv - t.q_len), (int64_t)0) * P.gs;
+      const uint8_t* kp = P.k8 + ((((int64_t)(there[c] ? id : 0) * P.H + h) << P.log2b) + (p & ((1 << P.log2b) - 1))) * D + 16 * hl;
+#pragma unroll
+      for (int k = 0; k < KS / 2; ++k) {
+        u4v v = {0, 0, 0, 0};
+        if (there[c]) v = *reinterpret_cast<const u4v*>(kp + 32 * k);
+        K[c][2 * k] = eight<CODE, QT>(v[0], v[1]);
+        K[c][2 * k + 1] = eight<CODE, QT>(v[2], v[3]);
+      }
+    }
+    // rows that see any of the workgroup's positions, and those that see all of them
+    const int64_t some = max((p0 - ((int64_t)t.kv - t.q_len)) * P.gs, r_begin) & ~(int64_t)(kStep - 1);
+    const int64_t all = (min(p0 + kTilePos, (int64_t)t.len) - 1 - ((int64_t)t.kv - t.q_len)) * P.gs;
+    const bool idle = p0 + 64 * wave >= t.len;
+    u4v raw[NL];
+    float2 nr;
+    auto load = [&](int64_t r0) {
+#pragma unroll
+      for (int k = 0; k < NL; ++k) {
+        const int64_t row = r0 + tr + k * (256 / TPR);
+        raw[k] = u4v{0, 0, 0, 0};
+        if (row < r_end)
+          raw[k] = *reinterpret_cast<const u4v*>((const uint16_t*)P.q + (t.q0 + row / P.gs) * P.sq_n +
+                                                 (h * P.gs + row % P.gs) * P.sq_h + 8 * tc);
+      }
+      if (threadIdx.x < kStep) nr = r0 + threadIdx.x < r_end ? norm[r0 + threadIdx.x] : make_float2(kInf, 0.0f);
+    };
+    if (some < r_end) load(some);
+    int buf = 0;
+    for (int64_t r0 = some; r0 < r_end; r0 += kStep, buf ^= 1) {
+      uint8_t* T = tile[buf];
+#pragma unroll
+      for (int k = 0; k < NL; ++k) *reinterpret_cast<u4v*>(T + (tr + k * (256 / TPR)) * kPitch<D> + 16 * tc) = raw[k];
+      if (threadIdx.x < kStep) top[buf][threadIdx.x] = nr.x, inv[buf][threadIdx.x] = nr.y;
+      if (r0 + kStep < r_end) load(r0 + kStep);
+      __syncthreads();
+      const bool edge = r0 < all || r0 + kStep > r_end;
+      if (!idle) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          f16v acc[2] = {};
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            const u4v a = *reinterpret_cast<const u4v*>(T + (32 * s + l) * kPitch<D> + 2 * channel<true>(k, hl));
+#pragma unroll
+            for (int c = 0; c < 2; ++c) acc[c] = mfma32<QT>(a, K[c][k], acc[c]);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const f4 mm = *reinterpret_cast<const f4*>(&top[buf][32 * s + prow(i, hl)]);
+            const f4 li = *reinterpret_cast<const f4*>(&inv[buf][32 * s + prow(i, hl)]);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float e = exp2_(fmaf(acc[c][i + j], f[c], -mm[j])) * li[j];
+                const int64_t row = r0 + 32 * s + prow(i, hl) + j;
+                sum[c] += !edge || (row >= first[c] && row < r_end) ? e : 0.0f;
+              }
+          }
+        }
+      }
+    }
+    __syncthreads();            // (the next positions' first tile goes where this one's last may still be read)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int64_t p = p0 + 64 * wave + 32 * c + l;
+      float v = sum[c] + __shfl_xor(sum[c], 32, 64);
+      if (!there[c]) v = 0.0f;
+      if (hl != 0 || p >= t.len) continue;
+      if (P.row_splits == 1) finish(P, t, r, h, (int)p, v);
+      else P.sums[((int64_t)rs * P.n * P.H + (int64_t)r * P.H + h) * cap + p] = v;
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void weigh_add_kernel(const Weigh P) {
+  const int h = blockIdx.x % P.H, w = blockIdx.x / P.H, split = w % P.pos_splits, r = w / P.pos_splits;
+  const Req t = request(P, r);
+  const int64_t n_rows = (int64_t)t.q_len * P.gs, per = per_row_split(n_rows, P.row_splits);
+  const int used = max((int)((n_rows + per - 1) / per), 1);
+  const int64_t cap = (int64_t)P.max_blocks << P.log2b, step = (int64_t)P.n * P.H * cap;
+  for (int64_t p = (int64_t)split * 256 + threadIdx.x; p < t.len; p += (int64_t)P.pos_splits * 256) {
+    float s = 0.0f;
+    for (int k = 0; k < used; ++k) s += P.sums[k * step + ((int64_t)r * P.H + h) * cap + p];
+    finish(P, t, r, h, (int)p, s);
+  }
+}
+
+template <int CODE, int QT, int D>
+int launch(Weigh P, hipStream_t st) {
+  if (!P.cu) {
+    weigh_rows_kernel<CODE, QT, D><<<P.n * P.H * P.splits, 256, 0, st>>>(P);
+    KVT_CHECK_LAUNCH();
+    weigh_columns_kernel<<<P.n * P.H * P.pos_splits, 256, 0, st>>>(P);
+    KVT_CHECK_LAUNCH();
+    return KVT_OK;
+  }
+  const int items = (int)((int64_t)P.n_q * P.gs / kTileRows) + P.n;
+  weigh_norm_kernel<CODE, QT, D><<<items * P.H * P.splits, 256, 0, st>>>(P, items);
+  KVT_CHECK_LAUNCH();
+  if (P.splits > 1 && P.n_q > 0) {
+    weigh_join_kernel<<<(int)(((int64_t)P.H * P.n_q * P.gs + 255) / 256), 256, 0, st>>>(P);
+    KVT_CHECK_LAUNCH();
+  }
+  weigh_sums_kernel<CODE, QT, D><<<P.n * P.row_splits * P.H * P.pos_splits, 256, 0, st>>>(P);
+  KVT_CHECK_LAUNCH();
+  if (P.row_splits > 1) {
+    weigh_add_kernel<<<P.n * P.H * P.pos_splits, 256, 0, st>>>(P);
+    KVT_CHECK_LAUNCH();
+  }
+  return KVT_OK;
+}
+template <int CODE, int QT>
+int launch_d(const Weigh& P, int D, hipStream_t st) {
+  return D == 64 ? launch<CODE, QT, 64>(P, st) : D == 128 ? launch<CODE, QT, 128>(P, st) : launch<CODE, QT, 256>(P, st);
+}
+
+// Floats of the workspace's parts: scores or norm, part, sums.
+struct Space { int64_t scores, part, norm, sums; };
+Space space(int n, int n_q, int H, int gs, int64_t cap, bool chunk, int splits, int row_splits) {
+  if (!chunk) return {(int64_t)n * H * gs * cap, (int64_t)n * H * splits * 32, 0, 0};
+  const int64_t rows = (int64_t)H * n_q * gs;
+  return {0, splits > 1 ? splits * rows * 2 : 0, rows * 2, row_splits > 1 ? (int64_t)row_splits * n * H * cap : 0};
+}
+
+}  // namespace
+
+extern "C" int kvt_block_weigh(const void* q, int64_t sq_n, int64_t sq_h, int q_type, const void* cu_q, int n_q,
+                               const void* kv_lens, int n, int H, int Hq, int D, int code, const void* k8, const void* ks,
+                               int n_blocks, int block, const void* block_table, int64_t bt_stride, int n_rows,
+                               int max_blocks, const void* rows, float scale, const void* since, const void* weights,
+                               int64_t sw_r, int64_t sw_h, void* out, int64_t so_r, int64_t so_h, int splits,
+                               int row_splits, int pos_splits, void* work, int64_t work_floats, void* stream) {
+  if (n < 1 || n > kMaxReq || H < 1 || Hq < H || Hq % H || Hq / H > 16 || n_q < 0 || n_blocks < 1 || n_rows < 1 ||
+      max_blocks < 1 || bt_stride < max_blocks || (!rows && n_rows < n) || (!cu_q && n_q < n))
+    return KVT_EINVAL;
+  if ((D != 64 && D != 128 && D != 256) || (block != 16 && block != 32 && block != 64)) return KVT_EINVAL;
+  if ((code != kE4M3 && code != kI8) || (q_type != kBF16 && q_type != kF16) || !(scale > 0.0f)) return KVT_EINVAL;
+  if (((uintptr_t)q | (uintptr_t)k8 | (uintptr_t)work) & 15 || (sq_n | sq_h) & 7) return KVT_EINVAL;
+  if (splits < 1 || splits > kMostSplits || row_splits < 1 || row_splits > kMostSplits || pos_splits < 1) return KVT_EINVAL;
+  const int gs = Hq / H;
+  const int64_t cap = (int64_t)max_blocks * block;
+  if (cap > kMostPositions) return KVT_ERANGE;
+  const int64_t items = (int64_t)n_q * gs / kTileRows + n;
+  const int64_t most = 1 << 24;                                     // (2^32 threads of a launch)
+  if ((cu_q ? items : (int64_t)n) * H * splits >= most || (int64_t)n * H * row_splits * pos_splits >= most ||
+      (int64_t)H * n_q * gs >= most * 128)
+    return KVT_ERANGE;
+  const Space s = space(n, n_q, H, gs, cap, cu_q != nullptr, splits, row_splits);
+  if (s.scores + s.part + s.norm + s.sums > work_floats) return KVT_EINVAL;
+  Weigh P;
+  P.q = q, P.k8 = (const uint8_t*)k8, P.ks = (const float*)ks, P.table = (const int32_t*)block_table;
+  P.kv_lens = (const int32_t*)kv_lens, P.rows = (const int32_t*)rows, P.cu = (const int32_t*)cu_q;
+  P.since = (const int32_t*)since, P.prior = (const float*)weights, P.out = (float*)out;
+  float* x = (float*)work;
+  P.scores = x, P.part = (float2*)(x + s.scores), P.norm = (float2*)(x + s.scores + s.part);
+  P.sums = x + s.scores + s.part + s.norm;
+  P.sq_n = sq_n, P.sq_h = sq_h, P.stride = bt_stride, P.sw_r = sw_r, P.sw_h = sw_h, P.so_r = so_r, P.so_h = so_h;
+  P.scale_log2 = scale * kLog2e;
+  P.n = n, P.n_rows = n_rows, P.n_q = n_q, P.H = H, P.gs = gs, P.n_blocks = n_blocks, P.max_blocks = max_blocks;
+  P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6;
+  P.splits = splits, P.row_splits = row_splits, P.pos_splits = pos_splits;
+  hipStream_t st = (hipStream_t)stream;
+  if (code == kE4M3) return q_type == kBF16 ? launch_d<kE4M3, kBF16>(P, D, st) : launch_d<kE4M3, kF16>(P, D, st);
+  return q_type == kBF16 ? launch_d<kI8, kBF16>(P, D, st) : launch_d<kI8, kF16>(P, D, st);
+}

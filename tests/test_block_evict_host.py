@@ -1,0 +1,215 @@
+"""Refusals of the operators of a block cache within a budget and of rotary positions, on the host: wrong shapes, types,
+sizes and tensors off the GPU are errors before anything is launched; rotary frequencies against their formulas."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+
+def _i(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+def _pool(nb=4, H=2, B=16, D=64, dtype=torch.float8_e4m3fn):
+    return dict(k8=torch.zeros(nb, H, B, D, dtype=torch.int8).view(dtype), v8=torch.zeros(nb, H, B, D, dtype=torch.int8).view(dtype),
+                ks=torch.zeros(nb, H), vs=torch.zeros(nb, H), block_table=torch.zeros(2, 3, dtype=torch.int32))
+
+
+def _weigh(**over):
+    from kvtier.block_evict import kvt_block_weigh
+    p = _pool()
+    a = dict(q=torch.zeros(2, 4, 64, dtype=torch.bfloat16), k8=p["k8"], ks=p["ks"], block_table=p["block_table"],
+             kv_lens=_i(1, 1), weights=torch.zeros(2, 2, 48))
+    return kvt_block_weigh(**{**a, **over})
+
+
+def _keep(**over):
+    from kvtier.block_evict import kvt_block_keep
+    return kvt_block_keep(**{**dict(weights=torch.zeros(2, 2, 48), kv_lens=_i(40, 40), budget=16), **over})
+
+
+def _evict(**over):
+    from kvtier.block_evict import kvt_block_evict
+    return kvt_block_evict(**{**dict(src=torch.zeros(2, 2, 16, dtype=torch.int32), kv_lens=_i(40, 40), **_pool()), **over})
+
+
+def _trim(**over):
+    from kvtier.block_evict import kvt_block_trim
+    a = dict(seqs=_i(0), seq_lens=_i(40, 40), block_table=torch.zeros(2, 3, dtype=torch.int32), free_list=_i(0, 1),
+             free_head=_i(1), budget=16, block=16)
+    return kvt_block_trim(**{**a, **over})
+
+
+def _rope(**over):
+    from kvtier.rope import kvt_rope
+    a = dict(q=torch.zeros(3, 4, 64, dtype=torch.bfloat16), k=torch.zeros(3, 2, 64, dtype=torch.bfloat16),
+             positions=torch.zeros(3, dtype=torch.int64), inv_freq=torch.ones(16, dtype=torch.float64))
+    return kvt_rope(**{**a, **over})
+
+
+@pytest.mark.parametrize("call", [_weigh, _keep, _evict, _trim, _rope])
+def test_tensors_off_the_gpu_are_refused(kvt_pkg, call):
+    with pytest.raises(AssertionError):
+        call()
+
+
+@pytest.mark.parametrize("over", [dict(q=torch.zeros(2, 4, 64)), dict(q=torch.zeros(2, 4, 32, dtype=torch.bfloat16)),
+                                  dict(weights=torch.zeros(2, 2, 48, dtype=torch.float64)), dict(weights=torch.zeros(2, 48, 2).transpose(1, 2)),
+                                  dict(kv_lens=torch.zeros(2, dtype=torch.int64)), dict(since=torch.zeros(2)),
+                                  dict(cu_q=torch.zeros(3, dtype=torch.int64)), dict(out=torch.zeros(2, 2, 48, dtype=torch.bfloat16)),
+                                  dict(k8=torch.zeros(4, 2, 16, 64, dtype=torch.uint8))])
+def test_weigh_contract(kvt_pkg, over):
+    with pytest.raises(AssertionError):
+        _weigh(**over)
+
+
+@pytest.mark.parametrize("over", [dict(q=torch.zeros(3, 4, 64, dtype=torch.bfloat16)), dict(q=torch.zeros(2, 5, 64, dtype=torch.bfloat16)),
+                                  dict(q=torch.zeros(2, 34, 64, dtype=torch.bfloat16)), dict(weights=torch.zeros(1, 2, 48)),
+                                  dict(weights=torch.zeros(2, 2, 47)), dict(weights=torch.zeros(2, 1, 48)), dict(cu_q=_i(0, 1)),
+                                  dict(since=_i(0)), dict(seqs=_i(0)), dict(out=torch.zeros(2, 2, 40))])
+def test_weigh_sizes(kvt_pkg, over):
+    with pytest.raises(ValueError):
+        _weigh(**over)
+
+
+def test_keep_refusals(kvt_pkg):
+    pos, per_row = torch.zeros(2, 2, 48, dtype=torch.int32), _i(0, 0)
+    for bad in (dict(weights=torch.zeros(2, 2, 48, dtype=torch.float16)), dict(kv_lens=torch.zeros(2)),
+                dict(pos=pos.long(), held=per_row, evicted=per_row), dict(out=torch.zeros(2, 2, 16)),
+                dict(out=torch.zeros(2, 2, 17, dtype=torch.int32))):
+        with pytest.raises(AssertionError):
+            _keep(**bad)
+    for bad in (dict(budget=0), dict(recent=-1), dict(recent=10, sinks=7), dict(pos=pos), dict(pos=pos, held=per_row),
+                dict(pos=pos, held=per_row, evicted=_i(0)), dict(pos=pos[:1], held=per_row, evicted=per_row),
+                dict(kv_lens=_i(1, 1, 1)), dict(seqs=_i(0)), dict(weights=torch.zeros(2, 2, 0))):
+        with pytest.raises(ValueError):
+            _keep(**bad)
+
+
+def test_evict_refusals(kvt_pkg):
+    pos, per_row = torch.zeros(2, 2, 48, dtype=torch.int32), _i(0, 0)
+    for bad in (dict(src=torch.zeros(2, 2, 16, dtype=torch.int64)), dict(weights=torch.zeros(2, 2, 48, dtype=torch.float16)),
+                dict(src=torch.zeros(2, 2, 32, dtype=torch.int32)[..., ::2]), dict(v8=torch.zeros(4, 2, 16, 64, dtype=torch.int8))):
+        with pytest.raises(AssertionError):
+            _evict(**bad)
+    for bad in (dict(src=torch.zeros(2, 2, 24, dtype=torch.int32)), dict(src=torch.zeros(2, 2, 0, dtype=torch.int32)),
+                dict(src=torch.zeros(1, 2, 16, dtype=torch.int32)), dict(weights=torch.zeros(2, 2, 40)), dict(pos=pos),
+                dict(pos=pos, held=per_row), dict(pos=pos, held=_i(0), evicted=per_row), dict(seqs=_i(0))):
+        with pytest.raises(ValueError):
+            _evict(**bad)
+
+
+def test_trim_refusals(kvt_pkg):
+    for bad in (dict(seqs=torch.zeros(1)), dict(free_head=torch.zeros(1, dtype=torch.int64)), dict(block_table=torch.zeros(2, 3))):
+        with pytest.raises(AssertionError):
+            _trim(**bad)
+    for bad in (dict(budget=24), dict(budget=0), dict(block=48), dict(seq_lens=_i(1)), dict(held=_i(0, 0)),
+                dict(held=_i(0, 0), evicted=_i(0)), dict(free_head=_i())):
+        with pytest.raises(ValueError):
+            _trim(**bad)
+
+
+def test_rope_refusals(kvt_pkg):
+    x = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
+    for bad in (dict(q=x.double()), dict(k=x.float()), dict(k=x[:2]), dict(inv_freq=torch.ones(16)),
+                dict(positions=torch.zeros(3)), dict(cu=_i(0, 3), positions=torch.zeros(1, dtype=torch.int64)),
+                dict(out_q=x.float()), dict(out_q=x[:2]), dict(q=torch.zeros(3, 64, 4, dtype=torch.bfloat16).transpose(1, 2))):
+        with pytest.raises(AssertionError):
+            _rope(**bad)
+    two = torch.zeros(4, 4, 64, dtype=torch.bfloat16)
+    for bad in (dict(positions=torch.zeros(2, dtype=torch.int64)), dict(inv_freq=torch.ones(33, dtype=torch.float64)),
+                dict(inv_freq=torch.ones(0, dtype=torch.float64)), dict(seqs=_i(0)), dict(ahead=_i(0)),
+                dict(cu=_i(0), positions=_i(1)), dict(cu=_i(0, 3), positions=_i(3), seqs=_i()),
+                dict(cu=_i(0, 2, 3), positions=_i(3, 3), ahead=_i(0)), dict(k=None, out_k=x),
+                dict(q=two[1:], out_q=two[:3]), dict(q=x, k=x[:, :2], out_q=x.clone(), out_k=x[:, 1:3]),
+                dict(out_q=x[:1].expand(3, 4, 64)),
+                dict(q=torch.zeros(3, 1, 320, dtype=torch.bfloat16), k=None)):
+        with pytest.raises(ValueError):
+            _rope(**bad)
+
+
+def test_c_entries_refuse(kvt_pkg):
+    """NULL pointers and sizes out of range come back as a status, without a launch."""
+    lib = kvt_pkg._lib.lib()
+    N = None
+
+    def weigh(n=1, H=1, Hq=1, D=64, code=0, block=16, max_blocks=4, stride=4, rows=1, scale=1.0, splits=1, rs=1, ps=1,
+              floats=10 ** 6, q_type=0, cu=None, n_q=1, sq=64):
+        return lib.kvt_block_weigh(N, sq, 64, q_type, cu, n_q, N, n, H, Hq, D, code, N, N, 4, block, N, stride, rows, max_blocks,
+                                   N, scale, N, N, 0, 0, N, 0, 0, splits, rs, ps, N, floats, N)
+    for bad in (dict(n=0), dict(n=5000, rows=5000, n_q=5000), dict(Hq=17), dict(H=2, Hq=3), dict(D=96), dict(code=2), dict(block=48),
+                dict(stride=3), dict(n=2), dict(scale=0.0), dict(scale=math.nan), dict(splits=0), dict(splits=2000), dict(rs=0),
+                dict(ps=0), dict(floats=10), dict(q_type=2), dict(sq=63), dict(n_q=0)):
+        assert weigh(**bad) == -1, bad
+    assert weigh(max_blocks=2 ** 28, stride=2 ** 28) == -3
+    assert weigh(ps=1 << 24) == -3
+
+    def keep(n=1, H=1, rows=1, cap=64, budget=16, recent=0, sinks=0, pos=None, held=None):
+        return lib.kvt_block_keep(N, 0, 0, N, n, H, rows, N, cap, budget, recent, sinks, pos, 0, 0, held, N, N, N, N)
+    for bad in (dict(n=0), dict(n=2), dict(cap=0), dict(budget=0), dict(recent=17), dict(sinks=-1), dict(pos=16), dict(held=16)):
+        assert keep(**bad) == -1, bad
+    assert keep(cap=2 ** 31) == -3 and keep(n=1 << 22, rows=1 << 22) == -3
+
+    def evict(n=1, H=1, D=64, code=0, nb=4, block=16, stride=4, rows=1, mb=4, budget=16, pos=None, k8=None):
+        return lib.kvt_block_evict(N, N, n, H, D, code, k8, N, N, N, nb, block, N, stride, rows, mb, N, budget, N, 0, 0, pos, 0, 0,
+                                   N, N, N)
+    for bad in (dict(n=0), dict(n=2), dict(D=32), dict(code=3), dict(nb=0), dict(block=8), dict(stride=2), dict(budget=8),
+                dict(budget=24), dict(budget=80), dict(pos=16), dict(k8=8)):
+        assert evict(**bad) == -1, bad
+    assert evict(n=1 << 24, rows=1 << 24) == -3 and evict(mb=2 ** 27, stride=2 ** 27) == -3 and evict(nb=2 ** 28) == -3
+
+    def trim(n=1, rows=1, stride=4, mb=4, n_free=4, block=16, budget=16, held=None):
+        return lib.kvt_block_trim(n, N, N, rows, N, stride, mb, N, n_free, N, block, budget, held, N, N, N, N, 1, N)
+    for bad in (dict(n=0), dict(n=1025), dict(rows=0), dict(stride=3), dict(n_free=-1), dict(block=12), dict(budget=15), dict(held=16)):
+        assert trim(**bad) == -1, bad
+
+    def rope(Hq=1, Hk=0, dtype=0, N_=1, D=64, rot=64, cu=None, n=0, wide=0, ahead=None, rows=0, on=64):
+        return lib.kvt_rope(N, 64, 64, Hq, N, on, 64, N, 0, 0, Hk, N, 0, 0, dtype, N_, D, rot, N, N, wide, cu, n, N, ahead, rows, 1.0, 0,
+                            0, N)
+    for bad in (dict(Hq=0), dict(Hk=-1), dict(dtype=3), dict(D=258), dict(rot=66), dict(rot=7), dict(rot=0), dict(N_=-1),
+                dict(cu=16), dict(cu=16, n=5000), dict(cu=16, n=1, wide=1), dict(cu=16, n=1, ahead=16), dict(ahead=16), dict(on=128)):
+        assert rope(**bad) == -1, bad
+    assert rope(N_=1 << 24) == -3 and rope(N_=0) == 0
+    assert ctypes
+
+
+def test_cache_without_evicting_refuses(kvt_pkg):
+    from kvtier.block_kv import BlockKVCache
+    c = BlockKVCache(1, 1, 64, 2, 1, 2, device="cpu")
+    assert c.weights is None
+    for call in (lambda: c.weigh_decode(0, None, None), lambda: c.weigh_prefill(0, None, None), lambda: c.evict([0], 64)):
+        with pytest.raises(ValueError):
+            call()
+    c = BlockKVCache(2, 3, 64, 2, 1, 2, device="cpu", block=32, evicting=True)
+    assert c.weights.shape == c.pos.shape == (2, 1, 3, 64)
+    s = c.add_seq()
+    c.evicted[s] = c.held[s] = 9
+    c.release(s)
+    assert int(c.evicted[s]) == int(c.held[s]) == 0
+    c.status.fill_(16)
+    with pytest.raises(RuntimeError, match="handed out"):
+        c.check()
+
+
+def test_rotary_frequencies(kvt_pkg):
+    from kvtier.rope import rotary_frequencies
+    plain, one = rotary_frequencies(64, 1e4, device="cpu")
+    assert plain.dtype == torch.float64 and one == 1.0
+    assert [abs(float(x) - 1e4 ** (-i / 32)) <= 1e-15 for i, x in enumerate(plain)] == [True] * 32
+    assert torch.equal(rotary_frequencies(64, 1e4, "linear", 4.0, device="cpu")[0], plain / 4)
+    ntk = rotary_frequencies(64, 1e4, "ntk", 4.0, device="cpu")[0]
+    assert float(ntk[0]) == 1.0 and abs(float(ntk[-1] * 4 / plain[-1]) - 1) < 1e-12
+    long, scale = rotary_frequencies(64, 1e4, "yarn", 4.0, 4096, device="cpu")
+    assert abs(scale - (0.1 * math.log(4) + 1)) < 1e-15
+    turns = 4096 * plain / (2 * math.pi)
+    assert torch.equal(long[turns > 40], plain[turns > 40])                   # fast ones stay, slow ones are divided
+    assert torch.allclose(long[turns < 0.7], plain[turns < 0.7] / 4, rtol=1e-12)
+    assert ((long <= plain) & (long >= plain / 4 * (1 - 1e-12))).all()
+    own, s = rotary_frequencies(4, 100.0, factors=[1.0, 5.0], attention=1.5, device="cpu")
+    assert own.tolist() == [1.0, 0.1 / 5.0] and s == 1.5
+    for bad in (dict(dim=5), dict(dim=0), dict(method="other"), dict(factor=0.0), dict(base=-1.0), dict(factors=[1.0]),
+                dict(factors=[1.0] * 4, method="linear"), dict(method="yarn"), dict(method="yarn", original=100, beta_fast=1.0),
+                dict(dim=2, method="ntk")):
+        with pytest.raises(ValueError):
+            rotary_frequencies(**{**dict(dim=8, device="cpu"), **bad})

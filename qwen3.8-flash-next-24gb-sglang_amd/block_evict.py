@@ -32,6 +32,8 @@ from .block_kv import BLOCKS, CODE, FREE_OVER, _grown, _i32, _pool, _rows16, _st
 
 # Workgroups of a launch that few requests are split for.
 _WORKGROUPS = 2048
+_ROW_BLOCKS = 4096
+_CHUNK_BLOCKS = 4096
 
 
 @dataclass
@@ -91,14 +93,15 @@ def kvt_block_weigh(q: torch.Tensor, k8: torch.Tensor, ks: torch.Tensor, block_t
     gs, pairs = Hq // H, n * H
     row_splits = 1
     if cu_q is None:
-        splits = max(1, min(1024, _WORKGROUPS // pairs, -(-cap // 256)))
+        splits = max(1, min(256, _ROW_BLOCKS // pairs, -(-cap // 256)))
         pos_splits = max(1, min(_WORKGROUPS // pairs, -(-cap // 1024)))
         need = pairs * gs * cap + pairs * splits * 32
     else:
         items = rows * gs // 256 + n
-        splits = max(1, min(1024, _WORKGROUPS // (items * H), -(-cap // 256)))
-        pos_splits = max(1, min(2 * _WORKGROUPS // pairs, -(-cap // 256)))
-        row_splits = max(1, min(1024, _WORKGROUPS // (pairs * pos_splits), -(-rows * gs // 512)))
+        splits = max(1, min(1024, max(512 // (items * H), min(_CHUNK_BLOCKS // (items * H), cap // 1024))))
+        pos_splits = max(1, min(_CHUNK_BLOCKS // pairs, -(-cap // 256)))
+        each = pairs * pos_splits
+        row_splits = max(1, min(1024, max(512 // each, min(_CHUNK_BLOCKS // each, rows * gs // (1024 * n)))))
         need = rows * Hq * 2 * (splits + 1) + (row_splits * pairs * cap if row_splits > 1 else 0)
     ws = {} if workspace is None else workspace             # (held until the launch)
     work = _grown(ws, "weigh", need, q)

@@ -50,6 +50,7 @@ struct Weigh {
   float* sums;                 // chunks: [row_splits, n * H, cap]
   int64_t sq_n, sq_h, stride, sw_r, sw_h, so_r, so_h;
   float scale_log2;
+  uint32_t per_gs;             // ceil(2^32 / gs): row / gs is the high half of a product, exact for rows below 2^28
   int n, n_rows, n_q, H, gs, n_blocks, max_blocks, log2b, splits, row_splits, pos_splits;
 };
 
@@ -93,6 +94,8 @@ KVT_DEV f16v mfma32(u4v a, u4v b, f16v c) {
 // K's scale times the softmax scale in powers of two; NaN for a scale that is not finite (>= 0).
 KVT_DEV float factor(const Weigh& P, float sk) { return fmaf(P.scale_log2, sk, sk - sk); }
 
+KVT_DEV int query_of(const Weigh& P, int row) { return P.gs == 1 ? row : (int)__umulhi((uint32_t)row, P.per_gs); }
+
 struct Req {
   int trow, q0, q_len, kv, len;      // table row, first query, queries, entries, entries of the table
 };
@@ -108,6 +111,11 @@ KVT_DEV Req request(const Weigh& P, int r) {
   t.len = (int)min((int64_t)t.kv, (int64_t)P.max_blocks << P.log2b);
   if (t.trow < 0 || t.trow >= P.n_rows) t.len = 0, t.trow = 0;
   return t;
+}
+// Element offset of the q row of the request's row (query, q head of KV head h).
+KVT_DEV int64_t q_offset(const Weigh& P, const Req& t, int h, int row) {
+  const int i = query_of(P, row);
+  return (int64_t)(t.q0 + i) * P.sq_n + (int64_t)(h * P.gs + row - i * P.gs) * P.sq_h;
 }
 // Entries that query i of the request sees.
 KVT_DEV int sees(const Req& t, int i) { return (int)min((int64_t)t.len, max((int64_t)t.kv - t.q_len + i + 1, (int64_t)0)); }
@@ -213,7 +221,8 @@ __global__ __launch_bounds__(256) void weigh_rows_kernel(const Weigh P) {
   }
 }
 
-// Maximum and 1 / sum of the pair's rows from the splits' parts, then the columns of 1,024 positions at a time.
+// Maximum and 1 / sum of the pair's rows from the splits' parts, then the columns of 1,024 positions at a time, four per
+// thread.
 __global__ __launch_bounds__(256) void weigh_columns_kernel(const Weigh P) {
   __shared__ float2 J[16][16];
   __shared__ float2 norm[16];
@@ -221,10 +230,11 @@ __global__ __launch_bounds__(256) void weigh_columns_kernel(const Weigh P) {
   const Req t = request(P, r);
   if ((int64_t)split * 1024 >= t.len) return;
   const int64_t pair_id = (int64_t)r * P.H + h, cap = (int64_t)P.max_blocks << P.log2b;
-  const int used = (t.len + per_split(t.len, P.splits) - 1) / per_split(t.len, P.splits);
+  const int per = per_split(t.len, P.splits), used = (t.len + per - 1) / per;
   {
     const int l = threadIdx.x & 15, c = threadIdx.x >> 4;
     float m = -kInf, s = 0.0f;
+#pragma unroll 4
     for (int i = c; i < used; i += 16) {
       const float2 a = P.part[(pair_id * P.splits + i) * 16 + l];
       join(m, s, a.x, a.y);
@@ -236,26 +246,32 @@ __global__ __launch_bounds__(256) void weigh_columns_kernel(const Weigh P) {
     float2 a = J[0][threadIdx.x];
 #pragma unroll
     for (int c = 1; c < 16; ++c) join(a.x, a.y, J[c][threadIdx.x].x, J[c][threadIdx.x].y);
-    norm[threadIdx.x] = make_float2(a.x, 1.0f / a.y);
+    // (rows behind the last one: nothing)
+    norm[threadIdx.x] = (int)threadIdx.x < P.gs ? make_float2(a.x, 1.0f / a.y) : make_float2(kInf, 0.0f);
   }
   __syncthreads();
-  const float* score = P.scores + pair_id * P.gs * cap;
   for (int64_t base = (int64_t)split * 1024; base < t.len; base += (int64_t)P.pos_splits * 1024) {
+    const int p = (int)base + 4 * threadIdx.x;
+    if (p >= t.len) break;
+    const int id = P.table[(int64_t)t.trow * P.stride + (p >> P.log2b)];      // (four positions of one block)
+    const float* score = P.scores + pair_id * P.gs * cap + p;
     float sum[4] = {0, 0, 0, 0};
-    const int p = (int)base + threadIdx.x;
-    for (int g = 0; g < P.gs; ++g) {
-      const float2 a = norm[g];
+    for (int g = 0; g < P.gs; g += 4) {
+      f4 x[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (p + 256 * i < t.len) sum[i] = fmaf(exp2_(score[g * cap + p + 256 * i] - a.x), a.y, sum[i]);
-    }
+      for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const f4*>(score + min(g + k, P.gs - 1) * cap);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int e = p + 256 * i;
-      if (e >= t.len) break;
-      const int id = P.table[(int64_t)t.trow * P.stride + (e >> P.log2b)];
-      finish(P, t, r, h, e, id >= 0 && id < P.n_blocks ? sum[i] : 0.0f);
+      for (int k = 0; k < 4; ++k) {
+        const float2 a = norm[g + k];
+        if (g + k < P.gs)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[i] = fmaf(exp2_(x[k][i] - a.x), a.y, sum[i]);
+      }
     }
+    const bool there = id >= 0 && id < P.n_blocks;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (p + i < t.len) finish(P, t, r, h, p + i, there ? sum[i] : 0.0f);
   }
 }
 
@@ -273,18 +289,19 @@ KVT_DEV int prow(int i, int hl) { return 8 * (i >> 2) + 4 * hl + (i & 3); }
 
 // Maxima and sums of 256 rows over a split of the positions.
 template <int CODE, int QT, int D>
-__global__ __launch_bounds__(256) void weigh_norm_kernel(const Weigh P, int items) {
+__global__ __launch_bounds__(256, 2) void weigh_norm_kernel(const Weigh P, int items) {
   constexpr int KS = D / 16, NL = D / 64;     // products per tile of 32; 16-byte loads per thread and tile
   constexpr int TPR = D / 16;                 // threads per streamed row
   __shared__ __attribute__((aligned(16))) uint8_t tile[2][kStep * kPitch<D>];
-  const int item = blockIdx.x % items, w = blockIdx.x / items, h = w % P.H, split = w / P.H;
+  // (the last items see the most: they begin first)
+  const int item = items - 1 - blockIdx.x % items, w = blockIdx.x / items, h = w % P.H, split = w / P.H;
   const int r = find_request(P.cu, P.n, item, P.gs, kTileRows, 1);
   const Req t = request(P, r);
-  const int64_t row0 = (item - first_item(uniform(P.cu[r]), r, P.gs, kTileRows, 1)) * kTileRows;
-  const int64_t n_rows = (int64_t)t.q_len * P.gs;
-  if (row0 < 0 || row0 >= n_rows) return;
-  const int live = (int)min(n_rows - row0, (int64_t)kTileRows);
-  const int limit = sees(t, (int)((row0 + live - 1) / P.gs));
+  const int64_t begin = (item - first_item(uniform(P.cu[r]), r, P.gs, kTileRows, 1)) * kTileRows;
+  const int n_rows = t.q_len * P.gs;
+  if (begin < 0 || begin >= n_rows) return;
+  const int row0 = (int)begin, live = min(n_rows - row0, kTileRows);
+  const int limit = sees(t, query_of(P, row0 + live - 1));
   const int per = (((limit + kStep - 1) / kStep + P.splits - 1) / P.splits) * kStep;
   const int p_begin = (int)min((int64_t)split * per, (int64_t)limit), p_end = (int)min((int64_t)p_begin + per, (int64_t)limit);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 31, hl = lane >> 5;
@@ -292,18 +309,15 @@ __global__ __launch_bounds__(256) void weigh_norm_kernel(const Weigh P, int item
   u4v Q[2][KS];
   int see[2];
   float m[2] = {-kInf, -kInf}, sum[2] = {0, 0};
-  int64_t at_row[2];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const int mine = 64 * wave + 32 * c + l;
-    const int64_t row = row0 + (mine < live ? mine : 0);
-    at_row[c] = mine < live ? (int64_t)t.q0 * P.gs + row : -1;
-    see[c] = sees(t, (int)(row / P.gs));
-    const uint16_t* p = (const uint16_t*)P.q + (t.q0 + row / P.gs) * P.sq_n + (h * P.gs + row % P.gs) * P.sq_h;
+    const int mine = 64 * wave + 32 * c + l, row = row0 + (mine < live ? mine : 0);
+    see[c] = sees(t, query_of(P, row));
+    const uint16_t* p = (const uint16_t*)P.q + q_offset(P, t, h, row);
 #pragma unroll
     for (int k = 0; k < KS; ++k) Q[c][k] = *reinterpret_cast<const u4v*>(p + channel<false>(k, hl));
   }
-  const int all_see = sees(t, (int)(row0 / P.gs));
+  const int all_see = sees(t, query_of(P, row0));
   const bool idle = 64 * wave >= live;
   const int64_t tbl = (int64_t)t.trow * P.stride;
 
@@ -320,12 +334,10 @@ __global__ __launch_bounds__(256) void weigh_norm_kernel(const Weigh P, int item
   auto load = [&](int p0, int i) {
 #pragma unroll
     for (int k = 0; k < NL; ++k) {
-      const int row = tr + k * (256 / TPR);
-      const int b = __shfl(id, 4 * i + (row >> 4), 64);
-      raw[k] = u4v{0, 0, 0, 0};
-      if (b >= 0)
-        raw[k] = *reinterpret_cast<const u4v*>(
-            P.k8 + ((((int64_t)b * P.H + h) << P.log2b) + ((p0 + row) & ((1 << P.log2b) - 1))) * D + 16 * tc);
+      const int row = tr + k * (256 / TPR);             // (a wavefront's rows are of one quarter)
+      const int b = max(__builtin_amdgcn_readlane(id, 4 * i + uniform(row >> 4)), 0);
+      raw[k] = *reinterpret_cast<const u4v*>(
+          P.k8 + ((((int64_t)b * P.H + h) << P.log2b) + ((p0 + row) & ((1 << P.log2b) - 1))) * D + 16 * tc);
     }
   };
   if (p_begin < p_end) {
@@ -365,24 +377,32 @@ __global__ __launch_bounds__(256) void weigh_norm_kernel(const Weigh P, int item
 #pragma unroll
           for (int c = 0; c < 2; ++c) acc[c] = mfma32<QT>(a, Q[c][k], acc[c]);
         }
+        if (edge) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int at = prow(i, hl);
+              const bool is = (at & 15) < valid[2 * s + (i >> 3)] && p0 + 32 * s + at < see[c];
+              acc[c][i] = is ? acc[c][i] * f[2 * s + (i >> 3)] : -kInf;
+            }
+        }
+        const float f0 = edge ? 1.0f : f[2 * s], f1 = edge ? 1.0f : f[2 * s + 1];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float x[16], top = m[c];
+          // (scales are >= 0: the largest score of a block is its largest product's)
+          float t0 = acc[c][0], t1 = acc[c][8];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int sub = 2 * s + (i >> 3);
-            x[i] = acc[c][i] * f[sub];
-            if (edge) {
-              const int at = prow(i, hl);
-              x[i] = (at & 15) < valid[sub] && p0 + 32 * s + at < see[c] ? x[i] : -kInf;
-            }
-            top = fmaxf(top, x[i]);
+          for (int i = 1; i < 8; ++i) t0 = fmaxf(t0, acc[c][i]), t1 = fmaxf(t1, acc[c][8 + i]);
+          const float top = fmaxf(m[c], fmaxf(t0 * f0, t1 * f1)), ref = top == -kInf ? 0.0f : top;
+          float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            s0 += exp2_(fmaf(acc[c][i], f0, -ref));
+            s1 += exp2_(fmaf(acc[c][8 + i], f1, -ref));
           }
-          const float ref = top == -kInf ? 0.0f : top;
-          sum[c] *= exp2_(m[c] - ref);
+          sum[c] = fmaf(sum[c], exp2_(m[c] - ref), s0 + s1);
           m[c] = top;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sum[c] += exp2_(x[i] - ref);
         }
       }
     }
@@ -391,34 +411,45 @@ __global__ __launch_bounds__(256) void weigh_norm_kernel(const Weigh P, int item
   for (int c = 0; c < 2; ++c) {
     const float m2 = __shfl_xor(m[c], 32, 64), s2 = __shfl_xor(sum[c], 32, 64);
     join(m[c], sum[c], m2, s2);
-    if (hl == 0 && at_row[c] >= 0) {
-      const int64_t at = (int64_t)h * P.n_q * P.gs + at_row[c];
+    const int mine = 64 * wave + 32 * c + l;
+    if (hl == 0 && mine < live) {
+      const int64_t at = ((int64_t)h * P.n_q + t.q0) * P.gs + row0 + mine;
       if (P.splits == 1) P.norm[at] = make_float2(m[c], 1.0f / sum[c]);
       else P.part[split * ((int64_t)P.H * P.n_q * P.gs) + at] = make_float2(m[c], sum[c]);
     }
   }
 }
 
+// Joins the splits' maxima and sums: LANES lanes per row.
+template <int LANES>
 __global__ __launch_bounds__(256) void weigh_join_kernel(const Weigh P) {
-  const int64_t total = (int64_t)P.H * P.n_q * P.gs, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  if ((i / P.gs) % P.n_q >= P.cu[P.n]) return;      // (padding: no parts)
+  constexpr int R = 64 / LANES;               // rows of a wavefront
+  const int per_head = P.n_q * P.gs, h = blockIdx.y, lane = threadIdx.x & 63;
+  const int i = blockIdx.x * 4 * R + (threadIdx.x >> 6) * R + lane % R;
+  const int64_t total = (int64_t)P.H * per_head, at = (int64_t)h * per_head + i;
+  const bool is = i < per_head && query_of(P, i) < P.cu[P.n];      // (padding has no parts)
   float m = -kInf, s = 0.0f;
-  for (int k = 0; k < P.splits; ++k) {
-    const float2 a = P.part[k * total + i];
-    join(m, s, a.x, a.y);
+  if (is) {
+#pragma unroll 4
+    for (int k = lane / R; k < P.splits; k += LANES) {
+      const float2 a = P.part[k * total + at];
+      join(m, s, a.x, a.y);
+    }
   }
-  P.norm[i] = make_float2(m, 1.0f / s);
+#pragma unroll
+  for (int o = R; o < 64; o <<= 1) {
+    const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
+    join(m, s, m2, s2);
+  }
+  if (is && lane < R) P.norm[at] = make_float2(m, 1.0f / s);
 }
 
-// Rows per split of a request's (query, q head) rows: equal shares in multiples of 64, 512 at least.
-KVT_DEV int64_t per_row_split(int64_t n_rows, int splits) { 
-  return max(((n_rows + splits - 1) / splits + 63) & ~(int64_t)63, (int64_t)512);
-}
+// Rows per split of a request's (query, q head) rows: equal shares in multiples of 64, 128 at least.
+KVT_DEV int per_row_split(int n_rows, int splits) { return max(((n_rows + splits - 1) / splits + 63) & ~63, 128); }
 
 // Column sums of 256 positions over a split of the request's rows.
 template <int CODE, int QT, int D>
-__global__ __launch_bounds__(256) void weigh_sums_kernel(const Weigh P) {
+__global__ __launch_bounds__(256, 2) void weigh_sums_kernel(const Weigh P) {
   constexpr int KS = D / 16, NL = D / 32;     // products per tile of 32 rows; 16-byte loads per thread and tile of Q
   constexpr int TPR = D / 8;
   __shared__ __attribute__((aligned(16))) uint8_t tile[2][kStep * kPitch<D>];
@@ -430,55 +461,54 @@ __global__ __launch_bounds__(256) void weigh_sums_kernel(const Weigh P) {
   w /= P.H;
   const int rs = w % P.row_splits, r = w / P.row_splits;
   const Req t = request(P, r);
-  const int64_t n_rows = (int64_t)t.q_len * P.gs, per = per_row_split(n_rows, P.row_splits);
-  const int64_t r_begin = rs * per, r_end = min(r_begin + per, n_rows);
+  const int n_rows = t.q_len * P.gs, per = per_row_split(n_rows, P.row_splits);
+  const int r_begin = (int)min((int64_t)rs * per, (int64_t)n_rows), r_end = min(r_begin + per, n_rows);
   if (r_begin >= r_end && rs > 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 31, hl = lane >> 5;
   const int64_t cap = (int64_t)P.max_blocks << P.log2b;
   const int tr = threadIdx.x / TPR, tc = threadIdx.x % TPR;
   const float2* norm = P.norm + ((int64_t)h * P.n_q + t.q0) * P.gs;
+  const int older = t.kv - t.q_len;           // entries before the queries' own (negative: some queries see nothing)
 
   for (int64_t p0 = (int64_t)split * kTilePos; p0 < t.len; p0 += (int64_t)P.pos_splits * kTilePos) {
     u4v K[2][KS];
     float f[2], sum[2] = {0, 0};
-    int64_t first[2];           // the first row that sees the lane's position
+    int first[2];               // the first row that sees the lane's position
     bool there[2];
+    // the first row that sees position p (the number of rows where none does)
+    auto row_of = [&](int64_t p) { return (int)min(max(p - older, (int64_t)0), (int64_t)t.q_len) * P.gs; };
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int64_t p = p0 + 64 * wave + 32 * c + l;
-      int id = p < t.len ? P.table[(int64_t)t.trow * P.stride + (p >> P.log2b)] : -1;
+      const int id = p < t.len ? P.table[(int64_t)t.trow * P.stride + (p >> P.log2b)] : -1;
       there[c] = id >= 0 && id < P.n_blocks;
       f[c] = there[c] ? factor(P, P.ks[(int64_t)id * P.H + h]) : 0.0f;
-      first[c] = max(p - ((int64_t)t.kv - t.q_len), (int64_t)0) * P.gs;
+      first[c] = row_of(p);
       const uint8_t* kp = P.k8 + ((((int64_t)(there[c] ? id : 0) * P.H + h) << P.log2b) + (p & ((1 << P.log2b) - 1))) * D + 16 * hl;
 #pragma unroll
       for (int k = 0; k < KS / 2; ++k) {
-        u4v v = {0, 0, 0, 0};
-        if (there[c]) v = *reinterpret_cast<const u4v*>(kp + 32 * k);
+        const u4v v = *reinterpret_cast<const u4v*>(kp + 32 * k);
         K[c][2 * k] = eight<CODE, QT>(v[0], v[1]);
         K[c][2 * k + 1] = eight<CODE, QT>(v[2], v[3]);
       }
     }
-    // rows that see any of the workgroup's positions, and those that see all of them
-    const int64_t some = max((p0 - ((int64_t)t.kv - t.q_len)) * P.gs, r_begin) & ~(int64_t)(kStep - 1);
-    const int64_t all = (min(p0 + kTilePos, (int64_t)t.len) - 1 - ((int64_t)t.kv - t.q_len)) * P.gs;
+    // the first rows that see any of the workgroup's positions, and all of them
+    const int some = max(row_of(p0), r_begin) & ~(kStep - 1);
+    const int all = row_of(min(p0 + kTilePos, (int64_t)t.len) - 1);
     const bool idle = p0 + 64 * wave >= t.len;
     u4v raw[NL];
     float2 nr;
-    auto load = [&](int64_t r0) {
+    auto load = [&](int r0) {
 #pragma unroll
       for (int k = 0; k < NL; ++k) {
-        const int64_t row = r0 + tr + k * (256 / TPR);
-        raw[k] = u4v{0, 0, 0, 0};
-        if (row < r_end)
-          raw[k] = *reinterpret_cast<const u4v*>((const uint16_t*)P.q + (t.q0 + row / P.gs) * P.sq_n +
-                                                 (h * P.gs + row % P.gs) * P.sq_h + 8 * tc);
+        const int row = min(r0 + tr + k * (256 / TPR), r_end - 1);      // (rows behind the last one count for nothing)
+        raw[k] = *reinterpret_cast<const u4v*>((const uint16_t*)P.q + q_offset(P, t, h, row) + 8 * tc);
       }
-      if (threadIdx.x < kStep) nr = r0 + threadIdx.x < r_end ? norm[r0 + threadIdx.x] : make_float2(kInf, 0.0f);
+      if (threadIdx.x < kStep) nr = r0 + (int)threadIdx.x < r_end ? norm[r0 + threadIdx.x] : make_float2(kInf, 0.0f);
     };
     if (some < r_end) load(some);
     int buf = 0;
-    for (int64_t r0 = some; r0 < r_end; r0 += kStep, buf ^= 1) {
+    for (int r0 = some; r0 < r_end; r0 += kStep, buf ^= 1) {
       uint8_t* T = tile[buf];
 #pragma unroll
       for (int k = 0; k < NL; ++k) *reinterpret_cast<u4v*>(T + (tr + k * (256 / TPR)) * kPitch<D> + 16 * tc) = raw[k];
@@ -500,14 +530,21 @@ __global__ __launch_bounds__(256) void weigh_sums_kernel(const Weigh P) {
           for (int i = 0; i < 16; i += 4) {
             const f4 mm = *reinterpret_cast<const f4*>(&top[buf][32 * s + prow(i, hl)]);
             const f4 li = *reinterpret_cast<const f4*>(&inv[buf][32 * s + prow(i, hl)]);
+            if (!edge) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+              for (int c = 0; c < 2; ++c)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float e = exp2_(fmaf(acc[c][i + j], f[c], -mm[j])) * li[j];
-                const int64_t row = r0 + 32 * s + prow(i, hl) + j;
-                sum[c] += !edge || (row >= first[c] && row < r_end) ? e : 0.0f;
-              }
+                for (int j = 0; j < 4; ++j) sum[c] = fmaf(exp2_(fmaf(acc[c][i + j], f[c], -mm[j])), li[j], sum[c]);
+            } else {
+              const int row = r0 + 32 * s + prow(i, hl);
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const float e = exp2_(fmaf(acc[c][i + j], f[c], -mm[j])) * li[j];
+                  sum[c] += row + j >= first[c] && row + j < r_end ? e : 0.0f;
+                }
+            }
           }
         }
       }
@@ -528,8 +565,8 @@ __global__ __launch_bounds__(256) void weigh_sums_kernel(const Weigh P) {
 __global__ __launch_bounds__(256) void weigh_add_kernel(const Weigh P) {
   const int h = blockIdx.x % P.H, w = blockIdx.x / P.H, split = w % P.pos_splits, r = w / P.pos_splits;
   const Req t = request(P, r);
-  const int64_t n_rows = (int64_t)t.q_len * P.gs, per = per_row_split(n_rows, P.row_splits);
-  const int used = max((int)((n_rows + per - 1) / per), 1);
+  const int n_rows = t.q_len * P.gs, per = per_row_split(n_rows, P.row_splits);
+  const int used = max((n_rows + per - 1) / per, 1);
   const int64_t cap = (int64_t)P.max_blocks << P.log2b, step = (int64_t)P.n * P.H * cap;
   for (int64_t p = (int64_t)split * 256 + threadIdx.x; p < t.len; p += (int64_t)P.pos_splits * 256) {
     float s = 0.0f;
@@ -551,7 +588,9 @@ int launch(Weigh P, hipStream_t st) {
   weigh_norm_kernel<CODE, QT, D><<<items * P.H * P.splits, 256, 0, st>>>(P, items);
   KVT_CHECK_LAUNCH();
   if (P.splits > 1 && P.n_q > 0) {
-    weigh_join_kernel<<<(int)(((int64_t)P.H * P.n_q * P.gs + 255) / 256), 256, 0, st>>>(P);
+    const int rows = P.n_q * P.gs;
+    if (P.splits <= 8) weigh_join_kernel<4><<<dim3((rows + 63) / 64, P.H), 256, 0, st>>>(P);
+    else weigh_join_kernel<32><<<dim3((rows + 7) / 8, P.H), 256, 0, st>>>(P);
     KVT_CHECK_LAUNCH();
   }
   weigh_sums_kernel<CODE, QT, D><<<P.n * P.row_splits * P.H * P.pos_splits, 256, 0, st>>>(P);
@@ -596,7 +635,7 @@ extern "C" int kvt_block_weigh(const void* q, int64_t sq_n, int64_t sq_h, int q_
   const int64_t items = (int64_t)n_q * gs / kTileRows + n;
   const int64_t most = 1 << 24;                                     // (2^32 threads of a launch)
   if ((cu_q ? items : (int64_t)n) * H * splits >= most || (int64_t)n * H * row_splits * pos_splits >= most ||
-      (int64_t)H * n_q * gs >= most * 128)
+      (int64_t)n_q * gs >= most * 16 || H > 65535)
     return KVT_ERANGE;
   const Space s = space(n, n_q, H, gs, cap, cu_q != nullptr, splits, row_splits);
   if (s.scores + s.part + s.norm + s.sums > work_floats) return KVT_EINVAL;
@@ -611,6 +650,7 @@ extern "C" int kvt_block_weigh(const void* q, int64_t sq_n, int64_t sq_h, int q_
   P.scale_log2 = scale * kLog2e;
   P.n = n, P.n_rows = n_rows, P.n_q = n_q, P.H = H, P.gs = gs, P.n_blocks = n_blocks, P.max_blocks = max_blocks;
   P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6;
+  P.per_gs = (uint32_t)((((uint64_t)1 << 32) + gs - 1) / gs);
   P.splits = splits, P.row_splits = row_splits, P.pos_splits = pos_splits;
   hipStream_t st = (hipStream_t)stream;
   if (code == kE4M3) return q_type == kBF16 ? launch_d<kE4M3, kBF16>(P, D, st) : launch_d<kE4M3, kF16>(P, D, st);

@@ -30,10 +30,16 @@ import torch
 from . import _lib
 from .block_kv import BLOCKS, CODE, FREE_OVER, _grown, _i32, _pool, _rows16, _stream
 
-# Workgroups of a launch that few requests are split for.
-_WORKGROUPS = 2048
+# Workgroups of the launches.  One query per request: the scores' (at most 256 splits of a pair, whose maxima and sums
+# every workgroup of the sums reads; us per call with 512 / 1,024 / 2,048 / 4,096: 32 requests x 2 heads, D 256, up to 16,384
+# positions 49 / 43 / 45 / 42, int8 64 x 8, D 128, up to 8,191 133 / 96 / 84 / 77) and the sums'.
 _ROW_BLOCKS = 4096
+_WORKGROUPS = 2048
+# Chunks: this many where the work allows pieces of 512 positions (rows) at least (1,024 / 2,048 / 4,096 / 8,192: a prompt
+# of 10,001, D 256, 1,071 / 890 / 867 / 890; 8 x 64 queries, D 128, 148 / 143 / 136 / 135), and as many as fit the CUs where it does not
+# (61 queries x 12 heads over 60,000 positions, D 128: 256 64.4, 512 53.5, 768 50.1, 1,024 53.2).
 _CHUNK_BLOCKS = 4096
+_CHUNK_FIT = {64: 1024, 128: 768, 256: 512}
 
 
 @dataclass
@@ -98,10 +104,12 @@ def kvt_block_weigh(q: torch.Tensor, k8: torch.Tensor, ks: torch.Tensor, block_t
         need = pairs * gs * cap + pairs * splits * 32
     else:
         items = rows * gs // 256 + n
-        splits = max(1, min(1024, max(512 // (items * H), min(_CHUNK_BLOCKS // (items * H), cap // 1024))))
+        fit = _CHUNK_FIT[D]
+        splits = min(max(fit // (items * H), min(_CHUNK_BLOCKS // (items * H), cap // 512)), cap // 128, 1024)
+        splits = max(splits, 1)
         pos_splits = max(1, min(_CHUNK_BLOCKS // pairs, -(-cap // 256)))
         each = pairs * pos_splits
-        row_splits = max(1, min(1024, max(512 // each, min(_CHUNK_BLOCKS // each, rows * gs // (1024 * n)))))
+        row_splits = max(1, min(1024, max(fit // each, min(_CHUNK_BLOCKS // each, rows * gs // (512 * n)))))
         need = rows * Hq * 2 * (splits + 1) + (row_splits * pairs * cap if row_splits > 1 else 0)
     ws = {} if workspace is None else workspace             # (held until the launch)
     work = _grown(ws, "weigh", need, q)

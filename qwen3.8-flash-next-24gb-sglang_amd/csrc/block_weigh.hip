@@ -16,6 +16,8 @@
 // their own: no atomics, the same bits for every call.
 //
 // Operands have q's type (codes of 8 bits are exact in bf16 and fp16); scores, maxima, sums and weights are fp32.
+#include <type_traits>
+
 #include "block_common.h"
 
 using namespace kvt;
@@ -50,7 +52,7 @@ struct Weigh {
   float* sums;                 // chunks: [row_splits, n * H, cap]
   int64_t sq_n, sq_h, stride, sw_r, sw_h, so_r, so_h;
   float scale_log2;
-  uint32_t per_gs;             // ceil(2^32 / gs): row / gs is the high half of a product, exact for rows below 2^28
+  uint32_t per_gs;             // ceil(2^31 / gs): row / gs is the high half of a product, exact for rows below 2^27
   int n, n_rows, n_q, H, gs, n_blocks, max_blocks, log2b, splits, row_splits, pos_splits;
 };
 
@@ -94,7 +96,7 @@ KVT_DEV f16v mfma32(u4v a, u4v b, f16v c) {
 // K's scale times the softmax scale in powers of two; NaN for a scale that is not finite (>= 0).
 KVT_DEV float factor(const Weigh& P, float sk) { return fmaf(P.scale_log2, sk, sk - sk); }
 
-KVT_DEV int query_of(const Weigh& P, int row) { return P.gs == 1 ? row : (int)__umulhi((uint32_t)row, P.per_gs); }
+KVT_DEV int query_of(const Weigh& P, int row) { return (int)__umulhi((uint32_t)row << 1, P.per_gs); }
 
 struct Req {
   int trow, q0, q_len, kv, len;      // table row, first query, queries, entries, entries of the table
@@ -284,6 +286,43 @@ template <int D> constexpr int kPitch = 2 * D + 16;
 template <bool SIXTEEN>
 KVT_DEV int channel(int k, int hl) { return SIXTEEN ? 32 * (k >> 1) + 16 * hl + 8 * (k & 1) : 16 * k + 8 * hl; }
 
+// BYTES per lane from each lane's address into lds + BYTES * lane.  M0 (the LDS base) is an input of the statement, so the
+// compiler sets it; the s_nop covers the wait states after that, which its hazard checks do not look for inside inline
+// assembly.  (With the builtin it waits for the copy before every later LDS read.)  The caller waits: vmcnt(0) and a
+// barrier.
+template <int BYTES>
+KVT_DEV void copy_to_lds(const void* from, void* lds) {
+  const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
+  if constexpr (BYTES == 16)
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(base) : "memory");
+  else
+    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" : : "v"(from), "{m0}"(base) : "memory");
+}
+
+// The products of a streamed tile of 32 rows, whose operand k is read(k), with two held ones: operands are read a batch
+// ahead of their products.  (By itself the compiler reads each one into the registers of the last, and every two
+// products wait for LDS.)
+template <int QT, int KS, class Read>
+KVT_DEV void products(Read read, const u4v (&held)[2][KS], f16v (&acc)[2]) {
+  constexpr int N = KS > 4 ? 2 : 4;           // (registers)
+  u4v a[2][N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[0][i] = read(i);
+#pragma unroll
+  for (int b = 0; b < KS / N; ++b) {
+    if (b + 1 < KS / N) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) a[(b + 1) & 1][i] = read(N * (b + 1) + i);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) acc[c] = mfma32<QT>(a[b & 1][i], held[c][N * b + i], acc[c]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // Row (of 32) that register i of a 32 x 32 product has in lanes of half hl.
 KVT_DEV int prow(int i, int hl) { return 8 * (i >> 2) + 4 * hl + (i & 3); }
 
@@ -317,8 +356,10 @@ __global__ __launch_bounds__(256, 2) void weigh_norm_kernel(const Weigh P, int i
 #pragma unroll
     for (int k = 0; k < KS; ++k) Q[c][k] = *reinterpret_cast<const u4v*>(p + channel<false>(k, hl));
   }
-  const int all_see = sees(t, query_of(P, row0));
+  // what all of the wavefront's rows see, and any of them
   const bool idle = 64 * wave >= live;
+  const int all_see = idle ? 0 : uniform(sees(t, query_of(P, row0 + 64 * wave)));
+  const int any_see = idle ? 0 : uniform(sees(t, query_of(P, row0 + min(64 * wave + 63, live - 1))));
   const int64_t tbl = (int64_t)t.trow * P.stride;
 
   int id = -1;
@@ -367,27 +408,25 @@ __global__ __launch_bounds__(256, 2) void weigh_norm_kernel(const Weigh P, int i
       load(p0 + kStep, slot);
     }
     __syncthreads();
-    if (!idle) {
+    auto take = [&](auto masked) {
+      constexpr bool EDGE = decltype(masked)::value;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         f16v acc[2] = {};
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const u4v a = *reinterpret_cast<const u4v*>(T + (32 * s + l) * kPitch<D> + 2 * channel<false>(k, hl));
-#pragma unroll
-          for (int c = 0; c < 2; ++c) acc[c] = mfma32<QT>(a, Q[c][k], acc[c]);
-        }
-        if (edge) {
+        products<QT, KS>(
+            [&](int k) { return *reinterpret_cast<const u4v*>(T + (32 * s + l) * kPitch<D> + 2 * channel<false>(k, hl)); }, Q, acc);
+        float f0 = f[2 * s], f1 = f[2 * s + 1];
+        if constexpr (EDGE) {
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int at = prow(i, hl);
               const bool is = (at & 15) < valid[2 * s + (i >> 3)] && p0 + 32 * s + at < see[c];
-              acc[c][i] = is ? acc[c][i] * f[2 * s + (i >> 3)] : -kInf;
+              acc[c][i] = is ? acc[c][i] * (i < 8 ? f0 : f1) : -kInf;
             }
+          f0 = f1 = 1.0f;
         }
-        const float f0 = edge ? 1.0f : f[2 * s], f1 = edge ? 1.0f : f[2 * s + 1];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           // (scales are >= 0: the largest score of a block is its largest product's)
@@ -404,6 +443,14 @@ __global__ __launch_bounds__(256, 2) void weigh_norm_kernel(const Weigh P, int i
           sum[c] = fmaf(sum[c], exp2_(m[c] - ref), s0 + s1);
           m[c] = top;
         }
+      }
+    };
+    if (p0 < any_see) {
+      if (__builtin_expect(edge, 0)) {
+        asm volatile("");                     // (a branch: without it the masks are computed for every tile)
+        take(std::true_type{});
+      } else {
+        take(std::false_type{});
       }
     }
   }
@@ -447,13 +494,15 @@ __global__ __launch_bounds__(256) void weigh_join_kernel(const Weigh P) {
 // Rows per split of a request's (query, q head) rows: equal shares in multiples of 64, 128 at least.
 KVT_DEV int per_row_split(int n_rows, int splits) { return max(((n_rows + splits - 1) / splits + 63) & ~63, 128); }
 
-// Column sums of 256 positions over a split of the request's rows.
+// Column sums of 256 positions over a split of the request's rows.  Q's tiles are copied to LDS without a detour by
+// registers: 16-byte chunk c of row i goes to place c ^ (i & 15) (D 64: & 7), so that a column of chunks is spread over the
+// banks.
 template <int CODE, int QT, int D>
 __global__ __launch_bounds__(256, 2) void weigh_sums_kernel(const Weigh P) {
-  constexpr int KS = D / 16, NL = D / 32;     // products per tile of 32 rows; 16-byte loads per thread and tile of Q
-  constexpr int TPR = D / 8;
-  __shared__ __attribute__((aligned(16))) uint8_t tile[2][kStep * kPitch<D>];
-  __shared__ __attribute__((aligned(16))) float top[2][kStep], inv[2][kStep];
+  constexpr int KS = D / 16, NL = D / 32;     // products per tile of 32 rows; 16-byte copies per thread and tile of Q
+  constexpr int TPR = D / 8, SW = TPR < 16 ? TPR - 1 : 15;
+  __shared__ __attribute__((aligned(16))) uint8_t tile[2][kStep * 2 * D];
+  __shared__ __attribute__((aligned(16))) float2 norms[2][kStep];
   int w = blockIdx.x;
   const int split = w % P.pos_splits;
   w /= P.pos_splits;
@@ -464,19 +513,19 @@ __global__ __launch_bounds__(256, 2) void weigh_sums_kernel(const Weigh P) {
   const int n_rows = t.q_len * P.gs, per = per_row_split(n_rows, P.row_splits);
   const int r_begin = (int)min((int64_t)rs * per, (int64_t)n_rows), r_end = min(r_begin + per, n_rows);
   if (r_begin >= r_end && rs > 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 31, hl = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), l = lane & 31, hl = lane >> 5;
   const int64_t cap = (int64_t)P.max_blocks << P.log2b;
   const int tr = threadIdx.x / TPR, tc = threadIdx.x % TPR;
   const float2* norm = P.norm + ((int64_t)h * P.n_q + t.q0) * P.gs;
   const int older = t.kv - t.q_len;           // entries before the queries' own (negative: some queries see nothing)
+  // the first row that sees position p (the number of rows where none does)
+  auto row_of = [&](int64_t p) { return (int)min(max(p - older, (int64_t)0), (int64_t)t.q_len) * P.gs; };
 
   for (int64_t p0 = (int64_t)split * kTilePos; p0 < t.len; p0 += (int64_t)P.pos_splits * kTilePos) {
     u4v K[2][KS];
     float f[2], sum[2] = {0, 0};
     int first[2];               // the first row that sees the lane's position
     bool there[2];
-    // the first row that sees position p (the number of rows where none does)
-    auto row_of = [&](int64_t p) { return (int)min(max(p - older, (int64_t)0), (int64_t)t.q_len) * P.gs; };
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int64_t p = p0 + 64 * wave + 32 * c + l;
@@ -492,60 +541,62 @@ __global__ __launch_bounds__(256, 2) void weigh_sums_kernel(const Weigh P) {
         K[c][2 * k + 1] = eight<CODE, QT>(v[2], v[3]);
       }
     }
-    // the first rows that see any of the workgroup's positions, and all of them
-    const int some = max(row_of(p0), r_begin) & ~(kStep - 1);
-    const int all = row_of(min(p0 + kTilePos, (int64_t)t.len) - 1);
-    const bool idle = p0 + 64 * wave >= t.len;
-    u4v raw[NL];
-    float2 nr;
-    auto load = [&](int r0) {
+    // the first rows that see any of the workgroup's positions, any of the wavefront's, and all of those
+    const int64_t pw = p0 + 64 * wave;
+    const int begin = max(row_of(p0), r_begin) & ~(kStep - 1);
+    const int some = pw < t.len ? row_of(pw) : r_end, all = row_of(min(pw + 64, (int64_t)t.len) - 1);
+    auto copy = [&](int r0, int buf) {
 #pragma unroll
       for (int k = 0; k < NL; ++k) {
-        const int row = min(r0 + tr + k * (256 / TPR), r_end - 1);      // (rows behind the last one count for nothing)
-        raw[k] = *reinterpret_cast<const u4v*>((const uint16_t*)P.q + q_offset(P, t, h, row) + 8 * tc);
+        const int at = tr + k * (256 / TPR), row = min(r0 + at, r_end - 1);   // (rows behind the last one count for nothing)
+        const uint16_t* from = (const uint16_t*)P.q + q_offset(P, t, h, row) + 8 * (tc ^ (at & SW));
+        copy_to_lds<16>(from, tile[buf] + 4096 * k + 1024 * wave);
       }
-      if (threadIdx.x < kStep) nr = r0 + (int)threadIdx.x < r_end ? norm[r0 + threadIdx.x] : make_float2(kInf, 0.0f);
+      if (wave < 2) {
+        const float* from = (const float*)(norm + min(r0 + 32 * wave + (lane >> 1), r_end - 1)) + (lane & 1);
+        copy_to_lds<4>(from, &norms[buf][32 * wave]);
+      }
     };
-    if (some < r_end) load(some);
+    if (begin < r_end) copy(begin, 0);
     int buf = 0;
-    for (int r0 = some; r0 < r_end; r0 += kStep, buf ^= 1) {
-      uint8_t* T = tile[buf];
-#pragma unroll
-      for (int k = 0; k < NL; ++k) *reinterpret_cast<u4v*>(T + (tr + k * (256 / TPR)) * kPitch<D> + 16 * tc) = raw[k];
-      if (threadIdx.x < kStep) top[buf][threadIdx.x] = nr.x, inv[buf][threadIdx.x] = nr.y;
-      if (r0 + kStep < r_end) load(r0 + kStep);
+    for (int r0 = begin; r0 < r_end; r0 += kStep, buf ^= 1) {
+      const uint8_t* T = tile[buf];
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (the tile's copies)
       __syncthreads();
-      const bool edge = r0 < all || r0 + kStep > r_end;
-      if (!idle) {
+      if (r0 + kStep < r_end) copy(r0 + kStep, buf ^ 1);
+      auto take = [&](auto masked) {
+        constexpr bool EDGE = decltype(masked)::value;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           f16v acc[2] = {};
+          products<QT, KS>(
+              [&](int k) {
+                return *reinterpret_cast<const u4v*>(T + (32 * s + l) * 2 * D + 16 * (channel<true>(k, hl) / 8 ^ (l & SW)));
+              }, K, acc);
 #pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            const u4v a = *reinterpret_cast<const u4v*>(T + (32 * s + l) * kPitch<D> + 2 * channel<true>(k, hl));
+          for (int i = 0; i < 16; i += 2) {
+            const f4 n2 = *reinterpret_cast<const f4*>(&norms[buf][32 * s + prow(i, hl)]);
+            const int row = r0 + 32 * s + prow(i, hl);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) acc[c] = mfma32<QT>(a, K[c][k], acc[c]);
-          }
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const f4 mm = *reinterpret_cast<const f4*>(&top[buf][32 * s + prow(i, hl)]);
-            const f4 li = *reinterpret_cast<const f4*>(&inv[buf][32 * s + prow(i, hl)]);
-            if (!edge) {
-#pragma unroll
-              for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sum[c] = fmaf(exp2_(fmaf(acc[c][i + j], f[c], -mm[j])), li[j], sum[c]);
-            } else {
-              const int row = r0 + 32 * s + prow(i, hl);
-#pragma unroll
-              for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const float e = exp2_(fmaf(acc[c][i + j], f[c], -mm[j])) * li[j];
-                  sum[c] += row + j >= first[c] && row + j < r_end ? e : 0.0f;
+              for (int j = 0; j < 2; ++j) {
+                float x = fmaf(acc[c][i + j], f[c], -n2[2 * j]), li = n2[2 * j + 1];
+                if constexpr (EDGE) {
+                  const bool is = (row + j >= first[c]) & (row + j < r_end);
+                  x = is ? x : -kInf, li = is ? li : 0.0f;
                 }
-            }
+                sum[c] = fmaf(exp2_(x), li, sum[c]);
+              }
           }
+        }
+      };
+      if (r0 + kStep > some) {
+        if (__builtin_expect(r0 < all || r0 + kStep > r_end, 0)) {
+          asm volatile("");
+          take(std::true_type{});
+        } else {
+          take(std::false_type{});
         }
       }
     }
@@ -635,7 +686,7 @@ extern "C" int kvt_block_weigh(const void* q, int64_t sq_n, int64_t sq_h, int q_
   const int64_t items = (int64_t)n_q * gs / kTileRows + n;
   const int64_t most = 1 << 24;                                     // (2^32 threads of a launch)
   if ((cu_q ? items : (int64_t)n) * H * splits >= most || (int64_t)n * H * row_splits * pos_splits >= most ||
-      (int64_t)n_q * gs >= most * 16 || H > 65535)
+      (int64_t)n_q * gs >= most * 8 || H > 65535)
     return KVT_ERANGE;
   const Space s = space(n, n_q, H, gs, cap, cu_q != nullptr, splits, row_splits);
   if (s.scores + s.part + s.norm + s.sums > work_floats) return KVT_EINVAL;
@@ -650,7 +701,7 @@ extern "C" int kvt_block_weigh(const void* q, int64_t sq_n, int64_t sq_h, int q_
   P.scale_log2 = scale * kLog2e;
   P.n = n, P.n_rows = n_rows, P.n_q = n_q, P.H = H, P.gs = gs, P.n_blocks = n_blocks, P.max_blocks = max_blocks;
   P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6;
-  P.per_gs = (uint32_t)((((uint64_t)1 << 32) + gs - 1) / gs);
+  P.per_gs = (uint32_t)((((uint64_t)1 << 31) + gs - 1) / gs);
   P.splits = splits, P.row_splits = row_splits, P.pos_splits = pos_splits;
   hipStream_t st = (hipStream_t)stream;
   if (code == kE4M3) return q_type == kBF16 ? launch_d<kE4M3, kBF16>(P, D, st) : launch_d<kE4M3, kF16>(P, D, st);

@@ -34,7 +34,7 @@ from .block_kv import BLOCKS, CODE, FREE_OVER, _grown, _i32, _pool, _rows16, _st
 # every workgroup of the sums reads; us per call with 512 / 1,024 / 2,048 / 4,096: 32 requests x 2 heads, D 256, up to 16,384
 # positions 49 / 43 / 45 / 42, int8 64 x 8, D 128, up to 8,191 133 / 96 / 84 / 77) and the sums'.
 _ROW_BLOCKS = 4096
-_WORKGROUPS = 2048
+_WORKGROUPS = 4096
 # Chunks: this many where the work allows pieces of 512 positions (rows) at least (1,024 / 2,048 / 4,096 / 8,192: a prompt
 # of 10,001, D 256, 1,071 / 890 / 867 / 890; 8 x 64 queries, D 128, 148 / 143 / 136 / 135), and as many as fit the CUs where it does not
 # (61 queries x 12 heads over 60,000 positions, D 128: 256 64.4, 512 53.5, 768 50.1, 1,024 53.2).
@@ -165,11 +165,14 @@ def kvt_block_keep(weights: torch.Tensor, kv_lens: torch.Tensor, budget: int, se
         raise ValueError("weights of no entries")
     st = _stream(weights, kv_lens, seqs, pos, held, evicted, out)
     ws = {} if workspace is None else workspace             # (held until the launch)
-    work = _grown(ws, "keep", n * H * budget, weights, torch.int32)
+    work, need = None, 0
+    if width > 32768 and width > budget:                    # (shorter ones are one workgroup's, in registers)
+        need = n * H * (6144 + 4 * min(256, -(-width // 4096)) + 12 + 2 * (budget + budget % 2))
+        work = _grown(ws, "keep", need, weights, torch.int32).data_ptr()
     sp = (0, 0) if pos is None else (pos.stride(0), pos.stride(1))
     _lib.call("kvt_block_keep", weights.data_ptr(), weights.stride(0), weights.stride(1), kv_lens.data_ptr(), n, H, rows,
               _lib.ptr(seqs), width, budget, recent, sinks, _lib.ptr(pos), *sp, _lib.ptr(held), _lib.ptr(evicted),
-              out.data_ptr(), work.data_ptr(), st)
+              out.data_ptr(), work, need, st)
     return out
 
 

@@ -15,7 +15,13 @@ using namespace kvt::blk;
 namespace {
 
 // ---------------------------------------------------------------------------------------------------------------- keep
+//
+// The budget-th largest key of a (request, KV head) by radix select (11 + 11 + 10 bits, histograms in LDS), ties to the
+// lowest entry, and the places of what moves, from ranks by ballots.  Up to kSmall entries one workgroup does it all
+// with the keys in registers, read once.  Longer ones take a launch per step, with kMostChunks workgroups a pair at most:
+// three histograms (joined by integer atomics: their order does not matter), counts per chunk, places.
 constexpr int kKeepThreads = 1024, kWaves = kKeepThreads / 64;
+constexpr int kSmall = 32768, kChunk = 4096, kMostChunks = 256, kBins = 2048;
 
 struct Keep {
   const float* weights;
@@ -25,18 +31,20 @@ struct Keep {
   const int32_t* held;
   const int32_t* evicted;
   int32_t* src;
-  int32_t* list;               // [n * H, budget]: entries that move
+  int32_t* work;               // per pair: 3 histograms, 4 counts per chunk, a Found per pass, sources, free places
   int64_t sw_r, sw_h, sp_r, sp_h, cap;
-  int n, n_rows, H, budget, recent, sinks;
+  int n, n_rows, H, budget, recent, sinks, chunks;
 };
+struct Found { int prefix, k, moves, pad; };
+KVT_DEV int64_t work_size(const Keep& P) { return 3 * kBins + 4 * P.chunks + 12 + 2 * (((int64_t)P.budget + 1) & ~1); }
 
-// Weights in the order of unsigned numbers: NaN below all, -0 as 0.
+// Weights in the order of unsigned numbers: NaN (1) below all, -0 as 0; 0 is no key.
 KVT_DEV uint32_t ordered(float w) {
   const uint32_t b = __float_as_uint(w + 0.0f);
-  return w != w ? 0u : b & 0x80000000u ? ~b : b | 0x80000000u;
+  return w != w ? 1u : b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// Sum over lanes before this one, and over all (a block of 16 wavefronts; sums: 16 entries).
+// Sum over the threads before this one, and over all (a block of 16 wavefronts; sums: 16 entries).
 KVT_DEV int before(int v, int* sums, int& all) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int x = v;
@@ -50,99 +58,307 @@ KVT_DEV int before(int v, int* sums, int& all) {
   __syncthreads();
   int b = 0;
   all = 0;
+#pragma unroll
   for (int i = 0; i < kWaves; ++i) {
-    if (i < w) b += sums[i];
-    all += sums[i];
+    const int s = sums[i];
+    b += i < w ? s : 0;
+    all += s;
   }
   return b + x - v;
 }
 
-// The keys' budget-th largest by radix select, 11 + 11 + 10 bits, each pass a histogram in LDS; ties to the lowest entry.
-// One workgroup per (request, KV head).
-__global__ __launch_bounds__(kKeepThreads) void keep_kernel(const Keep P) {
-  __shared__ int hist[2048], sums[kWaves], found[2];
-  const int h = blockIdx.x % P.H, j = blockIdx.x / P.H, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int row = P.rows ? P.rows[j] : j;
+// A (request, KV head): its entries' keys.
+struct Pair {
+  const float* w;
+  const int32_t* pos;
+  int32_t* src;
+  int64_t evicted, last;
+  int len, held, sinks;
+  KVT_DEV uint32_t key(int e) const {
+    const int64_t at = e < held ? (int64_t)pos[e] : e + evicted;
+    return e < sinks || at >= last ? 0xFFFFFFFFu : ordered(w[e]);
+  }
+};
+KVT_DEV Pair pair_of(const Keep& P, int id) {
+  const int h = id % P.H, j = id / P.H, row = P.rows ? P.rows[j] : j;
   const bool bad = row < 0 || row >= P.n_rows;
-  const int len = bad ? 0 : (int)min((int64_t)max(P.kv_lens[j], 0), P.cap);
-  int32_t* src = P.src + ((int64_t)j * P.H + h) * P.budget;
-  int32_t* list = P.list + ((int64_t)j * P.H + h) * P.budget;
-  if (len <= P.budget) {
-    for (int e = tid; e < P.budget; e += kKeepThreads) src[e] = e < len ? e : -1;
+  Pair t;
+  t.len = bad ? 0 : (int)min((int64_t)max(P.kv_lens[j], 0), P.cap);
+  t.src = P.src + ((int64_t)j * P.H + h) * P.budget;
+  const int64_t r = bad ? 0 : row;
+  t.w = P.weights + r * P.sw_r + h * P.sw_h;
+  t.pos = P.pos ? P.pos + r * P.sp_r + h * P.sp_h : nullptr;
+  t.held = P.pos ? min(max(P.held[r], 0), t.len) : 0;
+  t.evicted = P.pos ? P.evicted[r] : 0;
+  t.last = (int64_t)t.len + t.evicted - P.recent;
+  t.sinks = P.sinks;
+  return t;
+}
+
+// Where the k-th largest of a histogram's keys is: its bin and the k that is left within it.  found: two entries.
+KVT_DEV void find_bin(const int* hist, int k, int* sums, int* found, int& bin, int& left) {
+  // bins from the highest on: thread t has bins 2047 - 2 t and 2046 - 2 t
+  const int t = threadIdx.x, a = hist[kBins - 1 - 2 * t], b = hist[kBins - 2 - 2 * t];
+  int all;
+  const int above = before(a + b, sums, all);
+  if (above < k && k <= above + a) found[0] = kBins - 1 - 2 * t, found[1] = k - above;
+  else if (above + a < k && k <= above + a + b) found[0] = kBins - 2 - 2 * t, found[1] = k - above - a;
+  __syncthreads();
+  bin = found[0], left = found[1];
+}
+KVT_DEV int shift_of(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+KVT_DEV int bins_of(int pass) { return pass == 2 ? 1024 : 2048; }
+
+// One workgroup per pair of no more than 1,024 R entries: wavefront v has entries v * seg .., key i of a lane that of
+// entry v * seg + 64 i + lane.
+template <int R>
+__global__ __launch_bounds__(kKeepThreads) void keep_kernel(const Keep P) {
+  __shared__ int hist[kBins], sums[kWaves], found[2];
+  __shared__ uint16_t list[512 * R];            // (no more than half of the entries can move)
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Pair t = pair_of(P, blockIdx.x);
+  if (t.len <= P.budget) {
+    for (int e = tid; e < P.budget; e += kKeepThreads) t.src[e] = e < t.len ? e : -1;
     return;
   }
-  const float* w = P.weights + row * P.sw_r + h * P.sw_h;
-  const int32_t* pos = P.pos ? P.pos + row * P.sp_r + h * P.sp_h : nullptr;
-  const int held = pos ? min(max(P.held[row], 0), len) : 0;
-  const int64_t evicted = pos ? P.evicted[row] : 0, last = (int64_t)len + evicted - P.recent;
-  auto key = [&](int e) {
-    const int64_t at = e < held ? (int64_t)pos[e] : e + evicted;
-    return e < P.sinks || at >= last ? 0xFFFFFFFFu : ordered(w[e]);
-  };
-
+  if (t.len > 1024 * R) return;                 // (the launches behind this one)
+  const int steps = (t.len + kKeepThreads - 1) / kKeepThreads, e0 = wave * 64 * steps + lane;
+  uint32_t key[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int e = e0 + 64 * i;
+    key[i] = i < steps && e < t.len ? t.key(e) : 0u;
+  }
   uint32_t prefix = 0, mask = 0;
   int k = P.budget;
   for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    const int shift = shift_of(pass);
+    for (int i = tid; i < kBins; i += kKeepThreads) hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < 2048; i += kKeepThreads) hist[i] = 0;
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (key[i] && (key[i] & mask) == prefix) atomicAdd(&hist[(key[i] >> shift) & (bins_of(pass) - 1)], 1);
     __syncthreads();
-    for (int e = tid; e < len; e += kKeepThreads) {
-      const uint32_t u = key(e);
-      if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift) & ((1 << bits) - 1)], 1);
-    }
-    __syncthreads();
-    // bins from the highest on: thread t has bins 2047 - 2 t and 2046 - 2 t
-    const int a = hist[2047 - 2 * tid], b = hist[2046 - 2 * tid];
-    int all;
-    const int above = before(a + b, sums, all);
-    if (above < k && k <= above + a) found[0] = 2047 - 2 * tid, found[1] = k - above;
-    else if (above + a < k && k <= above + a + b) found[0] = 2046 - 2 * tid, found[1] = k - above - a;
-    __syncthreads();
-    prefix |= (uint32_t)found[0] << shift;
-    mask |= (uint32_t)((1 << bits) - 1) << shift;
-    k = found[1];
+    int bin;
+    find_bin(hist, k, sums, found, bin, k);
+    prefix |= (uint32_t)bin << shift;
+    mask |= (uint32_t)(bins_of(pass) - 1) << shift;
   }
 
-  // wavefront v has entries v * seg ..: the k first ties stay; ranks by ballots
-  const int seg = (((len + kWaves - 1) / kWaves) + 63) & ~63;
-  const int e0 = min(wave * seg, len), e1 = min(e0 + seg, len);
   const uint64_t lower = ((uint64_t)1 << lane) - 1;
   int count = 0, all;
-  for (int e = e0 + lane; e < e1; e += 64) count += key(e) == prefix;
-  int ties = before(count, sums, all);
-  ties = __shfl(ties, 0, 64);
-  auto walk = [&](auto f) {                 // f(entry, whether it stays), every lane of the wavefront in step
-    int t = ties;
+#pragma unroll
+  for (int i = 0; i < R; ++i) count += __popcll(__ballot(key[i] == prefix));
+  int ties = __shfl(before(lane == 0 ? count : 0, sums, all), 0, 64);
+  uint32_t stays = 0;                           // bit i: entry of key i stays
+  int moves = 0, frees = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int e = e0 + 64 * i;
+    if (i < steps) {
+      const bool tie = key[i] == prefix;
+      const uint64_t b = __ballot(tie);
+      const bool is = key[i] > prefix || (tie && ties + __popcll(b & lower) < k);
+      ties += __popcll(b);
+      stays |= (uint32_t)is << i;
+      moves += __popcll(__ballot(is && e >= P.budget));
+      frees += __popcll(__ballot(!is && e < P.budget));
+    }
+  }
+  // (both counts in one scan: neither leaves 16 bits)
+  int at = __shfl(before(lane == 0 ? moves << 16 | frees : 0, sums, all), 0, 64), m = at >> 16, f = at & 0xFFFF;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int e = e0 + 64 * i;
+    if (i < steps) {
+      const bool is = (stays >> i & 1) && e >= P.budget;
+      const uint64_t b = __ballot(is);
+      if (is) list[m + __popcll(b & lower)] = (uint16_t)e;
+      m += __popcll(b);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int e = e0 + 64 * i;
+    if (i < steps) {
+      const bool free = !(stays >> i & 1) && e < P.budget;
+      const uint64_t b = __ballot(free);
+      if (e < P.budget) t.src[e] = free ? (int)list[f + __popcll(b & lower)] : e;
+      f += __popcll(b);
+    }
+  }
+}
+
+// Pairs of more than kSmall entries.  Chunk c of a pair has entries c * per .. (a multiple of 1,024).
+struct Long {
+  int32_t* hist;
+  int32_t* counts;             // of a chunk: keys above the threshold below the budget and behind it, ties below and behind
+  Found* found;
+  int32_t* list;
+  int32_t* places;
+  int begin, end;
+};
+KVT_DEV bool long_of(const Keep& P, int id, const Pair& t, int c, Long& L) {
+  if (t.len <= P.budget || t.len <= kSmall) return false;
+  int32_t* w = P.work + id * work_size(P);
+  L.hist = w, L.counts = w + 3 * kBins, L.found = (Found*)(L.counts + 4 * P.chunks);
+  L.list = (int32_t*)(L.found + 3), L.places = L.list + P.budget;
+  const int per = ((t.len + P.chunks - 1) / P.chunks + 1023) & ~1023;
+  L.begin = (int)min((int64_t)c * per, (int64_t)t.len), L.end = (int)min((int64_t)L.begin + per, (int64_t)t.len);
+  return true;
+}
+
+__global__ __launch_bounds__(256) void keep_clear_kernel(const Keep P) {
+  int32_t* w = P.work + blockIdx.x * work_size(P);
+  for (int i = threadIdx.x; i < 3 * kBins; i += 256) w[i] = 0;
+}
+
+// What pass `pass` found so far: read, or for the pass before formed from its histogram and written (by chunk 0).
+KVT_DEV Found found_before(const Keep& P, const Long& L, int pass, int c, int* sums, int* found) {
+  Found f = {0, P.budget, 0, 0};
+  if (pass == 0) return f;
+  if (pass > 1) f = L.found[pass - 2];
+  int bin;
+  find_bin(L.hist + (pass - 1) * kBins, f.k, sums, found, bin, f.k);
+  f.prefix |= (int)((uint32_t)bin << shift_of(pass - 1));
+  if (c == 0 && threadIdx.x == 0) L.found[pass - 1] = f;
+  return f;
+}
+
+__global__ __launch_bounds__(kKeepThreads) void keep_hist_kernel(const Keep P, int pass) {
+  __shared__ int hist[kBins], sums[kWaves], found[2];
+  const int c = blockIdx.x % P.chunks, id = blockIdx.x / P.chunks, tid = threadIdx.x;
+  const Pair t = pair_of(P, id);
+  Long L;
+  if (!long_of(P, id, t, c, L)) return;
+  const Found f = found_before(P, L, pass, c, sums, found);
+  if (L.begin >= L.end) return;
+  const uint32_t prefix = (uint32_t)f.prefix, mask = pass == 0 ? 0u : ~0u << shift_of(pass - 1);
+  for (int i = tid; i < kBins; i += kKeepThreads) hist[i] = 0;
+  __syncthreads();
+#pragma unroll 4
+  for (int e = L.begin + tid; e < L.end; e += kKeepThreads) {
+    const uint32_t u = t.key(e);
+    if ((u & mask) == prefix) atomicAdd(&hist[(u >> shift_of(pass)) & (bins_of(pass) - 1)], 1);
+  }
+  __syncthreads();
+  for (int i = tid; i < kBins; i += kKeepThreads)
+    if (hist[i]) atomicAdd(&L.hist[pass * kBins + i], hist[i]);
+}
+
+__global__ __launch_bounds__(kKeepThreads) void keep_count_kernel(const Keep P) {
+  __shared__ int sums[kWaves], found[2], counts[4];
+  const int c = blockIdx.x % P.chunks, id = blockIdx.x / P.chunks, tid = threadIdx.x;
+  const Pair t = pair_of(P, id);
+  Long L;
+  if (!long_of(P, id, t, c, L)) return;
+  const uint32_t T = (uint32_t)found_before(P, L, 3, c, sums, found).prefix;
+  if (tid < 4) counts[tid] = 0;
+  __syncthreads();
+  int n[4] = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int e = L.begin + tid; e < L.end; e += kKeepThreads) {
+    const uint32_t u = t.key(e);
+    const bool behind = e >= P.budget;
+    n[0] += u > T && !behind, n[1] += u > T && behind, n[2] += u == T && !behind, n[3] += u == T && behind;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) n[i] += __shfl_xor(n[i], o, 64);
+    if ((tid & 63) == 0) atomicAdd(&counts[i], n[i]);
+  }
+  __syncthreads();
+  if (tid < 4) L.counts[4 * c + tid] = counts[tid];
+}
+
+// Entries that stay below the budget, and the lists of those that move and of the places that are free.
+__global__ __launch_bounds__(kKeepThreads) void keep_list_kernel(const Keep P) {
+  __shared__ int sums[kWaves], start[3];
+  const int c = blockIdx.x % P.chunks, id = blockIdx.x / P.chunks, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Pair t = pair_of(P, id);
+  Long L;
+  if (!long_of(P, id, t, c, L)) return;
+  const uint32_t T = (uint32_t)L.found[2].prefix;
+  const int k = L.found[2].k;
+  if (wave == 0) {
+    // ties, moves and free places before the chunk: the ties that stay follow from the number of ties before
+    int ties = 0, moves = 0, frees = 0, total = 0;
+    for (int base = 0; base < P.chunks; base += 64) {
+      const int i = base + lane;
+      const int4 n = i < P.chunks ? *reinterpret_cast<const int4*>(L.counts + 4 * i) : make_int4(0, 0, 0, 0);
+      int x = n.z + n.w;                                     // (ties are taken below the budget first: entries in order)
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(x, o, 64);
+        if (lane >= o) x += u;
+      }
+      const int first = ties + x - n.z - n.w;
+      const int low = min(max(k - first, 0), n.z), high = min(max(k - first - n.z, 0), n.w);
+      const int per = ((t.len + P.chunks - 1) / P.chunks + 1023) & ~1023;
+      const int64_t b = (int64_t)i * per;
+      const int below = i < P.chunks ? (int)(min(max((int64_t)P.budget - b, (int64_t)0), min((int64_t)per, max((int64_t)t.len - b, (int64_t)0)))) : 0;
+      int mv = n.y + high, fr = below - n.x - low;
+      total += mv;
+      if (i >= c) mv = fr = 0;
+      int tb = i < c ? n.z + n.w : 0;
+#pragma unroll
+      for (int o = 32; o; o >>= 1) mv += __shfl_xor(mv, o, 64), fr += __shfl_xor(fr, o, 64), tb += __shfl_xor(tb, o, 64);
+      moves += mv, frees += fr;
+      if (base <= c && c < base + 64 && lane == 0) start[0] = ties + tb;
+      ties += __shfl(x, 63, 64);
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o, 64);
+    if (lane == 0) {
+      start[1] = moves, start[2] = frees;
+      if (c == 0) L.found[2].moves = total;
+    }
+  }
+  __syncthreads();
+  if (L.begin >= L.end) return;
+  const int seg = ((L.end - L.begin + kKeepThreads - 1) / kKeepThreads) * 64;
+  const int e0 = min(L.begin + wave * seg, L.end), e1 = min(e0 + seg, L.end);
+  const uint64_t lower = ((uint64_t)1 << lane) - 1;
+  int count = 0, all;
+  for (int e = e0 + lane; e < e1; e += 64) count += t.key(e) == T;
+  int ties = start[0] + __shfl(before(count, sums, all), 0, 64);
+  auto walk = [&](auto f) {                     // f(entry, whether it is one, whether it stays), the wavefront in step
+    int n = ties;
     for (int base = e0; base < e1; base += 64) {
       const int e = base + lane;
-      const uint32_t u = e < e1 ? key(e) : 0u;
-      const bool tie = e < e1 && u == prefix;
+      const uint32_t u = e < e1 ? t.key(e) : 0u;
+      const bool tie = e < e1 && u == T;
       const uint64_t b = __ballot(tie);
-      const bool stays = e < e1 && (u > prefix || (tie && t + __popcll(b & lower) < k));
-      t += __popcll(b);
-      f(e, stays);
+      f(e, e < e1, e < e1 && (u > T || (tie && n + __popcll(b & lower) < k)));
+      n += __popcll(b);
     }
   };
   int moves = 0, frees = 0;
-  walk([&](int e, bool stays) {
+  walk([&](int e, bool is, bool stays) {
     moves += __popcll(__ballot(stays && e >= P.budget));
-    frees += __popcll(__ballot(!stays && e < P.budget && e < e1));
+    frees += __popcll(__ballot(is && !stays && e < P.budget));
   });
-  int m = __shfl(before(lane == 0 ? moves : 0, sums, all), 0, 64);
-  int f = __shfl(before(lane == 0 ? frees : 0, sums, all), 0, 64);
-  walk([&](int e, bool stays) {
-    const uint64_t b = __ballot(stays && e >= P.budget);
-    if (stays && e >= P.budget) list[m + __popcll(b & lower)] = e;
-    m += __popcll(b);
+  int m = start[1] + __shfl(before(lane == 0 ? moves : 0, sums, all), 0, 64);
+  int f = start[2] + __shfl(before(lane == 0 ? frees : 0, sums, all), 0, 64);
+  walk([&](int e, bool is, bool stays) {
+    const bool move = stays && e >= P.budget, free = is && !stays && e < P.budget;
+    const uint64_t b = __ballot(move), g = __ballot(free);
+    if (move) L.list[m + __popcll(b & lower)] = e;
+    if (free) L.places[f + __popcll(g & lower)] = e;
+    if (is && stays && e < P.budget) t.src[e] = e;
+    m += __popcll(b), f += __popcll(g);
   });
-  __syncthreads();
-  walk([&](int e, bool stays) {
-    const bool free = !stays && e < P.budget && e < e1;
-    const uint64_t b = __ballot(free);
-    if (e < P.budget && e < e1) src[e] = free ? list[f + __popcll(b & lower)] : e;
-    f += __popcll(b);
-  });
+}
+
+__global__ __launch_bounds__(256) void keep_place_kernel(const Keep P, int blocks) {
+  const int id = blockIdx.x / blocks;
+  const Pair t = pair_of(P, id);
+  Long L;
+  if (!long_of(P, id, t, 0, L)) return;
+  const int moves = L.found[2].moves;
+  for (int i = (blockIdx.x % blocks) * 256 + threadIdx.x; i < moves; i += blocks * 256) t.src[L.places[i]] = L.list[i];
 }
 
 // --------------------------------------------------------------------------------------------------------------- evict
@@ -390,17 +606,38 @@ __global__ __launch_bounds__(1024) void trim_kernel(const Trim P) {
 extern "C" int kvt_block_keep(const void* weights, int64_t sw_r, int64_t sw_h, const void* kv_lens, int n, int H,
                               int n_rows, const void* rows, int64_t cap, int budget, int recent, int sinks, const void* pos,
                               int64_t sp_r, int64_t sp_h, const void* held, const void* evicted, void* src, void* work,
-                              void* stream) {
+                              int64_t work_ints, void* stream) {
   if (n < 1 || H < 1 || n_rows < 1 || cap < 1 || budget < 1 || recent < 0 || sinks < 0 || (!rows && n_rows < n))
     return KVT_EINVAL;
   if ((int64_t)recent + sinks > budget || !pos != !held || !pos != !evicted) return KVT_EINVAL;
-  if (cap > ((int64_t)1 << 31) - 8192 || (int64_t)n * H >= 1 << 22) return KVT_ERANGE;
+  const int64_t pairs = (int64_t)n * H;
+  const int chunks = (int)(cap < (int64_t)kMostChunks * kChunk ? (cap + kChunk - 1) / kChunk : kMostChunks);
+  if (cap > ((int64_t)1 << 31) - 8192 || pairs >= 1 << 22 || (cap > kSmall && pairs * chunks >= 1 << 22)) return KVT_ERANGE;
   Keep P;
   P.weights = (const float*)weights, P.kv_lens = (const int32_t*)kv_lens, P.rows = (const int32_t*)rows;
   P.pos = (const int32_t*)pos, P.held = (const int32_t*)held, P.evicted = (const int32_t*)evicted;
-  P.src = (int32_t*)src, P.list = (int32_t*)work, P.sw_r = sw_r, P.sw_h = sw_h, P.sp_r = sp_r, P.sp_h = sp_h, P.cap = cap;
-  P.n = n, P.n_rows = n_rows, P.H = H, P.budget = budget, P.recent = recent, P.sinks = sinks;
-  keep_kernel<<<n * H, kKeepThreads, 0, (hipStream_t)stream>>>(P);
+  P.src = (int32_t*)src, P.work = (int32_t*)work, P.sw_r = sw_r, P.sw_h = sw_h, P.sp_r = sp_r, P.sp_h = sp_h, P.cap = cap;
+  P.n = n, P.n_rows = n_rows, P.H = H, P.budget = budget, P.recent = recent, P.sinks = sinks, P.chunks = chunks;
+  const bool many = cap > kSmall && cap > budget;
+  if (many && (((uintptr_t)work & 15) || work_ints < pairs * (3 * kBins + 4 * chunks + 12 + 2 * (((int64_t)budget + 1) & ~1))))
+    return KVT_EINVAL;
+  hipStream_t st = (hipStream_t)stream;
+  if (cap <= 8192) keep_kernel<8><<<(int)pairs, kKeepThreads, 0, st>>>(P);
+  else keep_kernel<kSmall / 1024><<<(int)pairs, kKeepThreads, 0, st>>>(P);
+  KVT_CHECK_LAUNCH();
+  if (!many) return KVT_OK;
+  const int grid = (int)pairs * chunks, blocks = min((budget + 255) / 256, 64);
+  keep_clear_kernel<<<(int)pairs, 256, 0, st>>>(P);
+  KVT_CHECK_LAUNCH();
+  for (int pass = 0; pass < 3; ++pass) {
+    keep_hist_kernel<<<grid, kKeepThreads, 0, st>>>(P, pass);
+    KVT_CHECK_LAUNCH();
+  }
+  keep_count_kernel<<<grid, kKeepThreads, 0, st>>>(P);
+  KVT_CHECK_LAUNCH();
+  keep_list_kernel<<<grid, kKeepThreads, 0, st>>>(P);
+  KVT_CHECK_LAUNCH();
+  keep_place_kernel<<<(int)pairs * blocks, 256, 0, st>>>(P, blocks);
   KVT_CHECK_LAUNCH();
   return KVT_OK;
 }

@@ -233,6 +233,18 @@ __global__ __launch_bounds__(256) void weigh_columns_kernel(const Weigh P) {
   if ((int64_t)split * 1024 >= t.len) return;
   const int64_t pair_id = (int64_t)r * P.H + h, cap = (int64_t)P.max_blocks << P.log2b;
   const int per = per_split(t.len, P.splits), used = (t.len + per - 1) / per;
+  const float* scores = P.scores + pair_id * P.gs * cap;
+  // four rows' scores of four positions, and the positions' block
+  f4 x[4];
+  int id = -1;
+  auto load = [&](int p, int g) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const f4*>(scores + min(g + k, P.gs - 1) * cap + p);
+  };
+  int64_t base = (int64_t)split * 1024;
+  const int first = min((int)base + 4 * (int)threadIdx.x, (t.len - 1) & ~3);
+  load(first, 0);                                 // (asked for before the parts)
+  id = P.table[(int64_t)t.trow * P.stride + (first >> P.log2b)];
   {
     const int l = threadIdx.x & 15, c = threadIdx.x >> 4;
     float m = -kInf, s = 0.0f;
@@ -252,16 +264,16 @@ __global__ __launch_bounds__(256) void weigh_columns_kernel(const Weigh P) {
     norm[threadIdx.x] = (int)threadIdx.x < P.gs ? make_float2(a.x, 1.0f / a.y) : make_float2(kInf, 0.0f);
   }
   __syncthreads();
-  for (int64_t base = (int64_t)split * 1024; base < t.len; base += (int64_t)P.pos_splits * 1024) {
+  for (bool again = false; base < t.len; base += (int64_t)P.pos_splits * 1024, again = true) {
     const int p = (int)base + 4 * threadIdx.x;
     if (p >= t.len) break;
-    const int id = P.table[(int64_t)t.trow * P.stride + (p >> P.log2b)];      // (four positions of one block)
-    const float* score = P.scores + pair_id * P.gs * cap + p;
+    if (again) {
+      load(p, 0);
+      id = P.table[(int64_t)t.trow * P.stride + (p >> P.log2b)];      // (four positions of one block)
+    }
     float sum[4] = {0, 0, 0, 0};
     for (int g = 0; g < P.gs; g += 4) {
-      f4 x[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const f4*>(score + min(g + k, P.gs - 1) * cap);
+      if (g) load(p, g);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float2 a = norm[g + k];

@@ -145,9 +145,10 @@ def test_c_entries_refuse(kvt_pkg):
     assert weigh(max_blocks=2 ** 28, stride=2 ** 28) == -3
     assert weigh(ps=1 << 24) == -3
 
-    def keep(n=1, H=1, rows=1, cap=64, budget=16, recent=0, sinks=0, pos=None, held=None):
-        return lib.kvt_block_keep(N, 0, 0, N, n, H, rows, N, cap, budget, recent, sinks, pos, 0, 0, held, N, N, N, N)
-    for bad in (dict(n=0), dict(n=2), dict(cap=0), dict(budget=0), dict(recent=17), dict(sinks=-1), dict(pos=16), dict(held=16)):
+    def keep(n=1, H=1, rows=1, cap=64, budget=16, recent=0, sinks=0, pos=None, held=None, ints=0, work=None):
+        return lib.kvt_block_keep(N, 0, 0, N, n, H, rows, N, cap, budget, recent, sinks, pos, 0, 0, held, N, N, work, ints, N)
+    for bad in (dict(n=0), dict(n=2), dict(cap=0), dict(budget=0), dict(recent=17), dict(sinks=-1), dict(pos=16), dict(held=16),
+                dict(cap=40_000, ints=6227), dict(cap=40_000, work=8, ints=10 ** 6)):
         assert keep(**bad) == -1, bad
     assert keep(cap=2 ** 31) == -3 and keep(n=1 << 22, rows=1 << 22) == -3
 

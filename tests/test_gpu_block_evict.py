@@ -210,6 +210,8 @@ KEEP = [
     ([2047, 2049, 1025], 1024, 0, 0, 2),
     ([5000], 4096, 1000, 4, 3),
     ([40_000, 33_000], 16_384, 300, 4, 1),
+    ([70_001, 32_769, 9000, 300], 301, 100, 4, 2),
+    ([1_100_000], 5001, 0, 0, 1),
 ]
 
 

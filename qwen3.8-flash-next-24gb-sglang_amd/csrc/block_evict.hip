@@ -72,12 +72,15 @@ struct Pair {
   const float* w;
   const int32_t* pos;
   int32_t* src;
-  int64_t evicted, last;
+  uint32_t evicted, last;      // (positions are below 2^32)
   int len, held, sinks;
-  KVT_DEV uint32_t key(int e) const {
-    const int64_t at = e < held ? (int64_t)pos[e] : e + evicted;
-    return e < sinks || at >= last ? 0xFFFFFFFFu : ordered(w[e]);
+  // of an entry's weight and, if it is one of those held, position (both loads without a branch around them)
+  KVT_DEV int place(int e) const { return pos ? pos[e] : 0; }
+  KVT_DEV uint32_t key(int e, float weight, int place) const {
+    const uint32_t at = e < held ? (uint32_t)place : e + evicted;
+    return e < sinks || at >= last ? 0xFFFFFFFFu : ordered(weight);
   }
+  KVT_DEV uint32_t key(int e) const { return key(e, w[e], place(e)); }
 };
 KVT_DEV Pair pair_of(const Keep& P, int id) {
   const int h = id % P.H, j = id / P.H, row = P.rows ? P.rows[j] : j;
@@ -89,8 +92,8 @@ KVT_DEV Pair pair_of(const Keep& P, int id) {
   t.w = P.weights + r * P.sw_r + h * P.sw_h;
   t.pos = P.pos ? P.pos + r * P.sp_r + h * P.sp_h : nullptr;
   t.held = P.pos ? min(max(P.held[r], 0), t.len) : 0;
-  t.evicted = P.pos ? P.evicted[r] : 0;
-  t.last = (int64_t)t.len + t.evicted - P.recent;
+  t.evicted = P.pos ? max(P.evicted[r], 0) : 0;
+  t.last = (uint32_t)max((int64_t)t.len + t.evicted - P.recent, (int64_t)0);
   t.sinks = P.sinks;
   return t;
 }
@@ -109,64 +112,123 @@ KVT_DEV void find_bin(const int* hist, int k, int* sums, int* found, int& bin, i
 KVT_DEV int shift_of(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
 KVT_DEV int bins_of(int pass) { return pass == 2 ? 1024 : 2048; }
 
-// One workgroup per pair of no more than 1,024 R entries: wavefront v has entries v * seg .., key i of a lane that of
-// entry v * seg + 64 i + lane.
-template <int R>
-__global__ __launch_bounds__(kKeepThreads) void keep_kernel(const Keep P) {
-  __shared__ int hist[kBins], sums[kWaves], found[2];
-  __shared__ uint16_t list[512 * R];            // (no more than half of the entries can move)
+// The same by every wavefront for itself: lane l has bins 2047 - 32 l and the 31 below.  Four words lie between those of
+// two lanes (padded), so that their 16-byte reads are spread over the banks.
+constexpr int kPadded = kBins + kBins / 8;
+KVT_DEV int padded(int bin) { return bin + (bin >> 5) * 4; }
+KVT_DEV int wave_before(int v) {                  // sum over the lanes up to this one
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(v, o, 64);
+    v += lane >= o ? u : 0;
+  }
+  return v;
+}
+KVT_DEV void find_bin_wave(const int* hist, int k, int& bin, int& left) {
+  const int lane = threadIdx.x & 63;
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int4 v = *reinterpret_cast<const int4*>(hist + 36 * (63 - lane) + 4 * i);
+    sum += v.x + v.y + v.z + v.w;
+  }
+  int x = wave_before(sum);
+  const int from = __ffsll((unsigned long long)__ballot(x - sum < k && k <= x)) - 1;
+  k -= __builtin_amdgcn_readlane(x - sum, from);
+  const int n = lane < 32 ? hist[36 * (63 - from) + 31 - lane] : 0;       // its bins, from the highest on
+  x = wave_before(n);
+  const int at = __ffsll((unsigned long long)__ballot(x - n < k && k <= x)) - 1;
+  bin = kBins - 1 - 32 * from - at, left = k - __builtin_amdgcn_readlane(x - n, at);
+}
+
+// One workgroup of T threads per pair of no more than T R entries: wavefront v has entries v * seg .., key i of a lane that
+// of entry v * seg + 64 i + lane.  Latency and its instructions bound it: 512 x 4,160
+// entries, keys re-read from memory by 1,024 threads 39 us, in registers 26, every wavefront finding a histogram's bin
+// for itself instead of three barriers more, 512 threads, 16 (256 threads 20, 1,024 19).
+template <int T, int R>
+__global__ __launch_bounds__(T) void keep_kernel(const Keep P) {
+  __shared__ __attribute__((aligned(16))) int hist[3][kPadded];
+  __shared__ int sums[2][T / 64];
+  __shared__ uint16_t list[T * R / 2];          // (no more than half of the entries can move)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Pair t = pair_of(P, blockIdx.x);
   if (t.len <= P.budget) {
-    for (int e = tid; e < P.budget; e += kKeepThreads) t.src[e] = e < t.len ? e : -1;
+    for (int e = tid; e < P.budget; e += T) t.src[e] = e < t.len ? e : -1;
     return;
   }
-  if (t.len > 1024 * R) return;                 // (the launches behind this one)
-  const int steps = (t.len + kKeepThreads - 1) / kKeepThreads, e0 = wave * 64 * steps + lane;
+  if (t.len > T * R) return;                    // (the launches behind this one)
+  const int steps = (t.len + T - 1) / T, e0 = wave * 64 * steps + lane;
   uint32_t key[R];
+  int place[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (i < steps) key[i] = __float_as_uint(t.w[min(e0 + 64 * i, t.len - 1)]);
+  if (t.held) {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (i < steps) place[i] = t.pos[min(e0 + 64 * i, t.len - 1)];
+  }
+  for (int i = tid; i < 3 * kPadded; i += T) hist[0][i] = 0;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int e = e0 + 64 * i;
-    key[i] = i < steps && e < t.len ? t.key(e) : 0u;
+    key[i] = i < steps && e < t.len ? t.key(e, __uint_as_float(key[i]), place[i]) : 0u;
   }
+  __syncthreads();
   uint32_t prefix = 0, mask = 0;
   int k = P.budget;
+#pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = shift_of(pass);
-    for (int i = tid; i < kBins; i += kKeepThreads) hist[i] = 0;
-    __syncthreads();
 #pragma unroll
     for (int i = 0; i < R; ++i)
-      if (key[i] && (key[i] & mask) == prefix) atomicAdd(&hist[(key[i] >> shift) & (bins_of(pass) - 1)], 1);
+      if (key[i] && (key[i] & mask) == prefix) atomicAdd(&hist[pass][padded((key[i] >> shift) & (bins_of(pass) - 1))], 1);
     __syncthreads();
     int bin;
-    find_bin(hist, k, sums, found, bin, k);
+    find_bin_wave(hist[pass], k, bin, k);
     prefix |= (uint32_t)bin << shift;
     mask |= (uint32_t)(bins_of(pass) - 1) << shift;
   }
 
-  const uint64_t lower = ((uint64_t)1 << lane) - 1;
-  int count = 0, all;
+  // what the wavefronts before this one have
+  auto earlier = [&](int v, int* s) {
+    if (lane == 0) s[wave] = v;
+    __syncthreads();
+    int b = 0;
 #pragma unroll
-  for (int i = 0; i < R; ++i) count += __popcll(__ballot(key[i] == prefix));
-  int ties = __shfl(before(lane == 0 ? count : 0, sums, all), 0, 64);
+    for (int i = 0; i < T / 64; ++i) b += i < wave ? s[i] : 0;
+    return b;
+  };
+  const uint64_t lower = ((uint64_t)1 << lane) - 1;
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (i < steps) count += __popcll(__ballot(key[i] == prefix));
+  int ties = earlier(count, sums[0]), all_ties = 0;
+#pragma unroll
+  for (int i = 0; i < T / 64; ++i) all_ties += sums[0][i];
   uint32_t stays = 0;                           // bit i: entry of key i stays
   int moves = 0, frees = 0;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int e = e0 + 64 * i;
     if (i < steps) {
-      const bool tie = key[i] == prefix;
-      const uint64_t b = __ballot(tie);
-      const bool is = key[i] > prefix || (tie && ties + __popcll(b & lower) < k);
-      ties += __popcll(b);
+      bool is = key[i] >= prefix;
+      if (all_ties > k) {                       // (not all of the ties stay)
+        const bool tie = key[i] == prefix;
+        const uint64_t b = __ballot(tie);
+        is = key[i] > prefix || (tie && ties + __popcll(b & lower) < k);
+        ties += __popcll(b);
+      }
       stays |= (uint32_t)is << i;
       moves += __popcll(__ballot(is && e >= P.budget));
       frees += __popcll(__ballot(!is && e < P.budget));
     }
   }
-  // (both counts in one scan: neither leaves 16 bits)
-  int at = __shfl(before(lane == 0 ? moves << 16 | frees : 0, sums, all), 0, 64), m = at >> 16, f = at & 0xFFFF;
+  // (both counts in one sum: neither leaves 16 bits)
+  const int at = earlier(moves << 16 | frees, sums[1]);
+  int m = at >> 16, f = at & 0xFFFF;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int e = e0 + 64 * i;
@@ -622,8 +684,8 @@ extern "C" int kvt_block_keep(const void* weights, int64_t sw_r, int64_t sw_h, c
   if (many && (((uintptr_t)work & 15) || work_ints < pairs * (3 * kBins + 4 * chunks + 12 + 2 * (((int64_t)budget + 1) & ~1))))
     return KVT_EINVAL;
   hipStream_t st = (hipStream_t)stream;
-  if (cap <= 8192) keep_kernel<8><<<(int)pairs, kKeepThreads, 0, st>>>(P);
-  else keep_kernel<kSmall / 1024><<<(int)pairs, kKeepThreads, 0, st>>>(P);
+  if (cap <= 8192) keep_kernel<512, 16><<<(int)pairs, 512, 0, st>>>(P);
+  else keep_kernel<1024, kSmall / 1024><<<(int)pairs, 1024, 0, st>>>(P);
   KVT_CHECK_LAUNCH();
   if (!many) return KVT_OK;
   const int grid = (int)pairs * chunks, blocks = min((budget + 255) / 256, 64);

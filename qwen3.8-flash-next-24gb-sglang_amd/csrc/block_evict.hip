@@ -439,48 +439,95 @@ struct Evict {
   int n, n_rows, H, n_blocks, max_blocks, log2b, budget;
 };
 
-// The largest finite magnitude of four codes.
+// The largest finite magnitude of sixteen codes, two bytes of a dword at a time.
+typedef int16_t s2 __attribute__((ext_vector_type(2)));
 template <int CODE>
-KVT_DEV float magnitude(uint32_t w) {
+KVT_DEV float magnitude(u4v v) {
   if constexpr (CODE == kE4M3) {
-    uint32_t m = w & 0x7F7F7F7Fu;
-    m &= ~((((m + 0x01010101u) & 0x80808080u) >> 7) * 0xFFu);          // (NaN codes count as 0)
-    const uint32_t a = max(m & 0xFFu, m >> 8 & 0xFFu), b = max(m >> 16 & 0xFFu, m >> 24);
-    return __builtin_amdgcn_cvt_f32_fp8((int)max(a, b), 0);            // (magnitudes are ordered as their codes are)
+    // (magnitudes are ordered as their codes are, NaN, 0x7F, above all)
+    s2 lo = {0, 0}, hi = {0, 0};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      lo = __builtin_elementwise_max(lo, __builtin_bit_cast(s2, v[c] & 0x007F007Fu));
+      hi = __builtin_elementwise_max(hi, __builtin_bit_cast(s2, v[c] & 0x7F007F00u));
+    }
+    const auto low = __builtin_bit_cast(uint32_t, lo), high = __builtin_bit_cast(uint32_t, hi) >> 8;
+    uint32_t top = max(max(low & 0xFFFFu, low >> 16), max(high & 0xFFu, high >> 16));
+    if (top == 0x7Fu) {                       // (NaN codes count as 0)
+      top = 0;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        const uint32_t x = v[c >> 2] >> (8 * (c & 3)) & 0x7Fu;
+        top = max(top, x == 0x7Fu ? 0u : x);
+      }
+    }
+    return __builtin_amdgcn_cvt_f32_fp8((int)top, 0);
   } else {
-    float x[4];
-    unpack4<CODE>(w, x);
-    return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+    s2 up = {0, 0}, down = {0, 0};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t w = v[c];                // (a bit cast of an element itself takes the first one)
+      const s2 even = __builtin_bit_cast(s2, w << 8) >> 8, odd = __builtin_bit_cast(s2, w) >> 8;
+      up = __builtin_elementwise_max(__builtin_elementwise_max(up, even), odd);
+      down = __builtin_elementwise_min(__builtin_elementwise_min(down, even), odd);
+    }
+    return (float)max(max((int)up.x, (int)up.y), -min((int)down.x, (int)down.y));
   }
 }
 
 // One workgroup per (request, KV head, block below the budget).  A block of which every row stays is left as it is.
 // Another one's scale is the smallest power of two that holds its rows' values, as if they were stored anew; a row that
 // stays is written again only if the scale changed.
-template <int CODE, int D>
+//
+// Latency and bytes bound it.  Both sides are asked for at once.  Where few rows move, all of the block's own rows come
+// as soon as src says so, and those that move in behind them, when the table has said where they are; where many move,
+// all rows then.
+template <int CODE, int D, int B>
 __global__ __launch_bounds__(256) void evict_kernel(const Evict P) {
-  constexpr int TPR = D / 16;                 // threads per row
-  constexpr int RPP = 256 / TPR;              // rows per pass
-  constexpr int NP = 64 / RPP > 0 ? 64 / RPP : 1;
-  __shared__ int from[64], moved[64];         // pool row of each row; whether it moves
-  __shared__ float scales[2][64];
-  __shared__ float part[4];
-  const int B = 1 << P.log2b, nb = P.budget >> P.log2b;
-  const int lp = blockIdx.x % nb, w = blockIdx.x / nb, h = w % P.H, j = w / P.H;
-  const int row = P.rows ? P.rows[j] : j;
+  constexpr int LOG2B = B == 16 ? 4 : B == 32 ? 5 : 6;
+  constexpr int TPR = D / 16, SIDE = B * TPR;                // threads per row (16 bytes each); units of 16 bytes per side
+  constexpr int T = 2 * SIDE < 256 ? 2 * SIDE : 256, NP = 2 * SIDE / T;   // threads; units of a thread, K's before V's
+  constexpr int kWavesPer = T / 64;
+  __shared__ int from[B], moved[B];           // pool row of each row; whether it moves
+  __shared__ float scales[2][B];
+  __shared__ float part[2][kWavesPer];
+  const int nb = P.budget >> LOG2B, lp = blockIdx.x % nb, w = blockIdx.x / nb, h = w % P.H, j = w / P.H;
+  const int row = P.rows ? uniform(P.rows[j]) : j;
   if (row < 0 || row >= P.n_rows) return;
-  const int len = (int)min((int64_t)max(P.kv_lens[j], 0), P.cap);
-  if (len <= P.budget) return;
   const int64_t tbl = row * P.stride;
-  const int block = P.table[tbl + lp];
+  const int t = threadIdx.x, e = (lp << LOG2B) + t;
+  const int block = uniform(P.table[tbl + lp]);
+  const int s = t < B ? P.src[((int64_t)j * P.H + h) * P.budget + e] : -1;
+  const int len = (int)min((int64_t)max(uniform(P.kv_lens[j]), 0), P.cap);
+  if (len <= P.budget) return;
   const bool there = block >= 0 && block < P.n_blocks;
-  const int t = threadIdx.x;
-  int moves = 0;
+  const bool comes = there && s >= P.budget && s < len;
+  int b = comes ? P.table[tbl + (s >> LOG2B)] : block;
+  const int count = __syncthreads_count(comes);
+  if (count == 0) {
+    if (P.pos && t < B && e >= P.held[row]) P.pos[row * P.sp_r + h * P.sp_h + e] = e + P.evicted[row];
+    return;
+  }
+  const int64_t v_from_k = P.codes[1] - P.codes[0];          // (a selected pointer would be loaded again for every use)
+  auto side_of = [&](int i) { return SIDE >= T ? i * T / SIDE : (t + T * i) / SIDE; };
+  auto row_of = [&](int i) { return ((t + T * i) / TPR) % B; };
+  auto code_at = [&](int i, int pool_row) {
+    return P.codes[0] + (side_of(i) ? v_from_k : (int64_t)0) +
+           ((((int64_t)(pool_row >> LOG2B) * P.H + h) << LOG2B) + (pool_row & (B - 1))) * D + 16 * (t % TPR);
+  };
+  u4v raw[NP];
+  const bool few = 4 * count <= B;
+  if (few) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) raw[i] = *reinterpret_cast<const u4v*>(code_at(i, (block << LOG2B) + row_of(i)));
+  }
   if (t < B) {
-    const int e = (lp << P.log2b) + t;
-    const int s = P.src[((int64_t)j * P.H + h) * P.budget + e];
-    int b = s >= P.budget && s < len ? P.table[tbl + (s >> P.log2b)] : -1;
-    moves = b >= 0 && b < P.n_blocks && there;
+    const bool moves = comes && b >= 0 && b < P.n_blocks;
+    if (!moves) b = block;
+    moved[t] = moves;
+    from[t] = (b << LOG2B) + ((moves ? s : e) & (B - 1));
+    const int64_t at = (int64_t)b * P.H + h;
+    scales[0][t] = P.scale[0][at], scales[1][t] = P.scale[1][at];
     if (P.weights && moves) {
       float* x = P.weights + row * P.sw_r + h * P.sw_h;
       x[e] = x[s];
@@ -490,75 +537,73 @@ __global__ __launch_bounds__(256) void evict_kernel(const Evict P) {
       const int held = P.held[row], gone = P.evicted[row], at = moves ? s : e;
       if (moves || e >= held) x[e] = at < held ? x[at] : at + gone;
     }
-    moved[t] = moves;
-    if (!moves) b = block;
-    from[t] = there ? (b << P.log2b) + ((moves ? s : e) & (B - 1)) : 0;
-    if (there) {
-      const int64_t at = (int64_t)b * P.H + h;
-      scales[0][t] = P.scale[0][at], scales[1][t] = P.scale[1][at];
-    }
   }
-  if (!__syncthreads_or(moves)) return;
-  const int tr = t / TPR, tc = t % TPR;
+  __syncthreads();
+  if (!few) {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) raw[i] = *reinterpret_cast<const u4v*>(code_at(i, from[row_of(i)]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+      if (moved[row_of(i)]) raw[i] = *reinterpret_cast<const u4v*>(code_at(i, from[row_of(i)]));
+  }
+  float top[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    float m = magnitude<CODE>(raw[i]);
+    const float f = scales[side_of(i)][row_of(i)];
+    // (infinity: a scale that is not finite)
+    m = f - f == 0.0f ? fminf(m * f, 3.402823466e38f) : __builtin_inff();
+    if (side_of(i)) top[1] = fmaxf(top[1], m);
+    else top[0] = fmaxf(top[0], m);
+  }
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
-    uint8_t* codes = P.codes[side];
-    u4v raw[NP];
-    float top = 0.0f;
-    bool fine = true;
+    top[side] = group_max<64>(top[side]);
+    if ((t & 63) == 0) part[side][t >> 6] = top[side];
+  }
+  __syncthreads();
+  float size[2], inv[2];
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int r = tr + i * RPP;
-      if (r >= B) continue;
-      const int at = from[r];
-      raw[i] = *reinterpret_cast<const u4v*>(
-          codes + ((((int64_t)(at >> P.log2b) * P.H + h) << P.log2b) + (at & (B - 1))) * D + 16 * tc);
-    }
+  for (int side = 0; side < 2; ++side) {
+    float x = part[side][0];
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int r = tr + i * RPP;
-      if (r >= B) continue;
-      float m = 0.0f;
+    for (int v = 1; v < kWavesPer; ++v) x = fmaxf(x, part[side][v]);
+    size[side] = x < __builtin_inff() ? pow2_scale<CODE>(x) : __builtin_nanf("");
+    inv[side] = 1.0f / size[side];
+    if (t == 0) P.scale[side][(int64_t)block * P.H + h] = size[side];
+  }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) m = fmaxf(m, magnitude<CODE>(raw[i][c]));
-      const float s = scales[side][r];
-      fine = fine && s - s == 0.0f;
-      top = fmaxf(top, m * s);
-    }
-    top = group_max<64>(fine ? fminf(top, 3.402823466e38f) : __builtin_inff());   // (infinity: a scale that is not finite)
-    __syncthreads();
-    if ((t & 63) == 0) part[t >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-    const bool finite = top < __builtin_inff();
-    const float size = finite ? pow2_scale<CODE>(top) : __builtin_nanf("");
-    const float inv = 1.0f / size;
+  for (int i = 0; i < NP; ++i) {
+    const int side = side_of(i), r = row_of(i);
+    const float f = scales[side][r], z = side ? size[1] : size[0], y = side ? inv[1] : inv[0];
+    const bool kept = f == z || z != z;                      // (NaN: the codes as they are)
+    if (kept && !moved[r]) continue;
+    u4v o = raw[i];
+    if (!kept) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int r = tr + i * RPP;
-      if (r >= B) continue;
-      const float s = scales[side][r];
-      if (!moved[r] && (!finite || s == size)) continue;
-      u4v o = raw[i];
-      if (finite && s != size) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float y[4];
-          unpack4<CODE>(raw[i][c], y);
-          o[c] = pack4<CODE>(y[0] * s * inv, y[1] * s * inv, y[2] * s * inv, y[3] * s * inv);
-        }
+      for (int c = 0; c < 4; ++c) {
+        float x[4];
+        unpack4<CODE>(raw[i][c], x);
+        o[c] = pack4<CODE>(x[0] * f * y, x[1] * f * y, x[2] * f * y, x[3] * f * y);
       }
-      *reinterpret_cast<u4v*>(codes + ((((int64_t)block * P.H + h) << P.log2b) + r) * D + 16 * tc) = o;
     }
-    if (t == 0) P.scale[side][(int64_t)block * P.H + h] = size;
+    *reinterpret_cast<u4v*>(code_at(i, (block << LOG2B) + r)) = o;
   }
 }
 
+template <int CODE, int D>
+void evict_launch(const Evict& P, int grid, hipStream_t st) {
+  auto threads = [](int b) { return min(256, 2 * b * (D / 16)); };
+  if (P.log2b == 4) evict_kernel<CODE, D, 16><<<grid, threads(16), 0, st>>>(P);
+  else if (P.log2b == 5) evict_kernel<CODE, D, 32><<<grid, threads(32), 0, st>>>(P);
+  else evict_kernel<CODE, D, 64><<<grid, threads(64), 0, st>>>(P);
+}
 template <int CODE>
-void evict_launch(const Evict& P, int D, int grid, hipStream_t st) {
-  if (D == 64) evict_kernel<CODE, 64><<<grid, 256, 0, st>>>(P);
-  else if (D == 128) evict_kernel<CODE, 128><<<grid, 256, 0, st>>>(P);
-  else evict_kernel<CODE, 256><<<grid, 256, 0, st>>>(P);
+void evict_launch_d(const Evict& P, int D, int grid, hipStream_t st) {
+  if (D == 64) evict_launch<CODE, 64>(P, grid, st);
+  else if (D == 128) evict_launch<CODE, 128>(P, grid, st);
+  else evict_launch<CODE, 256>(P, grid, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- trim
@@ -726,8 +771,8 @@ extern "C" int kvt_block_evict(const void* src, const void* kv_lens, int n, int 
   P.sw_r = sw_r, P.sw_h = sw_h, P.sp_r = sp_r, P.sp_h = sp_h, P.cap = (int64_t)max_blocks * block;
   P.n = n, P.n_rows = n_rows, P.H = H, P.n_blocks = n_blocks, P.max_blocks = max_blocks;
   P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.budget = budget;
-  if (code == kE4M3) evict_launch<kE4M3>(P, D, (int)grid, (hipStream_t)stream);
-  else evict_launch<kI8>(P, D, (int)grid, (hipStream_t)stream);
+  if (code == kE4M3) evict_launch_d<kE4M3>(P, D, (int)grid, (hipStream_t)stream);
+  else evict_launch_d<kI8>(P, D, (int)grid, (hipStream_t)stream);
   KVT_CHECK_LAUNCH();
   return KVT_OK;
 }

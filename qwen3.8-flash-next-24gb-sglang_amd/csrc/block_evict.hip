@@ -475,135 +475,105 @@ KVT_DEV float magnitude(u4v v) {
   }
 }
 
-// One workgroup per (request, KV head, block below the budget).  A block of which every row stays is left as it is.
+// One wavefront per (request, KV head, block below the budget, side).  A block of which every row stays is left as it is.
 // Another one's scale is the smallest power of two that holds its rows' values, as if they were stored anew; a row that
 // stays is written again only if the scale changed.
 //
-// Latency and bytes bound it.  Both sides are asked for at once.  Where few rows move, all of the block's own rows come
-// as soon as src says so, and those that move in behind them, when the table has said where they are; where many move,
-// all rows then.
+// Bytes and latency bound it.  Lane r has row r's source and scale (K's wavefronts: its weight and position); then 16 bytes
+// of a row at a time.
 template <int CODE, int D, int B>
 __global__ __launch_bounds__(256) void evict_kernel(const Evict P) {
   constexpr int LOG2B = B == 16 ? 4 : B == 32 ? 5 : 6;
-  constexpr int TPR = D / 16, SIDE = B * TPR;                // threads per row (16 bytes each); units of 16 bytes per side
-  constexpr int T = 2 * SIDE < 256 ? 2 * SIDE : 256, NP = 2 * SIDE / T;   // threads; units of a thread, K's before V's
-  constexpr int kWavesPer = T / 64;
-  __shared__ int from[B], moved[B];           // pool row of each row; whether it moves
-  __shared__ float scales[2][B];
-  __shared__ float part[2][kWavesPer];
-  const int nb = P.budget >> LOG2B, lp = blockIdx.x % nb, w = blockIdx.x / nb, h = w % P.H, j = w / P.H;
+  constexpr int TPR = D / 16, NP = B * TPR / 64;             // lanes per row; units of a lane and side
+  const int lane = threadIdx.x & 63, w = blockIdx.x * 4 + uniform((int)threadIdx.x >> 6), h = blockIdx.y, j = blockIdx.z;
+  const int lp = w >> 1, side = w & 1;
+  if (lp >= P.budget >> LOG2B) return;
   const int row = P.rows ? uniform(P.rows[j]) : j;
   if (row < 0 || row >= P.n_rows) return;
   const int64_t tbl = row * P.stride;
-  const int t = threadIdx.x, e = (lp << LOG2B) + t;
+  const int e = (lp << LOG2B) + lane;
+  const int s = lane < B ? P.src[((int64_t)j * P.H + h) * P.budget + e] : -1;
   const int block = uniform(P.table[tbl + lp]);
-  const int s = t < B ? P.src[((int64_t)j * P.H + h) * P.budget + e] : -1;
   const int len = (int)min((int64_t)max(uniform(P.kv_lens[j]), 0), P.cap);
   if (len <= P.budget) return;
-  const bool there = block >= 0 && block < P.n_blocks;
-  const bool comes = there && s >= P.budget && s < len;
-  int b = comes ? P.table[tbl + (s >> LOG2B)] : block;
-  const int count = __syncthreads_count(comes);
-  if (count == 0) {
-    if (P.pos && t < B && e >= P.held[row]) P.pos[row * P.sp_r + h * P.sp_h + e] = e + P.evicted[row];
+  const bool comes = block >= 0 && block < P.n_blocks && s >= P.budget && s < len;
+  int held = 0, gone = 0;
+  const bool has_pos = P.pos && side == 0;
+  if (has_pos) held = uniform(P.held[row]), gone = uniform(P.evicted[row]);
+  int32_t* pos = P.pos + (row * P.sp_r + h * P.sp_h);
+  if (!__any(comes)) {
+    if (has_pos && lane < B && e >= held) pos[e] = e + gone;
     return;
   }
-  const int64_t v_from_k = P.codes[1] - P.codes[0];          // (a selected pointer would be loaded again for every use)
-  auto side_of = [&](int i) { return SIDE >= T ? i * T / SIDE : (t + T * i) / SIDE; };
-  auto row_of = [&](int i) { return ((t + T * i) / TPR) % B; };
-  auto code_at = [&](int i, int pool_row) {
-    return P.codes[0] + (side_of(i) ? v_from_k : (int64_t)0) +
-           ((((int64_t)(pool_row >> LOG2B) * P.H + h) << LOG2B) + (pool_row & (B - 1))) * D + 16 * (t % TPR);
-  };
-  u4v raw[NP];
-  const bool few = 4 * count <= B;
-  if (few) {
+  int b = comes ? P.table[tbl + (s >> LOG2B)] : block;
+  const bool moves = comes && b >= 0 && b < P.n_blocks;
+  if (!moves) b = block;
+  const int64_t from = ((((int64_t)b * P.H + h) << LOG2B) + ((moves ? s : e) & (B - 1))) * D;
+  const int from_lo = (int)(uint32_t)from, from_hi = (int)(from >> 32);
+  uint8_t* codes = side ? P.codes[1] : P.codes[0];
+  float* scales = side ? P.scale[1] : P.scale[0];
+  const float scale = scales[(int64_t)b * P.H + h];
+  const uint64_t moved = __ballot(moves);
+  const int64_t to = (((int64_t)block * P.H + h) << LOG2B) * D;
+  auto row_of = [&](int i) { return (lane + 64 * i) / TPR; };
+  u4v x[NP];
 #pragma unroll
-    for (int i = 0; i < NP; ++i) raw[i] = *reinterpret_cast<const u4v*>(code_at(i, (block << LOG2B) + row_of(i)));
+  for (int i = 0; i < NP; ++i) {
+    const uint32_t lo = (uint32_t)__shfl(from_lo, row_of(i), 64), hi = (uint32_t)__shfl(from_hi, row_of(i), 64);
+    x[i] = *reinterpret_cast<const u4v*>(codes + (int64_t)((uint64_t)hi << 32 | lo) + 16 * (lane % TPR));
   }
-  if (t < B) {
-    const bool moves = comes && b >= 0 && b < P.n_blocks;
-    if (!moves) b = block;
-    moved[t] = moves;
-    from[t] = (b << LOG2B) + ((moves ? s : e) & (B - 1));
-    const int64_t at = (int64_t)b * P.H + h;
-    scales[0][t] = P.scale[0][at], scales[1][t] = P.scale[1][at];
-    if (P.weights && moves) {
-      float* x = P.weights + row * P.sw_r + h * P.sw_h;
+  if (lane < B) {
+    if (P.weights && side == 0 && moves) {
+      float* x = P.weights + (row * P.sw_r + h * P.sw_h);
       x[e] = x[s];
     }
-    if (P.pos) {
-      int32_t* x = P.pos + row * P.sp_r + h * P.sp_h;
-      const int held = P.held[row], gone = P.evicted[row], at = moves ? s : e;
-      if (moves || e >= held) x[e] = at < held ? x[at] : at + gone;
+    if (has_pos) {
+      const int at = moves ? s : e;
+      if (moves || e >= held) pos[e] = at < held ? pos[at] : at + gone;
     }
   }
-  __syncthreads();
-  if (!few) {
-#pragma unroll
-    for (int i = 0; i < NP; ++i) raw[i] = *reinterpret_cast<const u4v*>(code_at(i, from[row_of(i)]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < NP; ++i)
-      if (moved[row_of(i)]) raw[i] = *reinterpret_cast<const u4v*>(code_at(i, from[row_of(i)]));
-  }
-  float top[2] = {0.0f, 0.0f};
+  float top = 0.0f;
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    float m = magnitude<CODE>(raw[i]);
-    const float f = scales[side_of(i)][row_of(i)];
+    const float f = __shfl(scale, row_of(i), 64);
     // (infinity: a scale that is not finite)
-    m = f - f == 0.0f ? fminf(m * f, 3.402823466e38f) : __builtin_inff();
-    if (side_of(i)) top[1] = fmaxf(top[1], m);
-    else top[0] = fmaxf(top[0], m);
+    top = fmaxf(top, f - f == 0.0f ? fminf(magnitude<CODE>(x[i]) * f, 3.402823466e38f) : __builtin_inff());
   }
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    top[side] = group_max<64>(top[side]);
-    if ((t & 63) == 0) part[side][t >> 6] = top[side];
-  }
-  __syncthreads();
-  float size[2], inv[2];
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    float x = part[side][0];
-#pragma unroll
-    for (int v = 1; v < kWavesPer; ++v) x = fmaxf(x, part[side][v]);
-    size[side] = x < __builtin_inff() ? pow2_scale<CODE>(x) : __builtin_nanf("");
-    inv[side] = 1.0f / size[side];
-    if (t == 0) P.scale[side][(int64_t)block * P.H + h] = size[side];
-  }
+  top = group_max<64>(top);
+  const bool finite = top < __builtin_inff();
+  const float size = finite ? pow2_scale<CODE>(top) : __builtin_nanf(""), inv = 1.0f / size;
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
-    const int side = side_of(i), r = row_of(i);
-    const float f = scales[side][r], z = side ? size[1] : size[0], y = side ? inv[1] : inv[0];
-    const bool kept = f == z || z != z;                      // (NaN: the codes as they are)
-    if (kept && !moved[r]) continue;
-    u4v o = raw[i];
+    const int r = row_of(i);
+    const float f = __shfl(scale, r, 64);
+    const bool kept = f == size || !finite;                  // (not finite: the codes as they are)
+    if (kept && !(moved >> r & 1)) continue;
+    u4v o = x[i];
     if (!kept) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        float x[4];
-        unpack4<CODE>(raw[i][c], x);
-        o[c] = pack4<CODE>(x[0] * f * y, x[1] * f * y, x[2] * f * y, x[3] * f * y);
+        float y[4];
+        unpack4<CODE>(x[i][c], y);
+        o[c] = pack4<CODE>(y[0] * f * inv, y[1] * f * inv, y[2] * f * inv, y[3] * f * inv);
       }
     }
-    *reinterpret_cast<u4v*>(code_at(i, (block << LOG2B) + r)) = o;
+    *reinterpret_cast<u4v*>(codes + to + (64 * i + lane) * 16) = o;
   }
+  if (lane == 0) scales[(int64_t)block * P.H + h] = size;
 }
 
 template <int CODE, int D>
-void evict_launch(const Evict& P, int grid, hipStream_t st) {
-  auto threads = [](int b) { return min(256, 2 * b * (D / 16)); };
-  if (P.log2b == 4) evict_kernel<CODE, D, 16><<<grid, threads(16), 0, st>>>(P);
-  else if (P.log2b == 5) evict_kernel<CODE, D, 32><<<grid, threads(32), 0, st>>>(P);
-  else evict_kernel<CODE, D, 64><<<grid, threads(64), 0, st>>>(P);
+void evict_launch(const Evict& P, hipStream_t st) {
+  const dim3 grid(((P.budget >> P.log2b) + 1) / 2, P.H, P.n);
+  if (P.log2b == 4) evict_kernel<CODE, D, 16><<<grid, 256, 0, st>>>(P);
+  else if (P.log2b == 5) evict_kernel<CODE, D, 32><<<grid, 256, 0, st>>>(P);
+  else evict_kernel<CODE, D, 64><<<grid, 256, 0, st>>>(P);
 }
 template <int CODE>
-void evict_launch_d(const Evict& P, int D, int grid, hipStream_t st) {
-  if (D == 64) evict_launch<CODE, 64>(P, grid, st);
-  else if (D == 128) evict_launch<CODE, 128>(P, grid, st);
-  else evict_launch<CODE, 256>(P, grid, st);
+void evict_launch_d(const Evict& P, int D, hipStream_t st) {
+  if (D == 64) evict_launch<CODE, 64>(P, st);
+  else if (D == 128) evict_launch<CODE, 128>(P, st);
+  else evict_launch<CODE, 256>(P, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- trim
@@ -759,8 +729,8 @@ extern "C" int kvt_block_evict(const void* src, const void* kv_lens, int n, int 
   if ((D != 64 && D != 128 && D != 256) || (block != 16 && block != 32 && block != 64)) return KVT_EINVAL;
   if ((code != kE4M3 && code != kI8) || budget < block || budget % block || budget / block > max_blocks) return KVT_EINVAL;
   if (((uintptr_t)k8 | (uintptr_t)v8) & 15 || (pos && (!held || !evicted))) return KVT_EINVAL;
-  const int64_t grid = (int64_t)n * H * (budget / block);
-  if (grid >= 1 << 24 || (int64_t)max_blocks * block > ((int64_t)1 << 31) - 8192 ||
+  if (n > 65535 || H > 65535 || (int64_t)n * H * (budget / block + 1) >= 1 << 25 ||   // (2^32 threads)
+      (int64_t)max_blocks * block > ((int64_t)1 << 31) - 8192 ||
       (int64_t)n_blocks * block > (int64_t)1 << 31)
     return KVT_ERANGE;
   Evict P;
@@ -771,8 +741,8 @@ extern "C" int kvt_block_evict(const void* src, const void* kv_lens, int n, int 
   P.sw_r = sw_r, P.sw_h = sw_h, P.sp_r = sp_r, P.sp_h = sp_h, P.cap = (int64_t)max_blocks * block;
   P.n = n, P.n_rows = n_rows, P.H = H, P.n_blocks = n_blocks, P.max_blocks = max_blocks;
   P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.budget = budget;
-  if (code == kE4M3) evict_launch_d<kE4M3>(P, D, (int)grid, (hipStream_t)stream);
-  else evict_launch_d<kI8>(P, D, (int)grid, (hipStream_t)stream);
+  if (code == kE4M3) evict_launch_d<kE4M3>(P, D, (hipStream_t)stream);
+  else evict_launch_d<kI8>(P, D, (hipStream_t)stream);
   KVT_CHECK_LAUNCH();
   return KVT_OK;
 }

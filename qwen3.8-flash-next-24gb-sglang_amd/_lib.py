@@ -70,7 +70,7 @@ SIGNATURES = {
     "kvt_block_keep": [_P, _L, _L, _P, _I, _I, _I, _P, _L, _I, _I, _I, _P, _L, _L, _P, _P, _P, _P, _L, _P],
     "kvt_block_evict": [_P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P, _L, _I, _I, _P, _I, _P, _L, _L, _P, _L, _L,
                         _P, _P, _P],
-    "kvt_block_trim": [_I, _P, _P, _I, _P, _L, _I, _P, _I, _P, _I, _I, _P, _P, _P, _P, _P, _I, _P],
+    "kvt_block_trim": [_I, _P, _P, _I, _P, _L, _I, _P, _I, _P, _I, _I, _P, _P, _P, _P, _P, _I, _P, _P],
     "kvt_vmm_granularity": [_I, _P],
     "kvt_vmm_reserve": [_I, _U, _P, _P],
     "kvt_vmm_commit": [_P, _U],

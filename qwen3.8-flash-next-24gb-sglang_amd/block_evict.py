@@ -246,9 +246,9 @@ def kvt_block_trim(seqs: torch.Tensor, seq_lens: torch.Tensor, block_table: torc
     st = _stream(seqs, seq_lens, block_table, free_list, free_head, held, evicted, status)
     if n == 0:
         return BlockTrim(seqs.new_empty(0), free_head[:1].clamp(0, free_list.numel()))
-    kv_lens, next_head = seqs.new_empty(n + 1).split_with_sizes((n, 1))
+    work, kv_lens, next_head = seqs.new_empty(5 * n + 5).split_with_sizes((4 * n + 4, n, 1))       # (one allocation)
     _lib.call("kvt_block_trim", n, seqs.data_ptr(), seq_lens.data_ptr(), rows, block_table.data_ptr(), block_table.stride(0),
               block_table.shape[1], free_list.data_ptr(), free_list.numel(), free_head.data_ptr(), block, budget,
               _lib.ptr(held), _lib.ptr(evicted), kv_lens.data_ptr(), next_head.data_ptr(), _lib.ptr(status),
-              int(bool(commit)), st)
+              int(bool(commit)), work.data_ptr(), st)
     return BlockTrim(kv_lens, next_head)

@@ -578,6 +578,7 @@ void evict_launch_d(const Evict& P, int D, hipStream_t st) {
 
 // ---------------------------------------------------------------------------------------------------------------- trim
 constexpr int kMaxTrim = 1024, kStamps = 4096;
+constexpr int kFewBlocks = 4096;      // table entries behind the budget, of all requests, up to which one workgroup does it
 enum { kBadRow = 8, kFreeOver = 16 };
 
 struct Trim {
@@ -678,6 +679,86 @@ __global__ __launch_bounds__(1024) void trim_kernel(const Trim P) {
   }
 }
 
+// Many entries behind the budget: a workgroup per request, in two launches.  The first one says of request j: its table
+// row (-1: none, or one that an earlier request has), length and how many blocks it gives back.
+struct Back { int row, len, count, pad; };
+
+__global__ __launch_bounds__(256) void trim_count_kernel(const Trim P, Back* back) {
+  __shared__ int total;
+  const int j = blockIdx.x, t = threadIdx.x, lane = t & 63;
+  const int row = uniform(P.seqs[j]);
+  bool bad = row < 0 || row >= P.rows;
+  for (int i = t; i < j; i += 256) bad |= P.seqs[i] == row;
+  if (t == 0) total = 0;
+  bad = __syncthreads_or(bad);
+  const int len = bad ? 0 : max(uniform(P.seq_lens[row]), 0);
+  const int last = (int)min(((int64_t)len + (1 << P.log2b) - 1) >> P.log2b, (int64_t)P.max_blocks);
+  int c = 0;
+#pragma unroll 4
+  for (int lp = (P.budget >> P.log2b) + t; lp < last; lp += 256) {
+    const int id = P.table[row * P.stride + lp];
+    c += id >= 0 && id < P.n_free;
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o, 64);
+  if (lane == 0) atomicAdd(&total, c);
+  __syncthreads();
+  if (t == 0) {
+    back[j] = {bad ? -1 : row, len, total, 0};
+    P.kv_lens[j] = min(len, P.budget);
+    if (j == 0) back[P.n] = {min(max(*P.free_head, 0), P.n_free), 0, 0, 0};
+    if (bad && P.status) atomicOr(P.status, kBadRow);
+  }
+}
+
+__global__ __launch_bounds__(256) void trim_write_kernel(const Trim P, const Back* back) {
+  __shared__ int sums[2][4];
+  const int j = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const Back my = back[j];
+  const int head = back[P.n].row;
+  int earlier = 0, total = 0;
+  for (int i = t; i < P.n; i += 256) {
+    const int c = back[i].count;
+    total += c, earlier += i < j ? c : 0;
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o, 64), earlier += __shfl_xor(earlier, o, 64);
+  if (lane == 0) sums[0][wave] = total, sums[1][wave] = earlier;
+  __syncthreads();
+  total = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+  int to = head - total + sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
+  if (j == 0 && t == 0) {
+    *P.next_head = max(head - total, 0);
+    if (P.commit) *P.free_head = max(head - total, 0);
+    if (total > head && P.status) atomicOr(P.status, kFreeOver);
+  }
+  if (my.row < 0 || my.len <= P.budget) return;
+  const int first = P.budget >> P.log2b;
+  const int last = (int)min(((int64_t)my.len + (1 << P.log2b) - 1) >> P.log2b, (int64_t)P.max_blocks);
+  int32_t* table = P.table + my.row * P.stride;
+  for (int base = first; base < last; base += 256) {
+    const int lp = base + t;
+    const int id = lp < last ? table[lp] : -1;
+    const bool is = id >= 0 && id < P.n_free;
+    const uint64_t b = __ballot(is);
+    __syncthreads();                            // (the sums of the round before have been read)
+    if (lane == 0) sums[0][wave] = __popcll(b);
+    __syncthreads();
+    int k = to + __popcll(b & (((uint64_t)1 << lane) - 1));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      k += i < wave ? sums[0][i] : 0;
+      to += sums[0][i];
+    }
+    if (is && k >= 0) P.free_list[k] = id;
+    if (lp < last && P.commit) table[lp] = -1;
+  }
+  if (P.commit && t == 0) {
+    P.seq_lens[my.row] = P.budget;
+    if (P.evicted) P.evicted[my.row] += my.len - P.budget, P.held[my.row] = P.budget;
+  }
+}
+
 }  // namespace
 
 extern "C" int kvt_block_keep(const void* weights, int64_t sw_r, int64_t sw_h, const void* kv_lens, int n, int H,
@@ -750,7 +831,7 @@ extern "C" int kvt_block_evict(const void* src, const void* kv_lens, int n, int 
 extern "C" int kvt_block_trim(int n, const void* seqs, void* seq_lens, int rows, void* block_table, int64_t bt_stride,
                               int max_blocks, void* free_list, int n_free, void* free_head, int block, int budget,
                               void* held, void* evicted, void* kv_lens, void* next_head, void* status, int commit,
-                              void* stream) {
+                              void* work, void* stream) {
   if (n < 1 || n > kMaxTrim || rows < 1 || max_blocks < 1 || bt_stride < max_blocks || n_free < 0) return KVT_EINVAL;
   if ((block != 16 && block != 32 && block != 64) || budget < block || budget % block || !held != !evicted) return KVT_EINVAL;
   Trim P;
@@ -759,7 +840,14 @@ extern "C" int kvt_block_trim(int n, const void* seqs, void* seq_lens, int rows,
   P.evicted = (int32_t*)evicted, P.kv_lens = (int32_t*)kv_lens, P.next_head = (int32_t*)next_head;
   P.status = (int32_t*)status, P.stride = bt_stride, P.n = n, P.rows = rows, P.max_blocks = max_blocks;
   P.n_free = n_free, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.budget = budget, P.commit = commit;
-  trim_kernel<<<1, 1024, 0, (hipStream_t)stream>>>(P);
+  if ((int64_t)n * (max_blocks - budget / block) <= kFewBlocks) {
+    trim_kernel<<<1, 1024, 0, (hipStream_t)stream>>>(P);
+  } else {
+    if (!work || (uintptr_t)work & 15) return KVT_EINVAL;
+    trim_count_kernel<<<n, 256, 0, (hipStream_t)stream>>>(P, (Back*)work);
+    KVT_CHECK_LAUNCH();
+    trim_write_kernel<<<n, 256, 0, (hipStream_t)stream>>>(P, (const Back*)work);
+  }
   KVT_CHECK_LAUNCH();
   return KVT_OK;
 }

@@ -337,7 +337,8 @@ def test_evict_specials(kvt_pkg):
 
 
 # ------------------------------------------------------------------------------------------------------------------ trim
-@pytest.mark.parametrize("n,B,budget,longest", [(1, 64, 64, 65), (3, 16, 32, 300), (64, 64, 256, 400), (1024, 16, 16, 90), (5, 32, 64, 60)])
+@pytest.mark.parametrize("n,B,budget,longest", [(1, 64, 64, 65), (3, 16, 32, 300), (64, 64, 256, 400), (1024, 16, 16, 90), (5, 32, 64, 60),
+                                                (7, 16, 32, 20_000), (200, 16, 48, 900), (2, 64, 64, 300_000)])
 @pytest.mark.parametrize("commit", [True, False])
 @pytest.mark.parametrize("bad", [False, True])
 def test_trim(kvt_pkg, n, B, budget, longest, commit, bad):

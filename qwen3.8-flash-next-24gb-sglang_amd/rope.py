@@ -15,7 +15,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .block_kv import _stream, _strides
+from .block_kv import _i32, _stream, _strides
 
 METHODS = (None, "linear", "ntk", "yarn")
 
@@ -65,25 +65,33 @@ def _span(x: torch.Tensor) -> Tuple[int, int]:
     return first, first + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
 
 
-def _output(x: torch.Tensor, out: Optional[torch.Tensor], others: Sequence[Optional[torch.Tensor]]) -> torch.Tensor:
-    """The output of x (a new tensor for None); one that overlaps x or another of the call's tensors, other than as x
-    itself, is refused."""
-    if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    assert out.shape == x.shape and out.dtype == x.dtype and out.stride(2) == 1, "an output has its input's shape and type"
+def _output(x: torch.Tensor, out: torch.Tensor, others: Sequence[Optional[torch.Tensor]]) -> None:
+    """Refuses an output that overlaps x or another of the call's tensors, other than as x itself."""
+    assert out.shape == x.shape and out.dtype == x.dtype and (out.numel() == 0 or out.stride(2) == 1), \
+        "an output has its input's shape and type, and unit last stride"
     if out.numel() == 0:
-        return out
+        return
     if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
         raise ValueError("an output's elements have to be apart")
     if out.data_ptr() == x.data_ptr() and _strides(out) == _strides(x):
-        return out                                          # in place
+        return                                              # in place
     a, b = _span(out)
     for y in (x, *others):
         if y is not None and y.numel() and y.get_device() == out.get_device():
             c, d = _span(y)
             if a < d and c < b:
                 raise ValueError("an output overlaps an input: pass the input itself (in place), or other memory")
-    return out
+
+
+def _side(x: torch.Tensor, out: Optional[torch.Tensor]):
+    """The output of x (a new tensor for None), and the pointers, strides and heads of both."""
+    _, h, d = x.shape
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        so = (h * d, d)
+    else:
+        so = _strides(out)
+    return out, (x.data_ptr(), *_strides(x), h, out.data_ptr(), *so)
 
 
 def kvt_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -99,49 +107,50 @@ def kvt_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor
     last, and `ahead` (int32, by seqs[j], default j) is added to them -- the entries that were evicted.  Rows behind cu[n] are
     neither read nor written.  inverse=True rotates back by the same angles: the transpose, so the gradient of an input is
     the inverse of the output's."""
-    assert q.dim() == 3 and q.dtype in _lib.DTYPE_CODE and (q.numel() == 0 or q.stride(2) == 1), "rows are [N, heads, D]"
     N, Hq, D = q.shape
-    Hk = 0
+    dtype = _lib.DTYPE_CODE.get(q.dtype)
+    assert dtype is not None and (q.stride(2) == 1 or q.numel() == 0), "rows are [N, heads, D] in bf16, fp16 or fp32"
     if k is not None:
-        assert k.dim() == 3 and k.dtype == q.dtype and (k.numel() == 0 or k.stride(2) == 1)
-        assert k.shape[0] == N and k.shape[2] == D, f"keys of {tuple(k.shape)} beside queries of {tuple(q.shape)}"
-        Hk = k.shape[1]
+        n_k, Hk, d_k = k.shape
+        assert k.dtype == q.dtype and (k.stride(2) == 1 or k.numel() == 0)
+        assert n_k == N and d_k == D, f"keys of {tuple(k.shape)} beside queries of {tuple(q.shape)}"
     elif out_k is not None:
         raise ValueError("out_k without k")
+    else:
+        Hk = 0
     assert inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous(), "inv_freq is fp64 [rot / 2]"
     rot = 2 * inv_freq.numel()
     if not 2 <= rot <= D <= 256 or Hq < 1:
         raise ValueError(f"{rot} of {D} channels, {Hq} heads: up to 256 channels and a rotary part within them are served")
-    n = n_rows = 0
+    n = n_rows = wide = 0
     if cu is None:
-        assert positions.dtype in (torch.int32, torch.int64) and positions.dim() == 1 and positions.is_contiguous()
+        wide = int(positions.dtype == torch.int64)
+        assert (wide or positions.dtype == torch.int32) and positions.dim() == 1 and positions.is_contiguous()
         if positions.numel() < N:
             raise ValueError(f"{positions.numel()} positions for {N} tokens")
         if seqs is not None or ahead is not None:
             raise ValueError("seqs and ahead go with cu")
     else:
-        assert cu.dtype == positions.dtype == torch.int32 and cu.dim() == positions.dim() == 1
-        assert cu.is_contiguous() and positions.is_contiguous()
         n = positions.numel()
-        if cu.numel() < n + 1:
-            raise ValueError(f"cu has {cu.numel()} entries for {n} requests")
+        _i32("positions", positions, n)
+        _i32("cu", cu, n + 1)
         if seqs is not None:
-            assert seqs.dtype == torch.int32 and seqs.dim() == 1 and seqs.is_contiguous()
-            if seqs.numel() < n:
-                raise ValueError(f"seqs has {seqs.numel()} entries for {n} requests")
+            _i32("seqs", seqs, n)
         if ahead is not None:
-            assert ahead.dtype == torch.int32 and ahead.dim() == 1 and ahead.is_contiguous()
+            _i32("ahead", ahead, n if seqs is None else 0)
             n_rows = ahead.numel()
-            if seqs is None and n_rows < n:
-                raise ValueError(f"ahead has {n_rows} entries for {n} requests")
-    q_out = _output(q, out_q, (k,))
-    k_out = None if k is None else _output(k, out_k, (q, q_out))
+    if out_q is not None:
+        _output(q, out_q, (k,))
+    if out_k is not None:
+        _output(k, out_k, (q, out_q))
+    out_q, queries = _side(q, out_q)
+    keys = (None, 0, 0, 0, None, 0, 0)
+    if k is not None:
+        out_k, side = _side(k, out_k)
+        keys = side if Hk else keys
     if N == 0 or (cu is not None and n == 0):
-        return q_out, k_out
-    st = _stream(q, k, positions, inv_freq, cu, seqs, ahead, q_out, k_out)
-    keys = (None, 0, 0, 0, None, 0, 0) if Hk == 0 else (k.data_ptr(), *_strides(k), Hk, k_out.data_ptr(), *_strides(k_out))
-    _lib.call("kvt_rope", q.data_ptr(), *_strides(q), Hq, q_out.data_ptr(), *_strides(q_out), *keys,
-              _lib.DTYPE_CODE[q.dtype], N, D, rot, inv_freq.data_ptr(), positions.data_ptr(),
-              int(positions.dtype == torch.int64), _lib.ptr(cu), n, _lib.ptr(seqs), _lib.ptr(ahead), n_rows, float(scale),
-              int(bool(interleaved)), int(bool(inverse)), st)
-    return q_out, k_out
+        return out_q, out_k
+    st = _stream(q, k, positions, inv_freq, cu, seqs, ahead, out_q, out_k)
+    _lib.call("kvt_rope", *queries, *keys, dtype, N, D, rot, inv_freq.data_ptr(), positions.data_ptr(), wide, _lib.ptr(cu), n,
+              _lib.ptr(seqs), _lib.ptr(ahead), n_rows, scale, interleaved, inverse, st)
+    return out_q, out_k

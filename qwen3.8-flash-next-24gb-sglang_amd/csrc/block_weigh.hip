@@ -143,6 +143,7 @@ template <int CODE, int QT, int D>
 __global__ __launch_bounds__(256) void weigh_rows_kernel(const Weigh P) {
   constexpr int NC = D / 64;
   __shared__ float2 J[4][16];
+  __shared__ u4v Qs[D / 32][64];
   const int h = blockIdx.x % P.H, w = blockIdx.x / P.H, split = w % P.splits, r = w / P.splits;
   const Req t = request(P, r);
   const int per = per_split(t.len, P.splits);
@@ -152,14 +153,17 @@ __global__ __launch_bounds__(256) void weigh_rows_kernel(const Weigh P) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
   const bool live = l < P.gs;
   const uint16_t* qrow = (const uint16_t*)P.q + (int64_t)t.q0 * P.sq_n + (int64_t)(h * P.gs + (live ? l : 0)) * P.sq_h;
-  u4v Q[D / 32];
+  if (wave == 0) {
 #pragma unroll
-  for (int k = 0; k < D / 32; ++k) Q[k] = *reinterpret_cast<const u4v*>(qrow + 64 * (k >> 1) + 16 * g + 8 * (k & 1));
+    for (int k = 0; k < D / 32; ++k)
+      Qs[k][lane] = *reinterpret_cast<const u4v*>(qrow + 64 * (k >> 1) + 16 * g + 8 * (k & 1));
+  }
   const int64_t pair_id = (int64_t)r * P.H + h, cap = (int64_t)P.max_blocks << P.log2b;
   float* score = P.scores + (pair_id * P.gs + l) * cap;
   const uint32_t koff = (uint32_t)l * D + 16u * g;
   const int64_t tbl = (int64_t)t.trow * P.stride;
   float m = -kInf, sum = 0.0f;
+  __syncthreads();
 
   for (int base = p_begin + 32 * wave; base < p_end; base += 32 * 128) {
     // blocks and scales of the next 32 tiles: lane 2 i + s has half s of the tile at base + 128 i
@@ -185,14 +189,19 @@ __global__ __launch_bounds__(256) void weigh_rows_kernel(const Weigh P) {
         for (int c = 0; c < NC; ++c) kr[s][c] = *reinterpret_cast<const u4v*>(P.k8 + at + koff + 64u * c);
       }
       float x[2][4];
+      f4 accs[2] = {};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const u4v q0 = Qs[2 * c][lane], q1 = Qs[2 * c + 1][lane];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          accs[s] = mfma16<QT>(eight<CODE, QT>(kr[s][c][0], kr[s][c][1]), q0, accs[s]);
+          accs[s] = mfma16<QT>(eight<CODE, QT>(kr[s][c][2], kr[s][c][3]), q1, accs[s]);
+        }
+      }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        f4 acc = {0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          acc = mfma16<QT>(eight<CODE, QT>(kr[s][c][0], kr[s][c][1]), Q[2 * c], acc);
-          acc = mfma16<QT>(eight<CODE, QT>(kr[s][c][2], kr[s][c][3]), Q[2 * c + 1], acc);
-        }
+        const f4 acc = accs[s];
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[s][j] = 4 * g + j < valid[s] ? acc[j] * f[s] : -kInf;
         if (live && p0 + 16 * s < p_end) *reinterpret_cast<f4*>(score + p0 + 16 * s + 4 * g) = f4{x[s][0], x[s][1], x[s][2], x[s][3]};

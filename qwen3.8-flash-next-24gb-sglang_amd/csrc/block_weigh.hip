@@ -307,17 +307,13 @@ template <int D> constexpr int kPitch = 2 * D + 16;
 template <bool SIXTEEN>
 KVT_DEV int channel(int k, int hl) { return SIXTEEN ? 32 * (k >> 1) + 16 * hl + 8 * (k & 1) : 16 * k + 8 * hl; }
 
-// BYTES per lane from each lane's address into lds + BYTES * lane.  M0 (the LDS base) is an input of the statement, so the
-// compiler sets it; the s_nop covers the wait states after that, which its hazard checks do not look for inside inline
-// assembly.  (With the builtin it waits for the copy before every later LDS read.)  The caller waits: vmcnt(0) and a
-// barrier.
+// BYTES per lane from each lane's address into lds + BYTES * lane.  The caller waits: vmcnt(0) and a barrier.
 template <int BYTES>
 KVT_DEV void copy_to_lds(const void* from, void* lds) {
-  const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)lds);
-  if constexpr (BYTES == 16)
-    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "{m0}"(base) : "memory");
-  else
-    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" : : "v"(from), "{m0}"(base) : "memory");
+  const auto* g = (const __attribute__((address_space(1))) void*)from;
+  auto* l = (__attribute__((address_space(3))) void*)lds;
+  if constexpr (BYTES == 16) __builtin_amdgcn_global_load_lds(g, l, 16, 0, 0);
+  else __builtin_amdgcn_global_load_lds(g, l, 4, 0, 0);
 }
 
 // The products of a streamed tile of 32 rows, whose operand k is read(k), with two held ones: operands are read a batch
@@ -519,11 +515,12 @@ KVT_DEV int per_row_split(int n_rows, int splits) { return max(((n_rows + splits
 // registers: 16-byte chunk c of row i goes to place c ^ (i & 15) (D 64: & 7), so that a column of chunks is spread over the
 // banks.
 template <int CODE, int QT, int D>
-__global__ __launch_bounds__(256, 2) void weigh_sums_kernel(const Weigh P) {
+__global__ __launch_bounds__(256, D == 256 ? 2 : 3) void weigh_sums_kernel(const Weigh P) {
   constexpr int KS = D / 16, NL = D / 32;     // products per tile of 32 rows; 16-byte copies per thread and tile of Q
   constexpr int TPR = D / 8, SW = TPR < 16 ? TPR - 1 : 15;
-  __shared__ __attribute__((aligned(16))) uint8_t tile[2][kStep * 2 * D];
-  __shared__ __attribute__((aligned(16))) float2 norms[2][kStep];
+  // (arrays of their own, and a loop of two steps: the compiler makes a read of one buffer wait for copies into it only)
+  __shared__ __attribute__((aligned(16))) uint8_t tile0[kStep * 2 * D], tile1[kStep * 2 * D];
+  __shared__ __attribute__((aligned(16))) float2 norms0[kStep], norms1[kStep];
   int w = blockIdx.x;
   const int split = w % P.pos_splits;
   w /= P.pos_splits;
@@ -566,25 +563,23 @@ __global__ __launch_bounds__(256, 2) void weigh_sums_kernel(const Weigh P) {
     const int64_t pw = p0 + 64 * wave;
     const int begin = max(row_of(p0), r_begin) & ~(kStep - 1);
     const int some = pw < t.len ? row_of(pw) : r_end, all = row_of(min(pw + 64, (int64_t)t.len) - 1);
-    auto copy = [&](int r0, int buf) {
+    auto copy = [&](int r0, uint8_t* tile, float2* norms) {
 #pragma unroll
       for (int k = 0; k < NL; ++k) {
         const int at = tr + k * (256 / TPR), row = min(r0 + at, r_end - 1);   // (rows behind the last one count for nothing)
         const uint16_t* from = (const uint16_t*)P.q + q_offset(P, t, h, row) + 8 * (tc ^ (at & SW));
-        copy_to_lds<16>(from, tile[buf] + 4096 * k + 1024 * wave);
+        copy_to_lds<16>(from, tile + 4096 * k + 1024 * wave);
       }
       if (wave < 2) {
         const float* from = (const float*)(norm + min(r0 + 32 * wave + (lane >> 1), r_end - 1)) + (lane & 1);
-        copy_to_lds<4>(from, &norms[buf][32 * wave]);
+        copy_to_lds<4>(from, norms + 32 * wave);
       }
     };
-    if (begin < r_end) copy(begin, 0);
-    int buf = 0;
-    for (int r0 = begin; r0 < r_end; r0 += kStep, buf ^= 1) {
-      const uint8_t* T = tile[buf];
+    if (begin < r_end) copy(begin, tile0, norms0);
+    auto step = [&](int r0, const uint8_t* T, const float2* norms, uint8_t* next_tile, float2* next_norms) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // (the tile's copies)
       __syncthreads();
-      if (r0 + kStep < r_end) copy(r0 + kStep, buf ^ 1);
+      if (r0 + kStep < r_end) copy(r0 + kStep, next_tile, next_norms);
       auto take = [&](auto masked) {
         constexpr bool EDGE = decltype(masked)::value;
 #pragma unroll
@@ -596,7 +591,7 @@ __global__ __launch_bounds__(256, 2) void weigh_sums_kernel(const Weigh P) {
               }, K, acc);
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            const f4 n2 = *reinterpret_cast<const f4*>(&norms[buf][32 * s + prow(i, hl)]);
+            const f4 n2 = *reinterpret_cast<const f4*>(norms + 32 * s + prow(i, hl));
             const int row = r0 + 32 * s + prow(i, hl);
 #pragma unroll
             for (int c = 0; c < 2; ++c)
@@ -620,6 +615,10 @@ __global__ __launch_bounds__(256, 2) void weigh_sums_kernel(const Weigh P) {
           take(std::false_type{});
         }
       }
+    };
+    for (int r0 = begin; r0 < r_end; r0 += 2 * kStep) {
+      step(r0, tile0, norms0, tile1, norms1);
+      if (r0 + kStep < r_end) step(r0 + kStep, tile1, norms1, tile0, norms0);
     }
     __syncthreads();            // (the next positions' first tile goes where this one's last may still be read)
 #pragma unroll

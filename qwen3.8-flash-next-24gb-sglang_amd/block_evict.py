@@ -28,7 +28,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .block_kv import BLOCKS, CODE, FREE_OVER, _grown, _i32, _pool, _rows16, _stream
+from .block_kv import BLOCKS, CODE, FREE_OVER, _apart, _grown, _i32, _overlap, _pool, _rows16, _stream
 
 # Workgroups of the launches.  One query per request: the scores' (at most 256 splits of a pair, whose maxima and sums
 # every workgroup of the sums reads; us per call with 512 / 1,024 / 2,048 / 4,096: 32 requests x 2 heads, D 256, up to 16,384
@@ -66,7 +66,8 @@ def kvt_block_weigh(q: torch.Tensor, k8: torch.Tensor, ks: torch.Tensor, block_t
     request j owns rows cu_q[j] .. cu_q[j + 1]; they are its last positions and each sees the entries up to its own, as in
     kvt_block_prefill.  They may be the end of a longer chunk: its last queries alone, as a sample of all.
     Entries from since[j] on (int32 [n]; default: the call's own positions) start from zero, whatever `weights` holds there;
-    since = 0 weighs anew.  The sums go to `out` (default: weights itself; else a tensor of its own: a step that may be
+    since = 0 weighs anew.  (So a step that is not weighed leaves its entries' weights undefined: weigh every step, or give
+    since.)  The sums go to `out` (default: weights itself; else a tensor of its own: a step that may be
     taken back), entries behind kv_lens[j] are left as they are.  A query that sees nothing adds nothing; one that sees a
     NaN, or a block whose scale is not finite, makes NaN of every entry that it sees.  Rows of seqs have to be distinct.
     scale: > 0, default D ** -0.5.  workspace as in kvt_block_decode: its buffers follow from the table's width (one query
@@ -90,8 +91,11 @@ def kvt_block_weigh(q: torch.Tensor, k8: torch.Tensor, ks: torch.Tensor, block_t
     _per_entry("weights", weights, torch.float32, block_table.shape[0], H, cap)
     if out is None:
         out = weights
-    else:
+    elif out is not weights:
         _per_entry("out", out, torch.float32, block_table.shape[0], H, cap)
+        if _overlap(out, weights) and (out.data_ptr() != weights.data_ptr() or out.stride() != weights.stride()):
+            raise ValueError("out overlaps weights: pass weights itself, or other memory")
+    _apart(out)
     if n == 0:
         return out
     st = _stream(q, k8, ks, block_table, kv_lens, weights, cu_q, seqs, since, out)
@@ -200,7 +204,9 @@ def kvt_block_evict(src: torch.Tensor, kv_lens: torch.Tensor, k8: torch.Tensor, 
     rows, max_blocks = block_table.shape
     if weights is not None:
         _per_entry("weights", weights, torch.float32, rows, H, max_blocks * B)
+        _apart(weights)
     if pos is not None:
+        _apart(pos)
         if held is None or evicted is None:
             raise ValueError("pos goes with held and evicted")
         _per_entry("pos", pos, torch.int32, rows, H, max_blocks * B)

@@ -166,6 +166,25 @@ def _strides(x: torch.Tensor):
     return a if n > 1 else 0, b if h > 1 else 0
 
 
+def _apart(x: torch.Tensor) -> None:
+    """Refuses a tensor to be written of which several entries are the same memory (an expanded one)."""
+    if any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
+        raise ValueError("the entries of a tensor that is written have to be apart")
+
+
+def _span(x: torch.Tensor):
+    first = x.data_ptr()
+    return first, first + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
+
+
+def _overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether the spans of memory of two tensors meet."""
+    if x.numel() == 0 or y.numel() == 0 or x.get_device() != y.get_device():
+        return False
+    (a, b), (c, d) = _span(x), _span(y)
+    return a < d and c < b
+
+
 def _rows16(x: torch.Tensor, per16: int):
     """Rows that start at 16-byte boundaries (x itself, else a contiguous copy): tensor, pointer, strides of token and head."""
     p, (a, b, c) = x.data_ptr(), x.stride()

@@ -15,7 +15,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .block_kv import _i32, _stream, _strides
+from .block_kv import _apart, _i32, _overlap, _stream, _strides
 
 METHODS = (None, "linear", "ntk", "yarn")
 
@@ -60,27 +60,18 @@ def rotary_frequencies(dim: int, base: float = 10000.0, method: Optional[str] = 
     return inv.to(device), scale if attention is None else float(attention)
 
 
-def _span(x: torch.Tensor) -> Tuple[int, int]:
-    first = x.data_ptr()
-    return first, first + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
-
-
 def _output(x: torch.Tensor, out: torch.Tensor, others: Sequence[Optional[torch.Tensor]]) -> None:
     """Refuses an output that overlaps x or another of the call's tensors, other than as x itself."""
     assert out.shape == x.shape and out.dtype == x.dtype and (out.numel() == 0 or out.stride(2) == 1), \
         "an output has its input's shape and type, and unit last stride"
     if out.numel() == 0:
         return
-    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
-        raise ValueError("an output's elements have to be apart")
+    _apart(out)
     if out.data_ptr() == x.data_ptr() and _strides(out) == _strides(x):
         return                                              # in place
-    a, b = _span(out)
     for y in (x, *others):
-        if y is not None and y.numel() and y.get_device() == out.get_device():
-            c, d = _span(y)
-            if a < d and c < b:
-                raise ValueError("an output overlaps an input: pass the input itself (in place), or other memory")
+        if y is not None and _overlap(out, y):
+            raise ValueError("an output overlaps an input: pass the input itself (in place), or other memory")
 
 
 def _side(x: torch.Tensor, out: Optional[torch.Tensor]):
@@ -152,5 +143,5 @@ def kvt_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor
         return out_q, out_k
     st = _stream(q, k, positions, inv_freq, cu, seqs, ahead, out_q, out_k)
     _lib.call("kvt_rope", *queries, *keys, dtype, N, D, rot, inv_freq.data_ptr(), positions.data_ptr(), wide, _lib.ptr(cu), n,
-              _lib.ptr(seqs), _lib.ptr(ahead), n_rows, scale, interleaved, inverse, st)
+              _lib.ptr(seqs), _lib.ptr(ahead), n_rows, scale, bool(interleaved), bool(inverse), st)
     return out_q, out_k

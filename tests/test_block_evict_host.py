@@ -67,10 +67,20 @@ def test_weigh_contract(kvt_pkg, over):
 @pytest.mark.parametrize("over", [dict(q=torch.zeros(3, 4, 64, dtype=torch.bfloat16)), dict(q=torch.zeros(2, 5, 64, dtype=torch.bfloat16)),
                                   dict(q=torch.zeros(2, 34, 64, dtype=torch.bfloat16)), dict(weights=torch.zeros(1, 2, 48)),
                                   dict(weights=torch.zeros(2, 2, 47)), dict(weights=torch.zeros(2, 1, 48)), dict(cu_q=_i(0, 1)),
-                                  dict(since=_i(0)), dict(seqs=_i(0)), dict(out=torch.zeros(2, 2, 40))])
+                                  dict(since=_i(0)), dict(seqs=_i(0)), dict(out=torch.zeros(2, 2, 40)),
+                                  dict(weights=torch.zeros(2, 1, 48).expand(2, 2, 48)), dict(out=torch.zeros(1, 2, 48).expand(2, 2, 48))])
 def test_weigh_sizes(kvt_pkg, over):
     with pytest.raises(ValueError):
         _weigh(**over)
+
+
+def test_weigh_refuses_an_output_that_overlaps(kvt_pkg):
+    w = torch.zeros(3, 2, 48)
+    for out in (w[1:], torch.as_strided(w, (2, 2, 47), (96, 48, 1))):
+        with pytest.raises(ValueError):
+            _weigh(weights=w[:2], out=out)
+    with pytest.raises(AssertionError):            # (weights under another name are weights: on to the device's check)
+        _weigh(weights=w[:2], out=w[:2])
 
 
 def test_keep_refusals(kvt_pkg):
@@ -95,7 +105,9 @@ def test_evict_refusals(kvt_pkg):
             _evict(**bad)
     for bad in (dict(src=torch.zeros(2, 2, 24, dtype=torch.int32)), dict(src=torch.zeros(2, 2, 0, dtype=torch.int32)),
                 dict(src=torch.zeros(1, 2, 16, dtype=torch.int32)), dict(weights=torch.zeros(2, 2, 40)), dict(pos=pos),
-                dict(pos=pos, held=per_row), dict(pos=pos, held=_i(0), evicted=per_row), dict(seqs=_i(0))):
+                dict(pos=pos, held=per_row), dict(pos=pos, held=_i(0), evicted=per_row), dict(seqs=_i(0)),
+                dict(weights=torch.zeros(2, 1, 48).expand(2, 2, 48)),
+                dict(pos=pos[:, :1].expand(2, 2, 48), held=per_row, evicted=per_row)):
         with pytest.raises(ValueError):
             _evict(**bad)
 

@@ -161,6 +161,46 @@ def test_weigh_scale_and_strides(kvt_pkg):
     assert torch.equal(w[:, 0].cpu(), prior[:, 0]) and torch.equal(w[:, 2].cpu(), prior[:, 2])
 
 
+@pytest.mark.parametrize("counts", [None, True])
+def test_weigh_many_ragged_requests(kvt_pkg, counts):
+    """More requests than lanes, some without queries, some without entries."""
+    rng = random.Random(3)
+    lens = [rng.choice([0, 1, 5, 40, 130]) for _ in range(150)]
+    m = None if counts is None else [rng.choice([0, 0, 1, 2, 9]) if n else 0 for n in lens]
+    m = m if m is None else [min(a, b) for a, b in zip(m, lens)]
+    run_weigh((lens, m, 4, 2, 64, 16, "int8", "bf16", 31))
+
+
+def test_weigh_rows_and_lengths_out_of_range(kvt_pkg):
+    """Table rows that are not there are left out; chunks longer than their request, and requests longer than their table."""
+    from kvtier.block_evict import kvt_block_weigh
+    H, B, D, hq = 2, 16, 64, 4
+    sides, table, rows = pool([48, 30, 48], 3, 3, H, B, D, "fp8", 8)
+    g = torch.Generator().manual_seed(6)
+    prior = torch.rand(3, H, 48, generator=g)
+    for lens, counts, seqs in (([3, 100, 20], [5, 2, 1], rows), ([40, 30, 20], [1, 1, 1], [rows[0], 7, -1]),
+                               ([40, 30, 20], None, [rows[0], 3, -5])):
+        cu = prefix(counts or [1, 1, 1])
+        q = torch.randn(cu[-1], hq, D, generator=g).to(torch.bfloat16)
+        want, rel = ref.weigh(q.double(), cu, lens, seqs, table, values(sides[0]), prior.double(), None, D ** -0.5)
+        w = prior.to(dev)
+        kvt_block_weigh(q.to(dev), sides[0][0].to(dev), sides[0][1].to(dev), i32(table), i32(lens), w,
+                        i32(cu) if counts else None, i32(seqs))
+        ref.weigh_close(w, want, rel)
+
+
+def test_weigh_of_no_queries(kvt_pkg):
+    """An output of its own gets the weights as they are."""
+    from kvtier.block_evict import kvt_block_weigh
+    sides, table, rows = pool([48, 30], 3, 2, 1, 16, 64, "fp8", 8)
+    w = torch.rand(2, 1, 48, device=dev)
+    out = torch.zeros_like(w)
+    q = torch.zeros(0, 2, 64, dtype=torch.bfloat16, device=dev)
+    kvt_block_weigh(q, sides[0][0].to(dev), sides[0][1].to(dev), i32(table), i32([48, 30]), w, i32([0, 0, 0]), i32(rows), out=out)
+    assert torch.equal(out[rows[0]], w[rows[0]]) and torch.equal(out[rows[1], :, :30], w[rows[1], :, :30])
+    assert not out[rows[1], :, 30:].any()
+
+
 def test_weigh_far_offsets(kvt_pkg):
     """Code offsets past 2^31 bytes and weight offsets past 2^31 entries."""
     from kvtier.block_evict import kvt_block_weigh
@@ -334,6 +374,29 @@ def test_evict_specials(kvt_pkg):
                       (vs.cpu().double(), scales[1])):
         assert torch.equal(torch.isnan(got), torch.isnan(want))
         assert torch.equal(torch.nan_to_num(got, 1234.0), torch.nan_to_num(want, 1234.0))
+
+
+def test_evict_alone(kvt_pkg):
+    """Codes alone, without weights and positions; table rows that are not there; far blocks (offsets past 2^31 bytes)."""
+    from kvtier.block_evict import kvt_block_evict
+    H, B, D, nb = 8, 64, 256, 16_500
+    k8, v8 = (torch.zeros(nb, H, B, D, dtype=torch.int8, device=dev) for _ in range(2))
+    ks, vs = (torch.ones(nb, H, device=dev) for _ in range(2))
+    g = torch.Generator().manual_seed(3)
+    ids = [16_499, 3, 16_450]
+    small = [torch.randint(-127, 128, (3, H, B, D), generator=g, dtype=torch.int8) for _ in range(2)]
+    scale = [torch.exp2(torch.randint(-3, 4, (3, H), generator=g).float()) for _ in range(2)]
+    for x, z, c, s in ((k8, ks, small[0], scale[0]), (v8, vs, small[1], scale[1])):
+        x[ids], z[ids] = c.to(dev), s.to(dev)
+    src = [[list(range(B)) for _ in range(H)] for _ in range(3)]
+    for h in range(H):
+        src[1][h][5 + h], src[1][h][20] = 64 + h, 150
+    codes, scales = [c.double() for c in small], [s.double() for s in scale]
+    ref.evict(src, [170] * 3, [9, 0, -1], [[0, 1, 2]], codes, scales, "int8")
+    kvt_block_evict(i32(src), i32([170] * 3), k8, v8, ks, vs, i32([ids]), i32([9, 0, -1]))
+    for x, z, c, s in ((k8, ks, codes[0], scales[0]), (v8, vs, codes[1], scales[1])):
+        assert torch.equal(x[ids].cpu().double(), c) and torch.equal(z[ids].cpu().double(), s)
+    assert not k8[:3].any() and not v8[4:16_450].any() and (ks[4:16_450] == 1).all()
 
 
 # ------------------------------------------------------------------------------------------------------------------ trim

@@ -446,19 +446,28 @@ __global__ __launch_bounds__(256, 2) void weigh_norm_kernel(const Weigh P, int i
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          // (scales are >= 0: the largest score of a block is its largest product's)
-          float t0 = acc[c][0], t1 = acc[c][8];
+          auto exps = [&](float ref) {
+            float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
-          for (int i = 1; i < 8; ++i) t0 = fmaxf(t0, acc[c][i]), t1 = fmaxf(t1, acc[c][8 + i]);
-          const float top = fmaxf(m[c], fmaxf(t0 * f0, t1 * f1)), ref = top == -kInf ? 0.0f : top;
-          float s0 = 0.0f, s1 = 0.0f;
+            for (int i = 0; i < 8; ++i) {
+              s0 += exp2_(fmaf(acc[c][i], f0, -ref));
+              s1 += exp2_(fmaf(acc[c][8 + i], f1, -ref));
+            }
+            return s0 + s1;
+          };
+          // The reference m need not be the maximum: it stays while no sum leaves 2^90 (-inf at first: no sum is a number)
+          float more = EDGE ? kInf : exps(m[c]);
+          if (EDGE || __any(!(more <= 0x1p90f))) {
+            // (scales are >= 0: the largest score of a block is its largest product's)
+            float t0 = acc[c][0], t1 = acc[c][8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            s0 += exp2_(fmaf(acc[c][i], f0, -ref));
-            s1 += exp2_(fmaf(acc[c][8 + i], f1, -ref));
+            for (int i = 1; i < 8; ++i) t0 = fmaxf(t0, acc[c][i]), t1 = fmaxf(t1, acc[c][8 + i]);
+            const float top = fmaxf(m[c], fmaxf(t0 * f0, t1 * f1)), ref = top == -kInf ? 0.0f : top;
+            more = exps(ref);
+            sum[c] *= exp2_(m[c] - ref);
+            m[c] = top;
           }
-          sum[c] = fmaf(sum[c], exp2_(m[c] - ref), s0 + s1);
-          m[c] = top;
+          sum[c] += more;
         }
       }
     };

@@ -201,6 +201,42 @@ def test_weigh_of_no_queries(kvt_pkg):
     assert not out[rows[1], :, 30:].any()
 
 
+@pytest.mark.parametrize("counts", [None, [90, 2]])
+@pytest.mark.parametrize("scale", [0.25, 40.0])
+@pytest.mark.parametrize("order", ["rising", "falling"])
+def test_weigh_scores_far_apart(kvt_pkg, counts, scale, order):
+    """Scores that rise, or fall, by hundreds and by tens of thousands along the entries: maxima that lie far above the first tile's, and below."""
+    from kvtier.block_evict import kvt_block_weigh
+    lens, H, B, D, hq = [600, 300], 2, 64, 64, 4
+    sides, table, rows = pool(lens, 10, 2, H, B, D, "int8", 5)
+    k8, ks = sides[0]
+    ks = ks.clone()
+    for r, n in zip(rows, lens):
+        blocks = table[r][:-(-n // B)]
+        for i, b in enumerate(blocks if order == "rising" else reversed(blocks)):
+            ks[b] *= 2.0 ** (i - 4)
+    g = torch.Generator().manual_seed(6)
+    cu = prefix(counts or [1, 1])
+    q = torch.randn(cu[-1], hq, D, generator=g).to(torch.bfloat16)
+    prior = torch.rand(2, H, 640, generator=g)
+    want, rel = ref.weigh(q.double(), cu, lens, rows, table, values((k8, ks)), prior.double(), None, scale)
+    w = prior.to(dev)
+    kvt_block_weigh(q.to(dev), k8.to(dev), ks.to(dev), i32(table), i32(lens), w, None if counts is None else i32(cu), i32(rows),
+                    scale=scale)
+    got = w.double().cpu()
+    assert torch.isfinite(got).all()
+    # Large scores leave the weights few exact bits: `rel` is the bound of that while it is small, 1 + rel for e^rel.  And
+    # every query's weights sum to one, but for what the scores of the two launches differ by, each of them off by half of
+    # rel's first term, and the roundings of the sums: by rel in all.
+    most = float(rel.max())
+    if scale < 1:
+        assert most < 0.05 and ((got - want).abs() <= (rel + 2.0 ** -24) * want.abs() + 1e-30).all()
+    for i, r in enumerate(rows):
+        new = (got[r] - torch.where(torch.arange(640) < lens[i] - (cu[i + 1] - cu[i]), prior[r].double(), 0.0))[:, :lens[i]]
+        assert torch.allclose(new.sum(-1), torch.tensor(float((cu[i + 1] - cu[i]) * hq // H), dtype=torch.float64), rtol=most,
+                              atol=0)
+
+
 def test_weigh_far_offsets(kvt_pkg):
     """Code offsets past 2^31 bytes and weight offsets past 2^31 entries."""
     from kvtier.block_evict import kvt_block_weigh

@@ -433,8 +433,7 @@ int kvt_block_evict(const void* src, const void* kv_lens, int n, int H, int D, i
  * free_list[*free_head] in request order, kv_lens[j] = min(length, budget), *next_head the list's head after that.  commit:
  * their table entries become -1, seq_lens[row] = held[row] = budget, evicted[row] += the entries cut (held and evicted: both
  * or none), *free_head = *next_head.  status (may be NULL): 8 a row out of range or listed twice (kv_lens 0), 16 more blocks
- * than the list had handed out are or-ed in.  n <= 1,024.  work: int32 [4 * n + 4], 16-byte aligned (may be NULL where
- * n * (max_blocks - budget / block) <= 4,096). */
+ * than the list had handed out are or-ed in.  n <= 1,024.  work: int32 [4 * n + 4], 16-byte aligned. */
 int kvt_block_trim(int n, const void* seqs, void* seq_lens, int rows, void* block_table, int64_t bt_stride, int max_blocks,
                    void* free_list, int n_free, void* free_head, int block, int budget, void* held, void* evicted,
                    void* kv_lens, void* next_head, void* status, int commit, void* work, void* stream);

@@ -18,8 +18,9 @@ namespace {
 //
 // The budget-th largest key of a (request, KV head) by radix select (11 + 11 + 10 bits, histograms in LDS), ties to the
 // lowest entry, and the places of what moves, from ranks by ballots.  Up to kSmall entries one workgroup does it all
-// with the keys in registers, read once.  Longer ones take a launch per step, with kMostChunks workgroups a pair at most:
-// three histograms (joined by integer atomics: their order does not matter), counts per chunk, places.
+// with the keys in registers, read once.  Longer ones take a launch per step, with kMostChunks workgroups a pair at
+// most: three histograms (joined by integer atomics: their order does not matter), counts per chunk, places.  Two pairs
+// of 262,144 entries: 41 us, eight launches' latency (one workgroup a pair, which reads the keys seven times, 742).
 constexpr int kKeepThreads = 1024, kWaves = kKeepThreads / 64;
 constexpr int kSmall = 32768, kChunk = 4096, kMostChunks = 256, kBins = 2048;
 
@@ -112,8 +113,8 @@ KVT_DEV void find_bin(const int* hist, int k, int* sums, int* found, int& bin, i
 KVT_DEV int shift_of(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
 KVT_DEV int bins_of(int pass) { return pass == 2 ? 1024 : 2048; }
 
-// The same by every wavefront for itself: lane l has bins 2047 - 32 l and the 31 below.  Four words lie between those of
-// two lanes (padded), so that their 16-byte reads are spread over the banks.
+// The same by every wavefront for itself: lane l has bins 2047 - 32 l and the 31 below.  Four words lie between those
+// of two lanes (padded), so that their 16-byte reads are spread over the banks.
 constexpr int kPadded = kBins + kBins / 8;
 KVT_DEV int padded(int bin) { return bin + (bin >> 5) * 4; }
 KVT_DEV int wave_before(int v) {                  // sum over the lanes up to this one
@@ -142,10 +143,10 @@ KVT_DEV void find_bin_wave(const int* hist, int k, int& bin, int& left) {
   bin = kBins - 1 - 32 * from - at, left = k - __builtin_amdgcn_readlane(x - n, at);
 }
 
-// One workgroup of T threads per pair of no more than T R entries: wavefront v has entries v * seg .., key i of a lane that
-// of entry v * seg + 64 i + lane.  Latency and its instructions bound it: 512 x 4,160
-// entries, keys re-read from memory by 1,024 threads 39 us, in registers 26, every wavefront finding a histogram's bin
-// for itself instead of three barriers more, 512 threads, 16 (256 threads 20, 1,024 19).
+// One workgroup of T threads per pair of no more than T R entries: wavefront v has entries v * seg .., key i of a lane
+// that of entry v * seg + 64 i + lane.  Latency and its instructions bound it: 512 x 4,160 entries, keys re-read from
+// memory by 1,024 threads 39 us, in registers 26, every wavefront finding a histogram's bin for itself instead of three
+// barriers more, 512 threads, 16 (256 threads 20, 1,024 19).
 template <int T, int R>
 __global__ __launch_bounds__(T) void keep_kernel(const Keep P) {
   __shared__ __attribute__((aligned(16))) int hist[3][kPadded];
@@ -183,7 +184,8 @@ __global__ __launch_bounds__(T) void keep_kernel(const Keep P) {
     const int shift = shift_of(pass);
 #pragma unroll
     for (int i = 0; i < R; ++i)
-      if (key[i] && (key[i] & mask) == prefix) atomicAdd(&hist[pass][padded((key[i] >> shift) & (bins_of(pass) - 1))], 1);
+      if (key[i] && (key[i] & mask) == prefix)
+        atomicAdd(&hist[pass][padded((key[i] >> shift) & (bins_of(pass) - 1))], 1);
     __syncthreads();
     int bin;
     find_bin_wave(hist[pass], k, bin, k);
@@ -255,7 +257,7 @@ __global__ __launch_bounds__(T) void keep_kernel(const Keep P) {
 // Pairs of more than kSmall entries.  Chunk c of a pair has entries c * per .. (a multiple of 1,024).
 struct Long {
   int32_t* hist;
-  int32_t* counts;             // of a chunk: keys above the threshold below the budget and behind it, ties below and behind
+  int32_t* counts;             // of a chunk: keys above the threshold below the budget and behind it, ties likewise
   Found* found;
   int32_t* list;
   int32_t* places;
@@ -350,7 +352,7 @@ __global__ __launch_bounds__(kKeepThreads) void keep_list_kernel(const Keep P) {
     for (int base = 0; base < P.chunks; base += 64) {
       const int i = base + lane;
       const int4 n = i < P.chunks ? *reinterpret_cast<const int4*>(L.counts + 4 * i) : make_int4(0, 0, 0, 0);
-      int x = n.z + n.w;                                     // (ties are taken below the budget first: entries in order)
+      int x = n.z + n.w;                        // (ties are taken below the budget first: entries in order)
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         const int u = __shfl_up(x, o, 64);
@@ -360,13 +362,18 @@ __global__ __launch_bounds__(kKeepThreads) void keep_list_kernel(const Keep P) {
       const int low = min(max(k - first, 0), n.z), high = min(max(k - first - n.z, 0), n.w);
       const int per = ((t.len + P.chunks - 1) / P.chunks + 1023) & ~1023;
       const int64_t b = (int64_t)i * per;
-      const int below = i < P.chunks ? (int)(min(max((int64_t)P.budget - b, (int64_t)0), min((int64_t)per, max((int64_t)t.len - b, (int64_t)0)))) : 0;
+      const int64_t has = i < P.chunks ? min((int64_t)per, max((int64_t)t.len - b, (int64_t)0)) : 0;
+      const int below = (int)min(max((int64_t)P.budget - b, (int64_t)0), has);
       int mv = n.y + high, fr = below - n.x - low;
       total += mv;
       if (i >= c) mv = fr = 0;
       int tb = i < c ? n.z + n.w : 0;
 #pragma unroll
-      for (int o = 32; o; o >>= 1) mv += __shfl_xor(mv, o, 64), fr += __shfl_xor(fr, o, 64), tb += __shfl_xor(tb, o, 64);
+      for (int o = 32; o; o >>= 1) {
+        mv += __shfl_xor(mv, o, 64);
+        fr += __shfl_xor(fr, o, 64);
+        tb += __shfl_xor(tb, o, 64);
+      }
       moves += mv, frees += fr;
       if (base <= c && c < base + 64 && lane == 0) start[0] = ties + tb;
       ties += __shfl(x, 63, 64);
@@ -475,17 +482,20 @@ KVT_DEV float magnitude(u4v v) {
   }
 }
 
-// One wavefront per (request, KV head, block below the budget, side).  A block of which every row stays is left as it is.
-// Another one's scale is the smallest power of two that holds its rows' values, as if they were stored anew; a row that
-// stays is written again only if the scale changed.
+// One wavefront per (request, KV head, block below the budget, side).  A block of which every row stays is left as it
+// is. Another one's scale is the smallest power of two that holds its rows' values, as if they were stored anew; a row
+// that stays is written again only if the scale changed.
 //
-// Bytes and latency bound it.  Lane r has row r's source and scale (K's wavefronts: its weight and position); then 16 bytes
-// of a row at a time.
+// Bytes and latency bound it.  Lane r has row r's source and scale (K's wavefronts: its weight and position); then 16
+// bytes of a row at a time.  64 requests x 8 heads, D 128, 4,160 entries cut to 4,096, e4m3 (some 186 MB): 47 us, 4.0
+// TB/s; with a workgroup of 256 threads per block, one side after the other 74, both sides at once 69, a wavefront for
+// both sides 56.
 template <int CODE, int D, int B>
 __global__ __launch_bounds__(256) void evict_kernel(const Evict P) {
   constexpr int LOG2B = B == 16 ? 4 : B == 32 ? 5 : 6;
   constexpr int TPR = D / 16, NP = B * TPR / 64;             // lanes per row; units of a lane and side
-  const int lane = threadIdx.x & 63, w = blockIdx.x * 4 + uniform((int)threadIdx.x >> 6), h = blockIdx.y, j = blockIdx.z;
+  const int lane = threadIdx.x & 63, w = blockIdx.x * 4 + uniform((int)threadIdx.x >> 6);
+  const int h = blockIdx.y, j = blockIdx.z;
   const int lp = w >> 1, side = w & 1;
   if (lp >= P.budget >> LOG2B) return;
   const int row = P.rows ? uniform(P.rows[j]) : j;
@@ -578,7 +588,7 @@ void evict_launch_d(const Evict& P, int D, hipStream_t st) {
 
 // ---------------------------------------------------------------------------------------------------------------- trim
 constexpr int kMaxTrim = 1024, kStamps = 4096;
-constexpr int kFewBlocks = 4096;      // table entries behind the budget, of all requests, up to which one workgroup does it
+constexpr int kFewRounds = 4;         // of one workgroup's wavefronts
 enum { kBadRow = 8, kFreeOver = 16 };
 
 struct Trim {
@@ -596,8 +606,11 @@ struct Trim {
   int n, rows, max_blocks, n_free, log2b, budget, commit;
 };
 
-// One workgroup: a thread per request finds its length and whether an earlier request has its row, a wavefront per request
-// counts the blocks that it gives back, and after a scan writes them in request order.
+// One workgroup, where its 16 wavefronts have few rounds of a request and 64 blocks each: a thread per request finds its
+// length and whether an earlier request has its row, a wavefront per request counts the blocks that it gives back, and
+// after a scan writes them in request order.  us on the device, this / the two launches below: 64 requests of one block,
+// or 64, 5.9 / 5.3, 16 of 256 5.0 / 5.2 (one launch less for the host, 2 - 3 us); 64 of 128 7.5 / 5.3, 256 of 16 14.8 /
+// 5.5, one of 4,096 23.9 / 9.5, 200 of 400 40.4 / 6.0.
 __global__ __launch_bounds__(1024) void trim_kernel(const Trim P) {
   __shared__ int rows[kMaxTrim], lens[kMaxTrim], count[kMaxTrim], stamp[kStamps], sums[kWaves], flags;
   const int j = threadIdx.x, lane = j & 63, wave = j >> 6;
@@ -834,16 +847,17 @@ extern "C" int kvt_block_trim(int n, const void* seqs, void* seq_lens, int rows,
                               void* work, void* stream) {
   if (n < 1 || n > kMaxTrim || rows < 1 || max_blocks < 1 || bt_stride < max_blocks || n_free < 0) return KVT_EINVAL;
   if ((block != 16 && block != 32 && block != 64) || budget < block || budget % block || !held != !evicted) return KVT_EINVAL;
+  if (!work || (uintptr_t)work & 15) return KVT_EINVAL;
   Trim P;
   P.seqs = (const int32_t*)seqs, P.seq_lens = (int32_t*)seq_lens, P.table = (int32_t*)block_table;
   P.free_list = (int32_t*)free_list, P.free_head = (int32_t*)free_head, P.held = (int32_t*)held;
   P.evicted = (int32_t*)evicted, P.kv_lens = (int32_t*)kv_lens, P.next_head = (int32_t*)next_head;
   P.status = (int32_t*)status, P.stride = bt_stride, P.n = n, P.rows = rows, P.max_blocks = max_blocks;
   P.n_free = n_free, P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6, P.budget = budget, P.commit = commit;
-  if ((int64_t)n * (max_blocks - budget / block) <= kFewBlocks) {
+  const int64_t behind = max(max_blocks - budget / block, 0);
+  if ((n + kWaves - 1) / kWaves * ((behind + 63) / 64) <= kFewRounds) {
     trim_kernel<<<1, 1024, 0, (hipStream_t)stream>>>(P);
   } else {
-    if (!work || (uintptr_t)work & 15) return KVT_EINVAL;
     trim_count_kernel<<<n, 256, 0, (hipStream_t)stream>>>(P, (Back*)work);
     KVT_CHECK_LAUNCH();
     trim_write_kernel<<<n, 256, 0, (hipStream_t)stream>>>(P, (const Back*)work);

@@ -2,18 +2,27 @@
 //
 //   out[row, h, p] = prior[row, h, p] + sum over the request's queries i that see p and the q heads g of KV head h of
 //                    exp(x_igp - M_ig) / L_ig,   x_igp = scale * sk_p * q_ig . kc_p
-// with M and L the maximum and the sum of exponentials of (i, g)'s scores: the column sums of softmax(Q K^T), whose rows
-// have to be complete before any column can be.
+// with M and L the maximum and the sum of exponentials of (i, g)'s scores: the column sums of softmax(Q K^T), whose
+// rows have to be complete before any column can be.
 //
-// One query per request (a (request, KV head) has at most 16 rows): the scores are formed once, by 16 x 16 products with
-// K's codes from registers as they were loaded, and kept as fp32 (4 Hq / H bytes an entry against D bytes of codes: less
-// than a second read of K); a second launch joins the splits' maxima and sums and adds up the columns.
+// One query per request (a (request, KV head) has at most 16 rows): the scores are formed once, by 16 x 16 products
+// with K's codes from registers as they were loaded, and kept as fp32 (4 Hq / H bytes an entry against D bytes of
+// codes: less than a second read of K); a second launch joins the splits' maxima and sums and adds up the columns. 
+// Bytes bound both: 32 requests x 2 heads, D 256, up to 16,384 entries (103 MB of codes, 19 MB of scores written and
+// read) 31 + 9 us; int8, 64 x 8 heads, D 128, blocks of 16 (195 + 49 MB) 57 + 17, 4.3 TB/s.  (Tiles of 64 positions a
+// wavefront instead of 32: 57 -> 64; of 16: 59.)
 //
 // Chunks: a row has too many scores to keep, so they are formed twice.  The first launch holds 256 rows of Q in
-// registers (64 a wavefront) and streams K through LDS for maxima and sums; each lane keeps them for a row of its own, over the
-// positions that it sees, so that nothing crosses lanes in the loop.  The second one holds 256 positions of K in
-// registers and streams Q; a lane adds up the weights of its position.  Splits are joined in their order by launches of
-// their own: no atomics, the same bits for every call.
+// registers (64 a wavefront) and streams K through LDS for maxima and sums; each lane keeps them for a row of its own,
+// over the positions that it sees, so that nothing crosses lanes in the loop.  The second one holds 256 positions of K
+// in registers and streams Q; a lane adds up the weights of its position.  Splits are joined in their order by launches
+// of their own: no atomics, the same bits for every call.  64 rows (positions) a wavefront are what 256 registers hold
+// at D 256 with two wavefronts a SIMD, and halve the reads of the streamed tile against 32.  A prompt of 10,001 tokens,
+// 16 / 2 heads, D 256 (410 GFLOP a launch): 411 + 470 us, 998 and 872 TFLOP/s (a large library product 1,247); the
+// steps there: 856 + 1,405 with one wavefront a SIMD, 64-bit divisions for the rows and masks for every tile; 497 + 541
+// without the first two; 460 + 495 with operands read ahead of their products and Q copied straight to LDS; 429 with
+// masks by wavefront.  Exponentials and products take as long as each other at D 256; at D 128 and 64 the exponentials
+// bound it.
 //
 // Operands have q's type (codes of 8 bits are exact in bf16 and fp16); scores, maxima, sums and weights are fp32.
 #include <type_traits>
@@ -120,7 +129,9 @@ KVT_DEV int64_t q_offset(const Weigh& P, const Req& t, int h, int row) {
   return (int64_t)(t.q0 + i) * P.sq_n + (int64_t)(h * P.gs + row - i * P.gs) * P.sq_h;
 }
 // Entries that query i of the request sees.
-KVT_DEV int sees(const Req& t, int i) { return (int)min((int64_t)t.len, max((int64_t)t.kv - t.q_len + i + 1, (int64_t)0)); }
+KVT_DEV int sees(const Req& t, int i) {
+  return (int)min((int64_t)t.len, max((int64_t)t.kv - t.q_len + i + 1, (int64_t)0));
+}
 
 // x and its maximum and sum: a running pair takes another one.
 KVT_DEV void join(float& m, float& l, float m2, float l2) {
@@ -135,8 +146,8 @@ KVT_DEV void finish(const Weigh& P, const Req& t, int r, int h, int p, float sum
   P.out[t.trow * P.so_r + h * P.so_h + p] = sum;
 }
 
-// ------------------------------------------------------------------------------------------------- one query per request
-// Positions per split: equal shares in multiples of 128 (a tile of 32 for each wavefront), 256 at least.
+// ------------------------------------------------------------------------------------------------- one query per
+// request Positions per split: equal shares in multiples of 128 (a tile of 32 for each wavefront), 256 at least.
 KVT_DEV int per_split(int len, int splits) { return max(((len + splits - 1) / splits + 127) & ~127, 256); }
 
 template <int CODE, int QT, int D>
@@ -204,7 +215,8 @@ __global__ __launch_bounds__(256) void weigh_rows_kernel(const Weigh P) {
         const f4 acc = accs[s];
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[s][j] = 4 * g + j < valid[s] ? acc[j] * f[s] : -kInf;
-        if (live && p0 + 16 * s < p_end) *reinterpret_cast<f4*>(score + p0 + 16 * s + 4 * g) = f4{x[s][0], x[s][1], x[s][2], x[s][3]};
+        if (live && p0 + 16 * s < p_end)
+          *reinterpret_cast<f4*>(score + p0 + 16 * s + 4 * g) = f4{x[s][0], x[s][1], x[s][2], x[s][3]};
       }
       float top = m;
 #pragma unroll
@@ -232,8 +244,8 @@ __global__ __launch_bounds__(256) void weigh_rows_kernel(const Weigh P) {
   }
 }
 
-// Maximum and 1 / sum of the pair's rows from the splits' parts, then the columns of 1,024 positions at a time, four per
-// thread.
+// Maximum and 1 / sum of the pair's rows from the splits' parts, then the columns of 1,024 positions at a time, four
+// per thread.
 __global__ __launch_bounds__(256) void weigh_columns_kernel(const Weigh P) {
   __shared__ float2 J[16][16];
   __shared__ float2 norm[16];
@@ -343,7 +355,8 @@ KVT_DEV void products(Read read, const u4v (&held)[2][KS], f16v (&acc)[2]) {
 // Row (of 32) that register i of a 32 x 32 product has in lanes of half hl.
 KVT_DEV int prow(int i, int hl) { return 8 * (i >> 2) + 4 * hl + (i & 3); }
 
-// Maxima and sums of 256 rows over a split of the positions.
+// Maxima and sums of 256 rows over a split of the positions.  (The reference in the place of the running maximum: 52 of
+// some 290 vector instructions per 64 x 64 scores less, 429 -> 411 us.)
 template <int CODE, int QT, int D>
 __global__ __launch_bounds__(256, 2) void weigh_norm_kernel(const Weigh P, int items) {
   constexpr int KS = D / 16, NL = D / 64;     // products per tile of 32; 16-byte loads per thread and tile
@@ -359,7 +372,8 @@ __global__ __launch_bounds__(256, 2) void weigh_norm_kernel(const Weigh P, int i
   const int row0 = (int)begin, live = min(n_rows - row0, kTileRows);
   const int limit = sees(t, query_of(P, row0 + live - 1));
   const int per = (((limit + kStep - 1) / kStep + P.splits - 1) / P.splits) * kStep;
-  const int p_begin = (int)min((int64_t)split * per, (int64_t)limit), p_end = (int)min((int64_t)p_begin + per, (int64_t)limit);
+  const int p_begin = (int)min((int64_t)split * per, (int64_t)limit);
+  const int p_end = (int)min((int64_t)p_begin + per, (int64_t)limit);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 31, hl = lane >> 5;
 
   u4v Q[2][KS];
@@ -381,7 +395,8 @@ __global__ __launch_bounds__(256, 2) void weigh_norm_kernel(const Weigh P, int i
 
   int id = -1;
   float sk = 0.0f;
-  auto ids = [&](int base) {      // blocks and scales of the next 16 tiles: lane 4 i + s has quarter s of tile base / 64 + i
+  // blocks and scales of the next 16 tiles: lane 4 i + s has quarter s of tile base / 64 + i
+  auto ids = [&](int base) {
     const int p = base + 16 * lane;
     id = p < p_end ? P.table[tbl + (p >> P.log2b)] : -1;
     if (id < 0 || id >= P.n_blocks) id = -1;
@@ -431,7 +446,9 @@ __global__ __launch_bounds__(256, 2) void weigh_norm_kernel(const Weigh P, int i
       for (int s = 0; s < 2; ++s) {
         f16v acc[2] = {};
         products<QT, KS>(
-            [&](int k) { return *reinterpret_cast<const u4v*>(T + (32 * s + l) * kPitch<D> + 2 * channel<false>(k, hl)); }, Q, acc);
+            [&](int k) {
+              return *reinterpret_cast<const u4v*>(T + (32 * s + l) * kPitch<D> + 2 * channel<false>(k, hl));
+            }, Q, acc);
         float f0 = f[2 * s], f1 = f[2 * s + 1];
         if constexpr (EDGE) {
 #pragma unroll
@@ -455,7 +472,8 @@ __global__ __launch_bounds__(256, 2) void weigh_norm_kernel(const Weigh P, int i
             }
             return s0 + s1;
           };
-          // The reference m need not be the maximum: it stays while no sum leaves 2^90 (-inf at first: no sum is a number)
+          // The reference m need not be the maximum: it stays while no sum leaves 2^90 (-inf at first: no sum is a
+          // number)
           float more = EDGE ? kInf : exps(m[c]);
           if (EDGE || __any(!(more <= 0x1p90f))) {
             // (scales are >= 0: the largest score of a block is its largest product's)
@@ -521,13 +539,14 @@ __global__ __launch_bounds__(256) void weigh_join_kernel(const Weigh P) {
 KVT_DEV int per_row_split(int n_rows, int splits) { return max(((n_rows + splits - 1) / splits + 63) & ~63, 128); }
 
 // Column sums of 256 positions over a split of the request's rows.  Q's tiles are copied to LDS without a detour by
-// registers: 16-byte chunk c of row i goes to place c ^ (i & 15) (D 64: & 7), so that a column of chunks is spread over the
-// banks.
+// registers: 16-byte chunk c of row i goes to place c ^ (i & 15) (D 64: & 7), so that a column of chunks is spread over
+// the banks.
 template <int CODE, int QT, int D>
 __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void weigh_sums_kernel(const Weigh P) {
   constexpr int KS = D / 16, NL = D / 32;     // products per tile of 32 rows; 16-byte copies per thread and tile of Q
   constexpr int TPR = D / 8, SW = TPR < 16 ? TPR - 1 : 15;
-  // (arrays of their own, and a loop of two steps: the compiler makes a read of one buffer wait for copies into it only)
+  // (arrays of their own, and a loop of two steps: the compiler makes a read of one buffer wait for copies into it
+  // only)
   __shared__ __attribute__((aligned(16))) uint8_t tile0[kStep * 2 * D], tile1[kStep * 2 * D];
   __shared__ __attribute__((aligned(16))) float2 norms0[kStep], norms1[kStep];
   int w = blockIdx.x;
@@ -560,7 +579,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void weigh_sums_kernel(const
       there[c] = id >= 0 && id < P.n_blocks;
       f[c] = there[c] ? factor(P, P.ks[(int64_t)id * P.H + h]) : 0.0f;
       first[c] = row_of(p);
-      const uint8_t* kp = P.k8 + ((((int64_t)(there[c] ? id : 0) * P.H + h) << P.log2b) + (p & ((1 << P.log2b) - 1))) * D + 16 * hl;
+      const int64_t row = (((int64_t)(there[c] ? id : 0) * P.H + h) << P.log2b) + (p & ((1 << P.log2b) - 1));
+      const uint8_t* kp = P.k8 + row * D + 16 * hl;
 #pragma unroll
       for (int k = 0; k < KS / 2; ++k) {
         const u4v v = *reinterpret_cast<const u4v*>(kp + 32 * k);
@@ -575,7 +595,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void weigh_sums_kernel(const
     auto copy = [&](int r0, uint8_t* tile, float2* norms) {
 #pragma unroll
       for (int k = 0; k < NL; ++k) {
-        const int at = tr + k * (256 / TPR), row = min(r0 + at, r_end - 1);   // (rows behind the last one count for nothing)
+        const int at = tr + k * (256 / TPR), row = min(r0 + at, r_end - 1);   // (those behind the last count for nothing)
         const uint16_t* from = (const uint16_t*)P.q + q_offset(P, t, h, row) + 8 * (tc ^ (at & SW));
         copy_to_lds<16>(from, tile + 4096 * k + 1024 * wave);
       }
@@ -596,7 +616,8 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void weigh_sums_kernel(const
           f16v acc[2] = {};
           products<QT, KS>(
               [&](int k) {
-                return *reinterpret_cast<const u4v*>(T + (32 * s + l) * 2 * D + 16 * (channel<true>(k, hl) / 8 ^ (l & SW)));
+                const int chunk = channel<true>(k, hl) / 8;
+                return *reinterpret_cast<const u4v*>(T + (32 * s + l) * 2 * D + 16 * (chunk ^ (l & SW)));
               }, K, acc);
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
@@ -708,7 +729,8 @@ extern "C" int kvt_block_weigh(const void* q, int64_t sq_n, int64_t sq_h, int q_
   if ((D != 64 && D != 128 && D != 256) || (block != 16 && block != 32 && block != 64)) return KVT_EINVAL;
   if ((code != kE4M3 && code != kI8) || (q_type != kBF16 && q_type != kF16) || !(scale > 0.0f)) return KVT_EINVAL;
   if (((uintptr_t)q | (uintptr_t)k8 | (uintptr_t)work) & 15 || (sq_n | sq_h) & 7) return KVT_EINVAL;
-  if (splits < 1 || splits > kMostSplits || row_splits < 1 || row_splits > kMostSplits || pos_splits < 1) return KVT_EINVAL;
+  if (splits < 1 || splits > kMostSplits || row_splits < 1 || row_splits > kMostSplits || pos_splits < 1)
+    return KVT_EINVAL;
   const int gs = Hq / H;
   const int64_t cap = (int64_t)max_blocks * block;
   if (cap > kMostPositions) return KVT_ERANGE;

@@ -172,10 +172,10 @@ def test_c_entries_refuse(kvt_pkg):
         assert evict(**bad) == -1, bad
     assert evict(n=1 << 24, rows=1 << 24) == -3 and evict(mb=2 ** 27, stride=2 ** 27) == -3 and evict(nb=2 ** 28) == -3
 
-    def trim(n=1, rows=1, stride=4, mb=4, n_free=4, block=16, budget=16, held=None, work=None):
+    def trim(n=1, rows=1, stride=4, mb=4, n_free=4, block=16, budget=16, held=None, work=16):
         return lib.kvt_block_trim(n, N, N, rows, N, stride, mb, N, n_free, N, block, budget, held, N, N, N, N, 1, work, N)
     for bad in (dict(n=0), dict(n=1025), dict(rows=0), dict(stride=3), dict(n_free=-1), dict(block=12), dict(budget=15), dict(held=16),
-                dict(mb=5000, stride=5000), dict(mb=5000, stride=5000, work=8)):
+                dict(work=None), dict(work=8)):
         assert trim(**bad) == -1, bad
 
     def rope(Hq=1, Hk=0, dtype=0, N_=1, D=64, rot=64, cu=None, n=0, wide=0, ahead=None, rows=0, on=64):

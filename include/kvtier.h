@@ -412,7 +412,7 @@ int kvt_block_weigh(const void* q, int64_t sq_n, int64_t sq_h, int q_type, const
  * behind.  pos (int32, strides of row and head), held and evicted (int32 by table row), all or none: entry e sits at
  * position pos[e] if e < held, else at e + evicted (none: at e).  recent + sinks <= budget; n * H < 2^22.
  * cap <= 32,768 or <= budget: work may be NULL.  Else work: int32, 16-byte aligned, n * H * (6,156 + 4 c + 2 budget, budget rounded
- * up to even) with c = min(256, ceil(cap / 4,096)), and n * H * c < 2^22; calls that share it must not overlap. */
+ * up to even) with c = max(1, min(256, ceil(cap / 4,096), floor(1,024 / (n * H)))); calls that share it must not overlap. */
 int kvt_block_keep(const void* weights, int64_t sw_r, int64_t sw_h, const void* kv_lens, int n, int H, int n_rows,
                    const void* rows, int64_t cap, int budget, int recent, int sinks, const void* pos, int64_t sp_r,
                    int64_t sp_h, const void* held, const void* evicted, void* src, void* work,

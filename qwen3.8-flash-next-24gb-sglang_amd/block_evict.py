@@ -171,7 +171,8 @@ def kvt_block_keep(weights: torch.Tensor, kv_lens: torch.Tensor, budget: int, se
     ws = {} if workspace is None else workspace             # (held until the launch)
     work, need = None, 0
     if width > 32768 and width > budget:                    # (shorter ones are one workgroup's, in registers)
-        need = n * H * (6144 + 4 * min(256, -(-width // 4096)) + 12 + 2 * (budget + budget % 2))
+        chunks = max(1, min(256, -(-width // 4096), 1024 // (n * H)))
+        need = n * H * (6144 + 4 * chunks + 12 + 2 * (budget + budget % 2))
         work = _grown(ws, "keep", need, weights, torch.int32).data_ptr()
     sp = (0, 0) if pos is None else (pos.stride(0), pos.stride(1))
     _lib.call("kvt_block_keep", weights.data_ptr(), weights.stride(0), weights.stride(1), kv_lens.data_ptr(), n, H, rows,

@@ -17,12 +17,16 @@ namespace {
 // ---------------------------------------------------------------------------------------------------------------- keep
 //
 // The budget-th largest key of a (request, KV head) by radix select (11 + 11 + 10 bits, histograms in LDS), ties to the
-// lowest entry, and the places of what moves, from ranks by ballots.  Up to kSmall entries one workgroup does it all
-// with the keys in registers, read once.  Longer ones take a launch per step, with kMostChunks workgroups a pair at
-// most: three histograms (joined by integer atomics: their order does not matter), counts per chunk, places.  Two pairs
-// of 262,144 entries: 41 us, eight launches' latency (one workgroup a pair, which reads the keys seven times, 742).
+// lowest entry, and the places of what moves, from ranks by ballots.  Up to kSmall entries (kFew: one of 512 threads) one
+// workgroup does it all with the keys in registers, read once.  Longer ones take a launch per step, with kMostChunks
+// workgroups a pair at most: three histograms (joined by integer atomics: their order does not matter), counts per
+// chunk, places.  Lengths are on the device, so a wide table takes all launches, and each leaves the pairs alone that are
+// not its own.  us on the device: 64 x 8 pairs of 4,160 entries 13.3 (by the kernel of 1,024 threads 31), in tables of
+// 16,384 15.4, of 65,536 40.7; two pairs of 8,192 12.7, of 8,256 14.4; of 32,768 29, of 32,769 38; of 262,144 40 (one
+// workgroup a pair, which reads the keys seven times, 742); 64 x 8 of 32,768 62, of 32,769 233.
 constexpr int kKeepThreads = 1024, kWaves = kKeepThreads / 64;
-constexpr int kSmall = 32768, kChunk = 4096, kMostChunks = 256, kBins = 2048;
+constexpr int kFew = 8192, kSmall = 32768, kChunk = 4096, kMostChunks = 256, kBins = 2048;
+constexpr int64_t kChunkBlocks = 1024;        // workgroups of a step's launch, about
 
 struct Keep {
   const float* weights;
@@ -143,22 +147,22 @@ KVT_DEV void find_bin_wave(const int* hist, int k, int& bin, int& left) {
   bin = kBins - 1 - 32 * from - at, left = k - __builtin_amdgcn_readlane(x - n, at);
 }
 
-// One workgroup of T threads per pair of no more than T R entries: wavefront v has entries v * seg .., key i of a lane
+// One workgroup of T threads per pair of more than OVER and no more than T R entries: wavefront v has entries v * seg .., key i of a lane
 // that of entry v * seg + 64 i + lane.  Latency and its instructions bound it: 512 x 4,160 entries, keys re-read from
 // memory by 1,024 threads 39 us, in registers 26, every wavefront finding a histogram's bin for itself instead of three
 // barriers more, 512 threads, 16 (256 threads 20, 1,024 19).
-template <int T, int R>
+template <int T, int R, int OVER>
 __global__ __launch_bounds__(T) void keep_kernel(const Keep P) {
   __shared__ __attribute__((aligned(16))) int hist[3][kPadded];
   __shared__ int sums[2][T / 64];
   __shared__ uint16_t list[T * R / 2];          // (no more than half of the entries can move)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Pair t = pair_of(P, blockIdx.x);
-  if (t.len <= P.budget) {
+  if (OVER == 0 && t.len <= P.budget) {
     for (int e = tid; e < P.budget; e += T) t.src[e] = e < t.len ? e : -1;
     return;
   }
-  if (t.len > T * R) return;                    // (the launches behind this one)
+  if (t.len <= P.budget || t.len <= OVER || t.len > T * R) return;      // (another launch's)
   const int steps = (t.len + T - 1) / T, e0 = wave * 64 * steps + lane;
   uint32_t key[R];
   int place[R];
@@ -782,8 +786,8 @@ extern "C" int kvt_block_keep(const void* weights, int64_t sw_r, int64_t sw_h, c
     return KVT_EINVAL;
   if ((int64_t)recent + sinks > budget || !pos != !held || !pos != !evicted) return KVT_EINVAL;
   const int64_t pairs = (int64_t)n * H;
-  const int chunks = (int)(cap < (int64_t)kMostChunks * kChunk ? (cap + kChunk - 1) / kChunk : kMostChunks);
-  if (cap > ((int64_t)1 << 31) - 8192 || pairs >= 1 << 22 || (cap > kSmall && pairs * chunks >= 1 << 22)) return KVT_ERANGE;
+  const int chunks = (int)max(min(min((cap + kChunk - 1) / kChunk, (int64_t)kMostChunks), kChunkBlocks / pairs), (int64_t)1);
+  if (cap > ((int64_t)1 << 31) - 8192 || pairs >= 1 << 22) return KVT_ERANGE;
   Keep P;
   P.weights = (const float*)weights, P.kv_lens = (const int32_t*)kv_lens, P.rows = (const int32_t*)rows;
   P.pos = (const int32_t*)pos, P.held = (const int32_t*)held, P.evicted = (const int32_t*)evicted;
@@ -793,9 +797,12 @@ extern "C" int kvt_block_keep(const void* weights, int64_t sw_r, int64_t sw_h, c
   if (many && (((uintptr_t)work & 15) || work_ints < pairs * (3 * kBins + 4 * chunks + 12 + 2 * (((int64_t)budget + 1) & ~1))))
     return KVT_EINVAL;
   hipStream_t st = (hipStream_t)stream;
-  if (cap <= 8192) keep_kernel<512, 16><<<(int)pairs, 512, 0, st>>>(P);
-  else keep_kernel<1024, kSmall / 1024><<<(int)pairs, 1024, 0, st>>>(P);
+  keep_kernel<512, kFew / 512, 0><<<(int)pairs, 512, 0, st>>>(P);
   KVT_CHECK_LAUNCH();
+  if (cap > kFew && cap > budget) {
+    keep_kernel<1024, kSmall / 1024, kFew><<<(int)pairs, 1024, 0, st>>>(P);
+    KVT_CHECK_LAUNCH();
+  }
   if (!many) return KVT_OK;
   const int grid = (int)pairs * chunks, blocks = min((budget + 255) / 256, 64);
   keep_clear_kernel<<<(int)pairs, 256, 0, st>>>(P);

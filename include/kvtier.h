@@ -396,14 +396,17 @@ int kvt_rope(const void* q, int64_t sq_n, int64_t sq_h, int Hq, void* out_q, int
  * one that sees a NaN or a block whose scale is not finite makes NaN of every entry that it sees.  The table rows of a
  * call's requests have to be distinct.  Types, sizes and limits of q, k8, ks and the table as kvt_block_decode.
  * work: fp32, 16-byte aligned; with cap = max_blocks * block: cu_q NULL: n * Hq * cap + n * H * splits * 32; else
- * n_q * Hq * 2, splits times that more where splits > 1, and row_splits * n * H * cap where row_splits > 1.  splits (at most 1,024): workgroups that share the entries that a row or a tile of rows sees; row_splits
- * (1,024): those that share a request's rows; pos_splits: those that share its entries.  Results depend on the first two
- * by the order of fp32 sums only.  Calls that share work must not overlap. */
+ * n_q * Hq * 2, splits times that more where splits > 1, and row_splits * n * H * cap where row_splits > 1.
+ * splits and row_splits (at most 1,024): parts that the entries of a tile of rows, and a request's rows, may be divided
+ * into; groups: workgroups of a (request, KV head) in the launch of the sums.  How many of them a chunk uses follows from its
+ * own lengths, fit (workgroups that the chip holds at once) and most (those of a launch, about); the results depend on
+ * them by the order of fp32 sums only.  Calls that share work must not overlap. */
 int kvt_block_weigh(const void* q, int64_t sq_n, int64_t sq_h, int q_type, const void* cu_q, int n_q, const void* kv_lens,
                     int n, int H, int Hq, int D, int code, const void* k8, const void* ks, int n_blocks, int block,
                     const void* block_table, int64_t bt_stride, int n_rows, int max_blocks, const void* rows, float scale,
                     const void* since, const void* weights, int64_t sw_r, int64_t sw_h, void* out, int64_t so_r,
-                    int64_t so_h, int splits, int row_splits, int pos_splits, void* work, int64_t work_floats, void* stream);
+                    int64_t so_h, int splits, int row_splits, int groups, int fit, int most, void* work, int64_t work_floats,
+                    void* stream);
 
 /* The `budget` entries that a request (kv_lens[j] entries, at most cap) keeps of each KV head, into src int32
  * [n, H, budget]: entries below `sinks`, those at positions >= length + evicted - recent, then by weight, equal ones by the

@@ -66,7 +66,7 @@ SIGNATURES = {
     "kvt_rope": [_P, _L, _L, _I, _P, _L, _L, _P, _L, _L, _I, _P, _L, _L, _I, _I, _I, _I, _P, _P, _I, _P, _I, _P, _P, _I,
                  _F, _I, _I, _P],
     "kvt_block_weigh": [_P, _L, _L, _I, _P, _I, _P, _I, _I, _I, _I, _I, _P, _P, _I, _I, _P, _L, _I, _I, _P, _F, _P, _P,
-                        _L, _L, _P, _L, _L, _I, _I, _I, _P, _L, _P],
+                        _L, _L, _P, _L, _L, _I, _I, _I, _I, _I, _P, _L, _P],
     "kvt_block_keep": [_P, _L, _L, _P, _I, _I, _I, _P, _L, _I, _I, _I, _P, _L, _L, _P, _P, _P, _P, _L, _P],
     "kvt_block_evict": [_P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P, _L, _I, _I, _P, _I, _P, _L, _L, _P, _L, _L,
                         _P, _P, _P],

@@ -30,16 +30,16 @@ import torch
 from . import _lib
 from .block_kv import BLOCKS, CODE, FREE_OVER, _apart, _grown, _i32, _overlap, _pool, _rows16, _stream
 
-# Workgroups of the launches.  One query per request: the scores' (at most 256 splits of a pair, whose maxima and sums
-# every workgroup of the sums reads; us per call with 512 / 1,024 / 2,048 / 4,096: 32 requests x 2 heads, D 256, up to 16,384
-# positions 49 / 43 / 45 / 42, int8 64 x 8, D 128, up to 8,191 133 / 96 / 84 / 77) and the sums'.
+# Workgroups of the launches.  One query per request: of the scores (at most 256 splits of a pair, whose maxima and sums
+# every workgroup of the sums reads; us per call with 512 / 1,024 / 2,048 / 4,096: 32 requests x 2 heads, D 256, up to
+# 16,384 positions 49 / 43 / 45 / 42, int8 64 x 8, D 128, up to 8,191 133 / 96 / 84 / 77) and of their sums.
 _ROW_BLOCKS = 4096
-_WORKGROUPS = 4096
 # Chunks: this many where the work allows pieces of 512 positions (rows) at least (1,024 / 2,048 / 4,096 / 8,192: a prompt
-# of 10,001, D 256, 1,071 / 890 / 867 / 890; 8 x 64 queries, D 128, 148 / 143 / 136 / 135), and as many as fit the CUs where it does not
-# (61 queries x 12 heads over 60,000 positions, D 128: 256 64.4, 512 53.5, 768 50.1, 1,024 53.2).
+# of 10,001, D 256, 1,071 / 890 / 867 / 890; 8 x 64 queries, D 128, 148 / 143 / 136 / 135), and as many as fit the CUs
+# where it does not (61 queries x 12 heads over 60,000 positions, D 128: 256 64.4, 512 53.5, 768 50.1, 1,024 53.2).
 _CHUNK_BLOCKS = 4096
 _CHUNK_FIT = {64: 1024, 128: 768, 256: 512}
+_SUMS = 1 << 26          # partial sums of a call at most (256 MB)
 
 
 @dataclass
@@ -101,19 +101,24 @@ def kvt_block_weigh(q: torch.Tensor, k8: torch.Tensor, ks: torch.Tensor, block_t
     st = _stream(q, k8, ks, block_table, kv_lens, weights, cu_q, seqs, since, out)
     q, qp, qn, qh = _rows16(q, 8)
     gs, pairs = Hq // H, n * H
-    row_splits = 1
+    row_splits, fit = 1, 0
     if cu_q is None:
         splits = max(1, min(256, _ROW_BLOCKS // pairs, -(-cap // 256)))
-        pos_splits = max(1, min(_WORKGROUPS // pairs, -(-cap // 1024)))
+        groups = max(1, min(_ROW_BLOCKS // pairs, -(-cap // 1024)))
         need = pairs * gs * cap + pairs * splits * 32
     else:
-        items = rows * gs // 256 + n
-        fit = _CHUNK_FIT[D]
-        splits = min(max(fit // (items * H), min(_CHUNK_BLOCKS // (items * H), cap // 512)), cap // 128, 1024)
-        splits = max(splits, 1)
-        pos_splits = max(1, min(_CHUNK_BLOCKS // pairs, -(-cap // 256)))
-        each = pairs * pos_splits
-        row_splits = max(1, min(1024, max(fit // each, min(_CHUNK_BLOCKS // each, rows * gs // (512 * n)))))
+        # (the most that there may be: the kernels divide each request by its own lengths)
+        items, fit = rows * gs // 256 + n, _CHUNK_FIT[D]
+        splits = max(1, min(max(fit, _CHUNK_BLOCKS) // (items * H), cap // 128, 1024))
+        groups = max(1, _CHUNK_BLOCKS // pairs)
+        tiles = -(-cap // 256)
+        # Splits of the rows need another launch, of 4 to 10 us: for requests that may have 8,192 rows, more than 512 on
+        # average, or more than 128 and tiles that do not fill the CUs (8 x 64 queries x 8 heads over 12,000 positions 138 us
+        # with it, 127 without; 32 x 12 over 4,000 32 with it, 40 without).
+        row_splits = 1
+        if rows * gs >= 8192 or rows * gs > 512 * n or rows * gs > 128 * n and fit >= 2 * pairs * tiles:
+            row_splits = max(1, min(groups, -(-rows * gs // 128), _SUMS // (pairs * cap), 1024))
+        groups = min(groups, tiles * row_splits)
         need = rows * Hq * 2 * (splits + 1) + (row_splits * pairs * cap if row_splits > 1 else 0)
     ws = {} if workspace is None else workspace             # (held until the launch)
     work = _grown(ws, "weigh", need, q)
@@ -121,7 +126,7 @@ def kvt_block_weigh(q: torch.Tensor, k8: torch.Tensor, ks: torch.Tensor, block_t
               CODE[k8.dtype], k8.data_ptr(), ks.data_ptr(), nb, B, block_table.data_ptr(), block_table.stride(0),
               *block_table.shape, _lib.ptr(seqs), D ** -0.5 if scale is None else float(scale), _lib.ptr(since),
               weights.data_ptr(), weights.stride(0), weights.stride(1), out.data_ptr(), out.stride(0), out.stride(1), splits,
-              row_splits, pos_splits, work.data_ptr(), work.numel(), st)
+              row_splits, groups, fit, _CHUNK_BLOCKS, work.data_ptr(), work.numel(), st)
     return out
 
 

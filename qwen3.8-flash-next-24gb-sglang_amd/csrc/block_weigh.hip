@@ -62,7 +62,8 @@ struct Weigh {
   int64_t sq_n, sq_h, stride, sw_r, sw_h, so_r, so_h;
   float scale_log2;
   uint32_t per_gs;             // ceil(2^31 / gs): row / gs is the high half of a product, exact for rows below 2^27
-  int n, n_rows, n_q, H, gs, n_blocks, max_blocks, log2b, splits, row_splits, pos_splits;
+  int n, n_rows, n_q, H, gs, n_blocks, max_blocks, log2b, splits, row_splits, groups;
+  int fit, most;               // chunks: workgroups that the chip holds at once, and of a launch, about
 };
 
 KVT_DEV float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -133,6 +134,16 @@ KVT_DEV int sees(const Req& t, int i) {
   return (int)min((int64_t)t.len, max((int64_t)t.kv - t.q_len + i + 1, (int64_t)0));
 }
 
+// The request, KV head and part of a workgroup.  Parts that a request has no use for are the last ones, so parts are the
+// slow index: the workgroups at work are the first ones, on all CUs alike (the hardware deals them out in turn; with
+// parts as the fast index 32 short requests in a wide table ran on 2 CUs of 32: 25 us against 13).  From part to part
+// the pairs move on by one, so that the parts of a long request are not all on one XCD.
+struct Part { int r, h, k; };
+KVT_DEV Part part_of(const Weigh& P) {
+  const int pairs = P.n * P.H, k = blockIdx.x / pairs, pair = (blockIdx.x - k * pairs + k) % pairs;
+  return {uniform(pair / P.H), uniform(pair % P.H), uniform(k)};
+}
+
 // x and its maximum and sum: a running pair takes another one.
 KVT_DEV void join(float& m, float& l, float m2, float l2) {
   const float M = fmaxf(m, m2);
@@ -155,7 +166,7 @@ __global__ __launch_bounds__(256) void weigh_rows_kernel(const Weigh P) {
   constexpr int NC = D / 64;
   __shared__ float2 J[4][16];
   __shared__ u4v Qs[D / 32][64];
-  const int h = blockIdx.x % P.H, w = blockIdx.x / P.H, split = w % P.splits, r = w / P.splits;
+  const auto [r, h, split] = part_of(P);
   const Req t = request(P, r);
   const int per = per_split(t.len, P.splits);
   const int64_t from = (int64_t)split * per;
@@ -249,7 +260,7 @@ __global__ __launch_bounds__(256) void weigh_rows_kernel(const Weigh P) {
 __global__ __launch_bounds__(256) void weigh_columns_kernel(const Weigh P) {
   __shared__ float2 J[16][16];
   __shared__ float2 norm[16];
-  const int h = blockIdx.x % P.H, w = blockIdx.x / P.H, split = w % P.pos_splits, r = w / P.pos_splits;
+  const auto [r, h, split] = part_of(P);
   const Req t = request(P, r);
   if ((int64_t)split * 1024 >= t.len) return;
   const int64_t pair_id = (int64_t)r * P.H + h, cap = (int64_t)P.max_blocks << P.log2b;
@@ -285,7 +296,7 @@ __global__ __launch_bounds__(256) void weigh_columns_kernel(const Weigh P) {
     norm[threadIdx.x] = (int)threadIdx.x < P.gs ? make_float2(a.x, 1.0f / a.y) : make_float2(kInf, 0.0f);
   }
   __syncthreads();
-  for (bool again = false; base < t.len; base += (int64_t)P.pos_splits * 1024, again = true) {
+  for (bool again = false; base < t.len; base += (int64_t)P.groups * 1024, again = true) {
     const int p = (int)base + 4 * threadIdx.x;
     if (p >= t.len) break;
     if (again) {
@@ -355,6 +366,17 @@ KVT_DEV void products(Read read, const u4v (&held)[2][KS], f16v (&acc)[2]) {
 // Row (of 32) that register i of a 32 x 32 product has in lanes of half hl.
 KVT_DEV int prow(int i, int hl) { return 8 * (i >> 2) + 4 * hl + (i & 3); }
 
+// The host knows the table's width only, which a short request does not fill: how an item's positions, and a request's
+// rows, are divided follows from its own lengths, within what the launch has.
+//
+// Positions of a split of an item whose rows see `limit`: splits of 512 at least, or smaller ones, of 128 at least, as
+// long as the launch does not fill the chip.
+constexpr int kLeast = 9;
+KVT_DEV int per_norm_split(const Weigh& P, int limit, int items) {
+  const int many = max(P.fit / (items * P.H), limit >> kLeast), used = max(min(min(many, P.splits), (limit + 127) >> 7), 1);
+  return max(((limit + kStep - 1) / kStep + used - 1) / used, 1) * kStep;
+}
+
 // Maxima and sums of 256 rows over a split of the positions.  (The reference in the place of the running maximum: 52 of
 // some 290 vector instructions per 64 x 64 scores less, 429 -> 411 us.)
 template <int CODE, int QT, int D>
@@ -371,7 +393,8 @@ __global__ __launch_bounds__(256, 2) void weigh_norm_kernel(const Weigh P, int i
   if (begin < 0 || begin >= n_rows) return;
   const int row0 = (int)begin, live = min(n_rows - row0, kTileRows);
   const int limit = sees(t, query_of(P, row0 + live - 1));
-  const int per = (((limit + kStep - 1) / kStep + P.splits - 1) / P.splits) * kStep;
+  const int per = per_norm_split(P, limit, items);
+  if (split > 0 && (int64_t)split * per >= limit) return;
   const int p_begin = (int)min((int64_t)split * per, (int64_t)limit);
   const int p_end = (int)min((int64_t)p_begin + per, (int64_t)limit);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 31, hl = lane >> 5;
@@ -505,8 +528,10 @@ __global__ __launch_bounds__(256, 2) void weigh_norm_kernel(const Weigh P, int i
     const int mine = 64 * wave + 32 * c + l;
     if (hl == 0 && mine < live) {
       const int64_t at = ((int64_t)h * P.n_q + t.q0) * P.gs + row0 + mine;
-      if (P.splits == 1) P.norm[at] = make_float2(m[c], 1.0f / sum[c]);
-      else P.part[split * ((int64_t)P.H * P.n_q * P.gs) + at] = make_float2(m[c], sum[c]);
+      // (for the join: how many parts the row has)
+      if (split == 0)
+        P.norm[at] = P.splits == 1 ? make_float2(m[c], 1.0f / sum[c]) : make_float2(__int_as_float((limit + per - 1) / per), 0);
+      if (P.splits > 1) P.part[split * ((int64_t)P.H * P.n_q * P.gs) + at] = make_float2(m[c], sum[c]);
     }
   }
 }
@@ -521,8 +546,9 @@ __global__ __launch_bounds__(256) void weigh_join_kernel(const Weigh P) {
   const bool is = i < per_head && query_of(P, i) < P.cu[P.n];      // (padding has no parts)
   float m = -kInf, s = 0.0f;
   if (is) {
+    const int parts = max(__float_as_int(P.norm[at].x), 1);
 #pragma unroll 4
-    for (int k = lane / R; k < P.splits; k += LANES) {
+    for (int k = lane / R; k < parts; k += LANES) {
       const float2 a = P.part[k * total + at];
       join(m, s, a.x, a.y);
     }
@@ -535,8 +561,22 @@ __global__ __launch_bounds__(256) void weigh_join_kernel(const Weigh P) {
   if (is && lane < R) P.norm[at] = make_float2(m, 1.0f / s);
 }
 
-// Rows per split of a request's (query, q head) rows: equal shares in multiples of 64, 128 at least.
-KVT_DEV int per_row_split(int n_rows, int splits) { return max(((n_rows + splits - 1) / splits + 63) & ~63, 128); }
+// How a request's (positions, rows) are divided over the workgroups that it has per KV head: rows in equal splits of
+// multiples of 64, 512 at least, or smaller ones, of 128 at least, as long as the launch does not fill the chip; positions
+// in steps of 256 over `groups` workgroups for each of them.
+struct Cut { int splits, per, groups; };
+KVT_DEV Cut cut(const Weigh& P, const Req& t) {
+  const int n_rows = t.q_len * P.gs, tiles = max((t.len + kTilePos - 1) / kTilePos, 1);
+  Cut c = {1, max((n_rows + 63) & ~63, 64), min(P.groups, tiles)};
+  if (P.row_splits == 1 || n_rows <= 128) return c;
+  const int each = (int)min((int64_t)P.n * P.H * tiles, (int64_t)1 << 30);        // (32-bit divisions)
+  const int many = max(P.fit / each, min(P.most / each, n_rows >> kLeast));
+  c.splits = max(min(min(many, P.row_splits), P.groups / tiles), 1);
+  c.per = max(((n_rows + c.splits - 1) / c.splits + 63) & ~63, 128);
+  c.splits = max((n_rows + c.per - 1) / c.per, 1);
+  c.groups = min(P.groups / c.splits, tiles);
+  return {uniform(c.splits), uniform(c.per), uniform(c.groups)};
+}
 
 // Column sums of 256 positions over a split of the request's rows.  Q's tiles are copied to LDS without a detour by
 // registers: 16-byte chunk c of row i goes to place c ^ (i & 15) (D 64: & 7), so that a column of chunks is spread over
@@ -549,25 +589,23 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void weigh_sums_kernel(const
   // only)
   __shared__ __attribute__((aligned(16))) uint8_t tile0[kStep * 2 * D], tile1[kStep * 2 * D];
   __shared__ __attribute__((aligned(16))) float2 norms0[kStep], norms1[kStep];
-  int w = blockIdx.x;
-  const int split = w % P.pos_splits;
-  w /= P.pos_splits;
-  const int h = w % P.H;
-  w /= P.H;
-  const int rs = w % P.row_splits, r = w / P.row_splits;
+  // (a request's workgroups follow each other, positions first: 16 pairs of 24,000 rows 171 us, with part_of's order 183)
+  const int each = P.H * P.groups, r = blockIdx.x / each, mine = blockIdx.x - r * each;
   const Req t = request(P, r);
-  const int n_rows = t.q_len * P.gs, per = per_row_split(n_rows, P.row_splits);
-  const int r_begin = (int)min((int64_t)rs * per, (int64_t)n_rows), r_end = min(r_begin + per, n_rows);
-  if (r_begin >= r_end && rs > 0) return;
+  const Cut c = cut(P, t);
+  const int w = mine / c.groups, split = mine - w * c.groups, h = w % P.H, rs = w / P.H;
+  if (rs >= c.splits) return;
+  const int n_rows = t.q_len * P.gs, r_begin = min(rs * c.per, n_rows), r_end = min(r_begin + c.per, n_rows);
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), l = lane & 31, hl = lane >> 5;
   const int64_t cap = (int64_t)P.max_blocks << P.log2b;
   const int tr = threadIdx.x / TPR, tc = threadIdx.x % TPR;
   const float2* norm = P.norm + ((int64_t)h * P.n_q + t.q0) * P.gs;
+  const int splits = c.splits;
   const int older = t.kv - t.q_len;           // entries before the queries' own (negative: some queries see nothing)
   // the first row that sees position p (the number of rows where none does)
   auto row_of = [&](int64_t p) { return (int)min(max(p - older, (int64_t)0), (int64_t)t.q_len) * P.gs; };
 
-  for (int64_t p0 = (int64_t)split * kTilePos; p0 < t.len; p0 += (int64_t)P.pos_splits * kTilePos) {
+  for (int64_t p0 = (int64_t)split * kTilePos; p0 < t.len; p0 += (int64_t)c.groups * kTilePos) {
     u4v K[2][KS];
     float f[2], sum[2] = {0, 0};
     int first[2];               // the first row that sees the lane's position
@@ -657,19 +695,19 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void weigh_sums_kernel(const
       float v = sum[c] + __shfl_xor(sum[c], 32, 64);
       if (!there[c]) v = 0.0f;
       if (hl != 0 || p >= t.len) continue;
-      if (P.row_splits == 1) finish(P, t, r, h, (int)p, v);
+      if (splits == 1) finish(P, t, r, h, (int)p, v);
       else P.sums[((int64_t)rs * P.n * P.H + (int64_t)r * P.H + h) * cap + p] = v;
     }
   }
 }
 
 __global__ __launch_bounds__(256) void weigh_add_kernel(const Weigh P) {
-  const int h = blockIdx.x % P.H, w = blockIdx.x / P.H, split = w % P.pos_splits, r = w / P.pos_splits;
+  const auto [r, h, split] = part_of(P);
   const Req t = request(P, r);
-  const int n_rows = t.q_len * P.gs, per = per_row_split(n_rows, P.row_splits);
-  const int used = max((n_rows + per - 1) / per, 1);
+  const int used = cut(P, t).splits;
+  if (used == 1) return;                      // (done)
   const int64_t cap = (int64_t)P.max_blocks << P.log2b, step = (int64_t)P.n * P.H * cap;
-  for (int64_t p = (int64_t)split * 256 + threadIdx.x; p < t.len; p += (int64_t)P.pos_splits * 256) {
+  for (int64_t p = (int64_t)split * 256 + threadIdx.x; p < t.len; p += (int64_t)P.groups * 256) {
     float s = 0.0f;
     for (int k = 0; k < used; ++k) s += P.sums[k * step + ((int64_t)r * P.H + h) * cap + p];
     finish(P, t, r, h, (int)p, s);
@@ -681,7 +719,7 @@ int launch(Weigh P, hipStream_t st) {
   if (!P.cu) {
     weigh_rows_kernel<CODE, QT, D><<<P.n * P.H * P.splits, 256, 0, st>>>(P);
     KVT_CHECK_LAUNCH();
-    weigh_columns_kernel<<<P.n * P.H * P.pos_splits, 256, 0, st>>>(P);
+    weigh_columns_kernel<<<P.n * P.H * P.groups, 256, 0, st>>>(P);
     KVT_CHECK_LAUNCH();
     return KVT_OK;
   }
@@ -694,10 +732,10 @@ int launch(Weigh P, hipStream_t st) {
     else weigh_join_kernel<32><<<dim3((rows + 7) / 8, P.H), 256, 0, st>>>(P);
     KVT_CHECK_LAUNCH();
   }
-  weigh_sums_kernel<CODE, QT, D><<<P.n * P.row_splits * P.H * P.pos_splits, 256, 0, st>>>(P);
+  weigh_sums_kernel<CODE, QT, D><<<P.n * P.H * P.groups, 256, 0, st>>>(P);
   KVT_CHECK_LAUNCH();
   if (P.row_splits > 1) {
-    weigh_add_kernel<<<P.n * P.H * P.pos_splits, 256, 0, st>>>(P);
+    weigh_add_kernel<<<P.n * P.H * P.groups, 256, 0, st>>>(P);
     KVT_CHECK_LAUNCH();
   }
   return KVT_OK;
@@ -722,22 +760,22 @@ extern "C" int kvt_block_weigh(const void* q, int64_t sq_n, int64_t sq_h, int q_
                                int n_blocks, int block, const void* block_table, int64_t bt_stride, int n_rows,
                                int max_blocks, const void* rows, float scale, const void* since, const void* weights,
                                int64_t sw_r, int64_t sw_h, void* out, int64_t so_r, int64_t so_h, int splits,
-                               int row_splits, int pos_splits, void* work, int64_t work_floats, void* stream) {
+                               int row_splits, int groups, int fit, int most, void* work, int64_t work_floats, void* stream) {
   if (n < 1 || n > kMaxReq || H < 1 || Hq < H || Hq % H || Hq / H > 16 || n_q < 0 || n_blocks < 1 || n_rows < 1 ||
       max_blocks < 1 || bt_stride < max_blocks || (!rows && n_rows < n) || (!cu_q && n_q < n))
     return KVT_EINVAL;
   if ((D != 64 && D != 128 && D != 256) || (block != 16 && block != 32 && block != 64)) return KVT_EINVAL;
   if ((code != kE4M3 && code != kI8) || (q_type != kBF16 && q_type != kF16) || !(scale > 0.0f)) return KVT_EINVAL;
   if (((uintptr_t)q | (uintptr_t)k8 | (uintptr_t)work) & 15 || (sq_n | sq_h) & 7) return KVT_EINVAL;
-  if (splits < 1 || splits > kMostSplits || row_splits < 1 || row_splits > kMostSplits || pos_splits < 1)
+  if (splits < 1 || splits > kMostSplits || row_splits < 1 || row_splits > kMostSplits || groups < 1 || fit < 0 || most < 0)
     return KVT_EINVAL;
   const int gs = Hq / H;
   const int64_t cap = (int64_t)max_blocks * block;
   if (cap > kMostPositions) return KVT_ERANGE;
   const int64_t items = (int64_t)n_q * gs / kTileRows + n;
-  const int64_t most = 1 << 24;                                     // (2^32 threads of a launch)
-  if ((cu_q ? items : (int64_t)n) * H * splits >= most || (int64_t)n * H * row_splits * pos_splits >= most ||
-      (int64_t)n_q * gs >= most * 8 || H > 65535)
+  const int64_t top = 1 << 24;                                      // (2^32 threads of a launch)
+  if ((cu_q ? items : (int64_t)n) * H * splits >= top || (int64_t)n * H * groups >= top ||
+      (int64_t)n_q * gs >= top * 8 || H > 65535)
     return KVT_ERANGE;
   const Space s = space(n, n_q, H, gs, cap, cu_q != nullptr, splits, row_splits);
   if (s.scores + s.part + s.norm + s.sums > work_floats) return KVT_EINVAL;
@@ -753,7 +791,7 @@ extern "C" int kvt_block_weigh(const void* q, int64_t sq_n, int64_t sq_h, int q_
   P.n = n, P.n_rows = n_rows, P.n_q = n_q, P.H = H, P.gs = gs, P.n_blocks = n_blocks, P.max_blocks = max_blocks;
   P.log2b = block == 16 ? 4 : block == 32 ? 5 : 6;
   P.per_gs = (uint32_t)((((uint64_t)1 << 31) + gs - 1) / gs);
-  P.splits = splits, P.row_splits = row_splits, P.pos_splits = pos_splits;
+  P.splits = splits, P.row_splits = row_splits, P.groups = groups, P.fit = fit, P.most = most;
   hipStream_t st = (hipStream_t)stream;
   if (code == kE4M3) return q_type == kBF16 ? launch_d<kE4M3, kBF16>(P, D, st) : launch_d<kE4M3, kF16>(P, D, st);
   return q_type == kBF16 ? launch_d<kI8, kBF16>(P, D, st) : launch_d<kI8, kF16>(P, D, st);

@@ -146,16 +146,16 @@ def test_c_entries_refuse(kvt_pkg):
     lib = kvt_pkg._lib.lib()
     N = None
 
-    def weigh(n=1, H=1, Hq=1, D=64, code=0, block=16, max_blocks=4, stride=4, rows=1, scale=1.0, splits=1, rs=1, ps=1,
-              floats=10 ** 6, q_type=0, cu=None, n_q=1, sq=64):
+    def weigh(n=1, H=1, Hq=1, D=64, code=0, block=16, max_blocks=4, stride=4, rows=1, scale=1.0, splits=1, rs=1,
+              groups=1, fit=0, most=0, floats=10 ** 6, q_type=0, cu=None, n_q=1, sq=64):
         return lib.kvt_block_weigh(N, sq, 64, q_type, cu, n_q, N, n, H, Hq, D, code, N, N, 4, block, N, stride, rows, max_blocks,
-                                   N, scale, N, N, 0, 0, N, 0, 0, splits, rs, ps, N, floats, N)
+                                   N, scale, N, N, 0, 0, N, 0, 0, splits, rs, groups, fit, most, N, floats, N)
     for bad in (dict(n=0), dict(n=5000, rows=5000, n_q=5000), dict(Hq=17), dict(H=2, Hq=3), dict(D=96), dict(code=2), dict(block=48),
                 dict(stride=3), dict(n=2), dict(scale=0.0), dict(scale=math.nan), dict(splits=0), dict(splits=2000), dict(rs=0),
-                dict(ps=0), dict(floats=10), dict(q_type=2), dict(sq=63), dict(n_q=0)):
+                dict(groups=0), dict(fit=-1), dict(most=-1), dict(floats=10), dict(q_type=2), dict(sq=63), dict(n_q=0)):
         assert weigh(**bad) == -1, bad
     assert weigh(max_blocks=2 ** 28, stride=2 ** 28) == -3
-    assert weigh(ps=1 << 24) == -3
+    assert weigh(groups=1 << 24) == -3
 
     def keep(n=1, H=1, rows=1, cap=64, budget=16, recent=0, sinks=0, pos=None, held=None, ints=0, work=None):
         return lib.kvt_block_keep(N, 0, 0, N, n, H, rows, N, cap, budget, recent, sinks, pos, 0, 0, held, N, N, work, ints, N)

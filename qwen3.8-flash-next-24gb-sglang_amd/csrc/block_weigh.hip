@@ -546,7 +546,7 @@ __global__ __launch_bounds__(256) void weigh_join_kernel(const Weigh P) {
   const bool is = i < per_head && query_of(P, i) < P.cu[P.n];      // (padding has no parts)
   float m = -kInf, s = 0.0f;
   if (is) {
-    const int parts = max(__float_as_int(P.norm[at].x), 1);
+    const int parts = min(max(__float_as_int(P.norm[at].x), 1), P.splits);  // (rows of no request: anything)
 #pragma unroll 4
     for (int k = lane / R; k < parts; k += LANES) {
       const float2 a = P.part[k * total + at];

@@ -189,6 +189,27 @@ def test_weigh_rows_and_lengths_out_of_range(kvt_pkg):
         ref.weigh_close(w, want, rel)
 
 
+def test_weigh_queries_before_the_first_request(kvt_pkg):
+    """Queries before the first request's are nobody's; what a workspace holds from before does not matter."""
+    from kvtier.block_evict import kvt_block_weigh
+    H, B, D, hq, lens = 2, 16, 64, 8, [1300, 40]
+    sides, table, rows = pool(lens, 90, 2, H, B, D, "fp8", 8)
+    g = torch.Generator().manual_seed(9)
+    prior, cu = torch.rand(2, H, 90 * B, generator=g), [37, 70, 75]
+    q = torch.randn(80, hq, D, generator=g).to(torch.bfloat16)
+    want, rel = ref.weigh(q.double(), cu, lens, rows, table, values(sides[0]), prior.double(), None, D ** -0.5)
+    ws, outs = {}, []
+    for _ in range(2):
+        w = prior.to(dev)
+        kvt_block_weigh(q.to(dev), sides[0][0].to(dev), sides[0][1].to(dev), i32(table), i32(lens), w, i32(cu), i32(rows),
+                        workspace=ws)
+        ref.weigh_close(w, want, rel)
+        outs.append(w)
+        for buffer in ws.values():
+            buffer.fill_(1e9)
+    assert torch.equal(*outs)
+
+
 def test_weigh_of_no_queries(kvt_pkg):
     """An output of its own gets the weights as they are."""
     from kvtier.block_evict import kvt_block_weigh

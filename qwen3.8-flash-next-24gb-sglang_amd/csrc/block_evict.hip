@@ -22,7 +22,7 @@ namespace {
 // workgroups a pair at most: three histograms (joined by integer atomics: their order does not matter), counts per
 // chunk, places.  Lengths are on the device, so a wide table takes all launches, and each leaves the pairs alone that are
 // not its own.  us on the device: 64 x 8 pairs of 4,160 entries 13.3 (by the kernel of 1,024 threads 31), in tables of
-// 16,384 15.4, of 65,536 40.7; two pairs of 8,192 12.7, of 8,256 14.4; of 32,768 29, of 32,769 38; of 262,144 40 (one
+// 16,384 15.9, of 65,536 37.5; two pairs of 8,192 12.6, of 8,256 14.4; of 32,768 30, of 32,769 36; of 262,144 38 (one
 // workgroup a pair, which reads the keys seven times, 742); 64 x 8 of 32,768 62, of 32,769 233.
 constexpr int kKeepThreads = 1024, kWaves = kKeepThreads / 64;
 constexpr int kFew = 8192, kSmall = 32768, kChunk = 4096, kMostChunks = 256, kBins = 2048;
@@ -147,10 +147,10 @@ KVT_DEV void find_bin_wave(const int* hist, int k, int& bin, int& left) {
   bin = kBins - 1 - 32 * from - at, left = k - __builtin_amdgcn_readlane(x - n, at);
 }
 
-// One workgroup of T threads per pair of more than OVER and no more than T R entries: wavefront v has entries v * seg .., key i of a lane
-// that of entry v * seg + 64 i + lane.  Latency and its instructions bound it: 512 x 4,160 entries, keys re-read from
-// memory by 1,024 threads 39 us, in registers 26, every wavefront finding a histogram's bin for itself instead of three
-// barriers more, 512 threads, 16 (256 threads 20, 1,024 19).
+// One workgroup of T threads per pair of more than OVER and no more than T R entries: wavefront v has entries v * seg ..,
+// key i of a lane that of entry v * seg + 64 i + lane.  Latency and its instructions bound it: 512 x 4,160 entries, keys
+// re-read from memory by 1,024 threads 39 us, in registers 26, every wavefront finding a histogram's bin for itself
+// instead of three barriers more, 512 threads, 16 (256 threads 20, 1,024 19).
 template <int T, int R, int OVER>
 __global__ __launch_bounds__(T) void keep_kernel(const Keep P) {
   __shared__ __attribute__((aligned(16))) int hist[3][kPadded];
@@ -160,6 +160,11 @@ __global__ __launch_bounds__(T) void keep_kernel(const Keep P) {
   const Pair t = pair_of(P, blockIdx.x);
   if (OVER == 0 && t.len <= P.budget) {
     for (int e = tid; e < P.budget; e += T) t.src[e] = e < t.len ? e : -1;
+    return;
+  }
+  if (OVER > 0 && t.len > kSmall && t.len > P.budget) {                 // (the launches behind begin with zeros)
+    int32_t* w = P.work + blockIdx.x * work_size(P);
+    for (int i = tid; i < 3 * kBins; i += T) w[i] = 0;
     return;
   }
   if (t.len <= P.budget || t.len <= OVER || t.len > T * R) return;      // (another launch's)
@@ -277,11 +282,6 @@ KVT_DEV bool long_of(const Keep& P, int id, const Pair& t, int c, Long& L) {
   return true;
 }
 
-__global__ __launch_bounds__(256) void keep_clear_kernel(const Keep P) {
-  int32_t* w = P.work + blockIdx.x * work_size(P);
-  for (int i = threadIdx.x; i < 3 * kBins; i += 256) w[i] = 0;
-}
-
 // What pass `pass` found so far: read, or for the pass before formed from its histogram and written (by chunk 0).
 KVT_DEV Found found_before(const Keep& P, const Long& L, int pass, int c, int* sums, int* found) {
   Found f = {0, P.budget, 0, 0};
@@ -395,17 +395,23 @@ __global__ __launch_bounds__(kKeepThreads) void keep_list_kernel(const Keep P) {
   const int e0 = min(L.begin + wave * seg, L.end), e1 = min(e0 + seg, L.end);
   const uint64_t lower = ((uint64_t)1 << lane) - 1;
   int count = 0, all;
+#pragma unroll 4
   for (int e = e0 + lane; e < e1; e += 64) count += t.key(e) == T;
   int ties = start[0] + __shfl(before(count, sums, all), 0, 64);
   auto walk = [&](auto f) {                     // f(entry, whether it is one, whether it stays), the wavefront in step
     int n = ties;
-    for (int base = e0; base < e1; base += 64) {
-      const int e = base + lane;
-      const uint32_t u = e < e1 ? t.key(e) : 0u;
-      const bool tie = e < e1 && u == T;
-      const uint64_t b = __ballot(tie);
-      f(e, e < e1, e < e1 && (u > T || (tie && n + __popcll(b & lower) < k)));
-      n += __popcll(b);
+    for (int base = e0; base < e1; base += 256) {             // (four loads under way at once)
+      uint32_t u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = base + 64 * i + lane < e1 ? t.key(base + 64 * i + lane) : 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = base + 64 * i + lane;
+        const bool tie = e < e1 && u[i] == T;
+        const uint64_t b = __ballot(tie);
+        f(e, e < e1, e < e1 && (u[i] > T || (tie && n + __popcll(b & lower) < k)));
+        n += __popcll(b);
+      }
     }
   };
   int moves = 0, frees = 0;
@@ -805,8 +811,6 @@ extern "C" int kvt_block_keep(const void* weights, int64_t sw_r, int64_t sw_h, c
   }
   if (!many) return KVT_OK;
   const int grid = (int)pairs * chunks, blocks = min((budget + 255) / 256, 64);
-  keep_clear_kernel<<<(int)pairs, 256, 0, st>>>(P);
-  KVT_CHECK_LAUNCH();
   for (int pass = 0; pass < 3; ++pass) {
     keep_hist_kernel<<<grid, kKeepThreads, 0, st>>>(P, pass);
     KVT_CHECK_LAUNCH();

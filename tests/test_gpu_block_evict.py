@@ -112,6 +112,20 @@ def test_weigh(kvt_pkg, case):
     assert torch.equal(a, b)
 
 
+WIDE = [c for c in WEIGH if c[-1] in (2, 4, 12, 14, 15, 16, 17)] + [
+    ([1500, 90, 2600], [1500, 90, 700], 16, 2, 128, 64, "fp8", "bf16", 18),
+    ([3000, 7], [1200, 1], 8, 1, 64, 16, "int8", "f16", 19),
+]
+
+
+@pytest.mark.parametrize("case", WIDE, ids=[str(c[-1]) for c in WIDE])
+def test_weigh_in_wide_tables(kvt_pkg, case):
+    """Requests that fill little of their table, whose width is what the launch is sized by."""
+    ws = {}
+    run_weigh(case, ws=ws, spare=30000 // case[5])
+    run_weigh(case, fresh=True, apart=True, ws=ws, spare=1000 // case[5])
+
+
 @pytest.mark.parametrize("counts", [None, [40, 3, 20]])
 @pytest.mark.parametrize("what", ["gone", "stale", "nan key", "scale", "nan query", "zero"])
 def test_weigh_specials(kvt_pkg, counts, what):

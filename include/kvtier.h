@@ -426,7 +426,8 @@ int kvt_block_keep(const void* weights, int64_t sw_r, int64_t sw_h, const void* 
  * multiple of the block size.  A block that gets another entry takes as scale the smallest power of two that holds its rows'
  * finite values in the codes' range (within 2^-64 .. 2^122) and its rows are rounded to it; one of whose rows has a scale
  * that is not finite becomes NaN with it.  Other blocks are left as they are.  An entry of src that is neither e nor in
- * [budget, kv_lens[j]), or whose block is not there, stays.  n * H * (budget / block + 1) < 2^25; n, H <= 65,535. */
+ * [budget, kv_lens[j]), or whose block is not there, stays.  Rows of requests that are cut have to be distinct, and their
+ * blocks in no other row.  n * H * (budget / block + 1) < 2^25; n, H <= 65,535. */
 int kvt_block_evict(const void* src, const void* kv_lens, int n, int H, int D, int code, void* k8, void* v8, void* ks,
                     void* vs, int n_blocks, int block, const void* block_table, int64_t bt_stride, int n_rows,
                     int max_blocks, const void* rows, int budget, void* weights, int64_t sw_r, int64_t sw_h, void* pos,

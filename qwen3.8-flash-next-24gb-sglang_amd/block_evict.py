@@ -198,7 +198,8 @@ def kvt_block_evict(src: torch.Tensor, kv_lens: torch.Tensor, k8: torch.Tensor, 
     its rows, as if their values were stored anew: exact for e4m3 codes but for those that become subnormal, int8 codes are
     rounded to a scale that grew.  Where a row's scale is not finite, the block's becomes NaN.  An entry of src that is
     neither its own place nor behind the budget and within the length stays where it is.  weights and pos are optional; pos
-    takes held and evicted with it, which kvt_block_trim updates once all layers are done."""
+    takes held and evicted with it, which kvt_block_trim updates once all layers are done.  Rows of seqs have to be
+    distinct (kv_lens of a row that is listed again: 0), and a block may be in one row of the table only."""
     n = kv_lens.numel()
     nb, H, B, D = _pool(k8, v8, ks, vs, block_table, n, seqs)
     assert src.dtype == torch.int32 and src.dim() == 3 and src.is_contiguous(), "src is a contiguous int32 [n, H, budget]"

@@ -178,11 +178,21 @@ def _span(x: torch.Tensor):
 
 
 def _overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
-    """Whether the spans of memory of two tensors meet."""
+    """Whether two tensors share memory: their spans meet, and they are not different columns (heads) of one buffer."""
     if x.numel() == 0 or y.numel() == 0 or x.get_device() != y.get_device():
         return False
     (a, b), (c, d) = _span(x), _span(y)
-    return a < d and c < b
+    if b <= c or d <= a:
+        return False
+    # Of every `every` bytes, x has the first `mine` and y `yours` from `at` on: dimensions whose strides are multiples of
+    # it add nothing.
+    dims = [[((n - 1) * s * t.element_size(), s * t.element_size()) for n, s in zip(t.shape, t.stride()) if n > 1] for t in (x, y)]
+    for every in {s for side in dims for _, s in side if s}:
+        mine, yours = (t.element_size() + sum(length for length, s in side if s % every) for t, side in zip((x, y), dims))
+        at = (c - a) % every
+        if mine <= at and at + yours <= every:
+            return False
+    return True
 
 
 def _rows16(x: torch.Tensor, per16: int):

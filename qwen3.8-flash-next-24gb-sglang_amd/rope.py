@@ -67,9 +67,8 @@ def _output(x: torch.Tensor, out: torch.Tensor, others: Sequence[Optional[torch.
     if out.numel() == 0:
         return
     _apart(out)
-    if out.data_ptr() == x.data_ptr() and _strides(out) == _strides(x):
-        return                                              # in place
-    for y in (x, *others):
+    in_place = out.data_ptr() == x.data_ptr() and _strides(out) == _strides(x)
+    for y in others if in_place else (x, *others):
         if y is not None and _overlap(out, y):
             raise ValueError("an output overlaps an input: pass the input itself (in place), or other memory")
 
@@ -90,7 +89,8 @@ def kvt_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor
              seqs: Optional[torch.Tensor] = None, ahead: Optional[torch.Tensor] = None, inverse: bool = False,
              out_q: Optional[torch.Tensor] = None, out_k: Optional[torch.Tensor] = None):
     """Rotate the first 2 * len(inv_freq) channels of q [N, Hq, D] and k [N, H, D] (bf16 / fp16 / fp32; k may be None) to
-    their positions; returns (out_q, out_k), new tensors unless given.  out_q=q or out_k=k rotates in place.
+    their positions; returns (out_q, out_k), new tensors unless given.  out_q=q or out_k=k rotates in place; outputs share no
+    memory otherwise, with the inputs or each other (parts of one buffer are apart).
 
     Pairs are channels (i, i + rot / 2), or (2 i, 2 i + 1) with interleaved=True; cosines and sines are times `scale`.
     Positions: int32 or int64 [N], of any sign; angles are formed in 64 bits.  With cu (int32 [n + 1]) they are a step's, as

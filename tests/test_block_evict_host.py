@@ -2,6 +2,7 @@
 sizes and tensors off the GPU are errors before anything is launched; rotary frequencies against their formulas."""
 import ctypes
 import math
+import random
 
 import pytest
 import torch
@@ -227,3 +228,56 @@ def test_rotary_frequencies(kvt_pkg):
                 dict(dim=2, method="ntk")):
         with pytest.raises(ValueError):
             rotary_frequencies(**{**dict(dim=8, device="cpu"), **bad})
+
+
+def test_overlaps_are_of_elements(kvt_pkg):
+    """Views of one buffer against the elements that they hold: shared memory is always found, and column ranges, or heads,
+    of one buffer are apart although their spans meet."""
+    from kvtier.block_kv import _overlap
+    rng = random.Random(1)
+    where = torch.arange(4000, dtype=torch.int32)
+
+    def both(x, y):
+        return bool(set(x.flatten().tolist()) & set(y.flatten().tolist()))
+    for _ in range(3000):
+        views = []
+        for _ in range(2):
+            shape = [rng.choice([1, 2, 3, 5]) for _ in range(3)]
+            stride = [rng.choice([3, 8, 24, 40, 41, 64]), rng.choice([2, 4, 8, 13]), 1]
+            views.append(torch.as_strided(where, shape, stride, rng.randrange(80)))
+        assert _overlap(*views) or not both(*views)
+    rows = where[:7 * 240].view(7, 240)
+    parts = [rows[:, a:a + 8 * n].unflatten(1, (n, 8)) for a, n in ((0, 4), (32, 2), (48, 1), (56, 23), (40, 3))]
+    groups = where[:7 * 240].view(7, 10, 24)
+    parts += [groups[..., 0:8], groups[..., 8:16], groups[:, ::2, 16:24], groups[:, 1::2, 16:24]]
+    for x in parts:
+        for y in parts:
+            assert _overlap(x, y) == both(x, y) or x.stride() != y.stride() and not both(x, y)
+    for i, j in ((0, 1), (1, 2), (2, 3), (0, 4), (5, 6), (5, 7), (7, 8)):
+        assert not _overlap(parts[i], parts[j]) and not _overlap(parts[j], parts[i]), (i, j)
+
+
+def test_rope_outputs_and_the_other_tensors(kvt_pkg):
+    """An output in place must be apart from the other tensors too; parts of one buffer are apart (and go on to the
+    device's check)."""
+    x = torch.zeros(3, 6, 64, dtype=torch.bfloat16)
+    for bad in (dict(q=x, k=x[:, :2], out_q=x), dict(q=x, k=x, out_q=x), dict(q=x[:, 2:], k=x[:, 1:3], out_q=x[:, 2:]),
+                dict(q=x[:, :4], k=x[:, 2:4], out_k=x[:, 2:4]), dict(q=x, k=x, out_q=x, out_k=x),
+                dict(q=x[:, :2], k=x[:, 2:4], out_q=x[:, 2:4])):
+        with pytest.raises(ValueError):
+            _rope(**bad)
+    q, k = x[:, :4], x[:, 4:]
+    new = torch.zeros(3, 6, 64, dtype=torch.bfloat16)
+    for good in (dict(out_q=new[:, :4], out_k=new[:, 4:]), dict(q=q, k=k, out_q=q, out_k=k), dict(q=q, k=k, out_q=q),
+                 dict(q=q, k=k, out_q=new[:, 2:], out_k=new[:, :2]), dict(q=x[:, :2], k=x[:, 2:4], out_q=x[:, 4:])):
+        with pytest.raises(AssertionError, match="device tensors"):
+            _rope(**{**(dict(k=k, q=q) if "out_k" in good else {}), **good})
+
+
+def test_weigh_output_beside_its_weights(kvt_pkg):
+    """Sums and weights as parts of one buffer."""
+    w = torch.zeros(2, 2, 2, 48)
+    with pytest.raises(AssertionError, match="device tensors"):
+        _weigh(weights=w[:, 0], out=w[:, 1])
+    with pytest.raises(ValueError):
+        _weigh(weights=w[:, 0], out=w[:, 0, :, 1:].as_strided((2, 2, 47), w[:, 0].stride(), 1))

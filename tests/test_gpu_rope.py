@@ -174,3 +174,26 @@ def test_many_tokens(kvt_pkg):
     pos = torch.arange(n, dtype=torch.int32, device=dev)
     kvt_rope(q, None, pos, inv, scale, out_q=q)
     close(q[-40:], tail, list(range(n - 40, n)), inv, scale, False)
+
+
+@pytest.mark.parametrize("io", ["bf16", "f32"])
+@pytest.mark.parametrize("inter", [False, True])
+def test_outputs_in_one_buffer(kvt_pkg, io, inter):
+    """Both outputs as column ranges of one buffer, as heads in turn, and one of them in place beside the other: the bits
+    of separate outputs, and the rest of the buffer as it was."""
+    from kvtier.rope import kvt_rope, rotary_frequencies
+    n, hq, h, d, rot = 37, 4, 2, 64, 48
+    inv, scale = rotary_frequencies(rot, 1e4)
+    pos = torch.arange(500, 500 + n, device=dev)
+    q, k = rows(n, hq, d, DT[io], 1), rows(n, h, d, DT[io], 2)
+    a, b = kvt_rope(q, k, pos, inv, scale, interleaved=inter)
+    close(a, q, list(range(500, 500 + n)), inv, scale, inter)
+    buf = torch.full((n, hq + 2 * h, d), 3.0, dtype=DT[io], device=dev)
+    kvt_rope(q, k, pos, inv, scale, interleaved=inter, out_q=buf[:, h:h + hq], out_k=buf[:, h + hq:])
+    assert torch.equal(buf, torch.cat((torch.full_like(b, 3.0), a, b), 1))
+    two = torch.full((n, h, 2, d), 3.0, dtype=DT[io], device=dev)
+    kvt_rope(q[:, :h], k, pos, inv, scale, interleaved=inter, out_q=two[:, :, 0], out_k=two[:, :, 1])
+    assert torch.equal(two, torch.stack((a[:, :h], b), 2))
+    buf = torch.cat((q, k, k), 1)
+    kvt_rope(buf[:, :hq], buf[:, hq:hq + h], pos, inv, scale, interleaved=inter, out_q=buf[:, :hq], out_k=buf[:, hq + h:])
+    assert torch.equal(buf, torch.cat((a, k, b), 1))

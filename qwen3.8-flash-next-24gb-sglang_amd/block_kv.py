@@ -173,23 +173,40 @@ def _apart(x: torch.Tensor) -> None:
 
 
 def _span(x: torch.Tensor):
-    first = x.data_ptr()
-    return first, first + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
+    """The first byte of a tensor, the bytes that it spans, and its dimensions' (bytes from first to last entry, stride)."""
+    size = x.element_size()
+    dims = [((n - 1) * s * size, s * size) for n, s in zip(x.shape, x.stride()) if n > 1]
+    span = size
+    for length, _ in dims:
+        span += length
+    return x.data_ptr(), span, dims, size
 
 
 def _overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
     """Whether two tensors share memory: their spans meet, and they are not different columns (heads) of one buffer."""
     if x.numel() == 0 or y.numel() == 0 or x.get_device() != y.get_device():
         return False
-    (a, b), (c, d) = _span(x), _span(y)
-    if b <= c or d <= a:
+    strides = x.stride()
+    if strides == y.stride() and len(strides) == 3:         # (most calls': columns of one buffer, 3 us instead of 7)
+        every, head, unit = strides
+        (_, h, d), (_, h2, d2), size = x.shape, y.shape, x.element_size()
+        if size == y.element_size() and every:
+            at = (y.data_ptr() - x.data_ptr()) % (every * size)
+            if (h - 1) * head + (d - 1) * unit + 1 <= at // size and at + ((h2 - 1) * head + (d2 - 1) * unit + 1) * size <= every * size:
+                return False
+    (a, span_x, dims_x, size_x), (c, span_y, dims_y, size_y) = _span(x), _span(y)
+    if a + span_x <= c or c + span_y <= a:
         return False
     # Of every `every` bytes, x has the first `mine` and y `yours` from `at` on: dimensions whose strides are multiples of
     # it add nothing.
-    dims = [[((n - 1) * s * t.element_size(), s * t.element_size()) for n, s in zip(t.shape, t.stride()) if n > 1] for t in (x, y)]
-    for every in {s for side in dims for _, s in side if s}:
-        mine, yours = (t.element_size() + sum(length for length, s in side if s % every) for t, side in zip((x, y), dims))
-        at = (c - a) % every
+    for _, every in dims_x + dims_y:
+        if every == 0:
+            continue
+        at, mine, yours = (c - a) % every, size_x, size_y
+        for length, s in dims_x:
+            mine += length if s % every else 0
+        for length, s in dims_y:
+            yours += length if s % every else 0
         if mine <= at and at + yours <= every:
             return False
     return True

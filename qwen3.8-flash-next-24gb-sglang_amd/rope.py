@@ -133,7 +133,8 @@ def kvt_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor
     if out_q is not None:
         _output(q, out_q, (k,))
     if out_k is not None:
-        _output(k, out_k, (q, out_q))
+        # (no pair is looked at twice)
+        _output(k, out_k, (q, out_q) if out_q is not q else () if out_k is k else (q,))
     out_q, queries = _side(q, out_q)
     keys = (None, 0, 0, 0, None, 0, 0)
     if k is not None:

@@ -810,7 +810,8 @@ extern "C" int kvt_block_keep(const void* weights, int64_t sw_r, int64_t sw_h, c
     KVT_CHECK_LAUNCH();
   }
   if (!many) return KVT_OK;
-  const int grid = (int)pairs * chunks, blocks = min((budget + 255) / 256, 64);
+  // (a launch has fewer than 2^32 threads; the workgroups of a pair take turns)
+  const int grid = (int)pairs * chunks, blocks = max(min(min((budget + 255) / 256, 64), (int)(((1 << 24) - 1) / pairs)), 1);
   for (int pass = 0; pass < 3; ++pass) {
     keep_hist_kernel<<<grid, kKeepThreads, 0, st>>>(P, pass);
     KVT_CHECK_LAUNCH();

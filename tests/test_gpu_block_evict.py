@@ -369,6 +369,28 @@ def test_keep_rows_and_strides(kvt_pkg):
                 assert got[j, h].tolist() == ref.keep(w[r, 1, h].tolist(), n, 32, 0, 0)
 
 
+def test_keep_of_many_pairs(kvt_pkg):
+    """2^18 pairs of 16,130 entries each: 64 workgroups for each of them would be 2^32 threads.  Few are over the budget,
+    one of them the last pair."""
+    from kvtier.block_evict import kvt_block_keep
+    n, budget, width = 1 << 18, 16_130, 32_800
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("57 GB of sources and workspace")
+    g = torch.Generator().manual_seed(1)
+    w = torch.randint(0, 5000, (1, 1, width), generator=g).float()
+    lens = torch.full((n,), 7, dtype=torch.int32, device=dev)
+    long = {0: 32_790, 70_000: 32_769, 131_072: 20_000, n - 1: 32_800}
+    for j, x in long.items():
+        lens[j] = x
+    src = kvt_block_keep(w.to(dev), lens, budget, torch.zeros(n, dtype=torch.int32, device=dev), 100, 4)
+    for j, x in long.items():
+        assert src[j, 0].tolist() == ref.keep(w[0, 0].tolist(), x, budget, 100, 4)
+    short = torch.full((budget,), -1, dtype=torch.int32, device=dev)
+    short[:7] = torch.arange(7, device=dev)
+    at = torch.arange(1, n - 1, 997, device=dev)
+    assert (src[at[lens[at] == 7], 0] == short).all()
+
+
 @pytest.mark.parametrize("kv", ["fp8", "int8"])
 @pytest.mark.parametrize("H,B,D", [(1, 16, 64), (2, 32, 128), (2, 64, 256), (3, 64, 64), (1, 16, 256), (2, 64, 128)])
 @pytest.mark.parametrize("budget_blocks,share", [(1, 0.5), (4, 0.1), (5, 0.9)])

@@ -395,8 +395,9 @@ int kvt_rope(const void* q, int64_t sq_n, int64_t sq_h, int Hq, void* out_q, int
  * most n_q) are request j's last positions and see the entries up to their own.  A query that sees nothing adds nothing;
  * one that sees a NaN or a block whose scale is not finite makes NaN of every entry that it sees.  The table rows of a
  * call's requests have to be distinct.  Types, sizes and limits of q, k8, ks and the table as kvt_block_decode.
- * work: fp32, 16-byte aligned; with cap = max_blocks * block: cu_q NULL: n * Hq * cap + n * H * splits * 32; else
- * n_q * Hq * 2, splits times that more where splits > 1, and row_splits * n * H * cap where row_splits > 1.
+ * work: fp32, 16-byte aligned; with cap = max_blocks * block: cu_q NULL: Hq * cap + H * splits * 32 for each of the
+ * requests that go at once (as many as work_floats holds, one at least; the others follow in turns); else n_q * Hq * 2,
+ * splits times that more where splits > 1, and row_splits * n * H * cap where row_splits > 1.
  * splits and row_splits (at most 1,024): parts that the entries of a tile of rows, and a request's rows, may be divided
  * into; groups: workgroups of a (request, KV head) in the launch of the sums.  How many of them a chunk uses follows from its
  * own lengths, fit (workgroups that the chip holds at once) and most (those of a launch, about); the results depend on

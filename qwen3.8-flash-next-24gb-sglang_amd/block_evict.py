@@ -40,6 +40,7 @@ _ROW_BLOCKS = 4096
 _CHUNK_BLOCKS = 4096
 _CHUNK_FIT = {64: 1024, 128: 768, 256: 512}
 _SUMS = 1 << 26          # partial sums of a call at most (256 MB)
+_SCORES = 1 << 30        # scores of a call's requests at once (4 GB; of one request at least)
 
 
 @dataclass
@@ -71,7 +72,7 @@ def kvt_block_weigh(q: torch.Tensor, k8: torch.Tensor, ks: torch.Tensor, block_t
     taken back), entries behind kv_lens[j] are left as they are.  A query that sees nothing adds nothing; one that sees a
     NaN, or a block whose scale is not finite, makes NaN of every entry that it sees.  Rows of seqs have to be distinct.
     scale: > 0, default D ** -0.5.  workspace as in kvt_block_decode: its buffers follow from the table's width (one query
-    per request: 4 * Hq bytes per entry of every request)."""
+    per request: 4 * Hq bytes per entry of every request, up to 4 GB, where requests go in turns)."""
     n = kv_lens.numel()
     nb, H, B, D = _pool(k8, k8, ks, ks, block_table, n, seqs)
     assert q.dim() == 3 and q.dtype in (torch.bfloat16, torch.float16), "queries are bf16 or fp16 [rows, Hq, D]"
@@ -103,9 +104,10 @@ def kvt_block_weigh(q: torch.Tensor, k8: torch.Tensor, ks: torch.Tensor, block_t
     gs, pairs = Hq // H, n * H
     row_splits, fit = 1, 0
     if cu_q is None:
-        splits = max(1, min(256, _ROW_BLOCKS // pairs, -(-cap // 256)))
-        groups = max(1, min(_ROW_BLOCKS // pairs, -(-cap // 1024)))
-        need = pairs * gs * cap + pairs * splits * 32
+        at_once = min(n, max(1, _SCORES // (Hq * cap))) if cap else n   # (the others follow, launch after launch)
+        splits = max(1, min(256, _ROW_BLOCKS // (at_once * H), -(-cap // 256)))
+        groups = max(1, min(_ROW_BLOCKS // (at_once * H), -(-cap // 1024)))
+        need = at_once * (Hq * cap + H * splits * 32)
     else:
         # (the most that there may be: the kernels divide each request by its own lengths)
         items, fit = rows * gs // 256 + n, _CHUNK_FIT[D]
@@ -126,7 +128,7 @@ def kvt_block_weigh(q: torch.Tensor, k8: torch.Tensor, ks: torch.Tensor, block_t
               CODE[k8.dtype], k8.data_ptr(), ks.data_ptr(), nb, B, block_table.data_ptr(), block_table.stride(0),
               *block_table.shape, _lib.ptr(seqs), D ** -0.5 if scale is None else float(scale), _lib.ptr(since),
               weights.data_ptr(), weights.stride(0), weights.stride(1), out.data_ptr(), out.stride(0), out.stride(1), splits,
-              row_splits, groups, fit, _CHUNK_BLOCKS, work.data_ptr(), work.numel(), st)
+              row_splits, groups, fit, _CHUNK_BLOCKS, work.data_ptr(), need, st)
     return out
 
 

@@ -718,12 +718,23 @@ __global__ __launch_bounds__(256) void weigh_add_kernel(const Weigh P) {
 }
 
 template <int CODE, int QT, int D>
-int launch(Weigh P, hipStream_t st) {
+int launch(Weigh P, int at_once, hipStream_t st) {
   if (!P.cu) {
-    weigh_rows_kernel<CODE, QT, D><<<P.n * P.H * P.splits, 256, 0, st>>>(P);
-    KVT_CHECK_LAUNCH();
-    weigh_columns_kernel<<<P.n * P.H * P.groups, 256, 0, st>>>(P);
-    KVT_CHECK_LAUNCH();
+    // as many requests at once as the workspace holds scores of
+    for (int n = P.n; n > 0; n -= P.n) {
+      P.n = min(n, at_once);
+      weigh_rows_kernel<CODE, QT, D><<<P.n * P.H * P.splits, 256, 0, st>>>(P);
+      KVT_CHECK_LAUNCH();
+      weigh_columns_kernel<<<P.n * P.H * P.groups, 256, 0, st>>>(P);
+      KVT_CHECK_LAUNCH();
+      P.q = (const uint16_t*)P.q + P.n * P.sq_n, P.kv_lens += P.n;
+      if (P.since) P.since += P.n;
+      if (P.rows) {
+        P.rows += P.n;
+      } else {                                // (request j's row is j)
+        P.table += P.n * P.stride, P.prior += P.n * P.sw_r, P.out += P.n * P.so_r, P.n_rows -= P.n;
+      }
+    }
     return KVT_OK;
   }
   const int items = (int)((int64_t)P.n_q * P.gs / kTileRows) + P.n;
@@ -744,8 +755,9 @@ int launch(Weigh P, hipStream_t st) {
   return KVT_OK;
 }
 template <int CODE, int QT>
-int launch_d(const Weigh& P, int D, hipStream_t st) {
-  return D == 64 ? launch<CODE, QT, 64>(P, st) : D == 128 ? launch<CODE, QT, 128>(P, st) : launch<CODE, QT, 256>(P, st);
+int launch_d(const Weigh& P, int D, int at_once, hipStream_t st) {
+  return D == 64 ? launch<CODE, QT, 64>(P, at_once, st)
+                 : D == 128 ? launch<CODE, QT, 128>(P, at_once, st) : launch<CODE, QT, 256>(P, at_once, st);
 }
 
 // Floats of the workspace's parts: scores or norm, part, sums.
@@ -775,12 +787,16 @@ extern "C" int kvt_block_weigh(const void* q, int64_t sq_n, int64_t sq_h, int q_
   const int gs = Hq / H;
   const int64_t cap = (int64_t)max_blocks * block;
   if (cap > kMostPositions) return KVT_ERANGE;
+  // requests of a launch, and the tiles of rows of a chunk
+  const Space one = space(1, n_q, H, gs, cap, false, splits, row_splits);
+  const int at_once = cu_q ? n : (int)min((int64_t)n, work_floats / (one.scores + one.part));
   const int64_t items = (int64_t)n_q * gs / kTileRows + n;
   const int64_t top = 1 << 24;                                      // (2^32 threads of a launch)
-  if ((cu_q ? items : (int64_t)n) * H * splits >= top || (int64_t)n * H * groups >= top ||
+  if (at_once < 1) return KVT_EINVAL;
+  if ((cu_q ? items : (int64_t)at_once) * H * splits >= top || (int64_t)at_once * H * groups >= top ||
       (int64_t)n_q * gs >= top * 8 || H > 65535)
     return KVT_ERANGE;
-  const Space s = space(n, n_q, H, gs, cap, cu_q != nullptr, splits, row_splits);
+  const Space s = space(at_once, n_q, H, gs, cap, cu_q != nullptr, splits, row_splits);
   if (s.scores + s.part + s.norm + s.sums > work_floats) return KVT_EINVAL;
   Weigh P;
   P.q = q, P.k8 = (const uint8_t*)k8, P.ks = (const float*)ks, P.table = (const int32_t*)block_table;
@@ -796,6 +812,6 @@ extern "C" int kvt_block_weigh(const void* q, int64_t sq_n, int64_t sq_h, int q_
   P.per_gs = (uint32_t)((((uint64_t)1 << 31) + gs - 1) / gs);
   P.splits = splits, P.row_splits = row_splits, P.groups = groups, P.fit = fit, P.most = most;
   hipStream_t st = (hipStream_t)stream;
-  if (code == kE4M3) return q_type == kBF16 ? launch_d<kE4M3, kBF16>(P, D, st) : launch_d<kE4M3, kF16>(P, D, st);
-  return q_type == kBF16 ? launch_d<kI8, kBF16>(P, D, st) : launch_d<kI8, kF16>(P, D, st);
+  if (code == kE4M3) return q_type == kBF16 ? launch_d<kE4M3, kBF16>(P, D, at_once, st) : launch_d<kE4M3, kF16>(P, D, at_once, st);
+  return q_type == kBF16 ? launch_d<kI8, kBF16>(P, D, at_once, st) : launch_d<kI8, kF16>(P, D, at_once, st);
 }

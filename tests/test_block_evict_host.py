@@ -281,3 +281,21 @@ def test_weigh_output_beside_its_weights(kvt_pkg):
         _weigh(weights=w[:, 0], out=w[:, 1])
     with pytest.raises(ValueError):
         _weigh(weights=w[:, 0], out=w[:, 0, :, 1:].as_strided((2, 2, 47), w[:, 0].stride(), 1))
+
+
+def test_weigh_workspace_is_bounded(kvt_pkg, monkeypatch):
+    """One query per request: the scores of as many requests as 2^30 floats hold, of one at least; what the call is given
+    is what it asked for, whatever a workspace held before."""
+    from kvtier import block_evict
+    asked = []
+    monkeypatch.setattr(block_evict, "_stream", lambda *x: 0)
+    monkeypatch.setattr(block_evict._lib, "call", lambda name, *x: asked.append((name, x[-2])))
+    monkeypatch.setattr(block_evict, "_grown", lambda ws, what, need, like, *x: asked.append(need) or torch.zeros(1))
+    p = _pool(H=1)
+    for n, hq, blocks, most in ((2, 16, 3, 2), (80, 16, 1 << 16, 64), (3, 16, 1 << 23, 1)):
+        cap = 16 * blocks
+        asked.clear()
+        _weigh(q=torch.zeros(n, hq, 64, dtype=torch.bfloat16), k8=p["k8"], ks=p["ks"], kv_lens=torch.zeros(n, dtype=torch.int32),
+               block_table=torch.empty(n, blocks, dtype=torch.int32), weights=torch.empty(n, 1, cap))
+        assert most * hq * cap < asked[0] <= most * (hq * cap + 256 * 32), (n, asked)
+        assert asked[1] == ("kvt_block_weigh", asked[0])

@@ -272,6 +272,35 @@ def test_weigh_scores_far_apart(kvt_pkg, counts, scale, order):
                               atol=0)
 
 
+@pytest.mark.parametrize("at_once", [1, 2, 3, 100])
+def test_weigh_requests_in_turns(kvt_pkg, monkeypatch, at_once):
+    """Scores of a few requests at once: with rows and without, strides, given `since`; a workspace that an earlier call
+    left larger changes nothing."""
+    from kvtier import block_evict
+    lens, hq, H, B, D = [700, 0, 65, 1500, 16, 333, 1], 12, 2, 32, 128
+    n, mb = len(lens), 47
+    monkeypatch.setattr(block_evict, "_SCORES", at_once * hq * mb * B)
+    case = (lens, None, hq, H, D, B, "fp8", "bf16", 61)
+    ws = {}
+    outs = [run_weigh(case, fresh=True, apart=True, ws=w) for w in (ws, ws, {("weigh", 0): torch.empty(1 << 24, device=dev)}, None)]
+    run_weigh(case, ws=ws)
+    assert all(torch.equal(outs[0], x) for x in outs)
+    sides, table, rows = pool(lens, mb, n, H, B, D, "int8", 62)
+    table = [table[r] for r in rows]                       # (request j's row is j; one row more than requests)
+    table.append([-1] * mb)
+    g = torch.Generator().manual_seed(63)
+    q = torch.randn(n, hq, D, generator=g).to(torch.float16)
+    prior = torch.rand(n + 1, H, 2, mb * B, generator=g)
+    since = [100, 0, 65, 7, 16, 332, 1]
+    want, rel = ref.weigh(q.double(), list(range(n + 1)), lens, list(range(n)), table, values(sides[0]), prior[:, :, 1].double(),
+                          since, D ** -0.5)
+    w = prior.to(dev)
+    block_evict.kvt_block_weigh(q.to(dev), sides[0][0].to(dev), sides[0][1].to(dev), i32(table), i32(lens), w[:, :, 1],
+                                since=i32(since))
+    ref.weigh_close(w[:, :, 1], want, rel)
+    assert torch.equal(w[:, :, 0].cpu(), prior[:, :, 0])
+
+
 def test_weigh_far_offsets(kvt_pkg):
     """Code offsets past 2^31 bytes and weight offsets past 2^31 entries."""
     from kvtier.block_evict import kvt_block_weigh

@@ -301,6 +301,59 @@ def test_weigh_requests_in_turns(kvt_pkg, monkeypatch, at_once):
     assert torch.equal(w[:, :, 0].cpu(), prior[:, :, 0])
 
 
+LONG = [
+    # lens, counts (None: one query each), hq, H, D, B, kv, io, seed
+    ([9001, 5003, 1025], None, 8, 2, 64, 16, "fp8", "bf16", 71),
+    ([8197, 300], None, 12, 1, 256, 64, "int8", "f16", 72),
+    ([4099], None, 32, 2, 128, 32, "int8", "bf16", 73),
+    ([2501, 777, 1300], [100, 3, 61], 8, 2, 64, 16, "fp8", "bf16", 74),
+    ([2501, 1100], [101, 40], 12, 1, 256, 64, "int8", "bf16", 75),
+    ([1800, 2100], [1800, 33], 4, 2, 128, 32, "int8", "f16", 76),
+    ([2309], [2309], 2, 1, 256, 64, "fp8", "f16", 77),
+    ([1300] * 3, [700, 0, 1300], 16, 1, 64, 64, "int8", "bf16", 78),
+]
+
+
+@pytest.mark.parametrize("case", LONG, ids=[str(c[-1]) for c in LONG])
+def test_weigh_by_few_workgroups(kvt_pkg, monkeypatch, case):
+    """As few workgroups as many requests over long tables leave each pair: one split over more than 4,096 positions (one
+    query) or 1,024 (chunks), whose ids and scales are read again on the way, and workgroups of the sums that take
+    1,024 positions, or 256 of a chunk, after others."""
+    from kvtier import block_evict
+    monkeypatch.setattr(block_evict, "_ROW_BLOCKS", 1)
+    monkeypatch.setattr(block_evict, "_CHUNK_BLOCKS", 1)
+    monkeypatch.setattr(block_evict, "_CHUNK_FIT", {64: 1, 128: 1, 256: 1})
+    ws = {}
+    a = run_weigh(case, fresh=True, apart=True, ws=ws)
+    b = run_weigh(case, fresh=True, apart=True, ws=ws)
+    assert torch.equal(a, b)
+    run_weigh(case, spare=5)
+
+
+@pytest.mark.parametrize("groups,splits", [(2, 1), (3, 2), (5, 7)])
+def test_weigh_by_some_workgroups(kvt_pkg, groups, splits):
+    """The same by the C entry's own numbers: several groups and splits, each of which takes more than one turn."""
+    from kvtier import _lib
+    H, hq, D, B = 2, 8, 64, 32
+    for lens, counts, code, kv in (([9001, 2600], None, 0, "fp8"), ([3500, 1500], [150, 40], 1, "int8")):
+        max_blocks = -(-max(lens) // B)
+        sides, table, rows = pool(lens, max_blocks, 2, H, B, D, kv, 81)
+        g = torch.Generator().manual_seed(82)
+        cu = prefix(counts or [1, 1])
+        q = torch.randn(cu[-1], hq, D, generator=g).to(torch.bfloat16)
+        prior = torch.rand(2, H, max_blocks * B, generator=g)
+        want, rel = ref.weigh(q.double(), cu, lens, rows, table, values(sides[0]), prior.double(), None, D ** -0.5)
+        w, qd, k8, ks, t = prior.to(dev), q.to(dev), sides[0][0].to(dev), sides[0][1].to(dev), i32(table)
+        floats = 2 * (hq * max_blocks * B + H * splits * 32) if counts is None else cu[-1] * hq * 2 * (splits + 1)
+        work, n, c, r = torch.empty(floats, device=dev), i32(lens), i32(cu), i32(rows)
+        _lib.call("kvt_block_weigh", qd.data_ptr(), hq * D, D, _lib.DTYPE_CODE[q.dtype], c.data_ptr() if counts else None,
+                  cu[-1], n.data_ptr(), 2, H, hq, D, code, k8.data_ptr(), ks.data_ptr(), k8.shape[0], B, t.data_ptr(), max_blocks,
+                  2, max_blocks, r.data_ptr(), D ** -0.5, None, w.data_ptr(), w.stride(0), w.stride(1), w.data_ptr(),
+                  w.stride(0), w.stride(1), splits, 1, groups, 0, 1, work.data_ptr(), floats,
+                  torch.cuda.current_stream().cuda_stream)
+        ref.weigh_close(w, want, rel)
+
+
 def test_weigh_far_offsets(kvt_pkg):
     """Code offsets past 2^31 bytes and weight offsets past 2^31 entries."""
     from kvtier.block_evict import kvt_block_weigh

@@ -354,6 +354,54 @@ def test_weigh_by_some_workgroups(kvt_pkg, groups, splits):
         ref.weigh_close(w, want, rel)
 
 
+@pytest.mark.parametrize("counts", [None, [90, 2, 300], [1300, 2, 61]])
+@pytest.mark.parametrize("few", [False, True])
+@pytest.mark.parametrize("shape", ["1", "1/4", "16", "90 a tile", "91 a tile", "a jump", "waves"])
+def test_weigh_of_exact_scores(kvt_pkg, monkeypatch, counts, few, shape):
+    """Whole scores in powers of two, up to some 40,000 and exact in 32 bits, that rise along the entries for one q head, fall
+    for the second, and neither for the others: every weight within what exponential, sums and quotient round."""
+    from kvtier import block_evict
+    if few:
+        monkeypatch.setattr(block_evict, "_ROW_BLOCKS", 1)
+        monkeypatch.setattr(block_evict, "_CHUNK_BLOCKS", 1)
+        monkeypatch.setattr(block_evict, "_CHUNK_FIT", {64: 1})
+    lens, H, B, D, hq = [2501, 70, 1400], 2, 32, 64, 8
+    max_blocks = 80
+    rise = {"1": lambda p: p, "1/4": lambda p: p // 4, "16": lambda p: 16 * p, "90 a tile": lambda p: p // 64 * 90,
+            "91 a tile": lambda p: p // 64 * 91, "a jump": lambda p: 30_000 * (p > 1000), "waves": lambda p: abs(p % 700 - 350) * 3}[shape]
+    sides, table, rows = pool(lens, max_blocks, 4, H, B, D, "fp8", 91)
+    g = torch.Generator().manual_seed(92)
+    # channels 0 .. 3: a position's rise in digits of 16, times 1, 16, 256, 4,096 by the query; 4 .. 11: noise.  Blocks of
+    # scale 1 / 2 hold twice the value: all of it is exact in e4m3
+    k8 = torch.zeros(len(sides[0][1]), H, B, D)
+    ks = torch.exp2(-torch.randint(0, 2, sides[0][1].shape, generator=g).float())
+    k8[..., 4:12] = torch.randint(-1, 2, (*k8.shape[:3], 8), generator=g).float()
+    for r, n in zip(rows, lens):
+        for p in range(n):
+            v = rise(p)
+            k8[table[r][p // B], :, p % B, :4] = torch.tensor([float(v >> 4 * i & 15) for i in range(4)])
+    k8 = (k8 / ks[..., None, None]).to(torch.float8_e4m3fn)
+    m = counts or [1, 1, 1]
+    cu = prefix(m)
+    q = torch.zeros(cu[-1], hq, D)
+    q[..., 4:12] = torch.randint(-1, 2, (cu[-1], hq, 8), generator=g).float()
+    for h in range(hq):
+        q[:, h, :4] = torch.tensor([1.0, 16.0, 256.0, 4096.0]) * (1, -1, 0, 0)[h % 4]
+    q = q.to(torch.bfloat16)
+    prior = torch.rand(4, H, max_blocks * B, generator=g)
+    # (the scale is ln 2: in fp32 its product with log2 e rounds to 1)
+    assert float(torch.tensor(math.log(2), dtype=torch.float32) * torch.tensor(1 / math.log(2), dtype=torch.float32)) == 1.0
+    want, _ = ref.weigh(q.double(), cu, lens, rows, table, values((k8, ks)), prior.double(), None, math.log(2))
+    # exponential and quotient, and sums of up to `length` and of m * g terms; weights under 2^-99 are as good as none
+    rel = torch.zeros_like(want)
+    for r, n, c in zip(rows, lens, m):
+        rel[r] = (n + c * hq // H) * 2.0 ** -24 + 2.0 ** -20
+    w = prior.to(dev)
+    block_evict.kvt_block_weigh(q.to(dev), k8.to(dev), ks.to(dev), i32(table), i32(lens), w, None if counts is None else i32(cu),
+                                i32(rows), scale=math.log(2))
+    ref.weigh_close(w, want, rel)
+
+
 def test_weigh_far_offsets(kvt_pkg):
     """Code offsets past 2^31 bytes and weight offsets past 2^31 entries."""
     from kvtier.block_evict import kvt_block_weigh

@@ -843,3 +843,36 @@ def test_streams_of_their_own(kvt_pkg):
         torch.cuda.synchronize()
         for (a, b), (c, d) in zip(done, want):
             assert torch.equal(a, c) and torch.equal(b, d)
+
+
+def test_streams_with_a_workspace_each(kvt_pkg):
+    """Calls of two streams at once that use their workspaces: chunks in splits, single queries, a choice of more than
+    32,768 entries; over and over into the same buffers."""
+    from kvtier.block_evict import kvt_block_keep, kvt_block_weigh
+    lens, H, B, D, hq, width = [36_000, 900], 1, 64, 64, 8, 40_000
+    sides, table, rows = pool(lens, width // B, 2, H, B, D, "fp8", 3)
+    g = torch.Generator().manual_seed(6)
+    k8, ks = sides[0][0].to(dev), sides[0][1].to(dev)
+    t, n, r, cu = i32(table), i32(lens), i32(rows), i32([0, 30, 41])
+    qs = [torch.randn(41, hq, D, generator=g).to(torch.bfloat16).to(dev) for _ in range(2)]
+
+    def calls(q, ws):
+        w = torch.zeros(2, H, width, device=dev)
+        kvt_block_weigh(q, k8, ks, t, n, w, cu, r, workspace=ws)
+        kvt_block_weigh(q[:2], k8, ks, t, n, w, seqs=r, workspace=ws)
+        return w, kvt_block_keep(w, n, 2048, r, 20, 4, workspace=ws)
+    want = [calls(q, {}) for q in qs]
+    torch.cuda.synchronize()
+    assert not torch.equal(want[0][1], want[1][1])
+    streams, wss = [torch.cuda.Stream() for _ in range(2)], [{}, {}]
+    for _ in range(10):
+        done = []
+        for q, s, ws in zip(qs, streams, wss):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                done.append(calls(q, ws))
+        torch.cuda.synchronize()
+        for (a, b), (c, d) in zip(done, want):
+            assert torch.equal(a, c) and torch.equal(b, d)
+    # (the caching allocator knows no other stream's use: the workspaces are each its own)
+    assert all(k in ws for ws in wss for k in (("weigh", 0), ("keep", 0)))

@@ -652,6 +652,7 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void weigh_sums_kernel(const
       if (r0 + kStep < r_end) copy(r0 + kStep, next_tile, next_norms);
       auto take = [&](auto masked) {
         constexpr bool EDGE = decltype(masked)::value;
+        float more[2] = {0, 0};               // (a tile's own sum: long columns lose less)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           f16v acc[2] = {};
@@ -673,10 +674,11 @@ __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void weigh_sums_kernel(const
                   const bool is = (row + j >= first[c]) & (row + j < r_end);
                   x = is ? x : -kInf, li = is ? li : 0.0f;
                 }
-                sum[c] = fmaf(exp2_(x), li, sum[c]);
+                more[c] = fmaf(exp2_(x), li, more[c]);
               }
           }
         }
+        sum[0] += more[0], sum[1] += more[1];
       };
       if (r0 + kStep > some) {
         if (__builtin_expect(r0 < all || r0 + kStep > r_end, 0)) {

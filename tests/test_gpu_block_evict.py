@@ -402,6 +402,32 @@ def test_weigh_of_exact_scores(kvt_pkg, monkeypatch, counts, few, shape):
     ref.weigh_close(w, want, rel)
 
 
+@pytest.mark.parametrize("D,few", [(64, True), (128, True), (256, True), (64, False)])
+def test_weigh_long_columns(kvt_pkg, monkeypatch, D, few):
+    """8,192 rows that all pay 1 / 37 to the same 37 entries (the others' weights are 2^-192): sums are formed by tiles of 64
+    rows, and lose no more than that."""
+    from kvtier import block_evict
+    if few:
+        monkeypatch.setattr(block_evict, "_CHUNK_BLOCKS", 1)
+        monkeypatch.setattr(block_evict, "_CHUNK_FIT", {64: 1, 128: 1, 256: 1})
+    m, hq, H, B, top = 2048, 4, 1, 64, 37
+    n = m + top
+    nb = -(-n // B)
+    k8 = torch.zeros(nb, H, B, D)
+    k8.view(nb * B, D)[top:, 0] = -192.0
+    k8 = k8.to(torch.float8_e4m3fn)
+    q = torch.zeros(m, hq, D, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    w = torch.full((1, H, nb * B), 9.0, device=dev)
+    block_evict.kvt_block_weigh(q.to(dev), k8.to(dev), torch.ones(nb, H, device=dev), i32([list(range(nb))]), i32([n]), w, i32([0, m]),
+                                since=i32([0]), scale=math.log(2))
+    # Scores, exponentials and a row's sum, 37, are exact; one rounding of 1 / 37, 32 sums of a lane in a tile, one for each
+    # of at most 128 tiles (splits are joined by fewer), one of a lane's two halves.
+    got = w[0, 0, :n].double().cpu()
+    assert ((got[:top] * top / (m * hq) - 1).abs() <= (1 + 32 + 128 + 1) * 2.0 ** -24).all(), float((got[:top] * top / (m * hq) - 1).abs().max())
+    assert (got[top:] == 0).all() and (w[0, 0, n:] == 9).all()
+
+
 def test_weigh_far_offsets(kvt_pkg):
     """Code offsets past 2^31 bytes and weight offsets past 2^31 entries."""
     from kvtier.block_evict import kvt_block_weigh

@@ -37,10 +37,14 @@ _ROW_BLOCKS = 4096
 # Chunks: this many where the work allows pieces of 512 positions (rows) at least (1,024 / 2,048 / 4,096 / 8,192: a prompt
 # of 10,001, D 256, 1,071 / 890 / 867 / 890; 8 x 64 queries, D 128, 148 / 143 / 136 / 135), and as many as fit the CUs
 # where it does not (61 queries x 12 heads over 60,000 positions, D 128: 256 64.4, 512 53.5, 768 50.1, 1,024 53.2).
+# (D 64: four workgroups a CU, three with int8 codes and fp16 queries, where 8 x 64 queries x 64 / 8 heads over 12,000
+# positions take 183 / 181 / 183 us with 512 / 768 / 1,024.)
 _CHUNK_BLOCKS = 4096
 _CHUNK_FIT = {64: 1024, 128: 768, 256: 512}
 _SUMS = 1 << 26          # partial sums of a call at most (256 MB)
-_SCORES = 1 << 30        # scores of a call's requests at once (4 GB; of one request at least)
+# Scores of a call's requests at once (4 GB; of one request at least).  256 requests x 64 / 8 heads that hold 4,160 entries,
+# D 128, in tables of 262,144: 486 us in turns of 1 GB, 373 of 4 GB, 369 all at once (17 GB).
+_SCORES = 1 << 30
 
 
 @dataclass

@@ -21,9 +21,10 @@ namespace {
 // workgroup does it all with the keys in registers, read once.  Longer ones take a launch per step, with kMostChunks
 // workgroups a pair at most: three histograms (joined by integer atomics: their order does not matter), counts per
 // chunk, places.  Lengths are on the device, so a wide table takes all launches, and each leaves the pairs alone that are
-// not its own.  us on the device: 64 x 8 pairs of 4,160 entries 13.3 (by the kernel of 1,024 threads 31), in tables of
-// 16,384 15.9, of 65,536 37.5; two pairs of 8,192 12.6, of 8,256 14.4; of 32,768 30, of 32,769 36; of 262,144 38 (one
-// workgroup a pair, which reads the keys seven times, 742); 64 x 8 of 32,768 62, of 32,769 233.
+// not its own.  us a call, calls in a row: 64 x 8 pairs of 4,160 entries to 4,096 13.6 (14.2 with positions; by the kernel
+// of 1,024 threads 31), in tables of 16,384 16.4, of 65,536 38; nothing over the budget 3.6 and 28; two pairs of 8,192 13.3,
+// of 8,256 20, of 32,768 33, of 32,769 36; of 262,144 to 16,384 40 (one workgroup a pair, which reads the keys seven times,
+// 742); 64 x 8 of 16,384 47, of 32,768 68, of 32,769 236 (every key read seven times, by one or two workgroups a pair).
 constexpr int kKeepThreads = 1024, kWaves = kKeepThreads / 64;
 constexpr int kFew = 8192, kSmall = 32768, kChunk = 4096, kMostChunks = 256, kBins = 2048;
 constexpr int64_t kChunkBlocks = 1024;        // workgroups of a step's launch, about
@@ -150,7 +151,8 @@ KVT_DEV void find_bin_wave(const int* hist, int k, int& bin, int& left) {
 // One workgroup of T threads per pair of more than OVER and no more than T R entries: wavefront v has entries v * seg ..,
 // key i of a lane that of entry v * seg + 64 i + lane.  Latency and its instructions bound it: 512 x 4,160 entries, keys
 // re-read from memory by 1,024 threads 39 us, in registers 26, every wavefront finding a histogram's bin for itself
-// instead of three barriers more, 512 threads, 16 (256 threads 20, 1,024 19).
+// instead of three barriers more, 512 threads, 16 (256 threads 20, 1,024 19).  More than 8,192 entries: 101 registers at
+// 1,024 threads, so one workgroup a CU and nothing behind its barriers (512 x 32,768 entries 68, 67 MB of weights).
 template <int T, int R, int OVER>
 __global__ __launch_bounds__(T) void keep_kernel(const Keep P) {
   __shared__ __attribute__((aligned(16))) int hist[3][kPadded];

@@ -6,23 +6,27 @@
 // rows have to be complete before any column can be.
 //
 // One query per request (a (request, KV head) has at most 16 rows): the scores are formed once, by 16 x 16 products
-// with K's codes from registers as they were loaded, and kept as fp32 (4 Hq / H bytes an entry against D bytes of
-// codes: less than a second read of K); a second launch joins the splits' maxima and sums and adds up the columns. 
-// Bytes bound both: 32 requests x 2 heads, D 256, up to 16,384 entries (103 MB of codes, 19 MB of scores written and
-// read) 31 + 9 us; int8, 64 x 8 heads, D 128, blocks of 16 (195 + 49 MB) 57 + 17, 4.3 TB/s.  (Tiles of 64 positions a
+// with K's codes from registers as they were loaded, and kept as fp32; a second launch joins the splits' maxima and sums
+// and adds up the columns.  With gs q heads a KV head they are 8 gs bytes an entry, written and read back, against D bytes
+// of codes for a second read of K: less up to gs 8 at D 64 and 16 at D 128, where they are as much; twice as much at D 64
+// with gs 16, which is served alike.  Bytes bound both: 32 requests x 2 heads, D 256, up to 16,384 entries (103 MB of codes,
+// 19 MB of scores written and read) 31 + 9 us; int8, 64 x 8 heads, D 128, blocks of 16 (195 + 49 MB) 60 + 17, 4.1 TB/s;
+// 32 requests of 8,000, 4 heads of gs 8, D 64 (66 MB of codes, 33 of scores) 32 together.  (Tiles of 64 positions a
 // wavefront instead of 32: 57 -> 64; of 16: 59.)
 //
 // Chunks: a row has too many scores to keep, so they are formed twice.  The first launch holds 256 rows of Q in
 // registers (64 a wavefront) and streams K through LDS for maxima and sums; each lane keeps them for a row of its own,
 // over the positions that it sees, so that nothing crosses lanes in the loop.  The second one holds 256 positions of K
 // in registers and streams Q; a lane adds up the weights of its position.  Splits are joined in their order by launches
-// of their own: no atomics, the same bits for every call.  64 rows (positions) a wavefront are what 256 registers hold
-// at D 256 with two wavefronts a SIMD, and halve the reads of the streamed tile against 32.  A prompt of 10,001 tokens,
-// 16 / 2 heads, D 256 (410 GFLOP a launch): 411 + 470 us, 998 and 872 TFLOP/s (a large library product 1,247); the
-// steps there: 856 + 1,405 with one wavefront a SIMD, 64-bit divisions for the rows and masks for every tile; 497 + 541
-// without the first two; 460 + 495 with operands read ahead of their products and Q copied straight to LDS; 429 with
-// masks by wavefront.  Exponentials and products take as long as each other at D 256; at D 128 and 64 the exponentials
-// bound it.
+// of their own: no atomics, the same bits for every call.  64 rows (positions) a wavefront, which halve the reads of the
+// streamed tile against 32, are about what 256 registers hold at D 256 with two wavefronts a SIMD, and 168 at D 128 with
+// three: the second kernel spills two registers at both (four with int8 and fp16).  A prompt of
+// 10,001 tokens, 16 / 2 heads, D 256 (410 GFLOP a launch): 424 + 488 us, 967 and 840 TFLOP/s (a large library product
+// 1,241); the steps there: 856 + 1,405 with one wavefront a SIMD, 64-bit divisions for the rows and masks for every tile;
+// 497 + 541 without the first two; 460 + 495 with operands read ahead of their products and Q copied straight to LDS; 429
+// with masks by wavefront.  Vector instructions (6.5 and 7.4 a product at D 256, 13 at D 128, exponentials at a quarter of
+// the rate among them) take about as long as the products at D 256, and more than twice as long at D 128: they bound it
+// there and at D 64.
 //
 // Operands have q's type (codes of 8 bits are exact in bf16 and fp16); scores, maxima, sums and weights are fp32.
 #include <type_traits>
@@ -160,8 +164,8 @@ KVT_DEV void finish(const Weigh& P, const Req& t, int r, int h, int p, float sum
   P.out[t.trow * P.so_r + h * P.so_h + p] = sum;
 }
 
-// ------------------------------------------------------------------------------------------------- one query per
-// request Positions per split: equal shares in multiples of 128 (a tile of 32 for each wavefront), 256 at least.
+// ------------------------------------------------------------------------------------------- one query per request
+// Positions per split: equal shares in multiples of 128 (a tile of 32 for each wavefront), 256 at least.
 KVT_DEV int per_split(int len, int splits) { return max(((len + splits - 1) / splits + 127) & ~127, 256); }
 
 template <int CODE, int QT, int D>

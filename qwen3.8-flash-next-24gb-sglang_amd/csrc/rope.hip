@@ -12,7 +12,9 @@
 // A workgroup takes one token: its pairs' cosines and sines go to LDS once and serve all heads of q and k.  Bytes bound
 // it: every element is read once and written once, 16 bytes a lane (7,115 tokens of 64 + 8 heads x 128, fp16,
 // interleaved, out of one projection's output: 262 MB in 46 us, 5.7 TB/s).  64 tokens of 26 heads, a quarter of D 256:
-// 5.4 us, launch and load latency.
+// 5.4 us, launch and load latency.  Where rot / 2 (rot, interleaved), the rows or D are no multiples of 16 bytes, the whole
+// head goes by single elements: 4,096 tokens of 26 heads, D 256, rot 20 48 us, rot 64 25 (109 MB); of 40 heads, D 96, rot 24
+// 33, rot 48 19 (63 MB).
 #include "block_common.h"
 
 using namespace kvt;

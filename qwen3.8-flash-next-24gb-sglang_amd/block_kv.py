@@ -192,7 +192,8 @@ def _overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
         (_, h, d), (_, h2, d2), size = x.shape, y.shape, x.element_size()
         if size == y.element_size() and every:
             at = (y.data_ptr() - x.data_ptr()) % (every * size)
-            if (h - 1) * head + (d - 1) * unit + 1 <= at // size and at + ((h2 - 1) * head + (d2 - 1) * unit + 1) * size <= every * size:
+            mine, yours = ((i - 1) * head + (j - 1) * unit + 1 for i, j in ((h, d), (h2, d2)))
+            if mine * size <= at and at + yours * size <= every * size:
                 return False
     (a, span_x, dims_x, size_x), (c, span_y, dims_y, size_y) = _span(x), _span(y)
     if a + span_x <= c or c + span_y <= a:

@@ -20,11 +20,11 @@
 // in registers and streams Q; a lane adds up the weights of its position.  Splits are joined in their order by launches
 // of their own: no atomics, the same bits for every call.  64 rows (positions) a wavefront, which halve the reads of the
 // streamed tile against 32, are about what 256 registers hold at D 256 with two wavefronts a SIMD, and 168 at D 128 with
-// three: the second kernel spills two registers at both (four with int8 and fp16).  A prompt of
-// 10,001 tokens, 16 / 2 heads, D 256 (410 GFLOP a launch): 424 + 488 us, 967 and 840 TFLOP/s (a large library product
-// 1,241); the steps there: 856 + 1,405 with one wavefront a SIMD, 64-bit divisions for the rows and masks for every tile;
-// 497 + 541 without the first two; 460 + 495 with operands read ahead of their products and Q copied straight to LDS; 429
-// with masks by wavefront.  Vector instructions (6.5 and 7.4 a product at D 256, 13 at D 128, exponentials at a quarter of
+// three: the second kernel spills two registers at both (four with int8 and fp16).  A prompt of 10,001 tokens, 16 / 2
+// heads, D 256 (410 GFLOP a launch): 424 + 488 us, 967 and 840 TFLOP/s (a large library product 1,241); the steps
+// there: 856 + 1,405 with one wavefront a SIMD, 64-bit divisions for the rows and masks for every tile; 497 + 541
+// without the first two; 460 + 495 with operands read ahead of their products and Q copied straight to LDS; 429 with
+// masks by wavefront.  Vector instructions (6.5 and 7.4 a product at D 256, 13 at D 128, exponentials at a quarter of
 // the rate among them) take about as long as the products at D 256, and more than twice as long at D 128: they bound it
 // there and at D 64.
 //

@@ -37,8 +37,9 @@ def rotary_frequencies(dim: int, base: float = 10000.0, method: Optional[str] = 
         raise ValueError(f"method {method!r}: one of {METHODS}")
     if not (math.isfinite(base) and base > 0 and math.isfinite(factor) and factor > 0):
         raise ValueError(f"base {base} and factor {factor} have to be positive numbers")
-    if factors is not None and (method is not None or len(factors) != dim // 2):
-        raise ValueError(f"factors: {dim // 2} divisors, and no method beside them")
+    if factors is not None and (method is not None or len(factors) != dim // 2 or
+                                not all(math.isfinite(f) and f > 0 for f in factors)):
+        raise ValueError(f"factors: {dim // 2} divisors, positive numbers, and no method beside them")
     if method == "ntk":
         if dim < 4:
             raise ValueError("ntk: a rotary part of 4 channels at least")

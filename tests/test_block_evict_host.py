@@ -299,3 +299,10 @@ def test_weigh_workspace_is_bounded(kvt_pkg, monkeypatch):
                block_table=torch.empty(n, blocks, dtype=torch.int32), weights=torch.empty(n, 1, cap))
         assert most * hq * cap < asked[0] <= most * (hq * cap + 256 * 32), (n, asked)
         assert asked[1] == ("kvt_block_weigh", asked[0])
+
+
+@pytest.mark.parametrize("bad", [0.0, -2.0, math.inf, math.nan])
+def test_rotary_divisors_are_positive_numbers(kvt_pkg, bad):
+    from kvtier.rope import rotary_frequencies
+    with pytest.raises(ValueError):
+        rotary_frequencies(8, factors=[1.0, 2.0, bad, 4.0], device="cpu")
